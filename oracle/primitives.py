@@ -784,3 +784,147 @@ def random_split(keys, shape, **_):
 def random_fold_in(keys, msgs, **_):
     key = _single_key(keys)
     return _threefry_2x32_flat(key, np.array([0, np.asarray(msgs, u32).reshape(())], dtype=u32))
+
+
+# ------------------------------------------------------------------ operators of whole models
+# (no primitives of jax's own: the definitions, in 64 bits, rounded once)
+
+def _activation64(z, activation):
+    '''(activation(z), its derivative)'''
+    if activation == 'relu':
+        return np.where(z > 0, z, np.where(np.isnan(z), z, 0.0)), (z > 0).astype(np.float64)
+    if activation == 'silu':
+        s = 1.0 / (1.0 + np.exp(-z))
+        return z * s, s * (1.0 + z * (1.0 - s))
+    return z, np.ones_like(z)
+
+
+def _group_norm64(x, scale, shift, groups, eps):
+    x64 = np.asarray(x, np.float64).reshape(x.shape[0], math.prod(x.shape[1:-1]), groups, x.shape[-1] // groups)
+    if x64.shape[1] == 0:
+        mean = np.zeros((x.shape[0], 1, groups, 1))
+        rstd = np.zeros_like(mean)
+    else:
+        mean = x64.mean(axis=(1, 3), keepdims=True)
+        rstd = 1.0 / np.sqrt(((x64 - mean) ** 2).mean(axis=(1, 3), keepdims=True) + eps)
+    hat = (x64 - mean) * rstd
+    z = hat * np.asarray(scale, np.float64).reshape(groups, -1) + np.asarray(shift, np.float64).reshape(groups, -1)
+    return hat, z, mean, rstd
+
+
+def group_norm(x, scale, shift, groups, eps, activation):
+    with np.errstate(**_EW_ERR):
+        _, z, mean, rstd = _group_norm64(x, scale, shift, groups, eps)
+        y = _activation64(z, activation)[0]
+        stat = lambda v: v.reshape(x.shape[0], groups).astype(f32)
+        return y.reshape(x.shape).astype(f32), stat(mean), stat(rstd)
+
+
+def group_norm_grad(g, x, scale, shift, mean, rstd, groups, eps, activation):
+    with np.errstate(**_EW_ERR):
+        hat, z, _, inv = _group_norm64(x, scale, shift, groups, eps)
+        d = np.asarray(g, np.float64).reshape(z.shape) * _activation64(z, activation)[1]
+        dshift, dscale = d.sum(axis=(0, 1)).reshape(-1), (d * hat).sum(axis=(0, 1)).reshape(-1)
+        d = d * np.asarray(scale, np.float64).reshape(groups, -1)
+        if d.size:
+            d = inv * (d - d.mean(axis=(1, 3), keepdims=True) - hat * (d * hat).mean(axis=(1, 3), keepdims=True))
+        return d.reshape(x.shape).astype(f32), dscale.astype(f32), dshift.astype(f32)
+
+
+def _token_rows64(logits, tokens):
+    '''(scores, token, whether there is one, log of the sum, log probabilities, probabilities) of the rows'''
+    v = logits.shape[-1]
+    z = np.asarray(logits, np.float64).reshape(-1, v)
+    token = np.asarray(tokens, np.int64).reshape(-1)
+    given = (token >= 0) & (token < v)
+    best = z.max(axis=1)
+    empty = best == -np.inf
+    log_sum = np.where(empty, -np.inf, best + np.log(np.exp(z - np.where(empty, 0.0, best)[:, None]).sum(axis=1)))
+    logp = np.where(empty[:, None], -np.inf, z - np.where(empty, 0.0, log_sum)[:, None])
+    #(a row of which every score is -inf has no distribution: no probability anywhere)
+    return z, np.where(given, token, 0), given, log_sum, logp, np.exp(logp)
+
+
+def token_log_probs(logits, tokens, top):
+    with np.errstate(**_EW_ERR):
+        z, token, given, log_sum, logp, p = _token_rows64(logits, tokens)
+        entropy = -np.where(p == 0, 0.0, p * logp).sum(axis=1)
+        entropy = np.where(entropy == 0, 0.0, entropy)
+        shape = np.asarray(tokens).shape
+        rows = lambda v, empty: np.where(given, v, empty).reshape(shape).astype(f32)
+        outs = [rows(logp[np.arange(len(z)), token], 0.0), rows(entropy, 0.0), rows(log_sum, 0.0)]
+        if top:
+            #NaN before everything, then by score, equal ones by place
+            order = np.lexsort((np.broadcast_to(np.arange(z.shape[1]), z.shape), -z, ~np.isnan(z)), axis=1)[:, :top]
+            outs += [np.where(given[:, None], np.take_along_axis(logp, order, 1), 0.0).reshape(shape + (top,)).astype(f32),
+                     np.where(given[:, None], order, -1).reshape(shape + (top,)).astype(i32)]
+        return tuple(outs)
+
+
+def token_log_probs_grad(logits, tokens, log_sum, entropy, *cotangents, has_log_probs, has_entropy, top):
+    cotangents = [np.asarray(c) for c in cotangents]
+    with np.errstate(**_EW_ERR):
+        z, token, given, _, logp, p = _token_rows64(logits, tokens)
+        rows = np.arange(len(z))
+        d = np.zeros_like(z)
+        if has_log_probs:
+            g = cotangents.pop(0).astype(np.float64).reshape(-1)
+            d -= p * g[:, None]
+            d[rows, token] += np.where(p.sum(axis=1) == 0, 0.0, g)
+        if has_entropy:
+            g = cotangents.pop(0).astype(np.float64).reshape(-1)
+            plogp = np.where(p == 0, 0.0, p * logp)
+            d -= g[:, None] * (plogp - p * plogp.sum(axis=1, keepdims=True))
+        if top:
+            g, which = cotangents[0].astype(np.float64).reshape(-1, top), cotangents[1].reshape(-1, top)
+            d -= p * g.sum(axis=1, keepdims=True)
+            for j in range(top):
+                d[rows, np.maximum(which[:, j], 0)] += np.where(p.sum(axis=1) == 0, 0.0, g[:, j])
+        return np.where(given[:, None], d, 0.0).reshape(logits.shape).astype(f32)
+
+
+def _recurrence_factors64(factor, x, rest, gated, has_state, has_lengths):
+    '''(a, b, state, where a step is taken) of a recurrence, steps that are not taken as a = 1, b = 0'''
+    rest = list(rest)
+    batch, time, channels = x.shape
+    state = np.asarray(rest.pop(0), np.float64) if has_state else np.zeros((batch, channels))
+    inside = np.ones((batch, time, 1), bool)
+    if has_lengths:
+        inside = np.arange(time)[None, :, None] < np.asarray(rest.pop(0), np.int64)[:, None, None]
+    inside = np.broadcast_to(inside, x.shape)
+    f, x64 = np.where(inside, np.asarray(factor, np.float64), 0.0), np.where(inside, np.asarray(x, np.float64), 0.0)
+    a, rest_of_one = (1.0 / (1.0 + np.exp(-f)), 1.0 / (1.0 + np.exp(f))) if gated else (f, None)
+    b = rest_of_one * x64 if gated else x64
+    return np.where(inside, a, 1.0), np.where(inside, b, 0.0), rest_of_one, x64, state, inside, rest
+
+
+def linear_recurrence(factor, x, *rest, gated, reverse, has_state, has_lengths):
+    with np.errstate(**_EW_ERR):
+        a, b, _, _, state, inside, _ = _recurrence_factors64(factor, x, rest, gated, has_state, has_lengths)
+        h, now = np.empty_like(b), state
+        for t in (range(x.shape[1] - 1, -1, -1) if reverse else range(x.shape[1])):
+            now = h[:, t] = np.where(inside[:, t], a[:, t] * now + b[:, t], now)
+        return h.astype(f32), now.astype(f32)
+
+
+def linear_recurrence_grad(h, factor, x, *rest, gated, reverse, has_state, has_lengths, has_g, has_last):
+    with np.errstate(**_EW_ERR):
+        a, b, rest_of_one, x64, state, inside, rest = _recurrence_factors64(factor, x, rest, gated, has_state, has_lengths)
+        g = np.asarray(rest.pop(0), np.float64) if has_g else np.zeros_like(b)
+        adjoint = np.asarray(rest.pop(0), np.float64) if has_last else np.zeros_like(state)
+        steps = list(range(x.shape[1] - 1, -1, -1) if reverse else range(x.shape[1]))
+        before, now = np.empty_like(b), state
+        for t in steps:
+            before[:, t] = now
+            now = np.where(inside[:, t], a[:, t] * now + b[:, t], now)
+        df, dx = np.zeros_like(b), np.zeros_like(b)
+        for t in reversed(steps):
+            adjoint = adjoint + g[:, t]
+            if gated:
+                df[:, t] = adjoint * (before[:, t] - x64[:, t]) * a[:, t] * rest_of_one[:, t]
+                dx[:, t] = adjoint * rest_of_one[:, t]
+            else:
+                df[:, t], dx[:, t] = adjoint * before[:, t], adjoint
+            df[:, t], dx[:, t] = np.where(inside[:, t], df[:, t], 0.0), np.where(inside[:, t], dx[:, t], 0.0)
+            adjoint = np.where(inside[:, t], adjoint * a[:, t], adjoint)
+        return df.astype(f32), dx.astype(f32), adjoint.astype(f32)

@@ -60,7 +60,7 @@ def _reads(op) -> tp.List:
             return [b for b, _ in op.launch.buffers[1:] if b is not None]
         if op.meta[0] == 'softmax':
             return [op.meta[2]]
-        if op.meta[0] == 'rows':
+        if op.meta[0] in ('rows', 'operator'):
             return list(op.meta[2])
         if op.meta[0] == 'conv_pack':
             return [op.meta[2].buffer]
@@ -1458,7 +1458,7 @@ def _writes(op) -> tp.List:
         return [_out(op)]
     if op.meta is not None and op.meta[0] in ('iota', 'concat_part'):
         return [op.meta[1]]
-    if op.meta is not None and op.meta[0] in ('threefry', 'softmax', 'rows', 'relu_backward'):
+    if op.meta is not None and op.meta[0] in ('threefry', 'softmax', 'rows', 'relu_backward', 'operator'):
         return list(op.meta[1])
     return [b for b, _ in op.launch.buffers[:1] if b is not None]      #kernels write their first argument
 
@@ -1672,7 +1672,7 @@ def _small_out(op):
 
 def _may_write(op) -> tp.List:
     '''Buffers an op may change: its result where the op's structure is known, else everything it touches.'''
-    if op.chain is not None or op.conv is not None or (op.meta is not None and op.meta[0] in ('iota', 'concat_part', 'threefry', 'random_stream', 'reduce', 'update', 'window_sum', 'relu_backward', 'softmax', 'rows', 'conv_pack')):
+    if op.chain is not None or op.conv is not None or (op.meta is not None and op.meta[0] in ('iota', 'concat_part', 'threefry', 'random_stream', 'reduce', 'update', 'window_sum', 'relu_backward', 'softmax', 'rows', 'conv_pack', 'operator')):
         return _writes(op)
     return [b for b, _ in op.launch.buffers if b is not None]
 

@@ -2172,3 +2172,73 @@ def threefry2x32(out0: Buffer, out1: Buffer, key0: Buffer, key1: Buffer, x0: Buf
     return Launch(f'threefry2x32{"_k" if key_is_scalar else ""}_v{vec}', (_cdiv(_cdiv(n, vec), BLOCK), 1, 1), (BLOCK, 1, 1),
                   [(out0, 0), (out1, 0), (key0, 0), (key1, 0), (x0, 0), (x1, 0)], _u32(n, int(key_is_scalar)),
                   bytes_moved=16 * n, written=(0, 1))
+
+
+# ---------------------------------------------------------------- group norm (norm.hip)
+
+NORM_ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2}
+
+
+def _f32_word(value: float) -> int:
+    return int(np.asarray(value, np.float32).view(np.uint32))
+
+
+def _norm_shape(x: Buffer, groups: int):
+    n, c = x.shape[0], x.shape[-1]
+    return n, x.size // (n * c), c, c // groups
+
+
+def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shift: Buffer, groups: int, eps: float, activation, scratch) -> tp.List[Launch]:
+    n, s, c, cg = _norm_shape(x, groups)
+    params = _u32(0, s, c, groups, cg, NORM_ACTIVATIONS[activation], _f32_word(eps))
+    return [Launch('group_norm', (n * groups, 1, 1), (BLOCK, 1, 1), [(y, 0), (mean, 0), (rstd, 0), (x, 0), (scale, 0), (shift, 0)], params,
+                   bytes_moved=4 * (2 * x.size + 2 * c + 2 * n * groups), written=(0, 1, 2))]
+
+
+def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shift: Buffer, mean: Buffer, rstd: Buffer, groups: int, eps: float,
+                    activation, scratch) -> tp.List[Launch]:
+    n, s, c, cg = _norm_shape(x, groups)
+    shares = scratch((2, n, c))
+    params = _u32(0, s, c, groups, cg, NORM_ACTIVATIONS[activation], _f32_word(eps), n)
+    launches = [Launch('group_norm_grad', (n * groups, 1, 1), (BLOCK, 1, 1),
+                       [(dx, 0), (shares, 0), (g, 0), (x, 0), (scale, 0), (shift, 0), (mean, 0), (rstd, 0)], params,
+                       bytes_moved=4 * (3 * x.size + 2 * n * c), written=(0, 1))]
+    for k, out in enumerate((dscale, dshift)):
+        if out is not None:
+            total = _reduce_launch(out, shares, 1, n, c, 'reduce_sum', 1)[0]
+            launches.append(total._replace(buffers=[total.buffers[0], (shares, 4 * k * n * c)] + total.buffers[2:]))
+    return launches
+
+
+# ---------------------------------------------------------------- log probabilities of tokens (log_probs.hip)
+
+def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch) -> tp.List[Launch]:
+    v = logits.shape[-1]
+    rows = logits.size // v
+    return [Launch('log_probs', (rows, 1, 1), (BLOCK, 1, 1),
+                   [(log_prob, 0), (entropy, 0), (log_sum, 0), (top_log_prob, 0), (top_token, 0), (logits, 0), (tokens, 0)], _u32(0, v, top),
+                   bytes_moved=4 * (logits.size + rows * (4 + 2 * top)), written=(0, 1, 2, 3, 4))]
+
+
+def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Buffer, entropy: Buffer, g_log_prob, g_entropy, g_top, top_token,
+                         top: int) -> tp.List[Launch]:
+    v = logits.shape[-1]
+    rows = logits.size // v
+    return [Launch('log_probs_grad', (rows, 1, 1), (BLOCK, 1, 1),
+                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)], _u32(0, v, top),
+                   bytes_moved=4 * (2 * logits.size + rows * (5 + 2 * top)))]
+
+
+# ---------------------------------------------------------------- linear recurrences (recurrence.hip)
+
+def linear_recurrence(h, last, factor: Buffer, x: Buffer, state, lengths, gated: bool, reverse: bool, scratch) -> tp.List[Launch]:
+    b, t, c = x.shape
+    return [Launch('recurrence', (_cdiv(c, 64), b, 1), (64, 1, 1), [(v, 0) for v in (h, last, factor, x, state, lengths)],
+                   _u32(t, c, gated, reverse), bytes_moved=4 * 3 * x.size, written=(0, 1))]
+
+
+def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Buffer, state, lengths, g, g_last, gated: bool, reverse: bool,
+                           scratch) -> tp.List[Launch]:
+    b, t, c = x.shape
+    return [Launch('recurrence_grad', (_cdiv(c, 64), b, 1), (64, 1, 1), [(v, 0) for v in (dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last)],
+                   _u32(t, c, gated, reverse), bytes_moved=4 * 6 * x.size, written=(0, 1, 2))]

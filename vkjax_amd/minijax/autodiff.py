@@ -321,6 +321,37 @@ def _gather(g, operand, indices, out, dimension_numbers, slice_sizes, **_):
     return lax.scatter_add(_zeros_like(operand), indices, g, dn), None
 
 
+@_rule('group_norm')
+def _group_norm(gs, x, scale, shift, outs, groups, eps, activation):
+    if gs[1] is not None or gs[2] is not None:
+        raise NotImplementedError('differentiation through the statistics of group_norm')
+    g, (y, mean, rstd) = _materialize(gs[0], outs[0]), outs
+    return lax.group_norm_grad(g, x, scale, shift, mean, rstd, groups, eps, activation)
+
+
+def _or_none(g, like):
+    return None if g is None else _materialize(g, like)
+
+
+@_rule('token_log_probs')
+def _token_log_probs(gs, logits, tokens, outs, top):
+    if gs[2] is not None:
+        raise NotImplementedError('differentiation through the log of the sum of token_log_probs')
+    g_top = _or_none(gs[3], outs[3]) if top else None
+    return lax.token_log_probs_grad(logits, tokens, outs[2], outs[1], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), g_top,
+                                    outs[4] if g_top is not None else None), None
+
+
+@_rule('linear_recurrence')
+def _linear_recurrence(gs, factor, x, *rest, gated, reverse, has_state, has_lengths):
+    *optional, outs = rest
+    state   = optional[0] if has_state else None
+    lengths = optional[-1] if has_lengths else None
+    dfactor, dx, dstate = lax.linear_recurrence_grad(outs[0], factor, x, state, lengths, _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]),
+                                                     reverse, gated)
+    return (dfactor, dx) + ((dstate,) if has_state else ()) + ((None,) if has_lengths else ())
+
+
 _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', 'iota', 'and', 'or', 'not', 'xor', 'sign', 'floor', 'ceil',
                        'round', 'is_finite', 'shift_left', 'shift_right_logical', 'shift_right_arithmetic', 'threefry2x32',
                        'random_bits', 'random_split', 'random_wrap', 'random_unwrap', 'random_fold_in', 'random_seed'}
@@ -357,32 +388,33 @@ def _replay(jaxpr, consts, inputs, env, order):
     return [read(v) for v in jaxpr.outvars]
 
 
-def value_and_grad(fun: tp.Callable, argnums: tp.Union[int, tp.Sequence[int]] = 0, has_aux: bool = False):
-    '''`(value, gradient)` of a scalar-valued function with respect to the arguments `argnums` (pytrees of
-    float32 arrays). Must be called while tracing (inside a function given to `make_jaxpr` / `wrap`);
-    every traced value the function uses has to come in through its arguments.'''
-    single = isinstance(argnums, int)
-    wrt    = (argnums,) if single else tuple(argnums)
-
-    def wrapped(*args):
+class _Replayed:
+    '''A function's equations in the enclosing trace, and what its backward pass needs of them.'''
+    def __init__(self, fun, args, wrt, distinct=False):
         current_trace()
-        leaves, in_tree = tree_util.tree_flatten(tuple(args))
-        in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, leaves)]
+        self.leaves, in_tree = tree_util.tree_flatten(tuple(args))
+        if distinct:
+            #values are told apart by identity: one that is passed twice has a share of the gradient in each place
+            self.leaves = [Tracer(a._trace, a._var) if isinstance(a, Tracer) else np.array(a, dtype_of(a)[0]) for a in self.leaves]
+        in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, self.leaves)]
         jaxpr, consts, out_tree, _ = _trace_to_jaxpr(fun, in_avals, in_tree, {}, len(args))
-        env, order = {}, []
-        outs   = _replay(jaxpr, consts, leaves, env, order)
-        result = tree_util.tree_unflatten(out_tree, outs)
-        value, aux = result if has_aux else (result, None)
-        if _shape(value) != () or dtype_of(value)[0] != _f32:
-            raise TypeError('value_and_grad needs a function that returns a float32 scalar')
+        self.env, self.order = {}, []
+        outs        = _replay(jaxpr, consts, self.leaves, self.env, self.order)
+        self.result = tree_util.tree_unflatten(out_tree, outs)
+        #positions of the differentiated leaves
+        self.counts  = [len(tree_util.tree_leaves([a])) for a in args]
+        starts       = np.cumsum([0] + self.counts)
+        self.wrt     = wrt
+        self.wrt_pos = [p for i in wrt for p in range(starts[i], starts[i + 1])]
+        self.args    = args
 
-        #positions of the differentiated leaves, and the values that depend on them (by identity: inlined
-        #calls bind their own variables to the caller's values)
-        counts  = [len(tree_util.tree_leaves([a])) for a in args]
-        starts  = np.cumsum([0] + counts)
-        wrt_pos = [p for i in wrt for p in range(starts[i], starts[i + 1])]
+    def pull(self, seeds):
+        '''The gradient of every differentiated argument for the cotangents `seeds`, pairs (value of the trace, cotangent).'''
+        env, order, leaves = self.env, self.order, self.leaves
+        #the values that depend on the differentiated leaves (by identity: inlined calls bind their own variables to the
+        #caller's values)
         value_of = lambda v: v.val if core.is_literal(v) else env[v]
-        active  = {id(leaves[p]) for p in wrt_pos}
+        active  = {id(leaves[p]) for p in self.wrt_pos}
         for eqn in order:
             if any(id(value_of(v)) in active for v in eqn.invars):
                 active.update(id(env[v]) for v in eqn.outvars)
@@ -390,7 +422,8 @@ def value_and_grad(fun: tp.Callable, argnums: tp.Union[int, tp.Sequence[int]] = 
         cts: tp.Dict[int, tp.Any] = {}
         def add_ct(target, g):
             cts[id(target)] = g if id(target) not in cts else lax.add_any(cts[id(target)], g)
-        add_ct(value, np.float32(1.0))
+        for value, g in seeds:
+            add_ct(value, g)
         for eqn in reversed(order):
             outs_now = [env[v] for v in eqn.outvars]
             gs = [cts.get(id(o)) for o in outs_now]
@@ -414,17 +447,55 @@ def value_and_grad(fun: tp.Callable, argnums: tp.Union[int, tp.Sequence[int]] = 
                 if ct is not None and id(operand) in active:
                     add_ct(operand, ct() if callable(ct) else ct)
         grads = []
-        for p in wrt_pos:
+        for p in self.wrt_pos:
             g = cts.get(id(leaves[p]))
             grads.append(_materialize(g, leaves[p]) if g is not None else _zeros_like(leaves[p]))
         per_arg, k = [], 0
-        for i in wrt:
-            n = counts[i]
-            per_arg.append(tree_util.tree_unflatten(tree_util.tree_structure([args[i]]), grads[k:k + n])[0])
+        for i in self.wrt:
+            n = self.counts[i]
+            per_arg.append(tree_util.tree_unflatten(tree_util.tree_structure([self.args[i]]), grads[k:k + n])[0])
             k += n
-        gradient = per_arg[0] if single else tuple(per_arg)
+        return tuple(per_arg)
+
+
+def value_and_grad(fun: tp.Callable, argnums: tp.Union[int, tp.Sequence[int]] = 0, has_aux: bool = False):
+    '''`(value, gradient)` of a scalar-valued function with respect to the arguments `argnums` (pytrees of
+    float32 arrays). Must be called while tracing (inside a function given to `make_jaxpr` / `wrap`);
+    traced values that the function closes over are constants to it.'''
+    single = isinstance(argnums, int)
+    wrt    = (argnums,) if single else tuple(argnums)
+
+    def wrapped(*args):
+        replayed = _Replayed(fun, args, wrt)
+        value, aux = replayed.result if has_aux else (replayed.result, None)
+        if _shape(value) != () or dtype_of(value)[0] != _f32:
+            raise TypeError('value_and_grad needs a function that returns a float32 scalar')
+        per_arg  = replayed.pull([(value, np.float32(1.0))])
+        gradient = per_arg[0] if single else per_arg
         return ((value, aux), gradient) if has_aux else (value, gradient)
     return wrapped
+
+
+def vjp(fun: tp.Callable, *primals, has_aux: bool = False):
+    '''`(fun(*primals), pullback)`: pullback(cotangents), of the structure and shapes of the result, returns the tuple of the
+    primals' cotangents. With `has_aux` fun returns (result, aux), of which only the result is differentiated, and
+    (result, pullback, aux) comes back. Must be called while tracing; traced values that fun closes over are constants to it.'''
+    replayed = _Replayed(fun, primals, tuple(range(len(primals))), distinct=True)
+    result, aux = replayed.result if has_aux else (replayed.result, None)
+    outs, structure = tree_util.tree_flatten(result)
+    for o in outs:
+        if dtype_of(o)[0] != _f32:
+            raise TypeError(f'vjp: results must be float32, got {dtype_of(o)[0]} (return others with has_aux)')
+
+    def pullback(cotangents):
+        gs, given = tree_util.tree_flatten(cotangents)
+        if given != structure:
+            raise TypeError(f'vjp: cotangents of structure {given} for a result of structure {structure}')
+        for g, o in zip(gs, outs):
+            if _shape(g) != _shape(o) or dtype_of(g)[0] != _f32:
+                raise TypeError(f'vjp: a cotangent of {dtype_of(g)[0]} {_shape(g)} for a result of float32 {_shape(o)}')
+        return replayed.pull([(o, g if isinstance(g, Tracer) else np.asarray(g, np.float32)) for o, g in zip(outs, gs)])
+    return (result, pullback, aux) if has_aux else (result, pullback)
 
 
 def _materialize(g, like):

@@ -507,6 +507,136 @@ def scatter_add(operand, scatter_indices, updates, dimension_numbers: ScatterDim
                      update_jaxpr=None, update_consts=(), **({} if mode is None else dict(mode=mode))))
 
 
+# ---------------------------------------------------------------- operators of whole models
+#(no primitives of jax's own: one equation each, which the dispatch lowers to kernels of its own; `nn` has the functions
+#that programs call)
+
+def _f32_operand(x, what):
+    x = x if isinstance(x, Tracer) else np.asarray(x)
+    if dtype_of(x)[0] != _f32:
+        raise TypeError(f'{what} needs float32, got {dtype_of(x)[0]}')
+    return _as_dtype(x, _f32)
+
+
+GROUP_NORM_ACTIVATIONS = (None, 'relu', 'silu')
+
+
+def group_norm(x, scale, shift, groups: int, eps: float = 1e-5, activation=None):
+    '''activation((x - mean) / sqrt(var + eps) * scale + shift) of x [N, ..., C], mean and variance over everything of one sample
+    in one of `groups` runs of neighbouring channels; scale and shift are [C]. Returns (y, mean [N, groups],
+    1 / sqrt(var + eps) [N, groups]).'''
+    x, scale, shift = (_f32_operand(v, 'group_norm') for v in (x, scale, shift))
+    xs = _shape(x)
+    if len(xs) < 2:
+        raise TypeError(f'group_norm takes [samples, ..., channels], got {xs}')
+    groups, channels = int(groups), xs[-1]
+    if groups < 1 or channels < 1 or channels % groups:
+        raise ValueError(f'group_norm: {channels} channels do not fall into {groups} groups of equal size')
+    if _shape(scale) != (channels,) or _shape(shift) != (channels,):
+        raise TypeError(f'group_norm: scale and shift must have shape ({channels},), got {_shape(scale)} and {_shape(shift)}')
+    if not (0.0 < float(eps) < np.inf):
+        raise ValueError(f'group_norm: eps must be positive and finite, got {eps}')
+    if activation not in GROUP_NORM_ACTIVATIONS:
+        raise ValueError(f'group_norm: activation must be one of {GROUP_NORM_ACTIVATIONS}, got {activation!r}')
+    return tuple(emit('group_norm', [x, scale, shift], [_aval(xs, _f32), _aval((xs[0], groups), _f32), _aval((xs[0], groups), _f32)],
+                dict(groups=groups, eps=float(eps), activation=activation), multiple_results=True))
+
+
+def group_norm_grad(g, x, scale, shift, mean, rstd, groups: int, eps: float = 1e-5, activation=None):
+    '''(dx, dscale, dshift) for the cotangent g of group_norm's y; mean and rstd are what group_norm returned.'''
+    xs, cs = _shape(x), _shape(scale)
+    if _shape(g) != xs or _shape(mean) != (xs[0], groups) or _shape(rstd) != (xs[0], groups):
+        raise TypeError(f'group_norm_grad: shapes {_shape(g)}, {xs}, {_shape(mean)}, {_shape(rstd)} do not belong together')
+    return tuple(emit('group_norm_grad', [g, x, scale, shift, mean, rstd], [_aval(xs, _f32), _aval(cs, _f32), _aval(cs, _f32)],
+                dict(groups=int(groups), eps=float(eps), activation=activation), multiple_results=True))
+
+
+TOKEN_LOG_PROBS_MAX_TOP = 32
+
+
+def token_log_probs(logits, tokens, top: int = 0):
+    '''For rows of scores [..., V] and one token per row [...]: (log softmax(logits)[token], entropy of softmax(logits),
+    log(sum(exp(logits)))), all [...], and for top > 0 the log probabilities and numbers [..., top] of the most likely tokens.
+    `nn.token_log_probs` says what becomes of padded and masked rows.'''
+    logits = _f32_operand(logits, 'token_log_probs')
+    tokens = tokens if isinstance(tokens, Tracer) else np.asarray(tokens)
+    ls, top = _shape(logits), int(top)
+    if len(ls) < 1 or ls[-1] < 1:
+        raise TypeError(f'token_log_probs takes [..., vocabulary] with at least one token, got {ls}')
+    if dtype_of(tokens)[0] not in (_i32, _u32):
+        raise TypeError(f'token_log_probs: tokens must be integers, got {dtype_of(tokens)[0]}')
+    if _shape(tokens) != ls[:-1]:
+        raise TypeError(f'token_log_probs: one token per row of {ls} is needed, got {_shape(tokens)}')
+    if not 0 <= top <= builtins.min(ls[-1], TOKEN_LOG_PROBS_MAX_TOP):
+        raise ValueError(f'token_log_probs: top must be between 0 and {builtins.min(ls[-1], TOKEN_LOG_PROBS_MAX_TOP)} here, got {top}')
+    rows  = _aval(ls[:-1], _f32)
+    avals = [rows, rows, rows] + ([_aval(ls[:-1] + (top,), _f32), _aval(ls[:-1] + (top,), _i32)] if top else [])
+    return tuple(emit('token_log_probs', [logits, _as_dtype(tokens, dtype_of(tokens)[0])], avals, dict(top=top), multiple_results=True))
+
+
+def token_log_probs_grad(logits, tokens, log_sum, entropy, g_log_probs=None, g_entropy=None, g_top=None, top_tokens=None):
+    '''Cotangent of token_log_probs' logits for those of its results (None: zeros), of which log_sum, entropy and top_tokens are.'''
+    ls = _shape(logits)
+    optional = [g for g in (g_log_probs, g_entropy) if g is not None]
+    if _any_differs(ls[:-1], tokens, log_sum, entropy, *optional):
+        raise TypeError('token_log_probs_grad: one value per row is needed')
+    top = 0
+    if g_top is not None:
+        top = _shape(top_tokens)[-1]
+        if _any_differs(ls[:-1] + (top,), g_top, top_tokens):
+            raise TypeError('token_log_probs_grad: the alternatives and their cotangents must have the same shape')
+        optional += [g_top, top_tokens]
+    return emit('token_log_probs_grad', [logits, tokens, log_sum, entropy] + optional, [_aval(ls, _f32)],
+                dict(has_log_probs=g_log_probs is not None, has_entropy=g_entropy is not None, top=top))
+
+
+def _any_differs(shape, *arrays) -> bool:
+    return builtins.any(_shape(a) != tuple(shape) for a in arrays)
+
+
+def _recurrence_operands(name, factor, x, state, lengths):
+    factor, x = _f32_operand(factor, name), _f32_operand(x, name)
+    xs = _shape(x)
+    if len(xs) != 3 or _shape(factor) != xs:
+        raise TypeError(f'{name} takes two arrays [batch, time, channels], got {_shape(factor)} and {xs}')
+    operands = [factor, x]
+    if state is not None:
+        state = _f32_operand(state, name)
+        if _shape(state) != (xs[0], xs[2]):
+            raise TypeError(f'{name}: the state must have shape {(xs[0], xs[2])}, got {_shape(state)}')
+        operands.append(state)
+    if lengths is not None:
+        lengths = lengths if isinstance(lengths, Tracer) else np.asarray(lengths)
+        if dtype_of(lengths)[0] != _i32 or _shape(lengths) != (xs[0],):
+            raise TypeError(f'{name}: lengths must be int32 [{xs[0]}], got {dtype_of(lengths)[0]} {_shape(lengths)}')
+        operands.append(_as_dtype(lengths, _i32))
+    return operands, xs
+
+
+def linear_recurrence(factor, x, state=None, lengths=None, reverse: bool = False, gated: bool = False):
+    '''h[:, t] = factor[:, t] * h[:, t-1] + x[:, t] over [batch, time, channels] from h[:, -1] = state [batch, channels] (zeros if
+    None); `reverse`: from the last time to the first. `gated`: factor holds gates, h[:, t] = a h[:, t-1] + (1 - a) x[:, t] with
+    a = sigmoid(factor[:, t]). `lengths` (int32 [batch], taken as between 0 and time): at times from a sequence's length on the
+    state stays what it is, and what factor and x hold there is not looked at. Returns (h, the state behind the last step
+    [batch, channels]).'''
+    operands, xs = _recurrence_operands('gated_recurrence' if gated else 'linear_recurrence', factor, x, state, lengths)
+    return tuple(emit('linear_recurrence', operands, [_aval(xs, _f32), _aval((xs[0], xs[2]), _f32)],
+                dict(gated=bool(gated), reverse=bool(reverse), has_state=state is not None, has_lengths=lengths is not None),
+                multiple_results=True))
+
+
+def linear_recurrence_grad(h, factor, x, state=None, lengths=None, g=None, g_last=None, reverse: bool = False, gated: bool = False):
+    '''(dfactor, dx, dstate [batch, channels]) for the cotangents g and g_last (None: zeros) of linear_recurrence's results, of
+    which h is the first.'''
+    operands, xs = _recurrence_operands('linear_recurrence_grad', factor, x, state, lengths)
+    if (_any_differs(xs, h) or (g is not None and _shape(g) != xs) or (g_last is not None and _shape(g_last) != (xs[0], xs[2]))):
+        raise TypeError(f'linear_recurrence_grad: the cotangents and h do not belong to {xs}')
+    return tuple(emit('linear_recurrence_grad', [h] + operands + [v for v in (g, g_last) if v is not None],
+                [_aval(xs, _f32), _aval(xs, _f32), _aval((xs[0], xs[2]), _f32)],
+                dict(gated=bool(gated), reverse=bool(reverse), has_state=state is not None, has_lengths=lengths is not None,
+                     has_g=g is not None, has_last=g_last is not None), multiple_results=True))
+
+
 # ---------------------------------------------------------------- rng
 
 def threefry2x32(key0, key1, x0, x1):

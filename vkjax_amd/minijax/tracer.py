@@ -22,6 +22,16 @@ class Trace:
 
     def new_const(self, value: np.ndarray) -> core.Var:
         key = id(value)
+        if isinstance(value, Tracer):
+            #a value of an enclosing trace: an argument that the caller of this function passes along with the constants
+            if key not in self._const_ids:
+                self._const_ids[key] = core.Var(None, '', value.aval)
+                self.constvars.append(self._const_ids[key])
+                #(an object of its own: values are told apart by identity where functions are differentiated, and what a
+                #function closes over is a constant there, also if the same value is an argument)
+                self.consts.append(Tracer(value._trace, value._var))
+                self._keepalive = getattr(self, '_keepalive', []) + [value]
+            return self._const_ids[key]
         if key not in self._const_ids:
             value = np.asarray(value)
             aval  = core.ShapedArray(value.shape, core.canonicalize_dtype(value.dtype))
@@ -218,8 +228,12 @@ def to_invar(x, dtype: tp.Optional[np.dtype] = None) -> tp.Union[core.Var, core.
     trace = current_trace()
     if isinstance(x, Tracer):
         if x._trace is not trace:
-            raise NotImplementedError('a traced value from an enclosing function cannot be used '
-                                      'inside a nested jit; pass it as an argument instead')
+            outer = trace.parent
+            while outer is not None and outer is not x._trace:
+                outer = outer.parent
+            if outer is None:
+                raise NotImplementedError('a traced value cannot be used outside the function it belongs to')
+            return trace.new_const(x)
         return x._var
     arr = np.asarray(x)
     if dtype is None:
@@ -265,7 +279,7 @@ def _trace_to_jaxpr(fun, in_avals: tp.Sequence[core.ShapedArray], in_tree, stati
                 #a constant output: materialise it through a (free) view of a literal/const
                 from . import lax
                 leaf = lax.convert_element_type(leaf, dtype_of(leaf)[0], force=True)
-            outvars.append(leaf._var)
+            outvars.append(to_invar(leaf))
         jaxpr = core.Jaxpr(trace.constvars, invars, outvars, trace.eqns)
         return jaxpr, trace.consts, out_tree, [v.aval for v in outvars]
     finally:
@@ -282,6 +296,9 @@ def make_jaxpr(fun: tp.Callable, static_argnums: tp.Iterable[int] = (), return_s
         leaves, in_tree = tree_util.tree_flatten(dynamic)
         in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, leaves)]
         jaxpr, consts, out_tree, out_avals = _trace_to_jaxpr(fun, in_avals, in_tree, static, len(args))
+        if any(isinstance(c, Tracer) for c in consts):
+            raise NotImplementedError('a function given to make_jaxpr cannot use traced values of an enclosing function; '
+                                      'pass them as arguments instead')
         closed = core.ClosedJaxpr(jaxpr, consts)
         if not return_shape:
             return closed

@@ -1053,6 +1053,118 @@ def _uniform_constant(b):
     return first if (value.reshape(-1).view(np.uint8).reshape(value.size, -1) == np.asarray(first).reshape(1).view(np.uint8)).all() else None
 
 
+# ------------------------------------------------------------------ operators of whole models
+# One equation each, lowered to kernels of their own. No jax primitives have these names: programs get them from
+# minijax.nn / minijax.lax, where their definitions stand.
+
+def _operator_buffers(bufferpool, equation):
+    '''(operands, results - None for those nobody reads -, a function that makes scratch arrays at the equation's own position)'''
+    ins  = [bufferpool.get_buffer(v) for v in equation.invars]
+    outs = [None if core.is_dropped(v) else bufferpool.get_buffer(v) for v in equation.outvars]
+    position = bufferpool.op_counter
+    bufferpool.op_counter += 1
+
+    def scratch(shape, dtype=np.float32):
+        bufferpool.op_counter = position
+        b = bufferpool.new_temporary(np.dtype(dtype), shape)
+        bufferpool.op_counter = position + 1
+        return b
+    return ins, outs, scratch
+
+
+def _operator_ops(equation, launches) -> tp.List[Op]:
+    '''Ops of launches that say which of their arrays they write; the others are read.'''
+    def op(launch):
+        written = [b for i, (b, _) in enumerate(launch.buffers) if b is not None and i in launch.written]
+        read    = [b for i, (b, _) in enumerate(launch.buffers) if b is not None and i not in launch.written]
+        return Op(equation, launch=launch, meta=('operator', written, read))
+    return [op(launch) for launch in launches]
+
+
+def _with_elements(b):
+    return b if b is not None and b.size else None
+
+
+def group_norm(bufferpool, equation):
+    p = equation.params
+    (x, scale, shift), (y, mean, rstd), scratch = _operator_buffers(bufferpool, equation)
+    if any(_kind(b.dtype) != _F for b in (x, scale, shift)):
+        raise NotImplementedError(equation)
+    if x.size == 0:
+        return [Op(equation, launch=K.fill(b, 0)) for b in (mean, rstd) if _with_elements(b) is not None]      #statistics of nothing
+    return _operator_ops(equation, K.group_norm(y, mean, rstd, x, scale, shift, p['groups'], p['eps'], p['activation'], scratch))
+
+
+def group_norm_grad(bufferpool, equation):
+    p = equation.params
+    (g, x, scale, shift, mean, rstd), (dx, dscale, dshift), scratch = _operator_buffers(bufferpool, equation)
+    if any(_kind(b.dtype) != _F for b in (g, x, scale, shift, mean, rstd)):
+        raise NotImplementedError(equation)
+    if x.size == 0:
+        return [Op(equation, launch=K.fill(b, 0)) for b in (dscale, dshift) if b is not None]                  #sums over nothing
+    return _operator_ops(equation, K.group_norm_grad(dx, dscale, dshift, g, x, scale, shift, mean, rstd, p['groups'], p['eps'],
+                                                     p['activation'], scratch))
+
+
+def token_log_probs(bufferpool, equation):
+    (logits, tokens), (log_prob, entropy, log_sum, *top), scratch = _operator_buffers(bufferpool, equation)
+    if _kind(logits.dtype) != _F or _kind(tokens.dtype) not in (_I, _U):
+        raise NotImplementedError(equation)
+    top_log_prob, top_token = top or (None, None)
+    return _operator_ops(equation, K.token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits, tokens,
+                                                     int(equation.params['top']), scratch))
+
+
+def token_log_probs_grad(bufferpool, equation):
+    p = equation.params
+    (logits, tokens, log_sum, entropy, *optional), (dx,), _ = _operator_buffers(bufferpool, equation)
+    if _kind(logits.dtype) != _F or _kind(tokens.dtype) not in (_I, _U):
+        raise NotImplementedError(equation)
+    take = iter(optional)
+    g_log_prob = next(take) if p['has_log_probs'] else None
+    g_entropy  = next(take) if p['has_entropy'] else None
+    g_top, top_token = (next(take), next(take)) if p['top'] else (None, None)
+    return _operator_ops(equation, K.token_log_probs_grad(dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token,
+                                                          int(p['top'])))
+
+
+def _recurrence_buffers(ins, params):
+    factor, x, *rest = ins
+    state   = rest.pop(0) if params['has_state'] else None
+    lengths = rest.pop(0) if params['has_lengths'] else None
+    return factor, x, state, lengths, rest
+
+
+def linear_recurrence(bufferpool, equation):
+    p = equation.params
+    ins, (h, last), scratch = _operator_buffers(bufferpool, equation)
+    factor, x, state, lengths, _ = _recurrence_buffers(ins, p)
+    if x.size == 0:
+        return _held_state(equation, last, state)
+    return _operator_ops(equation, K.linear_recurrence(h, last, factor, x, state, lengths, p['gated'], p['reverse'], scratch))
+
+
+def linear_recurrence_grad(bufferpool, equation):
+    p = equation.params
+    (h, *ins), (dfactor, dx, dstate), scratch = _operator_buffers(bufferpool, equation)
+    factor, x, state, lengths, rest = _recurrence_buffers(ins, p)
+    g      = rest.pop(0) if p['has_g'] else None
+    g_last = rest.pop(0) if p['has_last'] else None
+    if x.size == 0:
+        return _held_state(equation, dstate, g_last)
+    return _operator_ops(equation, K.linear_recurrence_grad(dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last, p['gated'],
+                                                            p['reverse'], scratch))
+
+
+def _held_state(equation, out, source):
+    '''No step is taken: what goes in comes out.'''
+    if _with_elements(out) is None:
+        return []
+    if source is None:
+        return [Op(equation, launch=K.fill(out, 0))]
+    return [_copy_op(equation, out, EwOperand(source, 0, K.row_major_strides(out.shape)))]
+
+
 # ------------------------------------------------------------------ rng
 
 def threefry2x32(bufferpool, equation):
