@@ -2231,14 +2231,61 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
 
 # ---------------------------------------------------------------- linear recurrences (recurrence.hip)
 
-def linear_recurrence(h, last, factor: Buffer, x: Buffer, state, lengths, gated: bool, reverse: bool, scratch) -> tp.List[Launch]:
-    b, t, c = x.shape
-    return [Launch('recurrence', (_cdiv(c, 64), b, 1), (64, 1, 1), [(v, 0) for v in (h, last, factor, x, state, lengths)],
-                   _u32(t, c, gated, reverse), bytes_moved=4 * 3 * x.size, written=(0, 1))]
+RECURRENCE_THREADS = 256
+#steps per thread by channels per lane
+RECURRENCE_STEPS, RECURRENCE_GRAD_STEPS = {4: 8, 1: 16}, {4: 4, 1: 8}
+RECURRENCE_CHAIN_CHANNELS = 64          #channels of a tile whose state goes on to another one
+
+
+class RecurrenceTiling(tp.NamedTuple):
+    vec:     int            #channels per lane
+    steps:   int            #steps per thread
+    lanes:   int            #lanes per step
+    cstrips: int            #strips of channels per sequence
+    strips:  int
+    tiles:   int            #along time
+
+
+def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec: tp.Dict[int, int]) -> RecurrenceTiling:
+    '''How a recurrence is cut: as few groups of steps side by side as time needs, and with the lanes that leaves as many channels as
+    there are, but at most RECURRENCE_CHAIN_CHANNELS where time takes more than one tile.'''
+    vec   = 4 if channels % 4 == 0 else 1
+    steps = 1 if time == 1 else steps_by_vec[vec]
+    wide  = _pow2_at_least(_cdiv(channels, vec))
+    lanes = min(wide, RECURRENCE_THREADS // min(_pow2_at_least(_cdiv(time, steps)), RECURRENCE_THREADS))
+    lanes = max(lanes, min(wide, RECURRENCE_CHAIN_CHANNELS // vec))
+    cstrips = _cdiv(channels, lanes * vec)
+    tiles   = _cdiv(time, steps * (RECURRENCE_THREADS // lanes))
+    if batch * cstrips * tiles * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
+        raise NotImplementedError(f'a recurrence over {channels} channels in {batch} sequences of {time} steps')
+    return RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
+
+
+def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int) -> Launch:
+    _, t, c = shape
+    kernel  = f'{name}_v{tiling.vec}' + ('_l1' if tiling.steps == 1 else '') + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
+    #(what tiles hand on: a line for the ticket, then a word of 64 bits per channel and tile)
+    chain   = None if tiling.tiles == 1 else zeroed(16 + 2 * tiling.tiles * tiling.strips * tiling.lanes * tiling.vec, f'{kernel} {tuple(tiling)}')
+    buffers = [(v, 0) for v in arrays] + [(chain, 0)]
+    return Launch(kernel, (tiling.strips * tiling.tiles, 1, 1), (RECURRENCE_THREADS, 1, 1), buffers,
+                  _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=True,
+                  written=written + ((len(arrays),) if chain is not None else ()), scratch=(len(arrays),) if chain is not None else ())
+
+
+def _recurrence_shape(x: Buffer, lengths):
+    #single steps of all sequences lie side by side
+    return (1, 1, x.size) if x.shape[1] == 1 and lengths is None else x.shape
+
+
+def linear_recurrence(h, last, factor: Buffer, x: Buffer, state, lengths, gated: bool, reverse: bool, zeroed) -> tp.List[Launch]:
+    shape = _recurrence_shape(x, lengths)
+    return [_recurrence_launch('recurrence', x, recurrence_tiling(*shape, RECURRENCE_STEPS), shape, gated, reverse, zeroed,
+                               (h, last, factor, x, state, lengths), (0, 1), 4 * (3 * x.size + 2 * x.shape[0] * x.shape[2]))]
 
 
 def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Buffer, state, lengths, g, g_last, gated: bool, reverse: bool,
-                           scratch) -> tp.List[Launch]:
-    b, t, c = x.shape
-    return [Launch('recurrence_grad', (_cdiv(c, 64), b, 1), (64, 1, 1), [(v, 0) for v in (dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last)],
-                   _u32(t, c, gated, reverse), bytes_moved=4 * 6 * x.size, written=(0, 1, 2))]
+                           zeroed) -> tp.List[Launch]:
+    shape = _recurrence_shape(x, lengths)
+    return [_recurrence_launch('recurrence_grad', x, recurrence_tiling(*shape, RECURRENCE_GRAD_STEPS), shape, gated, reverse, zeroed,
+                               (dfactor, dx, dstate, h, factor, x if gated else None, state, lengths, g, g_last), (0, 1, 2),
+                               4 * ((5 + gated) * x.size + 2 * x.shape[0] * x.shape[2]))]

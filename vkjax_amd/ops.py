@@ -1137,23 +1137,24 @@ def _recurrence_buffers(ins, params):
 
 def linear_recurrence(bufferpool, equation):
     p = equation.params
-    ins, (h, last), scratch = _operator_buffers(bufferpool, equation)
+    ins, (h, last), _ = _operator_buffers(bufferpool, equation)
     factor, x, state, lengths, _ = _recurrence_buffers(ins, p)
     if x.size == 0:
         return _held_state(equation, last, state)
-    return _operator_ops(equation, K.linear_recurrence(h, last, factor, x, state, lengths, p['gated'], p['reverse'], scratch))
+    return _operator_ops(equation, K.linear_recurrence(h, last, factor, x, state, lengths, p['gated'], p['reverse'],
+                                                       bufferpool.zeroed_scratch))
 
 
 def linear_recurrence_grad(bufferpool, equation):
     p = equation.params
-    (h, *ins), (dfactor, dx, dstate), scratch = _operator_buffers(bufferpool, equation)
+    (h, *ins), (dfactor, dx, dstate), _ = _operator_buffers(bufferpool, equation)
     factor, x, state, lengths, rest = _recurrence_buffers(ins, p)
     g      = rest.pop(0) if p['has_g'] else None
     g_last = rest.pop(0) if p['has_last'] else None
     if x.size == 0:
         return _held_state(equation, dstate, g_last)
     return _operator_ops(equation, K.linear_recurrence_grad(dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last, p['gated'],
-                                                            p['reverse'], scratch))
+                                                            p['reverse'], bufferpool.zeroed_scratch))
 
 
 def _held_state(equation, out, source):
