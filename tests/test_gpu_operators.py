@@ -397,8 +397,11 @@ def test_a_token_models_training_step(kwargs):
         program.upload_inputs(*args)
         for _ in range(3):
             program.replay(1)
-            for a, b in zip(program.read_outputs(), again):
-                assert np.array_equal(a.reshape(b.shape), b)
+            for k, (a, b) in enumerate(zip(program.read_outputs(), again)):
+                #the embedding's gradient is added up by atomics, in any order: a row's sum of at most 132 terms, off by as many u of
+                #their magnitudes on either side, which are no larger than the largest value times their number
+                table = k == 2 + sorted(args[0]).index('table')
+                assert np.array_equal(a.reshape(b.shape), b) or (table and np.abs(a.reshape(b.shape) - b).max() <= 2 * 132 * U * 132 * np.abs(b).max())
 
 
 def test_operators_give_the_same_bits_every_time():

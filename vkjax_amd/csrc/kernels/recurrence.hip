@@ -8,7 +8,7 @@
 // A thread reads its L steps into registers and composes them to one map h -> A h + H; maps compose to maps
 // (A2 (A1 h + H1) + H2), so a scan across the lanes of a wave and the four waves tells every thread the map in front of its own
 // steps. What is still missing is the state in front of the tile; with it a thread goes through its steps once more, from
-// registers, and stores. Groups of 16 lanes x 4 channels read whole 256-byte pieces of every step, 16 KB per wave in flight.
+// registers, and stores. Groups of 8 lanes x 4 channels read whole lines of 128 bytes of every step, 32 KB per wave in flight.
 //
 // The state in front of a tile (where time has more than one): tiles hand it on within the launch. A tile publishes its map (A, H) as
 // soon as it has it, and the state behind it as soon as it knows that; it looks at the WINDOW tiles before it until one of them
@@ -20,7 +20,11 @@
 //     own use too) telling launches apart: its value alternates from launch to launch, and every launch writes every word. A state
 //     is marked by a NaN of its own in the place of A. No fence is needed, since a word holds all that is read, and nothing has to be
 //     cleared: the tickets count on through the launches, so their quotient is the launch's number.
-// Measured against the alternatives in this file's history: see the figures at the kernels.
+// What bounds it: memory, with two waves per SIMD; while a tile waits for its state the other block of its CU loads. 65536 steps of 1024
+// channels (805 MB) 152 us, 5.3 TB/s, where a large copy by a library reaches 5.1-5.5; 8 x 2048 x 2048 with ragged lengths 70 us, and
+// its gradient 140 us (716 MB). Smaller tiles have more words to look at and more ends to wait for: 8 steps per thread 160 us, 4 steps
+// 250. Strips of 64 channels 10-15 % slower (fewer chains side by side), of 16 20 % (half lines). Blocks that draw a tile ahead and
+// load it while they wait hold up the tiles behind it: 265 us.
 #include "common.h"
 
 struct RecurrenceParams {
@@ -28,7 +32,7 @@ struct RecurrenceParams {
     uint32_t T, C, cstrips, strips, log2_w, reverse;
 };
 
-constexpr uint32_t THREADS = 256, WINDOW = 16, CHAIN_CHANNELS = 64;
+constexpr uint32_t THREADS = 256, WINDOW = 16, CHAIN_CHANNELS = 32;
 constexpr uint32_t STATE_MARK = 0x7FC01230u, MAP_NAN = 0x7FE00000u;
 
 // sigmoid(gate) and 1 - sigmoid(gate), each rounded from the exponential: neither is the difference of the other to 1
@@ -46,7 +50,11 @@ __device__ __forceinline__ uint32_t length_of(const int32_t* lengths, uint32_t b
 }
 
 template <int VEC> __device__ __forceinline__ void load(float (&v)[VEC], __amdgpu_buffer_rsrc_t r, uint32_t at) {
-    if constexpr (VEC == 4) { const f32x4 t = buffer_load_x4(r, at); v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
+    // (past the caches: nothing is read twice. 3 % of a launch)
+    if constexpr (VEC == 4) {
+        const f32x4 t = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 2));
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    }
     else v[0] = buffer_load_x1(r, at);
 }
 template <int VEC> __device__ __forceinline__ void store(const float (&v)[VEC], __amdgpu_buffer_rsrc_t r, uint32_t at, bool stream = false) {
@@ -106,7 +114,7 @@ struct Tile {
     __device__ uint32_t state_at() const { return c0 + col * VEC < C ? col * VEC * 4u : NOWHERE; }
 
     // In: the map of this thread's steps. Out: the state in front of them, given the one in front of the first tile.
-    __device__ void state_before(float (&A)[VEC], float (&H)[VEC], const float (&initial)[VEC], float (&now)[VEC]) {
+    __device__ void state_before(float (&A)[VEC], float (&H)[VEC], const float* initial_states, float (&now)[VEC]) {
         __shared__ float parts[4][64][2 * VEC];
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         for (uint32_t off = W; off < 64u; off <<= 1) {
@@ -138,71 +146,63 @@ struct Tile {
                 fh[j] = __builtin_fmaf(pa, fh[j], ph); fa[j] *= pa;
             }
         float s[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[j] = initial[j];
-        if constexpr (CHAIN) state_of_tile(parts, initial, s);
+        if constexpr (CHAIN) state_of_tile(parts, initial_states, s);
+        else load<VEC>(s, state_rsrc(initial_states), state_at());
 #pragma unroll
         for (int j = 0; j < VEC; ++j) now[j] = __builtin_fmaf(before_a[j], __builtin_fmaf(fa[j], s[j], fh[j]), before_h[j]);
     }
 
-    // The state in front of this tile, from the tiles before it; publishes this one's map and state.
-    __device__ void state_of_tile(const float (&parts)[4][64][2 * VEC], const float (&initial)[VEC], float (&s)[VEC]) {
-        __shared__ unsigned long long window[WINDOW][CHAIN_CHANNELS];
+    // The state in front of this tile, from the tiles before it; publishes this one's map and state. The first wave does it, a lane per channel and half of
+    // the window: the halves' words are all in flight together, the second half's lanes go on from the state that the first one's have found.
+    __device__ void state_of_tile(const float (&parts)[4][64][2 * VEC], const float* initial_states, float (&s)[VEC]) {
         __shared__ float front[CHAIN_CHANNELS];
         const uint32_t channels = W * VEC;
-        const bool lead = group == 0u;                                    // the threads that follow the chain: the first group
-        unsigned long long* const own = words + ((uint64_t)k * strips + strip) * channels + col * VEC;
-        float ta[VEC], th[VEC];
-        if (lead) {
+        if (threadIdx.x < 64u) {
+            constexpr int HALF = WINDOW / 2;
+            const uint32_t channel = threadIdx.x & (CHAIN_CHANNELS - 1u), from = channel / VEC, j = channel % VEC;
+            const bool second = threadIdx.x >= CHAIN_CHANNELS, use = channel < channels;
+            unsigned long long* const mine = words + (uint64_t)strip * channels + (use ? channel : 0u);
+            const uint64_t step = (uint64_t)strips * channels;               // to the next tile's word
+            float a = 1.f, h = 0.f;
+            for (uint32_t p = 0; p < 4u; ++p) { const float pa = parts[p][use ? from : 0u][j], ph = parts[p][use ? from : 0u][VEC + j]; h = __builtin_fmaf(pa, h, ph); a *= pa; }
+            // A with its lowest bit cleared, rounded to nearest, ties to even: an error of up to 2^-23 of it once per tile, as much as two of the tile's
+            // own multiplications
+            const uint32_t bits = f2u(a), even = a != a ? MAP_NAN : (bits + ((bits >> 1) & 1u)) & ~1u;
+            a = u2f(even);
+            if (use && !second) __hip_atomic_store(mine + k * step, (unsigned long long)f2u(h) << 32 | even | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float initial = buffer_load_x1(state_rsrc(initial_states), use && c0 + channel < C ? channel * 4u : NOWHERE);
+            float state = initial;
+            if (k > 0u) {
+                const int e0 = (int)k - (int)WINDOW + (second ? HALF : 0);    // this lane's first tile (tile -1: what the sequence starts with)
+                for (;;) {
+                    unsigned long long word[HALF];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                ta[j] = 1.f; th[j] = 0.f;
-                for (uint32_t p = 0; p < 4u; ++p) { const float pa = parts[p][col][j], ph = parts[p][col][VEC + j]; th[j] = __builtin_fmaf(pa, th[j], ph); ta[j] *= pa; }
-                // A with its lowest bit cleared, rounded to nearest, ties to even: an error of up to 2^-23 of it once per tile, as much as two of the tile's
-                // own multiplications
-                const uint32_t bits = f2u(ta[j]), even = ta[j] != ta[j] ? MAP_NAN : (bits + ((bits >> 1) & 1u)) & ~1u;
-                ta[j] = u2f(even);
-                __hip_atomic_store(own + j, (unsigned long long)f2u(th[j]) << 32 | even | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
-        if (k > 0u) {
-            for (;;) {
-                for (uint32_t e = group; e < WINDOW; e += G) {
-                    const int p = (int)(k + e) - (int)WINDOW;             // (tile -1: what the sequence starts with)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        unsigned long long word = p == -1 ? (unsigned long long)f2u(initial[j]) << 32 | STATE_MARK | tag : (unsigned long long)(tag ^ 1u);
-                        if (p >= 0) word = __hip_atomic_load(words + ((uint64_t)p * strips + strip) * channels + col * VEC + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        window[e][col * VEC + j] = word;
+                    for (int e = 0; e < HALF; ++e) {
+                        word[e] = e0 + e == -1 ? (unsigned long long)f2u(initial) << 32 | STATE_MARK | tag : (unsigned long long)(tag ^ 1u);
+                        if (e0 + e >= 0) word[e] = __hip_atomic_load(mine + (uint64_t)(e0 + e) * step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                     }
-                }
-                __syncthreads();
-                bool known = true;
-                if (lead) {
+                    bool found = false;
+                    auto follow = [&]() {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        bool found = false;
-                        for (uint32_t e = 0; e < WINDOW; ++e) {
-                            const unsigned long long word = window[e][col * VEC + j];
-                            const uint32_t low = (uint32_t)word;
-                            const float value = u2f((uint32_t)(word >> 32));
-                            const bool current = (low & 1u) == tag, is_state = (low & ~1u) == STATE_MARK;
-                            s[j] = is_state ? value : __builtin_fmaf(u2f(low & ~1u), s[j], value);
-                            found = current && (is_state || found);
+                        for (int e = 0; e < HALF; ++e) {
+                            const uint32_t low = (uint32_t)word[e];
+                            const float value = u2f((uint32_t)(word[e] >> 32));
+                            const bool is_state = (low & ~1u) == STATE_MARK;
+                            state = is_state ? value : __builtin_fmaf(u2f(low & ~1u), state, value);
+                            found = (low & 1u) == tag && (is_state || found);
                         }
-                        known = known && found;
-                    }
+                    };
+                    follow();
+                    const float state_before = __shfl(state, channel);          // (of the first half)
+                    const bool found_before = __shfl((int)found, channel) != 0;
+                    if (second) { state = state_before; found = found_before; follow(); }
+                    if (__builtin_amdgcn_ballot_w64(second && use && !found) == 0ull) break;
+                    __builtin_amdgcn_s_sleep(1);
                 }
-                if (!__syncthreads_or(!known)) break;
-                __builtin_amdgcn_s_sleep(1);
             }
-        }
-        if (lead) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float behind = __builtin_fmaf(ta[j], s[j], th[j]);
-                __hip_atomic_store(own + j, (unsigned long long)f2u(behind) << 32 | STATE_MARK | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                front[col * VEC + j] = s[j];
+            if (second || k == 0u) {
+                if (use && second) __hip_atomic_store(mine + k * step, (unsigned long long)f2u(__builtin_fmaf(a, state, h)) << 32 | STATE_MARK | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (use) front[channel] = state;
             }
         }
         __syncthreads();
@@ -217,14 +217,13 @@ __device__ __forceinline__ void recurrence_body(float* h, float* last, const flo
                                                 const RecurrenceParams& P) {
     Tile<VEC, L, CHAIN> tile(P, lengths, chain, P.reverse != 0u);
     const __amdgpu_buffer_rsrc_t f_rsrc = tile.rsrc(factor), x_rsrc = tile.rsrc(x);
-    float a[L][VEC], b[L][VEC], A[VEC], H[VEC], initial[VEC], now[VEC];
+    float a[L][VEC], b[L][VEC], A[VEC], H[VEC], now[VEC];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
         const uint32_t at = tile.at(i, tile.inside(i));
         load<VEC>(a[i], f_rsrc, at);
         load<VEC>(b[i], x_rsrc, at);
     }
-    load<VEC>(initial, tile.state_rsrc(state), tile.state_at());
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { A[j] = 1.f; H[j] = 0.f; }
 #pragma unroll
@@ -241,7 +240,7 @@ __device__ __forceinline__ void recurrence_body(float* h, float* last, const flo
             H[j] = __builtin_fmaf(a[i][j], H[j], b[i][j]); A[j] *= a[i][j];
         }
     }
-    tile.state_before(A, H, initial, now);
+    tile.state_before(A, H, state, now);
     const __amdgpu_buffer_rsrc_t h_rsrc = tile.rsrc(h);
     const bool stream = streams_result(P.first);
 #pragma unroll
@@ -258,7 +257,7 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
                                                      const int32_t* lengths, const float* g, const float* g_last, unsigned long long* chain, const RecurrenceParams& P) {
     Tile<VEC, L, CHAIN> tile(P, lengths, chain, P.reverse == 0u);
     const __amdgpu_buffer_rsrc_t f_rsrc = tile.rsrc(factor), x_rsrc = tile.rsrc(GATED ? x : nullptr), g_rsrc = tile.rsrc(g), h_rsrc = tile.rsrc(h, P.reverse ? 1 : -1);
-    float gs[L][VEC], a[L][VEC], before[L][VEC], rest[GATED ? L : 1][VEC], A[VEC], H[VEC], initial[VEC], now[VEC];
+    float gs[L][VEC], a[L][VEC], before[L][VEC], rest[GATED ? L : 1][VEC], A[VEC], H[VEC], now[VEC];
     const uint32_t start = P.reverse ? P.T - 1u : 0u;                    // the time of the recurrence's first step
 #pragma unroll
     for (int i = 0; i < L; ++i) {
@@ -269,7 +268,6 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
         if constexpr (GATED) load<VEC>(rest[i], x_rsrc, tile.at(i, inside));
         if (first && state) load<VEC>(before[i], tile.state_rsrc(state), inside ? tile.state_at() : NOWHERE);
     }
-    load<VEC>(initial, tile.state_rsrc(g_last), tile.state_at());
 #pragma unroll
     for (int j = 0; j < VEC; ++j) { A[j] = 1.f; H[j] = 0.f; }
 #pragma unroll
@@ -287,7 +285,7 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
             H[j] = a[i][j] * (H[j] + gs[i][j]); A[j] *= a[i][j];
         }
     }
-    tile.state_before(A, H, initial, now);
+    tile.state_before(A, H, g_last, now);
     const __amdgpu_buffer_rsrc_t df_rsrc = tile.rsrc(dfactor), dx_rsrc = tile.rsrc(dx);
     const bool stream = streams_result(P.first);
 #pragma unroll
@@ -311,12 +309,12 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
 
 // Names: _v<channels per lane>_l<steps per thread>, _gated, _chain (more tiles than one along time)
 #define RECURRENCE(name, VEC, L, GATED, CHAIN)                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void recurrence_##name(float* h, float* last, const float* factor, const float* x, const float* state, \
+    extern "C" __global__ __launch_bounds__(256, 2) void recurrence_##name(float* h, float* last, const float* factor, const float* x, const float* state, \
                                                                         const int32_t* lengths, unsigned long long* chain, RecurrenceParams P) {        \
         recurrence_body<VEC, L, GATED, CHAIN>(h, last, factor, x, state, lengths, chain, P);                                                            \
     }
 #define RECURRENCE_GRAD(name, VEC, L, GATED, CHAIN)                                                                                                     \
-    extern "C" __global__ __launch_bounds__(256) void recurrence_grad_##name(float* dfactor, float* dx, float* dstate, const float* h, const float* factor, \
+    extern "C" __global__ __launch_bounds__(256, 2) void recurrence_grad_##name(float* dfactor, float* dx, float* dstate, const float* h, const float* factor, \
             const float* x, const float* state, const int32_t* lengths, const float* g, const float* g_last, unsigned long long* chain, RecurrenceParams P) { \
         recurrence_grad_body<VEC, L, GATED, CHAIN>(dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last, chain, P);                             \
     }
@@ -327,5 +325,5 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
     KERNEL(v1_l1, 1, 1, false, false)            KERNEL(v1_l1_gated, 1, 1, true, false)                             \
     KERNEL(v1, 1, LONG1, false, false)           KERNEL(v1_gated, 1, LONG1, true, false)                            \
     KERNEL(v1_chain, 1, LONG1, false, true)      KERNEL(v1_gated_chain, 1, LONG1, true, true)
-RECURRENCE_VARIANTS(RECURRENCE, 8, 16)
-RECURRENCE_VARIANTS(RECURRENCE_GRAD, 4, 8)
+RECURRENCE_VARIANTS(RECURRENCE, 16, 16)
+RECURRENCE_VARIANTS(RECURRENCE_GRAD, 6, 8)

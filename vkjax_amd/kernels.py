@@ -2233,8 +2233,8 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
 
 RECURRENCE_THREADS = 256
 #steps per thread by channels per lane
-RECURRENCE_STEPS, RECURRENCE_GRAD_STEPS = {4: 8, 1: 16}, {4: 4, 1: 8}
-RECURRENCE_CHAIN_CHANNELS = 64          #channels of a tile whose state goes on to another one
+RECURRENCE_STEPS, RECURRENCE_GRAD_STEPS = {4: 16, 1: 16}, {4: 6, 1: 8}
+RECURRENCE_CHAIN_CHANNELS = 32          #channels of a tile whose state goes on to another one
 
 
 class RecurrenceTiling(tp.NamedTuple):
