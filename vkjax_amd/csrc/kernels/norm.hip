@@ -5,87 +5,591 @@
 //   d = g act'(z);  dshift = sum d,  dscale = sum d hat  (over samples and positions)
 //   dx = rstd (d scale - mean(d scale) - hat mean(d scale hat))  (means over the group)
 //
-// Sums and statistics are held in 32 bits; the variance is summed from deviations from the mean, never as a difference of
-// squares, so that activations far from zero keep theirs.
+// Sums and statistics are held in 32 bits. The variance is never a difference of squares: a thread has mean and squared deviations of
+// its own values, and those are joined by n1 (mean1 - mean)^2 terms (Chan, Golub, LeVeque), so activations far from zero keep theirs.
+//
+// A block owns a span of channels (whole groups, or a piece of one that is too wide for a block): V lanes of VEC channels each read a
+// position's span, and 256 / V (1024 / V) positions are read side by side. A lane's channels stay the same, so what belongs to a channel
+// is in registers, and reading and writing are whole lines wherever a span has 32 channels. What the positions' lanes have found meets in
+// shared memory, where a few lanes per group add it up.
+//   * group_norm_held: samples small enough stay in registers: one launch that reads once and writes once. Several small samples share a
+//     block.
+//   * group_norm_stats / _apply: the others are cut along their positions. The first launch leaves mean and squared deviations of each
+//     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it).
+// The gradient has the same two forms; what dscale and dshift get from a block is a row of sums per block, added up by a last launch
+// (group_norm_columns) in a fixed order: no atomics.
 #include "common.h"
 
 enum Activation : uint32_t { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2 };
 
-struct NormParams { uint32_t first; uint32_t S, C, G, cg, act; float eps; };
+struct NormParams {
+    uint32_t first;                         // (bit 31: the result is stored past the caches)
+    uint32_t N, S, C, G, cg, act; float eps;
+    uint32_t span, spans, pieces;           // channels of a block, blocks per row of channels, blocks per group where it is wider than a block (else 1)
+    uint32_t V, P, M;                       // lanes per position, positions side by side (of one sample), samples side by side
+    uint32_t log2_lc, log2_lq;              // lanes per group in the joining step: along its channels, along positions
+    uint32_t chunks, chunk;                 // chunks of positions per sample, positions in one
+};
 
+constexpr uint32_t NOWHERE = 0x80000000u;
+
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);             // a Newton step
+}
+// 1 / (1 + exp(-z)); exp(-z) beyond fp32 is infinite and its reciprocal 0, where the Newton step would make a NaN of infinity times 0
+__device__ __forceinline__ float sigmoid(float z) {
+    const float e = expf(-z);
+    return e > 1e38f ? 0.f : reciprocal(1.f + e);
+}
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
     if (act == ACT_RELU) return (z > 0.f || z != z) ? z : 0.f;
-    if (act == ACT_SILU) return z / (1.f + expf(-z));
+    if (act == ACT_SILU) return z * sigmoid(z);
     return z;
 }
 // g * act'(z)
 __device__ __forceinline__ float act_gradient(float g, float z, uint32_t act) {
     if (act == ACT_RELU) return z > 0.f ? g : 0.f;
-    if (act == ACT_SILU) { const float s = 1.f / (1.f + expf(-z)); return g * (s * (1.f + z * (1.f - s))); }
+    if (act == ACT_SILU) { const float s = sigmoid(z); return g * (s * __builtin_fmaf(z, 1.f - s, 1.f)); }
     return g;
 }
 
-// The sum over a block of 256 threads, in every thread; `room`: 4 floats of LDS that nothing else uses.
-__device__ __forceinline__ float block_sum(float v, float* room) {
-    v = lanes_allreduce(v, 64u, [](float a, float b) { return a + b; });
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) room[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (room[0] + room[1]) + (room[2] + room[3]);
+template <int VEC> __device__ __forceinline__ void load(float (&v)[VEC], __amdgpu_buffer_rsrc_t r, uint32_t at) {
+    if constexpr (VEC == 4) { const f32x4 t = buffer_load_x4(r, at); v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
+    else v[0] = buffer_load_x1(r, at);
 }
-
-// One block per sample and group.
-extern "C" __global__ __launch_bounds__(256) void group_norm(float* y, float* mean_out, float* rstd_out, const float* x, const float* scale, const float* shift, NormParams P) {
-    __shared__ float room[4];
-    const uint32_t n = blockIdx.x / P.G, group = blockIdx.x % P.G;
-    const uint64_t base = (uint64_t)n * P.S * P.C + group * P.cg;
-    const uint64_t count = (uint64_t)P.S * P.cg;
-    auto place = [&](uint64_t e) { return base + e / P.cg * P.C + e % P.cg; };
-    float sum = 0.f;
-    for (uint64_t e = threadIdx.x; e < count; e += 256) sum += x[place(e)];
-    const float mean = block_sum(sum, room) / (float)count;
-    float square = 0.f;
-    for (uint64_t e = threadIdx.x; e < count; e += 256) { const float d = x[place(e)] - mean; square += d * d; }
-    const float rstd = 1.f / sqrtf(block_sum(square, room) / (float)count + P.eps);
-    if (threadIdx.x == 0) {
-        if (mean_out) mean_out[blockIdx.x] = mean;
-        if (rstd_out) rstd_out[blockIdx.x] = rstd;
-    }
-    if (y == nullptr) return;
-    for (uint64_t e = threadIdx.x; e < count; e += 256) {
-        const uint32_t c = group * P.cg + (uint32_t)(e % P.cg);
-        y[place(e)] = act_value((x[place(e)] - mean) * rstd * scale[c] + shift[c], P.act);
+template <int VEC> __device__ __forceinline__ void store(const float (&v)[VEC], __amdgpu_buffer_rsrc_t r, uint32_t at, bool stream) {
+    if constexpr (VEC == 4) {
+        const u32x4 t = u32x4{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+        if (stream) __builtin_amdgcn_raw_buffer_store_b128(t, r, at, 0, 2);
+        else __builtin_amdgcn_raw_buffer_store_b128(t, r, at, 0, 0);
+    } else {
+        if (stream) __builtin_amdgcn_raw_buffer_store_b32(f2u(v[0]), r, at, 0, 2);
+        else __builtin_amdgcn_raw_buffer_store_b32(f2u(v[0]), r, at, 0, 0);
     }
 }
 
-// One block per sample and group: dx, and the sample's share of dscale and dshift ([2, N, C]).
-extern "C" __global__ __launch_bounds__(256) void group_norm_grad(float* dx, float* shares, const float* g, const float* x, const float* scale, const float* shift,
-                                                                  const float* means, const float* rstds, NormParams P, uint32_t N) {
-    __shared__ float room[4];
-    const uint32_t n = blockIdx.x / P.G, group = blockIdx.x % P.G;
-    const uint64_t base = (uint64_t)n * P.S * P.C + group * P.cg;
-    const float mean = means[blockIdx.x], rstd = rstds[blockIdx.x];
-    float first = 0.f, second = 0.f;
-    for (uint32_t k = 0; k < P.cg; ++k) {
-        const uint32_t c = group * P.cg + k;
-        float d_sum = 0.f, dh_sum = 0.f;
-        for (uint32_t s = threadIdx.x; s < P.S; s += 256) {
-            const uint64_t at = base + (uint64_t)s * P.C + k;
-            const float hat = (x[at] - mean) * rstd, d = act_gradient(g[at], hat * scale[c] + shift[c], P.act);
-            d_sum += d; dh_sum += d * hat;
+extern __shared__ float room[];
+
+// A span of channels and this thread's part of it.
+template <int VEC>
+struct Span {
+    uint32_t c0, width, groups, g0;         // first channel, channels, whole groups in it (1 of a piece), its first group
+    uint32_t col, p, c;                     // this thread's lane within a position, its place among the positions, its first channel
+    __device__ Span(const NormParams& P, uint32_t number) {
+        if (P.pieces == 1u) {
+            c0 = number * P.span; width = min(P.span, P.C - c0);
+            groups = width / P.cg; g0 = c0 / P.cg;
+        } else {
+            const uint32_t piece = number % P.pieces;
+            g0 = number / P.pieces; groups = 1u;
+            c0 = g0 * P.cg + piece * P.span; width = min(P.span, P.cg - piece * P.span);
         }
-        d_sum = block_sum(d_sum, room); dh_sum = block_sum(dh_sum, room);
-        if (threadIdx.x == 0) { shares[(uint64_t)n * P.C + c] = dh_sum; shares[((uint64_t)N + n) * P.C + c] = d_sum; }
-        first += d_sum * scale[c]; second += dh_sum * scale[c];
+        p = threadIdx.x / P.V; col = threadIdx.x - p * P.V;
+        c = c0 + col * VEC;
     }
-    if (dx == nullptr) return;
+    __device__ bool owns() const { return col * VEC < width; }
+    __device__ uint32_t group_of(const NormParams& P, int j) const { return P.pieces == 1u ? (col * VEC + j) / P.cg : 0u; }      // within the span
+};
+
+// Goes through the entries of every group in shared memory, a few lanes to a group: entry.add for each, entry.join across the lanes, a second
+// round where entry.again(), and done(sample, group, whether this lane reports it, entry). Entries lie at (sample * P + position's lane) * span + channel.
+template <class Entry, class Done>
+__device__ __forceinline__ void for_groups(const NormParams& P, uint32_t groups, uint32_t channels_per_group, uint32_t samples, Entry entry, Done done) {
+    const uint32_t log2_lanes = P.log2_lc + P.log2_lq, lanes = 1u << log2_lanes, lane = threadIdx.x & (lanes - 1u);
+    const uint32_t lc = lane & ((1u << P.log2_lc) - 1u), lq = lane >> P.log2_lc, sets = blockDim.x >> log2_lanes;
+    const uint32_t all = groups * samples;
+    for (uint32_t at = threadIdx.x >> log2_lanes; at - (threadIdx.x >> log2_lanes) < all; at += sets) {      // (every lane goes round as often: lanes meet below)
+        const bool use = at < all;
+        const uint32_t m = use ? at / groups : 0u, g = use ? at - m * groups : 0u;
+        entry.start();
+        if (use)
+            for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq)
+                for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) entry.add((m * P.P + q) * P.span + g * channels_per_group + ch, q, g * channels_per_group + ch);
+        entry.join(lanes);
+        if (use && entry.again())
+            for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq)
+                for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) entry.add_again((m * P.P + q) * P.span + g * channels_per_group + ch, q);
+        entry.join_again(lanes);
+        if (use) done(m, g, lane == 0u, entry);
+    }
+}
+
+__device__ __forceinline__ float add_lanes(float v, uint32_t lanes) { return lanes_allreduce(v, lanes, [](float a, float b) { return a + b; }); }
+
+// Mean and squared deviations of a group from the sums and squared deviations of (thread, channel): `count(q)` values each.
+template <class Count>
+struct JoinStats {
+    const float *sums, *squares;
+    Count count;
+    float total, sum, mean, square;
+    __device__ void start() { total = sum = square = 0.f; mean = 0.f; }
+    __device__ void add(uint32_t at, uint32_t q, uint32_t) { sum += sums[at]; total += count(q); }
+    __device__ void join(uint32_t lanes) { sum = add_lanes(sum, lanes); total = add_lanes(total, lanes); mean = sum / total; }
+    __device__ bool again() const { return true; }
+    __device__ void add_again(uint32_t at, uint32_t q) {
+        const float n = count(q), d = n > 0.f ? sums[at] / n - mean : 0.f;
+        square += __builtin_fmaf(n * d, d, squares[at]);
+    }
+    __device__ void join_again(uint32_t lanes) { square = add_lanes(square, lanes); }
+};
+// The sums of scale * first and scale * second over a group.
+struct JoinSums {
+    const float *first, *second, *scale;       // (scale: of the span's first channel)
+    float a, b;
+    __device__ void start() { a = b = 0.f; }
+    __device__ void add(uint32_t at, uint32_t, uint32_t channel) { const float s = scale[channel]; a = __builtin_fmaf(s, first[at], a); b = __builtin_fmaf(s, second[at], b); }
+    __device__ void join(uint32_t lanes) { a = add_lanes(a, lanes); b = add_lanes(b, lanes); }
+    __device__ bool again() const { return false; }
+    __device__ void add_again(uint32_t, uint32_t) {}
+    __device__ void join_again(uint32_t) {}
+};
+
+// How many of `count` positions the lane q of `side` side by side has.
+__device__ __forceinline__ uint32_t share_of(uint32_t count, uint32_t q, uint32_t side) { return count > q ? (count - q - 1u) / side + 1u : 0u; }
+
+// ---------------------------------------------------------------------------------------------- samples that stay in registers
+
+template <int VEC, int K>
+__device__ __forceinline__ void held_body(float* y, float* means, float* rstds, const float* x, const float* scale, const float* shift, const NormParams& P) {
+    const Span<VEC> span(P, blockIdx.x % P.spans);
+    const uint32_t n0 = blockIdx.x / P.spans * P.M, m = span.p / P.P, q = span.p - m * P.P;
+    const bool use = m < P.M && n0 + m < P.N && span.owns();
+    const uint64_t base = (uint64_t)n0 * P.S * P.C + span.c0;
+    const uint32_t bytes = ((min(P.M, P.N - n0) * P.S - 1u) * P.C + span.width) * 4u;
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(x + base, bytes);
+    const uint32_t first = ((m * P.S + q) * P.C + span.col * VEC) * 4u, step = P.P * P.C * 4u;
+    const uint32_t mine = use ? share_of(P.S, q, P.P) : 0u;
+    float v[K][VEC];
+#pragma unroll
+    for (int i = 0; i < K; ++i) load<VEC>(v[i], x_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE);
+    float gamma[VEC], beta[VEC];
+    {
+        const __amdgpu_buffer_rsrc_t a = make_rsrc(scale + span.c0, span.width * 4u), b = make_rsrc(shift + span.c0, span.width * 4u);
+        load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
+        load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
+    }
+    const uint32_t entries = P.M * P.P * P.span, groups_at_most = P.span / P.cg * P.M;
+    float* const sums = room, * const squares = room + entries, * const mean_of = room + 2u * entries, * const rstd_of = mean_of + groups_at_most;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        float sum = 0.f, square = 0.f;
+#pragma unroll
+        for (int i = 0; i < K; ++i) sum += v[i][j];                      // (beyond the sample: zeros)
+        const float mean = sum / (float)max(mine, 1u);
+#pragma unroll
+        for (int i = 0; i < K; ++i) { const float d = (uint32_t)i < mine ? v[i][j] - mean : 0.f; square = __builtin_fmaf(d, d, square); }
+        if (m < P.M && span.col * VEC + j < P.span) { sums[span.p * P.span + span.col * VEC + j] = sum; squares[span.p * P.span + span.col * VEC + j] = square; }
+    }
+    __syncthreads();
+    auto count = [&](uint32_t lane_q) { return (float)share_of(P.S, lane_q, P.P); };
+    JoinStats<decltype(count)> join{sums, squares, count};
+    for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t sample, uint32_t g, bool reports, const JoinStats<decltype(count)>& found) {
+        if (!reports) return;
+        const float rstd = 1.f / sqrtf(found.square / found.total + P.eps);
+        mean_of[sample * span.groups + g] = found.mean; rstd_of[sample * span.groups + g] = rstd;
+        if (n0 + sample < P.N) {
+            const uint64_t at = (uint64_t)(n0 + sample) * P.G + span.g0 + g;
+            if (means) means[at] = found.mean;
+            if (rstds) rstds[at] = rstd;
+        }
+    });
+    __syncthreads();
+    if (!use || y == nullptr) return;
+    const bool stream = streams_result(P.first);
+    const __amdgpu_buffer_rsrc_t y_rsrc = make_rsrc(y + base, bytes);
+    float mean[VEC], factor[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const uint32_t g = m * span.groups + span.group_of(P, j);
+        mean[j] = mean_of[g]; factor[j] = rstd_of[g] * gamma[j];
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf(v[i][j] - mean[j], factor[j], beta[j]), P.act);
+        store<VEC>(v[i], y_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE, stream);
+    }
+}
+
+// The gradient of samples that stay in registers. Blocks take one set of samples after the other; the row of sums for dscale and dshift of
+// a block is written at its end.
+template <int VEC, int K>
+__device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
+                                               const float* means, const float* rstds, const NormParams& P) {
+    const Span<VEC> span(P, blockIdx.x % P.spans);
+    const uint32_t m = span.p / P.P, q = span.p - m * P.P, entries = P.M * P.P * P.span, sets = (P.N - 1u) / P.M + 1u, row = blockIdx.x / P.spans, rows = gridDim.x / P.spans;
+    float* const firsts = room, * const seconds = room + entries, * const a_of = room + 2u * entries, * const b_of = a_of + P.span / P.cg * P.M;
+    float gamma[VEC], beta[VEC], d_total[VEC], dh_total[VEC];
+    {
+        const __amdgpu_buffer_rsrc_t a = make_rsrc(scale + span.c0, span.width * 4u), b = make_rsrc(shift + span.c0, span.width * 4u);
+        load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
+        load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { d_total[j] = 0.f; dh_total[j] = 0.f; }
     const float inverse = 1.f / ((float)P.S * (float)P.cg);
-    first *= inverse; second *= inverse;
-    const uint64_t count = (uint64_t)P.S * P.cg;
-    for (uint64_t e = threadIdx.x; e < count; e += 256) {
-        const uint64_t at = base + e / P.cg * P.C + e % P.cg;
-        const uint32_t c = group * P.cg + (uint32_t)(e % P.cg);
-        const float hat = (x[at] - mean) * rstd, d = act_gradient(g[at], hat * scale[c] + shift[c], P.act);
-        dx[at] = rstd * (d * scale[c] - first - hat * second);
+    const bool stream = streams_result(P.first);
+    for (uint32_t set = row; set < sets; set += rows) {
+        const uint32_t n0 = set * P.M;
+        const bool use = m < P.M && n0 + m < P.N && span.owns();
+        const uint64_t base = (uint64_t)n0 * P.S * P.C + span.c0;
+        const uint32_t bytes = ((min(P.M, P.N - n0) * P.S - 1u) * P.C + span.width) * 4u;
+        const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(x + base, bytes), g_rsrc = make_rsrc(gs + base, bytes);
+        const uint32_t first = ((m * P.S + q) * P.C + span.col * VEC) * 4u, step = P.P * P.C * 4u;
+        const uint32_t mine = use ? share_of(P.S, q, P.P) : 0u;
+        float v[K][VEC], d[K][VEC], mean[VEC], rstd[VEC], A[VEC], B[VEC];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            load<VEC>(v[i], x_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE);
+            load<VEC>(d[i], g_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const uint64_t at = (uint64_t)(n0 + m) * P.G + span.g0 + span.group_of(P, j);
+            mean[j] = use && span.col * VEC + j < span.width ? means[at] : 0.f; rstd[j] = use && span.col * VEC + j < span.width ? rstds[at] : 0.f;
+            A[j] = 0.f; B[j] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[i][j] = (v[i][j] - mean[j]) * rstd[j];
+                d[i][j] = act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act);
+                d[i][j] = (uint32_t)i < mine ? d[i][j] : 0.f; v[i][j] = (uint32_t)i < mine ? v[i][j] : 0.f;
+                A[j] += d[i][j]; B[j] = __builtin_fmaf(d[i][j], v[i][j], B[j]);
+            }
+        __syncthreads();                                                 // (what the set before has left has been read)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if (m < P.M && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = A[j]; seconds[span.p * P.span + span.col * VEC + j] = B[j]; }
+            d_total[j] += A[j]; dh_total[j] += B[j];
+        }
+        if (dx == nullptr) continue;
+        __syncthreads();
+        JoinSums join{firsts, seconds, scale + span.c0};
+        for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t sample, uint32_t g, bool reports, const JoinSums& found) {
+            if (reports) { a_of[sample * span.groups + g] = found.a * inverse; b_of[sample * span.groups + g] = found.b * inverse; }
+        });
+        __syncthreads();
+        const __amdgpu_buffer_rsrc_t dx_rsrc = make_rsrc(dx + base, bytes);
+        float a[VEC], b[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const uint32_t g = m * span.groups + span.group_of(P, j);
+            a[j] = use && span.col * VEC + j < span.width ? a_of[g] : 0.f; b[j] = use && span.col * VEC + j < span.width ? b_of[g] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = rstd[j] * (__builtin_fmaf(d[i][j], gamma[j], -a[j]) - v[i][j] * b[j]);
+            store<VEC>(v[i], dx_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE, stream);
+        }
     }
+    // the block's sums per channel, over its positions' and samples' lanes
+    __syncthreads();
+    const uint32_t all = P.M * P.P;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        if (span.p < all && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = d_total[j]; seconds[span.p * P.span + span.col * VEC + j] = dh_total[j]; }
+    __syncthreads();
+    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
+        float a = 0.f, b = 0.f;
+        for (uint32_t k = 0; k < all; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
+        dshift_rows[(uint64_t)row * P.C + span.c0 + ch] = a;
+        dscale_rows[(uint64_t)row * P.C + span.c0 + ch] = b;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- samples in chunks
+
+// Which chunk of which sample and span a block has.
+struct Chunk {
+    uint32_t number, n, from, count, chunk;
+    __device__ Chunk(const NormParams& P) {
+        number = blockIdx.x % P.spans;
+        const uint32_t rest = blockIdx.x / P.spans;
+        chunk = rest % P.chunks; n = rest / P.chunks;
+        from = chunk * P.chunk; count = min(P.chunk, P.S - from);
+    }
+};
+
+// U positions of a chunk in flight at a time: step(values, how many of the U are there)
+template <int VEC, int U, class Step>
+__device__ __forceinline__ void walk(const NormParams& P, const Span<VEC>& span, const Chunk& chunk, const float* x, Step step) {
+    const uint32_t mine = span.p < P.P && span.owns() ? share_of(chunk.count, span.p, P.P) : 0u;
+    const uint64_t base = ((uint64_t)chunk.n * P.S + chunk.from) * P.C + span.c0;
+    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(x + base, ((chunk.count - 1u) * P.C + span.width) * 4u);
+    for (uint32_t i = 0; i < mine; i += U) {
+        float v[U][VEC];
+#pragma unroll
+        for (int k = 0; k < U; ++k) load<VEC>(v[k], rsrc, i + k < mine ? ((span.p + (i + k) * P.P) * P.C + span.col * VEC) * 4u : NOWHERE);
+        step(v, min(mine - i, (uint32_t)U), i);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void stats_body(float* partial, const float* x, const NormParams& P) {
+    const Chunk chunk(P);
+    const Span<VEC> span(P, chunk.number);
+    constexpr int U = 8;
+    float mean[VEC], square[VEC], n = 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { mean[j] = 0.f; square[j] = 0.f; }
+    walk<VEC, U>(P, span, chunk, x, [&](const float (&v)[U][VEC], uint32_t here, uint32_t) {
+        // mean and squared deviations of these, joined with those before
+        const float count = (float)here, inverse = 1.f / count, share = count / (n + count), both = n * share;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float sum = 0.f, sq = 0.f;
+#pragma unroll
+            for (int k = 0; k < U; ++k) sum += v[k][j];
+            const float m = sum * inverse;
+#pragma unroll
+            for (int k = 0; k < U; ++k) { const float d = (uint32_t)k < here ? v[k][j] - m : 0.f; sq = __builtin_fmaf(d, d, sq); }
+            const float d = m - mean[j];
+            square[j] += __builtin_fmaf(d * d, both, sq);
+            mean[j] = __builtin_fmaf(d, share, mean[j]);
+        }
+        n += count;
+    });
+    const uint32_t entries = P.P * P.span;
+    float* const sums = room, * const squares = room + entries;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        if (span.p < P.P && span.col * VEC + j < P.span) { sums[span.p * P.span + span.col * VEC + j] = mean[j] * n; squares[span.p * P.span + span.col * VEC + j] = square[j]; }
+    __syncthreads();
+    auto count = [&](uint32_t q) { return (float)share_of(chunk.count, q, P.P); };
+    JoinStats<decltype(count)> join{sums, squares, count};
+    const uint32_t piece = P.pieces == 1u ? 0u : chunk.number % P.pieces;
+    for_groups(P, span.groups, P.pieces == 1u ? P.cg : span.width, 1u, join, [&](uint32_t, uint32_t g, bool reports, const JoinStats<decltype(count)>& found) {
+        if (!reports) return;
+        float* const to = partial + 2u * ((((uint64_t)chunk.n * P.G + span.g0 + g) * P.pieces + piece) * P.chunks + chunk.chunk);
+        to[0] = found.mean; to[1] = found.square;
+    });
+}
+
+// Joins what the chunks and pieces of the groups of a span have left, a few lanes to a group; `use(group, mean or first sum, deviations or
+// second sum)` in the lane that reports. STATS: means and squared deviations; else two sums.
+template <bool STATS, int VEC, class Use>
+__device__ __forceinline__ void join_chunks(const NormParams& P, const Span<VEC>& span, uint32_t n, const float* partial, Use use) {
+    const uint32_t parts = P.chunks * P.pieces, log2_lanes = 31u - (uint32_t)__clz((int)min(parts, 64u)), lanes = 1u << log2_lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1u), sets = blockDim.x >> log2_lanes;
+    const uint32_t start = threadIdx.x >> log2_lanes;
+    for (uint32_t g = start; g - start < span.groups; g += sets) {
+        const bool there = g < span.groups;
+        const float* const from = partial + 2u * ((uint64_t)n * P.G + span.g0 + (there ? g : 0u)) * parts;
+        auto count = [&](uint32_t k) {
+            const uint32_t piece = k / P.chunks, c = k - piece * P.chunks;
+            const uint32_t channels = P.pieces == 1u ? P.cg : min(P.span, P.cg - piece * P.span);
+            return (float)min(P.chunk, P.S - c * P.chunk) * (float)channels;
+        };
+        float a = 0.f, b = 0.f, total = 0.f;
+        for (uint32_t k = lane; k < parts; k += lanes) {
+            if constexpr (STATS) { const float c = count(k); a = __builtin_fmaf(from[2u * k], c, a); total += c; }
+            else { a += from[2u * k]; b += from[2u * k + 1u]; }
+        }
+        a = add_lanes(a, lanes);
+        if constexpr (STATS) {
+            total = add_lanes(total, lanes);
+            a /= total;
+            for (uint32_t k = lane; k < parts; k += lanes) { const float d = from[2u * k] - a; b += __builtin_fmaf(count(k) * d, d, from[2u * k + 1u]); }
+        }
+        b = add_lanes(b, lanes);
+        if (there && lane == 0u) use(g, a, b);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void apply_body(float* y, float* means, float* rstds, const float* partial, const float* x, const float* scale, const float* shift, const NormParams& P) {
+    const Chunk chunk(P);
+    const Span<VEC> span(P, chunk.number);
+    float* const mean_of = room, * const rstd_of = room + max(P.span / P.cg, 1u);
+    const float inverse = 1.f / ((float)P.S * (float)P.cg);
+    join_chunks<true>(P, span, chunk.n, partial, [&](uint32_t g, float mean, float square) {
+        const float rstd = 1.f / sqrtf(square * inverse + P.eps);
+        mean_of[g] = mean; rstd_of[g] = rstd;
+        if (chunk.chunk == 0u && (P.pieces == 1u || chunk.number % P.pieces == 0u)) {
+            const uint64_t at = (uint64_t)chunk.n * P.G + span.g0 + g;
+            if (means) means[at] = mean;
+            if (rstds) rstds[at] = rstd;
+        }
+    });
+    __syncthreads();
+    if (y == nullptr || !span.owns()) return;
+    float mean[VEC], factor[VEC], beta[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const uint32_t g = span.group_of(P, j);
+        mean[j] = mean_of[g]; factor[j] = rstd_of[g] * scale[span.c + j]; beta[j] = shift[span.c + j];
+    }
+    const bool stream = streams_result(P.first);
+    const uint64_t base = ((uint64_t)chunk.n * P.S + chunk.from) * P.C + span.c0;
+    const __amdgpu_buffer_rsrc_t y_rsrc = make_rsrc(y + base, ((chunk.count - 1u) * P.C + span.width) * 4u);
+    constexpr int U = 8;
+    walk<VEC, U>(P, span, chunk, x, [&](float (&v)[U][VEC], uint32_t here, uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[k][j] = act_value(__builtin_fmaf(v[k][j] - mean[j], factor[j], beta[j]), P.act);
+            store<VEC>(v[k], y_rsrc, (uint32_t)k < here ? ((span.p + (i + k) * P.P) * P.C + span.col * VEC) * 4u : NOWHERE, stream);
+        }
+    });
+}
+
+// hat and d of U positions of x and g: step(hat, d, how many, the first one's number)
+template <int VEC, int U, class Step>
+__device__ __forceinline__ void walk_gradient(const NormParams& P, const Span<VEC>& span, const Chunk& chunk, const float* gs, const float* x, const float* scale, const float* shift,
+                                              const float* means, const float* rstds, float (&rstd)[VEC], float (&gamma)[VEC], Step step) {
+    const bool owns = span.p < P.P && span.owns();
+    float mean[VEC], beta[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const uint64_t at = (uint64_t)chunk.n * P.G + span.g0 + span.group_of(P, j);
+        mean[j] = owns ? means[at] : 0.f; rstd[j] = owns ? rstds[at] : 0.f;
+        gamma[j] = owns ? scale[span.c + j] : 0.f; beta[j] = owns ? shift[span.c + j] : 0.f;
+    }
+    const uint32_t mine = owns ? share_of(chunk.count, span.p, P.P) : 0u;
+    const uint64_t base = ((uint64_t)chunk.n * P.S + chunk.from) * P.C + span.c0;
+    const uint32_t bytes = ((chunk.count - 1u) * P.C + span.width) * 4u;
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(x + base, bytes), g_rsrc = make_rsrc(gs + base, bytes);
+    for (uint32_t i = 0; i < mine; i += U) {
+        float v[U][VEC], d[U][VEC];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const uint32_t at = i + k < mine ? ((span.p + (i + k) * P.P) * P.C + span.col * VEC) * 4u : NOWHERE;
+            load<VEC>(v[k], x_rsrc, at); load<VEC>(d[k], g_rsrc, at);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[k][j] = (v[k][j] - mean[j]) * rstd[j];
+                d[k][j] = act_gradient(d[k][j], __builtin_fmaf(v[k][j], gamma[j], beta[j]), P.act);
+            }
+        step(v, d, min(mine - i, (uint32_t)U), i);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void grad_sums_body(float* partial, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
+                                               const float* means, const float* rstds, const NormParams& P) {
+    const Chunk chunk(P);
+    const Span<VEC> span(P, chunk.number);
+    constexpr int U = 4;
+    float rstd[VEC], gamma[VEC], A[VEC], B[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { A[j] = 0.f; B[j] = 0.f; }
+    walk_gradient<VEC, U>(P, span, chunk, gs, x, scale, shift, means, rstds, rstd, gamma, [&](const float (&hat)[U][VEC], const float (&d)[U][VEC], uint32_t here, uint32_t) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float a = 0.f, b = 0.f;
+#pragma unroll
+            for (int k = 0; k < U; ++k) { const float dk = (uint32_t)k < here ? d[k][j] : 0.f; a += dk; b = (uint32_t)k < here ? __builtin_fmaf(dk, hat[k][j], b) : b; }
+            A[j] += a; B[j] += b;
+        }
+    });
+    const uint32_t entries = P.P * P.span;
+    float* const firsts = room, * const seconds = room + entries;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        if (span.p < P.P && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = A[j]; seconds[span.p * P.span + span.col * VEC + j] = B[j]; }
+    __syncthreads();
+    const uint32_t piece = P.pieces == 1u ? 0u : chunk.number % P.pieces;
+    JoinSums join{firsts, seconds, scale + span.c0};
+    for_groups(P, span.groups, P.pieces == 1u ? P.cg : span.width, 1u, join, [&](uint32_t, uint32_t g, bool reports, const JoinSums& found) {
+        if (!reports) return;
+        float* const to = partial + 2u * ((((uint64_t)chunk.n * P.G + span.g0 + g) * P.pieces + piece) * P.chunks + chunk.chunk);
+        to[0] = found.a; to[1] = found.b;
+    });
+    const uint64_t row = (uint64_t)chunk.n * P.chunks + chunk.chunk;
+    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
+        float a = 0.f, b = 0.f;
+        for (uint32_t k = 0; k < P.P; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
+        dshift_rows[row * P.C + span.c0 + ch] = a;
+        dscale_rows[row * P.C + span.c0 + ch] = b;
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void grad_apply_body(float* dx, const float* partial, const float* gs, const float* x, const float* scale, const float* shift, const float* means,
+                                                const float* rstds, const NormParams& P) {
+    const Chunk chunk(P);
+    const Span<VEC> span(P, chunk.number);
+    float* const a_of = room, * const b_of = room + max(P.span / P.cg, 1u);
+    const float inverse = 1.f / ((float)P.S * (float)P.cg);
+    join_chunks<false>(P, span, chunk.n, partial, [&](uint32_t g, float a, float b) { a_of[g] = a * inverse; b_of[g] = b * inverse; });
+    __syncthreads();
+    if (!span.owns()) return;
+    float rstd[VEC], gamma[VEC], a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { const uint32_t g = span.group_of(P, j); a[j] = a_of[g]; b[j] = b_of[g]; }
+    const bool stream = streams_result(P.first);
+    const uint64_t base = ((uint64_t)chunk.n * P.S + chunk.from) * P.C + span.c0;
+    const __amdgpu_buffer_rsrc_t dx_rsrc = make_rsrc(dx + base, ((chunk.count - 1u) * P.C + span.width) * 4u);
+    constexpr int U = 4;
+    walk_gradient<VEC, U>(P, span, chunk, gs, x, scale, shift, means, rstds, rstd, gamma, [&](float (&hat)[U][VEC], const float (&d)[U][VEC], uint32_t here, uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) hat[k][j] = rstd[j] * (__builtin_fmaf(d[k][j], gamma[j], -a[j]) - hat[k][j] * b[j]);
+            store<VEC>(hat[k], dx_rsrc, (uint32_t)k < here ? ((span.p + (i + k) * P.P) * P.C + span.col * VEC) * 4u : NOWHERE, stream);
+        }
+    });
+}
+
+// ---------------------------------------------------------------------------------------------- kernels
+
+#define HELD(VEC, K, THREADS)                                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_held_v##VEC##_k##K##_t##THREADS(float* y, float* means, float* rstds, const float* x,          \
+                                                                                                     const float* scale, const float* shift, NormParams P) {        \
+        held_body<VEC, K>(y, means, rstds, x, scale, shift, P);                                                                                                     \
+    }
+#define HELD_GRAD(VEC, K, THREADS)                                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_held_grad_v##VEC##_k##K##_t##THREADS(float* dx, float* dscale_rows, float* dshift_rows,        \
+            const float* g, const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                         \
+        held_grad_body<VEC, K>(dx, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                  \
+    }
+#define CHUNKED(VEC)                                                                                                                                                \
+    extern "C" __global__ __launch_bounds__(256) void group_norm_stats_v##VEC(float* partial, const float* x, NormParams P) { stats_body<VEC>(partial, x, P); }     \
+    extern "C" __global__ __launch_bounds__(256) void group_norm_apply_v##VEC(float* y, float* means, float* rstds, const float* partial, const float* x,           \
+                                                                              const float* scale, const float* shift, NormParams P) {                               \
+        apply_body<VEC>(y, means, rstds, partial, x, scale, shift, P);                                                                                              \
+    }                                                                                                                                                               \
+    extern "C" __global__ __launch_bounds__(256) void group_norm_grad_sums_v##VEC(float* partial, float* dscale_rows, float* dshift_rows, const float* g,           \
+            const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                                         \
+        grad_sums_body<VEC>(partial, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                \
+    }                                                                                                                                                               \
+    extern "C" __global__ __launch_bounds__(256) void group_norm_grad_apply_v##VEC(float* dx, const float* partial, const float* g, const float* x,                 \
+            const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                                                         \
+        grad_apply_body<VEC>(dx, partial, g, x, scale, shift, means, rstds, P);                                                                                     \
+    }
+HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 25, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 64, 1024) HELD(4, 4, 1024) HELD(1, 8, 1024)
+HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 12, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 32, 1024) HELD_GRAD(4, 2, 1024) HELD_GRAD(1, 4, 1024)
+CHUNKED(4)
+CHUNKED(1)
+
+// Sums of the columns of two arrays [rows, C]: 64 columns to a block, 16 waves that take every 16th row each.
+extern "C" __global__ __launch_bounds__(1024) void group_norm_columns(float* first, float* second, const float* first_rows, const float* second_rows, uint32_t rows, uint32_t C) {
+    __shared__ float parts[16][64];
+    const uint32_t blocks = (C + 63u) / 64u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = blockIdx.x % blocks * 64u + lane;
+    const bool other = blockIdx.x >= blocks;
+    const float* const from = other ? second_rows : first_rows;
+    float* const to = other ? second : first;
+    if (to == nullptr) return;
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+        uint32_t r = wave;
+        for (; r + 48u < rows; r += 64u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sums[k] += from[(uint64_t)(r + 16u * k) * C + c];
+        for (; r < rows; r += 16u) sums[0] += from[(uint64_t)r * C + c];
+    }
+    parts[wave][lane] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    __syncthreads();
+    if (wave != 0u || c >= C) return;
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) total += parts[k][lane];
+    to[c] = total;
 }

@@ -2183,30 +2183,145 @@ def _f32_word(value: float) -> int:
     return int(np.asarray(value, np.float32).view(np.uint32))
 
 
-def _norm_shape(x: Buffer, groups: int):
+#(threads, positions per thread) of the kernels whose samples stay in registers, by channels per lane
+NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 25)), 1: ((256, 4), (256, 16), (1024, 8), (1024, 64))}
+NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 12)), 1: ((256, 4), (256, 16), (1024, 4), (1024, 32))}
+NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
+NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
+
+
+class NormPlan(tp.NamedTuple):
+    kind:    str                    #'held' or 'chunked'
+    vec:     int
+    threads: int
+    k:       int                    #positions per thread (held)
+    span:    int
+    spans:   int
+    pieces:  int
+    V:       int
+    P:       int
+    M:       int
+    chunks:  int
+    chunk:   int
+
+
+def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPlan]:
+    '''The plan that keeps samples in registers, or None where they do not fit (or a launch of it would leave most of the machine idle).'''
+    for vec in ((4, 1) if c % 4 == 0 else (1,)):
+        unit  = int(np.lcm(cg, vec))
+        lines = _cdiv(min(NORM_FULL_LINE, c), unit) * unit
+        for threads, k in variants[vec]:
+            #whole lines where they fit, less where they do not, and where whole lines would be few blocks
+            for span in dict.fromkeys((c if s == 1 else lines, lines, max(unit, lines // 2 // unit * unit), unit)):
+                V = span // vec
+                if V > threads or (span * 4 < 64 and span < c and n * _cdiv(c, span) > 64):
+                    continue
+                side = threads // V
+                P    = min(side, s)
+                M    = min(side // P, n) if s <= side else 1
+                if _cdiv(s, P) > k or M * s * c * 4 >= 2**31:
+                    continue
+                blocks = _cdiv(n, M) * _cdiv(c, span)
+                if blocks < 64 and span > unit:
+                    continue
+                if blocks < 64 and s * c > 1 << 16:
+                    return None
+                return NormPlan('held', vec, threads, k, span, _cdiv(c, span), 1, V, P, M, 1, s)
+    return None
+
+
+def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
+    vec = 4 if c % 4 == 0 and (c <= 1024 or np.lcm(cg, 4) <= 1024 or cg % 4 == 0) else 1
+    most, unit = BLOCK * vec, int(np.lcm(cg, vec))
+    if c <= most:
+        span, spans, pieces = c, 1, 1
+    elif unit <= most:
+        span = most // unit * unit
+        spans, pieces = _cdiv(c, span), 1
+    else:
+        pieces = _cdiv(cg, most)
+        span   = min(most, _cdiv(_cdiv(cg, pieces), vec) * vec)
+        pieces = _cdiv(cg, span)
+        spans  = c // cg * pieces
+    V = span // vec
+    P = min(BLOCK // V, s)
+    chunks = max(1, min(_cdiv(NORM_BLOCKS, n * spans), _cdiv(s, 4 * P)))
+    chunks = max(chunks, _cdiv(s * c * 4, 2**31 - 1))
+    chunk  = _cdiv(s, chunks)
+    return NormPlan('chunked', vec, BLOCK, 0, span, spans, pieces, V, P, 1, _cdiv(s, chunk), chunk)
+
+
+def norm_plan(n: int, s: int, c: int, groups: int, gradient: bool) -> NormPlan:
+    cg = c // groups
+    return _norm_held(n, s, c, cg, NORM_HELD_GRAD if gradient else NORM_HELD) or _norm_chunked(n, s, c, cg)
+
+
+def _norm_launch(kernel: str, blocks: int, plan: NormPlan, shape, groups: int, eps: float, activation, lds_words: int, buffers, moved: int, **kwargs) -> Launch:
+    n, s, c = shape
+    cg = c // groups
+    per_group = min(cg, plan.span)
+    sets  = max(plan.span // cg, 1) * plan.M
+    lanes = min(64, max(1, _pow2_at_least(plan.threads // sets + 1) // 2))
+    lc    = min(_pow2_at_least(per_group), lanes)
+    lq    = min(lanes // lc, _pow2_at_least(plan.P))
+    if blocks * plan.threads >= 2**32 or plan.chunk * c * 4 >= 2**31:
+        raise NotImplementedError(f'group norm of {n} x {s} x {c}')
+    params = _u32(0, n, s, c, groups, cg, NORM_ACTIVATIONS[activation], _f32_word(eps), plan.span, plan.spans, plan.pieces, plan.V, plan.P, plan.M,
+                  lc.bit_length() - 1, lq.bit_length() - 1, plan.chunks, plan.chunk)
+    return Launch(kernel, (blocks, 1, 1), (plan.threads, 1, 1), buffers, params, lds=4 * lds_words, bytes_moved=moved, **kwargs)
+
+
+def _norm_shape(x: Buffer):
     n, c = x.shape[0], x.shape[-1]
-    return n, x.size // (n * c), c, c // groups
+    return n, x.size // (n * c), c
 
 
 def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shift: Buffer, groups: int, eps: float, activation, scratch) -> tp.List[Launch]:
-    n, s, c, cg = _norm_shape(x, groups)
-    params = _u32(0, s, c, groups, cg, NORM_ACTIVATIONS[activation], _f32_word(eps))
-    return [Launch('group_norm', (n * groups, 1, 1), (BLOCK, 1, 1), [(y, 0), (mean, 0), (rstd, 0), (x, 0), (scale, 0), (shift, 0)], params,
-                   bytes_moved=4 * (2 * x.size + 2 * c + 2 * n * groups), written=(0, 1, 2))]
+    shape = n, s, c = _norm_shape(x)
+    plan  = norm_plan(n, s, c, groups, False)
+    cg    = c // groups
+    args  = (plan, shape, groups, eps, activation)
+    of_groups = max(plan.span // cg, 1)
+    if plan.kind == 'held':
+        return [_norm_launch(f'group_norm_held_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
+                             2 * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
+                             4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
+    partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
+    blocks  = n * plan.chunks * plan.spans
+    return [_norm_launch(f'group_norm_stats_v{plan.vec}', blocks, *args, 2 * plan.P * plan.span, [(partial, 0), (x, 0)], 4 * x.size),
+            _norm_launch(f'group_norm_apply_v{plan.vec}', blocks, *args, 2 * of_groups, [(b, 0) for b in (y, mean, rstd, partial, x, scale, shift)],
+                         4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
+
+
+NORM_GRAD_ROWS = 512                #blocks that the samples held in registers are shared out to, by the sums that each leaves
 
 
 def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shift: Buffer, mean: Buffer, rstd: Buffer, groups: int, eps: float,
                     activation, scratch) -> tp.List[Launch]:
-    n, s, c, cg = _norm_shape(x, groups)
-    shares = scratch((2, n, c))
-    params = _u32(0, s, c, groups, cg, NORM_ACTIVATIONS[activation], _f32_word(eps), n)
-    launches = [Launch('group_norm_grad', (n * groups, 1, 1), (BLOCK, 1, 1),
-                       [(dx, 0), (shares, 0), (g, 0), (x, 0), (scale, 0), (shift, 0), (mean, 0), (rstd, 0)], params,
-                       bytes_moved=4 * (3 * x.size + 2 * n * c), written=(0, 1))]
-    for k, out in enumerate((dscale, dshift)):
-        if out is not None:
-            total = _reduce_launch(out, shares, 1, n, c, 'reduce_sum', 1)[0]
-            launches.append(total._replace(buffers=[total.buffers[0], (shares, 4 * k * n * c)] + total.buffers[2:]))
+    shape = n, s, c = _norm_shape(x)
+    plan  = norm_plan(n, s, c, groups, True)
+    cg    = c // groups
+    args  = (plan, shape, groups, eps, activation)
+    of_groups = max(plan.span // cg, 1)
+    rest  = [(b, 0) for b in (g, x, scale, shift, mean, rstd)]
+    rows  = min(_cdiv(n, plan.M), max(1, NORM_GRAD_ROWS // plan.spans)) if plan.kind == 'held' else n * plan.chunks
+    #a single row of sums is what they add up to
+    dscale_rows, dshift_rows = (dscale or scratch((c,)), dshift or scratch((c,))) if rows == 1 else (scratch((rows, c)), scratch((rows, c)))
+    if plan.kind == 'held':
+        launches = [_norm_launch(f'group_norm_held_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
+                                 2 * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
+                                 4 * (3 * x.size + 2 * rows * c), streamable=True, written=(0, 1, 2))]
+    else:
+        partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
+        blocks  = n * plan.chunks * plan.spans
+        launches = [_norm_launch(f'group_norm_grad_sums_v{plan.vec}', blocks, *args, 2 * plan.P * plan.span,
+                                 [(partial, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest, 4 * (2 * x.size + 2 * rows * c), written=(0, 1, 2))]
+        if dx is not None:
+            launches.append(_norm_launch(f'group_norm_grad_apply_v{plan.vec}', blocks, *args, 2 * of_groups, [(dx, 0), (partial, 0)] + rest,
+                                         4 * 3 * x.size, streamable=True))
+    if rows > 1 and (dscale is not None or dshift is not None):
+        launches.append(Launch('group_norm_columns', (2 * _cdiv(c, 64), 1, 1), (1024, 1, 1), [(b, 0) for b in (dscale, dshift, dscale_rows, dshift_rows)],
+                               _u32(rows, c), bytes_moved=4 * 2 * (rows + 1) * c, written=(0, 1)))
     return launches
 
 
