@@ -128,7 +128,7 @@ struct JoinStats {
     __device__ void join(uint32_t lanes) { sum = add_lanes(sum, lanes); total = add_lanes(total, lanes); mean = sum / total; }
     __device__ bool again() const { return true; }
     __device__ void add_again(uint32_t at, uint32_t q) {
-        const float n = count(q), d = n > 0.f ? sums[at] / n - mean : 0.f;
+        const float n = count(q), d = n > 0.f ? __builtin_fmaf(sums[at], reciprocal(n), -mean) : 0.f;
         square += __builtin_fmaf(n * d, d, squares[at]);
     }
     __device__ void join_again(uint32_t lanes) { square = add_lanes(square, lanes); }
@@ -152,8 +152,9 @@ __device__ __forceinline__ uint32_t share_of(uint32_t count, uint32_t q, uint32_
 
 template <int VEC, int K>
 __device__ __forceinline__ void held_body(float* y, float* means, float* rstds, const float* x, const float* scale, const float* shift, const NormParams& P) {
-    const Span<VEC> span(P, blockIdx.x % P.spans);
-    const uint32_t n0 = blockIdx.x / P.spans * P.M, m = span.p / P.P, q = span.p - m * P.P;
+    const uint32_t block = xcd_contiguous_block();                       // neighbouring spans share lines: on one XCD, one fetch
+    const Span<VEC> span(P, block % P.spans);
+    const uint32_t n0 = block / P.spans * P.M, m = span.p / P.P, q = span.p - m * P.P;
     const bool use = m < P.M && n0 + m < P.N && span.owns();
     const uint64_t base = (uint64_t)n0 * P.S * P.C + span.c0;
     const uint32_t bytes = ((min(P.M, P.N - n0) * P.S - 1u) * P.C + span.width) * 4u;
@@ -182,7 +183,8 @@ __device__ __forceinline__ void held_body(float* y, float* means, float* rstds, 
         if (m < P.M && span.col * VEC + j < P.span) { sums[span.p * P.span + span.col * VEC + j] = sum; squares[span.p * P.span + span.col * VEC + j] = square; }
     }
     __syncthreads();
-    auto count = [&](uint32_t lane_q) { return (float)share_of(P.S, lane_q, P.P); };
+    const uint32_t each = P.S / P.P, more = P.S % P.P;
+    auto count = [&](uint32_t lane_q) { return (float)(each + (lane_q < more ? 1u : 0u)); };
     JoinStats<decltype(count)> join{sums, squares, count};
     for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t sample, uint32_t g, bool reports, const JoinStats<decltype(count)>& found) {
         if (!reports) return;
@@ -217,8 +219,9 @@ __device__ __forceinline__ void held_body(float* y, float* means, float* rstds, 
 template <int VEC, int K>
 __device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
                                                const float* means, const float* rstds, const NormParams& P) {
-    const Span<VEC> span(P, blockIdx.x % P.spans);
-    const uint32_t m = span.p / P.P, q = span.p - m * P.P, entries = P.M * P.P * P.span, sets = (P.N - 1u) / P.M + 1u, row = blockIdx.x / P.spans, rows = gridDim.x / P.spans;
+    const uint32_t block = xcd_contiguous_block();
+    const Span<VEC> span(P, block % P.spans);
+    const uint32_t m = span.p / P.P, q = span.p - m * P.P, entries = P.M * P.P * P.span, sets = (P.N - 1u) / P.M + 1u, row = block / P.spans, rows = gridDim.x / P.spans;
     float* const firsts = room, * const seconds = room + entries, * const a_of = room + 2u * entries, * const b_of = a_of + P.span / P.cg * P.M;
     float gamma[VEC], beta[VEC], d_total[VEC], dh_total[VEC];
     {
@@ -301,14 +304,168 @@ __device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, fl
     }
 }
 
+// ---------------------------------------------------------------------------------------------- single positions
+
+// Samples of one position: rows of C values. A thread has the same channels of K rows, P rows apart; all of a block's rows and groups are joined
+// together. entry(row, channel) of the joining step are the values themselves.
+struct JoinRow {
+    const float* values;
+    float inverse, sum, mean, square;
+    __device__ void start() { sum = square = 0.f; mean = 0.f; }
+    __device__ void add(uint32_t at, uint32_t, uint32_t) { sum += values[at]; }
+    __device__ void join(uint32_t lanes) { mean = add_lanes(sum, lanes) * inverse; }
+    __device__ bool again() const { return true; }
+    __device__ void add_again(uint32_t at, uint32_t) { const float d = values[at] - mean; square = __builtin_fmaf(d, d, square); }
+    __device__ void join_again(uint32_t lanes) { square = add_lanes(square, lanes); }
+};
+
+template <int VEC, int K>
+__device__ __forceinline__ void rows_body(float* y, float* means, float* rstds, const float* x, const float* scale, const float* shift, const NormParams& P) {
+    const uint32_t block = xcd_contiguous_block();
+    const Span<VEC> span(P, block % P.spans);
+    const uint32_t n0 = block / P.spans * P.M, here = min(P.M, P.N - n0), side = P.M / K;
+    const bool use = span.p < side && span.owns();
+    const uint64_t base = (uint64_t)n0 * P.C + span.c0;
+    const uint32_t bytes = ((here - 1u) * P.C + span.width) * 4u;
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(x + base, bytes);
+    float v[K][VEC], gamma[VEC], beta[VEC];
+    auto at = [&](int i) { const uint32_t m = span.p + i * side; return use && m < here ? (m * P.C + span.col * VEC) * 4u : NOWHERE; };
+#pragma unroll
+    for (int i = 0; i < K; ++i) load<VEC>(v[i], x_rsrc, at(i));
+    {
+        const __amdgpu_buffer_rsrc_t a = make_rsrc(scale + span.c0, span.width * 4u), b = make_rsrc(shift + span.c0, span.width * 4u);
+        load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
+        load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
+    }
+    float* const values = room, * const mean_of = room + P.M * P.span, * const rstd_of = mean_of + P.span / P.cg * P.M;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) if (use) values[(span.p + i * side) * P.span + span.col * VEC + j] = v[i][j];
+    __syncthreads();
+    JoinRow join{values, 1.f / (float)P.cg};
+    for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t m, uint32_t g, bool reports, const JoinRow& found) {
+        if (!reports) return;
+        const float rstd = 1.f / sqrtf(found.square * join.inverse + P.eps);
+        mean_of[m * span.groups + g] = found.mean; rstd_of[m * span.groups + g] = rstd;
+        if (m < here) {
+            const uint64_t to = (uint64_t)(n0 + m) * P.G + span.g0 + g;
+            if (means) means[to] = found.mean;
+            if (rstds) rstds[to] = rstd;
+        }
+    });
+    __syncthreads();
+    if (!use || y == nullptr) return;
+    const bool stream = streams_result(P.first);
+    const __amdgpu_buffer_rsrc_t y_rsrc = make_rsrc(y + base, bytes);
+    uint32_t group[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) group[j] = span.group_of(P, j);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const uint32_t m = span.p + i * side;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const uint32_t g = m * span.groups + group[j];
+            v[i][j] = act_value(__builtin_fmaf((v[i][j] - mean_of[g]) * rstd_of[g], gamma[j], beta[j]), P.act);
+        }
+        store<VEC>(v[i], y_rsrc, at(i), stream);
+    }
+}
+
+template <int VEC, int K>
+__device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
+                                               const float* means, const float* rstds, const NormParams& P) {
+    const uint32_t block = xcd_contiguous_block();
+    const Span<VEC> span(P, block % P.spans);
+    const uint32_t side = P.M / K, sets = (P.N - 1u) / P.M + 1u, row = block / P.spans, rows = gridDim.x / P.spans;
+    const bool use = span.p < side && span.owns();
+    float* const firsts = room, * const seconds = room + P.M * P.span, * const a_of = seconds + P.M * P.span, * const b_of = a_of + P.span / P.cg * P.M;
+    float gamma[VEC], beta[VEC], d_total[VEC], dh_total[VEC];
+    uint32_t group[VEC];
+    {
+        const __amdgpu_buffer_rsrc_t a = make_rsrc(scale + span.c0, span.width * 4u), b = make_rsrc(shift + span.c0, span.width * 4u);
+        load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
+        load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { d_total[j] = 0.f; dh_total[j] = 0.f; group[j] = use ? span.group_of(P, j) : 0u; }
+    const float inverse = 1.f / (float)P.cg;
+    const bool stream = streams_result(P.first);
+    for (uint32_t set = row; set < sets; set += rows) {
+        const uint32_t n0 = set * P.M, here = min(P.M, P.N - n0);
+        const uint64_t base = (uint64_t)n0 * P.C + span.c0;
+        const uint32_t bytes = ((here - 1u) * P.C + span.width) * 4u;
+        const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(x + base, bytes), g_rsrc = make_rsrc(gs + base, bytes);
+        float v[K][VEC], d[K][VEC];
+        auto there = [&](int i) { return use && span.p + i * side < here; };
+        auto at = [&](int i) { return there(i) ? ((span.p + i * side) * P.C + span.col * VEC) * 4u : NOWHERE; };
+#pragma unroll
+        for (int i = 0; i < K; ++i) { load<VEC>(v[i], x_rsrc, at(i)); load<VEC>(d[i], g_rsrc, at(i)); }
+        // the statistics of these rows, by way of shared memory
+        __syncthreads();                                                 // (what the set before has left has been read)
+        for (uint32_t e = threadIdx.x; e < P.M * span.groups; e += blockDim.x) {
+            const uint32_t m = e / span.groups, g = e - m * span.groups;
+            const uint64_t from = (uint64_t)(n0 + m) * P.G + span.g0 + g;
+            a_of[e] = m < here ? means[from] : 0.f; b_of[e] = m < here ? rstds[from] : 0.f;
+        }
+        __syncthreads();
+        float rstd[K][VEC];
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const uint32_t e = use ? (span.p + i * side) * span.groups + group[j] : 0u;
+                rstd[i][j] = b_of[e];
+                v[i][j] = there(i) ? (v[i][j] - a_of[e]) * rstd[i][j] : 0.f;
+                d[i][j] = there(i) ? act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
+                d_total[j] += d[i][j]; dh_total[j] = __builtin_fmaf(d[i][j], v[i][j], dh_total[j]);
+                if (use) {
+                    firsts[(span.p + i * side) * P.span + span.col * VEC + j] = d[i][j];
+                    seconds[(span.p + i * side) * P.span + span.col * VEC + j] = d[i][j] * v[i][j];
+                }
+            }
+        if (dx == nullptr) continue;
+        __syncthreads();
+        JoinSums join{firsts, seconds, scale + span.c0};
+        for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t m, uint32_t g, bool reports, const JoinSums& found) {
+            if (reports) { a_of[m * span.groups + g] = found.a * inverse; b_of[m * span.groups + g] = found.b * inverse; }
+        });
+        __syncthreads();
+        const __amdgpu_buffer_rsrc_t dx_rsrc = make_rsrc(dx + base, bytes);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const uint32_t e = use ? (span.p + i * side) * span.groups + group[j] : 0u;
+                v[i][j] = rstd[i][j] * (__builtin_fmaf(d[i][j], gamma[j], -a_of[e]) - v[i][j] * b_of[e]);
+            }
+            store<VEC>(v[i], dx_rsrc, at(i), stream);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) if (use) { firsts[span.p * P.span + span.col * VEC + j] = d_total[j]; seconds[span.p * P.span + span.col * VEC + j] = dh_total[j]; }
+    __syncthreads();
+    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
+        float a = 0.f, b = 0.f;
+        for (uint32_t k = 0; k < side; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
+        dshift_rows[(uint64_t)row * P.C + span.c0 + ch] = a;
+        dscale_rows[(uint64_t)row * P.C + span.c0 + ch] = b;
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- samples in chunks
 
 // Which chunk of which sample and span a block has.
 struct Chunk {
     uint32_t number, n, from, count, chunk;
-    __device__ Chunk(const NormParams& P) {
-        number = blockIdx.x % P.spans;
-        const uint32_t rest = blockIdx.x / P.spans;
+    // `last_first`: in the opposite order. What a launch reads that another one has read just before is taken from its end: that is what the 256 MB
+    // behind the L2s still hold.
+    __device__ Chunk(const NormParams& P, bool last_first) {
+        const uint32_t block = last_first ? gridDim.x - 1u - blockIdx.x : blockIdx.x;
+        number = block % P.spans;
+        const uint32_t rest = block / P.spans;
         chunk = rest % P.chunks; n = rest / P.chunks;
         from = chunk * P.chunk; count = min(P.chunk, P.S - from);
     }
@@ -330,7 +487,7 @@ __device__ __forceinline__ void walk(const NormParams& P, const Span<VEC>& span,
 
 template <int VEC>
 __device__ __forceinline__ void stats_body(float* partial, const float* x, const NormParams& P) {
-    const Chunk chunk(P);
+    const Chunk chunk(P, false);
     const Span<VEC> span(P, chunk.number);
     constexpr int U = 8;
     float mean[VEC], square[VEC], n = 0.f;
@@ -359,7 +516,8 @@ __device__ __forceinline__ void stats_body(float* partial, const float* x, const
     for (int j = 0; j < VEC; ++j)
         if (span.p < P.P && span.col * VEC + j < P.span) { sums[span.p * P.span + span.col * VEC + j] = mean[j] * n; squares[span.p * P.span + span.col * VEC + j] = square[j]; }
     __syncthreads();
-    auto count = [&](uint32_t q) { return (float)share_of(chunk.count, q, P.P); };
+    const uint32_t each = chunk.count / P.P, more = chunk.count % P.P;
+    auto count = [&](uint32_t q) { return (float)(each + (q < more ? 1u : 0u)); };
     JoinStats<decltype(count)> join{sums, squares, count};
     const uint32_t piece = P.pieces == 1u ? 0u : chunk.number % P.pieces;
     for_groups(P, span.groups, P.pieces == 1u ? P.cg : span.width, 1u, join, [&](uint32_t, uint32_t g, bool reports, const JoinStats<decltype(count)>& found) {
@@ -402,7 +560,7 @@ __device__ __forceinline__ void join_chunks(const NormParams& P, const Span<VEC>
 
 template <int VEC>
 __device__ __forceinline__ void apply_body(float* y, float* means, float* rstds, const float* partial, const float* x, const float* scale, const float* shift, const NormParams& P) {
-    const Chunk chunk(P);
+    const Chunk chunk(P, true);
     const Span<VEC> span(P, chunk.number);
     float* const mean_of = room, * const rstd_of = room + max(P.span / P.cg, 1u);
     const float inverse = 1.f / ((float)P.S * (float)P.cg);
@@ -474,7 +632,7 @@ __device__ __forceinline__ void walk_gradient(const NormParams& P, const Span<VE
 template <int VEC>
 __device__ __forceinline__ void grad_sums_body(float* partial, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
                                                const float* means, const float* rstds, const NormParams& P) {
-    const Chunk chunk(P);
+    const Chunk chunk(P, false);
     const Span<VEC> span(P, chunk.number);
     constexpr int U = 4;
     float rstd[VEC], gamma[VEC], A[VEC], B[VEC];
@@ -514,7 +672,7 @@ __device__ __forceinline__ void grad_sums_body(float* partial, float* dscale_row
 template <int VEC>
 __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial, const float* gs, const float* x, const float* scale, const float* shift, const float* means,
                                                 const float* rstds, const NormParams& P) {
-    const Chunk chunk(P);
+    const Chunk chunk(P, true);
     const Span<VEC> span(P, chunk.number);
     float* const a_of = room, * const b_of = room + max(P.span / P.cg, 1u);
     const float inverse = 1.f / ((float)P.S * (float)P.cg);
@@ -550,6 +708,15 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
             const float* g, const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                         \
         held_grad_body<VEC, K>(dx, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                  \
     }
+#define ROWS(VEC, K, THREADS)                                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_rows_v##VEC##_k##K##_t##THREADS(float* y, float* means, float* rstds, const float* x,          \
+                                                                                                     const float* scale, const float* shift, NormParams P) {        \
+        rows_body<VEC, K>(y, means, rstds, x, scale, shift, P);                                                                                                     \
+    }                                                                                                                                                               \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_rows_grad_v##VEC##_k##K##_t##THREADS(float* dx, float* dscale_rows, float* dshift_rows,        \
+            const float* g, const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                         \
+        rows_grad_body<VEC, K>(dx, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                  \
+    }
 #define CHUNKED(VEC)                                                                                                                                                \
     extern "C" __global__ __launch_bounds__(256) void group_norm_stats_v##VEC(float* partial, const float* x, NormParams P) { stats_body<VEC>(partial, x, P); }     \
     extern "C" __global__ __launch_bounds__(256) void group_norm_apply_v##VEC(float* y, float* means, float* rstds, const float* partial, const float* x,           \
@@ -564,8 +731,9 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
             const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                                                         \
         grad_apply_body<VEC>(dx, partial, g, x, scale, shift, means, rstds, P);                                                                                     \
     }
-HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 25, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 64, 1024) HELD(4, 4, 1024) HELD(1, 8, 1024)
-HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 12, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 32, 1024) HELD_GRAD(4, 2, 1024) HELD_GRAD(1, 4, 1024)
+HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 4, 1024)  HELD(4, 13, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 8, 1024)
+HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 2, 1024)  HELD_GRAD(4, 4, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 4, 1024)
+ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)  ROWS(4, 8, 256)  ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)  ROWS(4, 1, 1024)  ROWS(1, 4, 1024) ROWS(4, 2, 1024) ROWS(1, 1, 1024)
 CHUNKED(4)
 CHUNKED(1)
 

@@ -2184,17 +2184,20 @@ def _f32_word(value: float) -> int:
 
 
 #(threads, positions per thread) of the kernels whose samples stay in registers, by channels per lane
-NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 25)), 1: ((256, 4), (256, 16), (1024, 8), (1024, 64))}
-NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 12)), 1: ((256, 4), (256, 16), (1024, 4), (1024, 32))}
+NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 13)), 1: ((256, 4), (256, 16), (1024, 8))}
+NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 4)), 1: ((256, 4), (256, 16), (1024, 4))}
+#(threads, rows per thread) of the kernels for samples of one position
+NORM_ROWS      = {4: ((256, 8), (256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
+NORM_ROWS_GRAD = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
 
 class NormPlan(tp.NamedTuple):
-    kind:    str                    #'held' or 'chunked'
+    kind:    str                    #'rows', 'held' or 'chunked'
     vec:     int
     threads: int
-    k:       int                    #positions per thread (held)
+    k:       int                    #positions (held) or rows per thread
     span:    int
     spans:   int
     pieces:  int
@@ -2212,13 +2215,13 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
         lines = _cdiv(min(NORM_FULL_LINE, c), unit) * unit
         for threads, k in variants[vec]:
             #whole lines where they fit, less where they do not, and where whole lines would be few blocks
-            for span in dict.fromkeys((c if s == 1 else lines, lines, max(unit, lines // 2 // unit * unit), unit)):
+            for span in dict.fromkeys((lines, max(unit, lines // 2 // unit * unit), unit)):
                 V = span // vec
                 if V > threads or (span * 4 < 64 and span < c and n * _cdiv(c, span) > 64):
                     continue
                 side = threads // V
-                P    = min(side, s)
-                M    = min(side // P, n) if s <= side else 1
+                P    = min(side, _cdiv(s, k))
+                M    = min(side // P, n)
                 if _cdiv(s, P) > k or M * s * c * 4 >= 2**31:
                     continue
                 blocks = _cdiv(n, M) * _cdiv(c, span)
@@ -2227,6 +2230,24 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
                 if blocks < 64 and s * c > 1 << 16:
                     return None
                 return NormPlan('held', vec, threads, k, span, _cdiv(c, span), 1, V, P, M, 1, s)
+    return None
+
+
+def _norm_rows(n: int, c: int, cg: int, variants, blocks_wanted: int) -> tp.Optional[NormPlan]:
+    '''Samples of one position: a span that fills a block's lanes best, as many rows per thread as leave blocks_wanted blocks.'''
+    for threads in (BLOCK, 4 * BLOCK):
+        spans = []
+        for vec in ((4, 1) if c % 4 == 0 else (1,)):
+            unit = int(np.lcm(cg, vec))
+            for many in range(1, min(c, threads * vec) // unit + 1):
+                V = many * unit // vec
+                spans.append((round(threads // V * V / threads, 2) * (1.0 if vec == 4 else 0.5), many * unit, vec, V))
+        if spans:
+            _, span, vec, V = max(spans)
+            side = threads // V
+            ks   = [k for t, k in variants[vec] if t == threads]
+            k    = next((k for k in ks if _cdiv(n, side * k) * _cdiv(c, span) >= blocks_wanted), ks[-1])
+            return NormPlan('rows', vec, threads, k, span, _cdiv(c, span), 1, V, 1, side * k, 1, 1) if side * k * c * 4 < 2**31 else None
     return None
 
 
@@ -2253,6 +2274,8 @@ def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
 
 def norm_plan(n: int, s: int, c: int, groups: int, gradient: bool) -> NormPlan:
     cg = c // groups
+    if s == 1:
+        return _norm_rows(n, c, cg, NORM_ROWS_GRAD if gradient else NORM_ROWS, NORM_BLOCKS) or _norm_chunked(n, s, c, cg)
     return _norm_held(n, s, c, cg, NORM_HELD_GRAD if gradient else NORM_HELD) or _norm_chunked(n, s, c, cg)
 
 
@@ -2282,9 +2305,9 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
     cg    = c // groups
     args  = (plan, shape, groups, eps, activation)
     of_groups = max(plan.span // cg, 1)
-    if plan.kind == 'held':
-        return [_norm_launch(f'group_norm_held_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
-                             2 * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
+    if plan.kind != 'chunked':
+        return [_norm_launch(f'group_norm_{plan.kind}_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
+                             (2 if plan.kind == 'held' else 1) * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
                              4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
     partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
     blocks  = n * plan.chunks * plan.spans
@@ -2293,7 +2316,7 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
                          4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
 
 
-NORM_GRAD_ROWS = 512                #blocks that the samples held in registers are shared out to, by the sums that each leaves
+NORM_GRAD_ROWS = 1024               #blocks that the samples held in registers are shared out to, by the sums that each leaves
 
 
 def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shift: Buffer, mean: Buffer, rstd: Buffer, groups: int, eps: float,
@@ -2304,11 +2327,11 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     args  = (plan, shape, groups, eps, activation)
     of_groups = max(plan.span // cg, 1)
     rest  = [(b, 0) for b in (g, x, scale, shift, mean, rstd)]
-    rows  = min(_cdiv(n, plan.M), max(1, NORM_GRAD_ROWS // plan.spans)) if plan.kind == 'held' else n * plan.chunks
+    rows  = min(_cdiv(n, plan.M), max(1, NORM_GRAD_ROWS // plan.spans)) if plan.kind != 'chunked' else n * plan.chunks
     #a single row of sums is what they add up to
     dscale_rows, dshift_rows = (dscale or scratch((c,)), dshift or scratch((c,))) if rows == 1 else (scratch((rows, c)), scratch((rows, c)))
-    if plan.kind == 'held':
-        launches = [_norm_launch(f'group_norm_held_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
+    if plan.kind != 'chunked':
+        launches = [_norm_launch(f'group_norm_{plan.kind}_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
                                  2 * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
                                  4 * (3 * x.size + 2 * rows * c), streamable=True, written=(0, 1, 2))]
     else:
