@@ -20,6 +20,8 @@
 // (group_norm_columns) in a fixed order: no atomics.
 #include "common.h"
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 enum Activation : uint32_t { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2 };
 
 struct NormParams {
@@ -37,11 +39,10 @@ __device__ __forceinline__ float reciprocal(float d) {
     const float r = __builtin_amdgcn_rcpf(d);
     return __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);             // a Newton step
 }
-// 1 / (1 + exp(-z)); exp(-z) beyond fp32 is infinite and its reciprocal 0, where the Newton step would make a NaN of infinity times 0
-__device__ __forceinline__ float sigmoid(float z) {
-    const float e = expf(-z);
-    return e > 1e38f ? 0.f : reciprocal(1.f + e);
-}
+// 1 / (1 + exp(-z)) in five instructions: the exponential in base 2, whose exponent z log2(e) is rounded twice, so that it is off by some 2 |z| 2^-24 of itself,
+// and the reciprocal to one unit of the last place. That is where this operator's launches have their instructions: 25 a value with the library's exponential and
+// a division bounded them. (exp(-z) beyond fp32 is infinite, and its reciprocal 0.)
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
     if (act == ACT_RELU) return (z > 0.f || z != z) ? z : 0.f;
     if (act == ACT_SILU) return z * sigmoid(z);
@@ -69,7 +70,14 @@ template <int VEC> __device__ __forceinline__ void store(const float (&v)[VEC], 
     }
 }
 
-extern __shared__ float room[];
+extern __shared__ __attribute__((aligned(16))) float room[];
+
+// to[0 .. VEC) = v in shared memory; whole vectors lie at multiples of 16 bytes
+template <int VEC> __device__ __forceinline__ void put(float* to, const float (&v)[VEC]) {
+    if constexpr (VEC == 4) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+    else to[0] = v[0];
+}
+
 
 // A span of channels and this thread's part of it.
 template <int VEC>
@@ -307,17 +315,64 @@ __device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, fl
 // ---------------------------------------------------------------------------------------------- single positions
 
 // Samples of one position: rows of C values. A thread has the same channels of K rows, P rows apart; all of a block's rows and groups are joined
-// together. entry(row, channel) of the joining step are the values themselves.
-struct JoinRow {
-    const float* values;
-    float inverse, sum, mean, square;
-    __device__ void start() { sum = square = 0.f; mean = 0.f; }
-    __device__ void add(uint32_t at, uint32_t, uint32_t) { sum += values[at]; }
-    __device__ void join(uint32_t lanes) { mean = add_lanes(sum, lanes) * inverse; }
-    __device__ bool again() const { return true; }
-    __device__ void add_again(uint32_t at, uint32_t) { const float d = values[at] - mean; square = __builtin_fmaf(d, d, square); }
-    __device__ void join_again(uint32_t lanes) { square = add_lanes(square, lanes); }
+// together from shared memory, where channels of a group need not be those of whole vectors (65 channels to a group: 4 to a lane).
+
+// done(row, group, lane 0 of the group's, first of its values in shared memory, how many lanes): lanes of one group go through its channels.
+template <class Done>
+__device__ __forceinline__ void for_row_groups(const NormParams& P, uint32_t groups, uint32_t rows, Done done) {
+    const uint32_t lanes = 1u << P.log2_lc, lane = threadIdx.x & (lanes - 1u), sets = blockDim.x >> P.log2_lc, all = groups * rows, start = threadIdx.x >> P.log2_lc;
+    for (uint32_t at = start; at - start < all; at += sets) {             // (every lane goes round as often: lanes meet in `done`)
+        const bool use = at < all;
+        const uint32_t m = use ? at / groups : 0u, g = use ? at - m * groups : 0u;
+        done(m, g, use && lane == 0u, m * P.span + g * P.cg, lane, lanes);
+    }
+}
+
+// The groups of a vector's channels: two at most, since groups of one channel have the kernels with one channel per lane.
+template <int VEC>
+struct TwoGroups {
+    uint32_t first, last, from;                  // channels from `from` on belong to `last`
+    __device__ TwoGroups(const NormParams& P, const Span<VEC>& span) {
+        first = span.owns() ? span.group_of(P, 0) : 0u; last = span.owns() ? span.group_of(P, VEC - 1) : 0u;
+        from = last * P.cg - span.col * VEC;
+    }
+    __device__ float pick(int j, float a, float b) const { return VEC > 1 && first != last && (uint32_t)j >= from ? b : a; }
 };
+
+// Mean and squared deviations of values[lane], values[lane + lanes] .. (`count` in all), by the lanes together. A lane goes through its values once: with
+// s = sum (x - k), q = sum (x - k)^2 of its n values, k the first of them, their squared deviations are q - s^2 / n. k being one of them, q is at most n times
+// that difference, whose error is then at most n u of itself: with at most some 64 values a lane that is a sum's own error. Lanes are joined by their means.
+__device__ __forceinline__ void row_stats(const float* values, uint32_t count, uint32_t lane, uint32_t lanes, float inverse, float& mean, float& square) {
+    const float k = lane < count ? values[lane] : 0.f;
+    float s = 0.f, q = 0.f;
+    uint32_t i = lane + lanes;
+    for (; i + 3u * lanes < count; i += 4u * lanes) {
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = values[i + e * lanes] - k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { s += d[e]; q = __builtin_fmaf(d[e], d[e], q); }
+    }
+    for (; i < count; i += lanes) { const float d = values[i] - k; s += d; q = __builtin_fmaf(d, d, q); }
+    const float n = lane < count ? (float)((count - lane - 1u) / lanes + 1u) : 0.f, own = n > 0.f ? __builtin_fmaf(s, reciprocal(n), k) : 0.f;
+    mean = add_lanes(own * n, lanes) * inverse;
+    const float d = own - mean;
+    square = n > 0.f ? fmaxf(__builtin_fmaf(-s * reciprocal(n), s, q), 0.f) : 0.f;
+    square = s != s ? s : square;                                         // (a maximum would lose a NaN)
+    square = add_lanes(__builtin_fmaf(n * d, d, square), lanes);
+}
+__device__ __forceinline__ float row_sum(const float* values, uint32_t count, uint32_t lane, uint32_t lanes) {
+    float s[2] = {0.f, 0.f};
+    uint32_t i = lane;
+    for (; i + 3u * lanes < count; i += 4u * lanes) {
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = values[i + e * lanes];
+        s[0] += d[0] + d[1]; s[1] += d[2] + d[3];
+    }
+    for (; i < count; i += lanes) s[0] += values[i];
+    return add_lanes(s[0] + s[1], lanes);
+}
 
 template <int VEC, int K>
 __device__ __forceinline__ void rows_body(float* y, float* means, float* rstds, const float* x, const float* scale, const float* shift, const NormParams& P) {
@@ -337,38 +392,34 @@ __device__ __forceinline__ void rows_body(float* y, float* means, float* rstds, 
         load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
         load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
     }
-    float* const values = room, * const mean_of = room + P.M * P.span, * const rstd_of = mean_of + P.span / P.cg * P.M;
+    float* const values = room;
+    f32x2* const stats_of = reinterpret_cast<f32x2*>(room + P.M * P.span);
 #pragma unroll
-    for (int i = 0; i < K; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) if (use) values[(span.p + i * side) * P.span + span.col * VEC + j] = v[i][j];
+    for (int i = 0; i < K; ++i) if (use) put<VEC>(values + (span.p + i * side) * P.span + span.col * VEC, v[i]);
     __syncthreads();
-    JoinRow join{values, 1.f / (float)P.cg};
-    for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t m, uint32_t g, bool reports, const JoinRow& found) {
+    const float inverse = 1.f / (float)P.cg;
+    for_row_groups(P, span.groups, here, [&](uint32_t m, uint32_t g, bool reports, uint32_t first, uint32_t lane, uint32_t lanes) {
+        float mean, square;
+        row_stats(values + first, P.cg, lane, lanes, inverse, mean, square);
         if (!reports) return;
-        const float rstd = 1.f / sqrtf(found.square * join.inverse + P.eps);
-        mean_of[m * span.groups + g] = found.mean; rstd_of[m * span.groups + g] = rstd;
-        if (m < here) {
-            const uint64_t to = (uint64_t)(n0 + m) * P.G + span.g0 + g;
-            if (means) means[to] = found.mean;
-            if (rstds) rstds[to] = rstd;
-        }
+        const float rstd = 1.f / sqrtf(square * inverse + P.eps);
+        stats_of[m * span.groups + g] = f32x2{mean, rstd};
+        const uint64_t to = (uint64_t)(n0 + m) * P.G + span.g0 + g;
+        if (means) means[to] = mean;
+        if (rstds) rstds[to] = rstd;
     });
     __syncthreads();
     if (!use || y == nullptr) return;
     const bool stream = streams_result(P.first);
     const __amdgpu_buffer_rsrc_t y_rsrc = make_rsrc(y + base, bytes);
-    uint32_t group[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) group[j] = span.group_of(P, j);
+    const TwoGroups<VEC> two(P, span);
 #pragma unroll
     for (int i = 0; i < K; ++i) {
         const uint32_t m = span.p + i * side;
+        const f32x2* const from = stats_of + (m < here ? m * span.groups : 0u);
+        const f32x2 a = from[two.first], b = from[two.last];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const uint32_t g = m * span.groups + group[j];
-            v[i][j] = act_value(__builtin_fmaf((v[i][j] - mean_of[g]) * rstd_of[g], gamma[j], beta[j]), P.act);
-        }
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf((v[i][j] - two.pick(j, a.x, b.x)) * two.pick(j, a.y, b.y), gamma[j], beta[j]), P.act);
         store<VEC>(v[i], y_rsrc, at(i), stream);
     }
 }
@@ -380,16 +431,17 @@ __device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, fl
     const Span<VEC> span(P, block % P.spans);
     const uint32_t side = P.M / K, sets = (P.N - 1u) / P.M + 1u, row = block / P.spans, rows = gridDim.x / P.spans;
     const bool use = span.p < side && span.owns();
-    float* const firsts = room, * const seconds = room + P.M * P.span, * const a_of = seconds + P.M * P.span, * const b_of = a_of + P.span / P.cg * P.M;
+    float* const firsts = room, * const seconds = room + P.M * P.span;
+    f32x2* const stats_of = reinterpret_cast<f32x2*>(seconds + P.M * P.span), * const sums_of = stats_of + P.span / P.cg * P.M;
     float gamma[VEC], beta[VEC], d_total[VEC], dh_total[VEC];
-    uint32_t group[VEC];
+    const TwoGroups<VEC> two(P, span);
     {
         const __amdgpu_buffer_rsrc_t a = make_rsrc(scale + span.c0, span.width * 4u), b = make_rsrc(shift + span.c0, span.width * 4u);
         load<VEC>(gamma, a, span.owns() ? span.col * VEC * 4u : NOWHERE);
         load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
     }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) { d_total[j] = 0.f; dh_total[j] = 0.f; group[j] = use ? span.group_of(P, j) : 0u; }
+    for (int j = 0; j < VEC; ++j) { d_total[j] = 0.f; dh_total[j] = 0.f; }
     const float inverse = 1.f / (float)P.cg;
     const bool stream = streams_result(P.first);
     for (uint32_t set = row; set < sets; set += rows) {
@@ -407,39 +459,42 @@ __device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, fl
         for (uint32_t e = threadIdx.x; e < P.M * span.groups; e += blockDim.x) {
             const uint32_t m = e / span.groups, g = e - m * span.groups;
             const uint64_t from = (uint64_t)(n0 + m) * P.G + span.g0 + g;
-            a_of[e] = m < here ? means[from] : 0.f; b_of[e] = m < here ? rstds[from] : 0.f;
+            stats_of[e] = m < here ? f32x2{means[from], rstds[from]} : f32x2{0.f, 0.f};
         }
         __syncthreads();
-        float rstd[K][VEC];
 #pragma unroll
-        for (int i = 0; i < K; ++i)
+        for (int i = 0; i < K; ++i) {
+            const f32x2* const from = stats_of + (use ? (span.p + i * side) * span.groups : 0u);
+            const f32x2 a = from[two.first], b = from[two.last];
+            float product[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const uint32_t e = use ? (span.p + i * side) * span.groups + group[j] : 0u;
-                rstd[i][j] = b_of[e];
-                v[i][j] = there(i) ? (v[i][j] - a_of[e]) * rstd[i][j] : 0.f;
+                v[i][j] = there(i) ? (v[i][j] - two.pick(j, a.x, b.x)) * two.pick(j, a.y, b.y) : 0.f;
                 d[i][j] = there(i) ? act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
                 d_total[j] += d[i][j]; dh_total[j] = __builtin_fmaf(d[i][j], v[i][j], dh_total[j]);
-                if (use) {
-                    firsts[(span.p + i * side) * P.span + span.col * VEC + j] = d[i][j];
-                    seconds[(span.p + i * side) * P.span + span.col * VEC + j] = d[i][j] * v[i][j];
-                }
+                d[i][j] *= gamma[j];
+                product[j] = d[i][j] * v[i][j];
             }
+            if (use) {
+                put<VEC>(firsts + (span.p + i * side) * P.span + span.col * VEC, d[i]);
+                put<VEC>(seconds + (span.p + i * side) * P.span + span.col * VEC, product);
+            }
+        }
         if (dx == nullptr) continue;
         __syncthreads();
-        JoinSums join{firsts, seconds, scale + span.c0};
-        for_groups(P, span.groups, P.cg, P.M, join, [&](uint32_t m, uint32_t g, bool reports, const JoinSums& found) {
-            if (reports) { a_of[m * span.groups + g] = found.a * inverse; b_of[m * span.groups + g] = found.b * inverse; }
+        for_row_groups(P, span.groups, here, [&](uint32_t m, uint32_t g, bool reports, uint32_t first, uint32_t lane, uint32_t lanes) {
+            const float a = row_sum(firsts + first, P.cg, lane, lanes), b = row_sum(seconds + first, P.cg, lane, lanes);
+            if (reports) sums_of[m * span.groups + g] = f32x2{a * inverse, b * inverse};
         });
         __syncthreads();
         const __amdgpu_buffer_rsrc_t dx_rsrc = make_rsrc(dx + base, bytes);
 #pragma unroll
         for (int i = 0; i < K; ++i) {
+            const uint32_t row0 = use ? (span.p + i * side) * span.groups : 0u;
+            const f32x2 a = sums_of[row0 + two.first], b = sums_of[row0 + two.last];
+            const float ra = stats_of[row0 + two.first].y, rb = stats_of[row0 + two.last].y;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const uint32_t e = use ? (span.p + i * side) * span.groups + group[j] : 0u;
-                v[i][j] = rstd[i][j] * (__builtin_fmaf(d[i][j], gamma[j], -a_of[e]) - v[i][j] * b_of[e]);
-            }
+            for (int j = 0; j < VEC; ++j) v[i][j] = two.pick(j, ra, rb) * (d[i][j] - two.pick(j, a.x, b.x) - v[i][j] * two.pick(j, a.y, b.y));
             store<VEC>(v[i], dx_rsrc, at(i), stream);
         }
     }

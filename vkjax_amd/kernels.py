@@ -2187,8 +2187,8 @@ def _f32_word(value: float) -> int:
 NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 13)), 1: ((256, 4), (256, 16), (1024, 8))}
 NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 4)), 1: ((256, 4), (256, 16), (1024, 4))}
 #(threads, rows per thread) of the kernels for samples of one position
-NORM_ROWS      = {4: ((256, 8), (256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
-NORM_ROWS_GRAD = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
+NORM_ROWS      = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
+NORM_ROWS_GRAD = {4: ((256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
@@ -2237,11 +2237,12 @@ def _norm_rows(n: int, c: int, cg: int, variants, blocks_wanted: int) -> tp.Opti
     '''Samples of one position: a span that fills a block's lanes best, as many rows per thread as leave blocks_wanted blocks.'''
     for threads in (BLOCK, 4 * BLOCK):
         spans = []
-        for vec in ((4, 1) if c % 4 == 0 else (1,)):
+        for vec in ((4, 1) if c % 4 == 0 and cg > 1 else (1,)):
             unit = int(np.lcm(cg, vec))
             for many in range(1, min(c, threads * vec) // unit + 1):
                 V = many * unit // vec
-                spans.append((round(threads // V * V / threads, 2) * (1.0 if vec == 4 else 0.5), many * unit, vec, V))
+                #the share of the lanes that have channels, the last span's among them
+                spans.append((round(threads // V * (c // vec) / (_cdiv(c, many * unit) * threads), 2) * (1.0 if vec == 4 else 0.5), many * unit, vec, V))
         if spans:
             _, span, vec, V = max(spans)
             side = threads // V
@@ -2327,12 +2328,13 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     args  = (plan, shape, groups, eps, activation)
     of_groups = max(plan.span // cg, 1)
     rest  = [(b, 0) for b in (g, x, scale, shift, mean, rstd)]
-    rows  = min(_cdiv(n, plan.M), max(1, NORM_GRAD_ROWS // plan.spans)) if plan.kind != 'chunked' else n * plan.chunks
+    sets  = _cdiv(n, plan.M)
+    rows  = _cdiv(sets, _cdiv(sets, max(1, NORM_GRAD_ROWS // plan.spans))) if plan.kind != 'chunked' else n * plan.chunks      #(as many sets each)
     #a single row of sums is what they add up to
     dscale_rows, dshift_rows = (dscale or scratch((c,)), dshift or scratch((c,))) if rows == 1 else (scratch((rows, c)), scratch((rows, c)))
     if plan.kind != 'chunked':
         launches = [_norm_launch(f'group_norm_{plan.kind}_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
-                                 2 * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
+                                 2 * plan.M * plan.P * plan.span + (4 if plan.kind == 'rows' else 2) * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
                                  4 * (3 * x.size + 2 * rows * c), streamable=True, written=(0, 1, 2))]
     else:
         partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
