@@ -2352,21 +2352,58 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 
 # ---------------------------------------------------------------- log probabilities of tokens (log_probs.hip)
 
+LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
+LOG_PROBS_SHORT     = 32            #vectors of rows that share a wave
+LOG_PROBS_WAVE_ROWS = 4             #times LOG_PROBS_AT_A_TIME: rows up to this length have a wave each, longer ones a block
+LOG_PROBS_BLOCKS    = 1024          #blocks from which rows are not cut into slices
+LOG_PROBS_MAX_KEYS  = 4096          #candidates of all slices of a row
+
+
 def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch) -> tp.List[Launch]:
     v = logits.shape[-1]
-    rows = logits.size // v
-    return [Launch('log_probs', (rows, 1, 1), (BLOCK, 1, 1),
-                   [(log_prob, 0), (entropy, 0), (log_sum, 0), (top_log_prob, 0), (top_token, 0), (logits, 0), (tokens, 0)], _u32(0, v, top),
-                   bytes_moved=4 * (logits.size + rows * (4 + 2 * top)), written=(0, 1, 2, 3, 4))]
+    rows    = logits.size // v
+    results = [(b, 0) for b in (log_prob, entropy, log_sum, top_log_prob, top_token)]
+    inputs  = [(logits, 0), (tokens, 0)]
+    moved   = 4 * (logits.size + rows * (4 + 2 * top))
+    vectors = _cdiv(v + (3 if v % 4 else 0), 4)                           #of a row, which may start inside one
+    if v >= 2**29 or rows * BLOCK >= 2**32:
+        raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
+    written = (0, 1, 2, 3, 4)
+    if vectors <= LOG_PROBS_SHORT:
+        lanes = _pow2_at_least(vectors)
+        return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
+                       _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
+    if vectors <= LOG_PROBS_WAVE_ROWS * LOG_PROBS_AT_A_TIME and rows >= LOG_PROBS_BLOCKS:
+        return [Launch('log_probs_wave', (_cdiv(rows, 4), 1, 1), (BLOCK, 1, 1), results + inputs, _u32(0, rows, v, top, 1, 0, 0),
+                       bytes_moved=moved, written=written)]
+    #few rows: slices of whole chunks, four waves to a slice
+    slices = max(1, min(_cdiv(LOG_PROBS_BLOCKS, rows), _cdiv(vectors, 4 * LOG_PROBS_AT_A_TIME), LOG_PROBS_MAX_KEYS // max(top, 1)))
+    slice_ = _cdiv(_cdiv(vectors, 4 * slices), 64) * 64
+    slices = _cdiv(vectors, 4 * slice_)
+    params = _u32(0, rows, v, top, slices, slice_, 0)
+    parts  = scratch((rows, slices, 4)) if slices > 1 else None
+    keys   = scratch((rows, slices, top, 2), np.uint32) if slices > 1 and top else None
+    launch = Launch('log_probs_block', (rows * slices, 1, 1), (BLOCK, 1, 1), (results if slices == 1 else [(None, 0)] * 5) + [(parts, 0), (keys, 0)] + inputs,
+                    params, bytes_moved=moved, written=written if slices == 1 else (5, 6))
+    if slices == 1:
+        return [launch]
+    return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, lds=8 * slices * top,
+                           bytes_moved=4 * rows * (4 + 2 * top + slices * (4 + 2 * top)), written=written)]
 
 
 def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Buffer, entropy: Buffer, g_log_prob, g_entropy, g_top, top_token,
                          top: int) -> tp.List[Launch]:
     v = logits.shape[-1]
-    rows = logits.size // v
-    return [Launch('log_probs_grad', (rows, 1, 1), (BLOCK, 1, 1),
-                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)], _u32(0, v, top),
-                   bytes_moved=4 * (2 * logits.size + rows * (5 + 2 * top)))]
+    rows    = logits.size // v
+    vectors = _cdiv(v + (3 if v % 4 else 0), 4)
+    #a block takes up to two rounds of 256 lanes x 4 vectors
+    slices  = _cdiv(vectors, 2 * 4 * BLOCK)
+    slice_  = _cdiv(_cdiv(vectors, slices), 4) * 4
+    if v >= 2**29 or rows * slices * BLOCK >= 2**32:
+        raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
+    return [Launch('log_probs_grad', (rows * slices, 1, 1), (BLOCK, 1, 1),
+                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)], _u32(0, rows, v, top, slices, slice_, 0),
+                   bytes_moved=4 * (2 * logits.size + rows * (5 + 2 * top)), streamable=True)]
 
 
 # ---------------------------------------------------------------- linear recurrences (recurrence.hip)
