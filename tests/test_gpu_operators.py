@@ -226,6 +226,14 @@ def test_log_probs_of_broken_rows():
     check_log_probs(z, np.array([5, 0, 1, 2, 0, -1], np.int32), 4)
 
 
+@pytest.mark.parametrize('rows,v', [(6, 30000), (1030, 3500), (3, 90001)])
+def test_log_probs_of_rows_that_break_late(rows, v):
+    z = normal(1, rows, v)
+    z[0, v - 100], z[1, v - 2], z[2, v - 1500], z[2, 1] = np.nan, np.inf, np.nan, np.inf
+    t = np.arange(rows, dtype=np.int32)
+    check_log_probs(z, t, 6)
+
+
 def test_log_probs_of_scores_far_from_zero():
     z = normal(1, 4, 900)
     z[0] += 3e4

@@ -13,10 +13,11 @@
 // scores in that one, the others' are masked). Every lane keeps a maximum and the two sums relative to it, changed when the maximum does,
 // once per 16 scores; lanes, waves and slices of a row are joined the same way.
 //
-// The alternatives: the k-th largest of the 64 lanes' maxima is no larger than the k-th largest score, so of the first 1024 scores only what is larger, and as
-// many equal ones as are missing, can be among the k largest: a few more than k scores, whose places are then counted. From then on only
-// scores above the k-th so far are looked at: one comparison per lane and 16 scores, and rarely more. They gather in a list of 64, which
-// is cut to k again when it is full. Where more stand out at once than the list holds, the largest are taken one by one.
+// The alternatives: with the lanes in k groups or more, the smallest of the groups' maxima is no larger than the k-th largest score: a bar, found in six steps
+// and raised by a few bisections where many lanes pass it. Of the first 1024 scores only what reaches the bar can be among the k largest: a few more than k
+// scores, which go into a list. From then on only scores above the bar are looked at: one comparison per lane and 16 scores, and rarely
+// more. The list is cut to k scores, and the bar raised, when it is long. Where more stand out at once than the list holds, the largest are
+// taken one by one. Places in the list are counted once, at the end.
 #include "common.h"
 
 struct LogProbsParams {
@@ -27,7 +28,7 @@ struct LogProbsParams {
 };
 
 constexpr uint32_t NOWHERE = 0x80000000u;
-constexpr uint32_t LIST = 64;
+constexpr uint32_t LIST = 128;
 constexpr int NV = 4;                            // vectors per lane at a time
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
@@ -72,6 +73,16 @@ __device__ __forceinline__ uint32_t place_token(uint64_t key) { return 0xFFFFFFF
 __device__ __forceinline__ uint32_t lanes_below(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u)); }
 __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, (int)lane);
+}
+// How many of the first `count` lanes' keys are larger than this lane's `mine`.
+__device__ __forceinline__ uint32_t place_of(uint64_t key, uint64_t mine, uint32_t count) {
+    uint32_t place = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < count; ++i) place += of_lane(key, i) > mine;
+    return place;
+}
 // put(place, key) for the `top` largest of `count` keys in shared memory, each lane having keys lane, lane + 64 ..: as many are larger as its place says.
 template <class Put>
 __device__ __forceinline__ void rank(const uint64_t* keys, uint32_t count, uint32_t top, Put put) {
@@ -79,121 +90,147 @@ __device__ __forceinline__ void rank(const uint64_t* keys, uint32_t count, uint3
         const uint32_t mine = at + __lane_id();
         const uint64_t key = mine < count ? keys[mine] : 0ull;
         uint32_t place = 0;
-        for (uint32_t i = 0; i < count; ++i) place += keys[i] > key;
+        if (count <= 64u) place = place_of(key, key, count);
+        else
+#pragma unroll 4
+            for (uint32_t i = 0; i < count; ++i) place += keys[i] > key;
         if (mine < count && place < top) put(place, key);
     }
 }
 
-// The k-th largest of the lanes' values (k <= 64): bit by bit, by how many lanes are no smaller.
+// A value that at least k (up to 32) of the lanes' values reach, and not many more: of 2^n >= k groups of lanes the smallest maximum, raised by bisection.
+__device__ __forceinline__ float bar_of(float lane_value, uint32_t k) {
+    const uint32_t group = 64u >> (32u - (uint32_t)__clz((int)k - 1));    // lanes to a group (k = 1: all)
+    float bar = lane_value, most = lane_value;
+    wave_butterfly([&](auto step) {                                       // from the widest step: the lanes of a group lie group's number apart
+        constexpr int S = decltype(step)::value;
+        const float other = lane_xor<S>(bar);
+        bar = (uint32_t)S >= 64u / group ? fmaxf(bar, other) : fminf(bar, other);
+        most = fmaxf(most, lane_xor<S>(most));
+    });
+    for (int i = 0; i < 8; ++i) {
+        if ((uint32_t)__popcll(__builtin_amdgcn_ballot_w64(lane_value >= bar)) <= k + (k >> 2) + 2u) break;
+        const float between = __builtin_fmaf(0.5f, bar, 0.5f * most);
+        const bool enough = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(lane_value >= between)) >= k;
+        bar = enough ? between : bar; most = enough ? most : between;
+    }
+    return bar;
+}
+
+// The k-th largest of the lanes' values, bit by bit, by how many lanes are no smaller.
 __device__ __forceinline__ float kth_largest(float lane_value, uint32_t k) {
     const uint32_t key = score_key(lane_value);
     uint32_t found = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t with = found | 1u << bit;
-        if ((uint32_t)__popcll(__builtin_amdgcn_ballot_w64(key >= with)) >= k) found = with;
-    }
+#pragma nounroll
+    for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1)
+        if ((uint32_t)__popcll(__builtin_amdgcn_ballot_w64(key >= (found | bit))) >= k) found |= bit;
     return key_score(found);
 }
+// The largest value smaller than x (x finite or +inf).
+__device__ __forceinline__ float below(float x) {
+    const uint32_t b = f2u(x);
+    return x == 0.f ? u2f(0x80000001u) : u2f(x > 0.f ? b - 1u : b + 1u);
+}
+
+// 64 x 4 NV scores of a row as a wave holds them: score (i, j) of a lane is that of token first + 256 i + j, if that is below `end`, else -inf.
+struct Chunk {
+    const float* row;
+    uint32_t first, end;
+    __device__ __forceinline__ uint32_t token(int i, int j) const { return first + 256u * i + j; }
+    __device__ __forceinline__ bool valid(int i, int j) const { return token(i, j) < end; }      // (tokens before the row: far above it)
+};
 
 // The list of a wave's candidates in shared memory.
 struct Candidates {
     uint64_t* keys;                              // LIST of them
     uint32_t count, top;
-    float bar;                                   // the k-th largest so far: later scores count where they are larger
+    float bar;                                   // at least `top` scores have been no smaller: later ones count where they are larger
 
     // cuts the list to the `top` largest, in order
     __device__ __forceinline__ void cut() {
         wave_fence();
-        const uint32_t lane = __lane_id();
-        const uint64_t key = lane < count ? keys[lane] : 0ull;
-        uint32_t place = 0;
-        for (uint32_t i = 0; i < count; ++i) place += keys[i] > key;
+        const uint32_t lane = __lane_id(), first = min(count, 64u), second = count - first;
+        const uint64_t a = lane < count ? keys[lane] : 0ull, b = lane + 64u < count ? keys[lane + 64u] : 0ull;
+        uint32_t place_a = place_of(a, a, first), place_b = 0u;
+        if (second != 0u) { place_a += place_of(b, a, second); place_b = place_of(a, b, first) + place_of(b, b, second); }
         wave_fence();
-        if (lane < count && place < top) keys[place] = key;
+        if (lane < count && place_a < top) keys[place_a] = a;
+        if (lane + 64u < count && place_b < top) keys[place_b] = b;
         wave_fence();
         count = min(count, top);
-        bar = key_score((uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(keys[top - 1u] >> 32)));
+        bar = key_score((uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(keys[count - 1u] >> 32)));
     }
-    // Takes from 64 x 4 NV scores, whose places rise with vector, lane and element, what may be among the largest; `token(i, j)` is a score's token and
-    // valid(i, j) whether it is one. `best`: the lane's largest.
-    template <class Token, class Valid>
-    __device__ __forceinline__ void take(const float (&v)[NV][4], float best, Token token, Valid valid) {
+    // Takes from a chunk, whose tokens are behind those of the chunks before, what may be among the largest. `best`: the largest number of each of the lane's
+    // vectors, `most` of all; `broken`: the lane has met a NaN, which does not show among the maxima but passes the comparisons that are made here.
+    __device__ __forceinline__ void take(const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
         const bool fresh = count == 0u;
-        if (!fresh && __builtin_amdgcn_ballot_w64(!(best <= bar)) == 0ull) return;
-        // (a lane's largest is a number; NaNs pass the comparisons below)
-        float above = fresh ? kth_largest(best, top) : bar;
-        for (;;) {
-            uint32_t n = count;
-            bool fits = true;
+        if (fresh) {
+            bar = bar_of(most, top);
+            if (bar == -INFINITY) bar = kth_largest(most, top);           // (much of it masked)
+        } else if (__builtin_amdgcn_ballot_w64(!(most <= bar) || broken) == 0ull) return;
+        // of the first scores those that reach the bar
+        const float from = fresh && bar != -INFINITY ? below(bar) : bar;
+        uint32_t n = count;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            if (__builtin_amdgcn_ballot_w64(!(best[i] <= from) || broken) == 0ull) continue;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool in = !(v[i][j] <= above);
-                    const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-                    if (mask != 0ull) {
-                        const uint32_t many = (uint32_t)__popcll(mask);
-                        fits = fits && n + many <= LIST;
-                        if (fits && in) keys[n + lanes_below(mask)] = place_key(v[i][j], token(i, j));
-                        n += many;
-                    }
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t mask = __builtin_amdgcn_ballot_w64(!(v[i][j] <= from));
+                if (mask != 0ull) {
+                    const uint32_t to = n + lanes_below(mask);
+                    if (!(v[i][j] <= from) && to < LIST) keys[to] = place_key(v[i][j], chunk.token(i, j));
+                    n += (uint32_t)__popcll(mask);
                 }
-            if (fits) { count = n; break; }
-            if (fresh || count == top) {                                  // more than the list holds: one by one
-                one_by_one(v, token, valid);
-                return;
             }
-            cut();
-            above = bar;
         }
-        if (fresh && count < top) {                                       // as many equal ones as are missing, the first ones
+        if (n > LIST) { one_by_one(chunk); return; }
+        count = n;
+        if (fresh && count < top) {                                       // masked scores: as many as are missing, the first of them
             uint32_t need = top - count;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                if (need == 0u) break;
                 uint32_t before = 0, all = 0;
                 bool is[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    is[j] = v[i][j] == above && valid(i, j);
+                    is[j] = v[i][j] == -INFINITY && chunk.valid(i, j);
                     const uint64_t mask = __builtin_amdgcn_ballot_w64(is[j]);
                     before += lanes_below(mask); all += (uint32_t)__popcll(mask);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (is[j] && before < need) keys[count + before] = place_key(v[i][j], token(i, j));
+                    if (is[j] && before < need) keys[count + before] = place_key(-INFINITY, chunk.token(i, j));
                     before += is[j];
                 }
                 const uint32_t taken = min(all, need);
                 count += taken; need -= taken;
             }
         }
-        if (fresh) {
-            if (count >= top) cut();
-            else { wave_fence(); bar = -INFINITY; }                       // (fewer scores than alternatives: the slice is short)
-        } else if (count > LIST - 16u) cut();
+        if (count > top + 24u) cut();                                     // (a bar that stays low lets ever more pass)
     }
-    // The `top` largest of the list, which is at its length after a cut or empty, and these scores.
-    template <class Token, class Valid>
-    __device__ __forceinline__ void one_by_one(const float (&v)[NV][4], Token token, Valid valid) {
+    // The `top` largest of the list and a chunk, one after the other, where more of the chunk pass than the list holds: many equal scores, or many large ones in few
+    // lanes. The scores are read again (they are in the caches), so that this takes no registers from the loop over the row.
+    __device__ __forceinline__ void one_by_one(const Chunk& chunk) {
         const uint32_t lane = __lane_id();
         wave_fence();
-        const uint64_t old = lane < count ? keys[lane] : 0ull;
+        const uint64_t a = lane < count ? keys[lane] : 0ull, b = lane + 64u < count ? keys[lane + 64u] : 0ull;
         uint64_t below = ~0ull;
         uint32_t n = 0;
+#pragma nounroll
         for (; n < top; ++n) {
-            uint64_t best = old < below ? old : 0ull;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint64_t key = valid(i, j) ? place_key(v[i][j], token(i, j)) : 0ull;
-                    if (key < below && key > best) best = key;
-                }
+            uint64_t best = a < below ? a : 0ull;
+            best = b < below && b > best ? b : best;
+#pragma unroll 4
+            for (int e = 0; e < 4 * NV; ++e) {
+                const uint32_t token = chunk.first + 256u * (e >> 2) + (e & 3);
+                const uint64_t key = token < chunk.end ? place_key(chunk.row[token], token) : 0ull;
+                if (key < below && key > best) best = key;
+            }
             best = lanes_allreduce(best, 64u, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
             if (best == 0ull) break;
             below = best;
+            wave_fence();
             if (lane == 0u) keys[n] = best;
         }
         wave_fence();
@@ -225,8 +262,8 @@ __device__ __forceinline__ void write_alternative(const Results& to, uint64_t ro
     if (to.top_token) to.top_token[row * top + place] = (int32_t)place_token(key);
 }
 
-// A wave's part of a row: vectors [q0, q1) of it, a vector being 16 aligned bytes.
-template <class Take>
+// A wave's part of a row: vectors [q0, q1) of it, a vector being 16 aligned bytes. SINGLE: no more than the wave takes at a time.
+template <bool SINGLE, class Take>
 __device__ __forceinline__ void read_row(const float* logits, uint64_t row, uint32_t V, uint32_t q0, uint32_t q1, Sums& sums, Take take) {
     const uint64_t start = row * V;
     const uint32_t lead = (uint32_t)start & 3u, lane = __lane_id();       // scores of other rows in the first vector
@@ -244,33 +281,59 @@ __device__ __forceinline__ void read_row(const float* logits, uint64_t row, uint
         float v[NV][4];
 #pragma unroll
         for (int i = 0; i < NV; ++i) { v[i][0] = next[i].x; v[i][1] = next[i].y; v[i][2] = next[i].z; v[i][3] = next[i].w; }
-        if (q + NV * 64u < q1) fetch(q + NV * 64u);
-        auto token = [&](int i, int j) { return (q + i * 64u + lane) * 4u + j - lead; };
-        auto valid = [&](int i, int j) { return q + i * 64u + lane < q1 && token(i, j) < V; };      // (before the row: far above V)
-        if (q == 0u || q + NV * 64u >= q1)
+        if (!SINGLE && q + NV * 64u < q1) fetch(q + NV * 64u);
+        const Chunk chunk{logits + start, (q + lane) * 4u - lead, min(q1 * 4u - lead, V)};
+        if (SINGLE || q == 0u || q + NV * 64u >= q1)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = valid(i, j) ? v[i][j] : -INFINITY;
-        float best = -INFINITY;
+                for (int j = 0; j < 4; ++j) v[i][j] = chunk.valid(i, j) ? v[i][j] : -INFINITY;
+        float best[NV], most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) best = fmaxf(best, v[i][j]);
-        sums.move(fmaxf(sums.m, best));
+        for (int i = 0; i < NV; ++i) {
+            best[i] = fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]));
+            most = fmaxf(most, best[i]);
+        }
+        sums.move(fmaxf(sums.m, most));
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) sums.add(v[i][j]);
-        take(v, best, token, valid);
+        take(v, best, most, sums.s != sums.s, chunk);
+        if (SINGLE) return;
     }
 }
 
+// put(place, key) for the `top` largest of `count` keys (up to 64 N; zeros are none), by a wave; `room` holds as many in shared memory. The alternatives' bar, for keys.
+template <int N, class Put>
+__device__ __forceinline__ void best_keys(const uint64_t* keys, uint32_t count, uint64_t* room, uint32_t top, Put put) {
+    const uint32_t lane = __lane_id(), group = 64u >> (32u - (uint32_t)__clz((int)top - 1));
+    uint64_t mine[N], bar = 0ull;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine[i] = i * 64u + lane < count ? keys[i * 64u + lane] : 0ull;
+#pragma unroll
+    for (int i = 0; i < N; ++i) bar = mine[i] > bar ? mine[i] : bar;
+    wave_butterfly([&](auto step) {
+        constexpr int S = decltype(step)::value;
+        const uint64_t other = lane_xor<S>(bar);
+        bar = ((uint32_t)S >= 64u / group) == (other > bar) ? other : bar;
+    });
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool in = mine[i] >= bar && mine[i] != 0ull;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+        if (in) room[n + lanes_below(mask)] = mine[i];
+        n += (uint32_t)__popcll(mask);
+    }
+    wave_fence();
+    rank(room, n, top, put);
+}
+
 // A row to a wave.
-extern "C" __global__ __launch_bounds__(256) void log_probs_wave(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,
-                                                                 const float* logits, const uint32_t* tokens, LogProbsParams P) {
+template <bool SINGLE>
+__device__ __forceinline__ void wave_body(const Results& to, const float* logits, const uint32_t* tokens, const LogProbsParams& P) {
     __shared__ uint64_t lists[4][LIST];
-    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint64_t row = (uint64_t)blockIdx.x * 4u + wave;
     if (row >= P.rows) return;
@@ -280,22 +343,32 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_wave(float* log_prob
     Sums sums; sums.start();
     Candidates found{lists[wave], 0u, P.top, 0.f};
     const uint32_t vectors = ((uint32_t)(row * P.V) & 3u) + P.V + 3u >> 2;
-    read_row(logits, row, P.V, 0u, vectors, sums, [&](const float (&v)[NV][4], float best, auto token_of, auto valid) { if (P.top != 0u) found.take(v, best, token_of, valid); });
+    read_row<SINGLE>(logits, row, P.V, 0u, vectors, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
+        if (P.top != 0u) found.take(v, best, most, broken, chunk);
+    });
     sums.join_lanes(64u);
     if (lane == 0u) write_sums(to, row, sums, score);
     if (P.top == 0u) return;
     wave_fence();
     rank(found.keys, found.count, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
 }
+#define LOG_PROBS_WAVE(name, SINGLE)                                                                                                                     \
+    extern "C" __global__ __launch_bounds__(256) void name(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,    \
+                                                           const float* logits, const uint32_t* tokens, LogProbsParams P) {                             \
+        wave_body<SINGLE>(Results{log_prob, entropy, log_sum, top_log_prob, top_token}, logits, tokens, P);                                             \
+    }
+LOG_PROBS_WAVE(log_probs_wave, true)
+LOG_PROBS_WAVE(log_probs_wave_long, false)
 
 // A row, or a slice of one, to a block of four waves. With slices: sums and candidates go to `parts` ([rows, slices, 4] floats: m, s, w) and
-// `keys` ([rows, slices, top]) for log_probs_join.
-extern "C" __global__ __launch_bounds__(256) void log_probs_block(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, float* parts, uint64_t* keys,
-                                                                  const float* logits, const uint32_t* tokens, LogProbsParams P) {
-    __shared__ uint64_t lists[4 * LIST];
-    __shared__ Sums of_wave[4];
-    __shared__ uint32_t counts[4];
+// `keys` ([rows, top, slices]) for log_probs_join.
+extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, float* parts, uint64_t* keys,
+                                                                     const float* logits, const uint32_t* tokens, LogProbsParams P) {
+    constexpr uint32_t WAVES = 4;
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
+    __shared__ uint64_t lists[WAVES * LIST];
+    __shared__ uint64_t all[WAVES * 32];
+    __shared__ Sums of_wave[WAVES];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, slice = blockIdx.x % P.slices;
     const uint64_t row = blockIdx.x / P.slices;
     const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
@@ -304,43 +377,42 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_block(float* log_pro
         return;                                                           // (the whole block)
     }
     const float score = logits[row * P.V + token];
-    const uint32_t vectors = ((uint32_t)(row * P.V) & 3u) + P.V + 3u >> 2, q0 = min((slice * 4u + wave) * P.slice, vectors), q1 = min(q0 + P.slice, vectors);
+    const uint32_t vectors = ((uint32_t)(row * P.V) & 3u) + P.V + 3u >> 2, q0 = min((slice * WAVES + wave) * P.slice, vectors), q1 = min(q0 + P.slice, vectors);
     Sums sums; sums.start();
     Candidates found{lists + wave * LIST, 0u, P.top, 0.f};
-    if (q0 < q1) read_row(logits, row, P.V, q0, q1, sums, [&](const float (&v)[NV][4], float best, auto token_of, auto valid) { if (P.top != 0u) found.take(v, best, token_of, valid); });
+    if (q0 < q1) read_row<false>(logits, row, P.V, q0, q1, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
+        if (P.top != 0u) found.take(v, best, most, broken, chunk);
+    });
     sums.join_lanes(64u);
-    if (P.top != 0u && found.count > P.top) found.cut();
-    if (lane == 0u) { of_wave[wave] = sums; counts[wave] = found.count; }
+    if (lane == 0u) of_wave[wave] = sums;
+    if (P.top != 0u) {
+        // the wave's largest, in order, and zeros where there are not as many
+        if (found.count != 0u) found.cut();
+        if (lane >= found.count && lane < P.top) found.keys[lane] = 0ull;
+    }
     __syncthreads();
     if (wave != 0u) return;
-#pragma unroll
-    for (int k = 1; k < 4; ++k) sums.join(of_wave[k]);
+    sums = of_wave[lane & (WAVES - 1)];
+    sums.join_lanes(WAVES);
     if (P.slices == 1u) {
         if (lane == 0u) write_sums(to, row, sums, score);
     } else if (lane < 3u) parts[(row * P.slices + slice) * 4u + lane] = lane == 0u ? sums.m : lane == 1u ? sums.s : sums.w;
     if (P.top == 0u) return;
-    // the four lists behind one another
-    uint32_t count = counts[0];
-#pragma unroll
-    for (uint32_t k = 1; k < 4u; ++k) {
-        const uint64_t key = lists[k * LIST + min(lane, LIST - 1u)];
-        wave_fence();
-        if (lane < counts[k]) lists[count + lane] = key;
-        wave_fence();
-        count += counts[k];
-    }
-    if (P.slices == 1u) rank(lists, count, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
-    else {
-        uint64_t* const out = keys + (row * P.slices + slice) * P.top;
-        if (count < P.top) for (uint32_t k = count + lane; k < P.top; k += 64u) out[k] = 0ull;      // (a slice of fewer scores)
-        rank(lists, count, P.top, [&](uint32_t place, uint64_t key) { out[place] = key; });
-    }
+    // place by place, so that every lane sees high places, and the bar over the lanes' largest is near
+    for (uint32_t e = lane; e < WAVES * P.top; e += 64u) all[e] = lists[(e & (WAVES - 1u)) * LIST + e / WAVES];
+    wave_fence();
+    uint64_t* const out = keys + row * P.slices * P.top + slice;          // (also place by place)
+    if (P.slices != 1u && lane < P.top) out[lane * P.slices] = 0ull;      // (a slice may have fewer scores)
+    best_keys<2>(all, WAVES * P.top, lists, P.top, [&](uint32_t place, uint64_t key) {
+        if (P.slices == 1u) write_alternative(to, row, P.top, place, key, sums);
+        else out[place * P.slices] = key;
+    });
 }
 
 // Joins the slices of a row: a wave to a row.
 extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, const float* parts,
                                                                 const uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
-    extern __shared__ uint64_t all[];                                     // slices * top of them
+    extern __shared__ uint64_t room[];                                    // slices * top of them
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
     const uint32_t lane = threadIdx.x;
     const uint64_t row = blockIdx.x;
@@ -355,30 +427,11 @@ extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob,
     sums.join_lanes(64u);
     if (lane == 0u) write_sums(to, row, sums, score);
     if (P.top == 0u) return;
-    // only what is no smaller than the k-th largest of the lanes' largest can be among the k largest
     const uint32_t count = P.slices * P.top;
-    const uint64_t* const from = keys + row * count;
-    uint64_t best = 0ull;
-    for (uint32_t k = lane; k < count; k += 64u) { const uint64_t key = from[k]; best = key > best ? key : best; }
-    uint64_t least = 0ull;
-#pragma unroll 8
-    for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t with = least | 1ull << bit;
-        if ((uint32_t)__popcll(__builtin_amdgcn_ballot_w64(best >= with)) >= P.top) least = with;
-    }
-    uint32_t n = 0;
-    for (uint32_t k = 0; k < count; k += 64u) {
-        const uint64_t key = k + lane < count ? from[k + lane] : 0ull;
-        const bool in = key >= least && key != 0ull;
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-        if (in) all[n + lanes_below(mask)] = key;
-        n += (uint32_t)__popcll(mask);
-    }
-    wave_fence();
-    rank(all, n, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
+    best_keys<16>(keys + row * count, count, room, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
 }
 
-// Short rows: 2^log2_lanes lanes to a row, a vector to a lane, and several rows to a wave. The alternatives one by one.
+// Short rows: 2^log2_lanes lanes to a row, four vectors to a lane, and several rows to a wave. The alternatives one by one.
 extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,
                                                                   const float* logits, const uint32_t* tokens, LogProbsParams P) {
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
@@ -391,36 +444,57 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_pro
     const uint32_t lead = (uint32_t)start & 3u;
     const float* const x = logits + start;
     const float score = given ? x[token] : 0.f;
-    float v[4], best = -INFINITY;
+    float v[NV][4], best = -INFINITY;
+    auto at = [&](int i, int j) { return (i * lanes + lane) * 4u + j - lead; };      // (before the row: far above V)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = -INFINITY;
-    auto at = [&](int j) { return lane * 4u + j - lead; };                // (before the row: far above V)
-    if (given) {
-        if (lane * 4u >= lead && lane * 4u + 4u <= lead + P.V) { const f32x4 t = *reinterpret_cast<const f32x4*>(logits + (start - lead) + lane * 4u); v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
-        else
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (at(j) < P.V) v[j] = x[at(j)];
+        for (int j = 0; j < 4; ++j) v[i][j] = -INFINITY;
+        const uint32_t first = (i * lanes + lane) * 4u;
+        if (given && first >= lead && first + 4u <= lead + P.V) {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(logits + (start - lead) + first);
+            v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
+        } else if (given)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (at(i, j) < P.V) v[i][j] = x[at(i, j)];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) best = fmaxf(best, v[j]);
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) best = fmaxf(best, v[i][j]);
     Sums sums; sums.start();
     sums.move(fmaxf(sums.m, best));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums.add(v[j]);
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums.add(v[i][j]);
     sums.join_lanes(lanes);
     if (there && !given) write_padding(to, row, lane, lanes, P.top);
     if (given && lane == 0u) write_sums(to, row, sums, score);
-    uint64_t below = ~0ull;
-    for (uint32_t k = 0; k < P.top; ++k) {
-        uint64_t key = 0ull;
+    if (P.top == 0u) return;
+    // A place's key is the score's; which of the equal ones it is, the number of the first one behind the last place tells.
+    uint32_t keys[NV][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint64_t mine = at(j) < P.V ? place_key(v[j], at(j)) : 0ull;
-            if (mine < below && mine > key) key = mine;
-        }
-        key = lanes_allreduce(key, lanes, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        below = key;
-        if (given && lane == (k & (lanes - 1u))) write_alternative(to, row, P.top, k, key, sums);
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keys[i][j] = at(i, j) < P.V ? score_key(v[i][j]) : 0u;
+    for (uint32_t k = 0; k < P.top; ++k) {
+        uint32_t key = 0u, number = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) key = max(key, keys[i][j]);
+        key = lanes_allreduce(key, lanes, [](uint32_t a, uint32_t b) { return max(a, b); });
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+            for (int j = 3; j >= 0; --j) number = keys[i][j] == key && key != 0u ? at(i, j) : number;
+        number = lanes_allreduce(number, lanes, [](uint32_t a, uint32_t b) { return min(a, b); });
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) keys[i][j] = at(i, j) == number ? 0u : keys[i][j];
+        if (given && lane == (k & (lanes - 1u))) write_alternative(to, row, P.top, k, (uint64_t)key << 32 | (0xFFFFFFFFu - number), sums);
     }
 }
 
@@ -441,8 +515,8 @@ __device__ __forceinline__ float grad_of(float x, float lse, float total, float 
 
 extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, const float* logits, const uint32_t* tokens, const float* log_sum, const float* entropy,
                                                                  const float* g_log_prob, const float* g_entropy, const float* g_top, const int32_t* top_token, LogProbsParams P) {
-    const uint32_t slice = blockIdx.x % P.slices;
-    const uint64_t row = blockIdx.x / P.slices, start = row * P.V;
+    const uint32_t block = gridDim.x - 1u - blockIdx.x, slice = block % P.slices;      // (the last rows first: those the forward pass has left behind the L2s)
+    const uint64_t row = block / P.slices, start = row * P.V;
     const uint32_t lead = (uint32_t)start & 3u, vectors = lead + P.V + 3u >> 2;
     const uint32_t q0 = slice * P.slice, q1 = min(q0 + P.slice, vectors);
     const uint32_t token = tokens[row];

@@ -2353,10 +2353,10 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 # ---------------------------------------------------------------- log probabilities of tokens (log_probs.hip)
 
 LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
-LOG_PROBS_SHORT     = 32            #vectors of rows that share a wave
-LOG_PROBS_WAVE_ROWS = 4             #times LOG_PROBS_AT_A_TIME: rows up to this length have a wave each, longer ones a block
-LOG_PROBS_BLOCKS    = 1024          #blocks from which rows are not cut into slices
-LOG_PROBS_MAX_KEYS  = 4096          #candidates of all slices of a row
+LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane
+LOG_PROBS_WAVE      = 1024          #rows of up to this many vectors have a wave each where there are enough of them, longer ones a block
+LOG_PROBS_ROWS      = 1024          #enough rows not to be cut
+LOG_PROBS_MAX_KEYS  = 1024          #candidates of all slices of a row
 
 
 def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch) -> tp.List[Launch]:
@@ -2370,21 +2370,22 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4)
     if vectors <= LOG_PROBS_SHORT:
-        lanes = _pow2_at_least(vectors)
+        lanes = _pow2_at_least(_cdiv(vectors, 4))
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
-    if vectors <= LOG_PROBS_WAVE_ROWS * LOG_PROBS_AT_A_TIME and rows >= LOG_PROBS_BLOCKS:
-        return [Launch('log_probs_wave', (_cdiv(rows, 4), 1, 1), (BLOCK, 1, 1), results + inputs, _u32(0, rows, v, top, 1, 0, 0),
-                       bytes_moved=moved, written=written)]
-    #few rows: slices of whole chunks, four waves to a slice
-    slices = max(1, min(_cdiv(LOG_PROBS_BLOCKS, rows), _cdiv(vectors, 4 * LOG_PROBS_AT_A_TIME), LOG_PROBS_MAX_KEYS // max(top, 1)))
+    if vectors <= LOG_PROBS_AT_A_TIME or (vectors <= LOG_PROBS_WAVE and rows >= LOG_PROBS_ROWS):
+        return [Launch('log_probs_wave' if vectors <= LOG_PROBS_AT_A_TIME else 'log_probs_wave_long', (_cdiv(rows, 4), 1, 1), (BLOCK, 1, 1),
+                       results + inputs, _u32(0, rows, v, top, 1, 0, 0), bytes_moved=moved, written=written)]
+    #a block to a row; where there are few, slices of whole chunks, joined by a second launch
+    slices = max(1, min(_cdiv(LOG_PROBS_ROWS, rows), _cdiv(vectors, 4 * LOG_PROBS_AT_A_TIME), LOG_PROBS_MAX_KEYS // max(top, 1)))
     slice_ = _cdiv(_cdiv(vectors, 4 * slices), 64) * 64
     slices = _cdiv(vectors, 4 * slice_)
     params = _u32(0, rows, v, top, slices, slice_, 0)
     parts  = scratch((rows, slices, 4)) if slices > 1 else None
     keys   = scratch((rows, slices, top, 2), np.uint32) if slices > 1 and top else None
-    launch = Launch('log_probs_block', (rows * slices, 1, 1), (BLOCK, 1, 1), (results if slices == 1 else [(None, 0)] * 5) + [(parts, 0), (keys, 0)] + inputs,
-                    params, bytes_moved=moved, written=written if slices == 1 else (5, 6))
+    launch = Launch('log_probs_block', (rows * slices, 1, 1), (BLOCK, 1, 1),
+                    (results if slices == 1 else [(None, 0)] * 5) + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=moved,
+                    written=written if slices == 1 else (5, 6))
     if slices == 1:
         return [launch]
     return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, lds=8 * slices * top,
