@@ -21,7 +21,7 @@
 #include "common.h"
 
 struct LogProbsParams {
-    uint32_t first;
+    uint32_t first;                              // (the gradient: the rows, and in bit 31 whether the result is stored past the caches)
     uint32_t rows, V, top;
     uint32_t slices, slice;                      // blocks per row, vectors of a row to a wave
     uint32_t log2_lanes;                         // lanes per row, where a wave has several rows
@@ -500,8 +500,11 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_pro
 
 // ---------------------------------------------------------------------------------------------- gradient
 
-// One read and one write per score: blocks of 256 lanes x 4 NV scores of a row. Cotangents that are null are zeros. The tokens whose own log probabilities have
-// cotangents are done once more behind the block's other stores: a score's value anew, and all its cotangents in one fixed order.
+// One read and one write per score. 2^log2_lanes lanes to a row (or to a slice of a long one), NV vectors of each in flight per lane; several rows to a block where
+// they are short. Cotangents that are null are zeros. The tokens whose own log probabilities have cotangents are done once more behind the
+// block's other stores: a score's value anew, and all its cotangents in one fixed order.
+// What bounds it: memory, 4096 rows of 32000 (1.02 GB) 170 us, 6.0 TB/s; rows from the last one on, since the forward pass has left those in the
+// 256 MB behind the L2s (198 us from the first one on).
 template <bool ENTROPY>
 __device__ __forceinline__ float grad_of(float x, float lse, float total, float gh, float H) {
     const float lp = x - lse;
@@ -515,48 +518,58 @@ __device__ __forceinline__ float grad_of(float x, float lse, float total, float 
 
 extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, const float* logits, const uint32_t* tokens, const float* log_sum, const float* entropy,
                                                                  const float* g_log_prob, const float* g_entropy, const float* g_top, const int32_t* top_token, LogProbsParams P) {
-    const uint32_t block = gridDim.x - 1u - blockIdx.x, slice = block % P.slices;      // (the last rows first: those the forward pass has left behind the L2s)
-    const uint64_t row = block / P.slices, start = row * P.V;
-    const uint32_t lead = (uint32_t)start & 3u, vectors = lead + P.V + 3u >> 2;
-    const uint32_t q0 = slice * P.slice, q1 = min(q0 + P.slice, vectors);
-    const uint32_t token = tokens[row];
-    const float lse = log_sum[row];
-    const bool nothing = token >= P.V || lse == -INFINITY;
+    const uint32_t lanes = 1u << P.log2_lanes, lane = threadIdx.x & (lanes - 1u), side = 256u >> P.log2_lanes;
+    const uint32_t rows = without_stream_bit(P.first), block = gridDim.x - 1u - blockIdx.x, slice = block % P.slices;
     const bool stream = streams_result(P.first);
-    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(logits + (start - lead), nothing ? 0u : (lead + P.V) * 4u), d_rsrc = make_rsrc(dx + (start - lead), (lead + P.V) * 4u);
-    const float own = g_log_prob ? g_log_prob[row] : 0.f, gh = g_entropy ? g_entropy[row] : 0.f, H = entropy[row];
+    const uint64_t row0 = (uint64_t)(block / P.slices) * side, row = row0 + (threadIdx.x >> P.log2_lanes), start0 = row0 * P.V;
+    const bool there = row < rows;
+    const uint32_t at0 = ((uint32_t)start0 & 3u) + (uint32_t)(row - row0) * P.V, lead = at0 & 3u;      // where the row starts in the block's scores
+    const uint32_t vectors = lead + P.V + 3u >> 2, q0 = slice * P.slice, q1 = there ? min(q0 + P.slice, vectors) : 0u;
+    const uint32_t bytes = (((uint32_t)start0 & 3u) + (uint32_t)min((uint64_t)side, rows - row0) * P.V) * 4u;
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(logits + (start0 - (start0 & 3u)), bytes), d_rsrc = make_rsrc(dx + (start0 - (start0 & 3u)), bytes);
+    const uint32_t token = there ? tokens[row] : 0xFFFFFFFFu;
+    const float lse = there ? log_sum[row] : 0.f, H = there ? entropy[row] : 0.f;
+    const bool nothing = token >= P.V || lse == -INFINITY;
+    const float own = g_log_prob && there ? g_log_prob[row] : 0.f, gh = g_entropy && there ? g_entropy[row] : 0.f;
     float total = own;
-    for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
-    for (uint32_t q = q0 + threadIdx.x; q < q1; q += 256u * NV) {
+    if (there) for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
+    const uint32_t from = at0 - lead;
+    for (uint32_t q = q0 + lane; q < q1; q += lanes * NV) {
         f32x4 v[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, q + i * 256u < q1 ? (q + i * 256u) * 16u : NOWHERE, 0, 0));
+        for (int i = 0; i < NV; ++i)
+            v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, q + i * lanes < q1 && !nothing ? (from + (q + i * lanes) * 4u) * 4u : NOWHERE, 0, 0));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t at = q + i * 256u;
+            const uint32_t at = q + i * lanes;
             f32x4 d;
+            if (g_entropy == nullptr)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : gh == 0.f ? grad_of<false>(v[i][j], lse, total, gh, H) : grad_of<true>(v[i][j], lse, total, gh, H);
+                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<false>(v[i][j], lse, total, gh, H);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<true>(v[i][j], lse, total, gh, H);
             if (at >= q1) continue;
             if (at * 4u >= lead && at * 4u + 4u <= lead + P.V) {
                 const u32x4 t = u32x4{f2u(d[0]), f2u(d[1]), f2u(d[2]), f2u(d[3])};
-                if (stream) __builtin_amdgcn_raw_buffer_store_b128(t, d_rsrc, at * 16u, 0, 2);
-                else __builtin_amdgcn_raw_buffer_store_b128(t, d_rsrc, at * 16u, 0, 0);
+                if (stream) __builtin_amdgcn_raw_buffer_store_b128(t, d_rsrc, (from + at * 4u) * 4u, 0, 2);
+                else __builtin_amdgcn_raw_buffer_store_b128(t, d_rsrc, (from + at * 4u) * 4u, 0, 0);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) if (at * 4u + j - lead < P.V) dx[start + (at * 4u + j - lead)] = d[j];
+                for (int j = 0; j < 4; ++j) if (at * 4u + j - lead < P.V) dx[row * P.V + (at * 4u + j - lead)] = d[j];
             }
         }
     }
-    if (nothing) return;
     __syncthreads();
-    // thread k < top: alternative k, thread `top`: the given token; in the block that has its score
-    const uint32_t k = threadIdx.x;
-    if (k > P.top) return;
-    const uint32_t mine = k < P.top ? (uint32_t)top_token[row * P.top + k] : token, vector = mine + lead >> 2;
-    if (mine >= P.V || vector < q0 || vector >= q1) return;
-    float d = grad_of<true>(logits[start + mine], lse, total, gh, H);
-    if (mine == token) d += own;
-    for (uint32_t i = 0; i < P.top; ++i) if ((uint32_t)top_token[row * P.top + i] == mine) d += g_top[row * P.top + i];
-    dx[start + mine] = d;
+    if (nothing || !there) return;
+    // number k < top: alternative k, number `top`: the given token; in the slice that has its score
+    for (uint32_t k = lane; k <= P.top; k += lanes) {
+        const uint32_t mine = k < P.top ? (uint32_t)top_token[row * P.top + k] : token, vector = mine + lead >> 2;
+        if (mine >= P.V || vector < q0 || vector >= q1) continue;
+        const float x = logits[row * P.V + mine];
+        float d = g_entropy == nullptr ? grad_of<false>(x, lse, total, gh, H) : grad_of<true>(x, lse, total, gh, H);
+        if (mine == token) d += own;
+        for (uint32_t i = 0; i < P.top; ++i) if ((uint32_t)top_token[row * P.top + i] == mine) d += g_top[row * P.top + i];
+        dx[row * P.V + mine] = d;
+    }
 }

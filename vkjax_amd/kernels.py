@@ -2397,13 +2397,16 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
     v = logits.shape[-1]
     rows    = logits.size // v
     vectors = _cdiv(v + (3 if v % 4 else 0), 4)
-    #a block takes up to two rounds of 256 lanes x 4 vectors
+    #four vectors to a lane, as few lanes to a row as that needs; of rows that are longer than a block's lanes, up to two rounds to a block
+    lanes   = min(_pow2_at_least(_cdiv(vectors, 4)), BLOCK)
     slices  = _cdiv(vectors, 2 * 4 * BLOCK)
     slice_  = _cdiv(_cdiv(vectors, slices), 4) * 4
-    if v >= 2**29 or rows * slices * BLOCK >= 2**32:
+    blocks  = _cdiv(rows, BLOCK // lanes) * slices
+    if v >= 2**29 or rows >= 2**31 or blocks * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
-    return [Launch('log_probs_grad', (rows * slices, 1, 1), (BLOCK, 1, 1),
-                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)], _u32(0, rows, v, top, slices, slice_, 0),
+    return [Launch('log_probs_grad', (blocks, 1, 1), (BLOCK, 1, 1),
+                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)],
+                   _u32(rows, rows, v, top, slices, slice_, lanes.bit_length() - 1),
                    bytes_moved=4 * (2 * logits.size + rows * (5 + 2 * top)), streamable=True)]
 
 
