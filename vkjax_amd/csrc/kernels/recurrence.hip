@@ -307,7 +307,8 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
     if (tile.at_the_end()) store<VEC>(now, tile.state_rsrc(dstate), tile.state_at());
 }
 
-// Names: _v<channels per lane>_l<steps per thread>, _gated, _chain (more tiles than one along time)
+// Names: _v<channels per lane>_l<steps per thread>, _gated, _chain (more tiles than one along time). Several numbers of steps, so that tiles need not reach far
+// beyond the last step.
 #define RECURRENCE(name, VEC, L, GATED, CHAIN)                                                                                                          \
     extern "C" __global__ __launch_bounds__(256, 2) void recurrence_##name(float* h, float* last, const float* factor, const float* x, const float* state, \
                                                                         const int32_t* lengths, unsigned long long* chain, RecurrenceParams P) {        \
@@ -318,12 +319,13 @@ __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, 
             const float* x, const float* state, const int32_t* lengths, const float* g, const float* g_last, unsigned long long* chain, RecurrenceParams P) { \
         recurrence_grad_body<VEC, L, GATED, CHAIN>(dfactor, dx, dstate, h, factor, x, state, lengths, g, g_last, chain, P);                             \
     }
-#define RECURRENCE_VARIANTS(KERNEL, LONG4, LONG1)                                                                   \
-    KERNEL(v4_l1, 4, 1, false, false)            KERNEL(v4_l1_gated, 4, 1, true, false)                             \
-    KERNEL(v4, 4, LONG4, false, false)           KERNEL(v4_gated, 4, LONG4, true, false)                            \
-    KERNEL(v4_chain, 4, LONG4, false, true)      KERNEL(v4_gated_chain, 4, LONG4, true, true)                       \
-    KERNEL(v1_l1, 1, 1, false, false)            KERNEL(v1_l1_gated, 1, 1, true, false)                             \
-    KERNEL(v1, 1, LONG1, false, false)           KERNEL(v1_gated, 1, LONG1, true, false)                            \
-    KERNEL(v1_chain, 1, LONG1, false, true)      KERNEL(v1_gated_chain, 1, LONG1, true, true)
-RECURRENCE_VARIANTS(RECURRENCE, 16, 16)
-RECURRENCE_VARIANTS(RECURRENCE_GRAD, 6, 8)
+#define RECURRENCE_VARIANTS(KERNEL, VEC, L)                                                                          \
+    KERNEL(v##VEC##_l##L, VEC, L, false, false)            KERNEL(v##VEC##_l##L##_gated, VEC, L, true, false)
+#define RECURRENCE_CHAINS(KERNEL, VEC, L)                                                                            \
+    KERNEL(v##VEC##_l##L##_chain, VEC, L, false, true)     KERNEL(v##VEC##_l##L##_gated_chain, VEC, L, true, true)
+RECURRENCE_VARIANTS(RECURRENCE, 4, 1)  RECURRENCE_VARIANTS(RECURRENCE, 4, 4)  RECURRENCE_VARIANTS(RECURRENCE, 4, 8)  RECURRENCE_VARIANTS(RECURRENCE, 4, 16)
+RECURRENCE_VARIANTS(RECURRENCE, 1, 1)  RECURRENCE_VARIANTS(RECURRENCE, 1, 4)  RECURRENCE_VARIANTS(RECURRENCE, 1, 16)
+RECURRENCE_CHAINS(RECURRENCE, 4, 8)    RECURRENCE_CHAINS(RECURRENCE, 4, 16)   RECURRENCE_CHAINS(RECURRENCE, 1, 16)
+RECURRENCE_VARIANTS(RECURRENCE_GRAD, 4, 1)  RECURRENCE_VARIANTS(RECURRENCE_GRAD, 4, 3)  RECURRENCE_VARIANTS(RECURRENCE_GRAD, 4, 6)  RECURRENCE_VARIANTS(RECURRENCE_GRAD, 4, 8)
+RECURRENCE_VARIANTS(RECURRENCE_GRAD, 1, 1)  RECURRENCE_VARIANTS(RECURRENCE_GRAD, 1, 4)  RECURRENCE_VARIANTS(RECURRENCE_GRAD, 1, 8)
+RECURRENCE_CHAINS(RECURRENCE_GRAD, 4, 4)    RECURRENCE_CHAINS(RECURRENCE_GRAD, 4, 6)    RECURRENCE_CHAINS(RECURRENCE_GRAD, 1, 8)

@@ -2413,9 +2413,13 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
 # ---------------------------------------------------------------- linear recurrences (recurrence.hip)
 
 RECURRENCE_THREADS = 256
-#steps per thread by channels per lane
-RECURRENCE_STEPS, RECURRENCE_GRAD_STEPS = {4: 16, 1: 16}, {4: 6, 1: 8}
+#steps per thread of the kernels by channels per lane: for a single tile along time, and for several
+RECURRENCE_STEPS      = {4: ((1, 4, 8, 16), (8, 16)), 1: ((1, 4, 16), (16,))}
+RECURRENCE_GRAD_STEPS = {4: ((1, 3, 6, 8), (4, 6)), 1: ((1, 4, 8), (8,))}
 RECURRENCE_CHAIN_CHANNELS = 32          #channels of a tile whose state goes on to another one
+#what a launch takes, by measurement (us): 3, and 0.28 for every step that a thread goes through, and what following the chain takes - 2, and 1 for
+#every 8 tiles in a row -; and its bytes at 5.3 MB a us, of a tile in a chain as if it had 96 steps more
+RECURRENCE_START, RECURRENCE_STEP, RECURRENCE_CHAIN, RECURRENCE_CHAIN_TILE, RECURRENCE_CHAIN_STEPS, RECURRENCE_RATE = 3.0, 0.28, 2.0, 0.125, 96, 5.3e6
 
 
 class RecurrenceTiling(tp.NamedTuple):
@@ -2427,16 +2431,28 @@ class RecurrenceTiling(tp.NamedTuple):
     tiles:   int            #along time
 
 
-def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec: tp.Dict[int, int]) -> RecurrenceTiling:
+def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays: int) -> RecurrenceTiling:
     '''How a recurrence is cut: as few groups of steps side by side as time needs, and with the lanes that leaves as many channels as
-    there are, but at most RECURRENCE_CHAIN_CHANNELS where time takes more than one tile.'''
-    vec   = 4 if channels % 4 == 0 else 1
-    steps = 1 if time == 1 else steps_by_vec[vec]
-    wide  = _pow2_at_least(_cdiv(channels, vec))
-    lanes = min(wide, RECURRENCE_THREADS // min(_pow2_at_least(_cdiv(time, steps)), RECURRENCE_THREADS))
-    lanes = max(lanes, min(wide, RECURRENCE_CHAIN_CHANNELS // vec))
+    there are, but at least a whole line of them; of the numbers of steps per thread the one that is estimated to take the least time
+    for reading and writing `arrays` arrays.'''
+    vec    = 4 if channels % 4 == 0 else 1
+    wide   = _pow2_at_least(_cdiv(channels, vec))
+    single, several = steps_by_vec[vec]
+    best   = None
+    for steps in sorted(set(single + several), reverse=True):
+        lanes  = min(wide, RECURRENCE_THREADS // min(_pow2_at_least(_cdiv(time, steps)), RECURRENCE_THREADS))
+        lanes  = max(lanes, min(wide, RECURRENCE_CHAIN_CHANNELS // vec))
+        covers = steps * (RECURRENCE_THREADS // lanes)
+        tiles  = _cdiv(time, covers)
+        if steps not in (single if tiles == 1 else several):
+            continue
+        chain = tiles > 1
+        moved = 4 * arrays * batch * _cdiv(channels, lanes * vec) * lanes * vec * tiles * (covers + RECURRENCE_CHAIN_STEPS * chain)
+        cost  = RECURRENCE_START + RECURRENCE_STEP * steps + (RECURRENCE_CHAIN + RECURRENCE_CHAIN_TILE * tiles) * chain + moved / RECURRENCE_RATE
+        if best is None or cost < best[0]:
+            best = (cost, steps, lanes, tiles)
+    _, steps, lanes, tiles = best
     cstrips = _cdiv(channels, lanes * vec)
-    tiles   = _cdiv(time, steps * (RECURRENCE_THREADS // lanes))
     if batch * cstrips * tiles * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
         raise NotImplementedError(f'a recurrence over {channels} channels in {batch} sequences of {time} steps')
     return RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
@@ -2444,7 +2460,7 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec: tp.Dic
 
 def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int) -> Launch:
     _, t, c = shape
-    kernel  = f'{name}_v{tiling.vec}' + ('_l1' if tiling.steps == 1 else '') + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
+    kernel  = f'{name}_v{tiling.vec}_l{tiling.steps}' + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
     #(what tiles hand on: a line for the ticket, then a word of 64 bits per channel and tile)
     chain   = None if tiling.tiles == 1 else zeroed(16 + 2 * tiling.tiles * tiling.strips * tiling.lanes * tiling.vec, f'{kernel} {tuple(tiling)}')
     buffers = [(v, 0) for v in arrays] + [(chain, 0)]
@@ -2460,13 +2476,13 @@ def _recurrence_shape(x: Buffer, lengths):
 
 def linear_recurrence(h, last, factor: Buffer, x: Buffer, state, lengths, gated: bool, reverse: bool, zeroed) -> tp.List[Launch]:
     shape = _recurrence_shape(x, lengths)
-    return [_recurrence_launch('recurrence', x, recurrence_tiling(*shape, RECURRENCE_STEPS), shape, gated, reverse, zeroed,
+    return [_recurrence_launch('recurrence', x, recurrence_tiling(*shape, RECURRENCE_STEPS, 3), shape, gated, reverse, zeroed,
                                (h, last, factor, x, state, lengths), (0, 1), 4 * (3 * x.size + 2 * x.shape[0] * x.shape[2]))]
 
 
 def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Buffer, state, lengths, g, g_last, gated: bool, reverse: bool,
                            zeroed) -> tp.List[Launch]:
     shape = _recurrence_shape(x, lengths)
-    return [_recurrence_launch('recurrence_grad', x, recurrence_tiling(*shape, RECURRENCE_GRAD_STEPS), shape, gated, reverse, zeroed,
+    return [_recurrence_launch('recurrence_grad', x, recurrence_tiling(*shape, RECURRENCE_GRAD_STEPS, 5 + gated), shape, gated, reverse, zeroed,
                                (dfactor, dx, dstate, h, factor, x if gated else None, state, lengths, g, g_last), (0, 1, 2),
                                4 * ((5 + gated) * x.size + 2 * x.shape[0] * x.shape[2]))]
