@@ -112,12 +112,16 @@ __device__ __forceinline__ void for_groups(const NormParams& P, uint32_t groups,
         const uint32_t m = use ? at / groups : 0u, g = use ? at - m * groups : 0u;
         entry.start();
         if (use)
-            for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq)
-                for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) entry.add((m * P.P + q) * P.span + g * channels_per_group + ch, q, g * channels_per_group + ch);
+            for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) {
+#pragma unroll 4
+                for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq) entry.add((m * P.P + q) * P.span + g * channels_per_group + ch, q, g * channels_per_group + ch);
+            }
         entry.join(lanes);
         if (use && entry.again())
-            for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq)
-                for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) entry.add_again((m * P.P + q) * P.span + g * channels_per_group + ch, q);
+            for (uint32_t ch = lc; ch < channels_per_group; ch += 1u << P.log2_lc) {
+#pragma unroll 4
+                for (uint32_t q = lq; q < P.P; q += 1u << P.log2_lq) entry.add_again((m * P.P + q) * P.span + g * channels_per_group + ch, q);
+            }
         entry.join_again(lanes);
         if (use) done(m, g, lane == 0u, entry);
     }
@@ -786,33 +790,36 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
             const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                                                         \
         grad_apply_body<VEC>(dx, partial, g, x, scale, shift, means, rstds, P);                                                                                     \
     }
-HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 4, 1024)  HELD(4, 13, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 8, 1024)
+HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 4, 1024)  HELD(4, 16, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 8, 1024)
 HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 2, 1024)  HELD_GRAD(4, 4, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 4, 1024)
 ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)  ROWS(4, 8, 256)  ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)  ROWS(4, 1, 1024)  ROWS(1, 4, 1024) ROWS(4, 2, 1024) ROWS(1, 1, 1024)
 CHUNKED(4)
 CHUNKED(1)
 
-// Sums of the columns of two arrays [rows, C]: 64 columns to a block, 16 waves that take every 16th row each.
+// Sums of the columns of two arrays [rows, C]: 32 columns to a block, and 32 lanes that take every 32nd row of them each. (1024 rows of 256: 64 columns to a
+// block 10 us, 32 6: a launch of few blocks, bound by how many loads a lane has behind one another.)
 extern "C" __global__ __launch_bounds__(1024) void group_norm_columns(float* first, float* second, const float* first_rows, const float* second_rows, uint32_t rows, uint32_t C) {
-    __shared__ float parts[16][64];
-    const uint32_t blocks = (C + 63u) / 64u, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = blockIdx.x % blocks * 64u + lane;
+    __shared__ float parts[32][33];
+    const uint32_t blocks = (C + 31u) / 32u, lane = threadIdx.x & 31u, side = threadIdx.x >> 5, c = blockIdx.x % blocks * 32u + lane;
     const bool other = blockIdx.x >= blocks;
     const float* const from = other ? second_rows : first_rows;
     float* const to = other ? second : first;
     if (to == nullptr) return;
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    float sums[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sums[k] = 0.f;
     if (c < C) {
-        uint32_t r = wave;
-        for (; r + 48u < rows; r += 64u)
+        uint32_t r = side;
+        for (; r + 224u < rows; r += 256u)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sums[k] += from[(uint64_t)(r + 16u * k) * C + c];
-        for (; r < rows; r += 16u) sums[0] += from[(uint64_t)r * C + c];
+            for (int k = 0; k < 8; ++k) sums[k] += from[(uint64_t)(r + 32u * k) * C + c];
+        for (; r < rows; r += 32u) sums[0] += from[(uint64_t)r * C + c];
     }
-    parts[wave][lane] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    parts[side][lane] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
     __syncthreads();
-    if (wave != 0u || c >= C) return;
-    float total = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) total += parts[k][lane];
-    to[c] = total;
+    // a half wave to a column
+    float total = parts[lane][side];
+    total = lanes_allreduce(total, 32u, [](float a, float b) { return a + b; });
+    const uint32_t column = blockIdx.x % blocks * 32u + side;
+    if (lane == 0u && column < C) to[column] = total;
 }

@@ -16,6 +16,8 @@
 // states in the same order, whatever it finds published, so the results do not depend on the order in which blocks run.
 //   * The wait ends: tiles are numbered in the order in which their blocks start (a ticket), a tile looks at earlier ones only, and
 //     the first tile without a state finds its predecessor's. So the earliest one always gets on, and then the next.
+//   * Neighbouring strips go to one XCD (every eighth block draws from a line of tickets of its own): where rows are no multiple of 128
+//     bytes they share lines, which are then fetched once. (8 x 15933 .. see the figures below; nothing depends on where blocks run.)
 //   * A channel's word, 64 bits stored at once: H above, A below, with the lowest bit of A (a rounding of 2^-23 of A, for the tile's
 //     own use too) telling launches apart: its value alternates from launch to launch, and every launch writes every word. A state
 //     is marked by a NaN of its own in the place of A. No fence is needed, since a word holds all that is read, and nothing has to be
@@ -29,10 +31,10 @@
 
 struct RecurrenceParams {
     uint32_t first;                      // (bit 31: the result is stored past the caches)
-    uint32_t T, C, cstrips, strips, log2_w, reverse;
+    uint32_t T, C, cstrips, strips, tiles, lines, log2_w, reverse;
 };
 
-constexpr uint32_t THREADS = 256, WINDOW = 16, CHAIN_CHANNELS = 32;
+constexpr uint32_t THREADS = 256, WINDOW = 16, CHAIN_CHANNELS = 32, LINES = 8;
 constexpr uint32_t STATE_MARK = 0x7FC01230u, MAP_NAN = 0x7FE00000u;
 
 // sigmoid(gate) and 1 - sigmoid(gate), each rounded from the exponential: neither is the difference of the other to 1
@@ -79,27 +81,32 @@ struct Tile {
     bool back;                                   // the scan runs from the last time to the first
     unsigned long long* words;
 
-    __device__ Tile(const RecurrenceParams& P, const int32_t* lengths, unsigned long long* chain, bool back_) : T(P.T), C(P.C), strips(P.strips), back(back_) {
+    bool there;                                  // (a block beyond the last tile has none)
+
+    __device__ Tile(const RecurrenceParams& P, const int32_t* lengths, unsigned long long* chain, bool back_) : T(P.T), C(P.C), strips(P.strips), back(back_), there(true) {
         __shared__ unsigned long long ticket;
         W = 1u << P.log2_w; G = THREADS >> P.log2_w;
         col = threadIdx.x & (W - 1u); group = threadIdx.x >> P.log2_w;
-        uint32_t tile = blockIdx.x;
-        tag = 0; words = nullptr;
+        tag = 0; words = nullptr; k = 0;
+        strip = blockIdx.x;
         if constexpr (CHAIN) {
-            if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(chain, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const uint32_t line = P.lines == 1u ? 0u : blockIdx.x & (LINES - 1u), per = gridDim.x / P.lines;
+            const uint32_t s0 = P.strips * line / P.lines, mine = P.strips * (line + 1u) / P.lines - s0;
+            if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(chain + line * 8u, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             const unsigned long long t = ticket;
             const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)t), hi = __builtin_amdgcn_readfirstlane((uint32_t)(t >> 32));
-            const unsigned long long mine = (unsigned long long)hi << 32 | lo, launch = mine / gridDim.x;
-            tile = (uint32_t)(mine - launch * gridDim.x);
+            const unsigned long long number = (unsigned long long)hi << 32 | lo, launch = number / per;
+            const uint32_t tile = (uint32_t)(number - launch * per);
             tag = (uint32_t)(launch + 1ull) & 1u;                          // (the first launch's words are odd: memory starts as zeros)
-            words = chain + 8;                                             // behind the ticket's line
+            words = chain + LINES * 8u;                                    // behind the tickets, a line each
+            there = tile < mine * P.tiles;
+            k = tile / mine; strip = s0 + tile % mine;
         }
-        k = tile / P.strips; strip = tile % P.strips;
         b = strip / P.cstrips; c0 = (strip % P.cstrips) * W * VEC;
         n = min(G * L, T - k * (G * L));
         tlow = back ? T - k * (G * L) - n : k * (G * L);
-        length = length_of(lengths, b, T);
+        length = there ? length_of(lengths, b, T) : 0u;
     }
     __device__ uint32_t row(uint32_t i) const { const uint32_t s = group * L + i; return back ? n - 1u - s : s; }       // of step i, from tlow on
     __device__ bool valid(uint32_t i) const { return group * L + i < n && c0 + col * VEC < C; }
@@ -216,6 +223,7 @@ template <int VEC, int L, bool GATED, bool CHAIN>
 __device__ __forceinline__ void recurrence_body(float* h, float* last, const float* factor, const float* x, const float* state, const int32_t* lengths, unsigned long long* chain,
                                                 const RecurrenceParams& P) {
     Tile<VEC, L, CHAIN> tile(P, lengths, chain, P.reverse != 0u);
+    if (CHAIN && !tile.there) return;
     const __amdgpu_buffer_rsrc_t f_rsrc = tile.rsrc(factor), x_rsrc = tile.rsrc(x);
     float a[L][VEC], b[L][VEC], A[VEC], H[VEC], now[VEC];
 #pragma unroll
@@ -256,6 +264,7 @@ template <int VEC, int L, bool GATED, bool CHAIN>
 __device__ __forceinline__ void recurrence_grad_body(float* dfactor, float* dx, float* dstate, const float* h, const float* factor, const float* x, const float* state,
                                                      const int32_t* lengths, const float* g, const float* g_last, unsigned long long* chain, const RecurrenceParams& P) {
     Tile<VEC, L, CHAIN> tile(P, lengths, chain, P.reverse == 0u);
+    if (CHAIN && !tile.there) return;
     const __amdgpu_buffer_rsrc_t f_rsrc = tile.rsrc(factor), x_rsrc = tile.rsrc(GATED ? x : nullptr), g_rsrc = tile.rsrc(g), h_rsrc = tile.rsrc(h, P.reverse ? 1 : -1);
     float gs[L][VEC], a[L][VEC], before[L][VEC], rest[GATED ? L : 1][VEC], A[VEC], H[VEC], now[VEC];
     const uint32_t start = P.reverse ? P.T - 1u : 0u;                    // the time of the recurrence's first step

@@ -2184,12 +2184,13 @@ def _f32_word(value: float) -> int:
 
 
 #(threads, positions per thread) of the kernels whose samples stay in registers, by channels per lane
-NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 13)), 1: ((256, 4), (256, 16), (1024, 8))}
+NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 16)), 1: ((256, 4), (256, 16), (1024, 8))}
 NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 4)), 1: ((256, 4), (256, 16), (1024, 4))}
 #(threads, rows per thread) of the kernels for samples of one position
 NORM_ROWS      = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
 NORM_ROWS_GRAD = {4: ((256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
+NORM_PARTIAL_LINES = 128 << 20      #bytes up to which samples are held in registers by less than whole lines (25 MB 15.5 us, in chunks 23; 205 MB 95-111, 100)
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
 
@@ -2218,6 +2219,8 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
             for span in dict.fromkeys((lines, max(unit, lines // 2 // unit * unit), unit)):
                 V = span // vec
                 if V > threads or (span * 4 < 64 and span < c and n * _cdiv(c, span) > 64):
+                    continue
+                if span < min(NORM_FULL_LINE, c) and n * s * c * 4 > NORM_PARTIAL_LINES:
                     continue
                 side = threads // V
                 P    = min(side, _cdiv(s, k))
@@ -2300,6 +2303,11 @@ def _norm_shape(x: Buffer):
     return n, x.size // (n * c), c
 
 
+def _norm_whole_lines(plan: NormPlan, c: int) -> bool:
+    #(parts of lines that are stored past the caches are not put together there: 8 x 128 channels' gradients 207 us instead of 142)
+    return plan.span == c or (plan.span % NORM_FULL_LINE == 0 and c % NORM_FULL_LINE == 0)
+
+
 def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shift: Buffer, groups: int, eps: float, activation, scratch) -> tp.List[Launch]:
     shape = n, s, c = _norm_shape(x)
     plan  = norm_plan(n, s, c, groups, False)
@@ -2309,12 +2317,12 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
     if plan.kind != 'chunked':
         return [_norm_launch(f'group_norm_{plan.kind}_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
                              (2 if plan.kind == 'held' else 1) * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
-                             4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
+                             4 * (2 * x.size + 2 * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
     partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
     blocks  = n * plan.chunks * plan.spans
     return [_norm_launch(f'group_norm_stats_v{plan.vec}', blocks, *args, 2 * plan.P * plan.span, [(partial, 0), (x, 0)], 4 * x.size),
             _norm_launch(f'group_norm_apply_v{plan.vec}', blocks, *args, 2 * of_groups, [(b, 0) for b in (y, mean, rstd, partial, x, scale, shift)],
-                         4 * (2 * x.size + 2 * c), streamable=True, written=(0, 1, 2))]
+                         4 * (2 * x.size + 2 * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
 
 
 NORM_GRAD_ROWS = 1024               #blocks that the samples held in registers are shared out to, by the sums that each leaves
@@ -2335,7 +2343,7 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     if plan.kind != 'chunked':
         launches = [_norm_launch(f'group_norm_{plan.kind}_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
                                  2 * plan.M * plan.P * plan.span + (4 if plan.kind == 'rows' else 2) * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
-                                 4 * (3 * x.size + 2 * rows * c), streamable=True, written=(0, 1, 2))]
+                                 4 * (3 * x.size + 2 * rows * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
     else:
         partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
         blocks  = n * plan.chunks * plan.spans
@@ -2343,9 +2351,9 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
                                  [(partial, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest, 4 * (2 * x.size + 2 * rows * c), written=(0, 1, 2))]
         if dx is not None:
             launches.append(_norm_launch(f'group_norm_grad_apply_v{plan.vec}', blocks, *args, 2 * of_groups, [(dx, 0), (partial, 0)] + rest,
-                                         4 * 3 * x.size, streamable=True))
+                                         4 * 3 * x.size, streamable=_norm_whole_lines(plan, c)))
     if rows > 1 and (dscale is not None or dshift is not None):
-        launches.append(Launch('group_norm_columns', (2 * _cdiv(c, 64), 1, 1), (1024, 1, 1), [(b, 0) for b in (dscale, dshift, dscale_rows, dshift_rows)],
+        launches.append(Launch('group_norm_columns', (2 * _cdiv(c, 32), 1, 1), (1024, 1, 1), [(b, 0) for b in (dscale, dshift, dscale_rows, dshift_rows)],
                                _u32(rows, c), bytes_moved=4 * 2 * (rows + 1) * c, written=(0, 1)))
     return launches
 
@@ -2413,6 +2421,7 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
 # ---------------------------------------------------------------- linear recurrences (recurrence.hip)
 
 RECURRENCE_THREADS = 256
+RECURRENCE_LINES   = 8                  #lines of tickets: as many as XCDs
 #steps per thread of the kernels by channels per lane: for a single tile along time, and for several
 RECURRENCE_STEPS      = {4: ((1, 4, 8, 16), (8, 16)), 1: ((1, 4, 16), (16,))}
 RECURRENCE_GRAD_STEPS = {4: ((1, 3, 6, 8), (4, 6)), 1: ((1, 4, 8), (8,))}
@@ -2453,7 +2462,7 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays
             best = (cost, steps, lanes, tiles)
     _, steps, lanes, tiles = best
     cstrips = _cdiv(channels, lanes * vec)
-    if batch * cstrips * tiles * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
+    if (batch * cstrips + RECURRENCE_LINES) * tiles * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
         raise NotImplementedError(f'a recurrence over {channels} channels in {batch} sequences of {time} steps')
     return RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
 
@@ -2461,11 +2470,13 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays
 def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int) -> Launch:
     _, t, c = shape
     kernel  = f'{name}_v{tiling.vec}_l{tiling.steps}' + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
-    #(what tiles hand on: a line for the ticket, then a word of 64 bits per channel and tile)
-    chain   = None if tiling.tiles == 1 else zeroed(16 + 2 * tiling.tiles * tiling.strips * tiling.lanes * tiling.vec, f'{kernel} {tuple(tiling)}')
+    #(what tiles hand on: lines of 64 bytes for the tickets, then a word of 64 bits per channel and tile)
+    lines   = RECURRENCE_LINES if tiling.strips >= 2 * RECURRENCE_LINES else 1
+    blocks  = tiling.strips if tiling.tiles == 1 else lines * _cdiv(tiling.strips, lines) * tiling.tiles
+    chain   = None if tiling.tiles == 1 else zeroed(16 * RECURRENCE_LINES + 2 * tiling.tiles * tiling.strips * tiling.lanes * tiling.vec, f'{kernel} {tuple(tiling)}')
     buffers = [(v, 0) for v in arrays] + [(chain, 0)]
-    return Launch(kernel, (tiling.strips * tiling.tiles, 1, 1), (RECURRENCE_THREADS, 1, 1), buffers,
-                  _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=True,
+    return Launch(kernel, (blocks, 1, 1), (RECURRENCE_THREADS, 1, 1), buffers,
+                  _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.tiles, lines, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=c % 32 == 0,
                   written=written + ((len(arrays),) if chain is not None else ()), scratch=(len(arrays),) if chain is not None else ())
 
 

@@ -534,7 +534,7 @@ def group_norm(x, scale, shift, groups: int, eps: float = 1e-5, activation=None)
         raise ValueError(f'group_norm: {channels} channels do not fall into {groups} groups of equal size')
     if _shape(scale) != (channels,) or _shape(shift) != (channels,):
         raise TypeError(f'group_norm: scale and shift must have shape ({channels},), got {_shape(scale)} and {_shape(shift)}')
-    if not (0.0 < float(eps) < np.inf):
+    if not (0.0 < float(np.float32(eps)) < np.inf):
         raise ValueError(f'group_norm: eps must be positive and finite, got {eps}')
     if activation not in GROUP_NORM_ACTIVATIONS:
         raise ValueError(f'group_norm: activation must be one of {GROUP_NORM_ACTIVATIONS}, got {activation!r}')
