@@ -771,7 +771,8 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
     extern "C" __global__ __launch_bounds__(THREADS) void group_norm_rows_v##VEC##_k##K##_t##THREADS(float* y, float* means, float* rstds, const float* x,          \
                                                                                                      const float* scale, const float* shift, NormParams P) {        \
         rows_body<VEC, K>(y, means, rstds, x, scale, shift, P);                                                                                                     \
-    }                                                                                                                                                               \
+    }
+#define ROWS_GRAD(VEC, K, THREADS)                                                                                                                                  \
     extern "C" __global__ __launch_bounds__(THREADS) void group_norm_rows_grad_v##VEC##_k##K##_t##THREADS(float* dx, float* dscale_rows, float* dshift_rows,        \
             const float* g, const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                         \
         rows_grad_body<VEC, K>(dx, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                  \
@@ -792,7 +793,10 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
     }
 HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 4, 1024)  HELD(4, 16, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 8, 1024)
 HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 2, 1024)  HELD_GRAD(4, 4, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 4, 1024)
-ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)  ROWS(4, 8, 256)  ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)  ROWS(4, 1, 1024)  ROWS(1, 4, 1024) ROWS(4, 2, 1024) ROWS(1, 1, 1024)
+ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)  ROWS(4, 1, 1024)  ROWS(4, 2, 1024)
+ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)  ROWS(1, 1, 1024)  ROWS(1, 4, 1024)
+ROWS_GRAD(4, 1, 256)  ROWS_GRAD(4, 2, 256)  ROWS_GRAD(4, 1, 1024)  ROWS_GRAD(4, 2, 1024)
+ROWS_GRAD(1, 1, 256)  ROWS_GRAD(1, 4, 256)  ROWS_GRAD(1, 8, 256)  ROWS_GRAD(1, 1, 1024)  ROWS_GRAD(1, 4, 1024)
 CHUNKED(4)
 CHUNKED(1)
 
