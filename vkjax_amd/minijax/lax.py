@@ -618,7 +618,12 @@ def linear_recurrence(factor, x, state=None, lengths=None, reverse: bool = False
     None); `reverse`: from the last time to the first. `gated`: factor holds gates, h[:, t] = a h[:, t-1] + (1 - a) x[:, t] with
     a = sigmoid(factor[:, t]). `lengths` (int32 [batch], taken as between 0 and time): at times from a sequence's length on the
     state stays what it is, and what factor and x hold there is not looked at. Returns (h, the state behind the last step
-    [batch, channels]).'''
+    [batch, channels]).
+
+    Parts of a sequence run side by side, by products of their factors. Those of gates, and of factors between -1 and 1, only get
+    smaller, and h is that of step by step but for rounding. Factors beyond that are for sequences in which no product of
+    neighbouring ones passes float32's range (inf and NaN appear where step by step 0 times it would be 0), nor falls below it and is
+    brought back by larger ones (what came before is lost then).'''
     operands, xs = _recurrence_operands('gated_recurrence' if gated else 'linear_recurrence', factor, x, state, lengths)
     return tuple(emit('linear_recurrence', operands, [_aval(xs, _f32), _aval((xs[0], xs[2]), _f32)],
                 dict(gated=bool(gated), reverse=bool(reverse), has_state=state is not None, has_lengths=lengths is not None),
