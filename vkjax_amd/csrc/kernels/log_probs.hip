@@ -29,6 +29,7 @@ struct LogProbsParams {
 
 constexpr uint32_t NOWHERE = 0x80000000u;
 constexpr uint32_t LIST = 128;
+constexpr uint64_t NO_ENTRY = ~0ull;             // (a token beyond every row's)
 constexpr int NV = 4;                            // vectors per lane at a time
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
@@ -54,10 +55,17 @@ struct Sums {
         s = lanes_allreduce(s, lanes, [](float a, float b) { return a + b; });
         w = lanes_allreduce(w, lanes, [](float a, float b) { return a + b; });
     }
-    __device__ __forceinline__ bool nothing() const { return s == 0.f; }
-    __device__ __forceinline__ float log_sum() const { return nothing() ? -INFINITY : m + logf(s); }
-    __device__ __forceinline__ float entropy() const { return nothing() ? 0.f : logf(s) - w / s; }
-    __device__ __forceinline__ float log_prob(float x) const { return nothing() ? -INFINITY : (x - m) - logf(s); }
+};
+// What a row's sums say. (The logarithm once: it is as many instructions as ten scores.)
+struct Distribution {
+    float m, log_s, entropy;
+    bool nothing;
+    __device__ __forceinline__ explicit Distribution(const Sums& sums) : m(sums.m), nothing(sums.s == 0.f) {
+        log_s = logf(sums.s);
+        entropy = nothing ? 0.f : log_s - sums.w / sums.s;
+    }
+    __device__ __forceinline__ float log_sum() const { return nothing ? -INFINITY : m + log_s; }
+    __device__ __forceinline__ float log_prob(float x) const { return nothing ? -INFINITY : (x - m) - log_s; }
 };
 
 // Larger for larger scores, NaN above all; -0 and 0 are equal. Neither 0 nor all ones.
@@ -76,9 +84,21 @@ __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_A
 __device__ __forceinline__ uint64_t of_lane(uint64_t v, uint32_t lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, (int)lane);
 }
-// How many of the first `count` lanes' keys are larger than this lane's `mine`.
+// How many of the first `count` lanes' keys are larger than this lane's `mine`: by their scores alone unless some are equal.
 __device__ __forceinline__ uint32_t place_of(uint64_t key, uint64_t mine, uint32_t count) {
+    const uint32_t high = (uint32_t)(key >> 32), own = (uint32_t)(mine >> 32);
     uint32_t place = 0;
+    uint64_t equal = 0;                                                   // lanes that meet their own score, which is no other key's if it is the same one
+#pragma unroll 4
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)high, (int)i);
+        place += other > own;
+        const uint64_t same = __builtin_amdgcn_ballot_w64(other == own);
+        equal |= same & ~(1ull << i);
+    }
+    // (where `mine` is of other keys than `key`, a lane's own number means nothing: its equals are looked for as well)
+    if ((equal | __builtin_amdgcn_ballot_w64(key != mine && high == own)) == 0ull) return place;
+    place = 0;
 #pragma unroll 4
     for (uint32_t i = 0; i < count; ++i) place += of_lane(key, i) > mine;
     return place;
@@ -140,9 +160,13 @@ struct Chunk {
     __device__ __forceinline__ bool valid(int i, int j) const { return token(i, j) < end; }      // (tokens before the row: far above it)
 };
 
+// A score with its token, as it goes into a list: becoming a key is left to the one lane that sorts it in.
+__device__ __forceinline__ uint64_t entry_of(float x, uint32_t token) { return (uint64_t)f2u(x) << 32 | token; }
+__device__ __forceinline__ uint64_t key_of(uint64_t entry) { return place_key(u2f((uint32_t)(entry >> 32)), (uint32_t)entry); }
+
 // The list of a wave's candidates in shared memory.
 struct Candidates {
-    uint64_t* keys;                              // LIST of them
+    uint64_t* entries;                           // LIST of them
     uint32_t count, top;
     float bar;                                   // at least `top` scores have been no smaller: later ones count where they are larger
 
@@ -150,15 +174,16 @@ struct Candidates {
     __device__ __forceinline__ void cut() {
         wave_fence();
         const uint32_t lane = __lane_id(), first = min(count, 64u), second = count - first;
-        const uint64_t a = lane < count ? keys[lane] : 0ull, b = lane + 64u < count ? keys[lane + 64u] : 0ull;
+        const uint64_t own_a = lane < count ? entries[lane] : 0ull, own_b = lane + 64u < count ? entries[lane + 64u] : 0ull;
+        const uint64_t a = lane < count ? key_of(own_a) : 0ull, b = lane + 64u < count ? key_of(own_b) : 0ull;
         uint32_t place_a = place_of(a, a, first), place_b = 0u;
         if (second != 0u) { place_a += place_of(b, a, second); place_b = place_of(a, b, first) + place_of(b, b, second); }
         wave_fence();
-        if (lane < count && place_a < top) keys[place_a] = a;
-        if (lane + 64u < count && place_b < top) keys[place_b] = b;
+        if (lane < count && place_a < top) entries[place_a] = own_a;
+        if (lane + 64u < count && place_b < top) entries[place_b] = own_b;
         wave_fence();
         count = min(count, top);
-        bar = key_score((uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(keys[count - 1u] >> 32)));
+        bar = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(entries[count - 1u] >> 32)));
     }
     // Takes from a chunk, whose tokens are behind those of the chunks before, what may be among the largest. `best`: the largest number of each of the lane's
     // vectors, `most` of all; `broken`: the lane has met a NaN, which does not show among the maxima but passes the comparisons that are made here.
@@ -178,9 +203,9 @@ struct Candidates {
             for (int j = 0; j < 4; ++j) {
                 const uint64_t mask = __builtin_amdgcn_ballot_w64(!(v[i][j] <= from));
                 if (mask != 0ull) {
-                    const uint32_t to = n + lanes_below(mask);
-                    if (!(v[i][j] <= from) && to < LIST) keys[to] = place_key(v[i][j], chunk.token(i, j));
-                    n += (uint32_t)__popcll(mask);
+                    const uint32_t more = (uint32_t)__popcll(mask);
+                    if (n + more <= LIST && !(v[i][j] <= from)) entries[n + lanes_below(mask)] = entry_of(v[i][j], chunk.token(i, j));
+                    n += more;
                 }
             }
         }
@@ -200,7 +225,7 @@ struct Candidates {
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (is[j] && before < need) keys[count + before] = place_key(-INFINITY, chunk.token(i, j));
+                    if (is[j] && before < need) entries[count + before] = entry_of(-INFINITY, chunk.token(i, j));
                     before += is[j];
                 }
                 const uint32_t taken = min(all, need);
@@ -214,7 +239,7 @@ struct Candidates {
     __device__ __forceinline__ void one_by_one(const Chunk& chunk) {
         const uint32_t lane = __lane_id();
         wave_fence();
-        const uint64_t a = lane < count ? keys[lane] : 0ull, b = lane + 64u < count ? keys[lane + 64u] : 0ull;
+        const uint64_t a = lane < count ? key_of(entries[lane]) : 0ull, b = lane + 64u < count ? key_of(entries[lane + 64u]) : 0ull;
         uint64_t below = ~0ull;
         uint32_t n = 0;
 #pragma nounroll
@@ -231,7 +256,7 @@ struct Candidates {
             if (best == 0ull) break;
             below = best;
             wave_fence();
-            if (lane == 0u) keys[n] = best;
+            if (lane == 0u) entries[n] = entry_of(key_score((uint32_t)(best >> 32)), place_token(best));
         }
         wave_fence();
         count = n;
@@ -252,13 +277,13 @@ __device__ __forceinline__ void write_padding(const Results& to, uint64_t row, u
         if (to.top_token) to.top_token[row * top + k] = -1;
     }
 }
-__device__ __forceinline__ void write_sums(const Results& to, uint64_t row, const Sums& sums, float score) {
-    if (to.log_prob) to.log_prob[row] = sums.log_prob(score);
-    if (to.entropy) to.entropy[row] = sums.entropy();
-    if (to.log_sum) to.log_sum[row] = sums.log_sum();
+__device__ __forceinline__ void write_sums(const Results& to, uint64_t row, const Distribution& p, float score) {
+    if (to.log_prob) to.log_prob[row] = p.log_prob(score);
+    if (to.entropy) to.entropy[row] = p.entropy;
+    if (to.log_sum) to.log_sum[row] = p.log_sum();
 }
-__device__ __forceinline__ void write_alternative(const Results& to, uint64_t row, uint32_t top, uint32_t place, uint64_t key, const Sums& sums) {
-    if (to.top_log_prob) to.top_log_prob[row * top + place] = sums.log_prob(key_score((uint32_t)(key >> 32)));
+__device__ __forceinline__ void write_alternative(const Results& to, uint64_t row, uint32_t top, uint32_t place, uint64_t key, const Distribution& p) {
+    if (to.top_log_prob) to.top_log_prob[row * top + place] = p.log_prob(key_score((uint32_t)(key >> 32)));
     if (to.top_token) to.top_token[row * top + place] = (int32_t)place_token(key);
 }
 
@@ -347,10 +372,14 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
         if (P.top != 0u) found.take(v, best, most, broken, chunk);
     });
     sums.join_lanes(64u);
-    if (lane == 0u) write_sums(to, row, sums, score);
+    const Distribution p(sums);
+    if (lane == 0u) write_sums(to, row, p, score);
     if (P.top == 0u) return;
+    if (found.count > 64u) found.cut();
     wave_fence();
-    rank(found.keys, found.count, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
+    const uint64_t key = lane < found.count ? key_of(found.entries[lane]) : 0ull;
+    const uint32_t place = place_of(key, key, found.count);
+    if (lane < found.count && place < P.top) write_alternative(to, row, P.top, place, key, p);
 }
 #define LOG_PROBS_WAVE(name, SINGLE)                                                                                                                     \
     extern "C" __global__ __launch_bounds__(256) void name(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,    \
@@ -388,23 +417,27 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
     if (P.top != 0u) {
         // the wave's largest, in order, and zeros where there are not as many
         if (found.count != 0u) found.cut();
-        if (lane >= found.count && lane < P.top) found.keys[lane] = 0ull;
+        if (lane >= found.count && lane < P.top) found.entries[lane] = NO_ENTRY;
     }
     __syncthreads();
     if (wave != 0u) return;
     sums = of_wave[lane & (WAVES - 1)];
     sums.join_lanes(WAVES);
+    const Distribution p(sums);
     if (P.slices == 1u) {
-        if (lane == 0u) write_sums(to, row, sums, score);
+        if (lane == 0u) write_sums(to, row, p, score);
     } else if (lane < 3u) parts[(row * P.slices + slice) * 4u + lane] = lane == 0u ? sums.m : lane == 1u ? sums.s : sums.w;
     if (P.top == 0u) return;
     // place by place, so that every lane sees high places, and the bar over the lanes' largest is near
-    for (uint32_t e = lane; e < WAVES * P.top; e += 64u) all[e] = lists[(e & (WAVES - 1u)) * LIST + e / WAVES];
+    for (uint32_t e = lane; e < WAVES * P.top; e += 64u) {
+        const uint64_t entry = lists[(e & (WAVES - 1u)) * LIST + e / WAVES];
+        all[e] = entry == NO_ENTRY ? 0ull : key_of(entry);
+    }
     wave_fence();
     uint64_t* const out = keys + row * P.slices * P.top + slice;          // (also place by place)
     if (P.slices != 1u && lane < P.top) out[lane * P.slices] = 0ull;      // (a slice may have fewer scores)
     best_keys<2>(all, WAVES * P.top, lists, P.top, [&](uint32_t place, uint64_t key) {
-        if (P.slices == 1u) write_alternative(to, row, P.top, place, key, sums);
+        if (P.slices == 1u) write_alternative(to, row, P.top, place, key, p);
         else out[place * P.slices] = key;
     });
 }
@@ -425,10 +458,11 @@ extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob,
         sums.join(Sums{part[0], part[1], part[2]});
     }
     sums.join_lanes(64u);
-    if (lane == 0u) write_sums(to, row, sums, score);
+    const Distribution p(sums);
+    if (lane == 0u) write_sums(to, row, p, score);
     if (P.top == 0u) return;
     const uint32_t count = P.slices * P.top;
-    best_keys<16>(keys + row * count, count, room, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, sums); });
+    best_keys<16>(keys + row * count, count, room, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, p); });
 }
 
 // Short rows: 2^log2_lanes lanes to a row, four vectors to a lane, and several rows to a wave. The alternatives one by one.
@@ -470,7 +504,8 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_pro
         for (int j = 0; j < 4; ++j) sums.add(v[i][j]);
     sums.join_lanes(lanes);
     if (there && !given) write_padding(to, row, lane, lanes, P.top);
-    if (given && lane == 0u) write_sums(to, row, sums, score);
+    const Distribution p(sums);
+    if (given && lane == 0u) write_sums(to, row, p, score);
     if (P.top == 0u) return;
     // A place's key is the score's; which of the equal ones it is, the number of the first one behind the last place tells.
     uint32_t keys[NV][4];
@@ -494,7 +529,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_pro
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) keys[i][j] = at(i, j) == number ? 0u : keys[i][j];
-        if (given && lane == (k & (lanes - 1u))) write_alternative(to, row, P.top, k, (uint64_t)key << 32 | (0xFFFFFFFFu - number), sums);
+        if (given && lane == (k & (lanes - 1u))) write_alternative(to, row, P.top, k, (uint64_t)key << 32 | (0xFFFFFFFFu - number), p);
     }
 }
 
