@@ -2361,7 +2361,8 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 # ---------------------------------------------------------------- log probabilities of tokens (log_probs.hip)
 
 LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
-LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane
+LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane. With many alternatives half as many:
+LOG_PROBS_MANY      = 5             #(65536 rows of 500 and top of 1, 5, 20: 32, 53, 132 us, a wave to a row 43, 50, 70; rows of 250: 17, 27, 66, and 42, 49, 75)
 LOG_PROBS_WAVE      = 1024          #rows of up to this many vectors have a wave each where there are enough of them, longer ones a block
 LOG_PROBS_ROWS      = 1024          #enough rows not to be cut
 LOG_PROBS_MAX_KEYS  = 1024          #candidates of all slices of a row
@@ -2377,7 +2378,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     if v >= 2**29 or rows * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4)
-    if vectors <= LOG_PROBS_SHORT:
+    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2):
         lanes = _pow2_at_least(_cdiv(vectors, 4))
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
