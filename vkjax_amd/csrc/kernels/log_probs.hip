@@ -84,38 +84,57 @@ __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_A
 __device__ __forceinline__ uint64_t of_lane(uint64_t v, uint32_t lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, (int)lane);
 }
-// How many of the first `count` lanes' keys are larger than this lane's `mine`: by their scores alone unless some are equal.
-__device__ __forceinline__ uint32_t place_of(uint64_t key, uint64_t mine, uint32_t count) {
-    const uint32_t high = (uint32_t)(key >> 32), own = (uint32_t)(mine >> 32);
-    uint32_t place = 0;
-    uint64_t equal = 0;                                                   // lanes that meet their own score, which is no other key's if it is the same one
-#pragma unroll 4
-    for (uint32_t i = 0; i < count; ++i) {
-        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)high, (int)i);
-        place += other > own;
-        const uint64_t same = __builtin_amdgcn_ballot_w64(other == own);
-        equal |= same & ~(1ull << i);
+// The places of `count` keys, of which a lane has numbers lane, lane + 64 .. (zeros beyond): how many others are larger, by the scores alone, four from shared memory
+// at a time, unless some of these are equal; then places are no permutation, which their sum tells. `scores`: 64 N words of shared memory.
+template <int N>
+__device__ __forceinline__ void places_of(const uint64_t (&keys)[N], uint32_t count, uint32_t* scores, uint32_t (&places)[N]) {
+    const uint32_t lane = __lane_id();
+    uint32_t sum = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) { scores[k * 64 + lane] = (uint32_t)(keys[k] >> 32); places[k] = 0u; }
+    wave_fence();
+    for (uint32_t at = 0; at < count; at += 4u) {
+        const u32x4 others = *reinterpret_cast<const u32x4*>(scores + at);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t own = (uint32_t)(keys[k] >> 32);
+            places[k] += others.x > own; places[k] += others.y > own; places[k] += others.z > own; places[k] += others.w > own;
+        }
     }
-    // (where `mine` is of other keys than `key`, a lane's own number means nothing: its equals are looked for as well)
-    if ((equal | __builtin_amdgcn_ballot_w64(key != mine && high == own)) == 0ull) return place;
-    place = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < count; ++i) place += of_lane(key, i) > mine;
-    return place;
+    wave_fence();
+#pragma unroll
+    for (int k = 0; k < N; ++k) sum += keys[k] != 0ull ? places[k] : 0u;
+    if (lanes_allreduce(sum, 64u, [](uint32_t a, uint32_t b) { return a + b; }) == count * (count - 1u) / 2u) return;
+#pragma unroll
+    for (int k = 0; k < N; ++k) places[k] = 0u;
+#pragma unroll
+    for (int m = 0; m < N; ++m)
+#pragma nounroll
+        for (uint32_t i = 0; i < 64u && m * 64u + i < count; ++i) {
+            const uint64_t other = of_lane(keys[m], i);
+#pragma unroll
+            for (int k = 0; k < N; ++k) places[k] += other > keys[k];
+        }
 }
-// put(place, key) for the `top` largest of `count` keys in shared memory, each lane having keys lane, lane + 64 ..: as many are larger as its place says.
+// put(place, key) for the `top` largest of `count` keys in shared memory, which is written over (256 bytes of it at least).
 template <class Put>
-__device__ __forceinline__ void rank(const uint64_t* keys, uint32_t count, uint32_t top, Put put) {
-    for (uint32_t at = 0; at < count; at += 64u) {
-        const uint32_t mine = at + __lane_id();
-        const uint64_t key = mine < count ? keys[mine] : 0ull;
-        uint32_t place = 0;
-        if (count <= 64u) place = place_of(key, key, count);
-        else
+__device__ __forceinline__ void rank(uint64_t* keys, uint32_t count, uint32_t top, Put put) {
+    const uint32_t lane = __lane_id();
+    if (count <= 64u) {
+        const uint64_t mine[1] = {lane < count ? keys[lane] : 0ull};
+        uint32_t place[1];
+        wave_fence();
+        places_of<1>(mine, count, reinterpret_cast<uint32_t*>(keys), place);
+        if (lane < count && place[0] < top) put(place[0], mine[0]);
+    } else
+        for (uint32_t at = 0; at < count; at += 64u) {
+            const uint32_t mine = at + lane;
+            const uint64_t key = mine < count ? keys[mine] : 0ull;
+            uint32_t place = 0;
 #pragma unroll 4
             for (uint32_t i = 0; i < count; ++i) place += keys[i] > key;
-        if (mine < count && place < top) put(place, key);
-    }
+            if (mine < count && place < top) put(place, key);
+        }
 }
 
 // A value that at least k (up to 32) of the lanes' values reach, and not many more: of 2^n >= k groups of lanes the smallest maximum, raised by bisection.
@@ -173,12 +192,22 @@ struct Candidates {
     // cuts the list to the `top` largest, in order
     __device__ __forceinline__ void cut() {
         wave_fence();
-        const uint32_t lane = __lane_id(), first = min(count, 64u), second = count - first;
+        const uint32_t lane = __lane_id();
         const uint64_t own_a = lane < count ? entries[lane] : 0ull, own_b = lane + 64u < count ? entries[lane + 64u] : 0ull;
         const uint64_t a = lane < count ? key_of(own_a) : 0ull, b = lane + 64u < count ? key_of(own_b) : 0ull;
-        uint32_t place_a = place_of(a, a, first), place_b = 0u;
-        if (second != 0u) { place_a += place_of(b, a, second); place_b = place_of(a, b, first) + place_of(b, b, second); }
+        uint32_t place_a, place_b = 0u;
         wave_fence();
+        if (count <= 64u) {
+            const uint64_t keys[1] = {a};
+            uint32_t places[1];
+            places_of<1>(keys, count, reinterpret_cast<uint32_t*>(entries), places);
+            place_a = places[0];
+        } else {
+            const uint64_t keys[2] = {a, b};
+            uint32_t places[2];
+            places_of<2>(keys, count, reinterpret_cast<uint32_t*>(entries), places);
+            place_a = places[0]; place_b = places[1];
+        }
         if (lane < count && place_a < top) entries[place_a] = own_a;
         if (lane + 64u < count && place_b < top) entries[place_b] = own_b;
         wave_fence();
@@ -358,7 +387,7 @@ __device__ __forceinline__ void best_keys(const uint64_t* keys, uint32_t count, 
 // A row to a wave.
 template <bool SINGLE>
 __device__ __forceinline__ void wave_body(const Results& to, const float* logits, const uint32_t* tokens, const LogProbsParams& P) {
-    __shared__ uint64_t lists[4][LIST];
+    __shared__ __attribute__((aligned(16))) uint64_t lists[4][LIST];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint64_t row = (uint64_t)blockIdx.x * 4u + wave;
     if (row >= P.rows) return;
@@ -377,9 +406,11 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
     if (P.top == 0u) return;
     if (found.count > 64u) found.cut();
     wave_fence();
-    const uint64_t key = lane < found.count ? key_of(found.entries[lane]) : 0ull;
-    const uint32_t place = place_of(key, key, found.count);
-    if (lane < found.count && place < P.top) write_alternative(to, row, P.top, place, key, p);
+    const uint64_t key[1] = {lane < found.count ? key_of(found.entries[lane]) : 0ull};
+    uint32_t place[1];
+    wave_fence();
+    places_of<1>(key, found.count, reinterpret_cast<uint32_t*>(found.entries), place);
+    if (lane < found.count && place[0] < P.top) write_alternative(to, row, P.top, place[0], key[0], p);
 }
 #define LOG_PROBS_WAVE(name, SINGLE)                                                                                                                     \
     extern "C" __global__ __launch_bounds__(256) void name(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,    \
@@ -395,7 +426,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
                                                                      const float* logits, const uint32_t* tokens, LogProbsParams P) {
     constexpr uint32_t WAVES = 4;
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
-    __shared__ uint64_t lists[WAVES * LIST];
+    __shared__ __attribute__((aligned(16))) uint64_t lists[WAVES * LIST];
     __shared__ uint64_t all[WAVES * 32];
     __shared__ Sums of_wave[WAVES];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, slice = blockIdx.x % P.slices;
@@ -445,7 +476,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
 // Joins the slices of a row: a wave to a row.
 extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, const float* parts,
                                                                 const uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
-    extern __shared__ uint64_t room[];                                    // slices * top of them
+    extern __shared__ __attribute__((aligned(16))) uint64_t room[];       // slices * top of them, and no less than 32 (256 bytes)
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
     const uint32_t lane = threadIdx.x;
     const uint64_t row = blockIdx.x;

@@ -2397,7 +2397,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
                     written=written if slices == 1 else (5, 6))
     if slices == 1:
         return [launch]
-    return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, lds=8 * slices * top,
+    return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, lds=max(8 * slices * top, BLOCK if top else 0),
                            bytes_moved=4 * rows * (4 + 2 * top + slices * (4 + 2 * top)), written=written)]
 
 
