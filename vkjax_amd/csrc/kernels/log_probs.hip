@@ -29,7 +29,6 @@ struct LogProbsParams {
 
 constexpr uint32_t NOWHERE = 0x80000000u;
 constexpr uint32_t LIST = 128;
-constexpr uint64_t NO_ENTRY = ~0ull;             // (a token beyond every row's)
 constexpr int NV = 4;                            // vectors per lane at a time
 constexpr float LOWEST = -3.402823466e38f, LOG2E = 1.4426950408889634f;
 
@@ -84,16 +83,17 @@ __device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_A
 __device__ __forceinline__ uint64_t of_lane(uint64_t v, uint32_t lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, (int)lane);
 }
-// The places of `count` keys, of which a lane has numbers lane, lane + 64 .. (zeros beyond): how many others are larger, by the scores alone, four from shared memory
-// at a time, unless some of these are equal; then places are no permutation, which their sum tells. `scores`: 64 N words of shared memory.
+// The places of keys, of which a lane has numbers lane, lane + 64 .., `count` of them among the first `end` numbers (the others are zeros): how many are larger, by
+// the scores alone, four from shared memory at a time, unless some of these are equal; then places are no permutation, which their sum tells. `scores`: 64 N words
+// of shared memory.
 template <int N>
-__device__ __forceinline__ void places_of(const uint64_t (&keys)[N], uint32_t count, uint32_t* scores, uint32_t (&places)[N]) {
+__device__ __forceinline__ void places_of(const uint64_t (&keys)[N], uint32_t end, uint32_t count, uint32_t* scores, uint32_t (&places)[N]) {
     const uint32_t lane = __lane_id();
     uint32_t sum = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) { scores[k * 64 + lane] = (uint32_t)(keys[k] >> 32); places[k] = 0u; }
     wave_fence();
-    for (uint32_t at = 0; at < count; at += 4u) {
+    for (uint32_t at = 0; at < end; at += 4u) {
         const u32x4 others = *reinterpret_cast<const u32x4*>(scores + at);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -110,7 +110,7 @@ __device__ __forceinline__ void places_of(const uint64_t (&keys)[N], uint32_t co
 #pragma unroll
     for (int m = 0; m < N; ++m)
 #pragma nounroll
-        for (uint32_t i = 0; i < 64u && m * 64u + i < count; ++i) {
+        for (uint32_t i = 0; i < 64u && m * 64u + i < end; ++i) {
             const uint64_t other = of_lane(keys[m], i);
 #pragma unroll
             for (int k = 0; k < N; ++k) places[k] += other > keys[k];
@@ -124,7 +124,7 @@ __device__ __forceinline__ void rank(uint64_t* keys, uint32_t count, uint32_t to
         const uint64_t mine[1] = {lane < count ? keys[lane] : 0ull};
         uint32_t place[1];
         wave_fence();
-        places_of<1>(mine, count, reinterpret_cast<uint32_t*>(keys), place);
+        places_of<1>(mine, count, count, reinterpret_cast<uint32_t*>(keys), place);
         if (lane < count && place[0] < top) put(place[0], mine[0]);
     } else
         for (uint32_t at = 0; at < count; at += 64u) {
@@ -200,12 +200,12 @@ struct Candidates {
         if (count <= 64u) {
             const uint64_t keys[1] = {a};
             uint32_t places[1];
-            places_of<1>(keys, count, reinterpret_cast<uint32_t*>(entries), places);
+            places_of<1>(keys, count, count, reinterpret_cast<uint32_t*>(entries), places);
             place_a = places[0];
         } else {
             const uint64_t keys[2] = {a, b};
             uint32_t places[2];
-            places_of<2>(keys, count, reinterpret_cast<uint32_t*>(entries), places);
+            places_of<2>(keys, count, count, reinterpret_cast<uint32_t*>(entries), places);
             place_a = places[0]; place_b = places[1];
         }
         if (lane < count && place_a < top) entries[place_a] = own_a;
@@ -316,27 +316,32 @@ __device__ __forceinline__ void write_alternative(const Results& to, uint64_t ro
     if (to.top_token) to.top_token[row * top + place] = (int32_t)place_token(key);
 }
 
-// A wave's part of a row: vectors [q0, q1) of it, a vector being 16 aligned bytes. SINGLE: no more than the wave takes at a time.
-template <bool SINGLE, class Take>
-__device__ __forceinline__ void read_row(const float* logits, uint64_t row, uint32_t V, uint32_t q0, uint32_t q1, Sums& sums, Take take) {
-    const uint64_t start = row * V;
-    const uint32_t lead = (uint32_t)start & 3u, lane = __lane_id();       // scores of other rows in the first vector
-    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(logits + (start - lead), (lead + V) * 4u);
-    f32x4 next[NV];
-    auto fetch = [&](uint32_t q) {
+// A row in vectors of 16 aligned bytes.
+struct Row {
+    const float* x;
+    uint32_t lead, V;                            // scores of other rows in the first vector; its own
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ Row(const float* logits, uint64_t row, uint32_t V) : x(logits + row * V), lead((uint32_t)(row * V) & 3u), V(V) { rsrc = make_rsrc(x - lead, (lead + V) * 4u); }
+    __device__ __forceinline__ uint32_t vectors() const { return (lead + V + 3u) >> 2; }
+    // vectors q + 64 i + lane, those below q1
+    __device__ __forceinline__ void fetch(f32x4 (&to)[NV], uint32_t q, uint32_t q1) const {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t at = q + i * 64u + lane;
-            next[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at < q1 ? at * 16u : NOWHERE, 0, 0));
+            const uint32_t at = q + i * 64u + __lane_id();
+            to[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at < q1 ? at * 16u : NOWHERE, 0, 0));
         }
-    };
-    fetch(q0);
+    }
+};
+
+// A wave's part of a row: vectors [q0, q1) of it, the first of which are in `next`. SINGLE: no more than the wave takes at a time.
+template <bool SINGLE, class Take>
+__device__ __forceinline__ void read_row(const Row& row, uint32_t q0, uint32_t q1, f32x4 (&next)[NV], Sums& sums, Take take) {
     for (uint32_t q = q0; q < q1; q += NV * 64u) {
         float v[NV][4];
 #pragma unroll
         for (int i = 0; i < NV; ++i) { v[i][0] = next[i].x; v[i][1] = next[i].y; v[i][2] = next[i].z; v[i][3] = next[i].w; }
-        if (!SINGLE && q + NV * 64u < q1) fetch(q + NV * 64u);
-        const Chunk chunk{logits + start, (q + lane) * 4u - lead, min(q1 * 4u - lead, V)};
+        if (!SINGLE && q + NV * 64u < q1) row.fetch(next, q + NV * 64u, q1);
+        const Chunk chunk{row.x, (q + __lane_id()) * 4u - row.lead, min(q1 * 4u - row.lead, row.V)};
         if (SINGLE || q == 0u || q + NV * 64u >= q1)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -393,11 +398,13 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
     if (row >= P.rows) return;
     const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
     if (token >= P.V) { write_padding(to, row, lane, 64u, P.top); return; }
-    const float score = logits[row * P.V + token];
+    const Row from(logits, row, P.V);
+    const float score = from.x[token];
     Sums sums; sums.start();
     Candidates found{lists[wave], 0u, P.top, 0.f};
-    const uint32_t vectors = ((uint32_t)(row * P.V) & 3u) + P.V + 3u >> 2;
-    read_row<SINGLE>(logits, row, P.V, 0u, vectors, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
+    f32x4 next[NV];
+    from.fetch(next, 0u, from.vectors());
+    read_row<SINGLE>(from, 0u, from.vectors(), next, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
         if (P.top != 0u) found.take(v, best, most, broken, chunk);
     });
     sums.join_lanes(64u);
@@ -409,7 +416,7 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
     const uint64_t key[1] = {lane < found.count ? key_of(found.entries[lane]) : 0ull};
     uint32_t place[1];
     wave_fence();
-    places_of<1>(key, found.count, reinterpret_cast<uint32_t*>(found.entries), place);
+    places_of<1>(key, found.count, found.count, reinterpret_cast<uint32_t*>(found.entries), place);
     if (lane < found.count && place[0] < P.top) write_alternative(to, row, P.top, place[0], key[0], p);
 }
 #define LOG_PROBS_WAVE(name, SINGLE)                                                                                                                     \
@@ -431,24 +438,29 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
     __shared__ Sums of_wave[WAVES];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, slice = blockIdx.x % P.slices;
     const uint64_t row = blockIdx.x / P.slices;
+    const Row from(logits, row, P.V);
+    const uint32_t q0 = min((slice * WAVES + wave) * P.slice, from.vectors()), q1 = min(q0 + P.slice, from.vectors());
+    f32x4 next[NV];
+    if (P.slices != 1u) from.fetch(next, q0, q1);                         // (few rows: one round trip to memory less to wait for, and little read in vain for padding)
     const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
     if (token >= P.V) {
         if (P.slices == 1u && wave == 0u) write_padding(to, row, lane, 64u, P.top);
         return;                                                           // (the whole block)
     }
-    const float score = logits[row * P.V + token];
-    const uint32_t vectors = ((uint32_t)(row * P.V) & 3u) + P.V + 3u >> 2, q0 = min((slice * WAVES + wave) * P.slice, vectors), q1 = min(q0 + P.slice, vectors);
+    const float score = from.x[token];
+    if (P.slices == 1u) from.fetch(next, q0, q1);
     Sums sums; sums.start();
     Candidates found{lists + wave * LIST, 0u, P.top, 0.f};
-    if (q0 < q1) read_row<false>(logits, row, P.V, q0, q1, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
+    if (q0 < q1) read_row<false>(from, q0, q1, next, sums, [&](const float (&v)[NV][4], const float (&best)[NV], float most, bool broken, const Chunk& chunk) {
         if (P.top != 0u) found.take(v, best, most, broken, chunk);
     });
     sums.join_lanes(64u);
     if (lane == 0u) of_wave[wave] = sums;
+    const uint32_t share = P.top <= 12u ? 16u : 32u;                      // keys that a wave may leave, in any order
     if (P.top != 0u) {
-        // the wave's largest, in order, and zeros where there are not as many
-        if (found.count != 0u) found.cut();
-        if (lane >= found.count && lane < P.top) found.entries[lane] = NO_ENTRY;
+        if (found.count > share) found.cut();
+        wave_fence();
+        if (lane < share) all[wave * share + lane] = lane < found.count ? key_of(found.entries[lane]) : 0ull;
     }
     __syncthreads();
     if (wave != 0u) return;
@@ -459,18 +471,28 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
         if (lane == 0u) write_sums(to, row, p, score);
     } else if (lane < 3u) parts[(row * P.slices + slice) * 4u + lane] = lane == 0u ? sums.m : lane == 1u ? sums.s : sums.w;
     if (P.top == 0u) return;
-    // place by place, so that every lane sees high places, and the bar over the lanes' largest is near
-    for (uint32_t e = lane; e < WAVES * P.top; e += 64u) {
-        const uint64_t entry = lists[(e & (WAVES - 1u)) * LIST + e / WAVES];
-        all[e] = entry == NO_ENTRY ? 0ull : key_of(entry);
-    }
-    wave_fence();
-    uint64_t* const out = keys + row * P.slices * P.top + slice;          // (also place by place)
-    if (P.slices != 1u && lane < P.top) out[lane * P.slices] = 0ull;      // (a slice may have fewer scores)
-    best_keys<2>(all, WAVES * P.top, lists, P.top, [&](uint32_t place, uint64_t key) {
+    uint64_t* const out = keys + row * P.slices * P.top + slice;
+    uint32_t* const scores = reinterpret_cast<uint32_t*>(lists);
+    auto keep = [&](uint32_t place, uint64_t key) {
+        if (key == 0ull || place >= P.top) return;
         if (P.slices == 1u) write_alternative(to, row, P.top, place, key, p);
         else out[place * P.slices] = key;
-    });
+    };
+    uint32_t count;
+    if (share == 16u) {
+        const uint64_t mine[1] = {all[lane]};
+        uint32_t places[1];
+        count = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(mine[0] != 0ull));
+        places_of<1>(mine, 64u, count, scores, places);
+        keep(places[0], mine[0]);
+    } else {
+        const uint64_t mine[2] = {all[lane], all[lane + 64u]};
+        uint32_t places[2];
+        count = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(mine[0] != 0ull)) + (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(mine[1] != 0ull));
+        places_of<2>(mine, 128u, count, scores, places);
+        keep(places[0], mine[0]); keep(places[1], mine[1]);
+    }
+    if (P.slices != 1u && lane >= count && lane < P.top) out[lane * P.slices] = 0ull;      // (a slice may have fewer scores)
 }
 
 // Joins the slices of a row: a wave to a row.
@@ -481,19 +503,21 @@ extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob,
     const uint32_t lane = threadIdx.x;
     const uint64_t row = blockIdx.x;
     const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
-    if (token >= P.V) { write_padding(to, row, lane, 64u, P.top); return; }
-    const float score = logits[row * P.V + token];
     Sums sums; sums.start();
-    for (uint32_t k = lane; k < P.slices; k += 64u) {
+    for (uint32_t k = lane; k < P.slices; k += 64u) {                     // (of padding: whatever is there)
         const float* const part = parts + (row * P.slices + k) * 4u;
         sums.join(Sums{part[0], part[1], part[2]});
     }
+    if (token >= P.V) { write_padding(to, row, lane, 64u, P.top); return; }
+    const float score = logits[row * P.V + token];
     sums.join_lanes(64u);
     const Distribution p(sums);
     if (lane == 0u) write_sums(to, row, p, score);
     if (P.top == 0u) return;
     const uint32_t count = P.slices * P.top;
-    best_keys<16>(keys + row * count, count, room, P.top, [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, p); });
+    auto put = [&](uint32_t place, uint64_t key) { write_alternative(to, row, P.top, place, key, p); };
+    if (count <= 256u) best_keys<4>(keys + row * count, count, room, P.top, put);
+    else best_keys<16>(keys + row * count, count, room, P.top, put);
 }
 
 // Short rows: 2^log2_lanes lanes to a row, four vectors to a lane, and several rows to a wave. The alternatives one by one.
