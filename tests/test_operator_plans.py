@@ -117,7 +117,7 @@ def check_recurrence(b, t, c, gated=True, lengths=True):
     zeroed = lambda n, use: buffer(n, dtype=np.uint32)
     args = (x, x, state, buffer(b, dtype=np.int32) if lengths else None)
     for launch, in (K.linear_recurrence(x, state, *args, gated, False, zeroed), K.linear_recurrence_grad(x, x, state, x, *args, x, state, gated, True, zeroed)):
-        _, T, C, cstrips, strips, tiles, lines, log2_w, _ = words(launch)
+        _, T, C, cstrips, strips, tiles, lines, of_each, log2_w, _ = words(launch)
         vec, steps = (int(n) for n in re.search(r'_v(\d)_l(\d+)', launch.kernel).groups())
         W, G = 1 << log2_w, 256 >> log2_w
         assert (T, C) in ([(t, c), (1, b * c)] if t == 1 and not lengths else [(t, c)]) and (vec == 1 or C % 4 == 0)
@@ -129,8 +129,10 @@ def check_recurrence(b, t, c, gated=True, lengths=True):
         else:
             #the words of every tile and channel behind the tickets' lines; 32 channels at most; a block for every tile of every line of tickets
             assert W * vec <= K.RECURRENCE_CHAIN_CHANNELS and chain.size >= 2 * (8 * K.RECURRENCE_LINES + tiles * strips * W * vec)
-            mine = [strips * (i + 1) // lines - strips * i // lines for i in range(lines)]
-            assert launch.grid[0] % lines == 0 and launch.grid[0] // lines >= max(mine) * tiles and min(mine) > 0
+            every = cstrips if of_each else strips
+            mine = [strips // every * (every * (i + 1) // lines - every * i // lines) for i in range(lines)]
+            assert lines in (1, 8)
+            assert launch.grid[0] % lines == 0 and launch.grid[0] // lines >= max(mine) * tiles and min(mine) > 0 and sum(mine) == strips
             assert launch.scratch == (len(launch.buffers) - 1,) and launch.scratch[0] in launch.written
         yield launch.kernel
 

@@ -16,9 +16,12 @@
 // states in the same order, whatever it finds published, so the results do not depend on the order in which blocks run.
 //   * The wait ends: tiles are numbered in the order in which their blocks start (a ticket), a tile looks at earlier ones only, and
 //     the first tile without a state finds its predecessor's. So the earliest one always gets on, and then the next.
-//   * Neighbouring strips go to one XCD (every eighth block draws from a line of tickets of its own): where rows are no multiple of 128
-//     bytes they share lines, which are then fetched once: 15933 steps of 1976 channels 100 -> 90 us, the gradient 226 -> 207, and 142
-//     with parts of lines stored through the caches, which put them together. No result depends on where blocks run.
+//   * There are eight lines of tickets, one for every eighth block: drawn from one alone, they follow one another some 10 ns apart (3 x 1021 x
+//     333 11 us instead of 8). A line has neighbouring strips, an eighth of all, or, where they come out even, of every sequence's, so that
+//     different lengths keep all lines busy (8 x 2048 x 2048 with ragged lengths, forward and gradient 222 -> 207 us). Every eighth block is on
+//     one XCD: where rows are no multiple of 128 bytes, neighbouring strips share lines of memory, which are fetched once there. (15933 steps
+//     of 1976 channels, factors as they are, 100 -> 90 us, the gradient 226 -> 207, and 142 with parts of lines stored through the
+//     caches, which put them together.) No result depends on where blocks run.
 //   * A channel's word, 64 bits stored at once: H above, A below, with the lowest bit of A (a rounding of 2^-23 of A, for the tile's
 //     own use too) telling launches apart: its value alternates from launch to launch, and every launch writes every word. A state
 //     is marked by a NaN of its own in the place of A. No fence is needed, since a word holds all that is read, and nothing has to be
@@ -32,7 +35,9 @@
 
 struct RecurrenceParams {
     uint32_t first;                      // (bit 31: the result is stored past the caches)
-    uint32_t T, C, cstrips, strips, tiles, lines, log2_w, reverse;
+    uint32_t T, C, cstrips, strips, tiles;
+    uint32_t lines, of_each;             // lines of tickets, and whether each has a part of every sequence's strips
+    uint32_t log2_w, reverse;
 };
 
 constexpr uint32_t THREADS = 256, WINDOW = 16, CHAIN_CHANNELS = 32, LINES = 8;
@@ -91,8 +96,9 @@ struct Tile {
         tag = 0; words = nullptr; k = 0;
         strip = blockIdx.x;
         if constexpr (CHAIN) {
-            const uint32_t line = P.lines == 1u ? 0u : blockIdx.x & (LINES - 1u), per = gridDim.x / P.lines;
-            const uint32_t s0 = P.strips * line / P.lines, mine = P.strips * (line + 1u) / P.lines - s0;
+            const uint32_t line = blockIdx.x & (P.lines - 1u), per = gridDim.x / P.lines;
+            const uint32_t all = P.of_each ? P.cstrips : P.strips, s0 = all * line / P.lines, neighbours = all * (line + 1u) / P.lines - s0;
+            const uint32_t mine = P.of_each ? P.strips / P.cstrips * neighbours : neighbours;
             if (threadIdx.x == 0) ticket = __hip_atomic_fetch_add(chain + line * 8u, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             const unsigned long long t = ticket;
@@ -102,7 +108,9 @@ struct Tile {
             tag = (uint32_t)(launch + 1ull) & 1u;                          // (the first launch's words are odd: memory starts as zeros)
             words = chain + LINES * 8u;                                    // behind the tickets, a line each
             there = tile < mine * P.tiles;
-            k = tile / mine; strip = s0 + tile % mine;
+            k = tile / mine;
+            const uint32_t at = tile - k * mine, sequence = at / neighbours;      // (0 where a line's strips are not of every sequence)
+            strip = sequence * P.cstrips + s0 + (at - sequence * neighbours);
         }
         b = strip / P.cstrips; c0 = (strip % P.cstrips) * W * VEC;
         n = min(G * L, T - k * (G * L));

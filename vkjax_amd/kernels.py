@@ -2441,6 +2441,18 @@ class RecurrenceTiling(tp.NamedTuple):
     tiles:   int            #along time
 
 
+def _recurrence_lines(tiling: RecurrenceTiling) -> tp.Tuple[int, bool, int]:
+    '''(lines of tickets, whether each has a part of every sequence's strips - if that leaves at most a sixteenth more to some -,
+    blocks of the launch, as many for every line as the longest one has tiles)'''
+    lines = RECURRENCE_LINES if tiling.tiles > 1 and tiling.strips >= 2 * RECURRENCE_LINES else 1
+    most  = _cdiv(tiling.cstrips, lines)
+    if 16 * (lines * most - tiling.cstrips) <= tiling.cstrips:
+        blocks = lines * most * (tiling.strips // tiling.cstrips) * tiling.tiles
+        if blocks * RECURRENCE_THREADS < 2**32:
+            return lines, True, blocks
+    return lines, False, lines * _cdiv(tiling.strips, lines) * tiling.tiles
+
+
 def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays: int) -> RecurrenceTiling:
     '''How a recurrence is cut: as few groups of steps side by side as time needs, and with the lanes that leaves as many channels as
     there are, but at least a whole line of them; of the numbers of steps per thread the one that is estimated to take the least time
@@ -2463,21 +2475,21 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays
             best = (cost, steps, lanes, tiles)
     _, steps, lanes, tiles = best
     cstrips = _cdiv(channels, lanes * vec)
-    if (batch * cstrips + RECURRENCE_LINES) * tiles * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
+    tiling = RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
+    if _recurrence_lines(tiling)[2] * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
         raise NotImplementedError(f'a recurrence over {channels} channels in {batch} sequences of {time} steps')
-    return RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
+    return tiling
 
 
 def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int) -> Launch:
     _, t, c = shape
     kernel  = f'{name}_v{tiling.vec}_l{tiling.steps}' + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
     #(what tiles hand on: lines of 64 bytes for the tickets, then a word of 64 bits per channel and tile)
-    lines   = RECURRENCE_LINES if tiling.strips >= 2 * RECURRENCE_LINES else 1
-    blocks  = tiling.strips if tiling.tiles == 1 else lines * _cdiv(tiling.strips, lines) * tiling.tiles
+    lines, of_each, blocks = _recurrence_lines(tiling)
     chain   = None if tiling.tiles == 1 else zeroed(16 * RECURRENCE_LINES + 2 * tiling.tiles * tiling.strips * tiling.lanes * tiling.vec, f'{kernel} {tuple(tiling)}')
     buffers = [(v, 0) for v in arrays] + [(chain, 0)]
     return Launch(kernel, (blocks, 1, 1), (RECURRENCE_THREADS, 1, 1), buffers,
-                  _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.tiles, lines, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=c % 32 == 0,
+                  _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.tiles, lines, of_each, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=c % 32 == 0,
                   written=written + ((len(arrays),) if chain is not None else ()), scratch=(len(arrays),) if chain is not None else ())
 
 
