@@ -13,10 +13,16 @@
 // is in registers, and reading and writing are whole lines wherever a span has 32 channels. What the positions' lanes have found meets in
 // shared memory, where a few lanes per group add it up.
 //   * group_norm_held: samples small enough stay in registers: one launch that reads once and writes once. Several small samples share a
-//     block.
+//     block. 1 x 7 x 7 x 512 5 us, as long as a launch and its three round trips to memory take; 32 x 56 x 56 x 64 in 32 groups 16 us (51 MB,
+//     3.2 TB/s: every block reads, waits and writes once, and there are no more blocks than CUs to take turns; by half or quarter
+//     lines, 512 or 1024 threads, 15.7-17).
+//   * group_norm_rows: samples of one position, several rows to a block (8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5: groups of
+//     65 channels are summed up from shared memory, because they do not begin where vectors do).
 //   * group_norm_stats / _apply: the others are cut along their positions. The first launch leaves mean and squared deviations of each
-//     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it).
-// The gradient has the same two forms; what dscale and dshift get from a block is a row of sums per block, added up by a last launch
+//     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it). 64 x 56 x 56 x 256: 35 and 68 us, and
+//     71 and 107 for the gradient's two, all at 5.8-6.1 TB/s: bound by memory, and by reading everything twice. (Each launch
+//     begins where the one before it ended, for what the caches still hold.)
+// The gradient has the same forms; what dscale and dshift get from a block is a row of sums per block, added up by a last launch
 // (group_norm_columns) in a fixed order: no atomics.
 #include "common.h"
 
@@ -156,6 +162,20 @@ struct JoinSums {
     __device__ void add_again(uint32_t, uint32_t) {}
     __device__ void join_again(uint32_t) {}
 };
+
+// A block's row of sums per channel, over `rows` entries of each in shared memory, a few lanes to a channel.
+__device__ __forceinline__ void write_channel_sums(const float* firsts, const float* seconds, uint32_t rows, uint32_t stride, uint32_t width, float* to_first, float* to_second) {
+    const uint32_t log2_lanes = min(31u - (uint32_t)__clz((int)min(max(blockDim.x / width, 1u), 64u)), 31u - (uint32_t)__clz((int)rows)), lanes = 1u << log2_lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1u);
+    for (uint32_t base = 0; base < width; base += blockDim.x >> log2_lanes) {      // (every lane goes round as often: lanes meet below)
+        const uint32_t ch = base + (threadIdx.x >> log2_lanes);
+        float a = 0.f, b = 0.f;
+        if (ch < width)
+            for (uint32_t k = lane; k < rows; k += lanes) { a += firsts[k * stride + ch]; b += seconds[k * stride + ch]; }
+        a = add_lanes(a, lanes); b = add_lanes(b, lanes);
+        if (ch < width && lane == 0u) { to_first[ch] = a; to_second[ch] = b; }
+    }
+}
 
 // How many of `count` positions the lane q of `side` side by side has.
 __device__ __forceinline__ uint32_t share_of(uint32_t count, uint32_t q, uint32_t side) { return count > q ? (count - q - 1u) / side + 1u : 0u; }
@@ -308,12 +328,8 @@ __device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, fl
     for (int j = 0; j < VEC; ++j)
         if (span.p < all && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = d_total[j]; seconds[span.p * P.span + span.col * VEC + j] = dh_total[j]; }
     __syncthreads();
-    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
-        float a = 0.f, b = 0.f;
-        for (uint32_t k = 0; k < all; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
-        dshift_rows[(uint64_t)row * P.C + span.c0 + ch] = a;
-        dscale_rows[(uint64_t)row * P.C + span.c0 + ch] = b;
-    }
+    const uint64_t to = (uint64_t)row * P.C + span.c0;
+    write_channel_sums(firsts, seconds, all, P.span, span.width, dshift_rows + to, dscale_rows + to);
 }
 
 // ---------------------------------------------------------------------------------------------- single positions
@@ -506,12 +522,8 @@ __device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, fl
 #pragma unroll
     for (int j = 0; j < VEC; ++j) if (use) { firsts[span.p * P.span + span.col * VEC + j] = d_total[j]; seconds[span.p * P.span + span.col * VEC + j] = dh_total[j]; }
     __syncthreads();
-    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
-        float a = 0.f, b = 0.f;
-        for (uint32_t k = 0; k < side; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
-        dshift_rows[(uint64_t)row * P.C + span.c0 + ch] = a;
-        dscale_rows[(uint64_t)row * P.C + span.c0 + ch] = b;
-    }
+    const uint64_t to = (uint64_t)row * P.C + span.c0;
+    write_channel_sums(firsts, seconds, side, P.span, span.width, dshift_rows + to, dscale_rows + to);
 }
 
 // ---------------------------------------------------------------------------------------------- samples in chunks
@@ -719,13 +731,8 @@ __device__ __forceinline__ void grad_sums_body(float* partial, float* dscale_row
         float* const to = partial + 2u * ((((uint64_t)chunk.n * P.G + span.g0 + g) * P.pieces + piece) * P.chunks + chunk.chunk);
         to[0] = found.a; to[1] = found.b;
     });
-    const uint64_t row = (uint64_t)chunk.n * P.chunks + chunk.chunk;
-    for (uint32_t ch = threadIdx.x; ch < span.width; ch += blockDim.x) {
-        float a = 0.f, b = 0.f;
-        for (uint32_t k = 0; k < P.P; ++k) { a += firsts[k * P.span + ch]; b += seconds[k * P.span + ch]; }
-        dshift_rows[row * P.C + span.c0 + ch] = a;
-        dscale_rows[row * P.C + span.c0 + ch] = b;
-    }
+    const uint64_t to = ((uint64_t)chunk.n * P.chunks + chunk.chunk) * P.C + span.c0;
+    write_channel_sums(firsts, seconds, P.P, P.span, span.width, dshift_rows + to, dscale_rows + to);
 }
 
 template <int VEC>

@@ -27,8 +27,8 @@
 //     is marked by a NaN of its own in the place of A. No fence is needed, since a word holds all that is read, and nothing has to be
 //     cleared: the tickets count on through the launches, so their quotient is the launch's number.
 // What bounds it: memory, with two waves per SIMD; while a tile waits for its state the other block of its CU loads. 65536 steps of 1024
-// channels (805 MB) 152 us, 5.3 TB/s, where a large copy by a library reaches 5.1-5.5; 8 x 2048 x 2048 with ragged lengths 70 us, and
-// its gradient 140 us (716 MB). Smaller tiles have more words to look at and more ends to wait for: 8 steps per thread 160 us, 4 steps
+// channels (805 MB) 150 us, 5.3 TB/s, where a large copy by a library reaches 5.1-5.5; 8 x 2048 x 2048 with ragged lengths 67-74 us, and
+// its gradient 138-143 us (716 MB); single steps of 64 x 2048 3 us, a launch. Smaller tiles have more words to look at and more ends to wait for: 8 steps per thread 160 us, 4 steps
 // 250. Strips of 64 channels 10-15 % slower (fewer chains side by side), of 16 20 % (half lines). Blocks that draw a tile ahead and
 // load it while they wait hold up the tiles behind it: 265 us.
 #include "common.h"

@@ -2191,6 +2191,7 @@ NORM_ROWS      = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((
 NORM_ROWS_GRAD = {4: ((256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_PARTIAL_LINES = 128 << 20      #bytes up to which samples are held in registers by less than whole lines (25 MB 15.5 us, in chunks 23; 205 MB 95-111, 100)
+NORM_HELD_BLOCKS = 256              #blocks that samples held in registers are shared out to
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
 
@@ -2224,7 +2225,8 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
                     continue
                 side = threads // V
                 P    = min(side, _cdiv(s, k))
-                M    = min(side // P, n)
+                #several samples to a block where that leaves enough of them
+                M    = min(side // P, _cdiv(n * _cdiv(c, span), NORM_HELD_BLOCKS))
                 if _cdiv(s, P) > k or M * s * c * 4 >= 2**31:
                     continue
                 blocks = _cdiv(n, M) * _cdiv(c, span)
@@ -2363,6 +2365,9 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
 LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane. With many alternatives half as many:
 LOG_PROBS_MANY      = 5             #(65536 rows of 500 and top of 1, 5, 20: 32, 53, 132 us, a wave to a row 43, 50, 70; rows of 250: 17, 27, 66, and 42, 49, 75)
+#of up to LOG_PROBS_FEW short rows too where there are more than LOG_PROBS_TURNS alternatives, each of which is a turn of half a microsecond there
+#(208 rows of 19, top of 19: 13.3 us, a wave to a row 5.5; 8000 of 100, top of 20 and 6: 15.8 and 7.9, 12.3 and 9.4)
+LOG_PROBS_FEW, LOG_PROBS_TURNS = 8192, 8
 LOG_PROBS_WAVE      = 1024          #rows of up to this many vectors have a wave each where there are enough of them, longer ones a block
 LOG_PROBS_ROWS      = 1024          #enough rows not to be cut
 LOG_PROBS_MAX_KEYS  = 1024          #candidates of all slices of a row
@@ -2378,7 +2383,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     if v >= 2**29 or rows * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4)
-    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2):
+    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2) and not (top > LOG_PROBS_TURNS and rows <= LOG_PROBS_FEW):
         lanes = _pow2_at_least(_cdiv(vectors, 4))
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
