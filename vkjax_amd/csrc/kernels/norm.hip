@@ -16,8 +16,8 @@
 //     block. 1 x 7 x 7 x 512 5 us, as long as a launch and its three round trips to memory take; 32 x 56 x 56 x 64 in 32 groups 16 us (51 MB,
 //     3.2 TB/s: every block reads, waits and writes once, and there are no more blocks than CUs to take turns; by half or quarter
 //     lines, 512 or 1024 threads, 15.7-17).
-//   * group_norm_rows: samples of one position, several rows to a block (8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5: groups of
-//     65 channels are summed up from shared memory, because they do not begin where vectors do).
+//   * group_norm_rows: samples of one position, several rows to a block (8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5; rows go
+//     through shared memory, because groups of 65 channels do not begin where vectors do; groups of 64 16.5 and 25).
 //   * group_norm_stats / _apply: the others are cut along their positions. The first launch leaves mean and squared deviations of each
 //     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it). 64 x 56 x 56 x 256: 35 and 68 us, and
 //     71 and 107 for the gradient's two, all at 5.8-6.1 TB/s: bound by memory, and by reading everything twice. (Each launch
