@@ -375,3 +375,57 @@ def test_arrays_without_elements_are_planned():
     z, t = np.zeros((0, 7), f32), np.zeros(0, np.int32)
     assert evaluate(probs, z, t, np.zeros(0, f32))[2].shape == (0, 7)
     JaxprInterpreter(mj.make_jaxpr(probs)(z, t, np.zeros(0, f32)), plan_only=True)
+
+
+# ------------------------------------------------------------------ gradients called by themselves
+
+def refused(error, f, *args):
+    with pytest.raises(error):
+        mj.make_jaxpr(f)(*args)
+
+
+@pytest.mark.parametrize('which,shape', [(0, (2, 5, 12)), (1, (2, 6, 8)), (2, (8,)), (3, (11,)), (3, (12, 1)), (4, (2, 4)), (4, (3, 3)), (5, (2,))])
+def test_group_norm_gradient_refuses_shapes_that_do_not_belong(which, shape):
+    shapes = [(2, 6, 12), (2, 6, 12), (12,), (12,), (2, 3), (2, 3)]
+    mj.make_jaxpr(lambda *a: lax.group_norm_grad(*a, 3))(*[np.zeros(s, f32) for s in shapes])
+    shapes[which] = shape
+    refused((TypeError, ValueError), lambda *a: lax.group_norm_grad(*a, 3), *[np.zeros(s, f32) for s in shapes])
+
+
+def test_group_norm_gradient_refuses_what_group_norm_refuses():
+    arrays = [np.zeros(s, f32) for s in [(2, 6, 12), (2, 6, 12), (12,), (12,), (2, 5), (2, 5)]]
+    refused(ValueError, lambda *a: lax.group_norm_grad(*a, 5), *arrays)
+    arrays[4:] = [np.zeros((2, 3), f32)] * 2
+    refused(ValueError, lambda *a: lax.group_norm_grad(*a, 3, eps=1e-60), *arrays)
+    refused(ValueError, lambda *a: lax.group_norm(*a, 3, eps=1e-60), *arrays[1:4])
+    refused(ValueError, lambda *a: lax.group_norm_grad(*a, 3, activation='tanh'), *arrays)
+    for k in range(6):
+        refused(TypeError, lambda *a: lax.group_norm_grad(*a, 3), *[v.astype(np.int32) if i == k else v for i, v in enumerate(arrays)])
+
+
+def test_log_probs_gradient_refuses():
+    z, t, row, top, ids = np.zeros((3, 9), f32), np.zeros(3, np.int32), np.zeros(3, f32), np.zeros((3, 2), f32), np.zeros((3, 2), np.int32)
+    mj.make_jaxpr(lax.token_log_probs_grad)(z, t, row, row, row, row, top, ids)
+    for args in [(z, t[:2], row, row, row), (z, t, row[:2], row, row), (z, t, row, row, row[:1]), (z, t, row, row, row, row, top, ids[:, :1]), (z, row, row, row, row),
+                 (z, t, row, row, t), (z, t, t, row, row), (z, t, row, row, row, row, ids, ids), (z, t, row, row, row, row, top, top), (z.astype(np.int32), t, row, row, row),
+                 (z, t, row, row, row, row, top[:, :0], ids[:, :0]), (z[:, :0], t, row, row, row)]:
+        refused(TypeError, lax.token_log_probs_grad, *args)
+
+
+def test_recurrence_gradient_refuses():
+    x, last = np.zeros((2, 5, 3), f32), np.zeros((2, 3), f32)
+    mj.make_jaxpr(lambda *a: lax.linear_recurrence_grad(*a[:4], None, *a[4:]))(x, x, x, last, x, last)
+    for k, bad in [(0, x[:, :4]), (0, x.astype(np.int32)), (1, x[:1]), (2, x[..., :2]), (3, last[:1]), (4, x[:, 1:]), (4, x.astype(np.int32)), (5, last[:, :1]), (5, x)]:
+        args = [x, x, x, last, x, last]
+        args[k] = bad
+        refused(TypeError, lambda *a: lax.linear_recurrence_grad(*a[:4], None, *a[4:]), *args)
+    refused(TypeError, lambda f, x: lax.linear_recurrence_grad(None, f, x), x, x)
+
+
+def test_gradients_have_no_gradients_of_their_own():
+    x, s = np.zeros((2, 6, 12), f32), np.ones(12, f32)
+
+    def twice(x, s):
+        inner = lambda x: lax.add(mj.numpy.sum(mj.grad(lambda v: mj.numpy.sum(nn.group_norm(v, s, s, 3)))(x)), np.float32(0))
+        return mj.grad(inner)(x)
+    refused(NotImplementedError, twice, x, s)

@@ -525,30 +525,37 @@ def group_norm(x, scale, shift, groups: int, eps: float = 1e-5, activation=None)
     '''activation((x - mean) / sqrt(var + eps) * scale + shift) of x [N, ..., C], mean and variance over everything of one sample
     in one of `groups` runs of neighbouring channels; scale and shift are [C]. Returns (y, mean [N, groups],
     1 / sqrt(var + eps) [N, groups]).'''
-    x, scale, shift = (_f32_operand(v, 'group_norm') for v in (x, scale, shift))
+    x, scale, shift, params = _group_norm_operands('group_norm', x, scale, shift, groups, eps, activation)
+    xs, stats = _shape(x), _aval((_shape(x)[0], params['groups']), _f32)
+    return tuple(emit('group_norm', [x, scale, shift], [_aval(xs, _f32), stats, stats], params, multiple_results=True))
+
+
+def _group_norm_operands(name, x, scale, shift, groups, eps, activation):
+    x, scale, shift = (_f32_operand(v, name) for v in (x, scale, shift))
     xs = _shape(x)
     if len(xs) < 2:
-        raise TypeError(f'group_norm takes [samples, ..., channels], got {xs}')
+        raise TypeError(f'{name} takes [samples, ..., channels], got {xs}')
     groups, channels = int(groups), xs[-1]
     if groups < 1 or channels < 1 or channels % groups:
-        raise ValueError(f'group_norm: {channels} channels do not fall into {groups} groups of equal size')
+        raise ValueError(f'{name}: {channels} channels do not fall into {groups} groups of equal size')
     if _shape(scale) != (channels,) or _shape(shift) != (channels,):
-        raise TypeError(f'group_norm: scale and shift must have shape ({channels},), got {_shape(scale)} and {_shape(shift)}')
+        raise TypeError(f'{name}: scale and shift must have shape ({channels},), got {_shape(scale)} and {_shape(shift)}')
     if not (0.0 < float(np.float32(eps)) < np.inf):
-        raise ValueError(f'group_norm: eps must be positive and finite, got {eps}')
+        raise ValueError(f'{name}: eps must be positive and finite, got {eps}')
     if activation not in GROUP_NORM_ACTIVATIONS:
-        raise ValueError(f'group_norm: activation must be one of {GROUP_NORM_ACTIVATIONS}, got {activation!r}')
-    return tuple(emit('group_norm', [x, scale, shift], [_aval(xs, _f32), _aval((xs[0], groups), _f32), _aval((xs[0], groups), _f32)],
-                dict(groups=groups, eps=float(eps), activation=activation), multiple_results=True))
+        raise ValueError(f'{name}: activation must be one of {GROUP_NORM_ACTIVATIONS}, got {activation!r}')
+    return x, scale, shift, dict(groups=groups, eps=float(eps), activation=activation)
 
 
 def group_norm_grad(g, x, scale, shift, mean, rstd, groups: int, eps: float = 1e-5, activation=None):
     '''(dx, dscale, dshift) for the cotangent g of group_norm's y; mean and rstd are what group_norm returned.'''
-    xs, cs = _shape(x), _shape(scale)
-    if _shape(g) != xs or _shape(mean) != (xs[0], groups) or _shape(rstd) != (xs[0], groups):
+    x, scale, shift, params = _group_norm_operands('group_norm_grad', x, scale, shift, groups, eps, activation)
+    g, mean, rstd = (_f32_operand(v, 'group_norm_grad') for v in (g, mean, rstd))
+    xs, cs, stats = _shape(x), _shape(scale), (_shape(x)[0], params['groups'])
+    if _shape(g) != xs or _shape(mean) != stats or _shape(rstd) != stats:
         raise TypeError(f'group_norm_grad: shapes {_shape(g)}, {xs}, {_shape(mean)}, {_shape(rstd)} do not belong together')
-    return tuple(emit('group_norm_grad', [g, x, scale, shift, mean, rstd], [_aval(xs, _f32), _aval(cs, _f32), _aval(cs, _f32)],
-                dict(groups=int(groups), eps=float(eps), activation=activation), multiple_results=True))
+    return tuple(emit('group_norm_grad', [g, x, scale, shift, mean, rstd], [_aval(xs, _f32), _aval(cs, _f32), _aval(cs, _f32)], params,
+                multiple_results=True))
 
 
 TOKEN_LOG_PROBS_MAX_TOP = 32
@@ -558,33 +565,46 @@ def token_log_probs(logits, tokens, top: int = 0):
     '''For rows of scores [..., V] and one token per row [...]: (log softmax(logits)[token], entropy of softmax(logits),
     log(sum(exp(logits)))), all [...], and for top > 0 the log probabilities and numbers [..., top] of the most likely tokens.
     `nn.token_log_probs` says what becomes of padded and masked rows.'''
-    logits = _f32_operand(logits, 'token_log_probs')
-    tokens = tokens if isinstance(tokens, Tracer) else np.asarray(tokens)
+    logits, tokens = _rows_and_tokens('token_log_probs', logits, tokens)
     ls, top = _shape(logits), int(top)
-    if len(ls) < 1 or ls[-1] < 1:
-        raise TypeError(f'token_log_probs takes [..., vocabulary] with at least one token, got {ls}')
-    if dtype_of(tokens)[0] not in (_i32, _u32):
-        raise TypeError(f'token_log_probs: tokens must be integers, got {dtype_of(tokens)[0]}')
-    if _shape(tokens) != ls[:-1]:
-        raise TypeError(f'token_log_probs: one token per row of {ls} is needed, got {_shape(tokens)}')
     if not 0 <= top <= builtins.min(ls[-1], TOKEN_LOG_PROBS_MAX_TOP):
         raise ValueError(f'token_log_probs: top must be between 0 and {builtins.min(ls[-1], TOKEN_LOG_PROBS_MAX_TOP)} here, got {top}')
     rows  = _aval(ls[:-1], _f32)
     avals = [rows, rows, rows] + ([_aval(ls[:-1] + (top,), _f32), _aval(ls[:-1] + (top,), _i32)] if top else [])
-    return tuple(emit('token_log_probs', [logits, _as_dtype(tokens, dtype_of(tokens)[0])], avals, dict(top=top), multiple_results=True))
+    return tuple(emit('token_log_probs', [logits, tokens], avals, dict(top=top), multiple_results=True))
+
+
+def _integer_operand(x, what):
+    x = x if isinstance(x, Tracer) else np.asarray(x)
+    if dtype_of(x)[0] not in (_i32, _u32):
+        raise TypeError(f'{what}: tokens must be integers, got {dtype_of(x)[0]}')
+    return _as_dtype(x, dtype_of(x)[0])
+
+
+def _rows_and_tokens(name, logits, tokens):
+    logits, tokens = _f32_operand(logits, name), _integer_operand(tokens, name)
+    ls = _shape(logits)
+    if len(ls) < 1 or ls[-1] < 1:
+        raise TypeError(f'{name} takes [..., vocabulary] with at least one token, got {ls}')
+    if _shape(tokens) != ls[:-1]:
+        raise TypeError(f'{name}: one token per row of {ls} is needed, got {_shape(tokens)}')
+    return logits, tokens
 
 
 def token_log_probs_grad(logits, tokens, log_sum, entropy, g_log_probs=None, g_entropy=None, g_top=None, top_tokens=None):
     '''Cotangent of token_log_probs' logits for those of its results (None: zeros), of which log_sum, entropy and top_tokens are.'''
+    name = 'token_log_probs_grad'
+    logits, tokens = _rows_and_tokens(name, logits, tokens)
+    log_sum, entropy, *optional = [_f32_operand(v, name) for v in (log_sum, entropy, g_log_probs, g_entropy) if v is not None]
     ls = _shape(logits)
-    optional = [g for g in (g_log_probs, g_entropy) if g is not None]
-    if _any_differs(ls[:-1], tokens, log_sum, entropy, *optional):
-        raise TypeError('token_log_probs_grad: one value per row is needed')
+    if _any_differs(ls[:-1], log_sum, entropy, *optional):
+        raise TypeError(f'{name}: one value per row is needed')
     top = 0
     if g_top is not None:
-        top = _shape(top_tokens)[-1]
-        if _any_differs(ls[:-1] + (top,), g_top, top_tokens):
-            raise TypeError('token_log_probs_grad: the alternatives and their cotangents must have the same shape')
+        g_top, top_tokens = _f32_operand(g_top, name), _integer_operand(top_tokens, name)
+        top = _shape(top_tokens)[-1] if _shape(top_tokens) else 0
+        if top < 1 or _any_differs(ls[:-1] + (top,), g_top, top_tokens):
+            raise TypeError(f'{name}: the alternatives and their cotangents must have the same shape')
         optional += [g_top, top_tokens]
     return emit('token_log_probs_grad', [logits, tokens, log_sum, entropy] + optional, [_aval(ls, _f32)],
                 dict(has_log_probs=g_log_probs is not None, has_entropy=g_entropy is not None, top=top))
@@ -634,7 +654,8 @@ def linear_recurrence_grad(h, factor, x, state=None, lengths=None, g=None, g_las
     '''(dfactor, dx, dstate [batch, channels]) for the cotangents g and g_last (None: zeros) of linear_recurrence's results, of
     which h is the first.'''
     operands, xs = _recurrence_operands('linear_recurrence_grad', factor, x, state, lengths)
-    if (_any_differs(xs, h) or (g is not None and _shape(g) != xs) or (g_last is not None and _shape(g_last) != (xs[0], xs[2]))):
+    h, g, g_last = (v if v is None else _f32_operand(v, 'linear_recurrence_grad') for v in (h, g, g_last))
+    if h is None or (_any_differs(xs, h) or (g is not None and _shape(g) != xs) or (g_last is not None and _shape(g_last) != (xs[0], xs[2]))):
         raise TypeError(f'linear_recurrence_grad: the cotangents and h do not belong to {xs}')
     return tuple(emit('linear_recurrence_grad', [h] + operands + [v for v in (g, g_last) if v is not None],
                 [_aval(xs, _f32), _aval(xs, _f32), _aval((xs[0], xs[2]), _f32)],
