@@ -627,7 +627,11 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
     const bool nothing = token >= P.V || lse == -INFINITY;
     const float own = g_log_prob && there ? g_log_prob[row] : 0.f, gh = g_entropy && there ? g_entropy[row] : 0.f;
     float total = own;
-    if (there) for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
+    if (there)
+#pragma unroll 4
+        for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
+    // rows of few lanes: every score looks for itself among the alternatives. (2319 rows of 12, all of them alternatives: 7 us, a lane to an alternative some 27)
+    const bool few = P.log2_lanes <= 2u;
     const uint32_t from = at0 - lead;
     for (uint32_t q = q0 + lane; q < q1; q += lanes * NV) {
         f32x4 v[NV];
@@ -644,6 +648,17 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
             else
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<true>(v[i][j], lse, total, gh, H);
+            if (few && !nothing) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] += at * 4u + j - lead == token ? own : 0.f;
+#pragma unroll 4
+                for (uint32_t k = 0; k < P.top; ++k) {
+                    const uint32_t which = (uint32_t)top_token[row * P.top + k] + lead - at * 4u;
+                    const float g = g_top[row * P.top + k];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) d[j] += which == (uint32_t)j ? g : 0.f;
+                }
+            }
             if (at >= q1) continue;
             if (at * 4u >= lead && at * 4u + 4u <= lead + P.V) {
                 const u32x4 t = u32x4{f2u(d[0]), f2u(d[1]), f2u(d[2]), f2u(d[3])};
@@ -655,6 +670,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
             }
         }
     }
+    if (few) return;
     __syncthreads();
     if (nothing || !there) return;
     // number k < top: alternative k, number `top`: the given token; in the slice that has its score

@@ -598,31 +598,50 @@ __device__ __forceinline__ void stats_body(float* partial, const float* x, const
     });
 }
 
-// Joins what the chunks and pieces of the groups of a span have left, a few lanes to a group; `use(group, mean or first sum, deviations or
-// second sum)` in the lane that reports. STATS: means and squared deviations; else two sums.
+// Joins what the chunks and pieces of the groups of a span have left, a few lanes to a group: all groups at once, but no more than eight parts to a lane, which it
+// reads together (2 x 1196 x 256 in 64 groups, 75 chunks, forward and gradient: a wave to a group 54 us, so 33). `use(group, mean or first sum, deviations or second sum)` in the lane that reports.
+// STATS: means and squared deviations; else two sums.
 template <bool STATS, int VEC, class Use>
 __device__ __forceinline__ void join_chunks(const NormParams& P, const Span<VEC>& span, uint32_t n, const float* partial, Use use) {
-    const uint32_t parts = P.chunks * P.pieces, log2_lanes = 31u - (uint32_t)__clz((int)min(parts, 64u)), lanes = 1u << log2_lanes;
+    constexpr uint32_t HELD = 8;
+    const uint32_t parts = P.chunks * P.pieces, groups = max(P.span / P.cg, 1u);
+    auto log2_below = [](uint32_t v) { return 31u - (uint32_t)__clz((int)v); };
+    const uint32_t log2_lanes = min(6u, max(log2_below(max(blockDim.x / groups, 1u)), log2_below(2u * ((parts - 1u) / HELD) + 1u))), lanes = 1u << log2_lanes;
     const uint32_t lane = threadIdx.x & (lanes - 1u), sets = blockDim.x >> log2_lanes;
     const uint32_t start = threadIdx.x >> log2_lanes;
     for (uint32_t g = start; g - start < span.groups; g += sets) {
         const bool there = g < span.groups;
-        const float* const from = partial + 2u * ((uint64_t)n * P.G + span.g0 + (there ? g : 0u)) * parts;
+        const f32x2* const from = reinterpret_cast<const f32x2*>(partial) + ((uint64_t)n * P.G + span.g0 + (there ? g : 0u)) * parts;
         auto count = [&](uint32_t k) {
             const uint32_t piece = k / P.chunks, c = k - piece * P.chunks;
             const uint32_t channels = P.pieces == 1u ? P.cg : min(P.span, P.cg - piece * P.span);
             return (float)min(P.chunk, P.S - c * P.chunk) * (float)channels;
         };
         float a = 0.f, b = 0.f, total = 0.f;
-        for (uint32_t k = lane; k < parts; k += lanes) {
-            if constexpr (STATS) { const float c = count(k); a = __builtin_fmaf(from[2u * k], c, a); total += c; }
-            else { a += from[2u * k]; b += from[2u * k + 1u]; }
-        }
-        a = add_lanes(a, lanes);
-        if constexpr (STATS) {
-            total = add_lanes(total, lanes);
-            a /= total;
-            for (uint32_t k = lane; k < parts; k += lanes) { const float d = from[2u * k] - a; b += __builtin_fmaf(count(k) * d, d, from[2u * k + 1u]); }
+        auto first = [&](f32x2 part, uint32_t k) {
+            if constexpr (STATS) { const float c = count(k); a = __builtin_fmaf(part.x, c, a); total += c; }
+            else { a += part.x; b += part.y; }
+        };
+        auto second = [&](f32x2 part, uint32_t k) { const float d = part.x - a; b += __builtin_fmaf(count(k) * d, d, part.y); };
+        if (parts <= HELD * lanes) {
+            f32x2 mine[HELD];
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) mine[i] = i * lanes + lane < parts ? from[i * lanes + lane] : f32x2{0.f, 0.f};
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) if (i * lanes + lane < parts) first(mine[i], i * lanes + lane);
+            a = add_lanes(a, lanes);
+            if constexpr (STATS) {
+                a /= add_lanes(total, lanes);
+#pragma unroll
+                for (uint32_t i = 0; i < HELD; ++i) if (i * lanes + lane < parts) second(mine[i], i * lanes + lane);
+            }
+        } else {
+            for (uint32_t k = lane; k < parts; k += lanes) first(from[k], k);
+            a = add_lanes(a, lanes);
+            if constexpr (STATS) {
+                a /= add_lanes(total, lanes);
+                for (uint32_t k = lane; k < parts; k += lanes) second(from[k], k);
+            }
         }
         b = add_lanes(b, lanes);
         if (there && lane == 0u) use(g, a, b);

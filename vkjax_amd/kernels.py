@@ -2365,9 +2365,9 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
 LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane. With many alternatives half as many:
 LOG_PROBS_MANY      = 5             #(65536 rows of 500 and top of 1, 5, 20: 32, 53, 132 us, a wave to a row 43, 50, 70; rows of 250: 17, 27, 66, and 42, 49, 75)
-#of up to LOG_PROBS_FEW short rows too where there are more than LOG_PROBS_TURNS alternatives, each of which is a turn of half a microsecond there
+#few short rows too: an alternative is a turn of half a microsecond where they share one, and 700 waves more take as long
 #(208 rows of 19, top of 19: 13.3 us, a wave to a row 5.5; 8000 of 100, top of 20 and 6: 15.8 and 7.9, 12.3 and 9.4)
-LOG_PROBS_FEW, LOG_PROBS_TURNS = 8192, 8
+LOG_PROBS_FEW       = 700
 LOG_PROBS_WAVE      = 1024          #rows of up to this many vectors have a wave each where there are enough of them, longer ones a block
 LOG_PROBS_ROWS      = 1024          #enough rows not to be cut
 LOG_PROBS_MAX_KEYS  = 1024          #candidates of all slices of a row
@@ -2383,7 +2383,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     if v >= 2**29 or rows * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4)
-    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2) and not (top > LOG_PROBS_TURNS and rows <= LOG_PROBS_FEW):
+    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2) and top <= 2 + rows // LOG_PROBS_FEW:
         lanes = _pow2_at_least(_cdiv(vectors, 4))
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
