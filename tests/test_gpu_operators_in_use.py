@@ -305,3 +305,27 @@ def test_recurrence_of_two_gigabytes(b, t, c):
         l = float(x[k]) + a * l
         ls.append(l * (1 - a))
     close(dx, np.array(ls[::-1]), 48 * U * 6 * 5)
+
+
+# ------------------------------------------------------------------ many alternatives, of which more stand out at once than there is room for
+
+@pytest.mark.parametrize('rows,v,levels', [(600, 167, None), (300, 511, 40), (500, 1000, None), (400, 4092, None), (200, 8000, 300), (150, 22133, None), (3, 127677, None),
+                                           (2, 127677, 7), (2, 100000, 1), (900, 19, 3), (64, 129, 2)])
+@pytest.mark.parametrize('top', [19, 24, 32])
+def test_many_alternatives(rows, v, levels, top):
+    '''Scores of any value, or of few different ones: which are alternatives, and in what order, is exact.'''
+    top = min(top, v)
+    rng = np.random.default_rng(rows + v + top)
+    z = normal(rows + v, rows, v, scale=2.0) if levels is None else rng.integers(0, levels, (rows, v)).astype(f32)
+    z[rng.random((rows, v)) < 0.3 * (np.arange(rows) % 3 == 0)[:, None]] = -np.inf
+    t = rng.integers(0, v, rows).astype(np.int32)
+    log_p, _, top_log_p, tokens = vkjax_amd.wrap(lambda z, t: nn.token_log_probs(z, t, top), frontend='minijax')(z, t)
+    order = np.argsort(-z, axis=1, kind='stable')[:, :top]
+    assert np.array_equal(tokens, order)
+    z64 = z.astype(np.float64)
+    most = z64.max(1)
+    logp = z64 - np.where(most == -np.inf, 0.0, most + np.log(np.exp(z64 - np.where(most == -np.inf, 0.0, most)[:, None]).sum(1)))[:, None]
+    #sums of up to 64 additions in a row, joined four times over, and roundings of values of at most 30 (and 300)
+    bound = (64 + 16) * 2 * U + 6 * U * (30 if levels is None else 300 + 12)
+    close(top_log_p, np.take_along_axis(logp, order, 1), bound)
+    close(log_p, logp[np.arange(rows), t], bound)

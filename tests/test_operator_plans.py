@@ -102,7 +102,7 @@ def check_log_probs(rows, v, top):
         elif launch.kernel == 'log_probs_block':
             assert slices * 4 * slice_ >= vectors and slice_ % 64 == 0 and launch.grid[0] == rows * slices
         else:
-            assert slices * top <= 1024 and launch.lds >= max(8 * slices * top, 256 if top else 0)
+            assert slices * top <= 1024 and launch.lds == 0
         yield launch.kernel
     launch, = K.token_log_probs_grad(z, z, t, r, r, r, r, k if top else None, k if top else None, top)
     rows_, R, V, T, slices, slice_, log2_lanes = words(launch)

@@ -16,8 +16,9 @@
 // The alternatives: with the lanes in k groups or more, the smallest of the groups' maxima is no larger than the k-th largest score: a bar, found in six steps
 // and raised by a few bisections where many lanes pass it. Of the first 1024 scores only what reaches the bar can be among the k largest: a few more than k
 // scores, which go into a list. From then on only scores above the bar are looked at: one comparison per lane and 16 scores, and rarely
-// more. The list is cut to k scores, and the bar raised, when it is long. Where more stand out at once than the list holds, the largest are
-// taken one by one. Places in the list are counted once, at the end.
+// more. The list is cut to k scores, and the bar raised, when it is long. Where more stand out at once than the list holds, a bisection of their
+// keys raises the bar; only where that many are equal, the largest are taken one by one, 60 us of a wave's time. (Without the bisection one wave in a hundred
+// came to that, and the launch waited for it: 32 of 1024 x 4092 82 us instead of 23.) Places in the list are counted once, at the end.
 //
 // What bounds it: without alternatives, memory (65536 rows of 1000 39 us, 6.8 TB/s; 4096 of 32000 89 us, 5.9; its gradient 172 us, 5.9). With them, the
 // instructions that look for them: 5 of 65536 x 1000 54 us, 20 63; 20 of 4096 x 32000 118. (Rows a few to a wave, the next one's scores asked for ahead, need
@@ -121,27 +122,6 @@ __device__ __forceinline__ void places_of(const uint64_t (&keys)[N], uint32_t en
             for (int k = 0; k < N; ++k) places[k] += other > keys[k];
         }
 }
-// put(place, key) for the `top` largest of `count` keys in shared memory, which is written over (256 bytes of it at least).
-template <class Put>
-__device__ __forceinline__ void rank(uint64_t* keys, uint32_t count, uint32_t top, Put put) {
-    const uint32_t lane = __lane_id();
-    if (count <= 64u) {
-        const uint64_t mine[1] = {lane < count ? keys[lane] : 0ull};
-        uint32_t place[1];
-        wave_fence();
-        places_of<1>(mine, count, count, reinterpret_cast<uint32_t*>(keys), place);
-        if (lane < count && place[0] < top) put(place[0], mine[0]);
-    } else
-        for (uint32_t at = 0; at < count; at += 64u) {
-            const uint32_t mine = at + lane;
-            const uint64_t key = mine < count ? keys[mine] : 0ull;
-            uint32_t place = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < count; ++i) place += keys[i] > key;
-            if (mine < count && place < top) put(place, key);
-        }
-}
-
 // A value that at least k (up to 32) of the lanes' values reach, and not many more: of 2^n >= k groups of lanes the smallest maximum, raised by bisection.
 __device__ __forceinline__ float bar_of(float lane_value, uint32_t k) {
     const uint32_t group = 64u >> (32u - (uint32_t)__clz((int)k - 1));    // lanes to a group (k = 1: all)
@@ -160,6 +140,8 @@ __device__ __forceinline__ float bar_of(float lane_value, uint32_t k) {
     }
     return bar;
 }
+
+__device__ __forceinline__ float wave_max(float v) { return lanes_allreduce(v, 64u, [](float a, float b) { return fmaxf(a, b); }); }
 
 // The k-th largest of the lanes' values, bit by bit, by how many lanes are no smaller.
 __device__ __forceinline__ float kth_largest(float lane_value, uint32_t k) {
@@ -228,22 +210,43 @@ struct Candidates {
             if (bar == -INFINITY) bar = kth_largest(most, top);           // (much of it masked)
         } else if (__builtin_amdgcn_ballot_w64(!(most <= bar) || broken) == 0ull) return;
         // of the first scores those that reach the bar
-        const float from = fresh && bar != -INFINITY ? below(bar) : bar;
-        uint32_t n = count;
+        float from = fresh && bar != -INFINITY ? below(bar) : bar;
+        uint32_t n;
+#pragma nounroll
+        for (bool again = false;; again = true) {
+            n = count;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (__builtin_amdgcn_ballot_w64(!(best[i] <= from) || broken) == 0ull) continue;
+            for (int i = 0; i < NV; ++i) {
+                if (__builtin_amdgcn_ballot_w64(!(best[i] <= from) || broken) == 0ull) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint64_t mask = __builtin_amdgcn_ballot_w64(!(v[i][j] <= from));
-                if (mask != 0ull) {
-                    const uint32_t more = (uint32_t)__popcll(mask);
-                    if (n + more <= LIST && !(v[i][j] <= from)) entries[n + lanes_below(mask)] = entry_of(v[i][j], chunk.token(i, j));
-                    n += more;
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t mask = __builtin_amdgcn_ballot_w64(!(v[i][j] <= from));
+                    if (mask != 0ull) {
+                        const uint32_t more = (uint32_t)__popcll(mask);
+                        if (n + more <= LIST && !(v[i][j] <= from)) entries[n + lanes_below(mask)] = entry_of(v[i][j], chunk.token(i, j));
+                        n += more;
+                    }
                 }
             }
+            if (n <= LIST) break;
+            if (again) { one_by_one(chunk); return; }
+            // more than there is room for: once more from a higher bar, that of the list cut to its largest or one that as many of these scores reach as do not
+            // fill the list, which a bisection of their keys finds
+            if (count > top) { cut(); from = bar; }
+            uint32_t low = score_key(from), high = score_key(wave_max(most));
+            for (int step = 0; step < 32 && high - low > 1u; ++step) {
+                const uint32_t between = low + ((high - low) >> 1);
+                const float x = key_score(between);
+                uint32_t passing = 0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) passing += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(!(v[i][j] <= x)));
+                if (passing < top) { high = between; continue; }
+                low = between; from = x;
+                if (count + passing <= LIST) break;
+            }
         }
-        if (n > LIST) { one_by_one(chunk); return; }
         count = n;
         if (fresh && count < top) {                                       // masked scores: as many as are missing, the first of them
             uint32_t need = top - count;
@@ -368,7 +371,8 @@ __device__ __forceinline__ void read_row(const Row& row, uint32_t q0, uint32_t q
     }
 }
 
-// put(place, key) for the `top` largest of `count` keys (up to 64 N; zeros are none), by a wave; `room` holds as many in shared memory. The alternatives' bar, for keys.
+// put(place, key) for the `top` largest of `count` keys (up to 64 N, no two the same; zeros are none), by a wave; `room` holds 64 in shared memory. The alternatives'
+// bar, for keys, raised until no more than 64 pass.
 template <int N, class Put>
 __device__ __forceinline__ void best_keys(const uint64_t* keys, uint32_t count, uint64_t* room, uint32_t top, Put put) {
     const uint32_t lane = __lane_id(), group = 64u >> (32u - (uint32_t)__clz((int)top - 1));
@@ -382,16 +386,47 @@ __device__ __forceinline__ void best_keys(const uint64_t* keys, uint32_t count, 
         const uint64_t other = lane_xor<S>(bar);
         bar = ((uint32_t)S >= 64u / group) == (other > bar) ? other : bar;
     });
+    auto passing = [&](auto passes) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(mine[i] != 0ull && passes(mine[i])));
+        return n;
+    };
+    bar = of_lane(bar, 0u);
+    if (passing([&](uint64_t key) { return key >= bar; }) > 64u) {
+        // by the scores alone, and, where too many are equal, by the tokens among them (of neighbouring bars one lets at most one key more through)
+        uint32_t low = (uint32_t)(bar >> 32), high = 0u, n = count;
+#pragma unroll
+        for (int i = 0; i < N; ++i) high = max(high, (uint32_t)(mine[i] >> 32));
+        high = lanes_allreduce(high, 64u, [](uint32_t a, uint32_t b) { return max(a, b); }) + 1u;
+#pragma nounroll
+        while (n > 64u && high - low > 1u) {
+            const uint32_t between = low + ((high - low) >> 1), here = passing([&](uint64_t key) { return (uint32_t)(key >> 32) >= between; });
+            if (here >= top) { low = between; n = here; } else high = between;
+        }
+        bar = (uint64_t)low << 32;
+        uint64_t most = (uint64_t)high << 32;
+#pragma nounroll
+        for (int i = 0; i < 33 && n > 64u; ++i) {
+            const uint64_t between = bar + ((most - bar) >> 1);
+            const uint32_t here = passing([&](uint64_t key) { return key >= between; });
+            if (here >= top) { bar = between; n = here; } else most = between;
+        }
+    }
     uint32_t n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const bool in = mine[i] >= bar && mine[i] != 0ull;
         const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-        if (in) room[n + lanes_below(mask)] = mine[i];
+        if (in && n + lanes_below(mask) < 64u) room[n + lanes_below(mask)] = mine[i];
         n += (uint32_t)__popcll(mask);
     }
     wave_fence();
-    rank(room, n, top, put);
+    const uint64_t found[1] = {lane < n ? room[lane] : 0ull};
+    uint32_t place[1];
+    wave_fence();
+    places_of<1>(found, n, n, reinterpret_cast<uint32_t*>(room), place);
+    if (lane < n && place[0] < top) put(place[0], found[0]);
 }
 
 // A row to a wave.
@@ -503,7 +538,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
 // Joins the slices of a row: a wave to a row.
 extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, const float* parts,
                                                                 const uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
-    extern __shared__ __attribute__((aligned(16))) uint64_t room[];       // slices * top of them, and no less than 32 (256 bytes)
+    __shared__ __attribute__((aligned(16))) uint64_t room[64];
     const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
     const uint32_t lane = threadIdx.x;
     const uint64_t row = blockIdx.x;
@@ -628,7 +663,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
     const float own = g_log_prob && there ? g_log_prob[row] : 0.f, gh = g_entropy && there ? g_entropy[row] : 0.f;
     float total = own;
     if (there)
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
     // rows of few lanes: every score looks for itself among the alternatives. (2319 rows of 12, all of them alternatives: 7 us, a lane to an alternative some 27)
     const bool few = P.log2_lanes <= 2u;
@@ -680,7 +715,8 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
         const float x = logits[row * P.V + mine];
         float d = g_entropy == nullptr ? grad_of<false>(x, lse, total, gh, H) : grad_of<true>(x, lse, total, gh, H);
         if (mine == token) d += own;
-        for (uint32_t i = 0; i < P.top; ++i) if ((uint32_t)top_token[row * P.top + i] == mine) d += g_top[row * P.top + i];
+#pragma unroll 8
+        for (uint32_t i = 0; i < P.top; ++i) d += (uint32_t)top_token[row * P.top + i] == mine ? g_top[row * P.top + i] : 0.f;
         dx[row * P.V + mine] = d;
     }
 }

@@ -2363,14 +2363,20 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
 # ---------------------------------------------------------------- log probabilities of tokens (log_probs.hip)
 
 LOG_PROBS_AT_A_TIME = 256           #vectors of four scores that a wave takes at a time
-LOG_PROBS_SHORT     = 128           #vectors of rows that share a wave: four to a lane. With many alternatives half as many:
-LOG_PROBS_MANY      = 5             #(65536 rows of 500 and top of 1, 5, 20: 32, 53, 132 us, a wave to a row 43, 50, 70; rows of 250: 17, 27, 66, and 42, 49, 75)
-#few short rows too: an alternative is a turn of half a microsecond where they share one, and 700 waves more take as long
-#(208 rows of 19, top of 19: 13.3 us, a wave to a row 5.5; 8000 of 100, top of 20 and 6: 15.8 and 7.9, 12.3 and 9.4)
-LOG_PROBS_FEW       = 700
+LOG_PROBS_SHORT     = 128           #vectors of rows that can share a wave: four to a lane
 LOG_PROBS_WAVE      = 1024          #rows of up to this many vectors have a wave each where there are enough of them, longer ones a block
 LOG_PROBS_ROWS      = 1024          #enough rows not to be cut
 LOG_PROBS_MAX_KEYS  = 1024          #candidates of all slices of a row
+
+
+def _log_probs_share(rows: int, lanes: int, top: int) -> bool:
+    '''Whether short rows of `lanes` lanes share waves, by what launches take beyond 4 us, by measurement. There every alternative is a turn, of
+    half a microsecond or of the lanes' instructions; a wave to a row takes 2 us for alternatives, and a nanosecond for a row. (Measured, us: 65536
+    rows of 500 and top of 1, 5, 20: 32, 53, 132, a wave each 43, 50, 70; of 100 and 20: 38, 86; 8000 of 100 and 20: 15.8, 12.3, and 6: 7.9, 9.4;
+    208 rows of 19 and 19: 13.3, 5.5.)'''
+    if not top:
+        return True
+    return 1e-5 * rows * lanes + top * max(0.5, 2.6e-6 * rows * lanes) <= 2 + rows * (6.5e-4 + 1.2e-5 * top)
 
 
 def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch) -> tp.List[Launch]:
@@ -2383,8 +2389,8 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     if v >= 2**29 or rows * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4)
-    if vectors <= (LOG_PROBS_SHORT if top < LOG_PROBS_MANY else LOG_PROBS_SHORT // 2) and top <= 2 + rows // LOG_PROBS_FEW:
-        lanes = _pow2_at_least(_cdiv(vectors, 4))
+    lanes = _pow2_at_least(_cdiv(vectors, 4))
+    if vectors <= LOG_PROBS_SHORT and _log_probs_share(rows, lanes, top):
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
     if vectors <= LOG_PROBS_AT_A_TIME or (vectors <= LOG_PROBS_WAVE and rows >= LOG_PROBS_ROWS):
@@ -2402,8 +2408,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
                     written=written if slices == 1 else (5, 6))
     if slices == 1:
         return [launch]
-    return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, lds=max(8 * slices * top, BLOCK if top else 0),
-                           bytes_moved=4 * rows * (4 + 2 * top + slices * (4 + 2 * top)), written=written)]
+    return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=4 * rows * (4 + 2 * top + slices * (4 + 2 * top)), written=written)]
 
 
 def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Buffer, entropy: Buffer, g_log_prob, g_entropy, g_top, top_token,
