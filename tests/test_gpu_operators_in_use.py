@@ -329,3 +329,13 @@ def test_many_alternatives(rows, v, levels, top):
     bound = (64 + 16) * 2 * U + 6 * U * (30 if levels is None else 300 + 12)
     close(top_log_p, np.take_along_axis(logp, order, 1), bound)
     close(log_p, logp[np.arange(rows), t], bound)
+
+
+@pytest.mark.parametrize('n,c,groups', [(1, 1194, 1), (3, 2049, 1), (700, 1194, 1), (2100, 8192, 1), (5, 16384, 2), (2, 16384, 1), (1, 20000, 1), (9, 6141, 3), (1300, 4100, 1), (3, 32772, 1),
+                                        (4, 8193, 1)])
+@pytest.mark.parametrize('activation', [None, 'silu'])
+def test_layer_norm_of_wide_rows(n, c, groups, activation):
+    x, scale, shift, g = (normal(n + c, n, c) + normal(2, c)).astype(f32), normal(3, c), normal(4, c), normal(5, n, c)
+    got, expected, _ = both(norm_program(groups, activation), x, scale, shift, g)
+    for name, a, b, bound in zip(('y', 'dx', 'dscale', 'dshift'), got, expected, norm_bounds(x, scale, shift, g, groups, 1e-5, activation)):
+        close(a, b, bound, name)

@@ -71,7 +71,10 @@ def check_norm(n, s, groups, cg):
                 assert pieces * span >= cg > (pieces - 1) * span and spans == groups * pieces and (vec == 1 or cg % 4 == 0)
             per_group = max(span // cg, 1)
             room = launch.lds // 4
-            if plan.kind == 'held':
+            if plan.kind == 'wide':
+                assert s == 1 and span == cg and spans == groups and cg % vec == 0 and plan.k * threads * vec >= cg and launch.lds == 0
+                assert launch.grid[0] % groups == 0 and (gradient or launch.grid[0] == n * groups)
+            elif plan.kind == 'held':
                 assert V * P * M <= threads and P * plan.k >= s and P <= s
                 assert room >= 2 * M * P * span + 2 * per_group * M and M * s * c * 4 < 2**31
             elif plan.kind == 'rows':
@@ -140,7 +143,7 @@ def check_recurrence(b, t, c, gated=True, lengths=True):
 def everything():
     rng, names = random.Random(5), set()
     for n, s, groups, cg in ([(1, 1, 1, 1), (1, 49, 32, 16), (32, 3136, 32, 2), (64, 3136, 32, 8), (8191, 1, 16, 65), (5, 1, 1, 8191), (100, 1, 1, 8192), (2, 12, 5, 1001), (3, 7, 1, 4100),
-                              (70000, 1, 1, 4), (1, 1 << 20, 4, 16), (2, 5, 1024, 1), (9, 4, 3, 1), (4096, 1, 1, 4096), (7, 1, 1, 1023), (300, 2, 2, 6), (64, 3, 2, 2044)]
+                              (70000, 1, 1, 4), (1, 1 << 20, 4, 16), (2, 5, 1024, 1), (9, 4, 3, 1), (4096, 1, 1, 4096), (7, 1, 1, 1023), (300, 2, 2, 6), (64, 3, 2, 2044), (300, 1, 1, 8192), (300, 1, 2, 16380), (17, 1, 1, 32768), (300, 1, 1, 1194), (9, 1, 3, 2047), (5, 1, 1, 40000)]
                              + [(log_int(rng, 1, 4096), log_int(rng, 1, 12544), rng.choice((1, 2, 3, 8, 32)), log_int(rng, 1, 300)) for _ in range(300)]
                              + [(log_int(rng, 1, 20000), 1, rng.choice((1, 2, 3, 8, 16, 64)), log_int(rng, 1, 3000)) for _ in range(150)]):
         names.update(check_norm(n, s, groups, cg))

@@ -666,7 +666,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
 #pragma unroll 8
         for (uint32_t k = 0; k < P.top; ++k) total += g_top[row * P.top + k];
     // rows of few lanes: every score looks for itself among the alternatives. (2319 rows of 12, all of them alternatives: 7 us, a lane to an alternative some 27)
-    const bool few = P.log2_lanes <= 2u;
+    const bool few = P.log2_lanes <= 4u;
     const uint32_t from = at0 - lead;
     for (uint32_t q = q0 + lane; q < q1; q += lanes * NV) {
         f32x4 v[NV];

@@ -18,6 +18,9 @@
 //     lines, 512 or 1024 threads, 15.7-17).
 //   * group_norm_rows: samples of one position, several rows to a block (8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5; rows go
 //     through shared memory, because groups of 65 channels do not begin where vectors do; groups of 64 16.5 and 25).
+//   * group_norm_wide: samples of one position with wide groups (layer norms): a block to a group, several vectors to a thread, a sum over the block
+//     for the mean and one for the deviations from it. 8191 x 8192 82 us, 6.5 TB/s, its gradient 175, 4.6: every row waits for its two sums, with
+//     four waves to a SIMD; 8191 x 1021 16 and 25.
 //   * group_norm_stats / _apply: the others are cut along their positions. The first launch leaves mean and squared deviations of each
 //     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it). 64 x 56 x 56 x 256: 35 and 68 us, and
 //     71 and 107 for the gradient's two, all at 5.8-6.1 TB/s: bound by memory, and by reading everything twice. (Each launch
@@ -526,6 +529,117 @@ __device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, fl
     write_channel_sums(firsts, seconds, side, P.span, span.width, dshift_rows + to, dscale_rows + to);
 }
 
+// ---------------------------------------------------------------------------------------------- single positions, wide groups
+
+// Samples of one position with wide groups: a block to a group of a row, K vectors of it to a thread.
+
+// The sum of v over the block, in every thread. `parts`: 16 floats of shared memory for this sum alone.
+__device__ __forceinline__ float block_sum(float v, float* parts) {
+    v = add_lanes(v, 64u);
+    const uint32_t waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63u) == 0u) parts[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return add_lanes((threadIdx.x & 15u) < waves ? parts[threadIdx.x & 15u] : 0.f, 16u);
+}
+
+template <int VEC, int K>
+struct Wide {
+    uint32_t g, cg, lane0;                       // the group, its channels, this thread's first
+    __device__ Wide(const NormParams& P, uint32_t group) : g(group), cg(P.cg), lane0(threadIdx.x * VEC) {}
+    __device__ uint32_t channel(int i) const { return lane0 + (uint32_t)i * blockDim.x * VEC; }      // (whole vectors: VEC divides cg)
+    __device__ bool there(int i) const { return channel(i) < cg; }
+    __device__ uint32_t at(int i) const { return there(i) ? channel(i) * 4u : NOWHERE; }
+    __device__ __amdgpu_buffer_rsrc_t of_row(const float* p, const NormParams& P, uint32_t n) const { return make_rsrc(p + (uint64_t)n * P.C + (uint64_t)g * cg, cg * 4u); }
+    __device__ __amdgpu_buffer_rsrc_t of_channels(const float* p) const { return make_rsrc(p + (uint64_t)g * cg, cg * 4u); }
+};
+
+template <int VEC, int K>
+__device__ __forceinline__ void wide_body(float* y, float* means, float* rstds, const float* x, const float* scale, const float* shift, const NormParams& P) {
+    __shared__ float parts[2][16];
+    const uint32_t n = blockIdx.x / P.G;
+    const Wide<VEC, K> wide(P, blockIdx.x - n * P.G);
+    const __amdgpu_buffer_rsrc_t x_rsrc = wide.of_row(x, P, n);
+    float v[K][VEC], sum = 0.f, square = 0.f;
+#pragma unroll
+    for (int i = 0; i < K; ++i) load<VEC>(v[i], x_rsrc, wide.at(i));
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum += v[i][j];                     // (beyond the group: zeros)
+    const float inverse = 1.f / (float)wide.cg, mean = block_sum(sum, parts[0]) * inverse;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { const float d = wide.there(i) ? v[i][j] - mean : 0.f; square = __builtin_fmaf(d, d, square); }
+    const float rstd = 1.f / sqrtf(block_sum(square, parts[1]) * inverse + P.eps);
+    if (threadIdx.x == 0u) {
+        if (means) means[(uint64_t)n * P.G + wide.g] = mean;
+        if (rstds) rstds[(uint64_t)n * P.G + wide.g] = rstd;
+    }
+    if (y == nullptr) return;
+    const bool stream = streams_result(P.first);
+    const __amdgpu_buffer_rsrc_t y_rsrc = wide.of_row(y, P, n), gammas = wide.of_channels(scale), betas = wide.of_channels(shift);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        float gamma[VEC], beta[VEC];
+        load<VEC>(gamma, gammas, wide.at(i)); load<VEC>(beta, betas, wide.at(i));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf((v[i][j] - mean) * rstd, gamma[j], beta[j]), P.act);
+        store<VEC>(v[i], y_rsrc, wide.at(i), stream);
+    }
+}
+
+// Its gradient: a block takes one row after the other, gridDim.x / G rows apart, and keeps what they add to its channels' dscale and dshift.
+template <int VEC, int K>
+__device__ __forceinline__ void wide_grad_body(float* dx, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
+                                               const float* means, const float* rstds, const NormParams& P) {
+    __shared__ float parts[4][16];
+    const uint32_t row = blockIdx.x / P.G, rows = gridDim.x / P.G;
+    const Wide<VEC, K> wide(P, blockIdx.x - row * P.G);
+    const __amdgpu_buffer_rsrc_t gammas = wide.of_channels(scale), betas = wide.of_channels(shift);
+    const float inverse = 1.f / (float)wide.cg;
+    const bool stream = streams_result(P.first);
+    float d_total[K][VEC], dh_total[K][VEC];
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { d_total[i][j] = 0.f; dh_total[i][j] = 0.f; }
+    uint32_t turn = 0;                                                    // (two rows' sums in turn: a wave may be one row ahead of another)
+    for (uint32_t n = row; n < P.N; n += rows, turn ^= 2u) {
+        const __amdgpu_buffer_rsrc_t x_rsrc = wide.of_row(x, P, n), g_rsrc = wide.of_row(gs, P, n);
+        const float mean = means[(uint64_t)n * P.G + wide.g], rstd = rstds[(uint64_t)n * P.G + wide.g];
+        float v[K][VEC], d[K][VEC], a = 0.f, b = 0.f;
+#pragma unroll
+        for (int i = 0; i < K; ++i) { load<VEC>(v[i], x_rsrc, wide.at(i)); load<VEC>(d[i], g_rsrc, wide.at(i)); }
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            float gamma[VEC], beta[VEC];
+            load<VEC>(gamma, gammas, wide.at(i)); load<VEC>(beta, betas, wide.at(i));
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[i][j] = wide.there(i) ? (v[i][j] - mean) * rstd : 0.f;
+                d[i][j] = wide.there(i) ? act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
+                d_total[i][j] += d[i][j]; dh_total[i][j] = __builtin_fmaf(d[i][j], v[i][j], dh_total[i][j]);
+                d[i][j] *= gamma[j];
+                a += d[i][j]; b = __builtin_fmaf(d[i][j], v[i][j], b);
+            }
+        }
+        if (dx == nullptr) continue;
+        a = block_sum(a, parts[turn]) * inverse; b = block_sum(b, parts[turn + 1u]) * inverse;
+        const __amdgpu_buffer_rsrc_t dx_rsrc = wide.of_row(dx, P, n);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = rstd * (d[i][j] - a - v[i][j] * b);
+            store<VEC>(v[i], dx_rsrc, wide.at(i), stream);
+        }
+    }
+    const uint64_t to = (uint64_t)row * P.C;
+    const __amdgpu_buffer_rsrc_t first = wide.of_channels(dshift_rows + to), second = wide.of_channels(dscale_rows + to);
+#pragma unroll
+    for (int i = 0; i < K; ++i) { store<VEC>(d_total[i], first, wide.at(i), false); store<VEC>(dh_total[i], second, wide.at(i), false); }
+}
+
 // ---------------------------------------------------------------------------------------------- samples in chunks
 
 // Which chunk of which sample and span a block has.
@@ -819,10 +933,22 @@ __device__ __forceinline__ void grad_apply_body(float* dx, const float* partial,
     }
 HELD(4, 4, 256)  HELD(4, 16, 256)  HELD(4, 4, 1024)  HELD(4, 16, 1024)  HELD(1, 4, 256)  HELD(1, 16, 256)  HELD(1, 8, 1024)
 HELD_GRAD(4, 2, 256)  HELD_GRAD(4, 8, 256)  HELD_GRAD(4, 2, 1024)  HELD_GRAD(4, 4, 1024)  HELD_GRAD(1, 4, 256)  HELD_GRAD(1, 16, 256)  HELD_GRAD(1, 4, 1024)
-ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)  ROWS(4, 1, 1024)  ROWS(4, 2, 1024)
-ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)  ROWS(1, 1, 1024)  ROWS(1, 4, 1024)
-ROWS_GRAD(4, 1, 256)  ROWS_GRAD(4, 2, 256)  ROWS_GRAD(4, 1, 1024)  ROWS_GRAD(4, 2, 1024)
-ROWS_GRAD(1, 1, 256)  ROWS_GRAD(1, 4, 256)  ROWS_GRAD(1, 8, 256)  ROWS_GRAD(1, 1, 1024)  ROWS_GRAD(1, 4, 1024)
+ROWS(4, 1, 256)  ROWS(4, 2, 256)  ROWS(4, 4, 256)
+ROWS(1, 1, 256)  ROWS(1, 4, 256)  ROWS(1, 8, 256)
+ROWS_GRAD(4, 1, 256)  ROWS_GRAD(4, 2, 256)
+ROWS_GRAD(1, 1, 256)  ROWS_GRAD(1, 4, 256)  ROWS_GRAD(1, 8, 256)
+#define WIDE(VEC, K, THREADS)                                                                                                                                       \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_wide_v##VEC##_k##K##_t##THREADS(float* y, float* means, float* rstds, const float* x,          \
+                                                                                                     const float* scale, const float* shift, NormParams P) {        \
+        wide_body<VEC, K>(y, means, rstds, x, scale, shift, P);                                                                                                     \
+    }
+#define WIDE_GRAD(VEC, K, THREADS)                                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(THREADS) void group_norm_wide_grad_v##VEC##_k##K##_t##THREADS(float* dx, float* dscale_rows, float* dshift_rows,        \
+            const float* g, const float* x, const float* scale, const float* shift, const float* means, const float* rstds, NormParams P) {                         \
+        wide_grad_body<VEC, K>(dx, dscale_rows, dshift_rows, g, x, scale, shift, means, rstds, P);                                                                  \
+    }
+WIDE(4, 2, 256)  WIDE(4, 8, 256)  WIDE(4, 8, 1024)  WIDE(1, 4, 256)  WIDE(1, 8, 256)  WIDE(1, 8, 1024)
+WIDE_GRAD(4, 2, 256)  WIDE_GRAD(4, 4, 256)  WIDE_GRAD(4, 4, 512)  WIDE_GRAD(4, 4, 1024)  WIDE_GRAD(1, 4, 256)  WIDE_GRAD(1, 8, 256)  WIDE_GRAD(1, 8, 1024)
 CHUNKED(4)
 CHUNKED(1)
 

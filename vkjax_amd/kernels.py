@@ -2186,9 +2186,15 @@ def _f32_word(value: float) -> int:
 #(threads, positions per thread) of the kernels whose samples stay in registers, by channels per lane
 NORM_HELD      = {4: ((256, 4), (256, 16), (1024, 4), (1024, 16)), 1: ((256, 4), (256, 16), (1024, 8))}
 NORM_HELD_GRAD = {4: ((256, 2), (256, 8), (1024, 2), (1024, 4)), 1: ((256, 4), (256, 16), (1024, 4))}
-#(threads, rows per thread) of the kernels for samples of one position
-NORM_ROWS      = {4: ((256, 4), (256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
-NORM_ROWS_GRAD = {4: ((256, 2), (256, 1), (1024, 2), (1024, 1)), 1: ((256, 8), (256, 4), (256, 1), (1024, 4), (1024, 1))}
+#rows per thread of the kernels for samples of one position
+NORM_ROWS      = {4: (4, 2, 1), 1: (8, 4, 1)}
+NORM_ROWS_GRAD = {4: (2, 1), 1: (8, 4, 1)}
+#(threads, vectors per thread) of the kernels for samples of one position with wide groups
+NORM_WIDE      = {4: ((256, 2), (256, 8), (1024, 8)), 1: ((256, 4), (256, 8), (1024, 8))}
+NORM_WIDE_GRAD = {4: ((256, 2), (256, 4), (512, 4), (1024, 4)), 1: ((256, 4), (256, 8), (1024, 8))}
+#channels of a group beyond which it has a block, by whether they are whole vectors (8191 rows, us here and by several rows to a block: groups of 768, 1024, 2048,
+#4096: 14, 15.6, 21, 43, and 12, 15.3, 43, 99; of 301, 521, 901: 12, 13.5, 15, and 35, 28, 34)
+NORM_WIDE_FROM = {4: 1024, 1: 256}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_PARTIAL_LINES = 128 << 20      #bytes up to which samples are held in registers by less than whole lines (25 MB 15.5 us, in chunks 23; 205 MB 95-111, 100)
 NORM_HELD_BLOCKS = 256              #blocks that samples held in registers are shared out to
@@ -2196,7 +2202,7 @@ NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut f
 
 
 class NormPlan(tp.NamedTuple):
-    kind:    str                    #'rows', 'held' or 'chunked'
+    kind:    str                    #'rows', 'wide', 'held' or 'chunked'
     vec:     int
     threads: int
     k:       int                    #positions (held) or rows per thread
@@ -2240,20 +2246,26 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
 
 def _norm_rows(n: int, c: int, cg: int, variants, blocks_wanted: int) -> tp.Optional[NormPlan]:
     '''Samples of one position: a span that fills a block's lanes best, as many rows per thread as leave blocks_wanted blocks.'''
-    for threads in (BLOCK, 4 * BLOCK):
-        spans = []
-        for vec in ((4, 1) if c % 4 == 0 and cg > 1 else (1,)):
-            unit = int(np.lcm(cg, vec))
-            for many in range(1, min(c, threads * vec) // unit + 1):
-                V = many * unit // vec
-                #the share of the lanes that have channels, the last span's among them
-                spans.append((round(threads // V * (c // vec) / (_cdiv(c, many * unit) * threads), 2) * (1.0 if vec == 4 else 0.5), many * unit, vec, V))
-        if spans:
-            _, span, vec, V = max(spans)
-            side = threads // V
-            ks   = [k for t, k in variants[vec] if t == threads]
-            k    = next((k for k in ks if _cdiv(n, side * k) * _cdiv(c, span) >= blocks_wanted), ks[-1])
-            return NormPlan('rows', vec, threads, k, span, _cdiv(c, span), 1, V, 1, side * k, 1, 1) if side * k * c * 4 < 2**31 else None
+    spans = []
+    for vec in ((4, 1) if c % 4 == 0 and cg > 1 else (1,)):
+        unit = int(np.lcm(cg, vec))
+        for many in range(1, min(c, BLOCK * vec) // unit + 1):
+            V = many * unit // vec
+            #the share of the lanes that have channels, the last span's among them
+            spans.append((round(BLOCK // V * (c // vec) / (_cdiv(c, many * unit) * BLOCK), 2) * (1.0 if vec == 4 else 0.5), many * unit, vec, V))
+    if not spans:
+        return None
+    _, span, vec, V = max(spans)
+    side = BLOCK // V
+    k    = next((k for k in variants[vec] if _cdiv(n, side * k) * _cdiv(c, span) >= blocks_wanted), variants[vec][-1])
+    return NormPlan('rows', vec, BLOCK, k, span, _cdiv(c, span), 1, V, 1, side * k, 1, 1) if side * k * c * 4 < 2**31 else None
+
+
+def _norm_wide(n: int, c: int, cg: int, variants) -> tp.Optional[NormPlan]:
+    vec = 4 if cg % 4 == 0 else 1
+    for threads, k in variants[vec]:
+        if cg <= threads * k * vec:
+            return NormPlan('wide', vec, threads, k, cg, c // cg, 1, cg // vec, 1, 1, 1, 1)
     return None
 
 
@@ -2280,6 +2292,10 @@ def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
 
 def norm_plan(n: int, s: int, c: int, groups: int, gradient: bool) -> NormPlan:
     cg = c // groups
+    if s == 1 and cg > NORM_WIDE_FROM[4 if cg % 4 == 0 else 1]:
+        wide = _norm_wide(n, c, cg, NORM_WIDE_GRAD if gradient else NORM_WIDE)
+        if wide:
+            return wide
     if s == 1:
         return _norm_rows(n, c, cg, NORM_ROWS_GRAD if gradient else NORM_ROWS, NORM_BLOCKS) or _norm_chunked(n, s, c, cg)
     return _norm_held(n, s, c, cg, NORM_HELD_GRAD if gradient else NORM_HELD) or _norm_chunked(n, s, c, cg)
@@ -2318,7 +2334,8 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
     of_groups = max(plan.span // cg, 1)
     if plan.kind != 'chunked':
         return [_norm_launch(f'group_norm_{plan.kind}_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
-                             (2 if plan.kind == 'held' else 1) * plan.M * plan.P * plan.span + 2 * of_groups * plan.M, [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
+                             0 if plan.kind == 'wide' else (2 if plan.kind == 'held' else 1) * plan.M * plan.P * plan.span + 2 * of_groups * plan.M,
+                             [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
                              4 * (2 * x.size + 2 * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
     partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
     blocks  = n * plan.chunks * plan.spans
@@ -2344,7 +2361,8 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     dscale_rows, dshift_rows = (dscale or scratch((c,)), dshift or scratch((c,))) if rows == 1 else (scratch((rows, c)), scratch((rows, c)))
     if plan.kind != 'chunked':
         launches = [_norm_launch(f'group_norm_{plan.kind}_grad_v{plan.vec}_k{plan.k}_t{plan.threads}', rows * plan.spans, *args,
-                                 2 * plan.M * plan.P * plan.span + (4 if plan.kind == 'rows' else 2) * of_groups * plan.M, [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
+                                 0 if plan.kind == 'wide' else 2 * plan.M * plan.P * plan.span + (4 if plan.kind == 'rows' else 2) * of_groups * plan.M,
+                                 [(dx, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest,
                                  4 * (3 * x.size + 2 * rows * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
     else:
         partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
