@@ -2198,6 +2198,10 @@ NORM_WIDE_FROM = {4: 1024, 1: 256}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_PARTIAL_LINES = 128 << 20      #bytes up to which samples are held in registers by less than whole lines (25 MB 15.5 us, in chunks 23; 205 MB 95-111, 100)
 NORM_HELD_BLOCKS = 256              #blocks that samples held in registers are shared out to
+#values of a sample up to which fewer than 64 blocks hold samples (us so, and in chunks: 9 x 584 x 32 11.1, 12.3; 17 x 450 x 72 15.2, 11.6; 8 x 3128 x 20 13.9, 11.4)
+NORM_ALONE     = 7 << 12
+#parts that a block of the second launch joins, all groups' (1 x 16384 x 256 in 32 groups: 1024 chunks 89 us, 256 22, 128 24, 64 32; 4 x 4096 x 320: 26, 26, 22, 22)
+NORM_JOIN      = 4096
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
 
@@ -2238,7 +2242,7 @@ def _norm_held(n: int, s: int, c: int, cg: int, variants) -> tp.Optional[NormPla
                 blocks = _cdiv(n, M) * _cdiv(c, span)
                 if blocks < 64 and span > unit:
                     continue
-                if blocks < 64 and s * c > 1 << 16:
+                if blocks < 64 and s * c > NORM_ALONE:
                     return None
                 return NormPlan('held', vec, threads, k, span, _cdiv(c, span), 1, V, P, M, 1, s)
     return None
@@ -2285,6 +2289,7 @@ def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
     V = span // vec
     P = min(BLOCK // V, s)
     chunks = max(1, min(_cdiv(NORM_BLOCKS, n * spans), _cdiv(s, 4 * P)))
+    chunks = min(chunks, max(32, NORM_JOIN // (max(span // cg, 1) * pieces)))
     chunks = max(chunks, _cdiv(s * c * 4, 2**31 - 1))
     chunk  = _cdiv(s, chunks)
     return NormPlan('chunked', vec, BLOCK, 0, span, spans, pieces, V, P, 1, _cdiv(s, chunk), chunk)
