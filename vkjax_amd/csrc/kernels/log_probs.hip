@@ -185,13 +185,15 @@ struct Candidates {
         uint32_t place_a, place_b = 0u;
         wave_fence();
         if (count <= 64u) {
-            const uint64_t keys[1] = {a};
+            uint64_t keys[1];
             uint32_t places[1];
+            keys[0] = a;
             places_of<1>(keys, count, count, reinterpret_cast<uint32_t*>(entries), places);
             place_a = places[0];
         } else {
-            const uint64_t keys[2] = {a, b};
+            uint64_t keys[2];
             uint32_t places[2];
+            keys[0] = a; keys[1] = b;
             places_of<2>(keys, count, count, reinterpret_cast<uint32_t*>(entries), places);
             place_a = places[0]; place_b = places[1];
         }
