@@ -21,7 +21,7 @@
 // came to that, and the launch waited for it: 32 of 1024 x 4092 82 us instead of 23.) Places in the list are counted once, at the end.
 //
 // What bounds it: without alternatives, memory (65536 rows of 1000 39 us, 6.8 TB/s; 4096 of 32000 89 us, 5.9; its gradient 172 us, 5.9). With them, the
-// instructions that look for them: 5 of 65536 x 1000 54 us, 20 63; 20 of 4096 x 32000 118. (Rows a few to a wave, the next one's scores asked for ahead, need
+// instructions that look for them: 5 of 65536 x 1000 54 us, 20 63; 20 of 4096 x 32000 120. (Rows a few to a wave, the next one's scores asked for ahead, need
 // 131 registers or memory for them: 88 us instead of 54.) A few rows of 32000 are cut into slices of 4000, a block each, and joined by a second launch: 8 rows
 // with 20 alternatives 7.8 + 4.3 us, without 3.4 + 2.6: one wave's chain of steps each, which nothing else hides.
 #include "common.h"

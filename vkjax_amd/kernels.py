@@ -2202,6 +2202,9 @@ NORM_HELD_BLOCKS = 256              #blocks that samples held in registers are s
 NORM_ALONE     = 7 << 12
 #parts that a block of the second launch joins, all groups' (1 x 16384 x 256 in 32 groups: 1024 chunks 89 us, 256 22, 128 24, 64 32; 4 x 4096 x 320: 26, 26, 22, 22)
 NORM_JOIN      = 4096
+#blocks below which spans are no wider than whole groups, whole lines and 64 channels need be: there are more of them then, with less to join (1 x 16384 x 256 in
+#32 groups 24 us, so 19, with gradient 57, 44; 1 x 3528 x 448 in 64 20, 13 and 49, 32; 100 x 450 x 1000 in 20 with gradient 282, so 315)
+NORM_NARROW    = 4096
 NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
 
 
@@ -2276,8 +2279,12 @@ def _norm_wide(n: int, c: int, cg: int, variants) -> tp.Optional[NormPlan]:
 def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
     vec = 4 if c % 4 == 0 and (c <= 1024 or np.lcm(cg, 4) <= 1024 or cg % 4 == 0) else 1
     most, unit = BLOCK * vec, int(np.lcm(cg, vec))
+    lines = int(np.lcm(cg, NORM_FULL_LINE))
     if c <= most:
         span, spans, pieces = c, 1, 1
+        if lines < c and n * max(32, NORM_JOIN // (c // cg)) < NORM_NARROW:
+            span  = lines * max(1, 2 * NORM_FULL_LINE // lines)
+            spans = _cdiv(c, span)
     elif unit <= most:
         span = most // unit * unit
         spans, pieces = _cdiv(c, span), 1
