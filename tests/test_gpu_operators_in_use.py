@@ -339,3 +339,13 @@ def test_layer_norm_of_wide_rows(n, c, groups, activation):
     got, expected, _ = both(norm_program(groups, activation), x, scale, shift, g)
     for name, a, b, bound in zip(('y', 'dx', 'dscale', 'dshift'), got, expected, norm_bounds(x, scale, shift, g, groups, 1e-5, activation)):
         close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('shape,groups', [((1, 80, 80, 96), 12), ((1, 70, 70, 320), 32), ((1, 60, 61, 200), 25), ((2, 49, 72, 448), 64), ((1, 130, 127, 36), 9), ((3, 90, 41, 100), 4),
+                                          ((1, 5000, 1100), 1), ((2, 4000, 66), 66)])
+def test_group_norm_in_spans_of_few_groups(shape, groups):
+    c = shape[-1]
+    x, scale, shift, g = (normal(c, *shape) + normal(2, c)).astype(f32), normal(3, c), normal(4, c), normal(5, *shape)
+    got, expected, _ = both(norm_program(groups, 'silu'), x, scale, shift, g)
+    for name, a, b, bound in zip(('y', 'dx', 'dscale', 'dshift'), got, expected, norm_bounds(x, scale, shift, g, groups, 1e-5, 'silu')):
+        close(a, b, bound, name)

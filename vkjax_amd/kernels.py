@@ -2283,7 +2283,7 @@ def _norm_chunked(n: int, s: int, c: int, cg: int) -> NormPlan:
     if c <= most:
         span, spans, pieces = c, 1, 1
         if lines < c and n * max(32, NORM_JOIN // (c // cg)) < NORM_NARROW:
-            span  = lines * max(1, 2 * NORM_FULL_LINE // lines)
+            span  = min(c, lines * max(1, 2 * NORM_FULL_LINE // lines))
             spans = _cdiv(c, span)
     elif unit <= most:
         span = most // unit * unit
