@@ -429,3 +429,21 @@ def test_gradients_have_no_gradients_of_their_own():
         inner = lambda x: lax.add(mj.numpy.sum(mj.grad(lambda v: mj.numpy.sum(nn.group_norm(v, s, s, 3)))(x)), np.float32(0))
         return mj.grad(inner)(x)
     refused(NotImplementedError, twice, x, s)
+
+
+def test_gradients_through_nested_jits():
+    x, s, b = normal(1, 2, 6, 12), normal(2, 12), normal(3, 12)
+
+    def norm(*a):
+        return nn.group_norm(*a, 3, activation='silu')
+
+    def with_gradient(f):
+        def g(*a):
+            y, pullback = mj.vjp(f, *a)
+            return (y,) + pullback(y)
+        return g
+    run = lambda f: eval_closed_jaxpr(mj.make_jaxpr(f)(x, s, b), x, s, b)
+    plain = run(with_gradient(norm))
+    for other in (with_gradient(mj.jit(norm)), lambda *a: mj.jit(with_gradient(norm))(*a), lambda *a: mj.jit(with_gradient(lambda *q: mj.jit(norm)(*q)))(*a)):
+        assert all(np.array_equal(p, q) for p, q in zip(run(other), plain))
+        JaxprInterpreter(mj.make_jaxpr(other)(x, s, b), plan_only=True)

@@ -2197,7 +2197,8 @@ NORM_WIDE_GRAD = {4: ((256, 2), (256, 4), (512, 4), (1024, 4)), 1: ((256, 4), (2
 NORM_WIDE_FROM = {4: 1024, 1: 256}
 NORM_FULL_LINE = 32                 #channels that fill a line of 128 bytes
 NORM_PARTIAL_LINES = 128 << 20      #bytes up to which samples are held in registers by less than whole lines (25 MB 15.5 us, in chunks 23; 205 MB 95-111, 100)
-NORM_HELD_BLOCKS = 256              #blocks that samples held in registers are shared out to
+#blocks that samples held in registers are shared out to (us for 64, 256, 1024: 105 x 28 x 8 10.1, 4.9, 4.9; 1000 x 16 x 128 6.8, 6.8, 7.6)
+NORM_HELD_BLOCKS = 256
 #values of a sample up to which fewer than 64 blocks hold samples (us so, and in chunks: 9 x 584 x 32 11.1, 12.3; 17 x 450 x 72 15.2, 11.6; 8 x 3128 x 20 13.9, 11.4)
 NORM_ALONE     = 7 << 12
 #parts that a block of the second launch joins, all groups' (1 x 16384 x 256 in 32 groups: 1024 chunks 89 us, 256 22, 128 24, 64 32; 4 x 4096 x 320: 26, 26, 22, 22)
@@ -2205,7 +2206,8 @@ NORM_JOIN      = 4096
 #blocks below which spans are no wider than whole groups, whole lines and 64 channels need be: there are more of them then, with less to join (1 x 16384 x 256 in
 #32 groups 24 us, so 19, with gradient 57, 44; 1 x 3528 x 448 in 64 20, 13 and 49, 32; 100 x 450 x 1000 in 20 with gradient 282, so 315)
 NORM_NARROW    = 4096
-NORM_BLOCKS    = 1024               #blocks that the chunks of samples are cut for
+#blocks that the chunks of samples are cut for (us with gradient for 512, 1024, 2048: 64 x 3136 x 256 285, 280, 286; 4 x 4096 x 320 47, 50, 58; 16 x 10000 x 96 91, 92, 97)
+NORM_BLOCKS    = 1024
 
 
 class NormPlan(tp.NamedTuple):
@@ -2356,7 +2358,8 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
                          4 * (2 * x.size + 2 * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
 
 
-NORM_GRAD_ROWS = 1024               #blocks that the samples held in registers are shared out to, by the sums that each leaves
+#blocks that the samples held in registers are shared out to, by the sums that each leaves (300 x 49 x 512, us with gradient for 512, 1024, 2048: 53, 44, 47)
+NORM_GRAD_ROWS = 1024
 
 
 def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shift: Buffer, mean: Buffer, rstd: Buffer, groups: int, eps: float,
