@@ -349,3 +349,17 @@ def test_group_norm_in_spans_of_few_groups(shape, groups):
     got, expected, _ = both(norm_program(groups, 'silu'), x, scale, shift, g)
     for name, a, b, bound in zip(('y', 'dx', 'dscale', 'dshift'), got, expected, norm_bounds(x, scale, shift, g, groups, 1e-5, 'silu')):
         close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('name,f,args', CASES, ids=[c[0] for c in CASES])
+def test_profiled_and_with_every_value_returned(name, f, args):
+    expected = mj.tree_leaves(vkjax_amd.wrap(f, frontend='minijax')(*args))
+    outs, info = vkjax_amd.wrap(f, frontend='minijax', profiling=True)(*args)
+    same(outs, expected)
+    assert info
+    closed = mj.make_jaxpr(f)(*args)
+    outs, values = JaxprInterpreter(closed, reuse_buffers=False).run(*args, return_all=True)
+    same(outs, expected)
+    #every result of the operators' equations that something reads
+    results = [v for eqn in closed.jaxpr.eqns if eqn.primitive.name in ('group_norm', 'token_log_probs', 'linear_recurrence') for v in eqn.outvars]
+    assert results and all(np.isfinite(np.asarray(values[v], np.float64)).any() for v in results if v in values)
