@@ -1,0 +1,33 @@
+'''Launches of group norms, log probabilities and recurrences at the largest sizes that their kernels address, as they are planned (nothing is
+allocated).'''
+import numpy as np
+import pytest
+
+from tests.test_operator_plans import buffer, check_recurrence
+from vkjax_amd import kernels as K
+
+
+# ------------------------------------------------------------------ recurrences: what a tile's descriptor covers
+
+@pytest.mark.parametrize('b,t,c', [(1, 1, 2**29 - 4), (1, 1, 2**29 - 1), (2, 1, 2**28 - 2), (1, 4, 2**27 - 3), (1, 4, 2**27 - 4), (3, 2, 2**28 - 4), (1, 16, 2**25 - 8), (1, 300, 2**21 - 4),
+                                   (1, 2000, 2**21 - 5)])
+@pytest.mark.parametrize('gradient', [False, True])
+def test_a_recurrences_tile_ends_before_the_place_of_lanes_without_an_element(b, t, c, gradient):
+    '''Lanes without an element load and store at offset 2^31 of their tile's descriptor, which has to be behind its end.'''
+    x, state = buffer(b, t, c), buffer(b, c)
+    zeroed = lambda n, use: buffer(n, dtype=np.uint32)
+    try:
+        if gradient:
+            launch, = K.linear_recurrence_grad(x, x, state, x, x, x, state, None, x, state, True, False, zeroed)
+        else:
+            launch, = K.linear_recurrence(x, state, x, x, state, None, True, False, zeroed)
+    except NotImplementedError:
+        return
+    _, T, C, cstrips, strips, tiles, lines, of_each, log2_w, _ = np.frombuffer(launch.params, np.uint32).astype(np.int64)
+    vec, steps = 4 if '_v4' in launch.kernel else 1, int(launch.kernel.split('_l')[1].split('_')[0])
+    assert ((256 >> log2_w) * steps * C + (vec << log2_w)) * 4 < 2**31
+
+
+def test_recurrences_below_that_are_planned():
+    for b, t, c in ((1, 1, 2**28), (1, 4, 2**26), (1, 300, 2**18)):
+        assert list(check_recurrence(b, t, c))

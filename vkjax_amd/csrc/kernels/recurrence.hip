@@ -121,9 +121,10 @@ struct Tile {
     __device__ bool valid(uint32_t i) const { return group * L + i < n && c0 + col * VEC < C; }
     __device__ bool inside(uint32_t i) const { return valid(i) && tlow + row(i) < length; }
     __device__ uint32_t at(uint32_t i, bool take) const { return take ? (row(i) * C + col * VEC) * 4u : NOWHERE; }
-    // a descriptor of the tile's part of an array [B, T, C], `shift` steps away (nothing where the array is null)
+    // a descriptor of the tile's part of an array [B, T, C], `shift` steps away (nothing where the array is null): it ends behind the last
+    // step's channels, in front of NOWHERE
     __device__ __amdgpu_buffer_rsrc_t rsrc(const float* p, int shift = 0) const {
-        return make_rsrc(p + (((int64_t)b * T + tlow + shift) * C + c0), p ? (n * C + min(C - c0, W * VEC)) * 4u : 0u);
+        return make_rsrc(p + (((int64_t)b * T + tlow + shift) * C + c0), p ? ((n - 1u) * C + min(C - c0, W * VEC)) * 4u : 0u);
     }
     // the same of an array [B, C]; its element of this thread
     __device__ __amdgpu_buffer_rsrc_t state_rsrc(const float* p) const { return make_rsrc(p + ((int64_t)b * C + c0), p ? min(C - c0, W * VEC) * 4u : 0u); }

@@ -2519,7 +2519,8 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays
     _, steps, lanes, tiles = best
     cstrips = _cdiv(channels, lanes * vec)
     tiling = RecurrenceTiling(vec, steps, lanes, cstrips, batch * cstrips, tiles)
-    if _recurrence_lines(tiling)[2] * RECURRENCE_THREADS >= 2**32 or steps * (RECURRENCE_THREADS // lanes) * channels >= 2**29:
+    #(lanes without an element are sent 2 GiB behind their tile's first one, where its descriptor has to have ended)
+    if _recurrence_lines(tiling)[2] * RECURRENCE_THREADS >= 2**32 or 4 * (steps * (RECURRENCE_THREADS // lanes) * channels + lanes * vec) >= 2**31:
         raise NotImplementedError(f'a recurrence over {channels} channels in {batch} sequences of {time} steps')
     return tiling
 
