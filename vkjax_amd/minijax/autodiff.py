@@ -434,7 +434,13 @@ class _Replayed:
                 continue
             operands = [value_of(v) for v in eqn.invars]
             if name in _CALL_PARAMS:
-                #a custom derivative rule (single result): rule(cotangent, result, *arguments)
+                #a custom derivative rule (single result): rule(cotangent, result, *arguments). In front of the arguments stands
+                #what the function closes over, which the rule says nothing about
+                n_consts = eqn.params.get('num_consts', 0)
+                if any(id(c) in active for c in operands[:n_consts]):
+                    raise NotImplementedError('a function with a derivative rule of its own closes over a value that is '
+                                              'differentiated; pass it as an argument instead')
+                operands = operands[n_consts:]
                 in_cts = eqn.params['jvp_jaxpr_thunk'](_materialize(gs[0], outs_now[0]), outs_now[0], *operands)
             else:
                 if name not in RULES:

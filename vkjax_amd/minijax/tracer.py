@@ -310,12 +310,14 @@ def make_jaxpr(fun: tp.Callable, static_argnums: tp.Iterable[int] = (), return_s
 
 def _call_nested(fun, primitive_name: str, jaxpr_param: str, extra_params: dict, closed: bool, args):
     '''Trace `fun` into an inner jaxpr and emit one call equation that carries it.
-    Constants the inner function closes over become leading arguments of the call.'''
+    Constants the inner function closes over become leading arguments of the call (`num_consts` of them, where the parameters tell).'''
     leaves, in_tree = tree_util.tree_flatten(tuple(args))
     in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, leaves)]
     jaxpr, consts, out_tree, out_avals = _trace_to_jaxpr(fun, in_avals, in_tree, {}, len(args))
     inner = core.Jaxpr([], list(jaxpr.constvars) + list(jaxpr.invars), jaxpr.outvars, jaxpr.eqns)
     params = dict(extra_params)
+    if 'num_consts' in params:
+        params['num_consts'] = len(consts)
     params[jaxpr_param] = core.ClosedJaxpr(inner, []) if closed else inner
     outs = emit(primitive_name, list(consts) + list(leaves), out_avals, params, multiple_results=True)
     return tree_util.tree_unflatten(out_tree, outs)
@@ -336,7 +338,8 @@ def custom_jvp(fun: tp.Callable):
     reference: vkjax/ops.py:246-260). A derivative rule can be attached with `.defvjp(rule)`,
     `rule(cotangent, result, *arguments) -> cotangents of the arguments`; reverse-mode
     differentiation then uses it instead of differentiating the body (the entry `jvp_jaxpr_thunk`
-    of the equation carries it; backends ignore that entry).'''
+    of the equation carries it; backends ignore that entry). What the function closes over is no argument:
+    the rule does not see it, and has no cotangent for it.'''
     def wrapped(*args):
         params = dict(num_consts=0, jvp_jaxpr_thunk=wrapped.vjp_rule)
         return _call_nested(fun, 'custom_jvp_call_jaxpr', 'fun_jaxpr', params, closed=True, args=args)
