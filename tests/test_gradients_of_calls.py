@@ -60,3 +60,43 @@ def test_what_a_function_with_a_rule_closes_over_has_no_gradient_of_it():
     #without a rule the function is differentiated like any other
     d, = evaluate(lambda x, w: mj.grad(lambda q: jnp.sum(mj.custom_jvp(lambda a: a * q)(x)))(w), X, W)
     assert np.array_equal(d, X)
+
+
+# ------------------------------------------------------------------ one value in several places
+
+def test_gradients_of_one_value_in_two_places():
+    '''f(a, b) = a^2 b^3 at a = b = x: 2 x^4 and 3 x^4.'''
+    f = lambda a, b: jnp.sum(a * a * b * b * b)
+    first, = evaluate(lambda x: mj.grad(f)(x, x), X)
+    second, = evaluate(lambda x: mj.grad(f, argnums=1)(x, x), X)
+    both = evaluate(lambda x: mj.grad(f, argnums=(0, 1))(x, x), X)
+    value, *of_leaves = evaluate(lambda x: mj.value_and_grad(lambda p: f(*p))([x, x]), X)
+    assert np.array_equal(first, 2 * X ** 4) and np.array_equal(second, 3 * X ** 4) and value == (X ** 5).sum()
+    for a, b in (both, of_leaves):
+        assert np.array_equal(a, first) and np.array_equal(b, second)
+
+
+@pytest.mark.parametrize('make', [lambda: np.array([1, 2, 3], f32), lambda: f32(3), lambda: 3.0], ids=['array', 'scalar', 'python'])
+def test_gradients_of_one_constant_in_two_places(make):
+    c = make()
+
+    def f(y):
+        return mj.grad(lambda a, b: jnp.sum(a * a * b * y), argnums=(0, 1))(c, c) + (mj.vjp(lambda a, b: jnp.sum(a * a * b * y), c, c)[1](f32(1)),)
+    da, db, (va, vb) = mj.tree_unflatten(mj.tree_structure((0, 0, (0, 0))), evaluate(f, X))
+    total = (lambda v: v) if np.ndim(c) else np.sum
+    assert np.array_equal(da, total(2 * c * c * X)) and np.array_equal(db, total(c * c * X)) and np.array_equal(va, da) and np.array_equal(vb, db)
+
+
+def test_a_constant_that_is_an_argument_and_closed_over():
+    c = X.copy()
+    d, pulled = evaluate(lambda y: (mj.grad(lambda a: jnp.sum(a * c * y))(c), mj.vjp(lambda a: a * c * y, c)[1](y)[0]), W)
+    assert np.array_equal(d, c * W) and np.array_equal(pulled, c * W * W)
+
+
+def test_a_recurrence_over_one_array_as_gate_and_as_input():
+    x, g = np.random.default_rng(0).standard_normal((2, 5, 3)).astype(f32), np.random.default_rng(1).standard_normal((2, 5, 3)).astype(f32)
+    f = lambda gate, x, g: mj.grad(lambda p, q: jnp.sum(nn.gated_recurrence(p, q)[0] * g), argnums=(0, 1))(gate, x)
+    apart, together = evaluate(f, x, x, g), evaluate(lambda x, g: f(x, x, g), x, g)
+    assert all(np.array_equal(a, b) for a, b in zip(apart, together)) and not np.array_equal(*apart)
+    through_vjp = evaluate(lambda x, g: mj.vjp(lambda p, q: nn.gated_recurrence(p, q)[0], x, x)[1](g), x, g)
+    assert all(np.array_equal(a, b) for a, b in zip(apart, through_vjp))

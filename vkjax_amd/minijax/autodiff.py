@@ -390,13 +390,12 @@ def _replay(jaxpr, consts, inputs, env, order):
 
 class _Replayed:
     '''A function's equations in the enclosing trace, and what its backward pass needs of them.'''
-    def __init__(self, fun, args, wrt, distinct=False):
+    def __init__(self, fun, args, wrt):
         current_trace()
-        self.leaves, in_tree = tree_util.tree_flatten(tuple(args))
-        if distinct:
-            #values are told apart by identity: one that is passed twice has a share of the gradient in each place
-            self.leaves = [Tracer(a._trace, a._var) if isinstance(a, Tracer) else np.array(a, dtype_of(a)[0]) for a in self.leaves]
-        in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, self.leaves)]
+        leaves, in_tree = tree_util.tree_flatten(tuple(args))
+        in_avals = [core.ShapedArray(a.shape, a.dtype) for a in map(_abstractify, leaves)]
+        #values are told apart by identity: one that is passed twice, or closed over too, has a share of the gradient in each place
+        self.leaves = [Tracer(a._trace, a._var) if isinstance(a, Tracer) else np.asarray(a, dtype_of(a)[0]).view() for a in leaves]
         jaxpr, consts, out_tree, _ = _trace_to_jaxpr(fun, in_avals, in_tree, {}, len(args))
         self.env, self.order = {}, []
         outs        = _replay(jaxpr, consts, self.leaves, self.env, self.order)
@@ -486,7 +485,7 @@ def vjp(fun: tp.Callable, *primals, has_aux: bool = False):
     '''`(fun(*primals), pullback)`: pullback(cotangents), of the structure and shapes of the result, returns the tuple of the
     primals' cotangents. With `has_aux` fun returns (result, aux), of which only the result is differentiated, and
     (result, pullback, aux) comes back. Must be called while tracing; traced values that fun closes over are constants to it.'''
-    replayed = _Replayed(fun, primals, tuple(range(len(primals))), distinct=True)
+    replayed = _Replayed(fun, primals, tuple(range(len(primals))))
     result, aux = replayed.result if has_aux else (replayed.result, None)
     outs, structure = tree_util.tree_flatten(result)
     for o in outs:
