@@ -100,3 +100,14 @@ def test_a_recurrence_over_one_array_as_gate_and_as_input():
     assert all(np.array_equal(a, b) for a, b in zip(apart, together)) and not np.array_equal(*apart)
     through_vjp = evaluate(lambda x, g: mj.vjp(lambda p, q: nn.gated_recurrence(p, q)[0], x, x)[1](g), x, g)
     assert all(np.array_equal(a, b) for a, b in zip(apart, through_vjp))
+
+
+# ------------------------------------------------------------------ functions that hand an argument on
+
+@pytest.mark.parametrize('f', [lambda a: a, lambda a: mj.jit(lambda b: b)(a)], ids=['itself', 'through a call'])
+def test_a_rule_of_a_function_that_returns_its_argument(f):
+    '''A gradient that is turned round or scaled on its way back: the function is the identity.'''
+    h = with_rule(f, lambda g, y, a: [g * f32(-3)])
+    d, twice, beside, constant = evaluate(lambda x: (mj.grad(lambda a: jnp.sum(h(a)))(x), mj.grad(lambda a: jnp.sum(h(h(a)) * a))(x),
+                                                     mj.grad(lambda a: jnp.sum(h(a) + a))(x), mj.grad(lambda a: jnp.sum(h(a)))(W)), X)
+    assert (d == -3).all() and np.array_equal(twice, 9 * X + X) and (beside == -2).all() and (constant == -3).all()

@@ -378,6 +378,8 @@ def _replay(jaxpr, consts, inputs, env, order):
             outs  = _replay(getattr(inner, 'jaxpr', inner), getattr(inner, 'consts', []), [read(v) for v in eqn.invars], env,
                             order if not callable(rule) else [])
             if callable(rule):
+                #(an argument that the function hands on is another value behind it: its cotangent goes through the rule)
+                outs = [Tracer(o._trace, o._var) if isinstance(o, Tracer) else np.asarray(o).view() for o in outs]
                 order.append(eqn)
         else:
             outs = emit(name, [read(v) for v in eqn.invars], [v.aval for v in eqn.outvars], eqn.params, eqn.primitive.multiple_results)
