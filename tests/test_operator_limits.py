@@ -3,7 +3,7 @@ allocated).'''
 import numpy as np
 import pytest
 
-from tests.test_operator_plans import buffer, check_recurrence
+from tests.test_operator_plans import buffer, check_recurrence, norm_launches
 from vkjax_amd import kernels as K
 
 
@@ -31,3 +31,18 @@ def test_a_recurrences_tile_ends_before_the_place_of_lanes_without_an_element(b,
 def test_recurrences_below_that_are_planned():
     for b, t, c in ((1, 1, 2**28), (1, 4, 2**26), (1, 300, 2**18)):
         assert list(check_recurrence(b, t, c))
+
+
+# ------------------------------------------------------------------ group norm of single positions: where pairs lie in shared memory
+
+@pytest.mark.parametrize('n,groups,cg', [(1, 1, 3), (1, 1, 5), (5, 1, 255), (3000, 1, 255), (7, 3, 85), (1, 5, 51), (2, 1, 4), (8191, 16, 65)])
+def test_statistics_of_rows_lie_at_even_words(n, groups, cg):
+    '''The rows' values, and behind them, from an even word on, mean and 1 / deviation of every row and group.'''
+    forward, backward = norm_launches(n, 1, groups, cg)
+    plan = K.norm_plan(n, 1, groups * cg, groups, False)
+    assert plan.kind == 'rows'
+    values, pairs = plan.M * plan.span, plan.M * plan.span // cg
+    assert forward[0].lds == 4 * (values + values % 2 + 2 * pairs)
+    #the gradient has two arrays of values in front of them: an even number of words
+    plan = K.norm_plan(n, 1, groups * cg, groups, True)
+    assert backward[0].lds == 4 * (2 * plan.M * plan.span + 4 * plan.M * plan.span // cg)

@@ -416,7 +416,7 @@ __device__ __forceinline__ void rows_body(float* y, float* means, float* rstds, 
         load<VEC>(beta, b, span.owns() ? span.col * VEC * 4u : NOWHERE);
     }
     float* const values = room;
-    f32x2* const stats_of = reinterpret_cast<f32x2*>(room + P.M * P.span);
+    f32x2* const stats_of = reinterpret_cast<f32x2*>(room + ((P.M * P.span + 1u) & ~1u));      // (pairs lie at even words)
 #pragma unroll
     for (int i = 0; i < K; ++i) if (use) put<VEC>(values + (span.p + i * side) * P.span + span.col * VEC, v[i]);
     __syncthreads();

@@ -2347,8 +2347,10 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
     args  = (plan, shape, groups, eps, activation)
     of_groups = max(plan.span // cg, 1)
     if plan.kind != 'chunked':
+        #(of rows: the values, and from the next even word on a pair for each row and group)
+        values = plan.M * plan.P * plan.span
         return [_norm_launch(f'group_norm_{plan.kind}_v{plan.vec}_k{plan.k}_t{plan.threads}', _cdiv(n, plan.M) * plan.spans, *args,
-                             0 if plan.kind == 'wide' else (2 if plan.kind == 'held' else 1) * plan.M * plan.P * plan.span + 2 * of_groups * plan.M,
+                             0 if plan.kind == 'wide' else (2 * values if plan.kind == 'held' else _cdiv(values, 2) * 2) + 2 * of_groups * plan.M,
                              [(b, 0) for b in (y, mean, rstd, x, scale, shift)],
                              4 * (2 * x.size + 2 * c), streamable=_norm_whole_lines(plan, c), written=(0, 1, 2))]
     partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
