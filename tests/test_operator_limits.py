@@ -1,10 +1,14 @@
 '''Launches of group norms, log probabilities and recurrences at the largest sizes that their kernels address, as they are planned (nothing is
 allocated).'''
+import os
+
 import numpy as np
 import pytest
 
-from tests.test_operator_plans import buffer, check_recurrence, norm_launches
+from tests.test_gpu_operator_kernels import NORM_SIZES, RECURRENCE_SIZES
+from tests.test_operator_plans import TOOLS, buffer, check_recurrence, kernels_of, norm_launches
 from vkjax_amd import kernels as K
+from vkjax_amd.csrc import build
 
 
 # ------------------------------------------------------------------ recurrences: what a tile's descriptor covers
@@ -46,3 +50,13 @@ def test_statistics_of_rows_lie_at_even_words(n, groups, cg):
     #the gradient has two arrays of values in front of them: an even number of words
     plan = K.norm_plan(n, 1, groups * cg, groups, True)
     assert backward[0].lds == 4 * (2 * plan.M * plan.span + 4 * plan.M * plan.span // cg)
+
+
+# ------------------------------------------------------------------ what the tests on the GPU reach
+
+@pytest.mark.skipif(not (TOOLS and all(os.path.exists(build.hsaco_path(m)) for m in ('norm', 'recurrence'))), reason='no code object, or no tool to look into it')
+def test_every_kernel_is_run_on_the_gpu(tmp_path):
+    found = set(kernels_of('norm', tmp_path)) | set(kernels_of('recurrence', tmp_path))
+    launched = {launch.kernel for size in NORM_SIZES for launches in norm_launches(*size) for launch in launches}
+    launched |= {kernel for b, t, c in RECURRENCE_SIZES for gated in (False, True) for kernel in check_recurrence(b, t, c, gated, b > 1)}
+    assert found == launched, (found - launched, launched - found)
