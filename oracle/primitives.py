@@ -845,7 +845,7 @@ def _token_rows64(logits, tokens):
     return z, np.where(given, token, 0), given, log_sum, logp, np.exp(logp)
 
 
-def token_log_probs(logits, tokens, top):
+def token_log_probs(logits, tokens, top, rest=False):
     with np.errstate(**_EW_ERR):
         z, token, given, log_sum, logp, p = _token_rows64(logits, tokens)
         entropy = -np.where(p == 0, 0.0, p * logp).sum(axis=1)
@@ -858,11 +858,14 @@ def token_log_probs(logits, tokens, top):
             order = np.lexsort((np.broadcast_to(np.arange(z.shape[1]), z.shape), -z, ~np.isnan(z)), axis=1)[:, :top]
             outs += [np.where(given[:, None], np.take_along_axis(logp, order, 1), 0.0).reshape(shape + (top,)).astype(f32),
                      np.where(given[:, None], order, -1).reshape(shape + (top,)).astype(i32)]
+        if rest:
+            rounded = log_sum.astype(f32).astype(np.float64)
+            outs.append(rows(np.where(log_sum == -np.inf, 0.0, log_sum - rounded), 0.0))
         return tuple(outs)
 
 
-def token_log_probs_grad(logits, tokens, log_sum, entropy, *cotangents, has_log_probs, has_entropy, top):
-    cotangents = [np.asarray(c) for c in cotangents]
+def token_log_probs_grad(logits, tokens, log_sum, entropy, *cotangents, has_log_probs, has_entropy, top, has_rest=False):
+    cotangents = [np.asarray(c) for c in cotangents[int(has_rest):]]
     with np.errstate(**_EW_ERR):
         z, token, given, _, logp, p = _token_rows64(logits, tokens)
         rows = np.arange(len(z))

@@ -3,11 +3,12 @@ in 64 bits. Bounds are those of the operators' own tests.'''
 import numpy as np
 import pytest
 
-from tests.test_gpu_operators import both, check_recurrence, close, norm_bounds, norm_program, recurrence_inputs
+from tests.test_gpu_operators import D, U, both, check_recurrence, close, norm_bounds, norm_program, probs_program, recurrence_inputs
 from tests.test_operators import normal
+from vkjax_amd import minijax as mj
 
 pytestmark = pytest.mark.gpu
-f32 = np.float32
+nn, f32 = mj.nn, np.float32
 
 
 def check_norm(shape, groups, activation):
@@ -54,3 +55,58 @@ RECURRENCE_SIZES = [(3, 1, 8), (3, 1, 7), (2, 4, 260), (2, 4, 77), (2, 5, 1000),
 def test_every_recurrence_kernel(b, t, c, gated):
     print(f'recurrence {b} x {t} x {c}, gated {gated}', flush=True)
     check_recurrence(recurrence_inputs(b, t, c, gated, True, b > 1, seed=b + t + c), gated, bool(t % 2))
+
+
+# ------------------------------------------------------------------ the gradient of log probabilities at scores far from zero
+
+@pytest.mark.parametrize('rows,v', [(6, 40), (700, 37), (9, 900), (1200, 3500), (5, 9001), (3, 60001)])
+@pytest.mark.parametrize('offset', [0.0, 100.0, -3e4, 3e4, 1e6])
+def test_log_probs_gradient_does_not_go_by_a_rounded_log_of_the_sum(rows, v, offset):
+    print(f'gradient of log probabilities {rows} x {v} around {offset}', flush=True)
+    rng = np.random.default_rng(rows + v)
+    z, t = (normal(1, rows, v, scale=2.5) + f32(offset)).astype(f32), rng.integers(0, v, rows).astype(np.int32)
+    t[1] = -1
+    g = [np.abs(normal(11, rows)) + f32(0.5), normal(12, rows), normal(13, rows, 3)]
+    got, expected, _ = both(probs_program(3), z, t, *g)
+    z64 = z.astype(np.float64)
+    best = z64.max(axis=1, keepdims=True)
+    e = np.exp(z64 - best)
+    s = e.sum(axis=1, keepdims=True)
+    p, spread, log_s = e / s, best - z64, np.log(s)
+    #log p = (x - (the log of the sum, rounded)) - its rest: their sum is m + log s to the last bit, log s off by the sum's error (every term by 4 u and
+    #by the roundings of its exponent, then added up) and the logarithm's 2 u; the two differences are rounded. Nothing of that goes with |m|.
+    mean_spread = (p * spread).sum(axis=1, keepdims=True)
+    e_s = (D + 6) * U + 3 * U * mean_spread
+    logp = spread + log_s
+    e_lp = e_s + 2 * U * log_s + 2 * U * (logp + log_s + 1)
+    mean_square = (p * spread ** 2).sum(axis=1, keepdims=True)
+    e_h = e_s * (1 + 2 * mean_spread) + ((D + 8) * mean_spread + 3 * mean_square) * U + 8 * U * (log_s + mean_spread + 1)
+    e_p = p * (e_lp + (3 * logp + 8) * U)
+    total, gh, entropy = sum(np.abs(a.reshape(rows, -1)).sum(axis=1, keepdims=True) for a in g), np.abs(g[1])[:, None], log_s + mean_spread
+    own = np.zeros_like(p)
+    np.put_along_axis(own, np.maximum(t, 0)[:, None], 1.0, 1)
+    for k in range(3):
+        np.put_along_axis(own, got[3][:, k:k + 1].clip(0).astype(np.int64), 1.0, 1)
+    e_d = e_p * (total + gh * (logp + entropy)) + p * (44 * U * total + gh * (e_lp + e_h + 4 * U * (logp + entropy))) + 8 * U * total * (own + p)
+    close(got[-1], expected[-1], e_d + 1e-37, 'gradient')
+    #cotangents of log probabilities alone: a row's gradient adds up to nothing, off by as much as its terms
+    (d,), _, _ = both(lambda z, t, g: mj.vjp(lambda v: nn.token_log_probs(v, t)[0], z)[1](g), z, t, g[0])
+    assert (np.abs(d.astype(np.float64).sum(axis=1)) <= (e_p * g[0][:, None] + 8 * U * p * g[0][:, None]).sum(axis=1) + 2 * U * g[0]).all()
+
+
+@pytest.mark.parametrize('v', [30, 2000, 40000])
+def test_log_probs_of_rows_that_hold_the_lowest_value_only(v):
+    '''A mask of the type's lowest value that leaves nothing: such rows have a distribution, the same for every score.'''
+    z = np.full((3, v), np.finfo(f32).min, f32)
+    z[1, 3] = 0.0
+    t, g = np.array([0, 3, v - 1], np.int32), np.ones(3, f32)
+    lp, entropy, d = both(lambda z, t, g: (lambda outs, pull: outs + pull((g, g)))(*mj.vjp(lambda q: nn.token_log_probs(q, t), z)), z, t, g)[0]
+    one = np.zeros(v)
+    close(lp, [-np.log(v), 0, -np.log(v)], 8 * U * np.log(v))
+    close(entropy, [np.log(v), 0, np.log(v)], 8 * U * np.log(v))
+    for row, token in ((0, 0), (2, v - 1)):
+        one[:] = 0
+        one[token] = 1
+        #(the entropy of equal probabilities has no gradient: what is left of it is log p + H, off by 16 u log v)
+        close(d[row], one - 1 / v, (24 * U * np.log(v) + 16 * U) / v + 2 * U * one)
+    assert not d[1].any()

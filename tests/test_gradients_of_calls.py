@@ -111,3 +111,37 @@ def test_a_rule_of_a_function_that_returns_its_argument(f):
     d, twice, beside, constant = evaluate(lambda x: (mj.grad(lambda a: jnp.sum(h(a)))(x), mj.grad(lambda a: jnp.sum(h(h(a)) * a))(x),
                                                      mj.grad(lambda a: jnp.sum(h(a) + a))(x), mj.grad(lambda a: jnp.sum(h(a)))(W)), X)
     assert (d == -3).all() and np.array_equal(twice, 9 * X + X) and (beside == -2).all() and (constant == -3).all()
+
+
+# ------------------------------------------------------------------ the log of the sum, and the rest of it
+
+def test_gradients_of_log_probabilities_have_the_log_of_the_sum_unrounded():
+    rng = np.random.default_rng(0)
+    z, t, g = (rng.standard_normal((5, 9)) * 2 + 1e4).astype(f32), np.array([0, 8, -1, 3, 9], np.int32), rng.standard_normal(5).astype(f32)
+    z[3] = -np.inf
+
+    def f(z, t, g):
+        inside = mj.jit(lambda v: nn.token_log_probs(v, t)[0])
+        return mj.vjp(inside, z)[1](g), mj.vjp(lambda v: nn.token_log_probs(v, t, 2)[2], z)[1](jnp.broadcast_to(jnp.reshape(g, (5, 1)), (5, 2)))
+
+    closed = mj.make_jaxpr(f)(z, t, g)
+    made  = [e.outvars[-1] for e in closed.jaxpr.eqns if e.primitive.name == 'token_log_probs']
+    grads = [e for e in closed.jaxpr.eqns if e.primitive.name == 'token_log_probs_grad']
+    assert len(made) == len(grads) == 2 and all(e.params['has_rest'] and e.invars[4] is rest for e, rest in zip(grads, made))
+    lp, entropy, log_sum, top_lp, top, rest = evaluate(lambda z, t: lax.token_log_probs(z, t, 2, with_rest=True), z, t)
+    assert all(np.array_equal(a, b) for a, b in zip((lp, entropy, log_sum, top_lp, top), evaluate(lambda z, t: lax.token_log_probs(z, t, 2), z, t)))
+    z64 = z[[0, 1]].astype(np.float64)
+    exact = z64.max(1) + np.log(np.exp(z64 - z64.max(1, keepdims=True)).sum(1))
+    assert not rest[2:].any() and np.allclose(log_sum[:2].astype(np.float64) + rest[:2], exact, rtol=0, atol=1e-10) and rest[:2].all()
+    #by itself, with the rest and without it
+    alone = evaluate(lambda *a: lax.token_log_probs_grad(*a[:5], log_sum_rest=a[5]), z, t, log_sum, entropy, g, rest)[0]
+    assert np.array_equal(alone, evaluate(lax.token_log_probs_grad, z, t, log_sum, entropy, g)[0])
+
+
+def test_the_rest_of_the_log_of_the_sum_is_one_value_per_row():
+    z, t, row = np.zeros((3, 9), f32), np.zeros(3, np.int32), np.zeros(3, f32)
+    for bad in (row[:2], t, np.zeros((3, 1), f32)):
+        with pytest.raises(TypeError):
+            mj.make_jaxpr(lambda *a: lax.token_log_probs_grad(*a[:5], log_sum_rest=a[5]))(z, t, row, row, row, bad)
+    with pytest.raises(NotImplementedError):
+        mj.make_jaxpr(lambda z: mj.grad(lambda v: jnp.sum(lax.token_log_probs(v, t, 0, with_rest=True)[3]))(z))(z)

@@ -5,6 +5,9 @@
 //   lse = m + log s,  log p = x - lse,  H = -sum p log p = log s - w / s
 //   dx[v] = -p[v] (sum of the cotangents of log probabilities) - gH p[v] (log p[v] + H) + the cotangents of v's own log probabilities
 //
+// log p is the difference to the maximum less log s. What the gradient gets of a row is lse, rounded, and the rest that its rounding lost: at scores around
+// 10^4 half a step of lse would be 5 10^-4 of every p of the row, and where all of them are the type's lowest value lse alone is one of them, and p 1.
+//
 // A token outside [0, V) marks its row as padding: results are 0 (alternatives: token -1), the row's scores are not read. Scores of
 // -inf are masked: p = 0, and p log p counts as 0. Where every score of a row is -inf there is no distribution: log p = -inf, H = 0,
 // gradient 0. NaN and +inf make their row NaN by themselves (+inf - +inf).
@@ -70,6 +73,11 @@ struct Distribution {
         entropy = nothing ? 0.f : log_s - sums.w / sums.s;
     }
     __device__ __forceinline__ float log_sum() const { return nothing ? -INFINITY : m + log_s; }
+    // what the rounding of log_sum has lost, exactly (Knuth's sum of two numbers)
+    __device__ __forceinline__ float log_sum_rest() const {
+        const float sum = m + log_s, second = sum - m;
+        return nothing ? 0.f : (m - (sum - second)) + (log_s - second);
+    }
     __device__ __forceinline__ float log_prob(float x) const { return nothing ? -INFINITY : (x - m) - log_s; }
 };
 
@@ -303,13 +311,14 @@ struct Candidates {
     }
 };
 
-struct Results { float *log_prob, *entropy, *log_sum, *top_log_prob; int32_t* top_token; };
+struct Results { float *log_prob, *entropy, *log_sum, *top_log_prob; int32_t* top_token; float* log_sum_rest; };
 
 __device__ __forceinline__ void write_padding(const Results& to, uint64_t row, uint32_t lane, uint32_t lanes, uint32_t top) {
     if (lane == 0u) {
         if (to.log_prob) to.log_prob[row] = 0.f;
         if (to.entropy) to.entropy[row] = 0.f;
         if (to.log_sum) to.log_sum[row] = 0.f;
+        if (to.log_sum_rest) to.log_sum_rest[row] = 0.f;
     }
     for (uint32_t k = lane; k < top; k += lanes) {
         if (to.top_log_prob) to.top_log_prob[row * top + k] = 0.f;
@@ -320,6 +329,7 @@ __device__ __forceinline__ void write_sums(const Results& to, uint64_t row, cons
     if (to.log_prob) to.log_prob[row] = p.log_prob(score);
     if (to.entropy) to.entropy[row] = p.entropy;
     if (to.log_sum) to.log_sum[row] = p.log_sum();
+    if (to.log_sum_rest) to.log_sum_rest[row] = p.log_sum_rest();
 }
 __device__ __forceinline__ void write_alternative(const Results& to, uint64_t row, uint32_t top, uint32_t place, uint64_t key, const Distribution& p) {
     if (to.top_log_prob) to.top_log_prob[row * top + place] = p.log_prob(key_score((uint32_t)(key >> 32)));
@@ -463,18 +473,18 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
 }
 #define LOG_PROBS_WAVE(name, SINGLE)                                                                                                                     \
     extern "C" __global__ __launch_bounds__(256) void name(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,    \
-                                                           const float* logits, const uint32_t* tokens, LogProbsParams P) {                             \
-        wave_body<SINGLE>(Results{log_prob, entropy, log_sum, top_log_prob, top_token}, logits, tokens, P);                                             \
+                                                           float* log_sum_rest, const float* logits, const uint32_t* tokens, LogProbsParams P) {        \
+        wave_body<SINGLE>(Results{log_prob, entropy, log_sum, top_log_prob, top_token, log_sum_rest}, logits, tokens, P);                               \
     }
 LOG_PROBS_WAVE(log_probs_wave, true)
 LOG_PROBS_WAVE(log_probs_wave_long, false)
 
 // A row, or a slice of one, to a block of four waves. With slices: sums and candidates go to `parts` ([rows, slices, 4] floats: m, s, w) and
 // `keys` ([rows, top, slices]) for log_probs_join.
-extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, float* parts, uint64_t* keys,
-                                                                     const float* logits, const uint32_t* tokens, LogProbsParams P) {
+extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, float* log_sum_rest,
+                                                                     float* parts, uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
     constexpr uint32_t WAVES = 4;
-    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
+    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token, log_sum_rest};
     __shared__ __attribute__((aligned(16))) uint64_t lists[WAVES * LIST];
     __shared__ uint64_t all[WAVES * 32];
     __shared__ Sums of_wave[WAVES];
@@ -538,10 +548,10 @@ extern "C" __global__ __launch_bounds__(256, 4) void log_probs_block(float* log_
 }
 
 // Joins the slices of a row: a wave to a row.
-extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, const float* parts,
-                                                                const uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
+extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token, float* log_sum_rest,
+                                                                const float* parts, const uint64_t* keys, const float* logits, const uint32_t* tokens, LogProbsParams P) {
     __shared__ __attribute__((aligned(16))) uint64_t room[64];
-    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
+    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token, log_sum_rest};
     const uint32_t lane = threadIdx.x;
     const uint64_t row = blockIdx.x;
     const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
@@ -564,8 +574,8 @@ extern "C" __global__ __launch_bounds__(64) void log_probs_join(float* log_prob,
 
 // Short rows: 2^log2_lanes lanes to a row, four vectors to a lane, and several rows to a wave. The alternatives one by one.
 extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_prob, float* entropy, float* log_sum, float* top_log_prob, int32_t* top_token,
-                                                                  const float* logits, const uint32_t* tokens, LogProbsParams P) {
-    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token};
+                                                                  float* log_sum_rest, const float* logits, const uint32_t* tokens, LogProbsParams P) {
+    const Results to{log_prob, entropy, log_sum, top_log_prob, top_token, log_sum_rest};
     const uint32_t lanes = 1u << P.log2_lanes, lane = threadIdx.x & (lanes - 1u);
     const uint64_t row = ((uint64_t)blockIdx.x * 256u + threadIdx.x) >> P.log2_lanes;
     const bool there = row < P.rows;
@@ -638,8 +648,8 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_short(float* log_pro
 // What bounds it: memory, 4096 rows of 32000 (1.02 GB) 170 us, 6.0 TB/s; rows from the last one on, since the forward pass has left those in the
 // 256 MB behind the L2s (198 us from the first one on).
 template <bool ENTROPY>
-__device__ __forceinline__ float grad_of(float x, float lse, float total, float gh, float H) {
-    const float lp = x - lse;
+__device__ __forceinline__ float grad_of(float x, float lse, float rest, float total, float gh, float H) {
+    const float lp = (x - lse) - rest;
     // exp(lp): base 2, with the part of the exponent that its rounding loses
     const float t = lp * LOG2E, lost = __builtin_fmaf(lp, LOG2E, -t);
     float p = __builtin_amdgcn_exp2f(t);
@@ -648,8 +658,8 @@ __device__ __forceinline__ float grad_of(float x, float lse, float total, float 
     return p == 0.f ? 0.f : -p * d;
 }
 
-extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, const float* logits, const uint32_t* tokens, const float* log_sum, const float* entropy,
-                                                                 const float* g_log_prob, const float* g_entropy, const float* g_top, const int32_t* top_token, LogProbsParams P) {
+extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, const float* logits, const uint32_t* tokens, const float* log_sum, const float* log_sum_rest,
+                                                                 const float* entropy, const float* g_log_prob, const float* g_entropy, const float* g_top, const int32_t* top_token, LogProbsParams P) {
     const uint32_t lanes = 1u << P.log2_lanes, lane = threadIdx.x & (lanes - 1u), side = 256u >> P.log2_lanes;
     const uint32_t rows = without_stream_bit(P.first), block = gridDim.x - 1u - blockIdx.x, slice = block % P.slices;
     const bool stream = streams_result(P.first);
@@ -660,7 +670,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
     const uint32_t bytes = (((uint32_t)start0 & 3u) + (uint32_t)min((uint64_t)side, rows - row0) * P.V) * 4u;
     const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(logits + (start0 - (start0 & 3u)), bytes), d_rsrc = make_rsrc(dx + (start0 - (start0 & 3u)), bytes);
     const uint32_t token = there ? tokens[row] : 0xFFFFFFFFu;
-    const float lse = there ? log_sum[row] : 0.f, H = there ? entropy[row] : 0.f;
+    const float lse = there ? log_sum[row] : 0.f, rest = there && log_sum_rest ? log_sum_rest[row] : 0.f, H = there ? entropy[row] : 0.f;
     const bool nothing = token >= P.V || lse == -INFINITY;
     const float own = g_log_prob && there ? g_log_prob[row] : 0.f, gh = g_entropy && there ? g_entropy[row] : 0.f;
     float total = own;
@@ -681,10 +691,10 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
             f32x4 d;
             if (g_entropy == nullptr)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<false>(v[i][j], lse, total, gh, H);
+                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<false>(v[i][j], lse, rest, total, gh, H);
             else
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<true>(v[i][j], lse, total, gh, H);
+                for (int j = 0; j < 4; ++j) d[j] = nothing ? 0.f : grad_of<true>(v[i][j], lse, rest, total, gh, H);
             if (few && !nothing) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[j] += at * 4u + j - lead == token ? own : 0.f;
@@ -715,7 +725,7 @@ extern "C" __global__ __launch_bounds__(256) void log_probs_grad(float* dx, cons
         const uint32_t mine = k < P.top ? (uint32_t)top_token[row * P.top + k] : token, vector = mine + lead >> 2;
         if (mine >= P.V || vector < q0 || vector >= q1) continue;
         const float x = logits[row * P.V + mine];
-        float d = g_entropy == nullptr ? grad_of<false>(x, lse, total, gh, H) : grad_of<true>(x, lse, total, gh, H);
+        float d = g_entropy == nullptr ? grad_of<false>(x, lse, rest, total, gh, H) : grad_of<true>(x, lse, rest, total, gh, H);
         if (mine == token) d += own;
 #pragma unroll 8
         for (uint32_t i = 0; i < P.top; ++i) d += (uint32_t)top_token[row * P.top + i] == mine ? g_top[row * P.top + i] : 0.f;

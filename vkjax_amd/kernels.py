@@ -2414,16 +2414,17 @@ def _log_probs_share(rows: int, lanes: int, top: int) -> bool:
     return 1e-5 * rows * lanes + top * max(0.5, 2.6e-6 * rows * lanes) <= 2 + rows * (6.5e-4 + 1.2e-5 * top)
 
 
-def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch) -> tp.List[Launch]:
+def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits: Buffer, tokens: Buffer, top: int, scratch,
+                    log_sum_rest=None) -> tp.List[Launch]:
     v = logits.shape[-1]
     rows    = logits.size // v
-    results = [(b, 0) for b in (log_prob, entropy, log_sum, top_log_prob, top_token)]
+    results = [(b, 0) for b in (log_prob, entropy, log_sum, top_log_prob, top_token, log_sum_rest)]
     inputs  = [(logits, 0), (tokens, 0)]
     moved   = 4 * (logits.size + rows * (4 + 2 * top))
     vectors = _cdiv(v + (3 if v % 4 else 0), 4)                           #of a row, which may start inside one
     if v >= 2**29 or rows * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
-    written = (0, 1, 2, 3, 4)
+    written = (0, 1, 2, 3, 4, 5)
     lanes = _pow2_at_least(_cdiv(vectors, 4))
     if vectors <= LOG_PROBS_SHORT and _log_probs_share(rows, lanes, top):
         return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
@@ -2439,15 +2440,15 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     parts  = scratch((rows, slices, 4)) if slices > 1 else None
     keys   = scratch((rows, slices, top, 2), np.uint32) if slices > 1 and top else None
     launch = Launch('log_probs_block', (rows * slices, 1, 1), (BLOCK, 1, 1),
-                    (results if slices == 1 else [(None, 0)] * 5) + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=moved,
-                    written=written if slices == 1 else (5, 6))
+                    (results if slices == 1 else [(None, 0)] * 6) + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=moved,
+                    written=written if slices == 1 else (6, 7))
     if slices == 1:
         return [launch]
     return [launch, Launch('log_probs_join', (rows, 1, 1), (64, 1, 1), results + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=4 * rows * (4 + 2 * top + slices * (4 + 2 * top)), written=written)]
 
 
 def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Buffer, entropy: Buffer, g_log_prob, g_entropy, g_top, top_token,
-                         top: int) -> tp.List[Launch]:
+                         top: int, log_sum_rest=None) -> tp.List[Launch]:
     v = logits.shape[-1]
     rows    = logits.size // v
     vectors = _cdiv(v + (3 if v % 4 else 0), 4)
@@ -2459,7 +2460,7 @@ def token_log_probs_grad(dx: Buffer, logits: Buffer, tokens: Buffer, log_sum: Bu
     if v >= 2**29 or rows >= 2**31 or blocks * BLOCK >= 2**32:
         raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     return [Launch('log_probs_grad', (blocks, 1, 1), (BLOCK, 1, 1),
-                   [(b, 0) for b in (dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token)],
+                   [(b, 0) for b in (dx, logits, tokens, log_sum, log_sum_rest, entropy, g_log_prob, g_entropy, g_top, top_token)],
                    _u32(rows, rows, v, top, slices, slice_, lanes.bit_length() - 1),
                    bytes_moved=4 * (2 * logits.size + rows * (5 + 2 * top)), streamable=True)]
 

@@ -333,13 +333,21 @@ def _or_none(g, like):
     return None if g is None else _materialize(g, like)
 
 
+def _with_log_sum_rest(eqn):
+    '''The gradient of log probabilities needs the log of the sum unrounded: the equation with that result too.'''
+    if eqn.params.get('rest'):
+        return eqn
+    rest = core.Var(None, '', eqn.outvars[2].aval)
+    return core.JaxprEqn(eqn.invars, list(eqn.outvars) + [rest], eqn.primitive, dict(eqn.params, rest=True))
+
+
 @_rule('token_log_probs')
-def _token_log_probs(gs, logits, tokens, outs, top):
-    if gs[2] is not None:
+def _token_log_probs(gs, logits, tokens, outs, top, rest):
+    if gs[2] is not None or gs[-1] is not None:
         raise NotImplementedError('differentiation through the log of the sum of token_log_probs')
     g_top = _or_none(gs[3], outs[3]) if top else None
     return lax.token_log_probs_grad(logits, tokens, outs[2], outs[1], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), g_top,
-                                    outs[4] if g_top is not None else None), None
+                                    outs[4] if g_top is not None else None, log_sum_rest=outs[-1]), None
 
 
 @_rule('linear_recurrence')
@@ -359,6 +367,10 @@ _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', '
 
 # ---------------------------------------------------------------- driver
 
+#what becomes of equations whose backward pass needs more than their results
+_FOR_GRADIENTS = {'token_log_probs': _with_log_sum_rest}
+
+
 def _replay(jaxpr, consts, inputs, env, order):
     '''Emit the equations of `jaxpr` into the current trace (calls are inlined). `env` maps the jaxpr's
     variables to values of the current trace; `order` collects the equations with non-call primitives.'''
@@ -370,6 +382,7 @@ def _replay(jaxpr, consts, inputs, env, order):
         env[v] = x
     for eqn in jaxpr.eqns:
         name = eqn.primitive.name
+        eqn  = _FOR_GRADIENTS.get(name, lambda e: e)(eqn)
         if name in _CALL_PARAMS:
             inner = eqn.params[_CALL_PARAMS[name]]
             rule  = eqn.params.get('jvp_jaxpr_thunk') if name.startswith('custom_jvp') else None

@@ -561,9 +561,10 @@ def group_norm_grad(g, x, scale, shift, mean, rstd, groups: int, eps: float = 1e
 TOKEN_LOG_PROBS_MAX_TOP = 32
 
 
-def token_log_probs(logits, tokens, top: int = 0):
+def token_log_probs(logits, tokens, top: int = 0, with_rest: bool = False):
     '''For rows of scores [..., V] and one token per row [...]: (log softmax(logits)[token], entropy of softmax(logits),
     log(sum(exp(logits)))), all [...], and for top > 0 the log probabilities and numbers [..., top] of the most likely tokens.
+    With `with_rest` also, behind them, what the rounding of log(sum(exp(logits))) has lost [...], for token_log_probs_grad.
     `nn.token_log_probs` says what becomes of padded and masked rows.'''
     logits, tokens = _rows_and_tokens('token_log_probs', logits, tokens)
     ls, top = _shape(logits), int(top)
@@ -571,6 +572,8 @@ def token_log_probs(logits, tokens, top: int = 0):
         raise ValueError(f'token_log_probs: top must be between 0 and {builtins.min(ls[-1], TOKEN_LOG_PROBS_MAX_TOP)} here, got {top}')
     rows  = _aval(ls[:-1], _f32)
     avals = [rows, rows, rows] + ([_aval(ls[:-1] + (top,), _f32), _aval(ls[:-1] + (top,), _i32)] if top else [])
+    if with_rest:
+        return tuple(emit('token_log_probs', [logits, tokens], avals + [rows], dict(top=top, rest=True), multiple_results=True))
     return tuple(emit('token_log_probs', [logits, tokens], avals, dict(top=top), multiple_results=True))
 
 
@@ -591,12 +594,16 @@ def _rows_and_tokens(name, logits, tokens):
     return logits, tokens
 
 
-def token_log_probs_grad(logits, tokens, log_sum, entropy, g_log_probs=None, g_entropy=None, g_top=None, top_tokens=None):
-    '''Cotangent of token_log_probs' logits for those of its results (None: zeros), of which log_sum, entropy and top_tokens are.'''
+def token_log_probs_grad(logits, tokens, log_sum, entropy, g_log_probs=None, g_entropy=None, g_top=None, top_tokens=None, log_sum_rest=None):
+    '''Cotangent of token_log_probs' logits for those of its results (None: zeros), of which log_sum, entropy, top_tokens and
+    log_sum_rest are. Without log_sum_rest every probability of a row is off by the rounding of its log_sum: half a step of that,
+    which is 5e-4 at scores around 1e4. (Gradients through `vjp` and `grad` have it.)'''
     name = 'token_log_probs_grad'
     logits, tokens = _rows_and_tokens(name, logits, tokens)
     log_sum, entropy, *optional = [_f32_operand(v, name) for v in (log_sum, entropy, g_log_probs, g_entropy) if v is not None]
     ls = _shape(logits)
+    if log_sum_rest is not None:
+        optional.insert(0, _f32_operand(log_sum_rest, name))
     if _any_differs(ls[:-1], log_sum, entropy, *optional):
         raise TypeError(f'{name}: one value per row is needed')
     top = 0
@@ -607,7 +614,7 @@ def token_log_probs_grad(logits, tokens, log_sum, entropy, g_log_probs=None, g_e
             raise TypeError(f'{name}: the alternatives and their cotangents must have the same shape')
         optional += [g_top, top_tokens]
     return emit('token_log_probs_grad', [logits, tokens, log_sum, entropy] + optional, [_aval(ls, _f32)],
-                dict(has_log_probs=g_log_probs is not None, has_entropy=g_entropy is not None, top=top))
+                dict(has_log_probs=g_log_probs is not None, has_entropy=g_entropy is not None, top=top, has_rest=log_sum_rest is not None))
 
 
 def _any_differs(shape, *arrays) -> bool:

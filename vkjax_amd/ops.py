@@ -1107,12 +1107,14 @@ def group_norm_grad(bufferpool, equation):
 
 
 def token_log_probs(bufferpool, equation):
+    p = equation.params
     (logits, tokens), (log_prob, entropy, log_sum, *top), scratch = _operator_buffers(bufferpool, equation)
     if _kind(logits.dtype) != _F or _kind(tokens.dtype) not in (_I, _U):
         raise NotImplementedError(equation)
+    log_sum_rest = top.pop() if p.get('rest') else None
     top_log_prob, top_token = top or (None, None)
     return _operator_ops(equation, K.token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits, tokens,
-                                                     int(equation.params['top']), scratch))
+                                                     int(p['top']), scratch, log_sum_rest))
 
 
 def token_log_probs_grad(bufferpool, equation):
@@ -1121,11 +1123,12 @@ def token_log_probs_grad(bufferpool, equation):
     if _kind(logits.dtype) != _F or _kind(tokens.dtype) not in (_I, _U):
         raise NotImplementedError(equation)
     take = iter(optional)
+    log_sum_rest = next(take) if p.get('has_rest') else None
     g_log_prob = next(take) if p['has_log_probs'] else None
     g_entropy  = next(take) if p['has_entropy'] else None
     g_top, top_token = (next(take), next(take)) if p['top'] else (None, None)
     return _operator_ops(equation, K.token_log_probs_grad(dx, logits, tokens, log_sum, entropy, g_log_prob, g_entropy, g_top, top_token,
-                                                          int(p['top'])))
+                                                          int(p['top']), log_sum_rest))
 
 
 def _recurrence_buffers(ins, params):
