@@ -3,12 +3,13 @@ in 64 bits. Bounds are those of the operators' own tests.'''
 import numpy as np
 import pytest
 
+import vkjax_amd
 from tests.test_gpu_operators import D, U, both, check_recurrence, close, norm_bounds, norm_program, probs_program, recurrence_inputs
 from tests.test_operators import normal
-from vkjax_amd import minijax as mj
+from vkjax_amd import kernels as K, minijax as mj
 
 pytestmark = pytest.mark.gpu
-nn, f32 = mj.nn, np.float32
+lax, nn, f32 = mj.lax, mj.nn, np.float32
 
 
 def check_norm(shape, groups, activation):
@@ -110,3 +111,29 @@ def test_log_probs_of_rows_that_hold_the_lowest_value_only(v):
         #(the entropy of equal probabilities has no gradient: what is left of it is log p + H, off by 16 u log v)
         close(d[row], one - 1 / v, (24 * U * np.log(v) + 16 * U) / v + 2 * U * one)
     assert not d[1].any()
+
+
+# ------------------------------------------------------------------ the relu of the forward pass and that of the gradient
+
+#(samples, positions, groups, channels of a group): both directions in registers, in chunks, forward in registers and the gradient in chunks, rows, wide rows, forward
+#wide and the gradient in chunks
+@pytest.mark.parametrize('n,s,groups,cg,kinds', [(2, 49, 64, 16, ('held', 'held')), (3, 17, 5, 129, ('held', 'held')), (1, 4000, 32, 16, ('chunked', 'chunked')), (1, 4001, 7, 33, ('chunked', 'chunked')),
+                                                 (80, 49, 32, 16, ('held', 'held')), (70, 1200, 4, 8, ('held', 'chunked')), (24, 1, 16, 65, ('rows', 'rows')), (24, 1, 2, 2048, ('wide', 'wide')),
+                                                 (24, 1, 1, 20000, ('wide', 'chunked'))])
+def test_the_gradient_goes_through_where_the_result_is_positive(n, s, groups, cg, kinds):
+    '''Every channel's shift puts one of its values next to zero; the cotangents are 1, 2, 4 .., so that the shift's gradient tells which values went through.'''
+    c = groups * cg
+    assert tuple(K.norm_plan(n, s, c, groups, gradient).kind for gradient in (False, True)) == kinds
+    shape = (n, s, c) if s > 1 else (n, c)
+    x, scale = (normal(c, *shape) + normal(2, c)).astype(f32), (0.5 + np.random.default_rng(c).random(c)).astype(f32)
+    _, mean, rstd = vkjax_amd.wrap(lambda *a: lax.group_norm(*a, groups), frontend='minijax')(x, scale, np.zeros(c, f32))
+    rows, places = x.reshape(n * s, c), 20
+    which = np.arange(c) % places
+    sample, group = which // s, np.arange(c) // cg
+    hat = (rows[which, np.arange(c)] - mean[sample, group]) * rstd[sample, group]
+    shift = -(hat * scale)
+    g = np.zeros((n * s, c), f32)
+    g[:places] = 2.0 ** np.arange(places)[:, None]
+    y, _, _, dshift = vkjax_amd.wrap(norm_program(groups, 'relu'), frontend='minijax')(x, scale, shift, g.reshape(shape))
+    passed = (y.reshape(n * s, c)[:places] > 0) * g[:places].astype(np.float64)
+    assert np.array_equal(dshift, passed.sum(axis=0)), int((dshift != passed.sum(axis=0)).sum())

@@ -52,6 +52,9 @@ __device__ __forceinline__ float reciprocal(float d) {
 // and the reciprocal to one unit of the last place. That is where this operator's launches have their instructions: 25 a value with the library's exponential and
 // a division bounded them. (exp(-z) beyond fp32 is infinite, and its reciprocal 0.)
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
+// What the activation is taken of, hat = (x - mean) rstd: rounded alike in every kernel, so that next to zero a gradient is that of the relu that the
+// forward pass has taken.
+__device__ __forceinline__ float z_of(float hat, float gamma, float beta) { return __builtin_fmaf(hat, gamma, beta); }
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
     if (act == ACT_RELU) return (z > 0.f || z != z) ? z : 0.f;
     if (act == ACT_SILU) return z * sigmoid(z);
@@ -235,16 +238,16 @@ __device__ __forceinline__ void held_body(float* y, float* means, float* rstds, 
     if (!use || y == nullptr) return;
     const bool stream = streams_result(P.first);
     const __amdgpu_buffer_rsrc_t y_rsrc = make_rsrc(y + base, bytes);
-    float mean[VEC], factor[VEC];
+    float mean[VEC], rstd[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const uint32_t g = m * span.groups + span.group_of(P, j);
-        mean[j] = mean_of[g]; factor[j] = rstd_of[g] * gamma[j];
+        mean[j] = mean_of[g]; rstd[j] = rstd_of[g];
     }
 #pragma unroll
     for (int i = 0; i < K; ++i) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf(v[i][j] - mean[j], factor[j], beta[j]), P.act);
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(z_of((v[i][j] - mean[j]) * rstd[j], gamma[j], beta[j]), P.act);
         store<VEC>(v[i], y_rsrc, (uint32_t)i < mine ? first + i * step : NOWHERE, stream);
     }
 }
@@ -293,7 +296,7 @@ __device__ __forceinline__ void held_grad_body(float* dx, float* dscale_rows, fl
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] = (v[i][j] - mean[j]) * rstd[j];
-                d[i][j] = act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act);
+                d[i][j] = act_gradient(d[i][j], z_of(v[i][j], gamma[j], beta[j]), P.act);
                 d[i][j] = (uint32_t)i < mine ? d[i][j] : 0.f; v[i][j] = (uint32_t)i < mine ? v[i][j] : 0.f;
                 A[j] += d[i][j]; B[j] = __builtin_fmaf(d[i][j], v[i][j], B[j]);
             }
@@ -442,7 +445,7 @@ __device__ __forceinline__ void rows_body(float* y, float* means, float* rstds, 
         const f32x2* const from = stats_of + (m < here ? m * span.groups : 0u);
         const f32x2 a = from[two.first], b = from[two.last];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf((v[i][j] - two.pick(j, a.x, b.x)) * two.pick(j, a.y, b.y), gamma[j], beta[j]), P.act);
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(z_of((v[i][j] - two.pick(j, a.x, b.x)) * two.pick(j, a.y, b.y), gamma[j], beta[j]), P.act);
         store<VEC>(v[i], y_rsrc, at(i), stream);
     }
 }
@@ -493,7 +496,7 @@ __device__ __forceinline__ void rows_grad_body(float* dx, float* dscale_rows, fl
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] = there(i) ? (v[i][j] - two.pick(j, a.x, b.x)) * two.pick(j, a.y, b.y) : 0.f;
-                d[i][j] = there(i) ? act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
+                d[i][j] = there(i) ? act_gradient(d[i][j], z_of(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
                 d_total[j] += d[i][j]; dh_total[j] = __builtin_fmaf(d[i][j], v[i][j], dh_total[j]);
                 d[i][j] *= gamma[j];
                 product[j] = d[i][j] * v[i][j];
@@ -584,7 +587,7 @@ __device__ __forceinline__ void wide_body(float* y, float* means, float* rstds, 
         float gamma[VEC], beta[VEC];
         load<VEC>(gamma, gammas, wide.at(i)); load<VEC>(beta, betas, wide.at(i));
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(__builtin_fmaf((v[i][j] - mean) * rstd, gamma[j], beta[j]), P.act);
+        for (int j = 0; j < VEC; ++j) v[i][j] = act_value(z_of((v[i][j] - mean) * rstd, gamma[j], beta[j]), P.act);
         store<VEC>(v[i], y_rsrc, wide.at(i), stream);
     }
 }
@@ -618,7 +621,7 @@ __device__ __forceinline__ void wide_grad_body(float* dx, float* dscale_rows, fl
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] = wide.there(i) ? (v[i][j] - mean) * rstd : 0.f;
-                d[i][j] = wide.there(i) ? act_gradient(d[i][j], __builtin_fmaf(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
+                d[i][j] = wide.there(i) ? act_gradient(d[i][j], z_of(v[i][j], gamma[j], beta[j]), P.act) : 0.f;
                 d_total[i][j] += d[i][j]; dh_total[i][j] = __builtin_fmaf(d[i][j], v[i][j], dh_total[i][j]);
                 d[i][j] *= gamma[j];
                 a += d[i][j]; b = __builtin_fmaf(d[i][j], v[i][j], b);
@@ -779,11 +782,11 @@ __device__ __forceinline__ void apply_body(float* y, float* means, float* rstds,
     });
     __syncthreads();
     if (y == nullptr || !span.owns()) return;
-    float mean[VEC], factor[VEC], beta[VEC];
+    float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const uint32_t g = span.group_of(P, j);
-        mean[j] = mean_of[g]; factor[j] = rstd_of[g] * scale[span.c + j]; beta[j] = shift[span.c + j];
+        mean[j] = mean_of[g]; rstd[j] = rstd_of[g]; gamma[j] = scale[span.c + j]; beta[j] = shift[span.c + j];
     }
     const bool stream = streams_result(P.first);
     const uint64_t base = ((uint64_t)chunk.n * P.S + chunk.from) * P.C + span.c0;
@@ -793,7 +796,7 @@ __device__ __forceinline__ void apply_body(float* y, float* means, float* rstds,
 #pragma unroll
         for (int k = 0; k < U; ++k) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[k][j] = act_value(__builtin_fmaf(v[k][j] - mean[j], factor[j], beta[j]), P.act);
+            for (int j = 0; j < VEC; ++j) v[k][j] = act_value(z_of((v[k][j] - mean[j]) * rstd[j], gamma[j], beta[j]), P.act);
             store<VEC>(v[k], y_rsrc, (uint32_t)k < here ? ((span.p + (i + k) * P.P) * P.C + span.col * VEC) * 4u : NOWHERE, stream);
         }
     });
@@ -827,7 +830,7 @@ __device__ __forceinline__ void walk_gradient(const NormParams& P, const Span<VE
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[k][j] = (v[k][j] - mean[j]) * rstd[j];
-                d[k][j] = act_gradient(d[k][j], __builtin_fmaf(v[k][j], gamma[j], beta[j]), P.act);
+                d[k][j] = act_gradient(d[k][j], z_of(v[k][j], gamma[j], beta[j]), P.act);
             }
         step(v, d, min(mine - i, (uint32_t)U), i);
     }
