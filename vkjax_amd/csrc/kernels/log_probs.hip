@@ -447,8 +447,9 @@ __device__ __forceinline__ void wave_body(const Results& to, const float* logits
     __shared__ __attribute__((aligned(16))) uint64_t lists[4][LIST];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint64_t row = (uint64_t)blockIdx.x * 4u + wave;
+    // (asked for before it is known whether there is such a row, so that all arguments come with one wait: 65536 rows of 1000 67.0 us a pass, so 64.5)
+    const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[min(row, (uint64_t)P.rows - 1u)]);
     if (row >= P.rows) return;
-    const uint32_t token = __builtin_amdgcn_readfirstlane(tokens[row]);
     if (token >= P.V) { write_padding(to, row, lane, 64u, P.top); return; }
     const Row from(logits, row, P.V);
     const float score = from.x[token];
