@@ -137,3 +137,30 @@ def test_the_gradient_goes_through_where_the_result_is_positive(n, s, groups, cg
     y, _, _, dshift = vkjax_amd.wrap(norm_program(groups, 'relu'), frontend='minijax')(x, scale, shift, g.reshape(shape))
     passed = (y.reshape(n * s, c)[:places] > 0) * g[:places].astype(np.float64)
     assert np.array_equal(dshift, passed.sum(axis=0)), int((dshift != passed.sum(axis=0)).sum())
+
+
+# ------------------------------------------------------------------ recurrences whose products of factors leave the range of fp32
+
+@pytest.mark.parametrize('t,c', [(40, 8), (700, 12), (700, 7), (3000, 20)])
+@pytest.mark.parametrize('gated,reverse', [(False, False), (True, True)])
+def test_recurrences_behind_many_small_factors(gated, reverse, t, c):
+    '''A state of 1e38 behind which products of factors fall below 2^-149: an error of 2^-140 of it; an infinite one leaves no finite value in its channel, and
+    the others as they are.'''
+    print(f'recurrence 2 x {t} x {c}, gated {gated}, small factors', flush=True)
+    x, state = np.abs(normal(1, 2, t, c)), np.zeros((2, c), f32)
+    factor = np.full((2, t, c), -1.5 if gated else 0.25, f32)
+    state[0, 1::2] = 1e38
+    got, expected, _ = both(lambda *a: (nn.gated_recurrence if gated else lax.linear_recurrence)(*a, reverse=reverse), factor, x, state)
+    #24 u a step of what is kept, of a geometric series (below twice its largest term) of values of at most 6, and of the state
+    a = 1 / (1 + np.exp(1.5)) if gated else 0.25
+    left = np.abs(state[:, None].astype(np.float64)) * a ** np.arange(1, t + 1)[None, :, None]
+    left = left[:, ::-1] if reverse else left
+    steps = np.arange(1, t + 1)[None, :, None]
+    steps = steps[:, ::-1] if reverse else steps
+    for k, bound in ((0, 24 * U * (12 + steps * left) + 2.0 ** -140 * np.abs(state[:, None])), (1, 24 * U * (12 + t * left[:, 0 if reverse else -1]) + 2.0 ** -140 * np.abs(state))):
+        close(got[k], expected[k], bound + 1e-37, ('h', 'last')[k])
+    state[0, 0] = np.inf
+    broken, _, _ = both(lambda *a: (nn.gated_recurrence if gated else lax.linear_recurrence)(*a, reverse=reverse), factor, x, state)
+    assert not np.isfinite(broken[0][0, :, 0]).any() and not np.isfinite(broken[1][0, 0])
+    broken[0][0, :, 0], broken[1][0, 0] = got[0][0, :, 0], got[1][0, 0]
+    assert np.array_equal(broken[0], got[0]) and np.array_equal(broken[1], got[1])

@@ -14,6 +14,8 @@
 // soon as it has it, and the state behind it as soon as it knows that; it looks at the WINDOW tiles before it until one of them
 // shows its state and all after that one their maps, then applies those maps in turn. Every tile applies the same maps to the same
 // states in the same order, whatever it finds published, so the results do not depend on the order in which blocks run.
+//   * A map's factor is a product of up to 512 steps' and may fall out of fp32's range where the state times each of them in turn would not: at 16 steps a thread, six
+//     products across a wave, four waves and 16 tiles an error of up to 2^-150 each, 2^-144 of the state in all.
 //   * The wait ends: tiles are numbered in the order in which their blocks start (a ticket), a tile looks at earlier ones only, and
 //     the first tile without a state finds its predecessor's. So the earliest one always gets on, and then the next.
 //   * There are eight lines of tickets, one for every eighth block: drawn from one alone, they follow one another some 10 ns apart (3 x 1021 x

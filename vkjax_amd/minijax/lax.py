@@ -648,9 +648,12 @@ def linear_recurrence(factor, x, state=None, lengths=None, reverse: bool = False
     [batch, channels]).
 
     Parts of a sequence run side by side, by products of their factors. Those of gates, and of factors between -1 and 1, only get
-    smaller, and h is that of step by step but for rounding. Factors beyond that are for sequences in which no product of
-    neighbouring ones passes float32's range (inf and NaN appear where step by step 0 times it would be 0), nor falls below it and is
-    brought back by larger ones (what came before is lost then).'''
+    smaller, and h is that of step by step but for rounding and for what a product loses at the lower end of float32's range: over
+    many small factors it falls below 2^-149 and is 0. What stood in front of them, the state among it, counts with an error of up
+    to 2^-140 of itself there (next to a state of 1e38 that is 1e-4, also where step by step less would be left of it), and
+    an infinite value is NaN behind them, where step by step it would stay infinite. Gradients go by the same products. Factors
+    beyond that are for sequences in which no product of neighbouring ones passes float32's range (inf and NaN appear where step by
+    step 0 times it would be 0), nor falls below it and is brought back by larger ones (what came before is lost then).'''
     operands, xs = _recurrence_operands('gated_recurrence' if gated else 'linear_recurrence', factor, x, state, lengths)
     return tuple(emit('linear_recurrence', operands, [_aval(xs, _f32), _aval((xs[0], xs[2]), _f32)],
                 dict(gated=bool(gated), reverse=bool(reverse), has_state=state is not None, has_lengths=lengths is not None),

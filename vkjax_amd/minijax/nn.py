@@ -68,5 +68,6 @@ def gated_recurrence(gate, x, state=None, lengths=None, reverse=False):
     a = sigmoid(gate). Returns (h, the state [batch, channels] behind the last step), so that a sequence can go on later: `state`
     is where it starts (zeros if None), and time may be 1, or 0. `lengths` int32 [batch]: a padded batch, in which a sequence's
     state stays what it is from its length on (in h too) and what gate and x hold there is not looked at; `reverse`: from the last
-    time to the first. Differentiable with respect to gate, x and state. `lax.linear_recurrence` takes factors and addends.'''
+    time to the first. Differentiable with respect to gate, x and state. `lax.linear_recurrence` takes factors and addends, and says
+    what becomes of values that many small factors leave next to nothing of, and of infinite ones.'''
     return lax.linear_recurrence(gate, x, state, lengths, reverse, gated=True)
