@@ -1,12 +1,14 @@
 '''The kernels of group norms, log probabilities and recurrences one by one: sizes that are planned for each of them, against the definitions
 in 64 bits. Bounds are those of the operators' own tests.'''
+import ctypes
+
 import numpy as np
 import pytest
 
 import vkjax_amd
 from tests.test_gpu_operators import D, U, both, check_recurrence, close, norm_bounds, norm_program, probs_program, recurrence_inputs
 from tests.test_operators import normal
-from vkjax_amd import kernels as K, minijax as mj
+from vkjax_amd import hip, kernels as K, minijax as mj
 
 pytestmark = pytest.mark.gpu
 lax, nn, f32 = mj.lax, mj.nn, np.float32
@@ -164,3 +166,15 @@ def test_recurrences_behind_many_small_factors(gated, reverse, t, c):
     assert not np.isfinite(broken[0][0, :, 0]).any() and not np.isfinite(broken[1][0, 0])
     broken[0][0, :, 0], broken[1][0, 0] = got[0][0, :, 0], got[1][0, 0]
     assert np.array_equal(broken[0], got[0]) and np.array_equal(broken[1], got[1])
+
+
+# ------------------------------------------------------------------ beside other users of the runtime
+
+def test_looking_for_a_kernel_leaves_no_error_behind():
+    '''The kernel is in the last of the modules that are searched: the searches that fail are nobody's error.'''
+    runtime = ctypes.CDLL('libamdhip64.so.7')
+    runtime.hipGetLastError()
+    device = hip.Device(hip.Device.get().index)
+    f = vkjax_amd.wrap(lambda a, x: lax.linear_recurrence(a, x)[0], frontend='minijax', device=device)
+    h = f(np.full((1, 3, 4), 0.5, f32), np.ones((1, 3, 4), f32))
+    assert runtime.hipPeekAtLastError() == 0 and np.array_equal(h[0, :, 0], [1, 1.5, 1.75])

@@ -874,6 +874,8 @@ int vkj_module_get_function(vkj_handle h, vkj_handle mh, const char* name, vkj_h
     hipError_t e = hipModuleGetFunction(&f->fn, m->module, name);
     if (e != hipSuccess) {
         delete f;
+        // kernels are looked for in one module after the other: the runtime's own record of this one must not reach whoever asks for it next
+        (void)hipGetLastError();
         g_last_error = std::string("kernel '") + name + "' not found in module: " + hipGetErrorString(e);
         return (int)e;
     }
