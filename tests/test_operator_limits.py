@@ -7,8 +7,11 @@ import pytest
 
 from tests.test_gpu_operator_kernels import NORM_SIZES, RECURRENCE_SIZES
 from tests.test_operator_plans import TOOLS, buffer, check_recurrence, kernels_of, norm_launches
-from vkjax_amd import kernels as K
+from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.csrc import build
+from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
+
+lax, f32 = mj.lax, np.float32
 
 
 # ------------------------------------------------------------------ recurrences: what a tile's descriptor covers
@@ -60,3 +63,21 @@ def test_every_kernel_is_run_on_the_gpu(tmp_path):
     launched = {launch.kernel for size in NORM_SIZES for launches in norm_launches(*size) for launch in launches}
     launched |= {kernel for b, t, c in RECURRENCE_SIZES for gated in (False, True) for kernel in check_recurrence(b, t, c, gated, b > 1)}
     assert found == launched, (found - launched, launched - found)
+
+
+# ------------------------------------------------------------------ results that are stored past the caches
+
+@pytest.mark.parametrize('read', ['dfactor', 'dx', 'both', 'neither'])
+def test_a_recurrences_gradient_is_stored_past_the_caches_where_neither_result_is_read(read):
+    '''One flag is about both results: those that a later launch reads stay with the caches.'''
+    shape = (2, 4096, 2048)
+    large, small = np.broadcast_to(f32(0), shape), np.zeros((2, 2048), f32)
+
+    def f(factor, x, h, g, last):
+        dfactor, dx, dstate = lax.linear_recurrence_grad(h, factor, x, None, None, g, last)
+        #(a product that has to have its operand in memory)
+        reads = lambda v: lax.linear_recurrence(v, x)[1]
+        return (reads(dfactor) if read in ('dfactor', 'both') else dfactor), (reads(dx) if read in ('dx', 'both') else dx), dstate
+    program = JaxprInterpreter(mj.make_jaxpr(f)(large, large, large, large, small), plan_only=True)
+    launch, = [l for l in program.launches if l.kernel.startswith('recurrence_grad')]
+    assert bool(np.frombuffer(launch.params, np.uint32)[0] >> 31) == (read == 'neither')

@@ -138,10 +138,9 @@ class JaxprInterpreter:
             launch = launches[k]
             members = launch.members or (launch,)
             if launch.streamable and not launch.members:
-                out = launch.buffers[0][0]
-                nbytes = out.size * 4 if out is not None else 0
-                if (out is not None and out.tensor is not None and id(out.tensor) not in touched_later
-                        and K.STREAM_RESULT_MIN_BYTES <= nbytes < 2**32):
+                outs = [launch.buffers[i][0] for i in launch.streamed if launch.buffers[i][0] is not None]
+                if (outs and all(out.tensor is not None and id(out.tensor) not in touched_later
+                                 and K.STREAM_RESULT_MIN_BYTES <= out.size * 4 < 2**32 for out in outs)):
                     result[k] = K.with_streamed_result(launch)
             for m in members:
                 #(an array a later launch only writes - the next part of a concatenation - is not read by it; kernels that

@@ -98,13 +98,15 @@ class Launch(tp.NamedTuple):
     #a batch launch: the launches it evaluates, described to the kernel by a table in device memory
     #that is written when the launch is recorded (it holds device addresses)
     members: tp.Tuple['Launch', ...] = ()
-    #the kernel stores its result (its first array) past the caches when bit 31 of its first parameter word is set
-    #(see with_streamed_result)
+    #the kernel stores its result (its first array, or those in `streamed`) past the caches when bit 31 of its first parameter word
+    #is set (see with_streamed_result)
     streamable: bool = False
     #which of `buffers` the kernel writes (positions); everything else it only reads
     written: tp.Tuple[int, ...] = (0,)
     #which of `buffers` are scratch that other launches use too and that holds nothing (counters: zeros) between launches
     scratch: tp.Tuple[int, ...] = ()
+    #which of `buffers` a streamable kernel's flag is about (positions)
+    streamed: tp.Tuple[int, ...] = (0,)
 
 
 def _u32(*values) -> bytes:
@@ -2528,7 +2530,8 @@ def recurrence_tiling(batch: int, time: int, channels: int, steps_by_vec, arrays
     return tiling
 
 
-def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int) -> Launch:
+def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, gated: bool, reverse: bool, zeroed, arrays, written, moved: int,
+                       streamed=(0,)) -> Launch:
     _, t, c = shape
     kernel  = f'{name}_v{tiling.vec}_l{tiling.steps}' + ('_gated' if gated else '') + ('_chain' if tiling.tiles > 1 else '')
     #(what tiles hand on: lines of 64 bytes for the tickets, then a word of 64 bits per channel and tile)
@@ -2537,7 +2540,7 @@ def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, ga
     buffers = [(v, 0) for v in arrays] + [(chain, 0)]
     return Launch(kernel, (blocks, 1, 1), (RECURRENCE_THREADS, 1, 1), buffers,
                   _u32(0, t, c, tiling.cstrips, tiling.strips, tiling.tiles, lines, of_each, tiling.lanes.bit_length() - 1, reverse), bytes_moved=moved, streamable=c % 32 == 0,
-                  written=written + ((len(arrays),) if chain is not None else ()), scratch=(len(arrays),) if chain is not None else ())
+                  written=written + ((len(arrays),) if chain is not None else ()), scratch=(len(arrays),) if chain is not None else (), streamed=streamed)
 
 
 def _recurrence_shape(x: Buffer, lengths):
@@ -2556,4 +2559,4 @@ def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Bu
     shape = _recurrence_shape(x, lengths)
     return [_recurrence_launch('recurrence_grad', x, recurrence_tiling(*shape, RECURRENCE_GRAD_STEPS, 5 + gated), shape, gated, reverse, zeroed,
                                (dfactor, dx, dstate, h, factor, x if gated else None, state, lengths, g, g_last), (0, 1, 2),
-                               4 * ((5 + gated) * x.size + 2 * x.shape[0] * x.shape[2]))]
+                               4 * ((5 + gated) * x.size + 2 * x.shape[0] * x.shape[2]), streamed=(0, 1))]
