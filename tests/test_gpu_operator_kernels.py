@@ -11,7 +11,7 @@ from tests.test_operators import normal
 from vkjax_amd import hip, kernels as K, minijax as mj
 
 pytestmark = pytest.mark.gpu
-lax, nn, f32 = mj.lax, mj.nn, np.float32
+jnp, lax, nn, f32 = mj.numpy, mj.lax, mj.nn, np.float32
 
 
 def check_norm(shape, groups, activation):
@@ -178,3 +178,24 @@ def test_looking_for_a_kernel_leaves_no_error_behind():
     f = vkjax_amd.wrap(lambda a, x: lax.linear_recurrence(a, x)[0], frontend='minijax', device=device)
     h = f(np.full((1, 3, 4), 0.5, f32), np.ones((1, 3, 4), f32))
     assert runtime.hipPeekAtLastError() == 0 and np.array_equal(h[0, :, 0], [1, 1.5, 1.75])
+
+
+# ------------------------------------------------------------------ more rows than 24 bits count
+
+@pytest.mark.parametrize('v,top', [(20, 0), (124, 5)])
+def test_log_probs_of_more_rows_than_a_block_each_can_be_launched_for(v, top):
+    rows = 2**24 + 5
+    print(f'log probabilities {rows} x {v}, top {top}', flush=True)
+    row, t = normal(v, v), (np.arange(rows) % v).astype(np.int32)
+    t[3], t[rows - 2] = -1, v
+    got = vkjax_amd.wrap(lambda row, t: nn.token_log_probs(jnp.broadcast_to(jnp.reshape(row, (1, v)), (rows, v)), t, top)[:3], frontend='minijax')(row, t)
+    logp = row.astype(np.float64)
+    logp = logp - (logp.max() + np.log(np.exp(logp - logp.max()).sum()))
+    #sums of at most 64 additions in a row, twice over, and roundings of values of at most 20
+    bound = 160 * U + 6 * U * 20
+    given = (t >= 0) & (t < v)
+    expected = np.where(given, logp[np.where(given, t, 0)], 0.0)
+    close(got[0], expected, bound)
+    close(got[1], np.where(given, -(np.exp(logp) * logp).sum(), 0.0), 20 * bound)
+    if top:
+        close(got[2][-9:], np.where(given[-9:, None], np.sort(logp)[::-1][:top], 0.0), bound)

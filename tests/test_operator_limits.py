@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from tests.test_gpu_operator_kernels import NORM_SIZES, RECURRENCE_SIZES
-from tests.test_operator_plans import TOOLS, buffer, check_recurrence, kernels_of, norm_launches
+from tests.test_operator_plans import TOOLS, buffer, check_log_probs, check_recurrence, kernels_of, norm_launches
 from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.csrc import build
 from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
@@ -81,3 +81,16 @@ def test_a_recurrences_gradient_is_stored_past_the_caches_where_neither_result_i
     program = JaxprInterpreter(mj.make_jaxpr(f)(large, large, large, large, small), plan_only=True)
     launch, = [l for l in program.launches if l.kernel.startswith('recurrence_grad')]
     assert bool(np.frombuffer(launch.params, np.uint32)[0] >> 31) == (read == 'neither')
+
+
+# ------------------------------------------------------------------ many rows
+
+@pytest.mark.parametrize('rows,v,top', [(2**24, 20, 0), (2**24 + 3, 130, 5), (2**25, 10, 10), (2**26 - 8, 100, 0), (2**26 - 8, 1000, 5)])
+def test_log_probs_of_many_rows_are_planned(rows, v, top):
+    assert all(not name.startswith('log_probs_block') for name in check_log_probs(rows, v, top))
+
+
+@pytest.mark.parametrize('rows,v,top', [(2**31, 1, 0), (2**26, 1000, 5), (2**24, 5000, 0), (2**24 + 1, 4092, 0)])
+def test_log_probs_of_too_many_rows_are_refused(rows, v, top):
+    with pytest.raises(NotImplementedError):
+        list(check_log_probs(rows, v, top))

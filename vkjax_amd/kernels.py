@@ -2424,15 +2424,18 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     inputs  = [(logits, 0), (tokens, 0)]
     moved   = 4 * (logits.size + rows * (4 + 2 * top))
     vectors = _cdiv(v + (3 if v % 4 else 0), 4)                           #of a row, which may start inside one
-    if v >= 2**29 or rows * BLOCK >= 2**32:
-        raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
     written = (0, 1, 2, 3, 4, 5)
+
+    def blocks(n):
+        if v >= 2**29 or rows >= 2**31 or n * BLOCK >= 2**32:
+            raise NotImplementedError(f'log probabilities of {rows} rows of {v}')
+        return (n, 1, 1)
     lanes = _pow2_at_least(_cdiv(vectors, 4))
     if vectors <= LOG_PROBS_SHORT and _log_probs_share(rows, lanes, top):
-        return [Launch('log_probs_short', (_cdiv(rows * lanes, BLOCK), 1, 1), (BLOCK, 1, 1), results + inputs,
+        return [Launch('log_probs_short', blocks(_cdiv(rows * lanes, BLOCK)), (BLOCK, 1, 1), results + inputs,
                        _u32(0, rows, v, top, 1, 0, lanes.bit_length() - 1), bytes_moved=moved, written=written)]
     if vectors <= LOG_PROBS_AT_A_TIME or (vectors <= LOG_PROBS_WAVE and rows >= LOG_PROBS_ROWS):
-        return [Launch('log_probs_wave' if vectors <= LOG_PROBS_AT_A_TIME else 'log_probs_wave_long', (_cdiv(rows, 4), 1, 1), (BLOCK, 1, 1),
+        return [Launch('log_probs_wave' if vectors <= LOG_PROBS_AT_A_TIME else 'log_probs_wave_long', blocks(_cdiv(rows, 4)), (BLOCK, 1, 1),
                        results + inputs, _u32(0, rows, v, top, 1, 0, 0), bytes_moved=moved, written=written)]
     #a block to a row; where there are few, slices of whole chunks, joined by a second launch
     slices = max(1, min(_cdiv(LOG_PROBS_ROWS, rows), _cdiv(vectors, 4 * LOG_PROBS_AT_A_TIME), LOG_PROBS_MAX_KEYS // max(top, 1)))
@@ -2441,7 +2444,7 @@ def token_log_probs(log_prob, entropy, log_sum, top_log_prob, top_token, logits:
     params = _u32(0, rows, v, top, slices, slice_, 0)
     parts  = scratch((rows, slices, 4)) if slices > 1 else None
     keys   = scratch((rows, slices, top, 2), np.uint32) if slices > 1 and top else None
-    launch = Launch('log_probs_block', (rows * slices, 1, 1), (BLOCK, 1, 1),
+    launch = Launch('log_probs_block', blocks(rows * slices), (BLOCK, 1, 1),
                     (results if slices == 1 else [(None, 0)] * 6) + [(parts, 0), (keys, 0)] + inputs, params, bytes_moved=moved,
                     written=written if slices == 1 else (6, 7))
     if slices == 1:
