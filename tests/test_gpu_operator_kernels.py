@@ -199,3 +199,20 @@ def test_log_probs_of_more_rows_than_a_block_each_can_be_launched_for(v, top):
     close(got[1], np.where(given, -(np.exp(logp) * logp).sum(), 0.0), 20 * bound)
     if top:
         close(got[2][-9:], np.where(given[-9:, None], np.sort(logp)[::-1][:top], 0.0), bound)
+
+
+# ------------------------------------------------------------------ single steps of more than two gigabytes
+
+def test_single_steps_of_more_than_two_gigabytes():
+    b, c = 2**19 + 3, 1020
+    gate, x, state = normal(1, c), normal(2, b), normal(3, b)
+
+    def f(gate, x, state):
+        spread = lambda v: jnp.broadcast_to(jnp.reshape(v, (b, 1, 1)), (b, 1, c))
+        start = jnp.broadcast_to(jnp.reshape(state, (b, 1)), (b, c))
+        h, last = nn.gated_recurrence(jnp.broadcast_to(jnp.reshape(gate, (1, 1, c)), (b, 1, c)), spread(x), start)
+        return h[b - 7:, 0], last[b // 2 - 3:b // 2 + 3], h[:5, 0]
+    a = 1 / (1 + np.exp(-gate.astype(np.float64)))
+    exact = lambda part: a * state[part, None].astype(np.float64) + (1 - a) * x[part, None].astype(np.float64)
+    for got, part in zip(vkjax_amd.wrap(f, frontend='minijax')(gate, x, state), (slice(b - 7, b), slice(b // 2 - 3, b // 2 + 3), slice(0, 5))):
+        close(got, exact(part), 24 * U * (np.abs(state[part, None]) + np.abs(x[part, None])))

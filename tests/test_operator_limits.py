@@ -94,3 +94,16 @@ def test_log_probs_of_many_rows_are_planned(rows, v, top):
 def test_log_probs_of_too_many_rows_are_refused(rows, v, top):
     with pytest.raises(NotImplementedError):
         list(check_log_probs(rows, v, top))
+
+
+# ------------------------------------------------------------------ many single steps
+
+@pytest.mark.parametrize('b,c', [(2**19 + 1, 1024), (2**20, 1024), (300000, 2049), (2**19 - 1, 1024), (1, 2**29 - 2048)])
+def test_single_steps_of_two_gigabytes_and_more_are_planned(b, c):
+    x, state = buffer(b, 1, c), buffer(b, c)
+    zeroed = lambda n, use: buffer(n, dtype=np.uint32)
+    for launch, in (K.linear_recurrence(x, state, x, x, state, None, True, False, zeroed), K.linear_recurrence_grad(x, x, state, x, x, x, state, None, x, state, True, False, zeroed)):
+        _, T, C, cstrips, strips, tiles, _, _, log2_w, _ = np.frombuffer(launch.params, np.uint32).astype(np.int64)
+        vec = 4 if '_v4' in launch.kernel else 1
+        assert T == tiles == 1 and strips * C == b * c * cstrips and cstrips * (vec << log2_w) >= C and launch.grid[0] == strips
+        assert 4 * ((256 >> log2_w) * int(launch.kernel.split('_l')[1].split('_')[0]) * C + (vec << log2_w)) < 2**31 and launch.grid[0] * 256 < 2**32

@@ -2547,8 +2547,8 @@ def _recurrence_launch(name: str, x: Buffer, tiling: RecurrenceTiling, shape, ga
 
 
 def _recurrence_shape(x: Buffer, lengths):
-    #single steps of all sequences lie side by side
-    return (1, 1, x.size) if x.shape[1] == 1 and lengths is None else x.shape
+    #single steps of all sequences lie side by side (as many as a tile's descriptor addresses, see recurrence_tiling)
+    return (1, 1, x.size) if x.shape[1] == 1 and lengths is None and 4 * (x.size + 4 * RECURRENCE_THREADS) < 2**31 else x.shape
 
 
 def linear_recurrence(h, last, factor: Buffer, x: Buffer, state, lengths, gated: bool, reverse: bool, zeroed) -> tp.List[Launch]:
