@@ -7,6 +7,7 @@ import pytest
 
 import vkjax_amd
 from tests.test_gpu_operators import D, U, both, check_recurrence, close, norm_bounds, norm_program, probs_program, recurrence_inputs
+from tests.test_operator_plans import norm_launches
 from tests.test_operators import normal
 from vkjax_amd import hip, kernels as K, minijax as mj
 
@@ -216,3 +217,13 @@ def test_single_steps_of_more_than_two_gigabytes():
     exact = lambda part: a * state[part, None].astype(np.float64) + (1 - a) * x[part, None].astype(np.float64)
     for got, part in zip(vkjax_amd.wrap(f, frontend='minijax')(gate, x, state), (slice(b - 7, b), slice(b // 2 - 3, b // 2 + 3), slice(0, 5))):
         close(got, exact(part), 24 * U * (np.abs(state[part, None]) + np.abs(x[part, None])))
+
+
+# ------------------------------------------------------------------ many samples of few positions with wide groups: one row of channel sums for several of them
+
+@pytest.mark.parametrize('n,s,groups,cg', [(700, 1, 1, 16388), (643, 2, 1, 8195), (1300, 3, 1, 4100), (601, 1, 1, 8197), (259, 15, 1, 16500), (900, 1, 2, 16500)])
+def test_chunked_samples_that_share_a_row_of_sums(n, s, groups, cg):
+    c = groups * cg
+    backward = norm_launches(n, s, groups, cg)[1]
+    assert K.norm_plan(n, s, c, groups, True).kind == 'chunked' and backward[0].grid[0] < n * K.norm_plan(n, s, c, groups, True).spans
+    check_norm((n, s, c) if s > 1 else (n, c), groups, 'silu')

@@ -107,3 +107,18 @@ def test_single_steps_of_two_gigabytes_and_more_are_planned(b, c):
         vec = 4 if '_v4' in launch.kernel else 1
         assert T == tiles == 1 and strips * C == b * c * cstrips and cstrips * (vec << log2_w) >= C and launch.grid[0] == strips
         assert 4 * ((256 >> log2_w) * int(launch.kernel.split('_l')[1].split('_')[0]) * C + (vec << log2_w)) < 2**31 and launch.grid[0] * 256 < 2**32
+
+
+# ------------------------------------------------------------------ what a group norm's gradient needs beside its operands
+
+@pytest.mark.parametrize('n,s,groups,cg', [(8192, 1, 1, 16384), (8192, 1, 1, 16388), (8192, 1, 1, 8195), (4096, 4, 1, 8192), (100000, 2, 1, 8193), (5000, 15, 1, 9000), (4096, 16, 1, 9000), (64, 3136, 32, 8),
+                                           (3000, 1, 2, 40000)])
+def test_the_sums_of_channels_take_less_than_the_samples(n, s, groups, cg):
+    c, taken = groups * cg, []
+
+    def scratch(shape, dtype=np.float32):
+        taken.append(int(np.prod(shape)))
+        return buffer(*shape, dtype=dtype)
+    x, small, stats = buffer(n, s, c), buffer(c), buffer(n, groups)
+    K.group_norm_grad(x, small, small, x, x, small, small, stats, stats, groups, 1e-5, None, scratch)
+    assert sum(taken) <= max(n * s * c // 4, 2 * 1024 * c)

@@ -836,38 +836,55 @@ __device__ __forceinline__ void walk_gradient(const NormParams& P, const Span<VE
     }
 }
 
+// A block takes one sample after the other, as many apart as there are blocks for each chunk and span (of most sizes: one), and leaves one row of sums for dscale
+// and dshift of all of them. (A row for each of many samples of few positions would be as large as the samples.)
 template <int VEC>
 __device__ __forceinline__ void grad_sums_body(float* partial, float* dscale_rows, float* dshift_rows, const float* gs, const float* x, const float* scale, const float* shift,
                                                const float* means, const float* rstds, const NormParams& P) {
-    const Chunk chunk(P, false);
+    Chunk chunk(P, false);
     const Span<VEC> span(P, chunk.number);
     constexpr int U = 4;
-    float rstd[VEC], gamma[VEC], A[VEC], B[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { A[j] = 0.f; B[j] = 0.f; }
-    walk_gradient<VEC, U>(P, span, chunk, gs, x, scale, shift, means, rstds, rstd, gamma, [&](const float (&hat)[U][VEC], const float (&d)[U][VEC], uint32_t here, uint32_t) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            float a = 0.f, b = 0.f;
-#pragma unroll
-            for (int k = 0; k < U; ++k) { const float dk = (uint32_t)k < here ? d[k][j] : 0.f; a += dk; b = (uint32_t)k < here ? __builtin_fmaf(dk, hat[k][j], b) : b; }
-            A[j] += a; B[j] += b;
-        }
-    });
-    const uint32_t entries = P.P * P.span;
+    const uint32_t first_n = chunk.n, side = gridDim.x / (P.spans * P.chunks), entries = P.P * P.span;
     float* const firsts = room, * const seconds = room + entries;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-        if (span.p < P.P && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = A[j]; seconds[span.p * P.span + span.col * VEC + j] = B[j]; }
-    __syncthreads();
     const uint32_t piece = P.pieces == 1u ? 0u : chunk.number % P.pieces;
-    JoinSums join{firsts, seconds, scale + span.c0};
-    for_groups(P, span.groups, P.pieces == 1u ? P.cg : span.width, 1u, join, [&](uint32_t, uint32_t g, bool reports, const JoinSums& found) {
-        if (!reports) return;
-        float* const to = partial + 2u * ((((uint64_t)chunk.n * P.G + span.g0 + g) * P.pieces + piece) * P.chunks + chunk.chunk);
-        to[0] = found.a; to[1] = found.b;
-    });
-    const uint64_t to = ((uint64_t)chunk.n * P.chunks + chunk.chunk) * P.C + span.c0;
+    auto leave = [&](const float (&a)[VEC], const float (&b)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (span.p < P.P && span.col * VEC + j < P.span) { firsts[span.p * P.span + span.col * VEC + j] = a[j]; seconds[span.p * P.span + span.col * VEC + j] = b[j]; }
+        __syncthreads();
+    };
+    float rstd[VEC], gamma[VEC], A_total[VEC], B_total[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { A_total[j] = 0.f; B_total[j] = 0.f; }
+    for (; chunk.n < P.N; chunk.n += side) {
+        float A[VEC], B[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { A[j] = 0.f; B[j] = 0.f; }
+        walk_gradient<VEC, U>(P, span, chunk, gs, x, scale, shift, means, rstds, rstd, gamma, [&](const float (&hat)[U][VEC], const float (&d)[U][VEC], uint32_t here, uint32_t) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float a = 0.f, b = 0.f;
+#pragma unroll
+                for (int k = 0; k < U; ++k) { const float dk = (uint32_t)k < here ? d[k][j] : 0.f; a += dk; b = (uint32_t)k < here ? __builtin_fmaf(dk, hat[k][j], b) : b; }
+                A[j] += a; B[j] += b;
+            }
+        });
+        if (chunk.n != first_n) __syncthreads();                          // (what the sample before has left has been read)
+        leave(A, B);
+        JoinSums join{firsts, seconds, scale + span.c0};
+        for_groups(P, span.groups, P.pieces == 1u ? P.cg : span.width, 1u, join, [&](uint32_t, uint32_t g, bool reports, const JoinSums& found) {
+            if (!reports) return;
+            float* const to = partial + 2u * ((((uint64_t)chunk.n * P.G + span.g0 + g) * P.pieces + piece) * P.chunks + chunk.chunk);
+            to[0] = found.a; to[1] = found.b;
+        });
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { A_total[j] += A[j]; B_total[j] += B[j]; }
+    }
+    if (first_n + side < P.N) {                                           // (else they are there)
+        __syncthreads();
+        leave(A_total, B_total);
+    }
+    const uint64_t to = ((uint64_t)first_n * P.chunks + chunk.chunk) * P.C + span.c0;
     write_channel_sums(firsts, seconds, P.P, P.span, span.width, dshift_rows + to, dscale_rows + to);
 }
 

@@ -2364,6 +2364,9 @@ def group_norm(y: tp.Optional[Buffer], mean, rstd, x: Buffer, scale: Buffer, shi
 
 #blocks that the samples held in registers are shared out to, by the sums that each leaves (300 x 49 x 512, us with gradient for 512, 1024, 2048: 53, 44, 47)
 NORM_GRAD_ROWS = 1024
+#positions of whole samples in chunks below which they are shared out likewise: a row for each would be an eighth of them and more (8192 x 16388 in one group, 1.0 GB of
+#rows beside 0.5 GB: 1844 us, by 1024, 4096, 16384 blocks 1678, 1716, 1784; 4096 x 4 x 8192 858, and 821, 857, 916)
+NORM_ROWS_SHARED = 16
 
 
 def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shift: Buffer, mean: Buffer, rstd: Buffer, groups: int, eps: float,
@@ -2375,7 +2378,10 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     of_groups = max(plan.span // cg, 1)
     rest  = [(b, 0) for b in (g, x, scale, shift, mean, rstd)]
     sets  = _cdiv(n, plan.M)
-    rows  = _cdiv(sets, _cdiv(sets, max(1, NORM_GRAD_ROWS // plan.spans))) if plan.kind != 'chunked' else n * plan.chunks      #(as many sets each)
+    if plan.kind != 'chunked' or (plan.chunks == 1 and s < NORM_ROWS_SHARED):
+        rows = _cdiv(sets, _cdiv(sets, max(1, NORM_GRAD_ROWS // plan.spans)))      #(as many sets each)
+    else:
+        rows = n * plan.chunks
     #a single row of sums is what they add up to
     dscale_rows, dshift_rows = (dscale or scratch((c,)), dshift or scratch((c,))) if rows == 1 else (scratch((rows, c)), scratch((rows, c)))
     if plan.kind != 'chunked':
@@ -2386,7 +2392,7 @@ def group_norm_grad(dx, dscale, dshift, g: Buffer, x: Buffer, scale: Buffer, shi
     else:
         partial = scratch((n, groups, plan.pieces, plan.chunks, 2))
         blocks  = n * plan.chunks * plan.spans
-        launches = [_norm_launch(f'group_norm_grad_sums_v{plan.vec}', blocks, *args, 2 * plan.P * plan.span,
+        launches = [_norm_launch(f'group_norm_grad_sums_v{plan.vec}', rows * plan.spans, *args, 2 * plan.P * plan.span,
                                  [(partial, 0), (dscale_rows, 0), (dshift_rows, 0)] + rest, 4 * (2 * x.size + 2 * rows * c), written=(0, 1, 2))]
         if dx is not None:
             launches.append(_norm_launch(f'group_norm_grad_apply_v{plan.vec}', blocks, *args, 2 * of_groups, [(dx, 0), (partial, 0)] + rest,
