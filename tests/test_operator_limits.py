@@ -11,7 +11,7 @@ from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.csrc import build
 from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
-lax, f32 = mj.lax, np.float32
+lax, nn, f32 = mj.lax, mj.nn, np.float32
 
 
 # ------------------------------------------------------------------ recurrences: what a tile's descriptor covers
@@ -122,3 +122,23 @@ def test_the_sums_of_channels_take_less_than_the_samples(n, s, groups, cg):
     x, small, stats = buffer(n, s, c), buffer(c), buffer(n, groups)
     K.group_norm_grad(x, small, small, x, x, small, small, stats, stats, groups, 1e-5, None, scratch)
     assert sum(taken) <= max(n * s * c // 4, 2 * 1024 * c)
+
+
+# ------------------------------------------------------------------ what recurrences keep from launch to launch
+
+@pytest.mark.parametrize('two_lanes', [False, True])
+def test_recurrences_that_share_their_tickets_agree_on_everything_that_counts_them(two_lanes):
+    '''Launches with one array of tickets and words have one kernel, one grid and one tiling, and run on one lane.'''
+    def f(a, b, c):
+        outs = [lax.linear_recurrence(v, v, reverse=r)[0] for v in (a, b, c) for r in (False, True)]
+        outs += [nn.gated_recurrence(v, v)[1] for v in (a, b, c)]
+        return outs + [mj.grad(lambda v: mj.numpy.sum(nn.gated_recurrence(v, v)[0]))(v) for v in (a, b, c)]
+    args = [np.zeros(shape, f32) for shape in ((2, 2000, 64), (2, 2001, 64), (4, 2000, 36))]
+    program = JaxprInterpreter(mj.make_jaxpr(f)(*args), plan_only=True, two_lanes=two_lanes)
+    sharing, lanes = {}, program.lane_plan.lane if two_lanes else [0] * len(program.launches)
+    for launch, lane in zip(program.launches, lanes):
+        if launch.kernel.startswith('recurrence') and launch.kernel.endswith('_chain'):
+            chain, = (launch.buffers[i][0] for i in launch.scratch)
+            same = (launch.kernel, launch.grid, bytes(launch.params[12:36]), lane)      #(strips, tiles, lines of tickets, their parts, lanes)
+            assert sharing.setdefault(id(chain), same) == same
+    assert len(sharing) >= 6

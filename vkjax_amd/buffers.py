@@ -211,8 +211,11 @@ class BufferPool:
         return self.buffers[key]
 
     def zeroed_scratch(self, n_words: int, use: str = '') -> Buffer:
-        '''n_words of uint32 that hold zeros when the program is built and are never handed to anything else.
-        Launches that use them leave them zero again, so launches of one size and use share one array.'''
+        '''n_words of uint32 that hold zeros when the program is built and are never handed to anything else, for launches of one
+        size and use that run one after the other. Such launches leave what the next one of them expects: counters are zero again;
+        a recurrence's tickets count on, and its words keep the parity of the launch that wrote them (recurrence.hip). So a
+        use names everything that such a launch has to agree on with the one before - there the kernel, the tiling and with it the
+        grid -, and nobody else writes to the array, not even zeros: a launch would wait for words that are not to come.'''
         key = ('zeroed', int(n_words), use)
         if key not in self.buffers:
             b = Buffer(self.device.tensor(np.zeros(n_words, np.uint32)), np.dtype('uint32'), (n_words,))
@@ -232,7 +235,8 @@ class BufferPool:
         return b
 
     def second_set(self, b: Buffer) -> Buffer:
-        '''Scratch like `b` (one of the two kinds above, with storage) that is not `b`, for launches that run beside those using `b`.'''
+        '''Scratch like `b` (one of the two kinds above, with storage; zeros as in the beginning) that is not `b`, for launches that run
+        beside those using `b`.'''
         key = next(k for k, other in self.buffers.items() if other is b)
         key = key[:-1] + (f'{key[-1]}, second set',)
         if key not in self.buffers:

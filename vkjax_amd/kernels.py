@@ -103,7 +103,8 @@ class Launch(tp.NamedTuple):
     streamable: bool = False
     #which of `buffers` the kernel writes (positions); everything else it only reads
     written: tp.Tuple[int, ...] = (0,)
-    #which of `buffers` are scratch that other launches use too and that holds nothing (counters: zeros) between launches
+    #which of `buffers` are scratch that other launches use too: nothing in it is a result, and launches that share it run one after
+    #the other, each leaving what the next one expects (BufferPool.zeroed_scratch)
     scratch: tp.Tuple[int, ...] = ()
     #which of `buffers` a streamable kernel's flag is about (positions)
     streamed: tp.Tuple[int, ...] = (0,)

@@ -68,8 +68,9 @@ def touched_and_written(op, launch) -> tp.Tuple[tp.Set[int], tp.Set[int]]:
 
 
 def with_scratch_of_their_lane(launches, plan_: 'LanePlan', second_set: tp.Callable) -> tp.List:
-    '''The launches, those on the second lane with a second set of the scratch arrays that products with a shared contraction have in
-    common and that hold nothing from one launch to the next (kernels.Launch.scratch).'''
+    '''The launches, those on the second lane with a second set of the scratch arrays that launches of one kind have in common
+    (kernels.Launch.scratch: those of products with a shared contraction, and of recurrences over several tiles of time). A set
+    belongs to its lane for good: what a launch leaves there, the next one on that lane finds.'''
     def moved(launch):
         return launch._replace(buffers=[(second_set(b), offset) if i in launch.scratch else (b, offset)
                                         for i, (b, offset) in enumerate(launch.buffers)])
