@@ -16,14 +16,15 @@
 //     block. 1 x 7 x 7 x 512 5 us, as long as a launch and its three round trips to memory take; 32 x 56 x 56 x 64 in 32 groups 16 us (51 MB,
 //     3.2 TB/s: every block reads, waits and writes once, and there are no more blocks than CUs to take turns; by half or quarter
 //     lines, 512 or 1024 threads, 15.7-17).
-//   * group_norm_rows: samples of one position, several rows to a block (8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5; rows go
-//     through shared memory, because groups of 65 channels do not begin where vectors do; groups of 64 16.5 and 25).
+//   * group_norm_rows: samples of one position, several rows to a block. 8191 x 1040 in 16 groups 17 us, 4.0 TB/s; its gradient 29, 3.5: a block loads, puts its rows
+//     into shared memory, waits, sums, waits and stores, with nothing of the next rows on the way. (They go through shared memory because groups of 65 channels do
+//     not begin where vectors do; groups of 64 take 16.5 and 25 by the same kernels.)
 //   * group_norm_wide: samples of one position with wide groups (layer norms): a block to a group, several vectors to a thread, a sum over the block
-//     for the mean and one for the deviations from it. 8191 x 8192 82 us, 6.5 TB/s, its gradient 175, 4.6: every row waits for its two sums, with
-//     four waves to a SIMD; 8191 x 1021 16 and 25.
+//     for the mean and one for the deviations from it. 8191 x 8192 82 us, 6.5 TB/s, its gradient 175, 4.6: every row waits for its two sums, one after
+//     the other, before the next one's operands are asked for, with four waves to a SIMD; 8191 x 1021 16 and 25.
 //   * group_norm_stats / _apply: the others are cut along their positions. The first launch leaves mean and squared deviations of each
 //     chunk, the second joins a sample's chunks and reads x again (from the caches where they hold it). 64 x 56 x 56 x 256: 35 and 68 us, and
-//     71 and 107 for the gradient's two, all at 5.8-6.1 TB/s: bound by memory, and by reading everything twice. (Each launch
+//     68 and 107 for the gradient's two, all at 5.8-6.1 TB/s: bound by memory, and by reading everything twice. (Each launch
 //     begins where the one before it ended, for what the caches still hold.)
 // The gradient has the same forms; what dscale and dshift get from a block is a row of sums per block, added up by a last launch
 // (group_norm_columns) in a fixed order: no atomics.

@@ -7,8 +7,8 @@
 // One pass over the data. A block takes a tile: W lanes of VEC channels each, and 256 / W groups of L steps that follow one another.
 // A thread reads its L steps into registers and composes them to one map h -> A h + H; maps compose to maps
 // (A2 (A1 h + H1) + H2), so a scan across the lanes of a wave and the four waves tells every thread the map in front of its own
-// steps. What is still missing is the state in front of the tile; with it a thread goes through its steps once more, from
-// registers, and stores. Groups of 8 lanes x 4 channels read whole lines of 128 bytes of every step, 32 KB per wave in flight.
+// steps. What is still missing is the state in front of the tile (below: single-pass scans with look-back, as published for prefix sums);
+// with it a thread goes through its steps once more, from registers, and stores. Groups of 8 lanes x 4 channels read whole lines of 128 bytes of every step, 32 KB per wave in flight.
 //
 // The state in front of a tile (where time has more than one): tiles hand it on within the launch. A tile publishes its map (A, H) as
 // soon as it has it, and the state behind it as soon as it knows that; it looks at the WINDOW tiles before it until one of them
