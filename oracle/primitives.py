@@ -931,3 +931,119 @@ def linear_recurrence_grad(h, factor, x, *rest, gated, reverse, has_state, has_l
             df[:, t], dx[:, t] = np.where(inside[:, t], df[:, t], 0.0), np.where(inside[:, t], dx[:, t], 0.0)
             adjoint = np.where(inside[:, t], adjoint * a[:, t], adjoint)
         return df.astype(f32), dx.astype(f32), adjoint.astype(f32)
+
+
+def _sequence_ends(lengths, batch, time):
+    return np.full(batch, time) if lengths is None else np.clip(np.asarray(lengths, np.int64), 0, time)
+
+
+def _optional(rest, *flags):
+    rest = list(rest)
+    return [np.asarray(rest.pop(0)) if flag else None for flag in flags]
+
+
+def _silu64(z):
+    s = 1.0 / (1.0 + np.exp(-z))
+    return z * s, s * (1.0 + z * (1.0 - s))
+
+
+def _causal_conv64(x, kernel, bias, state, lengths, activation):
+    '''(rows of each sequence with the state in front, where they have ended, z, y, dy/dz)'''
+    (batch, time, channels), width = x.shape, kernel.shape[0]
+    ends   = _sequence_ends(lengths, batch, time)
+    inside = np.arange(time)[None, :, None] < ends[:, None, None]
+    front  = np.zeros((batch, width - 1, channels)) if state is None else np.asarray(state, np.float64)
+    rows   = np.concatenate([front, np.where(inside, np.asarray(x, np.float64), 0.0)], axis=1)
+    z = np.zeros(x.shape) if bias is None else np.broadcast_to(np.asarray(bias, np.float64), x.shape)
+    for k in range(width):
+        z = z + np.asarray(kernel[k], np.float64) * rows[:, k:k + time]
+    y, slope = _silu64(z) if activation == 'silu' else (z, np.ones_like(z))
+    return rows, ends, inside, np.where(inside, y, 0.0), np.where(inside, slope, 0.0)
+
+
+def causal_conv(x, kernel, *rest, activation, has_bias, has_state, has_lengths):
+    bias, state, lengths = _optional(rest, has_bias, has_state, has_lengths)
+    width = kernel.shape[0]
+    with np.errstate(**_EW_ERR):
+        rows, ends, _, y, _ = _causal_conv64(x, kernel, bias, state, lengths, activation)
+        last = np.stack([rows[i, n:n + width - 1] for i, n in enumerate(ends)]) if len(ends) else rows[:, :width - 1]
+        return y.astype(f32), last.astype(f32)
+
+
+def causal_conv_grad(x, kernel, *rest, activation, has_bias, has_state, has_lengths, has_g, has_last):
+    bias, state, lengths, g, g_last = _optional(rest, has_bias, has_state, has_lengths, has_g, has_last)
+    (batch, time, channels), width = x.shape, kernel.shape[0]
+    with np.errstate(**_EW_ERR):
+        rows, ends, inside, _, slope = _causal_conv64(x, kernel, bias, state, lengths, activation)
+        d = np.where(inside, slope * np.asarray(g, np.float64), 0.0) if g is not None else np.zeros(x.shape)
+        drows, dkernel = np.zeros_like(rows), np.zeros(kernel.shape)
+        for k in range(width):
+            drows[:, k:k + time] += np.asarray(kernel[k], np.float64) * d
+            dkernel[k] = (d * np.where(inside, rows[:, k:k + time], 0.0)).sum(axis=(0, 1))
+        if g_last is not None:
+            for i, n in enumerate(ends):
+                drows[i, n:n + width - 1] += np.asarray(g_last[i], np.float64)
+        outs = [np.where(inside, drows[:, width - 1:], 0.0), dkernel]
+        outs += ([d.sum(axis=(0, 1))] if has_bias else []) + ([drows[:, :width - 1]] if has_state else [])
+        return tuple(v.astype(f32) for v in outs)
+
+
+def _selective_scan64(x, delta, a, b, c, d, gate, state, lengths, bias, softplus):
+    (batch, time, channels), n = x.shape, a.shape[1]
+    ends   = _sequence_ends(lengths, batch, time)
+    inside = np.arange(time)[None, :, None] < ends[:, None, None]
+    clean  = lambda v: np.where(inside, np.asarray(v, np.float64), 0.0)
+    x, delta, b, c = clean(x), clean(delta), clean(b), clean(c)
+    pre = delta if bias is None else delta + np.asarray(bias, np.float64)
+    w   = np.where(inside, np.maximum(pre, 0.0) + np.log1p(np.exp(-np.abs(pre))) if softplus else pre, 0.0)
+    a   = np.asarray(a, np.float64)
+    h   = np.zeros((time + 1, batch, channels, n))
+    if state is not None:
+        h[0] = state
+    for t in range(time):
+        taken = inside[:, t, :, None]
+        step  = np.exp(w[:, t, :, None] * a) * h[t] + (w[:, t] * x[:, t])[:, :, None] * b[:, t, None, :]
+        h[t + 1] = np.where(taken, step, h[t])
+    seen = np.einsum('tbcn,btn->btc', h[1:], c) + (0.0 if d is None else np.asarray(d, np.float64) * x)
+    open_, slope = _silu64(clean(gate)) if gate is not None else (np.ones_like(x), np.zeros_like(x))
+    return ends, inside, x, b, c, a, pre, w, h, seen, open_, slope
+
+
+def selective_scan(x, delta, a, b, c, *rest, softplus, kept, has_d, has_gate, has_state, has_lengths, has_bias):
+    d, gate, state, lengths, bias = _optional(rest, has_d, has_gate, has_state, has_lengths, has_bias)
+    with np.errstate(**_EW_ERR):
+        _, inside, _, _, _, _, _, _, h, seen, open_, _ = _selective_scan64(x, delta, a, b, c, d, gate, state, lengths, bias, softplus)
+        outs = [np.where(inside, seen * open_, 0.0), h[-1]]
+        if kept:
+            outs.append(h[:-1][::8].transpose(0, 1, 3, 2))
+        return tuple(v.astype(f32) for v in outs)
+
+
+def selective_scan_grad(kept, x, delta, a, b, c, *rest, softplus, has_d, has_gate, has_state, has_lengths, has_bias, has_g, has_last):
+    d, gate, state, lengths, bias, g, g_last = _optional(rest, has_d, has_gate, has_state, has_lengths, has_bias, has_g, has_last)
+    time = x.shape[1]
+    with np.errstate(**_EW_ERR):
+        _, inside, x, b, c, a, pre, w, h, seen, open_, slope = _selective_scan64(x, delta, a, b, c, d, gate, state, lengths, bias, softplus)
+        g  = np.where(inside, np.asarray(g, np.float64), 0.0) if g is not None else np.zeros_like(x)
+        gy = g * open_
+        l  = np.zeros(h.shape[1:]) if g_last is None else np.asarray(g_last, np.float64)
+        dx, dw, db, dc, da = np.zeros_like(x), np.zeros_like(x), np.zeros_like(b), np.zeros_like(c), np.zeros_like(a)
+        for t in range(time - 1, -1, -1):
+            f = np.exp(w[:, t, :, None] * a)
+            l = l + gy[:, t, :, None] * c[:, t, None, :]
+            dc[:, t] = (gy[:, t, :, None] * h[t + 1]).sum(axis=1)
+            lb = (l * b[:, t, None, :]).sum(axis=2)
+            db[:, t] = (l * (w[:, t] * x[:, t])[:, :, None]).sum(axis=1)
+            l = l * f
+            e = l * h[t]
+            da += (e * w[:, t, :, None]).sum(axis=0)
+            dw[:, t] = (e * a).sum(axis=2) + lb * x[:, t]
+            dx[:, t] = lb * w[:, t] + (0.0 if d is None else np.asarray(d, np.float64) * gy[:, t])
+        clean  = lambda v: np.where(inside, v, 0.0)
+        ddelta = clean(dw / (1.0 + np.exp(-pre)) if softplus else dw)
+        outs = [clean(dx), ddelta, da, clean(db), clean(dc)]
+        outs += [(gy * x).sum(axis=(0, 1))] if has_d else []
+        outs += [clean(g * seen * slope)] if has_gate else []
+        outs += [l] if has_state else []
+        outs += [ddelta.sum(axis=(0, 1))] if has_bias else []
+        return tuple(v.astype(f32) for v in outs)

@@ -1,0 +1,216 @@
+'''Short causal convolutions and selective scans on the GPU against their definitions in 64 bits (the oracle), at the sizes, lengths and
+options where they can go wrong.
+
+Tolerances. u = 2^-24 is half a step of fp32. Every multiply-add, product and sum is off by u of its result; a sum of n terms one after the other by at most n u
+times the sum of their magnitudes. The sigmoid 1 / (1 + exp2(-z log2 e)) is off by (2 |z| + 6) u of itself (its exponent is rounded twice, the exponential and the
+reciprocal are off by at most 2 u each).'''
+import numpy as np
+import pytest
+
+from tests.test_gpu_operators import U, both, close
+from tests.test_operators import normal
+from tests.test_token_model_operators import OPTIONAL, scan_inputs, scan_program
+from vkjax_amd import minijax as mj
+
+pytestmark = pytest.mark.gpu
+jnp, lax, nn = mj.numpy, mj.lax, mj.nn
+f32 = np.float32
+
+
+def inside_of(shape, lengths):
+    return np.ones((shape[0], shape[1], 1), bool) if lengths is None else np.arange(shape[1])[None, :, None] < np.clip(np.asarray(lengths), 0, shape[1])[:, None, None]
+
+
+def spoiled(v, inside):
+    '''What stands behind a sequence's end is not to be looked at.'''
+    return np.where(inside, v, np.where(np.arange(v.shape[1])[None, :, None] % 2 == 0, np.nan, np.inf)).astype(f32)
+
+
+# ------------------------------------------------------------------ short causal convolutions
+
+def conv_program(lengths, activation, bias, state):
+    def f(x, kernel, g, g_last, *rest):
+        given = dict(zip([n for n, has in (('bias', bias), ('state', state)) if has], rest))
+        outs, pullback = mj.vjp(lambda x, kernel, given: nn.causal_conv(x, kernel, lengths=lengths, activation=activation, **given), x, kernel, given)
+        dx, dkernel, rest = pullback((g, g_last))
+        return tuple(outs) + (dx, dkernel) + tuple(rest[n] for n in ('bias', 'state') if n in rest)
+    return f
+
+
+def conv_bounds(x, kernel, g, g_last, bias, state, lengths, activation):
+    (batch, time, channels), width = x.shape, kernel.shape[0]
+    inside = inside_of(x.shape, lengths)
+    front = np.zeros((batch, width - 1, channels)) if state is None else np.abs(state.astype(np.float64))
+    rows = np.concatenate([front, np.where(inside, np.abs(x.astype(np.float64)), 0.0)], axis=1)
+    k = np.abs(kernel.astype(np.float64))
+    size = sum(k[i] * rows[:, i:i + time] for i in range(width)) + (0 if bias is None else np.abs(bias.astype(np.float64)))
+    e_z = (width + 1) * U * size
+    #silu and its slope: at most 1.1 and |z| + 1 times as large as what they are taken of, slopes at most 1.1 and 0.5
+    silu = activation == 'silu'
+    e_y = 1.1 * e_z + (2 * size + 10) * U * size if silu else e_z
+    e_slope = 0.5 * e_z + (2 * size + 12) * U * (size + 1) if silu else 0 * e_z
+    gs = np.where(inside, np.abs(g.astype(np.float64)), 0.0)
+    d, e_d = 1.1 * gs, gs * e_slope + 2 * U * gs
+    drows, e_drows = np.zeros_like(rows), np.zeros_like(rows)
+    n = batch * time                                            #terms of the sums over time
+    dkernel = np.zeros(k.shape)
+    for i in range(width):
+        drows[:, i:i + time] += k[i] * d
+        e_drows[:, i:i + time] += k[i] * e_d
+        dkernel[i] = (e_d * rows[:, i:i + time] + (n + 2) * U * d * rows[:, i:i + time]).sum(axis=(0, 1))
+    for i in range(batch):
+        end = time if lengths is None else min(max(int(lengths[i]), 0), time)
+        drows[i, end:end + width - 1] += np.abs(g_last[i])
+    e_drows += (width + 1) * U * drows
+    tiny = 1e-37
+    last = np.zeros((batch, width - 1, channels))
+    found = [e_y + tiny, last, e_drows[:, width - 1:] + tiny, dkernel + tiny]
+    return found + ([(e_d + (n + 1) * U * d).sum(axis=(0, 1)) + tiny] if bias is not None else []) + ([e_drows[:, :width - 1] + tiny] if state is not None else [])
+
+
+#(shape, width, lengths): one of everything, time shorter than the window, odd channels, more than a tile along time and along channels, steps that are no multiple of a thread's
+CONVS = [((1, 1, 1), 2, None), ((2, 1, 64), 4, None), ((2, 1, 64), 4, [0, 1]), ((3, 2, 5), 8, [2, 0, 1]), ((2, 17, 36), 3, [17, 5]), ((1, 300, 8), 4, None), ((4, 33, 130), 5, [33, 32, 2, 0]),
+         ((2, 64, 1028), 4, [64, 63]), ((1, 7, 333), 6, [-3]), ((2, 1021, 12), 4, [2000, 700]), ((3, 130, 257), 7, [1, 129, 130]), ((5, 8, 4), 8, [7, 8, 6, 3, 0]), ((1, 5000, 4), 2, None),
+         ((40, 9, 32), 4, None)]
+
+
+@pytest.mark.parametrize('options', [(None, True, True), ('silu', True, False), ('silu', False, True), (None, False, False)], ids=str)
+@pytest.mark.parametrize('shape,width,lengths', CONVS, ids=str)
+def test_causal_conv_and_gradient(shape, width, lengths, options):
+    print(f'causal conv {shape} by {width}, lengths {lengths}, {options}', flush=True)
+    activation, has_bias, has_state = options
+    inside = inside_of(shape, lengths)
+    x, kernel, g = normal(1, *shape), normal(2, width, shape[2]), normal(3, *shape)
+    g_last, bias, state = normal(4, shape[0], width - 1, shape[2]), normal(5, shape[2]) if has_bias else None, normal(6, shape[0], width - 1, shape[2]) if has_state else None
+    n = None if lengths is None else np.array(lengths, np.int32)
+    rest = [v for v in (bias, state) if v is not None]
+    got, expected, _ = both(conv_program(n, activation, has_bias, has_state), spoiled(x, inside), kernel, spoiled(g, inside), g_last, *rest)
+    names = ['y', 'last', 'dx', 'dkernel'] + ['dbias'] * has_bias + ['dstate'] * has_state
+    for name, a, b, bound in zip(names, got, expected, conv_bounds(x, kernel, g, g_last, bias, state, lengths, activation)):
+        close(a, b, bound, name)
+
+
+def test_causal_conv_keeps_what_is_not_finite_to_its_window():
+    x, kernel = normal(1, 2, 40, 8), normal(2, 4, 8)
+    x[0, 10, 3], x[1, 20, 5] = np.nan, np.inf
+    got, expected, _ = both(lambda x, k: nn.causal_conv(x, k, activation=None), x, kernel)
+    assert np.array_equal(np.isfinite(got[0]), np.isfinite(expected[0])) and (~np.isfinite(got[0])).sum() == 8
+
+
+# ------------------------------------------------------------------ selective scans
+
+def scan_bounds(v, g, g_last, lengths, softplus):
+    '''How far every result of scan_program may be off. Along with the magnitudes H of the states and L of their adjoints (everything positive) goes a bound of their
+    errors; a factor exp(w a) is off by what its exponent is (rounded thrice, and w a sum over up to a chunk's steps, T terms) and 2 u.'''
+    x, a = v['x'].astype(np.float64), v['a'].astype(np.float64)
+    (batch, time, channels), n = x.shape, a.shape[1]
+    inside = inside_of(x.shape, lengths)
+    clean = lambda w: np.where(inside, w.astype(np.float64), 0.0)
+    magnitude = lambda name: np.abs(clean(v[name])) if name in v else None
+    pre = clean(v['delta']) + (v['delta_bias'].astype(np.float64) if 'delta_bias' in v else 0.0)
+    #delta + bias is rounded; softplus' series, reciprocal, exponential: (|v| + 14) u of itself, and its slope is at most itself (log(1 + e^v) >= sigmoid(v) / 2 for v <= 0.. so 2 times)
+    rounded = U * (np.abs(clean(v['delta'])) + (np.abs(v['delta_bias'].astype(np.float64)) if 'delta_bias' in v else 0.0))
+    w = np.where(inside, np.maximum(pre, 0) + np.log1p(np.exp(-np.abs(pre))) if softplus else pre, 0.0)
+    e_w = np.where(inside, 2 * rounded * np.minimum(w, 1) + (2 * np.abs(pre) + 14) * U * w if softplus else rounded, 0.0)
+    xs, bs, cs = np.abs(clean(v['x'])), magnitude('b'), magnitude('c')
+    D = np.abs(v['d'].astype(np.float64)) if 'd' in v else 0.0
+    open_, e_open, slope = 1.0, 0.0, 0.0
+    if 'gate' in v:
+        z = clean(v['gate'])
+        open_, e_open, slope = np.abs(z / (1 + np.exp(-z))), (2 * np.abs(z) + 10) * U * np.abs(z / (1 + np.exp(-z))), 1.1
+    gs = np.abs(clean(g))
+    f = np.exp(w[..., None] * a)
+    k = f * ((time + 5) * U * np.abs(w[..., None] * a) + e_w[..., None] * np.abs(a) + 2 * U)            #how far a factor is off
+    u = w * xs
+    e_u = e_w * xs + U * u
+    H, E = np.zeros((time + 1, batch, channels, n)), np.zeros((time + 1, batch, channels, n))
+    if 'state' in v:
+        H[0] = np.abs(v['state'])
+    for t in range(time):
+        add, e_add = u[:, t, :, None] * bs[:, t, None], e_u[:, t, :, None] * bs[:, t, None]
+        H[t + 1] = f[:, t] * H[t] + add
+        E[t + 1] = f[:, t] * E[t] + k[:, t] * (H[t] + E[t]) + e_add + 2 * U * add + U * H[t + 1]
+        E[t + 1], H[t + 1] = np.where(inside[:, t, :, None], E[t + 1], E[t]), np.where(inside[:, t, :, None], H[t + 1], H[t])
+    seen = np.einsum('tbcn,btn->btc', H[1:], cs) + D * xs
+    e_seen = np.einsum('tbcn,btn->btc', E[1:], cs) + (n + 3) * U * seen
+    e_y = np.where(inside, e_seen * open_ + seen * e_open + 2 * U * seen * open_, 0)
+    gy, e_gy = gs * open_, gs * e_open + 2 * U * gs * open_
+    #slope of silu: (|z| + 1)(..), off by some (2 |z| + 12) u of (|z| + 1)
+    e_dgate = gs * (slope * e_seen + seen * (2 * np.abs(clean(v['gate'])) + 12) * (np.abs(clean(v['gate'])) + 1) * U) if 'gate' in v else None
+    L, F = np.abs(g_last.astype(np.float64)), np.zeros((batch, channels, n))
+    e_dx, e_dw, e_db, e_dc, e_da, e_dd = np.zeros_like(x), np.zeros_like(x), np.zeros_like(bs), np.zeros_like(cs), np.zeros_like(a), 0.0
+    dw = np.zeros_like(x)
+    rows = batch * time                                         #terms of sums over time
+    absa = np.abs(a)
+    for t in range(time - 1, -1, -1):
+        add = gy[:, t, :, None] * cs[:, t, None]
+        L = L + add
+        F = F + e_gy[:, t, :, None] * cs[:, t, None] + U * L
+        e_dc[:, t] = (gy[:, t, :, None] * E[t + 1] + e_gy[:, t, :, None] * H[t + 1] + (channels + 2) * U * gy[:, t, :, None] * H[t + 1]).sum(axis=1)
+        lb, e_lb = (L * bs[:, t, None]).sum(axis=2), ((F + (n + 1) * U * L) * bs[:, t, None]).sum(axis=2)
+        e_db[:, t] = ((F + (channels + 2) * U * L) * u[:, t, :, None] + L * e_u[:, t, :, None]).sum(axis=1)
+        back, e_back = f[:, t] * L, f[:, t] * F + k[:, t] * (L + F) + U * f[:, t] * L
+        e, e_e = back * H[t], back * E[t] + e_back * (H[t] + E[t]) + U * back * H[t]
+        e_da += ((e_e + (rows + 2) * U * e) * w[:, t, :, None] + e * e_w[:, t, :, None]).sum(axis=0)
+        dw[:, t] = (e * absa).sum(axis=2) + lb * xs[:, t]
+        e_dw[:, t] = ((e_e + (n + 5) * U * e) * absa).sum(axis=2) + e_lb * xs[:, t] + 3 * U * dw[:, t]
+        e_dx[:, t] = e_lb * w[:, t] + lb * e_w[:, t] + D * e_gy[:, t] + 3 * U * (lb * w[:, t] + D * gy[:, t])
+        L, F = np.where(inside[:, t, :, None], back, L), np.where(inside[:, t, :, None], e_back, F)
+    e_ddelta = np.where(inside, e_dw + dw * ((np.abs(pre) + 10) * U + rounded) if softplus else e_dw, 0)
+    e_dd = (e_gy * xs + (rows + 2) * U * gy * xs).sum(axis=(0, 1))
+    found = dict(x=np.where(inside, e_dx, 0), delta=e_ddelta, a=e_da, b=np.where(inside, e_db, 0), c=np.where(inside, e_dc, 0), d=e_dd,
+                 gate=None if e_dgate is None else np.where(inside, e_dgate, 0), state=F + U * L, delta_bias=(e_ddelta + (rows + 2) * U * np.where(inside, dw, 0)).sum(axis=(0, 1)))
+    return [b + 1e-36 for b in [e_y, E[time]] + [found[name] for name in v]]
+
+
+#(batch, time, channels, states, lengths): single steps; states that are no power of two and channels that are no multiple of a wave's; time in chunks (several hundred
+#steps), with sequences that end in the first chunk, at its border and behind it; more states than a wave holds
+SCANS = [(1, 1, 1, 1, None), (2, 1, 64, 16, None), (3, 1, 5, 7, [0, 1, 1]), (2, 1, 33, 64, None), (1, 2, 3, 4, None), (2, 9, 70, 5, [9, 3]), (1, 130, 64, 16, None), (2, 300, 33, 16, [300, 0]),
+         (1, 700, 8, 24, None), (2, 257, 65, 64, [64, 257]), (3, 64, 130, 8, [8, 16, 63]), (1, 1000, 4, 3, None), (4, 40, 200, 2, [40, 1, 39, -5]), (2, 513, 128, 16, [512, 4000]), (1, 129, 1, 33, None),
+         (9, 15, 16, 12, None)]
+
+
+@pytest.mark.parametrize('given,softplus', [(OPTIONAL, True), (('gate',), False), (('d', 'state'), True), ((), False), (('delta_bias', 'state'), False)], ids=str)
+@pytest.mark.parametrize('batch,time,channels,n,lengths', SCANS, ids=str)
+def test_selective_scan_and_gradient(batch, time, channels, n, lengths, given, softplus):
+    print(f'selective scan {batch} x {time} x {channels} x {n}, lengths {lengths}, {given}, softplus {softplus}', flush=True)
+    arrays, g, g_last = scan_inputs(batch, time, channels, n, given, softplus)
+    inside = inside_of((batch, time), lengths)
+    dirty = {k: spoiled(v, inside) if k in ('x', 'delta', 'b', 'c', 'gate') else v for k, v in arrays.items()}
+    got, expected, _ = both(scan_program(list(arrays), None if lengths is None else np.array(lengths, np.int32), softplus), spoiled(g, inside), g_last, *dirty.values())
+    for name, a, b, bound in zip(['y', 'last'] + [f'd{k}' for k in arrays], got, expected, scan_bounds(arrays, g, g_last, lengths, softplus)):
+        close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('batch,time,channels,n,lengths', SCANS, ids=str)
+def test_selective_scan_alone(batch, time, channels, n, lengths):
+    '''Without a gradient: single steps have a kernel of their own, and no states are kept.'''
+    print(f'selective scan {batch} x {time} x {channels} x {n}, lengths {lengths}', flush=True)
+    for given, softplus in ((OPTIONAL, True), ((), False)):
+        arrays, g, g_last = scan_inputs(batch, time, channels, n, given, softplus, seed=1)
+        inside = inside_of((batch, time), lengths)
+        dirty = {k: spoiled(v, inside) if k in ('x', 'delta', 'b', 'c', 'gate') else v for k, v in arrays.items()}
+        l = None if lengths is None else np.array(lengths, np.int32)
+        names = list(arrays)
+        got, expected, _ = both(lambda *v: nn.selective_scan(**dict(zip(names, v)), lengths=l, softplus=softplus), *dirty.values())
+        for name, a, b, bound in zip(('y', 'last'), got, expected, scan_bounds(arrays, g, g_last, lengths, softplus)):
+            close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('value', [-200.0, -90.0, -30.0, -17.0, -10.0, -1.0, 0.0, 1.0, 20.0, 200.0])
+def test_step_widths_far_out(value):
+    '''softplus where exp(v) is next to nothing beside 1, and where it is infinite.'''
+    arrays, g, g_last = scan_inputs(1, 12, 8, 4, ('state',), True)
+    arrays['delta'] = np.full_like(arrays['delta'], value)
+    got, expected, _ = both(scan_program(list(arrays), None, True), g, g_last, *arrays.values())
+    for name, a, b, bound in zip(['y', 'last'] + [f'd{k}' for k in arrays], got, expected, scan_bounds(arrays, g, g_last, None, True)):
+        close(a, b, bound, name)
+
+
+def test_selective_scan_keeps_what_is_not_finite_to_its_channel():
+    arrays, _, _ = scan_inputs(2, 200, 70, 16, (), False)
+    arrays['x'][0, 100, 66] = np.nan
+    y, last = mj.tree_leaves(both(lambda *v: nn.selective_scan(*v), *arrays.values())[0])
+    broken = np.zeros(y.shape, bool)
+    broken[0, 100:, 66] = True
+    assert np.array_equal(np.isnan(y), broken) and np.isnan(last[0, 66]).all() and np.isfinite(last).sum() == last.size - 16

@@ -1,0 +1,241 @@
+'''Operators of a recurrent token model as programs: what they and their gradients are (the oracle against torch in 64 bits and against
+differences), what is refused, and how they are planned.'''
+import numpy as np
+import pytest
+import torch
+
+from oracle import primitives as P
+from tests.test_operators import ROUNDED, evaluate, normal, refused
+from vkjax_amd import minijax as mj
+from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
+
+jnp, lax, nn = mj.numpy, mj.lax, mj.nn
+f32 = np.float32
+
+
+def leaf(v):
+    return None if v is None else torch.tensor(np.asarray(v, np.float64), requires_grad=True)
+
+
+def same_as_torch(got, expected):
+    for a, b in zip(got, expected):
+        assert np.allclose(a, b.detach().numpy(), **dict(ROUNDED, atol=1e-12)), float(np.abs(a - b.detach().numpy()).max())
+
+
+# ------------------------------------------------------------------ short causal convolutions
+
+def torch_conv(x, kernel, bias, state, ends, silu):
+    '''One sequence after the other, position by position.'''
+    ys, lasts = [], []
+    width = kernel.shape[0]
+    for i, n in enumerate(ends):
+        front = torch.zeros(width - 1, x.shape[2], dtype=x.dtype) if state is None else state[i]
+        rows = torch.cat([front, x[i, :n]])
+        out = [(kernel * rows[t:t + width]).sum(0) + (0 if bias is None else bias) for t in range(n)]
+        y = torch.stack(out) if out else x[i, :0]
+        ys.append(torch.cat([torch.nn.functional.silu(y) if silu else y, torch.zeros_like(x[i, n:])]))
+        lasts.append(rows[n:])
+    return torch.stack(ys), torch.stack(lasts)
+
+
+@pytest.mark.parametrize('activation', [None, 'silu'])
+@pytest.mark.parametrize('width,shape,bias,state,lengths', [(2, (2, 5, 3), True, True, None), (4, (3, 6, 2), True, False, [6, 0, 2]), (8, (2, 3, 4), False, True, [1, 3]),
+                                                            (3, (1, 1, 1), False, False, None), (4, (2, 1, 3), True, True, [0, 1])])
+def test_causal_conv_oracle_is_torchs(width, shape, bias, state, lengths, activation):
+    x, kernel, g, g_last = normal(1, *shape), normal(2, width, shape[2]), normal(3, *shape), normal(4, shape[0], width - 1, shape[2])
+    b, s = normal(5, shape[2]) if bias else None, normal(6, *g_last.shape) if state else None
+    ends = [shape[1]] * shape[0] if lengths is None else lengths
+    n = None if lengths is None else np.array(lengths, np.int32)
+
+    def f(x, kernel, *rest):
+        rest = list(rest)
+        given = dict(bias=rest.pop(0) if bias else None, state=rest.pop(0) if state else None)
+        outs, pullback = mj.vjp(lambda x, kernel, given: nn.causal_conv(x, kernel, lengths=n, activation=activation, **given), x, kernel, given)
+        dx, dkernel, rest = pullback((g, g_last))
+        return tuple(outs) + (dx, dkernel) + tuple(v for v in (rest['bias'], rest['state']) if v is not None)
+    got = evaluate(f, x, kernel, *[v for v in (b, s) if v is not None])
+    leaves = [leaf(v) for v in (x, kernel, b, s)]
+    y, last = torch_conv(*leaves, ends, activation == 'silu')
+    ((y * torch.tensor(g)).sum() + (last * torch.tensor(g_last)).sum()).backward()
+    same_as_torch(got, [y, last] + [v.grad for v in leaves if v is not None])
+
+
+def test_causal_conv_goes_on_token_by_token():
+    x, kernel, bias = normal(1, 2, 7, 3), normal(2, 4, 3), normal(3, 3)
+
+    def whole(x, kernel, bias):
+        return nn.causal_conv(x, kernel, bias, activation='silu')
+
+    def steps(x, kernel, bias):
+        state, ys = None, []
+        for t in range(7):
+            y, state = nn.causal_conv(x[:, t:t + 1], kernel, bias, state, activation='silu')
+            ys.append(y)
+        return jnp.concatenate(ys, axis=1), state
+    for a, b in zip(evaluate(whole, x, kernel, bias), evaluate(steps, x, kernel, bias)):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=np.ones((2, 12), f32)), TypeError), (dict(x=np.ones((2, 3, 4), np.int32)), TypeError), (dict(kernel=np.ones((4, 5), f32)), TypeError),
+    (dict(kernel=np.ones((1, 4), f32)), ValueError), (dict(kernel=np.ones((9, 4), f32)), ValueError), (dict(kernel=np.ones((3, 4), f32)), TypeError),
+    (dict(bias=np.ones(3, f32)), TypeError), (dict(state=np.ones((2, 4, 4), f32)), TypeError), (dict(state=np.ones((2, 3, 4), np.int32)), TypeError),
+    (dict(lengths=np.ones(3, np.int32)), TypeError), (dict(lengths=np.ones(2, f32)), TypeError), (dict(activation='relu'), ValueError)])
+def test_causal_conv_refuses(change, error):
+    given = dict(dict(x=np.ones((2, 3, 4), f32), kernel=np.ones((4, 4), f32), bias=np.ones(4, f32), state=np.ones((2, 3, 4), f32), lengths=np.ones(2, np.int32), activation='silu'), **change)
+    activation = given.pop('activation')
+    refused(error, lambda *a: nn.causal_conv(*a, activation), *given.values())
+    refused(error, lambda *a: lax.causal_conv_grad(*a, None, None, activation), *given.values())
+
+
+def test_causal_conv_gradient_refuses_cotangents_of_other_shapes():
+    x, kernel = np.ones((2, 3, 4), f32), np.ones((4, 4), f32)
+    refused(TypeError, lambda x, k, g: lax.causal_conv_grad(x, k, g=g), x, kernel, np.ones((2, 4, 4), f32))
+    refused(TypeError, lambda x, k, g: lax.causal_conv_grad(x, k, g_last=g), x, kernel, x.repeat(2, 1))
+
+
+# ------------------------------------------------------------------ selective scans
+
+def torch_scan(x, delta, a, b, c, d, gate, state, bias, ends, softplus):
+    ys, lasts = [], []
+    for i, n in enumerate(ends):
+        h = torch.zeros(a.shape, dtype=a.dtype) if state is None else state[i]
+        out = []
+        for t in range(n):
+            w = delta[i, t] if bias is None else delta[i, t] + bias
+            w = torch.nn.functional.softplus(w, threshold=1e9) if softplus else w
+            h = torch.exp(w[:, None] * a) * h + (w * x[i, t])[:, None] * b[i, t]
+            y = h @ c[i, t]
+            y = y if d is None else y + d * x[i, t]
+            out.append(y if gate is None else y * torch.nn.functional.silu(gate[i, t]))
+        ys.append(torch.cat([torch.stack(out), torch.zeros_like(x[i, n:])]) if out else torch.zeros_like(x[i]))
+        lasts.append(h + 0)
+    return torch.stack(ys), torch.stack(lasts)
+
+
+OPTIONAL = ('d', 'gate', 'state', 'delta_bias')
+
+
+def scan_inputs(batch, time, channels, n, given, softplus, seed=0):
+    '''Operands as a model has them: step widths around 0.05, states that decay.'''
+    rng = np.random.default_rng(seed + 7 * time + channels)
+    draw = lambda *s: rng.standard_normal(s).astype(f32)
+    found = dict(x=draw(batch, time, channels),
+                 delta=(0.7 * draw(batch, time, channels) - (0.0 if 'delta_bias' in given else 3.0)).astype(f32) if softplus else (0.01 + 0.1 * rng.random((batch, time, channels))).astype(f32),
+                 a=(-(0.5 + rng.random((channels, n))) * np.arange(1, n + 1)).astype(f32), b=draw(batch, time, n), c=draw(batch, time, n))
+    shapes = dict(d=(channels,), gate=(batch, time, channels), state=(batch, channels, n), delta_bias=(channels,))
+    found.update({name: draw(*shapes[name]) for name in OPTIONAL if name in given})
+    if 'delta_bias' in given:
+        found['delta_bias'] = (found['delta_bias'] - 3.0).astype(f32) if softplus else (0.01 * rng.random(channels)).astype(f32)
+    return found, draw(batch, time, channels), draw(batch, channels, n)
+
+
+def scan_program(names, lengths, softplus):
+    '''Results and gradients of every operand, in the order of `names`.'''
+    def f(g, g_last, *arrays):
+        outs, pullback = mj.vjp(lambda *v: nn.selective_scan(**dict(zip(names, v)), lengths=lengths, softplus=softplus), *arrays)
+        return tuple(outs) + pullback((g, g_last))
+    return f
+
+
+@pytest.mark.parametrize('softplus', [False, True])
+@pytest.mark.parametrize('batch,time,channels,n,given,lengths', [(2, 5, 3, 4, OPTIONAL, None), (3, 6, 2, 1, ('gate',), [6, 0, 2]), (1, 1, 4, 16, ('state', 'delta_bias'), None),
+                                                                 (2, 17, 3, 5, ('d', 'state'), [17, 9]), (2, 9, 1, 3, (), None)])
+def test_selective_scan_oracle_is_torchs(batch, time, channels, n, given, lengths, softplus):
+    arrays, g, g_last = scan_inputs(batch, time, channels, n, given, softplus)
+    got = evaluate(scan_program(list(arrays), None if lengths is None else np.array(lengths, np.int32), softplus), g, g_last, *arrays.values())
+    leaves = {k: leaf(v) for k, v in arrays.items()}
+    y, last = torch_scan(*[leaves[k] for k in ('x', 'delta', 'a', 'b', 'c')], *[leaves.get(k) for k in OPTIONAL], [time] * batch if lengths is None else lengths, softplus)
+    ((y * torch.tensor(g)).sum() + (last * torch.tensor(g_last)).sum()).backward()
+    grad = lambda v: torch.zeros_like(v) if v.grad is None else v.grad
+    same_as_torch(got, [y, last] + [grad(v) for v in leaves.values()])
+
+
+def test_selective_scan_gradient_is_that_of_differences():
+    arrays, g, g_last = scan_inputs(2, 4, 2, 3, OPTIONAL, True)
+    names = list(arrays)
+    flags = dict(softplus=True, has_d=True, has_gate=True, has_state=True, has_lengths=False, has_bias=True)
+
+    def loss(values):
+        _, inside, _, _, _, _, _, _, h, seen, open_, _ = P._selective_scan64(*[values[k] for k in ('x', 'delta', 'a', 'b', 'c', 'd', 'gate', 'state')], None, values['delta_bias'], True)
+        return (seen * open_ * g).sum() + (h[-1] * g_last).sum()
+    wide = {k: v.astype(np.float64) for k, v in arrays.items()}
+    grads = dict(zip(names, P.selective_scan_grad(None, *arrays.values(), g, g_last, has_g=True, has_last=True, **flags)))
+    for name in names:
+        for at in np.ndindex(*wide[name].shape):
+            ends = []
+            for step in (1e-5, -1e-5):
+                moved = dict(wide, **{name: wide[name].copy()})
+                moved[name][at] += step
+                ends.append(loss(moved))
+            assert abs((ends[0] - ends[1]) / 2e-5 - grads[name][at]) < 2e-5 * max(1.0, abs(grads[name][at])), (name, at)
+
+
+def test_selective_scan_goes_on_in_pieces():
+    arrays, _, _ = scan_inputs(2, 9, 3, 4, ('d', 'gate', 'delta_bias'), True)
+    per_step = ('x', 'delta', 'b', 'c', 'gate')
+
+    def whole(arrays):
+        return nn.selective_scan(**arrays, softplus=True)
+
+    def pieces(arrays):
+        state, ys = None, []
+        for lo, hi in ((0, 5), (5, 6), (6, 6), (6, 9)):
+            y, state = nn.selective_scan(**{k: v[:, lo:hi] if k in per_step else v for k, v in arrays.items()}, state=state, softplus=True)
+            ys.append(y)
+        return jnp.concatenate(ys, axis=1), state
+    #(the state is rounded to fp32 between pieces)
+    for a, b in zip(evaluate(whole, arrays), evaluate(pieces, arrays)):
+        assert np.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+BAD_SCANS = [(dict(x=np.ones((2, 12), f32)), TypeError), (dict(x=np.ones((2, 3, 4), np.int32)), TypeError), (dict(delta=np.ones((2, 3, 5), f32)), TypeError),
+             (dict(a=np.ones((5, 6), f32)), TypeError), (dict(a=np.ones((4, 65), f32), b=np.ones((2, 3, 65), f32), c=np.ones((2, 3, 65), f32), state=np.ones((2, 4, 65), f32)), ValueError),
+             (dict(a=np.ones((4, 0), f32)), ValueError), (dict(b=np.ones((2, 3, 5), f32)), TypeError), (dict(c=np.ones((2, 4, 6), f32)), TypeError), (dict(d=np.ones(3, f32)), TypeError),
+             (dict(gate=np.ones((2, 3, 1), f32)), TypeError), (dict(state=np.ones((2, 6, 4), f32)), TypeError), (dict(lengths=np.ones(2, f32)), TypeError),
+             (dict(lengths=np.ones((2, 1), np.int32)), TypeError), (dict(delta_bias=np.ones((1, 4), f32)), TypeError), (dict(delta=np.ones((2, 3, 4), bool)), TypeError)]
+
+
+@pytest.mark.parametrize('change,error', BAD_SCANS)
+def test_selective_scan_refuses(change, error):
+    given = dict(dict(x=np.ones((2, 3, 4), f32), delta=np.ones((2, 3, 4), f32), a=np.ones((4, 6), f32), b=np.ones((2, 3, 6), f32), c=np.ones((2, 3, 6), f32), d=np.ones(4, f32),
+                      gate=np.ones((2, 3, 4), f32), state=np.ones((2, 4, 6), f32), lengths=np.ones(2, np.int32), delta_bias=np.ones(4, f32)), **change)
+    refused(error, lambda *a: nn.selective_scan(*a), *given.values())
+    refused(error, lambda *a: lax.selective_scan_grad(np.ones((1, 2, 6, 4), f32), *a), *given.values())
+
+
+def test_selective_scan_gradient_refuses_what_does_not_belong():
+    x, a, b = np.ones((2, 9, 4), f32), np.ones((4, 6), f32), np.ones((2, 9, 6), f32)
+    kept = np.ones((2, 2, 6, 4), f32)
+    refused(TypeError, lambda *v: lax.selective_scan_grad(*v), kept[:1], x, x, a, b, b)
+    refused(TypeError, lambda *v: lax.selective_scan_grad(*v[:6], g=v[6]), kept, x, x, a, b, b, b)
+    refused(TypeError, lambda *v: lax.selective_scan_grad(*v[:6], g_last=v[6]), kept, x, x, a, b, b, np.ones((2, 6, 4), f32))
+    refused(NotImplementedError, lambda *v: mj.vjp(lambda x: lax.selective_scan(x, *v[1:], with_kept=True)[2], x)[1](kept), x, x, a, b, b)
+
+
+# ------------------------------------------------------------------ planning
+
+@pytest.mark.parametrize('shape', [(0, 5, 4), (3, 0, 4), (3, 5, 0)])
+def test_arrays_without_elements_are_planned(shape):
+    batch, time, channels = shape
+    x, kernel, state, g_last = np.zeros(shape, f32), normal(1, 4, channels), normal(2, batch, 3, channels), normal(3, batch, 3, channels)
+
+    def conv(x, kernel, state, g_last):
+        outs, pullback = mj.vjp(lambda x, k, s: nn.causal_conv(x, k, None, s), x, kernel, state)
+        return tuple(outs) + pullback((x, g_last))
+    y, last, dx, dkernel, dstate = evaluate(conv, x, kernel, state, g_last)
+    assert np.array_equal(last, state) and np.array_equal(dstate, g_last) and y.shape == dx.shape == shape and not dkernel.any()
+    JaxprInterpreter(mj.make_jaxpr(conv)(x, kernel, state, g_last), plan_only=True)
+    arrays, g, g_last = scan_inputs(batch, time, channels, 3, OPTIONAL, True)
+    f = scan_program(list(arrays), None, True)
+    outs = evaluate(f, g, g_last, *arrays.values())
+    assert np.array_equal(outs[1], arrays['state']) and not outs[4].any() and np.array_equal(outs[2 + list(arrays).index('state')], g_last)
+    JaxprInterpreter(mj.make_jaxpr(f)(g, g_last, *arrays.values()), plan_only=True)
+
+
+def test_the_states_that_a_gradient_needs_are_kept_only_then():
+    arrays, g, g_last = scan_inputs(1, 40, 8, 4, (), False)
+    names = list(arrays)
+    kept = lambda program: [e.params['kept'] for e in mj.make_jaxpr(program)(g, g_last, *arrays.values()).jaxpr.eqns if e.primitive.name == 'selective_scan']
+    assert kept(lambda g, last, *v: nn.selective_scan(**dict(zip(names, v)))) == [False]
+    assert kept(scan_program(names, None, False)) == [True]

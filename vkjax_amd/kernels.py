@@ -2570,3 +2570,135 @@ def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Bu
     return [_recurrence_launch('recurrence_grad', x, recurrence_tiling(*shape, RECURRENCE_GRAD_STEPS, 5 + gated), shape, gated, reverse, zeroed,
                                (dfactor, dx, dstate, h, factor, x if gated else None, state, lengths, g, g_last), (0, 1, 2),
                                4 * ((5 + gated) * x.size + 2 * x.shape[0] * x.shape[2]), streamed=(0, 1))]
+
+
+# ---------------------------------------------------------------- short causal convolutions (causal_conv.hip)
+
+CAUSAL_CONV_WIDTHS = range(2, 9)
+CAUSAL_CONV_STEPS  = 8                  #of a thread, where time has more than one
+#blocks that the gradient's tiles of time are shared out to
+CAUSAL_CONV_GRAD_BLOCKS = 1024
+
+
+def _causal_conv_tiling(batch: int, time: int, channels: int):
+    '''(channels per lane, steps per thread, lanes per step, strips of channels, tiles of time)'''
+    vec   = 4 if channels % 4 == 0 else 1
+    steps = 1 if time == 1 else CAUSAL_CONV_STEPS
+    wide  = _pow2_at_least(_cdiv(channels, vec))
+    #lanes along channels, as few groups of steps beside them as time needs; at least a whole line of channels
+    lanes = min(wide, BLOCK // min(_pow2_at_least(_cdiv(time, steps)), BLOCK))
+    lanes = max(lanes, min(wide, 64 // vec))
+    return vec, steps, lanes, _cdiv(channels, lanes * vec), _cdiv(time, steps * (BLOCK // lanes))
+
+
+def _causal_conv_blocks(x: Buffer, blocks: int):
+    if blocks * BLOCK >= 2**32 or max(x.shape[1:]) >= 2**30:
+        raise NotImplementedError(f'a causal convolution over {x.shape}')
+    return (blocks, 1, 1)
+
+
+def causal_conv(y, last, x: Buffer, kernel: Buffer, bias, state, lengths, activation) -> tp.List[Launch]:
+    (b, t, c), k = x.shape, kernel.shape[0]
+    vec, steps, lanes, cstrips, tiles = _causal_conv_tiling(b, t, c)
+    return [Launch(f'causal_conv_k{k}_v{vec}_l{steps}', _causal_conv_blocks(x, b * cstrips * tiles), (BLOCK, 1, 1),
+                   [(v, 0) for v in (y, last, x, kernel, bias, state, lengths)],
+                   _u32(0, t, c, cstrips, tiles, 1, lanes.bit_length() - 1, activation == 'silu'), bytes_moved=8 * x.size, written=(0, 1), streamable=y is not None)]
+
+
+def causal_conv_grad(dx, dkernel, dbias, dstate, x: Buffer, kernel: Buffer, bias, state, lengths, g, g_last, activation, scratch) -> tp.List[Launch]:
+    (b, t, c), k = x.shape, kernel.shape[0]
+    vec, _, lanes, cstrips, tiles = _causal_conv_tiling(b, max(t, 2), c)
+    turns  = max(1, min(tiles, b * cstrips * tiles // CAUSAL_CONV_GRAD_BLOCKS))
+    rows   = b * _cdiv(tiles, turns)
+    sums   = scratch((rows, k + 1, c)) if dkernel is not None or dbias is not None else None
+    launch = Launch(f'causal_conv_grad_k{k}_v{vec}_l{CAUSAL_CONV_STEPS}', _causal_conv_blocks(x, rows * cstrips), (BLOCK, 1, 1),
+                    [(v, 0) for v in (dx, dstate, sums, x, kernel, bias, state, lengths, g, g_last)],
+                    _u32(0, t, c, cstrips, tiles, turns, lanes.bit_length() - 1, activation == 'silu'), lds=4 * BLOCK * vec * (k + 1),
+                    bytes_moved=12 * x.size, written=(0, 1, 2), streamable=dx is not None)
+    if sums is None:
+        return [launch]
+    return [launch, Launch('causal_conv_sums', (_cdiv((k + 1) * c, 64), 1, 1), (1024, 1, 1), [(dkernel, 0), (dbias, 0), (sums, 0)],
+                           _u32(rows, c, k), bytes_moved=4 * sums.size, written=(0, 1))]
+
+
+# ---------------------------------------------------------------- selective scans (selective_scan.hip)
+
+SELECTIVE_SCAN_KEPT       = 8           #steps between two states that a gradient's forward pass keeps
+SELECTIVE_SCAN_MAX_STATES = 64
+#waves that fill the machine; time is cut into chunks where there are fewer, of at least so many steps
+SELECTIVE_SCAN_WAVES, SELECTIVE_SCAN_CHUNK = 2048, 64
+
+
+class ScanTiling(tp.NamedTuple):
+    states: int             #per lane
+    waves:  int             #of a block, one for each so many states
+    strips: int             #of 64 channels
+    chunks: int
+    chunk:  int             #steps of one
+
+
+def selective_scan_tiling(batch: int, time: int, channels: int, n: int) -> ScanTiling:
+    states = 4 if n <= 4 else 8
+    waves  = _pow2_at_least(_cdiv(n, states))
+    strips = _cdiv(channels, 64)
+    chunks = max(1, min(_cdiv(SELECTIVE_SCAN_WAVES, batch * strips * waves), time // SELECTIVE_SCAN_CHUNK))
+    chunk  = _cdiv(_cdiv(time, chunks), SELECTIVE_SCAN_KEPT) * SELECTIVE_SCAN_KEPT
+    tiling = ScanTiling(states, waves, strips, _cdiv(time, chunk), chunk)
+    if batch * strips * tiling.chunks * 64 * waves >= 2**32 or batch * channels * n >= 2**31 or max(time, channels) >= 2**30:
+        raise NotImplementedError(f'a selective scan over {channels} channels of {n} states in {batch} sequences of {time} steps')
+    return tiling
+
+
+def _scan_launch(name: str, x: Buffer, tiling: ScanTiling, n: int, softplus, arrays, written, moved: int, streamed=()) -> Launch:
+    b, t, c = x.shape
+    return Launch(f'{name}_n{tiling.states}_m{tiling.waves}', (b * tiling.strips * tiling.chunks, 1, 1), (64 * tiling.waves, 1, 1), [(v, 0) for v in arrays],
+                  _u32(0, b, t, c, n, tiling.strips, tiling.chunks, tiling.chunk, bool(softplus)), bytes_moved=moved, written=written, streamable=bool(streamed), streamed=streamed or (0,))
+
+
+def _scan_join(states, end, sums, a: Buffer, initial, x: Buffer, tiling: ScanTiling, back: bool) -> Launch:
+    (b, _, c), n = x.shape, a.shape[1]
+    return Launch('selective_scan_join', (_cdiv(b * c * n, 64), 1, 1), (64, 1, 1), [(v, 0) for v in (states, end, sums, a, initial)],
+                  _u32(0, b, c, n, tiling.chunks, back), bytes_moved=8 * b * c * n * tiling.chunks, written=(0, 1))
+
+
+def selective_scan(y, last, kept, x: Buffer, delta: Buffer, a: Buffer, b: Buffer, c: Buffer, d, gate, state, lengths, bias, softplus, scratch) -> tp.List[Launch]:
+    (batch, time, channels), n = x.shape, a.shape[1]
+    if time == 1 and kept is None:
+        lanes = _pow2_at_least(_cdiv(n, 4))
+        if batch * channels * lanes >= 2**32 - BLOCK:
+            raise NotImplementedError(f'a step of a selective scan over {channels} channels of {n} states in {batch} sequences')
+        return [Launch('selective_scan_step', (_cdiv(batch * channels * lanes, BLOCK), 1, 1), (BLOCK, 1, 1),
+                       [(v, 0) for v in (y, last, x, delta, a, b, c, d, gate, state, lengths, bias)],
+                       _u32(0, batch, channels, n, lanes.bit_length() - 1, bool(softplus), 0), bytes_moved=8 * batch * channels * n, written=(0, 1))]
+    tiling = selective_scan_tiling(batch, time, channels, n)
+    moved  = 4 * x.size * (3 + (gate is not None))
+    states, launches = None, []
+    if tiling.chunks > 1:
+        sums, states = scratch((tiling.chunks, batch, channels)), scratch((tiling.chunks, batch, n, channels))
+        launches = [_scan_launch('selective_scan_chunk', x, tiling, n, softplus, (sums, states, x, delta, a, b, bias, lengths), (0, 1), 8 * x.size),
+                    _scan_join(states, None, sums, a, state, x, tiling, False)]
+    return launches + [_scan_launch('selective_scan', x, tiling, n, softplus, (y, last, kept, x, delta, a, b, c, d, gate, state, lengths, bias, states),
+                                    (0, 1, 2), moved, (0,) if y is not None else ())]
+
+
+def selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept: Buffer, x: Buffer, delta: Buffer, a: Buffer, b: Buffer, c: Buffer, d, gate, lengths, bias,
+                        g, g_last, softplus, scratch) -> tp.List[Launch]:
+    (batch, time, channels), n = x.shape, a.shape[1]
+    tiling = selective_scan_tiling(batch, time, channels, n)
+    adjoints, launches = None, []
+    if tiling.chunks > 1 or dstate is not None:
+        sums, adjoints = scratch((tiling.chunks, batch, channels)), scratch((tiling.chunks, batch, n, channels))
+        launches = [_scan_launch('selective_scan_grad_chunk', x, tiling, n, softplus, (sums, adjoints, delta, a, c, gate, bias, lengths, g), (0, 1), 12 * x.size),
+                    _scan_join(adjoints, dstate, sums, a, g_last, x, tiling, True)]
+    maps = scratch((tiling.strips, batch * time, 2, n))
+    rows = scratch((batch * tiling.chunks, n + 2, channels))
+    launches.append(_scan_launch('selective_scan_grad', x, tiling, n, softplus,
+                                 (dx, ddelta, dgate, maps, rows, x, delta, a, b, c, d, gate, lengths, bias, kept, g, g_last, adjoints), (0, 1, 2, 3, 4),
+                                 4 * x.size * (5 + 2 * (gate is not None)), tuple(i for i, v in enumerate((dx, ddelta, dgate)) if v is not None)))
+    map_blocks = _cdiv(batch * time * 2 * n, 1024)
+    blocks     = map_blocks + _cdiv((n + 2) * channels, 64)
+    if blocks * 1024 >= 2**32 or batch * time >= 2**31:
+        raise NotImplementedError(f'the gradient of a selective scan over {channels} channels of {n} states in {batch} sequences of {time} steps')
+    launches.append(Launch('selective_scan_sums', (blocks, 1, 1), (1024, 1, 1), [(v, 0) for v in (da, db, dc, dd, dbias, maps, rows)],
+                           _u32(0, batch * tiling.chunks, channels, n, tiling.strips, batch * time, map_blocks), bytes_moved=4 * (maps.size + rows.size), written=(0, 1, 2, 3, 4)))
+    return launches

@@ -360,6 +360,37 @@ def _linear_recurrence(gs, factor, x, *rest, gated, reverse, has_state, has_leng
     return (dfactor, dx) + ((dstate,) if has_state else ()) + ((None,) if has_lengths else ())
 
 
+@_rule('causal_conv')
+def _causal_conv(gs, x, kernel, *rest, activation, has_bias, has_state, has_lengths):
+    *optional, outs = rest
+    bias    = optional.pop(0) if has_bias else None
+    state   = optional.pop(0) if has_state else None
+    lengths = optional.pop(0) if has_lengths else None
+    grads = lax.causal_conv_grad(x, kernel, bias, state, lengths, _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), activation)
+    return grads + ((None,) if has_lengths else ())
+
+
+def _with_kept_states(eqn):
+    '''The gradient of a selective scan starts from states that the forward pass keeps: the equation with that result too.'''
+    if eqn.params['kept']:
+        return eqn
+    (batch, time, channels), n = eqn.invars[0].aval.shape, eqn.invars[2].aval.shape[1]
+    kept = core.Var(None, '', core.ShapedArray((-(-time // lax.SELECTIVE_SCAN_KEPT), batch, n, channels), _f32))
+    return core.JaxprEqn(eqn.invars, list(eqn.outvars) + [kept], eqn.primitive, dict(eqn.params, kept=True))
+
+
+@_rule('selective_scan')
+def _selective_scan(gs, x, delta, a, b, c, *rest, softplus, kept, has_d, has_gate, has_state, has_lengths, has_bias):
+    *optional, outs = rest
+    if gs[2] is not None:
+        raise NotImplementedError('differentiation through the kept states of selective_scan')
+    d, gate, state, lengths, bias = (optional.pop(0) if has else None for has in (has_d, has_gate, has_state, has_lengths, has_bias))
+    grads = list(lax.selective_scan_grad(outs[2], x, delta, a, b, c, d, gate, state, lengths, bias, _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), softplus))
+    if has_lengths:
+        grads.insert(5 + has_d + has_gate + has_state, None)
+    return tuple(grads)
+
+
 _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', 'iota', 'and', 'or', 'not', 'xor', 'sign', 'floor', 'ceil',
                        'round', 'is_finite', 'shift_left', 'shift_right_logical', 'shift_right_arithmetic', 'threefry2x32',
                        'random_bits', 'random_split', 'random_wrap', 'random_unwrap', 'random_fold_in', 'random_seed'}
@@ -368,7 +399,7 @@ _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', '
 # ---------------------------------------------------------------- driver
 
 #what becomes of equations whose backward pass needs more than their results
-_FOR_GRADIENTS = {'token_log_probs': _with_log_sum_rest}
+_FOR_GRADIENTS = {'token_log_probs': _with_log_sum_rest, 'selective_scan': _with_kept_states}
 
 
 def _replay(jaxpr, consts, inputs, env, order):

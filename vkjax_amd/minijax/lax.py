@@ -673,6 +673,120 @@ def linear_recurrence_grad(h, factor, x, state=None, lengths=None, g=None, g_las
                      has_g=g is not None, has_last=g_last is not None), multiple_results=True))
 
 
+CAUSAL_CONV_ACTIVATIONS = (None, 'silu')
+CAUSAL_CONV_MAX_WIDTH   = 8
+
+
+def _lengths_operand(name, lengths, batch):
+    lengths = lengths if isinstance(lengths, Tracer) else np.asarray(lengths)
+    if dtype_of(lengths)[0] != _i32 or _shape(lengths) != (batch,):
+        raise TypeError(f'{name}: lengths must be int32 [{batch}], got {dtype_of(lengths)[0]} {_shape(lengths)}')
+    return _as_dtype(lengths, _i32)
+
+
+def _shaped_operand(name, what, v, shape):
+    v = _f32_operand(v, name)
+    if _shape(v) != tuple(shape):
+        raise TypeError(f'{name}: {what} must have shape {tuple(shape)}, got {_shape(v)}')
+    return v
+
+
+def _causal_conv_operands(name, x, kernel, bias, state, lengths, activation):
+    x, kernel = _f32_operand(x, name), _f32_operand(kernel, name)
+    xs, ks = _shape(x), _shape(kernel)
+    if len(xs) != 3 or len(ks) != 2 or ks[1] != xs[2]:
+        raise TypeError(f'{name} takes x [batch, time, channels] and a kernel [width, channels], got {xs} and {ks}')
+    if not 2 <= ks[0] <= CAUSAL_CONV_MAX_WIDTH:
+        raise ValueError(f'{name}: a width between 2 and {CAUSAL_CONV_MAX_WIDTH} is needed, got {ks[0]}')
+    if activation not in CAUSAL_CONV_ACTIVATIONS:
+        raise ValueError(f'{name}: activation must be one of {CAUSAL_CONV_ACTIVATIONS}, got {activation!r}')
+    operands = [x, kernel]
+    if bias is not None:
+        operands.append(_shaped_operand(name, 'the bias', bias, (xs[2],)))
+    if state is not None:
+        operands.append(_shaped_operand(name, 'the state', state, (xs[0], ks[0] - 1, xs[2])))
+    if lengths is not None:
+        operands.append(_lengths_operand(name, lengths, xs[0]))
+    return operands, xs, ks, dict(activation=activation, has_bias=bias is not None, has_state=state is not None, has_lengths=lengths is not None)
+
+
+def causal_conv(x, kernel, bias=None, state=None, lengths=None, activation=None):
+    '''activation(bias + sum_k kernel[k] * row[:, t + k]) over [batch, time, channels], channel by channel, where a sequence's rows are
+    `state` [batch, width - 1, channels] (zeros if None) and x behind it. `lengths` (int32 [batch], taken as between 0 and time): from a
+    sequence's length on the result is 0 and x is not looked at. Returns (y, the last width - 1 rows in front of each sequence's end).'''
+    operands, xs, ks, params = _causal_conv_operands('causal_conv', x, kernel, bias, state, lengths, activation)
+    return tuple(emit('causal_conv', operands, [_aval(xs, _f32), _aval((xs[0], ks[0] - 1, xs[2]), _f32)], params, multiple_results=True))
+
+
+def causal_conv_grad(x, kernel, bias=None, state=None, lengths=None, g=None, g_last=None, activation=None):
+    '''(dx, dkernel, and dbias and dstate where there is a bias, a state) for the cotangents g and g_last (None: zeros) of causal_conv's results.'''
+    name = 'causal_conv_grad'
+    operands, xs, ks, params = _causal_conv_operands(name, x, kernel, bias, state, lengths, activation)
+    last = (xs[0], ks[0] - 1, xs[2])
+    if g is not None:
+        operands.append(_shaped_operand(name, 'the cotangent', g, xs))
+    if g_last is not None:
+        operands.append(_shaped_operand(name, "the last rows' cotangent", g_last, last))
+    avals = [_aval(xs, _f32), _aval(ks, _f32)] + ([_aval((xs[2],), _f32)] if bias is not None else []) + ([_aval(last, _f32)] if state is not None else [])
+    return tuple(emit(name, operands, avals, dict(params, has_g=g is not None, has_last=g_last is not None), multiple_results=True))
+
+
+SELECTIVE_SCAN_MAX_STATES = 64
+SELECTIVE_SCAN_KEPT       = 8           #steps between two of the states that a gradient needs
+
+
+def _selective_scan_operands(name, x, delta, a, b, c, d, gate, state, lengths, delta_bias, softplus):
+    x, a = _f32_operand(x, name), _f32_operand(a, name)
+    xs, shape_a = _shape(x), _shape(a)
+    if len(xs) != 3 or len(shape_a) != 2 or shape_a[0] != xs[2]:
+        raise TypeError(f'{name} takes x [batch, time, channels] and a [channels, states], got {xs} and {shape_a}')
+    batch, time, channels, n = *xs, shape_a[1]
+    if not 1 <= n <= SELECTIVE_SCAN_MAX_STATES:
+        raise ValueError(f'{name}: between 1 and {SELECTIVE_SCAN_MAX_STATES} states are supported, got {n}')
+    operands = [x, _shaped_operand(name, 'delta', delta, xs), a, _shaped_operand(name, 'b', b, (batch, time, n)), _shaped_operand(name, 'c', c, (batch, time, n))]
+    for what, v, shape in (('d', d, (channels,)), ('the gate', gate, xs), ('the state', state, (batch, channels, n))):
+        if v is not None:
+            operands.append(_shaped_operand(name, what, v, shape))
+    if lengths is not None:
+        operands.append(_lengths_operand(name, lengths, batch))
+    if delta_bias is not None:
+        operands.append(_shaped_operand(name, 'the bias of delta', delta_bias, (channels,)))
+    return operands, xs, n, dict(softplus=bool(softplus), has_d=d is not None, has_gate=gate is not None, has_state=state is not None,
+                                 has_lengths=lengths is not None, has_bias=delta_bias is not None)
+
+
+def selective_scan(x, delta, a, b, c, d=None, gate=None, state=None, lengths=None, delta_bias=None, softplus: bool = False, with_kept: bool = False):
+    '''The recurrence h[:, t, k, i] = exp(w a[k, i]) h[:, t-1, k, i] + w x[:, t, k] b[:, t, i] over [batch, time, channels] with the states i of
+    every channel k, w = delta[:, t, k] (+ delta_bias[k], and through softplus), and y[:, t, k] = (sum_i c[:, t, i] h[:, t, k, i] + d[k] x[:, t, k])
+    * silu(gate[:, t, k]). `state` [batch, channels, states] is where it starts (zeros if None). `lengths` (int32 [batch], taken as between 0 and
+    time): from a sequence's length on its state stays, y is 0 and the operands are not looked at. Returns (y, the state behind the last step).
+    With `with_kept` also the state in front of every 8th step [ceil(time / 8), batch, states, channels], for selective_scan_grad.
+
+    Parts of a long sequence run side by side, by products of their factors, exp(a sum w): for a w <= 0 (which a model has) h is that of step by step
+    but for rounding. A product of factors that falls below float32's range is 0; where a w > 0 lets one pass it, infinities appear.'''
+    operands, xs, n, params = _selective_scan_operands('selective_scan', x, delta, a, b, c, d, gate, state, lengths, delta_bias, softplus)
+    avals = [_aval(xs, _f32), _aval((xs[0], xs[2], n), _f32)]
+    if with_kept:
+        avals.append(_aval((-(-xs[1] // SELECTIVE_SCAN_KEPT), xs[0], n, xs[2]), _f32))
+    return tuple(emit('selective_scan', operands, avals, dict(params, kept=bool(with_kept)), multiple_results=True))
+
+
+def selective_scan_grad(kept, x, delta, a, b, c, d=None, gate=None, state=None, lengths=None, delta_bias=None, g=None, g_last=None, softplus: bool = False):
+    '''(dx, ddelta, da, db, dc, and those of d, gate, state and delta_bias where there are such) for the cotangents g and g_last (None: zeros) of
+    selective_scan's results; `kept` is what it returned with `with_kept`.'''
+    name = 'selective_scan_grad'
+    operands, xs, n, params = _selective_scan_operands(name, x, delta, a, b, c, d, gate, state, lengths, delta_bias, softplus)
+    kept = _shaped_operand(name, 'the kept states', kept, (-(-xs[1] // SELECTIVE_SCAN_KEPT), xs[0], n, xs[2]))
+    if g is not None:
+        operands.append(_shaped_operand(name, 'the cotangent', g, xs))
+    if g_last is not None:
+        operands.append(_shaped_operand(name, "the last state's cotangent", g_last, (xs[0], xs[2], n)))
+    maps  = _aval((xs[0], xs[1], n), _f32)
+    avals = [_aval(xs, _f32), _aval(xs, _f32), _aval((xs[2], n), _f32), maps, maps]
+    avals += [_aval(shape, _f32) for v, shape in ((d, (xs[2],)), (gate, xs), (state, (xs[0], xs[2], n)), (delta_bias, (xs[2],))) if v is not None]
+    return tuple(emit(name, [kept] + operands, avals, dict(params, has_g=g is not None, has_last=g_last is not None), multiple_results=True))
+
+
 # ---------------------------------------------------------------- rng
 
 def threefry2x32(key0, key1, x0, x1):

@@ -71,3 +71,23 @@ def gated_recurrence(gate, x, state=None, lengths=None, reverse=False):
     time to the first. Differentiable with respect to gate, x and state. `lax.linear_recurrence` takes factors and addends, and says
     what becomes of values that many small factors leave next to nothing of, and of infinite ones.'''
     return lax.linear_recurrence(gate, x, state, lengths, reverse, gated=True)
+
+
+def causal_conv(x, kernel, bias=None, state=None, lengths=None, activation=None):
+    '''A short causal convolution along time over x [batch, time, channels], channel by channel, with the activation behind it (None or 'silu'):
+    y[:, t] = activation(bias + sum_k kernel[k] * x[:, t - width + 1 + k]) for a kernel [width, channels], width 2 to 8. Returns (y, the last
+    width - 1 inputs [batch, width - 1, channels]), so that a sequence can go on later, token by token: `state` is what stands in front of it
+    (zeros if None). `lengths` int32 [batch]: a padded batch, in which y is 0 from a sequence's length on, x is not looked at there, and the last
+    inputs are those in front of the length. Differentiable with respect to x, kernel, bias and state.'''
+    return lax.causal_conv(x, kernel, bias, state, lengths, activation)
+
+
+def selective_scan(x, delta, a, b, c, d=None, gate=None, state=None, lengths=None, delta_bias=None, softplus=False):
+    '''A selective state space over x [batch, time, channels], with `states` (1 to 64) states h per channel:
+    h[t] = exp(w a) h[t-1] + w x[t] b[t], y[t] = (sum over the states of c[t] h[t] + d x[t]) * silu(gate[t]), where w = delta[t], or
+    softplus(delta[t] + delta_bias) (`softplus`); delta and gate are [batch, time, channels], a [channels, states], b and c [batch, time, states],
+    d and delta_bias [channels]; d, gate and delta_bias may be None. Returns (y, the state [batch, channels, states] behind the last step), so that a
+    sequence can go on later, token by token: `state` is where it starts (zeros if None), and time may be 1, or 0. `lengths` int32 [batch]: a
+    padded batch, in which a sequence's state stays and y is 0 from its length on, and nothing else is looked at there. Differentiable with respect to
+    every float32 operand. `lax.selective_scan` says what long products of factors come to.'''
+    return lax.selective_scan(x, delta, a, b, c, d, gate, state, lengths, delta_bias, softplus)

@@ -1169,6 +1169,67 @@ def _held_state(equation, out, source):
     return [_copy_op(equation, out, EwOperand(source, 0, K.row_major_strides(out.shape)))]
 
 
+def _float_operands(equation, *buffers):
+    if any(b is not None and _kind(b.dtype) != _F for b in buffers):
+        raise NotImplementedError(equation)
+
+
+def _causal_conv_buffers(equation, ins):
+    p = equation.params
+    x, kernel, *rest = ins
+    bias, state, lengths, g, g_last = (rest.pop(0) if p.get(name) else None for name in ('has_bias', 'has_state', 'has_lengths', 'has_g', 'has_last'))
+    _float_operands(equation, x, kernel, bias, state, g, g_last)
+    return x, kernel, bias, state, lengths, g, g_last
+
+
+def causal_conv(bufferpool, equation):
+    ins, (y, last), _ = _operator_buffers(bufferpool, equation)
+    x, kernel, bias, state, lengths, _, _ = _causal_conv_buffers(equation, ins)
+    if x.size == 0:
+        return _held_state(equation, last, state)
+    return _operator_ops(equation, K.causal_conv(_with_elements(y), _with_elements(last), x, kernel, bias, state, lengths, equation.params['activation']))
+
+
+def causal_conv_grad(bufferpool, equation):
+    p = equation.params
+    ins, (dx, dkernel, *outs), scratch = _operator_buffers(bufferpool, equation)
+    x, kernel, bias, state, lengths, g, g_last = _causal_conv_buffers(equation, ins)
+    dbias  = outs.pop(0) if p['has_bias'] else None
+    dstate = outs.pop(0) if p['has_state'] else None
+    if x.size == 0:
+        return [Op(equation, launch=K.fill(v, 0)) for v in (dkernel, dbias) if _with_elements(v) is not None] + _held_state(equation, dstate, g_last)
+    return _operator_ops(equation, K.causal_conv_grad(dx, dkernel, dbias, dstate, x, kernel, bias, state, lengths, g, g_last, p['activation'], scratch))
+
+
+def _selective_scan_buffers(equation, ins):
+    p = equation.params
+    x, delta, a, b, c, *rest = ins
+    d, gate, state, lengths, bias, g, g_last = (rest.pop(0) if p.get(name) else None
+                                                for name in ('has_d', 'has_gate', 'has_state', 'has_lengths', 'has_bias', 'has_g', 'has_last'))
+    _float_operands(equation, x, delta, a, b, c, d, gate, state, bias, g, g_last)
+    return x, delta, a, b, c, d, gate, state, lengths, bias, g, g_last
+
+
+def selective_scan(bufferpool, equation):
+    p = equation.params
+    ins, (y, last, *kept), scratch = _operator_buffers(bufferpool, equation)
+    x, delta, a, b, c, d, gate, state, lengths, bias, _, _ = _selective_scan_buffers(equation, ins)
+    if x.size == 0:
+        return _held_state(equation, last, state)
+    return _operator_ops(equation, K.selective_scan(y, last, kept[0] if kept else None, x, delta, a, b, c, d, gate, state, lengths, bias, p['softplus'], scratch))
+
+
+def selective_scan_grad(bufferpool, equation):
+    p = equation.params
+    (kept, *ins), (dx, ddelta, da, db, dc, *outs), scratch = _operator_buffers(bufferpool, equation)
+    x, delta, a, b, c, d, gate, state, lengths, bias, g, g_last = _selective_scan_buffers(equation, ins)
+    dd, dgate, dstate, dbias = (outs.pop(0) if p[name] else None for name in ('has_d', 'has_gate', 'has_state', 'has_bias'))
+    if x.size == 0:
+        return ([Op(equation, launch=K.fill(v, 0)) for v in (da, db, dc, dd, dbias) if _with_elements(v) is not None] + _held_state(equation, dstate, g_last))
+    return _operator_ops(equation, K.selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept, x, delta, a, b, c, d, gate, lengths, bias,
+                                                         g, g_last, p['softplus'], scratch))
+
+
 # ------------------------------------------------------------------ rng
 
 def threefry2x32(bufferpool, equation):
