@@ -7,8 +7,8 @@
 //   dA = sum e dt;  dD = sum gy x;  ddelta = ddt sigmoid(delta + bias);  dbias = sum ddelta;  dgate = g seen silu'(gate);  dstate = f l at the first step
 // From a sequence's length on the state stays (dt = 0) and y is 0; nothing is looked at there and nothing comes back.
 //
-// A block has 64 channels, a lane of each of its M waves one of them and NS of its states in registers, so b and c, which all channels of a sequence share, are scalars of the
-// wave. What a step needs once per channel (dt, the gates, loads and stores) is shared out: of every 8 steps a wave prepares 8 / M and puts them into shared memory, all waves go
+// A block has 64 channels, a lane of each of its M waves one of them and NS of its states in registers, so b and c, which all channels of a sequence share, come
+// from shared memory, a vector for all lanes. What a step needs once per channel (dt, the gates, loads and stores) is shared out: of every 8 steps a wave prepares 8 / M and puts them into shared memory, all waves go
 // through the 8 steps with their states and leave their parts of the sums over n there, and the wave that has prepared a step adds those up and stores its results. Bound by the
 // vector instructions: an exponential is four of them, a state and step eight, in the gradient 21.
 // A block goes through its steps one after the other; where batch and channels are too few to fill the machine, time is cut into chunks: a first launch leaves each chunk's
@@ -67,15 +67,18 @@ struct Place {
     __device__ int64_t state(const ScanParams& P, int i) const { return ((int64_t)b * P.C + c) * P.N + n0 + i; }
     __device__ bool has(const ScanParams& P, int i) const { return n0 + i < P.N; }
     __device__ int own(int q) const { return (int)wave * OWN + q; }
-    // the states' values of a step from [B, T, N]
-    __device__ void maps(float (&v)[NS], const float* __restrict__ p, const ScanParams& P, int t) const {
-        const float* const row = p + ((int64_t)b * P.T + t) * P.N;
-        if (P.N == NS * M) {
+    // This thread's element of the eight steps' values from [B, T, N], as they lie in shared memory, [step][NS * M]: zeros for states that there are not
+    static constexpr int STAGED = KEPT * NS * M;
+    __device__ float staged(const float* __restrict__ p, const ScanParams& P, int t0) const {
+        const uint32_t s = threadIdx.x / (uint32_t)(NS * M), n = threadIdx.x % (uint32_t)(NS * M);
+        return threadIdx.x < (uint32_t)STAGED && n < P.N ? p[((int64_t)b * P.T + min(t0 + (int)s, stop - 1)) * P.N + n] : 0.f;
+    }
+    // ... and from there to the registers of the wave that has these states
+    __device__ void maps(float (&v)[NS], const float (&rows)[KEPT][NS * M], int s) const {
 #pragma unroll
-            for (int i = 0; i < NS; ++i) v[i] = row[n0 + i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < NS; ++i) { const float w = row[min(n0 + i, P.N - 1u)]; v[i] = has(P, i) ? w : 0.f; }
+        for (int i = 0; i < NS; i += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4*>(&rows[s][n0 + i]);
+            v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
         }
     }
     __device__ void factors(float (&a2)[NS], const float* __restrict__ a, const ScanParams& P) const {
@@ -91,8 +94,9 @@ template <int NS, int M>
 __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float* __restrict__ states, const float* __restrict__ x, const float* __restrict__ delta, const float* __restrict__ a,
                                                 const float* __restrict__ bmap, const float* __restrict__ bias, const int32_t* __restrict__ lengths, const ScanParams& P) {
     __shared__ float prepared[2][2][KEPT][64];                       // [turn's parity][dt, dt x][step][lane]
+    __shared__ __attribute__((aligned(16))) float map[2][KEPT][NS * M];
     const Place<NS, M> at(P, lengths);
-    float a2[NS], h[NS] = {}, sum = 0.f;
+    float a2[NS], h[NS] = {}, sum = 0.f, mapped;
     at.factors(a2, a, P);
     const float add = bias ? bias[at.c] : 0.f;
     float xs[at.OWN], ds[at.OWN];
@@ -102,6 +106,7 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
             const int64_t row = at.row(P, min(t0 + at.own(q), at.stop - 1));
             xs[q] = x[row]; ds[q] = delta[row];
         }
+        mapped = at.staged(bmap, P, t0);
     };
     if (at.begin < at.stop) request(at.begin);
     int parity = 0;
@@ -113,17 +118,18 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
             prepared[parity][0][at.own(q)][at.lane] = taken ? w : 0.f;
             prepared[parity][1][at.own(q)][at.lane] = taken ? w * xs[q] : 0.f;
         }
+        if (threadIdx.x < (uint32_t)at.STAGED) (&map[parity][0][0])[threadIdx.x] = mapped;
         if (t0 + KEPT < at.stop) request(t0 + KEPT);
         at.meet();
         float dt[KEPT], u[KEPT], bs[NS], next[NS];
 #pragma unroll
         for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[parity][0][s][at.lane]; u[s] = prepared[parity][1][s][at.lane]; }
-        at.maps(next, bmap, P, t0);
+        at.maps(next, map[parity], 0);
 #pragma unroll
         for (int s = 0; s < KEPT; ++s) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) bs[i] = next[i];
-            if (s + 1 < KEPT) at.maps(next, bmap, P, min(t0 + s + 1, at.stop - 1));
+            if (s + 1 < KEPT) at.maps(next, map[parity], s + 1);
             sum += dt[s];
 #pragma unroll
             for (int i = 0; i < NS; ++i) h[i] = __builtin_fmaf(exp2_of(a2[i] * dt[s]), h[i], u[s] * bs[i]);
@@ -172,8 +178,9 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
                                           const float* __restrict__ gate, const float* __restrict__ state, const int32_t* __restrict__ lengths, const float* __restrict__ bias,
                                           const float* __restrict__ states, const ScanParams& P) {
     __shared__ float prepared[2][KEPT][64], parts[M][KEPT][64];      // [dt, dt x][step][lane], sums over a wave's states
+    __shared__ __attribute__((aligned(16))) float map[2][KEPT][NS * M];
     const Place<NS, M> at(P, lengths);
-    float a2[NS], h[NS];
+    float a2[NS], h[NS], mapped[2];
     at.factors(a2, a, P);
 #pragma unroll
     for (int i = 0; i < NS; ++i) h[i] = !at.has(P, i) ? 0.f : states ? states[at.held(P, at.chunk, i)] : state ? state[at.state(P, i)] : 0.f;
@@ -187,6 +194,7 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
             xs[q] = x[row]; ds[q] = delta[row];
             if (gate) gs[q] = gate[row];
         }
+        mapped[0] = at.staged(bmap, P, t0); mapped[1] = at.staged(cmap, P, t0);
     };
     if (at.begin < at.stop) request(at.begin);
     for (int t0 = at.begin; t0 < at.end; t0 += KEPT) {
@@ -205,21 +213,19 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
                 ys[q] = D * xs[q];
                 open[q] = gate ? gs[q] * sigmoid(gs[q]) : 1.f;
             }
+            if (threadIdx.x < (uint32_t)at.STAGED) { (&map[0][0][0])[threadIdx.x] = mapped[0]; (&map[1][0][0])[threadIdx.x] = mapped[1]; }
             if (t0 + KEPT < at.stop) request(t0 + KEPT);
             at.meet();
             float dt[KEPT], u[KEPT], bs[NS], cs[NS], next_b[NS], next_c[NS];
 #pragma unroll
             for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[0][s][at.lane]; u[s] = prepared[1][s][at.lane]; }
-            at.maps(next_b, bmap, P, t0);
-            at.maps(next_c, cmap, P, t0);
+            at.maps(next_b, map[0], 0);
+            at.maps(next_c, map[1], 0);
 #pragma unroll
             for (int s = 0; s < KEPT; ++s) {
 #pragma unroll
                 for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                if (s + 1 < KEPT) {
-                    at.maps(next_b, bmap, P, min(t0 + s + 1, at.stop - 1));
-                    at.maps(next_c, cmap, P, min(t0 + s + 1, at.stop - 1));
-                }
+                if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) {
@@ -309,8 +315,9 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
                                                      const float* __restrict__ gate, const float* __restrict__ bias, const int32_t* __restrict__ lengths, const float* __restrict__ g,
                                                      const ScanParams& P) {
     __shared__ float prepared[2][2][KEPT][64];                       // [turn's parity][dt, gy][step][lane]
+    __shared__ __attribute__((aligned(16))) float map[2][KEPT][NS * M];
     const Place<NS, M> at(P, lengths);
-    float a2[NS], l[NS] = {}, sum = 0.f;
+    float a2[NS], l[NS] = {}, sum = 0.f, mapped;
     at.factors(a2, a, P);
     const float add = bias ? bias[at.c] : 0.f;
     const int turns = at.begin < at.stop ? (at.stop - at.begin + KEPT - 1) / KEPT : 0;
@@ -322,6 +329,7 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
             ds[q] = delta[row]; gs[q] = g ? g[row] : 0.f;
             if (gate) gates[q] = gate[row];
         }
+        mapped = at.staged(cmap, P, t0);
     };
     if (turns) request(at.begin + (turns - 1) * KEPT);
     for (int turn = turns - 1; turn >= 0; --turn) {
@@ -332,17 +340,18 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
             prepared[parity][0][at.own(q)][at.lane] = taken ? width_of(ds[q], add, P.softplus) : 0.f;
             prepared[parity][1][at.own(q)][at.lane] = taken ? (gate ? gs[q] * (gates[q] * sigmoid(gates[q])) : gs[q]) : 0.f;
         }
+        if (threadIdx.x < (uint32_t)at.STAGED) (&map[parity][0][0])[threadIdx.x] = mapped;
         if (turn > 0) request(t0 - KEPT);
         at.meet();
         float dt[KEPT], gy[KEPT], cs[NS], next[NS];
 #pragma unroll
         for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[parity][0][s][at.lane]; gy[s] = prepared[parity][1][s][at.lane]; }
-        at.maps(next, cmap, P, min(t0 + KEPT - 1, at.stop - 1));
+        at.maps(next, map[parity], KEPT - 1);
 #pragma unroll
         for (int s = KEPT - 1; s >= 0; --s) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) cs[i] = next[i];
-            if (s > 0) at.maps(next, cmap, P, min(t0 + s - 1, at.stop - 1));
+            if (s > 0) at.maps(next, map[parity], s - 1);
             sum += dt[s];
 #pragma unroll
             for (int i = 0; i < NS; ++i) l[i] = exp2_of(a2[i] * dt[s]) * __builtin_fmaf(gy[s], cs[i], l[i]);
@@ -395,6 +404,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                                                const float* __restrict__ adjoints, const ScanParams& P) {
     // [dt, x, gy][step][lane]; a wave's sums over its states [seen, l b, e A][step][lane]; its sums over channels [db, dc][step][state]
     __shared__ float prepared[3][KEPT][64], parts[M][3][KEPT][64], mapped[2][KEPT][NS * M];
+    __shared__ __attribute__((aligned(16))) float map[2][KEPT][NS * M];
     const Place<NS, M> at(P, lengths);
     const OverChannels<NS> over;
     float a2[NS], l[NS], da[NS] = {}, dD = 0.f, dbias = 0.f;
@@ -404,7 +414,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
     const float add = bias ? bias[at.c] : 0.f, D = through ? through[at.c] : 0.f;
     const int turns = (at.end - at.begin + KEPT - 1) / KEPT;
     const bool stream = streams_result(P.first);
-    float rx[at.OWN], rd[at.OWN], rg[at.OWN], rz[at.OWN], rh[NS];
+    float rx[at.OWN], rd[at.OWN], rg[at.OWN], rz[at.OWN], rh[NS], rmap[2];
     auto request = [&](int t0) {
 #pragma unroll
         for (int q = 0; q < at.OWN; ++q) {
@@ -414,6 +424,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) rh[i] = at.has(P, i) ? kept[at.held(P, (uint32_t)t0 / KEPT, i)] : 0.f;
+        rmap[0] = at.staged(bmap, P, t0); rmap[1] = at.staged(cmap, P, t0);
     };
     bool requested = false;
     for (int turn = turns - 1; turn >= 0; --turn) {
@@ -438,19 +449,19 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             float h[NS], before[KEPT][NS];
 #pragma unroll
             for (int i = 0; i < NS; ++i) h[i] = rh[i];
+            if (threadIdx.x < (uint32_t)at.STAGED) { (&map[0][0][0])[threadIdx.x] = rmap[0]; (&map[1][0][0])[threadIdx.x] = rmap[1]; }
             if (turn > 0) request(t0 - KEPT);
             at.meet();
             float dt[KEPT], xs[KEPT], gy[KEPT], bs[NS], cs[NS], next_b[NS], next_c[NS];
 #pragma unroll
             for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[0][s][at.lane]; xs[s] = prepared[1][s][at.lane]; gy[s] = prepared[2][s][at.lane]; }
-            at.maps(next_b, bmap, P, t0);
-            at.maps(next_c, cmap, P, t0);
+            at.maps(next_b, map[0], 0);
+            at.maps(next_c, map[1], 0);
 #pragma unroll
             for (int s = 0; s < KEPT; ++s) {
-                const int t = min(t0 + s, at.stop - 1), follow = min(t0 + s + 1, at.stop - 1);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                if (s + 1 < KEPT) { at.maps(next_b, bmap, P, follow); at.maps(next_c, cmap, P, follow); }
+                if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
                 float part[NS], seen = 0.f;
                 const float u = dt[s] * xs[s];
 #pragma unroll
@@ -465,14 +476,13 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 if (over.stores) mapped[1][s][at.n0 + over.index] = sum;
                 STEP_FENCE();
             }
-            at.maps(next_b, bmap, P, min(t0 + KEPT - 1, at.stop - 1));
-            at.maps(next_c, cmap, P, min(t0 + KEPT - 1, at.stop - 1));
+            at.maps(next_b, map[0], KEPT - 1);
+            at.maps(next_c, map[1], KEPT - 1);
 #pragma unroll
             for (int s = KEPT - 1; s >= 0; --s) {
-                const int follow = min(t0 + s - 1, at.stop - 1);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                if (s > 0) { at.maps(next_b, bmap, P, follow); at.maps(next_c, cmap, P, follow); }
+                if (s > 0) { at.maps(next_b, map[0], s - 1); at.maps(next_c, map[1], s - 1); }
                 float part[NS], lb = 0.f, ea = 0.f;
                 const float u = dt[s] * xs[s];
 #pragma unroll
@@ -557,7 +567,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                                                                                                 ScanParams P) {                                                                    \
         scan_grad_chunk_body<NS, M>(sums, states, delta, a, cmap, gate, bias, lengths, g, P);                                                                                      \
     }                                                                                                                                                                              \
-    extern "C" __global__ __launch_bounds__(64 * M) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* maps, float* channel_sums, const float* x, \
+    extern "C" __global__ __launch_bounds__(64 * M, 2) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* maps, float* channel_sums, const float* x, \
                                                                                           const float* delta, const float* a, const float* bmap, const float* cmap,                \
                                                                                           const float* through, const float* gate, const int32_t* lengths, const float* bias,      \
                                                                                           const float* kept, const float* g, const float* g_last, const float* adjoints,           \
