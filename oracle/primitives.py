@@ -1047,3 +1047,39 @@ def selective_scan_grad(kept, x, delta, a, b, c, *rest, softplus, has_d, has_gat
         outs += [l] if has_state else []
         outs += [ddelta.sum(axis=(0, 1))] if has_bias else []
         return tuple(v.astype(f32) for v in outs)
+
+
+def _linear_scores64(x, weights, tokens, transposed):
+    w = np.asarray(weights, np.float64)
+    w = w.T if transposed else w
+    token = np.asarray(tokens, np.int64).reshape(-1)
+    given = (token >= 0) & (token < w.shape[1])
+    rows  = np.where(given[:, None], np.asarray(x, np.float64).reshape(-1, w.shape[0]), 0.0)
+    s = rows @ w
+    peak = s.max(axis=1)
+    return w, rows, s, np.where(given, token, 0), given, peak, np.exp(s - peak[:, None]).sum(axis=1)
+
+
+def linear_log_probs(x, weights, tokens, transposed):
+    with np.errstate(**_EW_ERR):
+        if np.size(tokens) == 0:
+            return (np.zeros(np.shape(tokens), f32),) * 4
+        _, _, s, token, given, peak, total = _linear_scores64(x, weights, tokens, transposed)
+        rows = lambda v, empty: np.where(given, v, empty).reshape(np.shape(tokens)).astype(f32)
+        log_sum = peak + np.log(total)
+        return rows(s[np.arange(len(s)), token] - log_sum, 0.0), rows(log_sum, 0.0), rows(peak, 0.0), rows(total, 1.0)
+
+
+def linear_log_probs_grad(x, weights, tokens, peaks, totals, *cotangents, transposed, has_log_probs, has_log_sums):
+    cotangents = [np.asarray(c, np.float64).reshape(-1) for c in cotangents]
+    with np.errstate(**_EW_ERR):
+        if np.size(tokens) == 0:
+            return np.zeros(x.shape, f32), np.zeros(weights.shape, f32)
+        w, rows, s, token, given, peak, total = _linear_scores64(x, weights, tokens, transposed)
+        of_token = np.where(given, cotangents.pop(0) if has_log_probs else 0.0, 0.0)
+        of_sum   = np.where(given, cotangents.pop(0) if has_log_sums else 0.0, 0.0) - of_token
+        d = np.exp(s - peak[:, None]) / total[:, None] * of_sum[:, None]
+        d[np.arange(len(s)), token] += of_token
+        d[~given] = 0.0
+        dw = rows.T @ d
+        return (d @ w.T).reshape(x.shape).astype(f32), (dw.T if transposed else dw).astype(f32)

@@ -1,4 +1,4 @@
-'''Short causal convolutions and selective scans on the GPU against their definitions in 64 bits (the oracle), at the sizes, lengths and
+'''Short causal convolutions, selective scans and log probabilities from weights on the GPU against their definitions in 64 bits (the oracle), at the sizes, lengths and
 options where they can go wrong.
 
 Tolerances. u = 2^-24 is half a step of fp32. Every multiply-add, product and sum is off by u of its result; a sum of n terms one after the other by at most n u
@@ -9,8 +9,8 @@ import pytest
 
 from tests.test_gpu_operators import U, both, close
 from tests.test_operators import normal
-from tests.test_token_model_operators import OPTIONAL, scan_inputs, scan_program
-from vkjax_amd import minijax as mj
+from tests.test_token_model_operators import OPTIONAL, loss_program, scan_inputs, scan_program
+from vkjax_amd import kernels as K, minijax as mj
 
 pytestmark = pytest.mark.gpu
 jnp, lax, nn = mj.numpy, mj.lax, mj.nn
@@ -214,3 +214,117 @@ def test_selective_scan_keeps_what_is_not_finite_to_its_channel():
     broken = np.zeros(y.shape, bool)
     broken[0, 100:, 66] = True
     assert np.array_equal(np.isnan(y), broken) and np.isnan(last[0, 66]).all() and np.isfinite(last).sum() == last.size - 16
+
+
+# ------------------------------------------------------------------ log probabilities from weights
+
+def product_error(a, b, terms):
+    '''How far a @ b may be off, for magnitudes a and b: operands and products by 12 u of each product (numbers to 2^-22 twice, and what is left out), and by 2^-49 of the operands' largest
+    ones; a sum that is rounded twice per 16 terms, and three times where it is put together. (fp32 products are below that.)'''
+    return (terms / 8 + 24) * U * (a @ b) + 2.0 ** -49 * terms * a.max(initial=0) * b.max(initial=0)
+
+
+def loss_bounds(x, w, tokens, g, gs, transposed):
+    v64 = w.astype(np.float64).T if transposed else w.astype(np.float64)
+    hidden, vocabulary = v64.shape
+    given = (tokens >= 0) & (tokens < vocabulary)
+    rows = np.where(given[:, None], x.astype(np.float64), 0.0)
+    s, e_s = rows @ v64, product_error(np.abs(rows), np.abs(v64), hidden)
+    peak = s.max(axis=1, keepdims=True)
+    p = np.exp(s - peak)
+    p /= p.sum(axis=1, keepdims=True)
+    token, at = np.where(given, tokens, 0), np.arange(len(s))
+    log_sum = s[at, token] - np.log(p[at, token])
+    #exponentials are off by (2 |their argument| + 4) u; the sum of a row's is rounded in a lane (64 times), between lanes and tiles (64 times)
+    e_sum = (p * (e_s + (2 * np.abs(s - peak) + 4) * U)).sum(axis=1) + 130 * U
+    e_log_sum = e_sum + 4 * U * (np.abs(log_sum) + np.abs(peak[:, 0]))
+    e_log_prob = e_log_sum + e_s[at, token] + 4 * U * np.abs(s[at, token])
+    of_token, of_sum = np.where(given, g, 0.0).astype(np.float64), np.where(given, gs.astype(np.float64) - g, 0.0)
+    #(the largest score and the sum are those of the forward pass: as far off again; q is held to 2^-22 of itself and 2^-49 of its row's larger cotangent)
+    relative = e_s + e_s.max(axis=1, keepdims=True) + e_sum[:, None] + (2 * np.abs(s - peak) + 12) * U
+    d, e_d = p * np.abs(of_sum)[:, None], p * np.abs(of_sum)[:, None] * relative
+    d[at, token] += np.abs(of_token)
+    most = np.maximum(np.abs(of_token), np.abs(of_sum))
+    e_d += 6 * U * d + 2.0 ** -49 * most[:, None]
+    w_abs = np.abs(v64).T
+    e_dx = e_d @ w_abs + product_error(d, w_abs, vocabulary)
+    e_dw = np.abs(rows).T @ e_d + product_error((np.abs(rows) * most[:, None]).T, d / np.maximum(most, 1e-300)[:, None], len(s))
+    tiny = 1e-36
+    return [e_log_prob * given + tiny, e_log_sum * given + tiny, e_dx * given[:, None] + tiny, (e_dw.T if transposed else e_dw) + tiny]
+
+
+def check_loss(x, w, tokens, g, gs, transposed, dirty=None):
+    got, expected, _ = both(loss_program(transposed), x if dirty is None else dirty, w, tokens, g, gs)
+    for name, a, b, bound in zip(('log_probs', 'log_sums', 'dx', 'dweights'), got, expected, loss_bounds(x, w, tokens, g, gs, transposed)):
+        close(a, b, bound, name)
+
+
+def loss_inputs(rows, hidden, vocabulary, transposed, seed=0):
+    rng = np.random.default_rng(seed + rows + 3 * hidden + 7 * vocabulary)
+    x, w = rng.standard_normal((rows, hidden)).astype(f32), (rng.standard_normal((hidden, vocabulary)) * 2 / np.sqrt(hidden)).astype(f32)
+    tokens = rng.integers(0, vocabulary, rows).astype(np.int32)
+    tokens[rng.random(rows) < 0.2] = -1
+    tokens[rng.random(rows) < 0.1] = vocabulary
+    return x, np.ascontiguousarray(w.T) if transposed else w, tokens, (rng.standard_normal(rows) / rows).astype(f32), (0.1 * rng.standard_normal(rows) / rows).astype(f32)
+
+
+#(rows, hidden, vocabulary): one of everything; rows that the fp32 instructions take, in one block of 32 and in two, at the border and behind it; contractions of no whole pair of steps; vocabularies that are
+#smaller than a vector, end inside a vector, a tile, a block of 32; several tiles each way
+LOSSES = [(1, 1, 1), (1, 8, 4), (3, 5, 7), (2, 64, 3), (64, 32, 128), (65, 33, 129), (8, 64, 300), (33, 100, 1001), (130, 70, 515), (257, 128, 4099), (100, 300, 3), (66, 17, 2), (20, 515, 2050),
+          (300, 40, 640), (5, 1030, 131), (128, 128, 128), (1100, 9, 1300), (64, 7, 2049)]
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('rows,hidden,vocabulary', LOSSES, ids=str)
+def test_linear_log_probs_and_gradient(rows, hidden, vocabulary, transposed):
+    print(f'linear log probs {rows} x {hidden} x {vocabulary}, transposed {transposed}', flush=True)
+    x, w, tokens, g, gs = loss_inputs(rows, hidden, vocabulary, transposed)
+    given = (tokens >= 0) & (tokens < vocabulary)
+    check_loss(x, w, tokens, g, gs, transposed, np.where(given[:, None], x, np.nan).astype(f32))
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+def test_linear_log_probs_gradient_in_pieces_of_the_vocabulary(transposed, monkeypatch):
+    monkeypatch.setattr(K, 'LINEAR_PIECE', 1)
+    for rows, hidden, vocabulary in ((140, 70, 600), (40, 130, 513), (520, 33, 300)):
+        print(f'in pieces: {rows} x {hidden} x {vocabulary}', flush=True)
+        check_loss(*loss_inputs(rows, hidden, vocabulary, transposed), transposed)
+
+
+def test_linear_log_probs_of_numbers_far_apart():
+    '''Rows and columns a thousand times as large as others, and tokens with next to no probability in every row.'''
+    x, w, tokens, g, gs = loss_inputs(150, 60, 700, False)
+    x *= (10.0 ** np.linspace(-3, 3, 150))[:, None].astype(f32) / 100
+    w *= (10.0 ** np.linspace(-4, 0, 700))[None].astype(f32)
+    check_loss(x.astype(f32), w.astype(f32), tokens, (g * 1e-6).astype(f32), gs, False)
+    x, w, tokens, g, gs = loss_inputs(150, 60, 700, False)
+    x[:, 0], w[0] = 1.0, np.linspace(-40, 0, 700)
+    check_loss(x, w, tokens, g, gs, False)
+
+
+def test_linear_log_probs_of_one_result_only():
+    x, w, tokens, g, _ = loss_inputs(90, 40, 200, False)
+    zero = np.zeros_like(g)
+    for which in (0, 1):
+        f = lambda x, w, tokens, g: mj.vjp(lambda x, w: nn.linear_log_probs(x, w, tokens)[which], x, w)[1](g)
+        got, expected, _ = both(f, x, w, tokens, g)
+        bounds = loss_bounds(x, w, tokens, *((g, zero) if which == 0 else (zero, g)), False)[2:]
+        for name, a, b, bound in zip(('dx', 'dweights'), got, expected, bounds):
+            close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('rows', [9, 200])
+def test_linear_log_probs_keep_what_is_not_finite_to_its_row(rows):
+    x, w, tokens, g, gs = loss_inputs(rows, 40, 300, False)
+    tokens[:] = np.arange(rows) % 300
+    x[3, 5], x[6, 0] = np.nan, np.inf
+    got = mj.tree_leaves(both(loss_program(False), x, w, tokens, g, gs)[0])
+    bad = np.isin(np.arange(rows), (3, 6))
+    assert np.array_equal(np.isnan(got[0]), bad) and np.array_equal(np.isnan(got[1]), bad) and np.array_equal(np.isnan(got[2]).all(axis=1), bad) and np.isfinite(got[2][~bad]).all()
+
+
+def test_linear_log_probs_of_nothing_but_padding():
+    for rows in (7, 100):
+        x, w, tokens, g, gs = loss_inputs(rows, 40, 300, False)
+        got = mj.tree_leaves(both(loss_program(False), np.full_like(x, np.nan), w, np.full_like(tokens, -1), g, gs)[0])
+        assert not any(v.any() for v in got)

@@ -239,3 +239,69 @@ def test_the_states_that_a_gradient_needs_are_kept_only_then():
     kept = lambda program: [e.params['kept'] for e in mj.make_jaxpr(program)(g, g_last, *arrays.values()).jaxpr.eqns if e.primitive.name == 'selective_scan']
     assert kept(lambda g, last, *v: nn.selective_scan(**dict(zip(names, v)))) == [False]
     assert kept(scan_program(names, None, False)) == [True]
+
+
+# ------------------------------------------------------------------ log probabilities from weights
+
+def loss_program(transposed):
+    def f(x, weights, tokens, g_log_probs, g_log_sums):
+        outs, pullback = mj.vjp(lambda x, w: nn.linear_log_probs(x, w, tokens, transposed), x, weights)
+        return tuple(outs) + pullback((g_log_probs, g_log_sums))
+    return f
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('shape,hidden,vocabulary', [((5,), 7, 11), ((2, 3), 4, 6), ((), 3, 5), ((4,), 1, 1)])
+def test_linear_log_probs_oracle_is_torchs(shape, hidden, vocabulary, transposed):
+    x, w = normal(1, *shape, hidden), normal(2, *((vocabulary, hidden) if transposed else (hidden, vocabulary)))
+    tokens = np.random.default_rng(3).integers(-1, vocabulary + 1, shape).astype(np.int32)
+    g, gs = normal(4, *shape) if shape else f32(0.7), normal(5, *shape) if shape else f32(-0.2)
+    got = evaluate(loss_program(transposed), x, w, tokens, g, gs)
+    tx, tw = leaf(x), leaf(w)
+    scores = tx @ (tw.T if transposed else tw)
+    token  = torch.tensor(np.asarray(tokens, np.int64))
+    given  = (token >= 0) & (token < vocabulary)
+    log_sum = torch.where(given, torch.logsumexp(scores, -1), 0.0)
+    log_prob = torch.where(given, torch.gather(torch.log_softmax(scores, -1), -1, token.clamp(0, vocabulary - 1)[..., None])[..., 0], 0.0)
+    ((log_prob * torch.tensor(g)).sum() + (log_sum * torch.tensor(gs)).sum()).backward()
+    same_as_torch(got, [log_prob, log_sum, tx.grad, tw.grad])
+
+
+def test_linear_log_probs_are_the_log_probs_of_the_product():
+    x, w, tokens = normal(1, 6, 5), normal(2, 5, 9), np.array([0, 8, -1, 3, 9, 3], np.int32)
+    a = evaluate(lambda x, w: nn.linear_log_probs(x, w, tokens)[0], x, w)[0]
+    b = evaluate(lambda x, w: nn.token_log_probs(jnp.dot(x, w), tokens)[0], x, w)[0]
+    assert np.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=np.ones((3, 5), f32)), TypeError), (dict(x=np.ones((3, 4), np.int32)), TypeError), (dict(weights=np.ones((7, 4), f32)), TypeError), (dict(weights=np.ones(4, f32)), TypeError),
+    (dict(weights=np.ones((4, 0), f32)), TypeError), (dict(x=np.ones((3, 0), f32), weights=np.ones((0, 7), f32)), TypeError), (dict(tokens=np.ones(4, np.int32)), TypeError),
+    (dict(tokens=np.ones((3, 1), np.int32)), TypeError), (dict(tokens=np.ones(3, f32)), TypeError), (dict(x=np.ones((), f32), tokens=np.ones((), np.int32)), TypeError)])
+def test_linear_log_probs_refuse(change, error):
+    given = dict(dict(x=np.ones((3, 4), f32), weights=np.ones((4, 7), f32), tokens=np.ones(3, np.int32)), **change)
+    refused(error, lambda *a: nn.linear_log_probs(*a), *given.values())
+    refused(error, lambda *a: lax.linear_log_probs_grad(*a, np.ones(3, f32), np.ones(3, f32)), *given.values())
+
+
+def test_linear_log_probs_refuse_weights_the_other_way_round():
+    x, t = np.ones((3, 4), f32), np.ones(3, np.int32)
+    refused(TypeError, lambda x, w, t: nn.linear_log_probs(x, w, t, transposed=True), x, np.ones((4, 7), f32), t)
+    refused(TypeError, lambda x, w, t: nn.linear_log_probs(x, w, t), x, np.ones((7, 4), f32), t)
+
+
+def test_linear_log_probs_gradient_refuses_what_does_not_belong():
+    x, w, t, row = np.ones((3, 4), f32), np.ones((4, 7), f32), np.ones(3, np.int32), np.ones(3, f32)
+    for bad in (np.ones(4, f32), np.ones((3, 1), f32), np.ones(3, np.int32)):
+        for at in range(4):
+            values = [row] * 4
+            values[at] = bad
+            refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a), x, w, t, *values)
+    refused(NotImplementedError, lambda x, w, t, g: mj.vjp(lambda x: lax.linear_log_probs(x, w, t)[2], x)[1](g), x, w, t, row)
+
+
+def test_log_probs_of_no_rows_are_planned():
+    x, w, t, g = np.zeros((0, 4), f32), normal(1, 4, 7), np.zeros(0, np.int32), np.zeros(0, f32)
+    _, _, dx, dw = evaluate(loss_program(False), x, w, t, g, g)
+    assert dx.shape == (0, 4) and not dw.any()
+    JaxprInterpreter(mj.make_jaxpr(loss_program(False))(x, w, t, g, g), plan_only=True)

@@ -24,7 +24,7 @@ DEVICE_FLAGS = ['-O3', f'--offload-arch={ARCH}', '--genco', '-munsafe-fp-atomics
                 '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-Wno-pass-failed']
 
 KERNEL_SOURCES = ['elementwise', 'rows', 'conv_gemm', 'wgrad_gemm', 'reduce', 'index', 'threefry', 'norm', 'log_probs', 'recurrence',
-                  'causal_conv', 'selective_scan']
+                  'causal_conv', 'selective_scan', 'linear_log_probs']
 
 
 def shim_path():
@@ -85,7 +85,7 @@ def build_call(force=True):
 
 def build_kernel(name, force=True):
     src  = os.path.join(CSRC, 'kernels', f'{name}.hip')
-    deps = [src] + [os.path.join(CSRC, 'kernels', h) for h in ('common.h', 'ew_opcodes.h', 'ew_apply.h', 'conv_quad.h', 'conv_split.h', 'split_bf16.h', 'wgrad_split.h')]
+    deps = [src] + [os.path.join(CSRC, 'kernels', h) for h in ('common.h', 'ew_opcodes.h', 'ew_apply.h', 'conv_quad.h', 'conv_split.h', 'split_bf16.h', 'wgrad_split.h', 'half_product.h')]
     out  = hsaco_path(name)
     if not force and _newer(out, deps):
         return out

@@ -2702,3 +2702,130 @@ def selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept: 
     launches.append(Launch('selective_scan_sums', (blocks, 1, 1), (1024, 1, 1), [(v, 0) for v in (da, db, dc, dd, dbias, maps, rows)],
                            _u32(0, batch * tiling.chunks, channels, n, tiling.strips, batch * time, map_blocks), bytes_moved=4 * (maps.size + rows.size), written=(0, 1, 2, 3, 4)))
     return launches
+
+
+# ---------------------------------------------------------------- products on the fp16 matrix cores (half_product.h)
+
+HALF_TILE = 128                         #rows and columns of a block's tile
+HALF_BLOCKS = 512                       #blocks that the machine runs at once
+
+
+def _half_steps(k: int) -> int:
+    '''Steps of 16 of a contraction, which come in pairs.'''
+    return 2 * _cdiv(k, 32)
+
+
+def _half_words(i: int, k: int) -> int:
+    '''Words of an operand [i, k] that has been taken apart.'''
+    return _cdiv(i, 32) * _half_steps(k) * 512
+
+
+def _u64(*values) -> bytes:
+    return np.asarray([int(v) for v in values], dtype=np.uint64).tobytes()
+
+
+# ---------------------------------------------------------------- log probabilities from weights (linear_log_probs.hip)
+
+LINEAR_ROWS       = 64                  #rows up to which the weights are read as they are
+LINEAR_PIECE      = 256 << 20           #bytes of the scores' cotangents that are there at a time
+LINEAR_SLICE      = 16                  #pairs of steps of a slice of a contraction, at least
+_PACK_WEIGHTS, _PACK_ROWS, _PACK_SCALED = 0, 1, 2
+
+
+class LinearShape(tp.NamedTuple):
+    rows:   int
+    hidden: int
+    tokens: int
+
+
+def _linear_shape(x: Buffer, w: Buffer, transposed: bool) -> LinearShape:
+    h, v   = reversed(w.shape) if transposed else w.shape
+    shape  = LinearShape(x.size // h, h, v)
+    #(indices of rows, tokens and steps are 32 bits, addresses 64)
+    if max(shape) >= 2**27 or _cdiv(shape.rows, HALF_TILE) * _cdiv(v, HALF_TILE) >= 2**23:
+        raise NotImplementedError(f'log probabilities of {shape.rows} rows of {h} over {v} tokens')
+    return shape
+
+
+def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, cotangents, scratch):
+    '''The operands that the products need, taken apart: (launches, W contracted over h, x, their scales; with cotangents also W contracted over the
+    vocabulary, x with its rows' factors contracted over the rows, and the factors).'''
+    rows, h, v = shape
+    weight_blocks = max(1, min(512, _cdiv(h * v, 4096)))
+    row_blocks    = max(1, min(256, _cdiv(rows, 4)))
+    largest = scratch((weight_blocks + 2 * row_blocks,))
+    factors = scratch((rows, 3)) if cotangents else None
+    scales  = scratch((4,), np.int32)
+    g_log_probs, g_log_sums = cotangents or (None, None)
+    by_v, by_h = ((h, 1), (1, h)) if transposed else ((1, v), (v, 1))                       #element strides of (token, h) and (h, token)
+    jobs = [(v, h, _PACK_WEIGHTS, by_v), (rows, h, _PACK_ROWS, (h, 1))]
+    if cotangents:
+        jobs += [(h, v, _PACK_WEIGHTS, by_h), (h, rows, _PACK_SCALED, (1, h))]
+    parts  = [scratch((_half_words(i, k),), np.uint32) for i, k, _, _ in jobs]
+    params, blocks = _u32(weight_blocks, row_blocks, v, 0), 0
+    for i, k, kind, strides in jobs:
+        steps  = _half_steps(k)
+        each   = min(steps, 8)
+        blocks += _cdiv(_cdiv(i, 32) * _cdiv(steps, each), 4)
+        params += _u32(_cdiv(_cdiv(i, 32) * _cdiv(steps, each), 4), i, k, each, kind, steps) + _u64(*strides)
+    params += bytes(40) * (4 - len(jobs))
+    launches = [Launch('linear_largest', (weight_blocks + row_blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (largest, factors, x, w, tokens, g_log_probs, g_log_sums)],
+                       _u32(0, rows, h, v, weight_blocks, row_blocks), bytes_moved=4 * (x.size + w.size), written=(0, 1)),
+                Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in parts] + [(None, 0)] * (4 - len(parts)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors)],
+                       params, bytes_moved=8 * (x.size + w.size) * (1 + bool(cotangents)), written=(0, 1, 2, 3, 4))]
+    return launches, parts, scales, factors
+
+
+def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch) -> tp.List[Launch]:
+    shape = rows, h, v = _linear_shape(x, w, transposed)
+    tiles    = _cdiv(v, HALF_TILE)
+    of_tiles = [scratch((tiles, rows)), scratch((tiles, rows)), scratch((rows,))]           #peak and sum of each tile's scores, the token's score
+    if rows <= LINEAR_ROWS and v >= 4:
+        launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles, 1, 1), (512, 1, 1), [(b, 0) for b in (*of_tiles, x, w, tokens)],
+                           _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2))]
+    else:
+        launches, (w_parts, x_parts), scales, _ = _linear_prepare(shape, x, w, tokens, transposed, None, scratch)
+        launches.append(Launch('linear_scores', (tiles * _cdiv(rows, HALF_TILE), 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (*of_tiles, w_parts, x_parts, tokens, scales)],
+                               _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, _cdiv(rows, HALF_TILE), _cdiv(v, 32), _cdiv(rows, 32), 0, 0, 0),
+                               bytes_moved=4 * (w_parts.size + x_parts.size), flops=2 * rows * h * v, written=(0, 1, 2)))
+    return launches + [Launch('linear_join', (_cdiv(rows, 64), 1, 1), (1024, 1, 1), [(b, 0) for b in (log_probs, log_sums, peaks, totals, *of_tiles, tokens)],
+                              _u32(0, rows, v, tiles), bytes_moved=8 * tiles * rows, written=(0, 1, 2, 3))]
+
+
+def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch) -> tp.List[Launch]:
+    shape = rows, h, v = _linear_shape(x, w, transposed)
+    launches, (w_parts, x_parts, w_by_h, x_scaled), scales, factors = _linear_prepare(shape, x, w, tokens, transposed, (g_log_probs, g_log_sums), scratch)
+    #pieces of the vocabulary, of whole tiles
+    row_blocks, all_tiles = _cdiv(rows, 32), _cdiv(v, HALF_TILE)
+    pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (8 * 32 * row_blocks * HALF_TILE)))
+    each   = _cdiv(all_tiles, pieces)
+    pieces = _cdiv(all_tiles, each)
+    width  = each * HALF_TILE
+    by_row, by_token = scratch((row_blocks * (width // 16) * 512,), np.uint32), scratch((width // 32 * 2 * row_blocks * 512,), np.uint32)
+    tiles_r, tiles_h = _cdiv(rows, HALF_TILE), _cdiv(h, HALF_TILE)
+    slices = max(1, min(_cdiv(HALF_BLOCKS, tiles_r * tiles_h), width // 32 // LINEAR_SLICE))
+    parts  = scratch((pieces * slices, rows, h)) if pieces * slices > 1 else dx
+
+    def product(out, offset, a, b, m, n, k_pairs, slices, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b, scale_a, scale_b, ld, slice_, by_rows):
+        tiles = (_cdiv(m, HALF_TILE), _cdiv(n, HALF_TILE))
+        return Launch('linear_product', (tiles[0] * tiles[1] * slices, 1, 1), (BLOCK, 1, 1), [(out, 4 * offset), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
+                      _u32(m, n, *tiles, slices, k_pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b) + _i32(scale_a, scale_b) + _u64(ld, slice_),
+                      bytes_moved=4 * (m + n) * 32 * k_pairs + 4 * m * n * slices, flops=64 * m * n * k_pairs)
+    for piece in range(pieces):
+        first = piece * each
+        tiles = min(each, all_tiles - first)
+        v0, n = first * HALF_TILE, min(width, v - first * HALF_TILE)
+        launches.append(Launch('linear_q', (tiles * tiles_r, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (by_row, by_token, w_parts, x_parts, tokens, scales, peaks, totals, factors)],
+                               _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, tiles_r, _cdiv(v, 32), row_blocks, first, width, 0),
+                               bytes_moved=8 * 32 * row_blocks * width, flops=2 * rows * h * n, written=(0, 1)))
+        launches.append(product(parts, piece * slices * rows * h, by_row, w_by_h, rows, h, _cdiv(n, 32), slices, row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), 0, v0 // 16,
+                                -1, _PACK_WEIGHTS, h, rows * h, True))
+        scaled, q = (x_scaled, _cdiv(h, 32), 2 * row_blocks), (by_token, tiles * 4, 2 * row_blocks)
+        if transposed:
+            launches.append(product(dw, v0 * h, q[0], scaled[0], n, h, row_blocks, 1, q[1], scaled[1], q[2], scaled[2], 0, 0, -1, _PACK_SCALED, h, 0, False))
+        else:
+            launches.append(product(dw, v0, scaled[0], q[0], h, n, row_blocks, 1, scaled[1], q[1], scaled[2], q[2], 0, 0, _PACK_SCALED, -1, v, 0, False))
+    if pieces * slices > 1:
+        launches.append(Launch('linear_sum', (_cdiv(rows * h, 4 * BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (parts, 0)], _u32(pieces * slices, 0) + _u64(rows * h),
+                               bytes_moved=4 * (parts.size + rows * h)))
+    return launches

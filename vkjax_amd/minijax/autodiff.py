@@ -391,6 +391,13 @@ def _selective_scan(gs, x, delta, a, b, c, *rest, softplus, kept, has_d, has_gat
     return tuple(grads)
 
 
+@_rule('linear_log_probs')
+def _linear_log_probs(gs, x, weights, tokens, outs, transposed):
+    if gs[2] is not None or gs[3] is not None:
+        raise NotImplementedError('differentiation through the largest scores and the sums of linear_log_probs')
+    return lax.linear_log_probs_grad(x, weights, tokens, outs[2], outs[3], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), transposed) + (None,)
+
+
 _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', 'iota', 'and', 'or', 'not', 'xor', 'sign', 'floor', 'ceil',
                        'round', 'is_finite', 'shift_left', 'shift_right_logical', 'shift_right_arithmetic', 'threefry2x32',
                        'random_bits', 'random_split', 'random_wrap', 'random_unwrap', 'random_fold_in', 'random_seed'}

@@ -787,6 +787,37 @@ def selective_scan_grad(kept, x, delta, a, b, c, d=None, gate=None, state=None, 
     return tuple(emit(name, [kept] + operands, avals, dict(params, has_g=g is not None, has_last=g_last is not None), multiple_results=True))
 
 
+def _linear_log_probs_operands(name, x, weights, tokens, transposed):
+    x, weights, tokens = _f32_operand(x, name), _f32_operand(weights, name), _integer_operand(tokens, name)
+    xs, ws = _shape(x), _shape(weights)
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1 if transposed else 0]:
+        raise TypeError(f'{name} takes x [..., hidden] and weights {"[vocabulary, hidden]" if transposed else "[hidden, vocabulary]"}, got {xs} and {ws}')
+    if 0 in ws:
+        raise TypeError(f'{name}: at least one token and one feature are needed, got weights {ws}')
+    if _shape(tokens) != xs[:-1]:
+        raise TypeError(f'{name}: one token per row of {xs} is needed, got {_shape(tokens)}')
+    return x, weights, tokens
+
+
+def linear_log_probs(x, weights, tokens, transposed: bool = False):
+    '''For rows x [..., hidden], weights [hidden, vocabulary] (`transposed`: [vocabulary, hidden]) and one token per row, with scores = x @ weights: (log softmax(scores)[token],
+    log(sum(exp(scores)))), and what linear_log_probs_grad needs of them: each row's largest score and the sum of exp(scores - largest), all [...]. The scores are
+    not kept. `nn.linear_log_probs` says what becomes of padded rows and how exact the products are.'''
+    x, weights, tokens = _linear_log_probs_operands('linear_log_probs', x, weights, tokens, transposed)
+    return tuple(emit('linear_log_probs', [x, weights, tokens], [_aval(_shape(tokens), _f32)] * 4, dict(transposed=bool(transposed)), multiple_results=True))
+
+
+def linear_log_probs_grad(x, weights, tokens, peaks, totals, g_log_probs=None, g_log_sums=None, transposed: bool = False):
+    '''(dx, dweights) for the cotangents (None: zeros) of linear_log_probs' first two results; peaks and totals are the others.'''
+    name = 'linear_log_probs_grad'
+    x, weights, tokens = _linear_log_probs_operands(name, x, weights, tokens, transposed)
+    rows = _shape(tokens)
+    operands = [x, weights, tokens] + [_shaped_operand(name, 'a value per row', v, rows) for v in (peaks, totals)]
+    operands += [_shaped_operand(name, 'a cotangent', v, rows) for v in (g_log_probs, g_log_sums) if v is not None]
+    return tuple(emit(name, operands, [_aval(_shape(x), _f32), _aval(_shape(weights), _f32)],
+                      dict(transposed=bool(transposed), has_log_probs=g_log_probs is not None, has_log_sums=g_log_sums is not None), multiple_results=True))
+
+
 # ---------------------------------------------------------------- rng
 
 def threefry2x32(key0, key1, x0, x1):

@@ -91,3 +91,17 @@ def selective_scan(x, delta, a, b, c, d=None, gate=None, state=None, lengths=Non
     padded batch, in which a sequence's state stays and y is 0 from its length on, and nothing else is looked at there. Differentiable with respect to
     every float32 operand. `lax.selective_scan` says what long products of factors come to.'''
     return lax.selective_scan(x, delta, a, b, c, d, gate, state, lengths, delta_bias, softplus)
+
+
+def linear_log_probs(x, weights, tokens, transposed=False):
+    '''Log probabilities of given tokens (or classes) under softmax(x @ weights), without keeping the scores: x [..., hidden], weights [hidden, vocabulary], or with `transposed` the
+    rows of an embedding, [vocabulary, hidden]; tokens int32 [...]. Returns (log_probs [...], log_sums [...]), the latter being log(sum(exp(scores))) of each row. A cross entropy is
+    -log_probs; the gradient works the scores out again, a piece of the vocabulary at a time.
+
+    * A row whose token lies outside the vocabulary (negative, say) is padding: its results are 0, no gradient comes from it, and its x is not looked at.
+    * Products are as exact as fp32's for numbers down to 2^-28 of the largest of their operand (x's given rows, the weights); smaller ones are off by up to 2^-51 of that
+      largest. (Up to 64 rows, without a gradient, are computed by fp32 products.)
+    * NaN and infinities in a row of x make that row's results NaN, in the weights those of every row.
+
+    Differentiable with respect to x and weights, through both results.'''
+    return lax.linear_log_probs(x, weights, tokens, transposed)[:2]

@@ -1230,6 +1230,30 @@ def selective_scan_grad(bufferpool, equation):
                                                          g, g_last, p['softplus'], scratch))
 
 
+def linear_log_probs(bufferpool, equation):
+    (x, weights, tokens), outs, scratch = _operator_buffers(bufferpool, equation)
+    _float_operands(equation, x, weights)
+    if _kind(tokens.dtype) not in (_I, _U):
+        raise NotImplementedError(equation)
+    return _operator_ops(equation, K.linear_log_probs(*outs, x, weights, tokens, equation.params['transposed'], scratch))
+
+
+def linear_log_probs_grad(bufferpool, equation):
+    p = equation.params
+    (x, weights, tokens, peaks, totals, *rest), (dx, dweights), scratch = _operator_buffers(bufferpool, equation)
+    g_log_probs = rest.pop(0) if p['has_log_probs'] else None
+    g_log_sums  = rest.pop(0) if p['has_log_sums'] else None
+    _float_operands(equation, x, weights, peaks, totals, g_log_probs, g_log_sums)
+    if _kind(tokens.dtype) not in (_I, _U):
+        raise NotImplementedError(equation)
+    if x.size == 0:
+        return [Op(equation, launch=K.fill(dweights, 0))] if dweights is not None else []          #a sum over no rows
+    if dx is None or dweights is None:
+        dx       = dx if dx is not None else scratch(x.shape)
+        dweights = dweights if dweights is not None else scratch(weights.shape)
+    return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch))
+
+
 # ------------------------------------------------------------------ rng
 
 def threefry2x32(bufferpool, equation):
