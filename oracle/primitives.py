@@ -1083,3 +1083,18 @@ def linear_log_probs_grad(x, weights, tokens, peaks, totals, *cotangents, transp
         d[~given] = 0.0
         dw = rows.T @ d
         return (d @ w.T).reshape(x.shape).astype(f32), (dw.T if transposed else dw).astype(f32)
+
+
+def orthogonalize(x, steps, coefficients, eps):
+    a, b, c = (np.float64(v) for v in coefficients)
+    if np.size(x) == 0:
+        return np.zeros(x.shape, f32)
+    with np.errstate(**_EW_ERR):
+        found = np.asarray(x, np.float64).reshape(-1, *x.shape[-2:]).copy()
+        for i, m in enumerate(found):
+            m = m / (np.sqrt((m * m).sum()) + np.float64(np.float32(eps)))
+            for _ in range(steps):
+                square = m @ m.T
+                m = a * m + (b * square + c * (square @ square)) @ m
+            found[i] = m
+        return found.reshape(x.shape).astype(f32)

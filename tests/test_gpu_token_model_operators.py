@@ -328,3 +328,71 @@ def test_linear_log_probs_of_nothing_but_padding():
         x, w, tokens, g, gs = loss_inputs(rows, 40, 300, False)
         got = mj.tree_leaves(both(loss_program(False), np.full_like(x, np.nan), w, np.full_like(tokens, -1), g, gs)[0])
         assert not any(v.any() for v in got)
+
+
+# ------------------------------------------------------------------ orthogonalised matrices
+
+def typical_error(a, b):
+    '''The root mean square of a product's error, 16 times over: 2^-24 of each term's, terms independent of one another, and what rounding a sum of terms of one sign 64 times leaves.'''
+    return 2.0 ** -20 * (np.sqrt((a * a) @ (b * b)) + np.abs(a @ b))
+
+
+def orthogonal_bound(x, steps, coefficients, eps=1e-7):
+    '''How far the result may be off (Frobenius norm). What a step leaves is raised by the steps behind it by no more than the largest difference quotient of their polynomial (of odd
+    matrix functions: Daleckii and Krein), the largest slope between 0 and the largest singular value, or value by its argument.'''
+    a, b, c = (float(f32(v)) for v in coefficients)
+    m = x.astype(np.float64)
+    m = m.T if m.shape[0] > m.shape[1] else m
+    m = m / (np.sqrt((m * m).sum()) + eps)
+    errors, tops = [2.0 ** -21 * np.linalg.norm(m)], []
+    for _ in range(steps):
+        tops.append(np.linalg.norm(m, 2))
+        square = m @ m.T
+        e_square = typical_error(m, m.T)
+        p = a * np.eye(len(m)) + b * square + c * square @ square
+        e_p = abs(b) * e_square + abs(c) * (2 * e_square @ np.abs(square) / np.sqrt(len(m)) + typical_error(square, square)) + 2.0 ** -21 * np.abs(p)
+        errors.append(np.linalg.norm(np.sqrt((e_p * e_p) @ (m * m))) + np.linalg.norm(typical_error(p, m)) + 2.0 ** -21 * np.linalg.norm(p @ m))
+        m = p @ m
+    total = 0.0
+    for i, e in enumerate(errors):
+        s = np.linspace(1e-9, 1.01 * (tops[i] if i < steps else 1.0), 2000)
+        at, slope = s, np.ones_like(s)
+        for _ in range(steps - i):
+            slope = slope * (a + 3 * b * at**2 + 5 * c * at**4)
+            at = a * at + b * at**3 + c * at**5
+        total += e * max(np.abs(slope).max(), np.abs(at / s).max())
+    return total + 1e-30
+
+
+#shapes: one element, fewer rows than a block of 32, wide and tall, no multiples of anything, one tile and several, stacks
+MATRICES = [(1, 1), (1, 9), (5, 3), (2, 7, 40), (33, 65), (128, 128), (3, 130, 100), (2, 2, 64, 200), (257, 129), (300, 520), (20, 32, 31), (129, 1000)]
+
+
+@pytest.mark.parametrize('steps,coefficients', [(5, (3.4445, -4.7750, 2.0315)), (1, (1.5, -0.5, 0.0)), (2, (2.0, -1.5, 0.5))], ids=str)
+@pytest.mark.parametrize('shape', MATRICES, ids=str)
+def test_orthogonalize(shape, steps, coefficients):
+    print(f'orthogonalize {shape}, {steps} steps, {coefficients}', flush=True)
+    x = normal(sum(shape), *shape, scale=1e-3)
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, steps, coefficients), x)
+    assert got.shape == shape
+    for a, b, m in zip(got.reshape(-1, *shape[-2:]), expected.reshape(-1, *shape[-2:]), x.reshape(-1, *shape[-2:])):
+        off, bound = np.linalg.norm(a.astype(np.float64) - b), orthogonal_bound(m, steps, coefficients)
+        assert off <= bound, (off, bound)
+
+
+@pytest.mark.parametrize('scale', [1e-12, 1e-7, 1e15])
+def test_orthogonalize_by_the_size_of_its_matrix(scale):
+    x = normal(1, 40, 50, scale=scale)
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x), x)
+    assert np.linalg.norm(got.astype(np.float64) - expected) <= orthogonal_bound(x, 5, (3.4445, -4.7750, 2.0315))
+
+
+def test_orthogonalize_a_matrix_of_a_low_rank_and_of_zeros():
+    x = normal(1, 4, 150, 90, scale=1e-2)
+    x[1] = normal(2, 150, 2) @ normal(3, 2, 90)
+    x[2] = 0.0
+    x[3, 7, 8] = np.nan
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x), x)
+    assert not got[2].any() and np.isnan(got[3]).all()
+    for i in (0, 1):
+        assert np.linalg.norm(got[i].astype(np.float64) - expected[i]) <= orthogonal_bound(x[i], 5, (3.4445, -4.7750, 2.0315))

@@ -6,7 +6,7 @@ import torch
 
 from oracle import primitives as P
 from tests.test_operators import ROUNDED, evaluate, normal, refused
-from vkjax_amd import minijax as mj
+from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
 jnp, lax, nn = mj.numpy, mj.lax, mj.nn
@@ -305,3 +305,62 @@ def test_log_probs_of_no_rows_are_planned():
     _, _, dx, dw = evaluate(loss_program(False), x, w, t, g, g)
     assert dx.shape == (0, 4) and not dw.any()
     JaxprInterpreter(mj.make_jaxpr(loss_program(False))(x, w, t, g, g), plan_only=True)
+
+
+# ------------------------------------------------------------------ orthogonalised matrices
+
+@pytest.mark.parametrize('shape', [(4, 7), (7, 4), (2, 3, 5, 5), (1, 1), (1, 6)])
+@pytest.mark.parametrize('steps,coefficients', [(5, (3.4445, -4.7750, 2.0315)), (1, (2.0, -1.5, 0.5)), (20, (1.5, -0.5, 0.0))])
+def test_orthogonalize_is_a_polynomial_of_the_singular_values(shape, steps, coefficients):
+    x = normal(1, *shape)
+    got, = evaluate(lambda x: nn.orthogonalize(x, steps, coefficients), x)
+    a, b, c = (float(f32(v)) for v in coefficients)
+    u, s, v = np.linalg.svd(x.astype(np.float64), full_matrices=False)
+    s = s / (np.sqrt((x.astype(np.float64) ** 2).sum(axis=(-2, -1), keepdims=True))[..., 0] + float(f32(1e-7)))
+    for _ in range(steps):
+        s = a * s + b * s**3 + c * s**5
+    #(64 bits, whose roundings the steps raise by 3.5^5 at most, then one to fp32 of values below 2)
+    assert np.allclose(got, u @ (s[..., None] * v), rtol=0, atol=1e-10 + 2.0 ** -23)
+
+
+def test_orthogonalize_brings_singular_values_to_one():
+    for shape in ((20, 30), (30, 20)):
+        s = np.linalg.svd(evaluate(lambda x: nn.orthogonalize(x), normal(2, *shape))[0], compute_uv=False)
+        assert s.min() > 0.6 and s.max() < 1.3
+        s = np.linalg.svd(evaluate(lambda x: nn.orthogonalize(x, 25, (1.5, -0.5, 0.0)), normal(2, *shape))[0], compute_uv=False)
+        assert np.allclose(s, 1.0, atol=1e-5)
+
+
+def test_orthogonalize_of_zeros_and_of_matrices_by_themselves():
+    x = normal(1, 3, 4, 6)
+    x[0], x[1, 2, 3] = 0.0, np.nan
+    got, = evaluate(lambda x: nn.orthogonalize(x), x)
+    alone, = evaluate(lambda x: nn.orthogonalize(x), x[2])
+    assert not got[0].any() and np.isnan(got[1]).all() and np.array_equal(got[2], alone)
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=np.ones(4, f32)), TypeError), (dict(x=np.ones((4, 4), np.int32)), TypeError), (dict(steps=0), ValueError), (dict(steps=33), ValueError), (dict(steps=2.5), ValueError),
+    (dict(coefficients=(1.0, 2.0)), ValueError), (dict(coefficients=(1.0, np.nan, 0.0)), ValueError), (dict(coefficients=(3.0, 2.0, 1.0)), ValueError), (dict(eps=0.0), ValueError),
+    (dict(eps=-1e-7), ValueError), (dict(eps=np.inf), ValueError)])
+def test_orthogonalize_refuses(change, error):
+    given = dict(dict(x=np.ones((4, 4), f32), steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7), **change)
+    refused(error, lambda x: nn.orthogonalize(x, given['steps'], given['coefficients'], given['eps']), given['x'])
+
+
+def test_orthogonalize_has_no_gradient_and_takes_no_elements():
+    refused(NotImplementedError, lambda x: mj.grad(lambda v: jnp.sum(nn.orthogonalize(v)))(x), np.ones((3, 4), f32))
+    for shape in ((0, 4), (4, 0), (0, 3, 4)):
+        assert evaluate(lambda x: nn.orthogonalize(x), np.zeros(shape, f32))[0].shape == shape
+        JaxprInterpreter(mj.make_jaxpr(lambda x: nn.orthogonalize(x))(np.zeros(shape, f32)), plan_only=True)
+
+
+def test_orthogonalize_knows_how_large_singular_values_become():
+    rng = np.random.default_rng(0)
+    for steps, coefficients in ((5, (3.4445, -4.7750, 2.0315)), (8, (3.4445, -4.7750, 2.0315)), (6, (1.5, -0.5, 0.0)), (4, (2.0, -1.5, 0.5)), (3, (1.0, 0.5, 0.25))):
+        a, b, c = coefficients
+        s = rng.random(200000)
+        for most, polynomial in K.orthogonal_bounds(steps, coefficients):
+            p = a + b * s**2 + c * s**4
+            assert 1.1 * np.abs(s).max() < most and 1.1 * np.abs(p).max() < polynomial and polynomial >= abs(a)
+            s = p * s

@@ -24,7 +24,7 @@ DEVICE_FLAGS = ['-O3', f'--offload-arch={ARCH}', '--genco', '-munsafe-fp-atomics
                 '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-Wno-pass-failed']
 
 KERNEL_SOURCES = ['elementwise', 'rows', 'conv_gemm', 'wgrad_gemm', 'reduce', 'index', 'threefry', 'norm', 'log_probs', 'recurrence',
-                  'causal_conv', 'selective_scan', 'linear_log_probs']
+                  'causal_conv', 'selective_scan', 'linear_log_probs', 'orthogonalize']
 
 
 def shim_path():

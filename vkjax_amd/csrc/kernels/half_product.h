@@ -97,3 +97,65 @@ __device__ __forceinline__ void half_tile_of(uint32_t block, uint32_t blocks, ui
     const uint32_t strip = id / (8u * tiles_m), width = min(8u, tiles_n - 8u * strip), at = id - strip * 8u * tiles_m;
     m = at / width; n = 8u * strip + at - m * width;
 }
+
+// ---- a tile of a result as an operand of products that follow: contracted over its rows, as the lanes have it (`by_column`: its index is the column), or over its columns (`by_row`),
+// turned in shared memory. value(block of rows i, of columns j, register, row, column) is what is taken apart, scaled; it is zero behind the result's last row and column.
+constexpr uint32_t HALF_PITCH = 132u;                    // words of a row in shared memory: lanes that read vectors of neighbouring rows meet no bank twice
+typedef uint32_t HalfTurned[HALF_TILE][HALF_PITCH];
+union HalfShared { HalfStage stages[2]; HalfTurned turned; };
+
+struct HalfTarget { u32x4* parts; uint32_t blocks, steps, block, step; };      // blocks of 32 of its index, steps of 16 k per block (all of them); where this tile's begin
+
+template <class F>
+__device__ __forceinline__ void half_store(HalfTurned& turned, const HalfTarget& by_column, const HalfTarget& by_row, F value) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t column = wn * 64u + 32u * j + (lane & 31u), block = by_column.block + wn * 2u + j;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t row0 = wm * 64u + 32u * i + 4u * (lane >> 5);
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t row = row0 + 8u * (k >> 1) + 2u * (k & 1);
+                half_parts(value(i, j, 2 * k, row, column), value(i, j, 2 * k + 1, row + 1u, column), hi[k], lo[k]);
+            }
+            if (by_column.parts && block < by_column.blocks)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t step = by_column.step + wm * 4u + 2u * i + s;
+                    if (step < by_column.steps) {
+                        u32x4* const to = by_column.parts + ((uint64_t)block * by_column.steps + step) * 128u + lane;
+                        to[0]  = u32x4{hi[4 * s], hi[4 * s + 1], hi[4 * s + 2], hi[4 * s + 3]};
+                        to[64] = u32x4{lo[4 * s], lo[4 * s + 1], lo[4 * s + 2], lo[4 * s + 3]};
+                    }
+                }
+            if (by_row.parts)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t h = k & 1 ? hi[k >> 1] >> 16 : hi[k >> 1] & 0xFFFFu, l = k & 1 ? lo[k >> 1] & 0xFFFF0000u : lo[k >> 1] << 16;
+                    turned[row0 + 8u * (k >> 2) + (k & 3)][column] = h | l;
+                }
+        }
+    }
+    if (!by_row.parts) return;
+    __syncthreads();
+    // wave: a block of 32 rows, the tile's eight steps of 16 columns
+    const uint32_t block = by_row.block + wave;
+    const uint32_t* const row = &turned[wave * 32u + (lane & 31u)][0];
+    if (block >= by_row.blocks) return;
+#pragma unroll
+    for (uint32_t s = 0; s < 8u; ++s) {
+        if (by_row.step + s >= by_row.steps) break;
+        u32x4 hi, lo;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16u * s + 8u * q + 4u * (lane >> 5));
+            hi[2 * q] = (t.x & 0xFFFFu) | t.y << 16; hi[2 * q + 1] = (t.z & 0xFFFFu) | t.w << 16;
+            lo[2 * q] = t.x >> 16 | (t.y & 0xFFFF0000u); lo[2 * q + 1] = t.z >> 16 | (t.w & 0xFFFF0000u);
+        }
+        u32x4* const to = by_row.parts + ((uint64_t)block * by_row.steps + by_row.step + s) * 128u + lane;
+        to[0] = hi; to[64] = lo;
+    }
+}

@@ -366,68 +366,31 @@ SCORES_ROWS(h_64, false, 2)
 extern "C" __global__ __launch_bounds__(256, 2) void linear_q(u32x4* __restrict__ by_row, u32x4* __restrict__ by_token, const u32x4* __restrict__ w, const u32x4* __restrict__ x,
                                                               const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, const float* __restrict__ row_peaks,
                                                               const float* __restrict__ row_totals, const float* __restrict__ factors, ScoresParams P) {
-    constexpr uint32_t PITCH = 132u;                     // words of a token's rows in shared memory: lanes that read vectors of neighbouring tokens meet no bank twice
-    __shared__ union { HalfStage stages[2]; uint32_t turned[128][PITCH]; } shared;
+    __shared__ HalfShared shared;
     uint32_t m, n;
     half_tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, m, n);
     HalfSums acc = {};
     half_product(acc, shared.stages, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, 0u, P.pairs);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]), up = power_of_two(Q_SCALE);
-    const uint32_t piece_steps = P.Vp / 16u, row_steps = P.blocks_x * 2u;
+    const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * 128u;
+    // of this lane's two columns
+    bool given[2];
+    uint32_t token[2];
+    float peak[2], part[2], one[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const uint32_t column = wn * 64u + j * 32u + (lane & 31u), r = n * 128u + column, at = min(r, P.rows - 1u), rb = n * 4u + wn * 2u + j;
-        const bool given = r < P.rows && is_token(tokens[at], P.V);
-        const uint32_t token = given ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
-        const float peak = row_peaks[at], all = given ? factors[3u * at + 1u] * up : 0.f, one = given ? factors[3u * at + 2u] * up : 0.f, part = all / row_totals[at];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t hi[8], lo[8];
-            float q[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const uint32_t v = (P.tile0 + m) * 128u + wm * 64u + 32u * i + 4u * (lane >> 5) + 8u * (k >> 2) + (k & 3);
-                const float s = __builtin_fmaf(acc.small[i][j][k], 1.f / HALF_REST, acc.large[i][j][k]) * down_w * down_x;
-                const float p = part * exp_of(s - peak) + (v == token ? one : 0.f);
-                q[k] = given && v < P.V ? p : 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) half_parts(q[2 * k], q[2 * k + 1], hi[k], lo[k]);
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint32_t step = (m * 128u + wm * 64u + 32u * i) / 16u + s;
-                if (by_row && rb < P.blocks_x) {
-                    u32x4* const to = by_row + ((uint64_t)rb * piece_steps + step) * 128u + lane;
-                    to[0]  = u32x4{hi[4 * s], hi[4 * s + 1], hi[4 * s + 2], hi[4 * s + 3]};
-                    to[64] = u32x4{lo[4 * s], lo[4 * s + 1], lo[4 * s + 2], lo[4 * s + 3]};
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const uint32_t h = k & 1 ? hi[k >> 1] >> 16 : hi[k >> 1] & 0xFFFFu, l = k & 1 ? lo[k >> 1] & 0xFFFF0000u : lo[k >> 1] << 16;
-                shared.turned[wm * 64u + 32u * i + 4u * (lane >> 5) + 8u * (k >> 2) + (k & 3)][column] = h | l;
-            }
-        }
+        const uint32_t r = n * 128u + wn * 64u + 32u * j + (lane & 31u), at = min(r, P.rows - 1u);
+        given[j] = r < P.rows && is_token(tokens[at], P.V);
+        token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
+        peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
-    __syncthreads();
-    if (!by_token) return;
-    // wave: a block of 32 tokens, the tile's eight steps of 16 rows
-    const uint32_t vb = m * 4u + wave;
-    const uint32_t* const row = &shared.turned[wave * 32u + (lane & 31u)][0];
-#pragma unroll
-    for (uint32_t s = 0; s < 8u; ++s) {
-        if (n * 8u + s >= row_steps) break;
-        u32x4 hi, lo;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16u * s + 8u * q + 4u * (lane >> 5));
-            hi[2 * q] = (t.x & 0xFFFFu) | t.y << 16; hi[2 * q + 1] = (t.z & 0xFFFFu) | t.w << 16;
-            lo[2 * q] = t.x >> 16 | (t.y & 0xFFFF0000u); lo[2 * q + 1] = t.z >> 16 | (t.w & 0xFFFF0000u);
-        }
-        u32x4* const to = by_token + ((uint64_t)vb * row_steps + n * 8u + s) * 128u + lane;
-        to[0] = hi; to[64] = lo;
-    }
+    half_store(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 4u, m * 8u}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 4u, n * 8u},
+               [&](int i, int j, int k, uint32_t row, uint32_t) {
+        const uint32_t v = v0 + row;
+        const float s = __builtin_fmaf(acc.small[i][j][k], 1.f / HALF_REST, acc.large[i][j][k]) * down_w * down_x;
+        const float q = part[j] * exp_of(s - peak[j]) + (v == token[j] ? one[j] : 0.f);
+        return given[j] && v < P.V ? q : 0.f;
+    });
 }
 
 // ---- a product of two operands to fp32 [M, N], rows by a factor each (every third word), slices of the contraction to arrays of their own

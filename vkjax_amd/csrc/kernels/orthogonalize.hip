@@ -1,0 +1,138 @@
+// Matrices with their singular values brought towards 1 by a polynomial: X = x / (|x| + eps) (Frobenius norm, per matrix), then `steps` times
+//   A = X X^T,  B = a I + b A + c A A,  X <- B X          (of the wide way round: a matrix with more rows than columns is transposed)
+// so that every singular value s becomes a s + b s^3 + c s^5. Products are those of half_product.h, between operands that never leave their taken-apart form: a product's tile
+// turns its results into the operands that the next ones need, contracted over its rows (as the lanes have them) and over its columns (turned in shared memory). A and B are symmetric:
+// of their tiles only those on and above the diagonal are computed, and stored both ways. Only A is kept as fp32 too, since b A is a term of B. X has 22 bits between the steps; no
+// operand's magnitude depends on the data beyond |x|, since a singular value's bound follows from the polynomial alone, so scales are known to the host.
+// Matrices of a stack lie side by side in every launch.
+#include "half_product.h"
+
+struct SquaresParams { uint32_t blocks, pad; uint64_t n; };
+// [matrix][block]: sums of squares
+extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __restrict__ sums, const float* __restrict__ x, SquaresParams P) {
+    __shared__ float part[4];
+    const uint32_t matrix = blockIdx.x / P.blocks, block = blockIdx.x % P.blocks;
+    const float* const from = x + matrix * P.n;
+    const uint64_t stride = (uint64_t)P.blocks * 256u;
+    float s[4] = {};
+    uint64_t at = (uint64_t)block * 256u + threadIdx.x;
+    for (; at + 3u * stride < P.n; at += 4u * stride)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const float v = from[at + k * stride]; s[k] = __builtin_fmaf(v, v, s[k]); }
+    for (; at < P.n; at += stride) s[0] = __builtin_fmaf(from[at], from[at], s[0]);
+    float t = (s[0] + s[1]) + (s[2] + s[3]);
+    wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
+    if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = t;
+    __syncthreads();
+    if (threadIdx.x == 0u) sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// X taken apart, contracted over its columns [rows][columns] and over its rows [columns][rows]. A wave takes up to `each` steps of a block of 32.
+struct OrthogonalPackParams {
+    uint32_t matrices, R, C, sum_blocks, each_c, each_r, blocks_row, blocks_column;      // blocks_..: of 256 threads, per matrix
+    uint64_t sr, sc;                                                                     // element strides of row and column
+    float eps; int32_t scale;
+};
+extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, u32x4* __restrict__ by_column, const float* __restrict__ x, const float* __restrict__ sums, OrthogonalPackParams P) {
+    __shared__ float part[4];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t per = P.blocks_row + P.blocks_column, matrix = blockIdx.x / per, block = blockIdx.x - matrix * per;
+    float t = 0.f;
+    for (uint32_t k = threadIdx.x; k < P.sum_blocks; k += 256u) t += sums[(uint64_t)matrix * P.sum_blocks + k];
+    wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
+    if (lane == 0u) part[wave] = t;
+    __syncthreads();
+    const float norm = __builtin_sqrtf((part[0] + part[1]) + (part[2] + part[3])) + P.eps, up = power_of_two(P.scale);
+    const bool rows = block < P.blocks_row;
+    const uint32_t I = rows ? P.R : P.C, K = rows ? P.C : P.R, steps = 2u * ((K + 31u) / 32u), each = rows ? P.each_c : P.each_r;
+    const uint64_t si = rows ? P.sr : P.sc, sk = rows ? P.sc : P.sr;
+    const uint32_t groups = (steps + each - 1u) / each, all = (rows ? block : block - P.blocks_row) * 4u + wave, blocks32 = (I + 31u) / 32u;
+    const bool along_k = sk == 1u;
+    const uint32_t rb = along_k ? all / groups : all % blocks32, group = along_k ? all % groups : all / blocks32;
+    if (rb >= blocks32 || group >= groups) return;
+    const uint32_t i = rb * 32u + (lane & 31u), h4 = 4u * (lane >> 5);
+    const float* const from = x + (uint64_t)matrix * P.R * P.C + (uint64_t)min(i, I - 1u) * si;
+    u32x4* const to = (rows ? by_row : by_column) + ((uint64_t)matrix * blocks32 + rb) * steps * 128u + lane;
+    for (uint32_t s = group * each; s < min(steps, (group + 1u) * each); ++s) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const uint32_t k = s * 16u + h4 + 8u * (q >> 2) + (q & 3);
+            v[q] = i < I && k < K ? from[(uint64_t)k * sk] / norm * up : 0.f;
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[2 * q], v[2 * q + 1], a, b); hi[q] = a; lo[q] = b; }
+        to[s * 128u] = hi; to[s * 128u + 64u] = lo;
+    }
+}
+
+// What a launch of products computes
+enum OrthogonalKind : uint32_t { SQUARE = 0, POLYNOMIAL = 1, NEXT = 2, LAST = 3 };
+struct OrthogonalParams {
+    uint32_t kind, M, N, K, tiles_m, tiles_n, tiles;     // tiles of a matrix: those on and above the diagonal of a square
+    int32_t scale_a, scale_b, scale_out;
+    float a, b, c; uint32_t pad;
+    uint64_t sr, sc;                                     // the last result's element strides
+};
+// (kinds in templates: their epilogues share no registers)
+template <uint32_t KIND>
+__device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u32x4* __restrict__ by_row, float* __restrict__ out, const u32x4* __restrict__ a, const u32x4* __restrict__ b,
+                                                const float* __restrict__ square, const OrthogonalParams& P) {
+    __shared__ HalfShared shared;
+    constexpr bool SYMMETRIC = KIND == SQUARE || KIND == POLYNOMIAL;
+    const uint32_t per = gridDim.x / 8u, id = per > 0u && blockIdx.x < per * 8u ? (blockIdx.x & 7u) * per + (blockIdx.x >> 3) : blockIdx.x;
+    const uint32_t matrix = id / P.tiles, at = id - matrix * P.tiles;
+    uint32_t m, n;
+    if constexpr (SYMMETRIC) {
+        // column by column of the triangle: n (n + 1) / 2 tiles in front of column n
+        n = (uint32_t)((__builtin_sqrtf(8.f * (float)at + 1.f) - 1.f) * 0.5f);
+        while ((n + 1u) * (n + 2u) / 2u <= at) ++n;
+        while (n * (n + 1u) / 2u > at) --n;
+        m = at - n * (n + 1u) / 2u;
+    } else {
+        const uint32_t strip = at / (8u * P.tiles_m), width = min(8u, P.tiles_n - 8u * strip), rest = at - strip * 8u * P.tiles_m;
+        m = rest / width; n = 8u * strip + rest - m * width;
+    }
+    const uint32_t steps_k = 2u * ((P.K + 31u) / 32u), blocks_m = (P.M + 31u) / 32u, blocks_n = (P.N + 31u) / 32u, steps_m = 2u * blocks_m, steps_n = 2u * blocks_n;
+    HalfSums acc = {};
+    half_product(acc, shared.stages, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u}, HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u},
+                 m, n, 0u, steps_k / 2u);
+    const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
+    const uint32_t row0 = m * 128u, column0 = n * 128u;
+    const uint64_t each = (uint64_t)matrix * P.M * P.N;
+    auto sum = [&](int i, int j, int k) { return __builtin_fmaf(acc.small[i][j][k], 1.f / HALF_REST, acc.large[i][j][k]) * down; };
+    if constexpr (KIND == LAST) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t row = row0 + (wave >> 1) * 64u + 32u * i + 8u * (k >> 2) + 4u * (lane >> 5) + (k & 3), column = column0 + (wave & 1u) * 64u + 32u * j + (lane & 31u);
+                    if (row < P.M && column < P.N) out[each + row * P.sr + column * P.sc] = sum(i, j, k);
+                }
+        return;
+    }
+    const HalfTarget columns{by_column ? by_column + (uint64_t)matrix * blocks_n * steps_m * 128u : nullptr, blocks_n, steps_m, n * 4u, m * 8u};
+    // (a tile on the diagonal of a square is its own mirror image)
+    const HalfTarget rows{by_row && !(SYMMETRIC && m == n) ? by_row + (uint64_t)matrix * blocks_m * steps_n * 128u : nullptr, blocks_m, steps_n, m * 4u, n * 8u};
+    half_store(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {
+        row += row0; column += column0;
+        if (row >= P.M || column >= P.N) return 0.f;
+        float v = sum(i, j, k);
+        if constexpr (KIND == SQUARE) out[each + (uint64_t)row * P.N + column] = v;
+        if constexpr (KIND == POLYNOMIAL) v = __builtin_fmaf(P.c, v, __builtin_fmaf(P.b, square[each + (uint64_t)row * P.N + column], row == column ? P.a : 0.f));
+        return v * up;
+    });
+}
+#define ORTHOGONAL(NAME, KIND)                                                                                                                                        \
+    extern "C" __global__ __launch_bounds__(256, 2) void orthogonal_##NAME(u32x4* by_column, u32x4* by_row, float* out, const u32x4* a, const u32x4* b, const float* square, \
+                                                                           OrthogonalParams P) {                                                                      \
+        orthogonal_body<KIND>(by_column, by_row, out, a, b, square, P);                                                                                               \
+    }
+ORTHOGONAL(square, SQUARE)
+ORTHOGONAL(polynomial, POLYNOMIAL)
+ORTHOGONAL(next, NEXT)
+ORTHOGONAL(last, LAST)

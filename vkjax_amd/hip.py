@@ -20,7 +20,7 @@ LIBDIR  = os.path.join(_PKG, 'lib')
 LIBPATH = os.path.join(LIBDIR, 'libvkjax_hip.so')
 
 KERNEL_MODULES = ('elementwise', 'rows', 'conv_gemm', 'wgrad_gemm', 'reduce', 'index', 'threefry', 'norm', 'log_probs', 'recurrence',
-                  'causal_conv', 'selective_scan', 'linear_log_probs')
+                  'causal_conv', 'selective_scan', 'linear_log_probs', 'orthogonalize')
 
 EVAL_SKIP_UPLOADS   = 1
 EVAL_SKIP_DOWNLOADS = 2

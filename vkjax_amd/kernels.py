@@ -7,6 +7,7 @@ block of one kernel (a struct of 32-bit fields that follows the pointer argument
 `struct ...Params` in vkjax_amd/csrc/kernels/*.hip) and picks grid, block and kernel variant.
 '''
 import contextlib
+import math
 import os
 import re
 import typing as tp
@@ -2828,4 +2829,66 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
     if pieces * slices > 1:
         launches.append(Launch('linear_sum', (_cdiv(rows * h, 4 * BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (parts, 0)], _u32(pieces * slices, 0) + _u64(rows * h),
                                bytes_moved=4 * (parts.size + rows * h)))
+    return launches
+
+
+# ---------------------------------------------------------------- orthogonalised matrices (orthogonalize.hip)
+
+ORTHOGONAL_LARGEST = 2.0**20            #of singular values, and of the polynomials' values, beyond which a polynomial is refused
+
+
+def orthogonal_bounds(steps: int, coefficients) -> tp.List[tp.Tuple[float, float]]:
+    '''For every step how large a singular value can be that it starts from, and the polynomial a + b s^2 + c s^4 of one: from the values of 4097 of them between 0 and 1, with a
+    quarter more for what lies between those and for roundings.'''
+    a, b, c = (float(v) for v in coefficients)
+    s, found = np.linspace(0.0, 1.0, 4097), []
+    with np.errstate(all='ignore'):
+        for _ in range(steps):
+            p = a + b * s**2 + c * s**4
+            found.append((1.25 * float(np.abs(s).max()), max(1.25 * float(np.abs(p).max()), abs(a))))
+            s = p * s
+    return found
+
+
+def _half_scale(largest: float) -> int:
+    '''The power of two that brings numbers up to `largest` below 2^15.'''
+    return 15 - int(math.frexp(largest)[1])
+
+
+def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, scratch) -> tp.List[Launch]:
+    rows, columns = x.shape[-2:]
+    n    = x.size // (rows * columns)
+    tall = rows > columns
+    r, c = (columns, rows) if tall else (rows, columns)
+    sr, sc = (1, columns) if tall else (columns, 1)                                         #element strides of the wide way round
+    if max(r, c) >= 2**20 or n * _cdiv(r, HALF_TILE) * _cdiv(c, HALF_TILE) >= 2**22 or n * (_cdiv(r, 32) * _half_steps(c) + _cdiv(c, 32) * _half_steps(r)) >= 2**28:
+        raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
+    sum_blocks = max(1, min(256, _cdiv(r * c, 4096)))
+    sums     = scratch((n, sum_blocks))
+    by_row   = scratch((n * _half_words(r, c),), np.uint32)
+    by_column = [scratch((n * _half_words(c, r),), np.uint32) for _ in range(2 if steps > 1 else 1)]
+    square, square_parts, polynomial = scratch((n, r, r)), scratch((n * _half_words(r, r),), np.uint32), scratch((n * _half_words(r, r),), np.uint32)
+    bounds   = orthogonal_bounds(steps, coefficients)
+    each     = [min(_half_steps(k), 8) for k in (c, r)]
+    blocks   = [_cdiv(_cdiv(i, 32) * _cdiv(_half_steps(k), e), 4) for i, k, e in ((r, c, each[0]), (c, r, each[1]))]
+    launches = [Launch('orthogonal_squares', (n * sum_blocks, 1, 1), (BLOCK, 1, 1), [(sums, 0), (x, 0)], _u32(sum_blocks, 0) + _u64(r * c), bytes_moved=4 * x.size),
+                Launch('orthogonal_pack', (n * sum(blocks), 1, 1), (BLOCK, 1, 1), [(by_row, 0), (by_column[0], 0), (x, 0), (sums, 0)],
+                       _u32(n, r, c, sum_blocks, *each, *blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])), bytes_moved=16 * x.size, written=(0, 1))]
+
+    def product(name, results, a, b, square, m, width, k, tiles, scales, written):
+        tiles_m, tiles_n = _cdiv(m, HALF_TILE), _cdiv(width, HALF_TILE)
+        kind = ('square', 'polynomial', 'next', 'last').index(name)
+        return Launch(f'orthogonal_{name}', (n * tiles, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, a, b, square)],
+                      _u32(kind, m, width, k, tiles_m, tiles_n, tiles) + _i32(*scales) + np.asarray(coefficients, np.float32).tobytes() + _u32(0) + _u64(sr, sc),
+                      bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=2 * n * m * width * k * (1 if tiles == tiles_m * tiles_n else tiles / (tiles_m * tiles_n)), written=written)
+    t = _cdiv(r, HALF_TILE)
+    triangle, all_tiles = t * (t + 1) // 2, t * _cdiv(c, HALF_TILE)
+    for i, (s, p) in enumerate(bounds):
+        scale_x, scale_a, scale_p = _half_scale(s), _half_scale(s * s), _half_scale(p)
+        launches += [product('square', (square_parts, square_parts, square), by_row, by_row, None, r, r, c, triangle, (scale_x, scale_x, scale_a), (0, 1, 2)),
+                     product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, triangle, (scale_a, scale_a, scale_p), (0, 1))]
+        last = i == steps - 1
+        scale_next = 0 if last else _half_scale(bounds[i + 1][0])
+        launches.append(product('last' if last else 'next', (None, None, out) if last else (by_column[(i + 1) & 1], by_row, None), polynomial, by_column[i & 1], None, r, c, r, all_tiles,
+                                (scale_p, scale_x, scale_next), (2,) if last else (0, 1)))
     return launches

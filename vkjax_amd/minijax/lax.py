@@ -818,6 +818,31 @@ def linear_log_probs_grad(x, weights, tokens, peaks, totals, g_log_probs=None, g
                       dict(transposed=bool(transposed), has_log_probs=g_log_probs is not None, has_log_sums=g_log_sums is not None), multiple_results=True))
 
 
+ORTHOGONALIZE_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+ORTHOGONALIZE_MAX_STEPS    = 32
+
+
+def orthogonalize(x, steps: int = 5, coefficients=ORTHOGONALIZE_COEFFICIENTS, eps: float = 1e-7):
+    '''For every matrix of x [..., rows, columns]: X = x / (|x| + eps) with its Frobenius norm, then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X, which turns every
+    singular value s into a s + b s^3 + c s^5.'''
+    from .. import kernels
+    x  = _f32_operand(x, 'orthogonalize')
+    xs = _shape(x)
+    if len(xs) < 2:
+        raise TypeError(f'orthogonalize takes matrices [..., rows, columns], got {xs}')
+    if int(steps) != steps or not 1 <= steps <= ORTHOGONALIZE_MAX_STEPS:
+        raise ValueError(f'orthogonalize: between 1 and {ORTHOGONALIZE_MAX_STEPS} steps are supported, got {steps}')
+    coefficients = tuple(float(np.float32(v)) for v in coefficients)
+    if len(coefficients) != 3 or not np.all(np.isfinite(coefficients)):
+        raise ValueError(f'orthogonalize: three finite coefficients are needed, got {coefficients}')
+    if not (0.0 < float(np.float32(eps)) < np.inf):
+        raise ValueError(f'orthogonalize: eps must be positive and finite, got {eps}')
+    for s, p in kernels.orthogonal_bounds(int(steps), coefficients):
+        if not builtins.max(s, s * s, p) < kernels.ORTHOGONAL_LARGEST:
+            raise ValueError(f'orthogonalize: with the coefficients {coefficients} singular values do not stay small over {steps} steps')
+    return emit('orthogonalize', [x], [_aval(xs, _f32)], dict(steps=int(steps), coefficients=coefficients, eps=float(eps)))
+
+
 # ---------------------------------------------------------------- rng
 
 def threefry2x32(key0, key1, x0, x1):

@@ -1254,6 +1254,13 @@ def linear_log_probs_grad(bufferpool, equation):
     return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch))
 
 
+def orthogonalize(bufferpool, equation):
+    p = equation.params
+    (x,), (out,), scratch = _operator_buffers(bufferpool, equation)
+    _float_operands(equation, x)
+    return _operator_ops(equation, K.orthogonalize(out, x, p['steps'], p['coefficients'], p['eps'], scratch))
+
+
 # ------------------------------------------------------------------ rng
 
 def threefry2x32(bufferpool, equation):
