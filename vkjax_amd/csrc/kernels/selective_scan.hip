@@ -435,7 +435,8 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             float own_dt[at.OWN], own_x[at.OWN], own_gy[at.OWN], slope[at.OWN], dgs[at.OWN];
 #pragma unroll
             for (int q = 0; q < at.OWN; ++q) {
-                const bool taken = t0 + at.own(q) < at.stop;
+                // (lanes behind the last channel have no part in the sums over channels)
+                const bool taken = t0 + at.own(q) < at.stop && at.there;
                 const float v = rd[q] + add, gv = taken ? rg[q] : 0.f, z = gate ? rz[q] : 0.f, open = gate ? sigmoid(z) : 1.f;
                 own_dt[q] = taken ? (P.softplus ? softplus_of(v) : v) : 0.f;
                 own_x[q]  = taken ? rx[q] : 0.f;
@@ -468,7 +469,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 for (int i = 0; i < NS; ++i) {
                     before[s][i] = h[i];
                     h[i] = __builtin_fmaf(exp2_of(a2[i] * dt[s]), h[i], u * bs[i]);
-                    part[i] = at.there ? gy[s] * h[i] : 0.f;
+                    part[i] = gy[s] * h[i];
                     seen = __builtin_fmaf(cs[i], h[i], seen);
                 }
                 if (gate) parts[at.wave][0][s][at.lane] = seen;
@@ -489,7 +490,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 for (int i = 0; i < NS; ++i) {
                     l[i] = __builtin_fmaf(gy[s], cs[i], l[i]);
                     lb = __builtin_fmaf(l[i], bs[i], lb);
-                    part[i] = at.there ? l[i] * u : 0.f;
+                    part[i] = l[i] * u;
                     l[i] *= exp2_of(a2[i] * dt[s]);
                     const float e = l[i] * before[s][i];
                     ea = __builtin_fmaf(e, a2[i], ea);
@@ -575,9 +576,9 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
         scan_grad_body<NS, M>(dx, ddelta, dgate, maps, channel_sums, x, delta, a, bmap, cmap, through, gate, lengths, bias, kept, g, g_last, adjoints, P);                         \
     }
 SELECTIVE_SCAN(4, 1)
-SELECTIVE_SCAN(8, 1)
-SELECTIVE_SCAN(8, 2)
-SELECTIVE_SCAN(8, 4)
+SELECTIVE_SCAN(4, 2)
+SELECTIVE_SCAN(4, 4)
+SELECTIVE_SCAN(4, 8)
 SELECTIVE_SCAN(8, 8)
 
 // What blocks have found, added up in their order: [strips][B T][2 N] to db and dc [B T, N], and [rows][N + 2][C] to dA [C, N], dD and dbias [C]. The first `map_blocks`

@@ -2627,7 +2627,7 @@ def causal_conv_grad(dx, dkernel, dbias, dstate, x: Buffer, kernel: Buffer, bias
 SELECTIVE_SCAN_KEPT       = 8           #steps between two states that a gradient's forward pass keeps
 SELECTIVE_SCAN_MAX_STATES = 64
 #waves that fill the machine; time is cut into chunks where there are fewer, of at least so many steps
-SELECTIVE_SCAN_WAVES, SELECTIVE_SCAN_CHUNK = 2048, 64
+SELECTIVE_SCAN_WAVES, SELECTIVE_SCAN_CHUNK = 4096, 64
 
 
 class ScanTiling(tp.NamedTuple):
@@ -2639,7 +2639,7 @@ class ScanTiling(tp.NamedTuple):
 
 
 def selective_scan_tiling(batch: int, time: int, channels: int, n: int) -> ScanTiling:
-    states = 4 if n <= 4 else 8
+    states = 4 if n <= 32 else 8
     waves  = _pow2_at_least(_cdiv(n, states))
     strips = _cdiv(channels, 64)
     chunks = max(1, min(_cdiv(SELECTIVE_SCAN_WAVES, batch * strips * waves), time // SELECTIVE_SCAN_CHUNK))
