@@ -35,86 +35,212 @@ __device__ __forceinline__ int half_scale(float largest) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)(127 + e) << 23); }          // (-126 <= e <= 127)
 
-// ---- the product of a tile of 128 x 128: four waves, 64 x 64 each. A pair of steps (32 k) of both operands, 32 KB, goes straight from memory into one of two buffers in shared
-// memory while the waves work on the other one; two blocks to a CU.
-constexpr int HALF_TILE = 128;
-typedef u32x4 HalfStage[2][4][2][2][64];                 // [operand][block of 32 rows][step][hi, lo][lane]
+// ---- the product of a tile: four waves, two by two, of T x T blocks of 32 x 32 each. Pairs of steps (32 k) of both operands go straight from memory into one of STAGES buffers in
+// shared memory while the waves work on another one.
+//   T = 2, STAGES = 2   tiles of 128, 64 KB, two blocks to a CU: for what fills the machine. 8192^3 378 TFLOP/s of fp32 products (an fp32 library product 153, an fp16 one a third of 1143)
+//   T = 2, STAGES = 4   the same with a block to a CU, whose three pairs on their way take the place of the other block: where there are no more tiles than CUs
+//   T = 1, STAGES = 4   tiles of 64, 64 KB: where tiles of 128 would be few
+// Few tiles, or those left behind whole rounds of the machine, share a tile's contraction among `slices` blocks: they leave their sums in memory, and the one that arrives last adds them
+// in the order of the slices. Nobody waits for another block.
+template <int T> struct HalfTileOf {
+    static constexpr int SIDE = 64 * T;
+    typedef u32x4 Stage[2][2 * T][2][2][64];             // [operand][block of 32 rows][step][hi, lo][lane]
+    static constexpr uint32_t PITCH = SIDE + 4;          // words of a row of results in shared memory: lanes that read vectors of neighbouring rows meet no bank twice
+    typedef uint32_t Turned[SIDE][PITCH];
+};
+template <int T, int STAGES> union HalfShared { typename HalfTileOf<T>::Stage stages[STAGES]; typename HalfTileOf<T>::Turned turned; uint32_t arrived; };
 
 struct HalfOperand {
     const u32x4* parts;
     uint32_t blocks, stride, first;                      // blocks of 32 rows, steps of 16 k per block, and the step at which the contraction starts (even)
 };
 
-struct HalfSums { f32x16 large[2][2], small[2][2]; };    // of a wave's 2 x 2 blocks of 32 x 32: hi.hi, and the others times 2^11
+template <int T> struct HalfSums { f32x16 large[T][T], small[T][T]; };      // of a wave's blocks of 32 x 32: hi.hi, and the others times 2^11
 
-__device__ __forceinline__ void half_request(HalfStage& to, const HalfOperand& a, const HalfOperand& b, uint32_t block_a, uint32_t block_b, uint32_t step) {
+template <int T>
+__device__ __forceinline__ void half_request(typename HalfTileOf<T>::Stage& to, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t step) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    // a wave brings a block of 32 rows of either operand (behind the last one, that one again: its results are nobody's)
-    const u32x4* const from_a = a.parts + ((uint64_t)min(block_a + wave, a.blocks - 1u) * a.stride + a.first + step) * 128u + lane;
-    const u32x4* const from_b = b.parts + ((uint64_t)min(block_b + wave, b.blocks - 1u) * b.stride + b.first + step) * 128u + lane;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_a + 64 * q), (__attribute__((address_space(3))) void*)&to[0][wave][q >> 1][q & 1][0], 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from_b + 64 * q), (__attribute__((address_space(3))) void*)&to[1][wave][q >> 1][q & 1][0], 16, 0, 0);
+    for (uint32_t u = 0; u < T; ++u) {
+        // a block of 32 rows of either operand (behind the last one, that one again: its results are nobody's)
+        const uint32_t unit = wave * T + u, of_b = unit / (2u * T), block = unit % (2u * T);
+        const HalfOperand& o = of_b ? b : a;
+        const u32x4* const from = o.parts + ((uint64_t)min((of_b ? n : m) * (2u * T) + block, o.blocks - 1u) * o.stride + o.first + step) * 128u + lane;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + 64 * q), (__attribute__((address_space(3))) void*)&to[of_b][block][q >> 1][q & 1][0], 16, 0, 0);
     }
 }
-__device__ __forceinline__ void half_multiply(HalfSums& sums, const HalfStage& from) {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
+// What a wave needs of a step of 16 k: its blocks' parts
+template <int T> struct HalfStep {
+    f16x8 a[T][2], b[T][2];
+    __device__ __forceinline__ void read(const typename HalfTileOf<T>::Stage& from, int s) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        f16x8 a[2][2], b[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                a[i][t] = __builtin_bit_cast(f16x8, from[0][2 * wm + i][s][t][lane]);
-                b[i][t] = __builtin_bit_cast(f16x8, from[1][2 * wn + i][s][t][lane]);
+                a[i][t] = __builtin_bit_cast(f16x8, from[0][T * wm + i][s][t][lane]);
+                b[i][t] = __builtin_bit_cast(f16x8, from[1][T * wn + i][s][t][lane]);
             }
+    }
+    __device__ __forceinline__ void multiply(HalfSums<T>& sums) const {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < T; ++j) {
                 sums.small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][1], sums.small[i][j], 0, 0, 0);
                 sums.large[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], sums.large[i][j], 0, 0, 0);
                 sums.small[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][1], b[j][0], sums.small[i][j], 0, 0, 0);
             }
     }
-}
-// The sums of tile (m, n) over `pairs` pairs of steps from pair `begin` on
-__device__ __forceinline__ void half_product(HalfSums& sums, HalfStage (&stages)[2], const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs) {
-    half_request(stages[0], a, b, 4u * m, 4u * n, 2u * begin);
-    __syncthreads();
-    for (uint32_t p = 0; p < pairs; ++p) {
-        if (p + 1u < pairs) half_request(stages[(p + 1u) & 1u], a, b, 4u * m, 4u * n, 2u * (begin + p + 1u));
-        half_multiply(sums, stages[p & 1u]);
-        __syncthreads();
+};
+// All but the last N loads of this wave have arrived (lgkmcnt and expcnt as they are)
+template <int N> __device__ __forceinline__ void loads_left() { __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 15 << 8 | (N >> 4) << 14); }
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); asm volatile("" ::: "memory"); }
+#define HALF_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// The sums of tile (m, n) over `pairs` pairs of steps (one at least) from pair `begin` on. With more than two buffers a wave has the parts of the next step in registers before it
+// multiplies those of this one: the barrier in front of a pair stands between the two steps of the pair before.
+template <int T, int STAGES>
+__device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs) {
+    static_assert(STAGES == 2 || STAGES == 4, "as many pairs are on their way as meet() counts");
+    constexpr int LOADS = 4 * T;                         // of a wave per stage
+    uint32_t asked = 0u;                                 // pairs that have been requested
+    auto request = [&](uint32_t at) { half_request<T>(shared.stages[at], a, b, m, n, 2u * (begin + asked)); ++asked; };
+    // pair p has arrived, for all waves (those asked for behind it may be on their way); and all have read what they wanted of the pair before the last
+    auto meet = [&](uint32_t p) {
+        const uint32_t behind = asked - 1u - p;
+        if (STAGES > 2 && behind >= 2u) loads_left<2 * LOADS>(); else if (STAGES > 2 && behind == 1u) loads_left<LOADS>(); else loads_left<0>();
+        in_order();
+        __builtin_amdgcn_s_barrier();
+        in_order();
+    };
+#pragma unroll
+    for (uint32_t p = 0; p < STAGES - 1; ++p)
+        if (p < pairs) request(p);
+    uint32_t at = 0u;
+    if constexpr (STAGES == 2) {
+        for (uint32_t p = 0; p < pairs; ++p) {
+            meet(p);
+            if (asked < pairs) request(at ^ 1u);
+            HalfStep<T> step;
+            step.read(shared.stages[at], 0);
+            step.multiply(sums);
+            step.read(shared.stages[at], 1);
+            step.multiply(sums);
+            at ^= 1u;
+        }
+    } else {
+        HalfStep<T> first, second;
+        meet(0u);
+        if (asked < pairs) request(STAGES - 1u);
+        first.read(shared.stages[0], 0);
+        for (uint32_t p = 0; p < pairs; ++p) {
+            second.read(shared.stages[at], 1);
+            HALF_FENCE();
+            first.multiply(sums);
+            HALF_FENCE();
+            const uint32_t next = at + 1u == STAGES ? 0u : at + 1u;
+            if (p + 1u < pairs) {
+                meet(p + 1u);
+                // (in the place of pair p - 1; reads of pair p may still be on their way)
+                if (p > 0u && asked < pairs) request(at == 0u ? STAGES - 1u : at - 1u);
+                first.read(shared.stages[next], 0);
+            }
+            HALF_FENCE();
+            second.multiply(sums);
+            HALF_FENCE();
+            at = next;
+        }
     }
+    __syncthreads();
 }
-// Consecutive blocks go to the 8 XCDs in turn; each works through a contiguous range of the tiles, in strips of 8 columns of tiles, row by row of a strip, so that the blocks of an
-// XCD that run together share rows and columns in its L2.
-__device__ __forceinline__ void half_tile_of(uint32_t block, uint32_t blocks, uint32_t tiles_m, uint32_t tiles_n, uint32_t& m, uint32_t& n) {
-    const uint32_t per = blocks / 8u, id = per > 0u && block < per * 8u ? (block & 7u) * per + (block >> 3) : block;
+
+// Consecutive blocks go to the 8 XCDs in turn; each works through a contiguous range of the numbers
+__device__ __forceinline__ uint32_t half_turn(uint32_t block, uint32_t blocks) {
+    const uint32_t per = blocks / 8u;
+    return per > 0u && block < per * 8u ? (block & 7u) * per + (block >> 3) : block;
+}
+// What a block of a launch does: the first `whole` tiles by a block each, the contraction of every one behind them by `slices` blocks
+struct HalfShares { uint32_t whole, slices; };
+__device__ __forceinline__ void half_work(uint32_t block, const HalfShares& P, uint32_t pairs, uint32_t& tile, uint32_t& slice, uint32_t& begin, uint32_t& end) {
+    tile = half_turn(block, P.whole); slice = 0u; begin = 0u; end = pairs;
+    if (block < P.whole) return;
+    const uint32_t rest = half_turn(block - P.whole, gridDim.x - P.whole);
+    tile = P.whole + rest / P.slices; slice = rest % P.slices;
+    begin = (uint32_t)((uint64_t)pairs * slice / P.slices); end = (uint32_t)((uint64_t)pairs * (slice + 1u) / P.slices);
+}
+// The sums of a tile behind the whole ones: true in the block that has all of them (in `large`, both kinds)
+template <int T, int STAGES>
+__device__ __forceinline__ bool half_join(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, float* partial, uint32_t* arrivals, uint32_t tile, uint32_t slice, const HalfShares& P) {
+    if (tile < P.whole || P.slices == 1u) return true;
+    constexpr uint32_t BYTES = HalfTileOf<T>::SIDE * HalfTileOf<T>::SIDE * 4u;
+    const uint32_t mine = tile - P.whole, tid = threadIdx.x;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(reinterpret_cast<char*>(partial) + (uint64_t)mine * P.slices * BYTES, P.slices * BYTES);
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(sums.small[i][j][4 * q + e], 1.f / HALF_REST, sums.large[i][j][4 * q + e]);
+                // (past the L2, which is not the other XCDs')
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, tid * 16u, slice * BYTES + (uint32_t)((i * T + j) * 4 + q) * 4096u, 16);
+            }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the stores have reached memory
+    __syncthreads();
+    if (tid == 0u) {
+        const uint32_t n = __hip_atomic_fetch_add(arrivals + mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (n + 1u == P.slices) __hip_atomic_store(arrivals + mine, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // (for the next launch)
+        shared.arrived = n;
+    }
+    __syncthreads();
+    const bool last = __builtin_amdgcn_readfirstlane(shared.arrived) + 1u == P.slices;
+    __syncthreads();
+    if (!last) return false;
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j) { sums.large[i][j] = f32x16{}; sums.small[i][j] = f32x16{}; }
+#pragma nounroll
+    for (uint32_t s = 0; s < P.slices; ++s)
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, tid * 16u, s * BYTES + (uint32_t)((i * T + j) * 4 + q) * 4096u, 16));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums.large[i][j][4 * q + e] += v[e];
+                }
+    return true;
+}
+// A result
+template <int T> __device__ __forceinline__ float half_sum(const HalfSums<T>& sums, int i, int j, int k) { return __builtin_fmaf(sums.small[i][j][k], 1.f / HALF_REST, sums.large[i][j][k]); }
+
+// Tiles in strips of 8 columns of tiles, row by row of a strip, so that blocks that run together share rows and columns in an XCD's L2
+__device__ __forceinline__ void half_tile(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t& m, uint32_t& n) {
     const uint32_t strip = id / (8u * tiles_m), width = min(8u, tiles_n - 8u * strip), at = id - strip * 8u * tiles_m;
     m = at / width; n = 8u * strip + at - m * width;
 }
 
 // ---- a tile of a result as an operand of products that follow: contracted over its rows, as the lanes have it (`by_column`: its index is the column), or over its columns (`by_row`),
 // turned in shared memory. value(block of rows i, of columns j, register, row, column) is what is taken apart, scaled; it is zero behind the result's last row and column.
-constexpr uint32_t HALF_PITCH = 132u;                    // words of a row in shared memory: lanes that read vectors of neighbouring rows meet no bank twice
-typedef uint32_t HalfTurned[HALF_TILE][HALF_PITCH];
-union HalfShared { HalfStage stages[2]; HalfTurned turned; };
-
 struct HalfTarget { u32x4* parts; uint32_t blocks, steps, block, step; };      // blocks of 32 of its index, steps of 16 k per block (all of them); where this tile's begin
 
-template <class F>
-__device__ __forceinline__ void half_store(HalfTurned& turned, const HalfTarget& by_column, const HalfTarget& by_row, F value) {
+template <int T, class F>
+__device__ __forceinline__ void half_store(typename HalfTileOf<T>::Turned& turned, const HalfTarget& by_column, const HalfTarget& by_row, F value) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t column = wn * 64u + 32u * j + (lane & 31u), block = by_column.block + wn * 2u + j;
+    for (int j = 0; j < T; ++j) {
+        const uint32_t column = (wn * T + j) * 32u + (lane & 31u), block = by_column.block + wn * T + j;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t row0 = wm * 64u + 32u * i + 4u * (lane >> 5);
+        for (int i = 0; i < T; ++i) {
+            const uint32_t row0 = (wm * T + i) * 32u + 4u * (lane >> 5);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -124,7 +250,7 @@ __device__ __forceinline__ void half_store(HalfTurned& turned, const HalfTarget&
             if (by_column.parts && block < by_column.blocks)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const uint32_t step = by_column.step + wm * 4u + 2u * i + s;
+                    const uint32_t step = by_column.step + (wm * T + i) * 2u + s;
                     if (step < by_column.steps) {
                         u32x4* const to = by_column.parts + ((uint64_t)block * by_column.steps + step) * 128u + lane;
                         to[0]  = u32x4{hi[4 * s], hi[4 * s + 1], hi[4 * s + 2], hi[4 * s + 3]};
@@ -141,21 +267,20 @@ __device__ __forceinline__ void half_store(HalfTurned& turned, const HalfTarget&
     }
     if (!by_row.parts) return;
     __syncthreads();
-    // wave: a block of 32 rows, the tile's eight steps of 16 columns
-    const uint32_t block = by_row.block + wave;
-    const uint32_t* const row = &turned[wave * 32u + (lane & 31u)][0];
-    if (block >= by_row.blocks) return;
+    // of the tile's 2 T blocks of 32 rows with 4 T steps of 16 columns a quarter to a wave
 #pragma unroll
-    for (uint32_t s = 0; s < 8u; ++s) {
-        if (by_row.step + s >= by_row.steps) break;
+    for (uint32_t q = 0; q < 2u * T * T; ++q) {
+        const uint32_t item = wave * (2u * T * T) + q, rb = item / (4u * T), s = item % (4u * T);
+        if (by_row.step + s >= by_row.steps || by_row.block + rb >= by_row.blocks) continue;
+        const uint32_t* const row = &turned[rb * 32u + (lane & 31u)][0];
         u32x4 hi, lo;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16u * s + 8u * q + 4u * (lane >> 5));
-            hi[2 * q] = (t.x & 0xFFFFu) | t.y << 16; hi[2 * q + 1] = (t.z & 0xFFFFu) | t.w << 16;
-            lo[2 * q] = t.x >> 16 | (t.y & 0xFFFF0000u); lo[2 * q + 1] = t.z >> 16 | (t.w & 0xFFFF0000u);
+        for (int e = 0; e < 2; ++e) {
+            const u32x4 t = *reinterpret_cast<const u32x4*>(row + 16u * s + 8u * e + 4u * (lane >> 5));
+            hi[2 * e] = (t.x & 0xFFFFu) | t.y << 16; hi[2 * e + 1] = (t.z & 0xFFFFu) | t.w << 16;
+            lo[2 * e] = t.x >> 16 | (t.y & 0xFFFF0000u); lo[2 * e + 1] = t.z >> 16 | (t.w & 0xFFFF0000u);
         }
-        u32x4* const to = by_row.parts + ((uint64_t)block * by_row.steps + by_row.step + s) * 128u + lane;
+        u32x4* const to = by_row.parts + ((uint64_t)(by_row.block + rb) * by_row.steps + by_row.step + s) * 128u + lane;
         to[0] = hi; to[64] = lo;
     }
 }

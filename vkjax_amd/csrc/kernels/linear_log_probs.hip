@@ -143,14 +143,14 @@ __device__ __forceinline__ float over_halves_sum(float v) { return v + lane_xor<
 
 extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, const u32x4* __restrict__ w,
                                                                    const u32x4* __restrict__ x, const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, ScoresParams P) {
-    __shared__ HalfStage stages[2];
+    __shared__ HalfShared<2, 2> shared;
     uint32_t m, n;
-    half_tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, m, n);
-    HalfSums acc = {};
-    half_product(acc, stages, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, 0u, P.pairs);
+    half_tile(half_turn(blockIdx.x, gridDim.x), P.tiles_m, P.tiles_n, m, n);
+    HalfSums<2> acc = {};
+    half_product<2, 2>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, 0u, P.pairs);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]);
-    float (*const met)[128][2] = reinterpret_cast<float (*)[128][2]>(&stages[0]);           // [wm][column][peak, sum]
+    float (*const met)[128][2] = reinterpret_cast<float (*)[128][2]>(&shared.stages[0]);           // [wm][column][peak, sum]
     const uint32_t v0 = m * 128u + wm * 64u + 4u * (lane >> 5);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -163,7 +163,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __rest
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
                 const uint32_t v = v0 + 32u * i + 8u * (q >> 2) + (q & 3);
-                float s = __builtin_fmaf(acc.small[i][j][q], 1.f / HALF_REST, acc.large[i][j][q]) * down_w * down_x;
+                float s = half_sum(acc, i, j, q) * down_w * down_x;
                 if (v == (uint32_t)token) { mine = s; has = true; }
                 s = v < P.V ? s : -__builtin_inff();
                 acc.large[i][j][q] = s;
@@ -366,11 +366,11 @@ SCORES_ROWS(h_64, false, 2)
 extern "C" __global__ __launch_bounds__(256, 2) void linear_q(u32x4* __restrict__ by_row, u32x4* __restrict__ by_token, const u32x4* __restrict__ w, const u32x4* __restrict__ x,
                                                               const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, const float* __restrict__ row_peaks,
                                                               const float* __restrict__ row_totals, const float* __restrict__ factors, ScoresParams P) {
-    __shared__ HalfShared shared;
+    __shared__ HalfShared<2, 2> shared;
     uint32_t m, n;
-    half_tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, m, n);
-    HalfSums acc = {};
-    half_product(acc, shared.stages, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, 0u, P.pairs);
+    half_tile(half_turn(blockIdx.x, gridDim.x), P.tiles_m, P.tiles_n, m, n);
+    HalfSums<2> acc = {};
+    half_product<2, 2>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, 0u, P.pairs);
     const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]), up = power_of_two(Q_SCALE);
     const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * 128u;
     // of this lane's two columns
@@ -384,10 +384,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_q(u32x4* __restrict_
         token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
         peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
-    half_store(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 4u, m * 8u}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 4u, n * 8u},
+    half_store<2>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 4u, m * 8u}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 4u, n * 8u},
                [&](int i, int j, int k, uint32_t row, uint32_t) {
         const uint32_t v = v0 + row;
-        const float s = __builtin_fmaf(acc.small[i][j][k], 1.f / HALF_REST, acc.large[i][j][k]) * down_w * down_x;
+        const float s = half_sum(acc, i, j, k) * down_w * down_x;
         const float q = part[j] * exp_of(s - peak[j]) + (v == token[j] ? one[j] : 0.f);
         return given[j] && v < P.V ? q : 0.f;
     });
@@ -401,13 +401,13 @@ struct ProductParams {
 };
 extern "C" __global__ __launch_bounds__(256, 2) void linear_product(float* __restrict__ out, const u32x4* __restrict__ a, const u32x4* __restrict__ b, const int32_t* __restrict__ scales,
                                                                     const float* __restrict__ factors, ProductParams P) {
-    __shared__ HalfStage stages[2];
+    __shared__ HalfShared<2, 2> shared;
     uint32_t m, n;
     const uint32_t tiles = P.tiles_m * P.tiles_n, slice = blockIdx.x / tiles;
-    half_tile_of(blockIdx.x - slice * tiles, tiles, P.tiles_m, P.tiles_n, m, n);
+    half_tile(half_turn(blockIdx.x - slice * tiles, tiles), P.tiles_m, P.tiles_n, m, n);
     const uint32_t begin = (uint32_t)((uint64_t)P.pairs * slice / P.slices), end = (uint32_t)((uint64_t)P.pairs * (slice + 1u) / P.slices);
-    HalfSums acc = {};
-    half_product(acc, stages, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
+    HalfSums<2> acc = {};
+    half_product<2, 2>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const float down = power_of_two(-(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a])), down_b = power_of_two(-(P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]));
     float* const to = out + P.slice * slice;
@@ -422,7 +422,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_product(float* __res
             for (int j = 0; j < 2; ++j) {
                 const uint32_t column = n * 128u + wn * 64u + 32u * j + (lane & 31u);
                 if (column < P.N) {
-                    const float s = __builtin_fmaf(acc.small[i][j][q], 1.f / HALF_REST, acc.large[i][j][q]) * down * down_b;
+                    const float s = half_sum(acc, i, j, q) * down * down_b;
                     to[P.ld * row + column] = factors ? (f == 0.f ? 0.f : s * f) : s;
                 }
             }

@@ -72,67 +72,79 @@ enum OrthogonalKind : uint32_t { SQUARE = 0, POLYNOMIAL = 1, NEXT = 2, LAST = 3 
 struct OrthogonalParams {
     uint32_t kind, M, N, K, tiles_m, tiles_n, tiles;     // tiles of a matrix: those on and above the diagonal of a square
     int32_t scale_a, scale_b, scale_out;
-    float a, b, c; uint32_t pad;
+    float a, b, c; HalfShares shares; uint32_t pad;
     uint64_t sr, sc;                                     // the last result's element strides
 };
 // (kinds in templates: their epilogues share no registers)
-template <uint32_t KIND>
-__device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u32x4* __restrict__ by_row, float* __restrict__ out, const u32x4* __restrict__ a, const u32x4* __restrict__ b,
-                                                const float* __restrict__ square, const OrthogonalParams& P) {
-    __shared__ HalfShared shared;
+template <uint32_t KIND, int T, int STAGES>
+__device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u32x4* __restrict__ by_row, float* __restrict__ out, float* __restrict__ partial, uint32_t* __restrict__ arrivals,
+                                                const u32x4* __restrict__ a, const u32x4* __restrict__ b, const float* __restrict__ square, const OrthogonalParams& P) {
+    __shared__ HalfShared<T, STAGES> shared;
     constexpr bool SYMMETRIC = KIND == SQUARE || KIND == POLYNOMIAL;
-    const uint32_t per = gridDim.x / 8u, id = per > 0u && blockIdx.x < per * 8u ? (blockIdx.x & 7u) * per + (blockIdx.x >> 3) : blockIdx.x;
-    const uint32_t matrix = id / P.tiles, at = id - matrix * P.tiles;
-    uint32_t m, n;
+    constexpr uint32_t SIDE = 64u * T;
+    const uint32_t steps_k = 2u * ((P.K + 31u) / 32u), blocks_m = (P.M + 31u) / 32u, blocks_n = (P.N + 31u) / 32u, steps_m = 2u * blocks_m, steps_n = 2u * blocks_n;
+    uint32_t tile, slice, begin, end, m, n;
+    half_work(blockIdx.x, P.shares, steps_k / 2u, tile, slice, begin, end);
+    const uint32_t matrix = tile / P.tiles, at = tile - matrix * P.tiles;
     if constexpr (SYMMETRIC) {
         // column by column of the triangle: n (n + 1) / 2 tiles in front of column n
         n = (uint32_t)((__builtin_sqrtf(8.f * (float)at + 1.f) - 1.f) * 0.5f);
         while ((n + 1u) * (n + 2u) / 2u <= at) ++n;
         while (n * (n + 1u) / 2u > at) --n;
         m = at - n * (n + 1u) / 2u;
-    } else {
-        const uint32_t strip = at / (8u * P.tiles_m), width = min(8u, P.tiles_n - 8u * strip), rest = at - strip * 8u * P.tiles_m;
-        m = rest / width; n = 8u * strip + rest - m * width;
-    }
-    const uint32_t steps_k = 2u * ((P.K + 31u) / 32u), blocks_m = (P.M + 31u) / 32u, blocks_n = (P.N + 31u) / 32u, steps_m = 2u * blocks_m, steps_n = 2u * blocks_n;
-    HalfSums acc = {};
-    half_product(acc, shared.stages, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u}, HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u},
-                 m, n, 0u, steps_k / 2u);
+    } else half_tile(at, P.tiles_m, P.tiles_n, m, n);
+    HalfSums<T> acc = {};
+    half_product<T, STAGES>(acc, shared, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u},
+                            HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
+    if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
-    const uint32_t row0 = m * 128u, column0 = n * 128u;
+    const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t lane_row = row0 + (wave >> 1) * 32u * T + 4u * (lane >> 5), lane_column = column0 + (wave & 1u) * 32u * T + (lane & 31u);
     const uint64_t each = (uint64_t)matrix * P.M * P.N;
-    auto sum = [&](int i, int j, int k) { return __builtin_fmaf(acc.small[i][j][k], 1.f / HALF_REST, acc.large[i][j][k]) * down; };
     if constexpr (KIND == LAST) {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < T; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const uint32_t row = row0 + (wave >> 1) * 64u + 32u * i + 8u * (k >> 2) + 4u * (lane >> 5) + (k & 3), column = column0 + (wave & 1u) * 64u + 32u * j + (lane & 31u);
-                    if (row < P.M && column < P.N) out[each + row * P.sr + column * P.sc] = sum(i, j, k);
+                    const uint32_t row = lane_row + 32u * i + 8u * (k >> 2) + (k & 3), column = lane_column + 32u * j;
+                    if (row < P.M && column < P.N) out[each + row * P.sr + column * P.sc] = half_sum(acc, i, j, k) * down;
                 }
         return;
     }
-    const HalfTarget columns{by_column ? by_column + (uint64_t)matrix * blocks_n * steps_m * 128u : nullptr, blocks_n, steps_m, n * 4u, m * 8u};
+    // (all at once, in front of the stores)
+    f32x16 squares[T][T] = {};
+    if constexpr (KIND == POLYNOMIAL)
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t row = min(lane_row + 32u * i + 8u * (k >> 2) + (k & 3), P.M - 1u), column = min(lane_column + 32u * j, P.N - 1u);
+                    squares[i][j][k] = square[each + (uint64_t)row * P.N + column];
+                }
+    const HalfTarget columns{by_column + (uint64_t)matrix * blocks_n * steps_m * 128u, blocks_n, steps_m, n * 2u * T, m * 4u * T};
     // (a tile on the diagonal of a square is its own mirror image)
-    const HalfTarget rows{by_row && !(SYMMETRIC && m == n) ? by_row + (uint64_t)matrix * blocks_m * steps_n * 128u : nullptr, blocks_m, steps_n, m * 4u, n * 8u};
-    half_store(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {
+    const HalfTarget rows{SYMMETRIC && m == n ? nullptr : by_row + (uint64_t)matrix * blocks_m * steps_n * 128u, blocks_m, steps_n, m * 2u * T, n * 4u * T};
+    half_store<T>(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {
         row += row0; column += column0;
         if (row >= P.M || column >= P.N) return 0.f;
-        float v = sum(i, j, k);
+        float v = half_sum(acc, i, j, k) * down;
         if constexpr (KIND == SQUARE) out[each + (uint64_t)row * P.N + column] = v;
-        if constexpr (KIND == POLYNOMIAL) v = __builtin_fmaf(P.c, v, __builtin_fmaf(P.b, square[each + (uint64_t)row * P.N + column], row == column ? P.a : 0.f));
+        if constexpr (KIND == POLYNOMIAL) v = __builtin_fmaf(P.c, v, __builtin_fmaf(P.b, squares[i][j][k], row == column ? P.a : 0.f));
         return v * up;
     });
 }
-#define ORTHOGONAL(NAME, KIND)                                                                                                                                        \
-    extern "C" __global__ __launch_bounds__(256, 2) void orthogonal_##NAME(u32x4* by_column, u32x4* by_row, float* out, const u32x4* a, const u32x4* b, const float* square, \
-                                                                           OrthogonalParams P) {                                                                      \
-        orthogonal_body<KIND>(by_column, by_row, out, a, b, square, P);                                                                                               \
+#define ORTHOGONAL(NAME, KIND, SUFFIX, T, STAGES, BLOCKS)                                                                                                             \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void orthogonal_##NAME##SUFFIX(u32x4* by_column, u32x4* by_row, float* out, float* partial, uint32_t* arrivals, \
+                                                                                        const u32x4* a, const u32x4* b, const float* square, OrthogonalParams P) {    \
+        orthogonal_body<KIND, T, STAGES>(by_column, by_row, out, partial, arrivals, a, b, square, P);                                                                 \
     }
-ORTHOGONAL(square, SQUARE)
-ORTHOGONAL(polynomial, POLYNOMIAL)
-ORTHOGONAL(next, NEXT)
-ORTHOGONAL(last, LAST)
+#define ORTHOGONAL_KINDS(SUFFIX, T, STAGES, BLOCKS)                                                                                                                   \
+    ORTHOGONAL(square, SQUARE, SUFFIX, T, STAGES, BLOCKS) ORTHOGONAL(polynomial, POLYNOMIAL, SUFFIX, T, STAGES, BLOCKS) ORTHOGONAL(next, NEXT, SUFFIX, T, STAGES, BLOCKS) \
+    ORTHOGONAL(last, LAST, SUFFIX, T, STAGES, BLOCKS)
+ORTHOGONAL_KINDS(_128, 2, 2, 2)
+ORTHOGONAL_KINDS(_128_alone, 2, 4, 1)
+ORTHOGONAL_KINDS(_64, 1, 4, 2)

@@ -2855,13 +2855,51 @@ def _half_scale(largest: float) -> int:
     return 15 - int(math.frexp(largest)[1])
 
 
-def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, scratch) -> tp.List[Launch]:
+class HalfPlan(tp.NamedTuple):
+    '''How a product is shared out (half_product.h): tiles of `side`, the first `whole` of them by a block each, the contraction of those behind by `slices` blocks.'''
+    kernel: str
+    side:   int
+    whole:  int
+    slices: int
+
+
+def half_plan(tiles_of, pairs: int) -> HalfPlan:
+    '''The plan with the smallest estimated time (us) for tiles_of(side) tiles and a contraction of so many pairs of steps.'''
+    best = None
+    for kernel, side, blocks_of_cu, start, alone, together in HALF_KERNELS:
+        tiles = tiles_of(side)
+        for slices in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32):
+            if slices > max(1, pairs // HALF_SLICE_PAIRS):
+                break
+            slots = 256 * blocks_of_cu
+            whole = tiles if slices == 1 else tiles // slots * slots
+            if slices > 1 and whole == tiles:
+                continue
+            def rounds(blocks, pairs):
+                #full rounds of the machine, then one with fewer blocks to a CU
+                full, rest = divmod(blocks, slots)
+                return full * (start + pairs * together) + (0 if rest == 0 else start + pairs * (alone if rest <= 256 else together))
+            cost = rounds(whole, pairs) + (rounds((tiles - whole) * slices, _cdiv(pairs, slices)) + HALF_JOIN + HALF_JOIN_SLICE * slices * (side / 128)**2 if whole < tiles else 0)
+            if slices == 1:
+                cost = rounds(tiles, pairs)
+            if best is None or cost < best[0]:
+                best = (cost, HalfPlan(kernel, side, whole, slices))
+    return best[1]
+
+
+#kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps with a block to a CU, with several)
+HALF_KERNELS = (('_128', 128, 2, 6.0, 0.95, 1.42), ('_128_alone', 128, 1, 6.0, 0.75, 0.75), ('_64', 64, 2, 4.0, 0.33, 0.45))
+HALF_SLICE_PAIRS = 4                    #pairs of steps of a slice, at least
+HALF_JOIN, HALF_JOIN_SLICE = 3.0, 0.6   #us of adding up slices, and for each of them
+
+
+def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, scratch, zeroed) -> tp.List[Launch]:
     rows, columns = x.shape[-2:]
     n    = x.size // (rows * columns)
     tall = rows > columns
     r, c = (columns, rows) if tall else (rows, columns)
     sr, sc = (1, columns) if tall else (columns, 1)                                         #element strides of the wide way round
-    if max(r, c) >= 2**20 or n * _cdiv(r, HALF_TILE) * _cdiv(c, HALF_TILE) >= 2**22 or n * (_cdiv(r, 32) * _half_steps(c) + _cdiv(c, 32) * _half_steps(r)) >= 2**28:
+    if max(r, c) >= 2**20 or n * _cdiv(r, 64) * _cdiv(c, 64) >= 2**24 or n * (_cdiv(r, 32) * _half_steps(c) + _cdiv(c, 32) * _half_steps(r)) >= 2**28:
         raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
     sum_blocks = max(1, min(256, _cdiv(r * c, 4096)))
     sums     = scratch((n, sum_blocks))
@@ -2875,20 +2913,26 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
                 Launch('orthogonal_pack', (n * sum(blocks), 1, 1), (BLOCK, 1, 1), [(by_row, 0), (by_column[0], 0), (x, 0), (sums, 0)],
                        _u32(n, r, c, sum_blocks, *each, *blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])), bytes_moved=16 * x.size, written=(0, 1))]
 
-    def product(name, results, a, b, square, m, width, k, tiles, scales, written):
-        tiles_m, tiles_n = _cdiv(m, HALF_TILE), _cdiv(width, HALF_TILE)
-        kind = ('square', 'polynomial', 'next', 'last').index(name)
-        return Launch(f'orthogonal_{name}', (n * tiles, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, a, b, square)],
-                      _u32(kind, m, width, k, tiles_m, tiles_n, tiles) + _i32(*scales) + np.asarray(coefficients, np.float32).tobytes() + _u32(0) + _u64(sr, sc),
-                      bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=2 * n * m * width * k * (1 if tiles == tiles_m * tiles_n else tiles / (tiles_m * tiles_n)), written=written)
-    t = _cdiv(r, HALF_TILE)
-    triangle, all_tiles = t * (t + 1) // 2, t * _cdiv(c, HALF_TILE)
+    def product(name, results, a, b, square, m, width, k, scales, written):
+        symmetric = name in ('square', 'polynomial')
+        of_matrix = lambda side: _cdiv(m, side) * (_cdiv(m, side) + 1) // 2 if symmetric else _cdiv(m, side) * _cdiv(width, side)
+        plan  = half_plan(lambda side: n * of_matrix(side), _half_steps(k) // 2)
+        tiles = n * of_matrix(plan.side)
+        rest  = tiles - plan.whole
+        partial  = scratch((rest * plan.slices, plan.side, plan.side)) if plan.slices > 1 else None
+        arrivals = zeroed(rest, 'arrivals at tiles of halves') if plan.slices > 1 else None
+        launch = Launch(f'orthogonal_{name}{plan.kernel}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
+                        _u32(('square', 'polynomial', 'next', 'last').index(name), m, width, k, _cdiv(m, plan.side), _cdiv(width, plan.side), of_matrix(plan.side)) + _i32(*scales)
+                        + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, 0) + _u64(sr, sc),
+                        bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=(1 if symmetric else 2) * n * m * width * k,
+                        written=written + ((3, 4) if plan.slices > 1 else ()), scratch=(4,) if plan.slices > 1 else ())
+        return launch
     for i, (s, p) in enumerate(bounds):
         scale_x, scale_a, scale_p = _half_scale(s), _half_scale(s * s), _half_scale(p)
-        launches += [product('square', (square_parts, square_parts, square), by_row, by_row, None, r, r, c, triangle, (scale_x, scale_x, scale_a), (0, 1, 2)),
-                     product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, triangle, (scale_a, scale_a, scale_p), (0, 1))]
+        launches += [product('square', (square_parts, square_parts, square), by_row, by_row, None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2)),
+                     product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, (scale_a, scale_a, scale_p), (0, 1))]
         last = i == steps - 1
         scale_next = 0 if last else _half_scale(bounds[i + 1][0])
-        launches.append(product('last' if last else 'next', (None, None, out) if last else (by_column[(i + 1) & 1], by_row, None), polynomial, by_column[i & 1], None, r, c, r, all_tiles,
+        launches.append(product('last' if last else 'next', (None, None, out) if last else (by_column[(i + 1) & 1], by_row, None), polynomial, by_column[i & 1], None, r, c, r,
                                 (scale_p, scale_x, scale_next), (2,) if last else (0, 1)))
     return launches

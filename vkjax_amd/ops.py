@@ -1258,7 +1258,7 @@ def orthogonalize(bufferpool, equation):
     p = equation.params
     (x,), (out,), scratch = _operator_buffers(bufferpool, equation)
     _float_operands(equation, x)
-    return _operator_ops(equation, K.orthogonalize(out, x, p['steps'], p['coefficients'], p['eps'], scratch))
+    return _operator_ops(equation, K.orthogonalize(out, x, p['steps'], p['coefficients'], p['eps'], scratch, bufferpool.zeroed_scratch))
 
 
 # ------------------------------------------------------------------ rng
