@@ -37,9 +37,11 @@ __device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)(127
 
 // ---- the product of a tile: four waves, two by two, of T x T blocks of 32 x 32 each. Pairs of steps (32 k) of both operands go straight from memory into one of STAGES buffers in
 // shared memory while the waves work on another one.
-//   T = 2, STAGES = 2   tiles of 128, 64 KB, two blocks to a CU: for what fills the machine. 8192^3 378 TFLOP/s of fp32 products (an fp32 library product 153, an fp16 one a third of 1143)
-//   T = 2, STAGES = 4   the same with a block to a CU, whose three pairs on their way take the place of the other block: where there are no more tiles than CUs
-//   T = 1, STAGES = 4   tiles of 64, 64 KB: where tiles of 128 would be few
+//   T = 2, STAGES = 2   tiles of 128, 64 KB, two blocks to a CU: for what fills the machine. 8192^3 354 to 378 TFLOP/s of fp32 products (an fp32 library product 153, a third of an fp16 one
+//                       381). Bound by power: the matrix cores are busy 57 % of the time at 1.73 GHz, 54 % at 1.96 for 4096^3.
+//   T = 1, STAGES = 4   tiles of 64, 64 KB, two blocks to a CU: few tiles, whose time is that of a pair of steps after the other: 0.38 us each, of 128 0.68
+//   T = 1, STAGES = 2   the same, 32 KB, four blocks to a CU: between the two
+// (Tiles of 128 with four buffers and a block to a CU: 0.76 us a pair.)
 // Few tiles, or those left behind whole rounds of the machine, share a tile's contraction among `slices` blocks: they leave their sums in memory, and the one that arrives last adds them
 // in the order of the slices. Nobody waits for another block.
 template <int T> struct HalfTileOf {

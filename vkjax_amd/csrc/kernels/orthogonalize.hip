@@ -7,6 +7,8 @@
 // Matrices of a stack lie side by side in every launch.
 #include "half_product.h"
 
+typedef f32x4 f32x4_anywhere __attribute__((aligned(4)));
+
 struct SquaresParams { uint32_t blocks, pad; uint64_t n; };
 // [matrix][block]: sums of squares
 extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __restrict__ sums, const float* __restrict__ x, SquaresParams P) {
@@ -15,11 +17,19 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __re
     const float* const from = x + matrix * P.n;
     const uint64_t stride = (uint64_t)P.blocks * 256u;
     float s[4] = {};
+    // (vectors wherever every matrix begins at one)
+    const uint64_t vectors = (P.n & 3u) == 0u ? P.n / 4u : 0u;
     uint64_t at = (uint64_t)block * 256u + threadIdx.x;
-    for (; at + 3u * stride < P.n; at += 4u * stride)
+    for (; at < vectors; at += 4u * stride) {
+        f32x4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { const float v = from[at + k * stride]; s[k] = __builtin_fmaf(v, v, s[k]); }
-    for (; at < P.n; at += stride) s[0] = __builtin_fmaf(from[at], from[at], s[0]);
+        for (int k = 0; k < 4; ++k) v[k] = at + k * stride < vectors ? reinterpret_cast<const f32x4*>(from)[at + k * stride] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(v[k][e], v[k][e], s[e]);
+    }
+    for (at = 4u * vectors + (uint64_t)block * 256u + threadIdx.x; at < P.n; at += stride) s[0] = __builtin_fmaf(from[at], from[at], s[0]);
     float t = (s[0] + s[1]) + (s[2] + s[3]);
     wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
     if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = t;
@@ -53,17 +63,32 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restr
     const uint32_t i = rb * 32u + (lane & 31u), h4 = 4u * (lane >> 5);
     const float* const from = x + (uint64_t)matrix * P.R * P.C + (uint64_t)min(i, I - 1u) * si;
     u32x4* const to = (rows ? by_row : by_column) + ((uint64_t)matrix * blocks32 + rb) * steps * 128u + lane;
-    for (uint32_t s = group * each; s < min(steps, (group + 1u) * each); ++s) {
-        float v[8];
+    // (the operands of four steps at once)
+    constexpr int AT_ONCE = 4;
+    const uint32_t end = min(steps, (group + 1u) * each);
+    for (uint32_t s0 = group * each; s0 < end; s0 += AT_ONCE) {
+        float v[AT_ONCE][8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const uint32_t k = s * 16u + h4 + 8u * (q >> 2) + (q & 3);
-            v[q] = i < I && k < K ? from[(uint64_t)k * sk] / norm * up : 0.f;
+        for (int t = 0; t < AT_ONCE; ++t)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t k = (s0 + t) * 16u + h4 + 8u * q;
+                if (along_k && k + 4u <= K && i < I) {
+                    const f32x4 w = *reinterpret_cast<const f32x4_anywhere*>(from + k);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[t][4 * q + e] = w[e];
+                } else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[t][4 * q + e] = i < I && k + e < K ? from[(uint64_t)(k + e) * sk] : 0.f;
+            }
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) {
+            if (s0 + t >= end) break;
+            u32x4 hi, lo;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[t][2 * q] / norm * up, v[t][2 * q + 1] / norm * up, a, b); hi[q] = a; lo[q] = b; }
+            to[(s0 + t) * 128u] = hi; to[(s0 + t) * 128u + 64u] = lo;
         }
-        u32x4 hi, lo;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[2 * q], v[2 * q + 1], a, b); hi[q] = a; lo[q] = b; }
-        to[s * 128u] = hi; to[s * 128u + 64u] = lo;
     }
 }
 
@@ -76,7 +101,7 @@ struct OrthogonalParams {
     uint64_t sr, sc;                                     // the last result's element strides
 };
 // (kinds in templates: their epilogues share no registers)
-template <uint32_t KIND, int T, int STAGES>
+template <uint32_t KIND, int T, int STAGES, bool SHARED>
 __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u32x4* __restrict__ by_row, float* __restrict__ out, float* __restrict__ partial, uint32_t* __restrict__ arrivals,
                                                 const u32x4* __restrict__ a, const u32x4* __restrict__ b, const float* __restrict__ square, const OrthogonalParams& P) {
     __shared__ HalfShared<T, STAGES> shared;
@@ -96,7 +121,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u},
                             HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
-    if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
     const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = row0 + (wave >> 1) * 32u * T + 4u * (lane >> 5), lane_column = column0 + (wave & 1u) * 32u * T + (lane & 31u);
@@ -137,14 +162,18 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
         return v * up;
     });
 }
-#define ORTHOGONAL(NAME, KIND, SUFFIX, T, STAGES, BLOCKS)                                                                                                             \
+#define ORTHOGONAL(NAME, KIND, SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                     \
     extern "C" __global__ __launch_bounds__(256, BLOCKS) void orthogonal_##NAME##SUFFIX(u32x4* by_column, u32x4* by_row, float* out, float* partial, uint32_t* arrivals, \
                                                                                         const u32x4* a, const u32x4* b, const float* square, OrthogonalParams P) {    \
-        orthogonal_body<KIND, T, STAGES>(by_column, by_row, out, partial, arrivals, a, b, square, P);                                                                 \
+        orthogonal_body<KIND, T, STAGES, SHARED>(by_column, by_row, out, partial, arrivals, a, b, square, P);                                                         \
     }
-#define ORTHOGONAL_KINDS(SUFFIX, T, STAGES, BLOCKS)                                                                                                                   \
-    ORTHOGONAL(square, SQUARE, SUFFIX, T, STAGES, BLOCKS) ORTHOGONAL(polynomial, POLYNOMIAL, SUFFIX, T, STAGES, BLOCKS) ORTHOGONAL(next, NEXT, SUFFIX, T, STAGES, BLOCKS) \
-    ORTHOGONAL(last, LAST, SUFFIX, T, STAGES, BLOCKS)
-ORTHOGONAL_KINDS(_128, 2, 2, 2)
-ORTHOGONAL_KINDS(_128_alone, 2, 4, 1)
-ORTHOGONAL_KINDS(_64, 1, 4, 2)
+#define ORTHOGONAL_KINDS(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                           \
+    ORTHOGONAL(square, SQUARE, SUFFIX, T, STAGES, BLOCKS, SHARED) ORTHOGONAL(polynomial, POLYNOMIAL, SUFFIX, T, STAGES, BLOCKS, SHARED)                               \
+    ORTHOGONAL(next, NEXT, SUFFIX, T, STAGES, BLOCKS, SHARED) ORTHOGONAL(last, LAST, SUFFIX, T, STAGES, BLOCKS, SHARED)
+// (contractions that are not shared have kernels of their own: what adds slices up costs registers, 372 -> 400 us for 4096^3)
+ORTHOGONAL_KINDS(_128, 2, 2, 2, false)
+ORTHOGONAL_KINDS(_128_shared, 2, 2, 2, true)
+ORTHOGONAL_KINDS(_64, 1, 4, 2, false)
+ORTHOGONAL_KINDS(_64_shared, 1, 4, 2, true)
+ORTHOGONAL_KINDS(_64_many, 1, 2, 4, false)
+ORTHOGONAL_KINDS(_64_many_shared, 1, 2, 4, true)

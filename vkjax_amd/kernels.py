@@ -2708,7 +2708,7 @@ def selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept: 
 # ---------------------------------------------------------------- products on the fp16 matrix cores (half_product.h)
 
 HALF_TILE = 128                         #rows and columns of a block's tile
-HALF_BLOCKS = 512                       #blocks that the machine runs at once
+HALF_BLOCKS = 512                       #blocks of such tiles that the machine runs at once
 
 
 def _half_steps(k: int) -> int:
@@ -2866,29 +2866,29 @@ class HalfPlan(tp.NamedTuple):
 def half_plan(tiles_of, pairs: int) -> HalfPlan:
     '''The plan with the smallest estimated time (us) for tiles_of(side) tiles and a contraction of so many pairs of steps.'''
     best = None
-    for kernel, side, blocks_of_cu, start, alone, together in HALF_KERNELS:
-        tiles = tiles_of(side)
+    for kernel, side, blocks_of_cu, start, pair, unit in HALF_KERNELS:
+        tiles, slots = tiles_of(side), HALF_CUS * blocks_of_cu
+
+        def time(blocks, pairs):
+            #full rounds of the machine, then one of fewer blocks to a CU
+            full, rest = divmod(blocks, slots)
+            return full * (start + pairs * max(pair, blocks_of_cu * unit)) + (start + pairs * max(pair, _cdiv(rest, HALF_CUS) * unit) if rest else 0)
         for slices in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32):
-            if slices > max(1, pairs // HALF_SLICE_PAIRS):
-                break
-            slots = 256 * blocks_of_cu
             whole = tiles if slices == 1 else tiles // slots * slots
-            if slices > 1 and whole == tiles:
+            if slices > 1 and (slices * HALF_SLICE_PAIRS > pairs or whole == tiles):
                 continue
-            def rounds(blocks, pairs):
-                #full rounds of the machine, then one with fewer blocks to a CU
-                full, rest = divmod(blocks, slots)
-                return full * (start + pairs * together) + (0 if rest == 0 else start + pairs * (alone if rest <= 256 else together))
-            cost = rounds(whole, pairs) + (rounds((tiles - whole) * slices, _cdiv(pairs, slices)) + HALF_JOIN + HALF_JOIN_SLICE * slices * (side / 128)**2 if whole < tiles else 0)
-            if slices == 1:
-                cost = rounds(tiles, pairs)
+            cost = time(whole, pairs)
+            if whole < tiles:
+                cost += time((tiles - whole) * slices, _cdiv(pairs, slices)) + HALF_JOIN + HALF_JOIN_SLICE * slices * (side / 128)**2
             if best is None or cost < best[0]:
                 best = (cost, HalfPlan(kernel, side, whole, slices))
     return best[1]
 
 
-#kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps with a block to a CU, with several)
-HALF_KERNELS = (('_128', 128, 2, 6.0, 0.95, 1.42), ('_128_alone', 128, 1, 6.0, 0.75, 0.75), ('_64', 64, 2, 4.0, 0.33, 0.45))
+HALF_CUS = 256
+#kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps at least, us of a CU for one), by measurement: products of 512 x 512 x 512 alone 18.5,
+#11.0 and 11.7 us, of 512 x 512 x 4096 96, 53 and 64, of 2048^3 64, 84 and 67, 192 tiles of 128 x 16 pairs 21, 21.6 and 18
+HALF_KERNELS = (('_128', 128, 2, 8.0, 0.68, 0.71), ('_64', 64, 2, 4.5, 0.38, 0.30), ('_64_many', 64, 4, 4.0, 0.47, 0.25))
 HALF_SLICE_PAIRS = 4                    #pairs of steps of a slice, at least
 HALF_JOIN, HALF_JOIN_SLICE = 3.0, 0.6   #us of adding up slices, and for each of them
 
@@ -2901,7 +2901,7 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
     sr, sc = (1, columns) if tall else (columns, 1)                                         #element strides of the wide way round
     if max(r, c) >= 2**20 or n * _cdiv(r, 64) * _cdiv(c, 64) >= 2**24 or n * (_cdiv(r, 32) * _half_steps(c) + _cdiv(c, 32) * _half_steps(r)) >= 2**28:
         raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
-    sum_blocks = max(1, min(256, _cdiv(r * c, 4096)))
+    sum_blocks = max(1, min(1024 if n == 1 else 256, _cdiv(r * c, 4096)))
     sums     = scratch((n, sum_blocks))
     by_row   = scratch((n * _half_words(r, c),), np.uint32)
     by_column = [scratch((n * _half_words(c, r),), np.uint32) for _ in range(2 if steps > 1 else 1)]
@@ -2921,7 +2921,7 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
         rest  = tiles - plan.whole
         partial  = scratch((rest * plan.slices, plan.side, plan.side)) if plan.slices > 1 else None
         arrivals = zeroed(rest, 'arrivals at tiles of halves') if plan.slices > 1 else None
-        launch = Launch(f'orthogonal_{name}{plan.kernel}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
+        launch = Launch(f'orthogonal_{name}{plan.kernel}{"_shared" if plan.slices > 1 else ""}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
                         _u32(('square', 'polynomial', 'next', 'last').index(name), m, width, k, _cdiv(m, plan.side), _cdiv(width, plan.side), of_matrix(plan.side)) + _i32(*scales)
                         + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, 0) + _u64(sr, sc),
                         bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=(1 if symmetric else 2) * n * m * width * k,
