@@ -1060,7 +1060,12 @@ def _linear_scores64(x, weights, tokens, transposed):
     return w, rows, s, np.where(given, token, 0), given, peak, np.exp(s - peak[:, None]).sum(axis=1)
 
 
-def linear_log_probs(x, weights, tokens, transposed):
+def linear_log_probs(x, weights, tokens, transposed, parts=False):
+    if parts:
+        #(what the device keeps of its operands for the gradient, which is worked out from the operands themselves here)
+        from vkjax_amd.kernels import linear_parts
+        kept = tuple(np.zeros(n, dtype) for n, dtype in zip(linear_parts(np.shape(x), np.shape(weights), transposed), (np.uint32, np.uint32, i32)))
+        return linear_log_probs(x, weights, tokens, transposed) + kept
     with np.errstate(**_EW_ERR):
         if np.size(tokens) == 0:
             return (np.zeros(np.shape(tokens), f32),) * 4
@@ -1070,8 +1075,8 @@ def linear_log_probs(x, weights, tokens, transposed):
         return rows(s[np.arange(len(s)), token] - log_sum, 0.0), rows(log_sum, 0.0), rows(peak, 0.0), rows(total, 1.0)
 
 
-def linear_log_probs_grad(x, weights, tokens, peaks, totals, *cotangents, transposed, has_log_probs, has_log_sums):
-    cotangents = [np.asarray(c, np.float64).reshape(-1) for c in cotangents]
+def linear_log_probs_grad(x, weights, tokens, peaks, totals, *cotangents, transposed, has_log_probs, has_log_sums, has_parts=False):
+    cotangents = [np.asarray(c, np.float64).reshape(-1) for c in cotangents[:has_log_probs + has_log_sums]]
     with np.errstate(**_EW_ERR):
         if np.size(tokens) == 0:
             return np.zeros(x.shape, f32), np.zeros(weights.shape, f32)

@@ -396,3 +396,13 @@ def test_orthogonalize_a_matrix_of_a_low_rank_and_of_zeros():
     assert not got[2].any() and np.isnan(got[3]).all()
     for i in (0, 1):
         assert np.linalg.norm(got[i].astype(np.float64) - expected[i]) <= orthogonal_bound(x[i], 5, (3.4445, -4.7750, 2.0315))
+
+
+def test_gradient_of_log_probs_with_and_without_the_operands_that_were_kept():
+    x, w, tokens, g, gs = loss_inputs(150, 70, 600, False)
+
+    def both_ways(x, w, tokens, g, gs):
+        outs = lax.linear_log_probs(x, w, tokens, with_parts=True)
+        return lax.linear_log_probs_grad(x, w, tokens, outs[2], outs[3], g, gs, parts=outs[4:]) + lax.linear_log_probs_grad(x, w, tokens, outs[2], outs[3], g, gs)
+    (dx, dw, dx2, dw2), _, _ = both(both_ways, x, w, tokens, g, gs)
+    assert np.array_equal(dx, dx2) and np.array_equal(dw, dw2)

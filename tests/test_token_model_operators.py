@@ -364,3 +364,21 @@ def test_orthogonalize_knows_how_large_singular_values_become():
             p = a + b * s**2 + c * s**4
             assert 1.1 * np.abs(s).max() < most and 1.1 * np.abs(p).max() < polynomial and polynomial >= abs(a)
             s = p * s
+
+
+def test_log_probs_keep_their_operands_for_a_gradient_only():
+    x, w, t, g = normal(1, 5, 4), normal(2, 4, 7), np.arange(5, dtype=np.int32), normal(3, 5)
+    kept = lambda program, *args: [e.params['parts'] for e in mj.make_jaxpr(program)(*args).jaxpr.eqns if e.primitive.name == 'linear_log_probs']
+    assert kept(lambda x, w: nn.linear_log_probs(x, w, t), x, w) == [False]
+    assert kept(loss_program(False), x, w, t, g, g) == [True]
+
+    def by_hand(x, w, t, g):
+        outs = lax.linear_log_probs(x, w, t, with_parts=True)
+        return lax.linear_log_probs_grad(x, w, t, outs[2], outs[3], g, parts=outs[4:]) + lax.linear_log_probs_grad(x, w, t, outs[2], outs[3], g)
+    dx, dw, dx2, dw2 = evaluate(by_hand, x, w, t, g)
+    assert np.array_equal(dx, dx2) and np.array_equal(dw, dw2)
+    words = [np.zeros(n, d) for n, d in zip(K.linear_parts(x.shape, w.shape, False), (np.uint32, np.uint32, np.int32))]
+    for at in range(3):
+        for bad in (words[at][:-1], words[at].astype(f32), words[at].reshape(1, -1)):
+            refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *(words[:at] + [bad] + words[at + 1:]))
+    refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *words[:2])

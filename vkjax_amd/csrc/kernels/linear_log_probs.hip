@@ -78,13 +78,14 @@ struct PackJob { uint32_t blocks, I, K, stride, kind, steps; uint64_t si, sk; };
 struct PackParams { uint32_t weight_blocks, row_blocks, V, pad; PackJob jobs[4]; };
 struct PackOuts { u32x4* parts[4]; };
 extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int32_t* __restrict__ scales, const float* __restrict__ x, const float* __restrict__ w,
-                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors, PackParams P) {
+                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors,
+                                                              const int32_t* __restrict__ known, PackParams P) {
     __shared__ float part[4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t block = blockIdx.x, job = 0u;
     while (job < 3u && block >= P.jobs[job].blocks) block -= P.jobs[job++].blocks;
     const PackJob J = P.jobs[job];
-    // the operand's scale, of its blocks' largest magnitudes
+    // the operand's scale, of its blocks' largest magnitudes, or the weights' that is known
     const bool weights = J.kind == PACK_WEIGHTS;
     float most = 0.f;
     for (uint32_t k = threadIdx.x; k < (weights ? P.weight_blocks : P.row_blocks); k += 256u)
@@ -92,7 +93,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
     most = wave_largest(most);
     if (lane == 0u) part[wave] = most;
     __syncthreads();
-    const int e = half_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+    const int e = weights && known ? known[PACK_WEIGHTS] : half_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
     if (block == 0u && threadIdx.x == 0u) scales[J.kind] = e;
     const float up = power_of_two(e);
     // waves beside one another along the side that is contiguous in memory
@@ -104,33 +105,40 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
     const float* const from = (weights ? w : x) + (uint64_t)min(i, J.I - 1u) * J.si;
     bool there = i < J.I;
     if (J.kind == PACK_ROWS) there = there && is_token(tokens[min(i, J.I - 1u)], P.V);
-    const bool vectors = along_k;
-    for (uint32_t s = group * J.stride; s < min(J.steps, (group + 1u) * J.stride); ++s) {
-        float v[8];
-        const uint32_t k0 = s * 16u + h4;
+    // (the operands of four steps at once)
+    constexpr int AT_ONCE = 4;
+    const uint32_t end = min(J.steps, (group + 1u) * J.stride);
+    u32x4* const to = outs.parts[job] + (uint64_t)rb * J.steps * 128u + lane;
+    for (uint32_t s0 = group * J.stride; s0 < end; s0 += AT_ONCE) {
+        float v[AT_ONCE][8];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const uint32_t k = k0 + 8u * q;
-            if (vectors && k + 4u <= J.K) {
-                const f32x4 t = there ? *reinterpret_cast<const f32x4_anywhere*>(from + k) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < AT_ONCE; ++t)
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) v[4 * q + e4] = t[e4];
-            } else
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t k = (s0 + t) * 16u + h4 + 8u * q;
+                if (along_k && k + 4u <= J.K && there) {
+                    const f32x4 f = *reinterpret_cast<const f32x4_anywhere*>(from + k);
 #pragma unroll
-                for (int e4 = 0; e4 < 4; ++e4) v[4 * q + e4] = there && k + e4 < J.K ? from[(uint64_t)(k + e4) * J.sk] : 0.f;
-        }
-        if (J.kind == PACK_SCALED)
+                    for (int e4 = 0; e4 < 4; ++e4) v[t][4 * q + e4] = f[e4];
+                } else
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const uint32_t k = k0 + 8u * (q >> 2) + (q & 3);
-                const float m = k < J.K ? factors[3u * k] : 0.f;
-                v[q] = m == 0.f ? 0.f : v[q] * m;                     // (a row without a cotangent has none, whatever its x is)
+                    for (int e4 = 0; e4 < 4; ++e4) v[t][4 * q + e4] = there && k + e4 < J.K ? from[(uint64_t)(k + e4) * J.sk] : 0.f;
             }
-        u32x4 hi, lo;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[2 * q] * up, v[2 * q + 1] * up, a, b); hi[q] = a; lo[q] = b; }
-        u32x4* const to = outs.parts[job] + ((uint64_t)rb * J.steps + s) * 128u + lane;
-        to[0] = hi; to[64] = lo;
+        for (int t = 0; t < AT_ONCE; ++t) {
+            if (s0 + t >= end) break;
+            if (J.kind == PACK_SCALED)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const uint32_t k = (s0 + t) * 16u + h4 + 8u * (q >> 2) + (q & 3);
+                    const float m = k < J.K ? factors[3u * k] : 0.f;
+                    v[t][q] = m == 0.f ? 0.f : v[t][q] * m;           // (a row without a cotangent has none, whatever its x is)
+                }
+            u32x4 hi, lo;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[t][2 * q] * up, v[t][2 * q + 1] * up, a, b); hi[q] = a; lo[q] = b; }
+            to[(s0 + t) * 128u] = hi; to[(s0 + t) * 128u + 64u] = lo;
+        }
     }
 }
 
@@ -190,34 +198,51 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __rest
     }
 }
 
-// A row's tiles joined, 64 rows to a block, every 16th tile to a wave
-struct JoinParams { uint32_t first, rows, V, tiles; };
+// A row's tiles joined. A block has R rows (a power of two up to 64): 1024 / R lanes to a row, which take tiles in turn, eight at a time, and meet by butterflies and in shared memory.
+struct JoinParams { uint32_t log2_rows, rows, V, tiles; };
+struct PeakSum {
+    float peak, sum;
+    __device__ __forceinline__ void add(float p, float s) {
+        const float next = fmaxf(peak, p), base = next == -__builtin_inff() ? 0.f : next;
+        sum = sum * exp_of(peak - base) + s * exp_of(p - base);
+        peak = next;
+    }
+};
 extern "C" __global__ __launch_bounds__(1024) void linear_join(float* __restrict__ log_probs, float* __restrict__ log_sums, float* __restrict__ row_peaks, float* __restrict__ row_totals,
                                                                const float* __restrict__ peaks, const float* __restrict__ sums, const float* __restrict__ of_token,
                                                                const int32_t* __restrict__ tokens, JoinParams P) {
     __shared__ float met[16][64][2];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, r = blockIdx.x * 64u + lane, at = min(r, P.rows - 1u);
-    float peak = -__builtin_inff(), sum = 0.f;
-    for (uint32_t t = wave; t < P.tiles; t += 16u) {
-        const float p = peaks[(uint64_t)t * P.rows + at], s = sums[(uint64_t)t * P.rows + at], next = fmaxf(peak, p), base = next == -__builtin_inff() ? 0.f : next;
-        sum = sum * exp_of(peak - base) + s * exp_of(p - base);
-        peak = next;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, R = 1u << P.log2_rows, row = lane & (R - 1u), r = blockIdx.x * R + row, at = min(r, P.rows - 1u);
+    const uint32_t groups = 1024u >> P.log2_rows, group = threadIdx.x >> P.log2_rows;
+    PeakSum all = {-__builtin_inff(), 0.f};
+    for (uint32_t t0 = group; t0 < P.tiles; t0 += 8u * groups) {
+        float p[8], s[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) {
+            const bool has = t0 + k * groups < P.tiles;
+            const uint64_t from = (uint64_t)min(t0 + k * groups, P.tiles - 1u) * P.rows + at;
+            const float pk = peaks[from], sk = sums[from];
+            p[k] = has ? pk : -__builtin_inff(); s[k] = has ? sk : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all.add(p[k], s[k]);
     }
-    met[wave][lane][0] = peak; met[wave][lane][1] = sum;
+    wave_butterfly([&](auto step) {
+        constexpr int S = decltype(step)::value;
+        const float p = lane_xor<S>(all.peak), s = lane_xor<S>(all.sum);
+        if ((uint32_t)S >= R) all.add(p, s);
+    });
+    met[wave][lane][0] = all.peak; met[wave][lane][1] = all.sum;
     __syncthreads();
-    if (wave != 0u || r >= P.rows) return;
+    if (wave != 0u || lane >= R || r >= P.rows) return;
 #pragma unroll
-    for (int q = 1; q < 16; ++q) peak = fmaxf(peak, met[q][lane][0]);
-    const float base = peak == -__builtin_inff() ? 0.f : peak;
-    sum = 0.f;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) sum += met[q][lane][1] * exp_of(met[q][lane][0] - base);
+    for (int q = 1; q < 16; ++q) all.add(met[q][lane][0], met[q][lane][1]);
     const bool given = is_token(tokens[r], P.V);
-    const float log_total = __builtin_amdgcn_logf(sum) * LN2;
-    if (log_probs) log_probs[r] = given ? (of_token[r] - peak) - log_total : 0.f;
-    if (log_sums)  log_sums[r]  = given ? peak + log_total : 0.f;
-    if (row_peaks)  row_peaks[r]  = given ? peak : 0.f;
-    if (row_totals) row_totals[r] = given ? sum : 1.f;
+    const float log_total = __builtin_amdgcn_logf(all.sum) * LN2;
+    if (log_probs) log_probs[r] = given ? (of_token[r] - all.peak) - log_total : 0.f;
+    if (log_sums)  log_sums[r]  = given ? all.peak + log_total : 0.f;
+    if (row_peaks)  row_peaks[r]  = given ? all.peak : 0.f;
+    if (row_totals) row_totals[r] = given ? all.sum : 1.f;
 }
 
 // ---- up to 32 NT rows: a block has 128 tokens, its waves parts of the contraction; W is read once. v_mfma_f32_32x32x2_f32: lane l has row l % 32 of a block of 32 and k = l / 32.
@@ -431,16 +456,15 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_product(float* __res
 
 struct SumParams { uint32_t parts, pad; uint64_t n; };
 extern "C" __global__ __launch_bounds__(256) void linear_sum(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {
-    const uint64_t at = ((uint64_t)blockIdx.x * 256u + threadIdx.x) * 4u;
+    const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
     if (at >= P.n) return;
-    if (at + 4u <= P.n && (P.n & 3u) == 0u) {
-        f32x4 s = *reinterpret_cast<const f32x4*>(parts + at);
-        for (uint32_t k = 1; k < P.parts; ++k) { const f32x4 t = *reinterpret_cast<const f32x4*>(parts + k * P.n + at); s += t; }
-        *reinterpret_cast<f32x4*>(out + at) = s;
-    } else
-        for (uint32_t e = 0; e < 4u && at + e < P.n; ++e) {
-            float s = parts[at + e];
-            for (uint32_t k = 1; k < P.parts; ++k) s += parts[k * P.n + at + e];
-            out[at + e] = s;
-        }
+    float s = 0.f;
+    for (uint32_t k0 = 0; k0 < P.parts; k0 += 8u) {
+        float v[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8u; ++k) v[k] = k0 + k < P.parts ? parts[(k0 + k) * P.n + at] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    out[at] = s;
 }

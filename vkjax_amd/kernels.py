@@ -2743,28 +2743,34 @@ def _linear_shape(x: Buffer, w: Buffer, transposed: bool) -> LinearShape:
     h, v   = reversed(w.shape) if transposed else w.shape
     shape  = LinearShape(x.size // h, h, v)
     #(indices of rows, tokens and steps are 32 bits, addresses 64)
-    if max(shape) >= 2**27 or _cdiv(shape.rows, HALF_TILE) * _cdiv(v, HALF_TILE) >= 2**23:
+    if max(shape) >= 2**27 or shape.rows * h >= 2**31 or _cdiv(shape.rows, HALF_TILE) * _cdiv(v, HALF_TILE) >= 2**23:
         raise NotImplementedError(f'log probabilities of {shape.rows} rows of {h} over {v} tokens')
     return shape
 
 
-def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, cotangents, scratch):
-    '''The operands that the products need, taken apart: (launches, W contracted over h, x, their scales; with cotangents also W contracted over the
-    vocabulary, x with its rows' factors contracted over the rows, and the factors).'''
+def linear_parts(x_shape, w_shape, transposed: bool) -> tp.Tuple[int, int, int]:
+    '''Words of the weights and of x, taken apart for the scores' product, and of their scales.'''
+    h, v = reversed(w_shape) if transposed else w_shape
+    return _half_words(v, h), _half_words(math.prod(x_shape) // h, h), 4
+
+
+def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, known=None, cotangents=None):
+    '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x) - or, where that has been done, with the weights' scale from `known` -, and with cotangents
+    for those behind it, into (the weights contracted over the vocabulary, x with its rows' factors contracted over the rows, the factors), which are returned. Scales go to `scales`.'''
     rows, h, v = shape
-    weight_blocks = max(1, min(512, _cdiv(h * v, 4096)))
     row_blocks    = max(1, min(256, _cdiv(rows, 4)))
+    weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if known is None else 0
     largest = scratch((weight_blocks + 2 * row_blocks,))
     factors = scratch((rows, 3)) if cotangents else None
-    scales  = scratch((4,), np.int32)
     g_log_probs, g_log_sums = cotangents or (None, None)
     by_v, by_h = ((h, 1), (1, h)) if transposed else ((1, v), (v, 1))                       #element strides of (token, h) and (h, token)
-    jobs = [(v, h, _PACK_WEIGHTS, by_v), (rows, h, _PACK_ROWS, (h, 1))]
+    jobs = [(forward[0], v, h, _PACK_WEIGHTS, by_v), (forward[1], rows, h, _PACK_ROWS, (h, 1))] if forward else []
+    behind = (None, None)
     if cotangents:
-        jobs += [(h, v, _PACK_WEIGHTS, by_h), (h, rows, _PACK_SCALED, (1, h))]
-    parts  = [scratch((_half_words(i, k),), np.uint32) for i, k, _, _ in jobs]
+        behind = scratch((_half_words(h, v),), np.uint32), scratch((_half_words(h, rows),), np.uint32)
+        jobs += [(behind[0], h, v, _PACK_WEIGHTS, by_h), (behind[1], h, rows, _PACK_SCALED, (1, h))]
     params, blocks = _u32(weight_blocks, row_blocks, v, 0), 0
-    for i, k, kind, strides in jobs:
+    for _, i, k, kind, strides in jobs:
         steps  = _half_steps(k)
         each   = min(steps, 8)
         blocks += _cdiv(_cdiv(i, 32) * _cdiv(steps, each), 4)
@@ -2772,30 +2778,41 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     params += bytes(40) * (4 - len(jobs))
     launches = [Launch('linear_largest', (weight_blocks + row_blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (largest, factors, x, w, tokens, g_log_probs, g_log_sums)],
                        _u32(0, rows, h, v, weight_blocks, row_blocks), bytes_moved=4 * (x.size + w.size), written=(0, 1)),
-                Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in parts] + [(None, 0)] * (4 - len(parts)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors)],
-                       params, bytes_moved=8 * (x.size + w.size) * (1 + bool(cotangents)), written=(0, 1, 2, 3, 4))]
-    return launches, parts, scales, factors
+                Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(j[0], 0) for j in jobs] + [(None, 0)] * (4 - len(jobs)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors, known)],
+                       params, bytes_moved=8 * sum(i * k for _, i, k, _, _ in jobs), written=(0, 1, 2, 3, 4))]
+    return launches, (*behind, factors)
 
 
-def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch) -> tp.List[Launch]:
+def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, parts=None) -> tp.List[Launch]:
     shape = rows, h, v = _linear_shape(x, w, transposed)
     tiles    = _cdiv(v, HALF_TILE)
     of_tiles = [scratch((tiles, rows)), scratch((tiles, rows)), scratch((rows,))]           #peak and sum of each tile's scores, the token's score
-    if rows <= LINEAR_ROWS and v >= 4:
+    if rows <= LINEAR_ROWS and v >= 4 and not parts:
         launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles, 1, 1), (512, 1, 1), [(b, 0) for b in (*of_tiles, x, w, tokens)],
                            _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2))]
     else:
-        launches, (w_parts, x_parts), scales, _ = _linear_prepare(shape, x, w, tokens, transposed, None, scratch)
+        w_parts, x_parts, scales = parts or [scratch((n,), dtype) for n, dtype in zip(linear_parts(x.shape, w.shape, transposed), (np.uint32, np.uint32, np.int32))]
+        launches, _ = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts))
         launches.append(Launch('linear_scores', (tiles * _cdiv(rows, HALF_TILE), 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (*of_tiles, w_parts, x_parts, tokens, scales)],
                                _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, _cdiv(rows, HALF_TILE), _cdiv(v, 32), _cdiv(rows, 32), 0, 0, 0),
                                bytes_moved=4 * (w_parts.size + x_parts.size), flops=2 * rows * h * v, written=(0, 1, 2)))
-    return launches + [Launch('linear_join', (_cdiv(rows, 64), 1, 1), (1024, 1, 1), [(b, 0) for b in (log_probs, log_sums, peaks, totals, *of_tiles, tokens)],
-                              _u32(0, rows, v, tiles), bytes_moved=8 * tiles * rows, written=(0, 1, 2, 3))]
+    #rows of a block: a line of them, fewer where there are few
+    join_rows = min(16, _pow2_at_least(rows))
+    return launches + [Launch('linear_join', (_cdiv(rows, join_rows), 1, 1), (1024, 1, 1), [(b, 0) for b in (log_probs, log_sums, peaks, totals, *of_tiles, tokens)],
+                              _u32(join_rows.bit_length() - 1, rows, v, tiles), bytes_moved=8 * tiles * rows, written=(0, 1, 2, 3))]
 
 
-def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch) -> tp.List[Launch]:
+def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch,
+                          parts=None) -> tp.List[Launch]:
     shape = rows, h, v = _linear_shape(x, w, transposed)
-    launches, (w_parts, x_parts, w_by_h, x_scaled), scales, factors = _linear_prepare(shape, x, w, tokens, transposed, (g_log_probs, g_log_sums), scratch)
+    scales = scratch((4,), np.int32)                       #of all that is taken apart here
+    if parts:
+        w_parts, x_parts, score_scales = parts
+        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None, score_scales, (g_log_probs, g_log_sums))
+    else:
+        w_parts, x_parts = [scratch((n,), np.uint32) for n in linear_parts(x.shape, w.shape, transposed)[:2]]
+        score_scales = scales
+        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts), None, (g_log_probs, g_log_sums))
     #pieces of the vocabulary, of whole tiles
     row_blocks, all_tiles = _cdiv(rows, 32), _cdiv(v, HALF_TILE)
     pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (8 * 32 * row_blocks * HALF_TILE)))
@@ -2816,7 +2833,7 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         first = piece * each
         tiles = min(each, all_tiles - first)
         v0, n = first * HALF_TILE, min(width, v - first * HALF_TILE)
-        launches.append(Launch('linear_q', (tiles * tiles_r, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (by_row, by_token, w_parts, x_parts, tokens, scales, peaks, totals, factors)],
+        launches.append(Launch('linear_q', (tiles * tiles_r, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors)],
                                _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, tiles_r, _cdiv(v, 32), row_blocks, first, width, 0),
                                bytes_moved=8 * 32 * row_blocks * width, flops=2 * rows * h * n, written=(0, 1)))
         launches.append(product(parts, piece * slices * rows * h, by_row, w_by_h, rows, h, _cdiv(n, 32), slices, row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), 0, v0 // 16,
@@ -2827,7 +2844,7 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         else:
             launches.append(product(dw, v0, scaled[0], q[0], h, n, row_blocks, 1, scaled[1], q[1], scaled[2], q[2], 0, 0, _PACK_SCALED, -1, v, 0, False))
     if pieces * slices > 1:
-        launches.append(Launch('linear_sum', (_cdiv(rows * h, 4 * BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (parts, 0)], _u32(pieces * slices, 0) + _u64(rows * h),
+        launches.append(Launch('linear_sum', (_cdiv(rows * h, BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (parts, 0)], _u32(pieces * slices, 0) + _u64(rows * h),
                                bytes_moved=4 * (parts.size + rows * h)))
     return launches
 

@@ -391,11 +391,20 @@ def _selective_scan(gs, x, delta, a, b, c, *rest, softplus, kept, has_d, has_gat
     return tuple(grads)
 
 
+def _with_parts(eqn):
+    '''The gradient of log probabilities from weights takes the same operands apart: the equation with them as results too.'''
+    if eqn.params['parts'] or 0 in eqn.invars[0].aval.shape:
+        return eqn
+    parts = [core.Var(None, '', a) for a in lax._linear_log_probs_parts(eqn.invars[0].aval, eqn.invars[1].aval, eqn.params['transposed'])]
+    return core.JaxprEqn(eqn.invars, list(eqn.outvars) + parts, eqn.primitive, dict(eqn.params, parts=True))
+
+
 @_rule('linear_log_probs')
-def _linear_log_probs(gs, x, weights, tokens, outs, transposed):
+def _linear_log_probs(gs, x, weights, tokens, outs, transposed, parts):
     if gs[2] is not None or gs[3] is not None:
         raise NotImplementedError('differentiation through the largest scores and the sums of linear_log_probs')
-    return lax.linear_log_probs_grad(x, weights, tokens, outs[2], outs[3], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), transposed) + (None,)
+    return lax.linear_log_probs_grad(x, weights, tokens, outs[2], outs[3], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), transposed,
+                                     tuple(outs[4:]) if parts else None) + (None,)
 
 
 _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', 'iota', 'and', 'or', 'not', 'xor', 'sign', 'floor', 'ceil',
@@ -406,7 +415,7 @@ _NOT_DIFFERENTIABLE = {'gt', 'ge', 'lt', 'le', 'eq', 'ne', 'argmax', 'argmin', '
 # ---------------------------------------------------------------- driver
 
 #what becomes of equations whose backward pass needs more than their results
-_FOR_GRADIENTS = {'token_log_probs': _with_log_sum_rest, 'selective_scan': _with_kept_states}
+_FOR_GRADIENTS = {'token_log_probs': _with_log_sum_rest, 'selective_scan': _with_kept_states, 'linear_log_probs': _with_parts}
 
 
 def _replay(jaxpr, consts, inputs, env, order):

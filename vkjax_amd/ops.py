@@ -1231,11 +1231,14 @@ def selective_scan_grad(bufferpool, equation):
 
 
 def linear_log_probs(bufferpool, equation):
-    (x, weights, tokens), outs, scratch = _operator_buffers(bufferpool, equation)
+    p = equation.params
+    (x, weights, tokens), (log_probs, log_sums, peaks, totals, *parts), scratch = _operator_buffers(bufferpool, equation)
     _float_operands(equation, x, weights)
     if _kind(tokens.dtype) not in (_I, _U):
         raise NotImplementedError(equation)
-    return _operator_ops(equation, K.linear_log_probs(*outs, x, weights, tokens, equation.params['transposed'], scratch))
+    if p.get('parts') and any(v is None for v in parts):
+        raise NotImplementedError(equation)
+    return _operator_ops(equation, K.linear_log_probs(log_probs, log_sums, peaks, totals, x, weights, tokens, p['transposed'], scratch, parts or None))
 
 
 def linear_log_probs_grad(bufferpool, equation):
@@ -1243,6 +1246,7 @@ def linear_log_probs_grad(bufferpool, equation):
     (x, weights, tokens, peaks, totals, *rest), (dx, dweights), scratch = _operator_buffers(bufferpool, equation)
     g_log_probs = rest.pop(0) if p['has_log_probs'] else None
     g_log_sums  = rest.pop(0) if p['has_log_sums'] else None
+    parts       = rest if p.get('has_parts') else None
     _float_operands(equation, x, weights, peaks, totals, g_log_probs, g_log_sums)
     if _kind(tokens.dtype) not in (_I, _U):
         raise NotImplementedError(equation)
@@ -1251,7 +1255,7 @@ def linear_log_probs_grad(bufferpool, equation):
     if dx is None or dweights is None:
         dx       = dx if dx is not None else scratch(x.shape)
         dweights = dweights if dweights is not None else scratch(weights.shape)
-    return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch))
+    return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch, parts))
 
 
 def orthogonalize(bufferpool, equation):
