@@ -102,12 +102,13 @@ template <int N> __device__ __forceinline__ void loads_left() { __builtin_amdgcn
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); asm volatile("" ::: "memory"); }
 #define HALF_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-// The sums of tile (m, n) over `pairs` pairs of steps (one at least) from pair `begin` on. With more than two buffers a wave has the parts of the next step in registers before it
+// The sums of tile (m, n) over `pairs` pairs of steps from pair `begin` on. With more than two buffers a wave has the parts of the next step in registers before it
 // multiplies those of this one: the barrier in front of a pair stands between the two steps of the pair before.
 template <int T, int STAGES>
 __device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs) {
     static_assert(STAGES == 2 || STAGES == 4, "as many pairs are on their way as meet() counts");
     constexpr int LOADS = 4 * T;                         // of a wave per stage
+    if (pairs == 0u) return;                             // (a slice of nothing)
     uint32_t asked = 0u;                                 // pairs that have been requested
     auto request = [&](uint32_t at) { half_request<T>(shared.stages[at], a, b, m, n, 2u * (begin + asked)); ++asked; };
     // pair p has arrived, for all waves (those asked for behind it may be on their way); and all have read what they wanted of the pair before the last

@@ -59,7 +59,16 @@ extern "C" __global__ __launch_bounds__(256) void linear_largest(float* __restri
                 factors[3u * r] = m; factors[3u * r + 1u] = plain ? all / m : 0.f; factors[3u * r + 2u] = plain ? lp / m : 0.f;
             }
             float row = 0.f;
-            if (given) for (uint32_t h = lane; h < P.H; h += 64u) row = fmaxf(row, magnitude(x[(uint64_t)r * P.H + h]));
+            const float* const from = x + (uint64_t)r * P.H;
+            if (given) {
+                uint32_t h = 4u * lane;
+                for (; h + 4u <= P.H; h += 256u) {
+                    const f32x4 v = *reinterpret_cast<const f32x4_anywhere*>(from + h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) row = fmaxf(row, magnitude(v[e]));
+                }
+                for (uint32_t e = 0; e < 4u; ++e) if (h + e < P.H) row = fmaxf(row, magnitude(from[h + e]));
+            }
             one = fmaxf(one, row); two = fmaxf(two, magnitude(row * m));
         }
     one = wave_largest(one); two = wave_largest(two);
@@ -277,7 +286,9 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
         return t;
     };
     if constexpr (ALONG_V) {
-        f32x4 ws[2][4], xs[2][NT];
+        // (DEPTH - 1 groups are on their way while one is multiplied)
+        constexpr uint32_t DEPTH = 4u;
+        f32x4 ws[DEPTH][4], xs[DEPTH][NT];
         auto request = [&](f32x4 (&wv)[4], f32x4 (&xv)[NT], uint32_t g) {
             const uint32_t h0 = g * 8u + 4u * half;
 #pragma unroll
@@ -293,13 +304,14 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
 #pragma unroll
                     for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(wv[q][i], xv[j][q], acc[i][j], 0, 0, 0);
         };
-        if (begin < end) request(ws[0], xs[0], begin);
-        for (uint32_t g = begin; g < end; g += 2u) {
-            if (g + 1u < end) request(ws[1], xs[1], g + 1u);
-            multiply(ws[0], xs[0]);
-            if (g + 2u < end) request(ws[0], xs[0], g + 2u);
-            if (g + 1u < end) multiply(ws[1], xs[1]);
-        }
+#pragma unroll
+        for (uint32_t k = 0; k < DEPTH - 1u; ++k) if (begin + k < end) request(ws[k], xs[k], begin + k);
+        for (uint32_t g = begin; g < end; g += DEPTH)
+#pragma unroll
+            for (uint32_t k = 0; k < DEPTH; ++k) {
+                if (g + k + DEPTH - 1u < end) request(ws[(k + DEPTH - 1u) % DEPTH], xs[(k + DEPTH - 1u) % DEPTH], g + k + DEPTH - 1u);
+                if (g + k < end) multiply(ws[k], xs[k]);
+            }
     } else {
         for (uint32_t g = begin; g < end; ++g) {
             const uint32_t h0 = g * 32u + 16u * half;
@@ -418,41 +430,66 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_q(u32x4* __restrict_
     });
 }
 
-// ---- a product of two operands to fp32 [M, N], rows by a factor each (every third word), slices of the contraction to arrays of their own
+// ---- a product of two operands to fp32 [M, N], rows by a factor each (every third word), added to what is there or in its place; not SHARED: a slice of the contraction to an array of its own
 struct ProductParams {
-    uint32_t M, N, tiles_m, tiles_n, slices, pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b;
+    uint32_t M, N, tiles_m, tiles_n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b, add;
     int32_t scale_a, scale_b;                            // the kind of operand whose scale it is, or -1: q
-    uint64_t ld, slice;                                  // elements from a row, a slice of the result to the next
+    HalfShares shares;
+    uint64_t ld, slice;                                  // elements from a row of the result to the next, from a slice's result to the next one's
 };
-extern "C" __global__ __launch_bounds__(256, 2) void linear_product(float* __restrict__ out, const u32x4* __restrict__ a, const u32x4* __restrict__ b, const int32_t* __restrict__ scales,
-                                                                    const float* __restrict__ factors, ProductParams P) {
-    __shared__ HalfShared<2, 2> shared;
-    uint32_t m, n;
-    const uint32_t tiles = P.tiles_m * P.tiles_n, slice = blockIdx.x / tiles;
-    half_tile(half_turn(blockIdx.x - slice * tiles, tiles), P.tiles_m, P.tiles_n, m, n);
-    const uint32_t begin = (uint32_t)((uint64_t)P.pairs * slice / P.slices), end = (uint32_t)((uint64_t)P.pairs * (slice + 1u) / P.slices);
-    HalfSums<2> acc = {};
-    half_product<2, 2>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
+template <int T, int STAGES, bool SHARED>
+__device__ __forceinline__ void linear_product_body(float* __restrict__ out, float* __restrict__ partial, uint32_t* __restrict__ arrivals, const u32x4* __restrict__ a, const u32x4* __restrict__ b,
+                                                    const int32_t* __restrict__ scales, const float* __restrict__ factors, const ProductParams& P) {
+    __shared__ HalfShared<T, STAGES> shared;
+    uint32_t m, n, tile, slice, begin, end;
+    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_tile(tile, P.tiles_m, P.tiles_n, m, n);
+    HalfSums<T> acc = {};
+    half_product<T, STAGES>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t lane_row = (m * 2u + (wave >> 1)) * 32u * T + 4u * (lane >> 5), lane_column = (n * 2u + (wave & 1u)) * 32u * T + (lane & 31u);
     const float down = power_of_two(-(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a])), down_b = power_of_two(-(P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]));
-    float* const to = out + P.slice * slice;
+    float* const to = out + (SHARED ? 0u : P.slice * slice);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < T; ++i) {
+        // (what is there is asked for at once, in front of the stores)
+        float before[T][16] = {};
+        if (P.add)
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+#pragma unroll
+                for (int j = 0; j < T; ++j) {
+                    const uint32_t row = lane_row + 32u * i + 8u * (q >> 2) + (q & 3), column = lane_column + 32u * j;
+                    if (row < P.M && column < P.N) before[j][q] = to[P.ld * row + column];
+                }
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            const uint32_t row = m * 128u + wm * 64u + 32u * i + 8u * (q >> 2) + 4u * (lane >> 5) + (q & 3);
+            const uint32_t row = lane_row + 32u * i + 8u * (q >> 2) + (q & 3);
             if (row >= P.M) continue;
             const float f = factors ? factors[3u * row] : 1.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t column = n * 128u + wn * 64u + 32u * j + (lane & 31u);
-                if (column < P.N) {
-                    const float s = half_sum(acc, i, j, q) * down * down_b;
-                    to[P.ld * row + column] = factors ? (f == 0.f ? 0.f : s * f) : s;
-                }
+            for (int j = 0; j < T; ++j) {
+                const uint32_t column = lane_column + 32u * j;
+                if (column >= P.N) continue;
+                float s = half_sum(acc, i, j, q) * down * down_b;
+                if (factors) s = f == 0.f ? 0.f : s * f;
+                to[P.ld * row + column] = s + before[j][q];
             }
         }
+    }
 }
+#define LINEAR_PRODUCT(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                               \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_product##SUFFIX(float* out, float* partial, uint32_t* arrivals, const u32x4* a, const u32x4* b,    \
+                                                                                     const int32_t* scales, const float* factors, ProductParams P) {                    \
+        linear_product_body<T, STAGES, SHARED>(out, partial, arrivals, a, b, scales, factors, P);                                                                       \
+    }
+LINEAR_PRODUCT(_128, 2, 2, 2, false)
+LINEAR_PRODUCT(_128_shared, 2, 2, 2, true)
+LINEAR_PRODUCT(_64, 1, 4, 2, false)
+LINEAR_PRODUCT(_64_shared, 1, 4, 2, true)
+LINEAR_PRODUCT(_64_many, 1, 2, 4, false)
+LINEAR_PRODUCT(_64_many_shared, 1, 2, 4, true)
 
 struct SumParams { uint32_t parts, pad; uint64_t n; };
 extern "C" __global__ __launch_bounds__(256) void linear_sum(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {

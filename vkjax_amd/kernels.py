@@ -2708,7 +2708,6 @@ def selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept: 
 # ---------------------------------------------------------------- products on the fp16 matrix cores (half_product.h)
 
 HALF_TILE = 128                         #rows and columns of a block's tile
-HALF_BLOCKS = 512                       #blocks of such tiles that the machine runs at once
 
 
 def _half_steps(k: int) -> int:
@@ -2725,11 +2724,49 @@ def _u64(*values) -> bytes:
     return np.asarray([int(v) for v in values], dtype=np.uint64).tobytes()
 
 
+class HalfPlan(tp.NamedTuple):
+    '''How a product is shared out (half_product.h): tiles of `side`, the first `whole` of them by a block each, the contraction of those behind by `slices` blocks.'''
+    kernel: str
+    side:   int
+    whole:  int
+    slices: int
+
+
+def half_plan(tiles_of, pairs: int) -> HalfPlan:
+    '''The plan with the smallest estimated time (us) for tiles_of(side) tiles and a contraction of so many pairs of steps.'''
+    best = None
+    for kernel, side, blocks_of_cu, start, pair, unit in HALF_KERNELS:
+        tiles, slots = tiles_of(side), HALF_CUS * blocks_of_cu
+
+        def time(blocks, pairs):
+            #full rounds of the machine, then one of fewer blocks to a CU
+            full, rest = divmod(blocks, slots)
+            return full * (start + pairs * max(pair, blocks_of_cu * unit)) + (start + pairs * max(pair, _cdiv(rest, HALF_CUS) * unit) if rest else 0)
+        for slices in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64):
+            whole = tiles if slices == 1 else tiles // slots * slots
+            if slices > 1 and (slices * HALF_SLICE_PAIRS > pairs or whole == tiles):
+                continue
+            cost = time(whole, pairs)
+            if whole < tiles:
+                cost += time((tiles - whole) * slices, _cdiv(pairs, slices)) + (HALF_JOIN + HALF_JOIN_SLICE * slices) * (side / 128)**2
+            if best is None or cost < best[0]:
+                best = (cost, HalfPlan(kernel, side, whole, slices))
+    return best[1]
+
+
+HALF_CUS = 256
+#kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps at least, us of a CU for one), by measurement: products of 512 x 512 x 512 alone 18.5,
+#11.0 and 11.7 us, of 512 x 512 x 4096 96, 53 and 64, of 2048^3 64, 84 and 67, 192 tiles of 128 x 16 pairs 21, 21.6 and 18. (A pair with a block of 128 to a CU: 0.68 us from the caches near by,
+#1.1 in 4096 x 1024 x 8064)
+HALF_KERNELS = (('_128', 128, 2, 8.0, 0.90, 0.71), ('_64', 64, 2, 4.5, 0.38, 0.30), ('_64_many', 64, 4, 4.0, 0.47, 0.25))
+HALF_SLICE_PAIRS = 4                    #pairs of steps of a slice, at least
+HALF_JOIN, HALF_JOIN_SLICE = 12.0, 0.6  #us of adding up slices of tiles of 128, and for each of them
+
+
 # ---------------------------------------------------------------- log probabilities from weights (linear_log_probs.hip)
 
 LINEAR_ROWS       = 64                  #rows up to which the weights are read as they are
 LINEAR_PIECE      = 256 << 20           #bytes of the scores' cotangents that are there at a time
-LINEAR_SLICE      = 16                  #pairs of steps of a slice of a contraction, at least
 _PACK_WEIGHTS, _PACK_ROWS, _PACK_SCALED = 0, 1, 2
 
 
@@ -2758,7 +2795,7 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x) - or, where that has been done, with the weights' scale from `known` -, and with cotangents
     for those behind it, into (the weights contracted over the vocabulary, x with its rows' factors contracted over the rows, the factors), which are returned. Scales go to `scales`.'''
     rows, h, v = shape
-    row_blocks    = max(1, min(256, _cdiv(rows, 4)))
+    row_blocks    = max(1, min(1024, _cdiv(rows, 4)))
     weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if known is None else 0
     largest = scratch((weight_blocks + 2 * row_blocks,))
     factors = scratch((rows, 3)) if cotangents else None
@@ -2802,7 +2839,7 @@ def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, t
                               _u32(join_rows.bit_length() - 1, rows, v, tiles), bytes_moved=8 * tiles * rows, written=(0, 1, 2, 3))]
 
 
-def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch,
+def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch, zeroed,
                           parts=None) -> tp.List[Launch]:
     shape = rows, h, v = _linear_shape(x, w, transposed)
     scales = scratch((4,), np.int32)                       #of all that is taken apart here
@@ -2820,15 +2857,26 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
     pieces = _cdiv(all_tiles, each)
     width  = each * HALF_TILE
     by_row, by_token = scratch((row_blocks * (width // 16) * 512,), np.uint32), scratch((width // 32 * 2 * row_blocks * 512,), np.uint32)
-    tiles_r, tiles_h = _cdiv(rows, HALF_TILE), _cdiv(h, HALF_TILE)
-    slices = max(1, min(_cdiv(HALF_BLOCKS, tiles_r * tiles_h), width // 32 // LINEAR_SLICE))
-    parts  = scratch((pieces * slices, rows, h)) if pieces * slices > 1 else dx
+    tiles_r = _cdiv(rows, HALF_TILE)
 
-    def product(out, offset, a, b, m, n, k_pairs, slices, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b, scale_a, scale_b, ld, slice_, by_rows):
-        tiles = (_cdiv(m, HALF_TILE), _cdiv(n, HALF_TILE))
-        return Launch('linear_product', (tiles[0] * tiles[1] * slices, 1, 1), (BLOCK, 1, 1), [(out, 4 * offset), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
-                      _u32(m, n, *tiles, slices, k_pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b) + _i32(scale_a, scale_b) + _u64(ld, slice_),
-                      bytes_moved=4 * (m + n) * 32 * k_pairs + 4 * m * n * slices, flops=64 * m * n * k_pairs)
+    def product(out, offset, a, b, m, n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_b, scale_a, scale_b, ld, by_rows=False, add=False, parts=0):
+        #(parts: slices to arrays of their own)
+        plan  = HalfPlan('_128', HALF_TILE, 0, parts) if parts else half_plan(lambda side: _cdiv(m, side) * _cdiv(n, side), pairs)
+        rest  = _cdiv(m, plan.side) * _cdiv(n, plan.side) - plan.whole
+        share = plan.slices > 1 and not parts
+        partial, arrivals = (scratch((rest * plan.slices, plan.side, plan.side)), zeroed(rest, 'arrivals at tiles of halves')) if share else (None, None)
+        return Launch(f'linear_product{plan.kernel}{"_shared" if share else ""}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1),
+                      [(out, 4 * offset), (partial, 0), (arrivals, 0), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
+                      _u32(m, n, _cdiv(m, plan.side), _cdiv(n, plan.side), pairs, blocks_a, blocks_b, steps_a, steps_b, 0, first_b, add) + _i32(scale_a, scale_b)
+                      + _u32(plan.whole, plan.slices) + _u64(ld, m * n), bytes_moved=4 * (m + n) * 32 * pairs + 4 * m * n, flops=64 * m * n * pairs,
+                      written=(0, 1, 2) if share else (0,), scratch=(2,) if share else ())
+    #dx has few tiles and a long contraction: slices are added up by a launch of their own, not by the blocks that arrive last (321 x 500 over 50001 tokens: 105 + 8 us, 117; a piece of
+    #4096 x 1024 over 8064: 202 + 8, 241, in one slice 277)
+    tiles_x = tiles_r * _cdiv(h, HALF_TILE)
+    parts   = 2 * HALF_CUS // tiles_x if tiles_x <= HALF_CUS else 0
+    parts   = min(parts, width // 32 // HALF_SLICE_PAIRS)
+    sums    = scratch((parts, rows, h)) if parts > 1 else dx
+    parts   = parts if parts > 1 else 0
     for piece in range(pieces):
         first = piece * each
         tiles = min(each, all_tiles - first)
@@ -2836,16 +2884,15 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         launches.append(Launch('linear_q', (tiles * tiles_r, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors)],
                                _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, tiles_r, _cdiv(v, 32), row_blocks, first, width, 0),
                                bytes_moved=8 * 32 * row_blocks * width, flops=2 * rows * h * n, written=(0, 1)))
-        launches.append(product(parts, piece * slices * rows * h, by_row, w_by_h, rows, h, _cdiv(n, 32), slices, row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), 0, v0 // 16,
-                                -1, _PACK_WEIGHTS, h, rows * h, True))
-        scaled, q = (x_scaled, _cdiv(h, 32), 2 * row_blocks), (by_token, tiles * 4, 2 * row_blocks)
+        launches.append(product(sums, 0, by_row, w_by_h, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), v0 // 16, -1, _PACK_WEIGHTS, h,
+                                by_rows=True, add=piece > 0, parts=parts))
+        steps = 2 * row_blocks
         if transposed:
-            launches.append(product(dw, v0 * h, q[0], scaled[0], n, h, row_blocks, 1, q[1], scaled[1], q[2], scaled[2], 0, 0, -1, _PACK_SCALED, h, 0, False))
+            launches.append(product(dw, v0 * h, by_token, x_scaled, n, h, row_blocks, tiles * 4, _cdiv(h, 32), steps, steps, 0, -1, _PACK_SCALED, h))
         else:
-            launches.append(product(dw, v0, scaled[0], q[0], h, n, row_blocks, 1, scaled[1], q[1], scaled[2], q[2], 0, 0, _PACK_SCALED, -1, v, 0, False))
-    if pieces * slices > 1:
-        launches.append(Launch('linear_sum', (_cdiv(rows * h, BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (parts, 0)], _u32(pieces * slices, 0) + _u64(rows * h),
-                               bytes_moved=4 * (parts.size + rows * h)))
+            launches.append(product(dw, v0, x_scaled, by_token, h, n, row_blocks, _cdiv(h, 32), tiles * 4, steps, steps, 0, _PACK_SCALED, -1, v))
+    if parts:
+        launches.append(Launch('linear_sum', (_cdiv(rows * h, BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (sums, 0)], _u32(parts, 0) + _u64(rows * h), bytes_moved=4 * (sums.size + rows * h)))
     return launches
 
 
@@ -2870,44 +2917,6 @@ def orthogonal_bounds(steps: int, coefficients) -> tp.List[tp.Tuple[float, float
 def _half_scale(largest: float) -> int:
     '''The power of two that brings numbers up to `largest` below 2^15.'''
     return 15 - int(math.frexp(largest)[1])
-
-
-class HalfPlan(tp.NamedTuple):
-    '''How a product is shared out (half_product.h): tiles of `side`, the first `whole` of them by a block each, the contraction of those behind by `slices` blocks.'''
-    kernel: str
-    side:   int
-    whole:  int
-    slices: int
-
-
-def half_plan(tiles_of, pairs: int) -> HalfPlan:
-    '''The plan with the smallest estimated time (us) for tiles_of(side) tiles and a contraction of so many pairs of steps.'''
-    best = None
-    for kernel, side, blocks_of_cu, start, pair, unit in HALF_KERNELS:
-        tiles, slots = tiles_of(side), HALF_CUS * blocks_of_cu
-
-        def time(blocks, pairs):
-            #full rounds of the machine, then one of fewer blocks to a CU
-            full, rest = divmod(blocks, slots)
-            return full * (start + pairs * max(pair, blocks_of_cu * unit)) + (start + pairs * max(pair, _cdiv(rest, HALF_CUS) * unit) if rest else 0)
-        for slices in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32):
-            whole = tiles if slices == 1 else tiles // slots * slots
-            if slices > 1 and (slices * HALF_SLICE_PAIRS > pairs or whole == tiles):
-                continue
-            cost = time(whole, pairs)
-            if whole < tiles:
-                cost += time((tiles - whole) * slices, _cdiv(pairs, slices)) + HALF_JOIN + HALF_JOIN_SLICE * slices * (side / 128)**2
-            if best is None or cost < best[0]:
-                best = (cost, HalfPlan(kernel, side, whole, slices))
-    return best[1]
-
-
-HALF_CUS = 256
-#kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps at least, us of a CU for one), by measurement: products of 512 x 512 x 512 alone 18.5,
-#11.0 and 11.7 us, of 512 x 512 x 4096 96, 53 and 64, of 2048^3 64, 84 and 67, 192 tiles of 128 x 16 pairs 21, 21.6 and 18
-HALF_KERNELS = (('_128', 128, 2, 8.0, 0.68, 0.71), ('_64', 64, 2, 4.5, 0.38, 0.30), ('_64_many', 64, 4, 4.0, 0.47, 0.25))
-HALF_SLICE_PAIRS = 4                    #pairs of steps of a slice, at least
-HALF_JOIN, HALF_JOIN_SLICE = 3.0, 0.6   #us of adding up slices, and for each of them
 
 
 def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, scratch, zeroed) -> tp.List[Launch]:

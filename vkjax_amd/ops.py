@@ -1255,7 +1255,8 @@ def linear_log_probs_grad(bufferpool, equation):
     if dx is None or dweights is None:
         dx       = dx if dx is not None else scratch(x.shape)
         dweights = dweights if dweights is not None else scratch(weights.shape)
-    return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch, parts))
+    return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch,
+                                                            bufferpool.zeroed_scratch, parts))
 
 
 def orthogonalize(bufferpool, equation):
