@@ -61,9 +61,10 @@ struct Place {
         length = sequence_length(lengths, b, P.T);
         begin = (int)(chunk * P.chunk); end = min(begin + (int)P.chunk, (int)P.T); stop = min(end, length);
     }
-    __device__ int64_t row(const ScanParams& P, int t) const { return ((int64_t)b * P.T + t) * P.C + c; }
-    // element of state i in [chunk or kept number][B][N][C]
-    __device__ int64_t held(const ScanParams& P, uint32_t number, int i) const { return (((int64_t)number * P.B + b) * P.N + n0 + i) * P.C + c; }
+    // a step's row of an array [B, T, C] (where it begins is the wave's, so that a lane's part of an address is its channel)
+    template <class V> __device__ V* row(V* p, const ScanParams& P, int t) const { return p + ((int64_t)b * P.T + t) * P.C; }
+    // state i's row in [chunk or kept number][B][N][C]
+    template <class V> __device__ V* held(V* p, const ScanParams& P, uint32_t number, int i) const { return p + (((int64_t)number * P.B + b) * P.N + n0 + i) * P.C; }
     __device__ int64_t state(const ScanParams& P, int i) const { return ((int64_t)b * P.C + c) * P.N + n0 + i; }
     __device__ bool has(const ScanParams& P, int i) const { return n0 + i < P.N; }
     __device__ int own(int q) const { return (int)wave * OWN + q; }
@@ -103,8 +104,8 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
     auto request = [&](int t0) {
 #pragma unroll
         for (int q = 0; q < at.OWN; ++q) {
-            const int64_t row = at.row(P, min(t0 + at.own(q), at.stop - 1));
-            xs[q] = x[row]; ds[q] = delta[row];
+            const int t = min(t0 + at.own(q), at.stop - 1);
+            xs[q] = at.row(x, P, t)[at.c]; ds[q] = at.row(delta, P, t)[at.c];
         }
         mapped = at.staged(bmap, P, t0);
     };
@@ -140,7 +141,7 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
     if (at.wave == 0u) sums[((int64_t)at.chunk * P.B + at.b) * P.C + at.c] = sum;
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-        if (at.has(P, i)) states[at.held(P, at.chunk, i)] = h[i];
+        if (at.has(P, i)) at.held(states, P, at.chunk, i)[at.c] = h[i];
 }
 
 // ---- the state in front of every chunk, in the place of its state from zero; the same for the adjoint from the last chunk on, and the initial state's cotangent
@@ -183,16 +184,16 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
     float a2[NS], h[NS], mapped[2];
     at.factors(a2, a, P);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) h[i] = !at.has(P, i) ? 0.f : states ? states[at.held(P, at.chunk, i)] : state ? state[at.state(P, i)] : 0.f;
+    for (int i = 0; i < NS; ++i) h[i] = !at.has(P, i) ? 0.f : states ? at.held(states, P, at.chunk, i)[at.c] : state ? state[at.state(P, i)] : 0.f;
     const float add = bias ? bias[at.c] : 0.f, D = through ? through[at.c] : 0.f;
     const bool stream = streams_result(P.first);
     float xs[at.OWN], ds[at.OWN], gs[at.OWN];
     auto request = [&](int t0) {
 #pragma unroll
         for (int q = 0; q < at.OWN; ++q) {
-            const int64_t row = at.row(P, min(t0 + at.own(q), at.stop - 1));
-            xs[q] = x[row]; ds[q] = delta[row];
-            if (gate) gs[q] = gate[row];
+            const int t = min(t0 + at.own(q), at.stop - 1);
+            xs[q] = at.row(x, P, t)[at.c]; ds[q] = at.row(delta, P, t)[at.c];
+            if (gate) gs[q] = at.row(gate, P, t)[at.c];
         }
         mapped[0] = at.staged(bmap, P, t0); mapped[1] = at.staged(cmap, P, t0);
     };
@@ -201,7 +202,7 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
         if (kept && at.there)
 #pragma unroll
             for (int i = 0; i < NS; ++i)
-                if (at.has(P, i)) kept[at.held(P, (uint32_t)t0 / KEPT, i)] = h[i];
+                if (at.has(P, i)) at.held(kept, P, (uint32_t)t0 / KEPT, i)[at.c] = h[i];
         float ys[at.OWN], open[at.OWN];
         if (t0 < at.stop) {
 #pragma unroll
@@ -250,7 +251,7 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
                 const int t = t0 + at.own(q);
                 if (t >= at.end) continue;
                 const float v = t < at.stop ? ys[q] : 0.f;
-                if (stream) __builtin_nontemporal_store(v, y + at.row(P, t)); else y[at.row(P, t)] = v;
+                if (stream) __builtin_nontemporal_store(v, at.row(y, P, t) + at.c); else at.row(y, P, t)[at.c] = v;
             }
     }
     if (last && at.there && at.chunk == P.chunks - 1u)
@@ -325,9 +326,9 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
     auto request = [&](int t0) {
 #pragma unroll
         for (int q = 0; q < at.OWN; ++q) {
-            const int64_t row = at.row(P, min(t0 + at.own(q), at.stop - 1));
-            ds[q] = delta[row]; gs[q] = g ? g[row] : 0.f;
-            if (gate) gates[q] = gate[row];
+            const int t = min(t0 + at.own(q), at.stop - 1);
+            ds[q] = at.row(delta, P, t)[at.c]; gs[q] = g ? at.row(g, P, t)[at.c] : 0.f;
+            if (gate) gates[q] = at.row(gate, P, t)[at.c];
         }
         mapped = at.staged(cmap, P, t0);
     };
@@ -362,38 +363,23 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
     if (at.wave == 0u) sums[((int64_t)at.chunk * P.B + at.b) * P.C + at.c] = sum;
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-        if (at.has(P, i)) states[at.held(P, at.chunk, i)] = l[i];
+        if (at.has(P, i)) at.held(states, P, at.chunk, i)[at.c] = l[i];
 }
 
-// Sums over a wave's channels of NS values per lane: a step of the butterfly leaves a lane half of them, then all lanes that have the same one add up. A lane has value `index` in
-// the end; of those that have it, one stores it.
-template <int NS>
-struct OverChannels {
-    uint32_t lane, index; bool stores;
-    __device__ OverChannels() {
-        lane = threadIdx.x & 63u;
-        // (bit 5 of the lane says which half of the values, bit 4 which half of that, ..)
-        index  = NS == 8 ? lane >> 3 : lane >> 4;
-        stores = (lane & (NS == 8 ? 7u : 15u)) == 0u;
-    }
-    __device__ float sum(float (&v)[NS]) const {
-        static_assert(NS == 8 || NS == 4, "");
-        // (in the lower half of the lanes both halves' v[i], in the upper one v[i + NS / 2])
+// Sums over a wave's channels of eight values per lane (of eight states, or of two steps' four): a step of the butterfly leaves a lane half of them, then the eight lanes that have the
+// same one add up. A lane has value lane / 8 in the end; of those that have it the first stores it.
+__device__ __forceinline__ float over_channels(float (&v)[8]) {
+    // (in the lower half of the lanes both halves' v[i], in the upper one v[i + 4])
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i) { const auto r = __builtin_amdgcn_permlane32_swap(f2u(v[i]), f2u(v[i + NS / 2]), false, false); v[i] = u2f(r[0]) + u2f(r[1]); }
+    for (int i = 0; i < 4; ++i) { const auto r = __builtin_amdgcn_permlane32_swap(f2u(v[i]), f2u(v[i + 4]), false, false); v[i] = u2f(r[0]) + u2f(r[1]); }
 #pragma unroll
-        for (int i = 0; i < NS / 4; ++i) { const auto r = __builtin_amdgcn_permlane16_swap(f2u(v[i]), f2u(v[i + NS / 4]), false, false); v[i] = u2f(r[0]) + u2f(r[1]); }
-        float s = v[0];
-        if constexpr (NS == 8) {
-            const bool upper = (lane & 8u) != 0u;
-            s = (upper ? v[1] : v[0]) + lane_xor<8>(upper ? v[0] : v[1]);
-        }
-        else s += lane_xor<8>(s);
-        s += lane_xor<4>(s);
-        s += lane_xor<2>(s);
-        return s + lane_xor<1>(s);
-    }
-};
+    for (int i = 0; i < 2; ++i) { const auto r = __builtin_amdgcn_permlane16_swap(f2u(v[i]), f2u(v[i + 2]), false, false); v[i] = u2f(r[0]) + u2f(r[1]); }
+    const bool upper = (threadIdx.x & 8u) != 0u;
+    float s = (upper ? v[1] : v[0]) + lane_xor<8>(upper ? v[0] : v[1]);
+    s += lane_xor<4>(s);
+    s += lane_xor<2>(s);
+    return s + lane_xor<1>(s);
+}
 
 // ---- the gradient of a chunk
 template <int NS, int M>
@@ -406,11 +392,13 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
     __shared__ float prepared[3][KEPT][64], parts[M][3][KEPT][64], mapped[2][KEPT][NS * M];
     __shared__ __attribute__((aligned(16))) float map[2][KEPT][NS * M];
     const Place<NS, M> at(P, lengths);
-    const OverChannels<NS> over;
+    constexpr int AT_ONCE = 8 / NS;                  // steps whose sums over channels go together
+    const uint32_t over = at.lane >> 3;              // the value of those that a lane has
+    const bool over_stores = (at.lane & 7u) == 0u;
     float a2[NS], l[NS], da[NS] = {}, dD = 0.f, dbias = 0.f;
     at.factors(a2, a, P);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) l[i] = !at.has(P, i) ? 0.f : adjoints ? adjoints[at.held(P, at.chunk, i)] : g_last ? g_last[at.state(P, i)] : 0.f;
+    for (int i = 0; i < NS; ++i) l[i] = !at.has(P, i) ? 0.f : adjoints ? at.held(adjoints, P, at.chunk, i)[at.c] : g_last ? g_last[at.state(P, i)] : 0.f;
     const float add = bias ? bias[at.c] : 0.f, D = through ? through[at.c] : 0.f;
     const int turns = (at.end - at.begin + KEPT - 1) / KEPT;
     const bool stream = streams_result(P.first);
@@ -418,12 +406,12 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
     auto request = [&](int t0) {
 #pragma unroll
         for (int q = 0; q < at.OWN; ++q) {
-            const int64_t row = at.row(P, min(t0 + at.own(q), at.stop - 1));
-            rx[q] = x[row]; rd[q] = delta[row]; rg[q] = g ? g[row] : 0.f;
-            if (gate) rz[q] = gate[row];
+            const int t = min(t0 + at.own(q), at.stop - 1);
+            rx[q] = at.row(x, P, t)[at.c]; rd[q] = at.row(delta, P, t)[at.c]; rg[q] = g ? at.row(g, P, t)[at.c] : 0.f;
+            if (gate) rz[q] = at.row(gate, P, t)[at.c];
         }
 #pragma unroll
-        for (int i = 0; i < NS; ++i) rh[i] = at.has(P, i) ? kept[at.held(P, (uint32_t)t0 / KEPT, i)] : 0.f;
+        for (int i = 0; i < NS; ++i) rh[i] = at.has(P, i) ? at.held(kept, P, (uint32_t)t0 / KEPT, i)[at.c] : 0.f;
         rmap[0] = at.staged(bmap, P, t0); rmap[1] = at.staged(cmap, P, t0);
     };
     bool requested = false;
@@ -459,47 +447,57 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             at.maps(next_b, map[0], 0);
             at.maps(next_c, map[1], 0);
 #pragma unroll
-            for (int s = 0; s < KEPT; ++s) {
+            for (int s0 = 0; s0 < KEPT; s0 += AT_ONCE) {
+                float part[8];
 #pragma unroll
-                for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
-                float part[NS], seen = 0.f;
-                const float u = dt[s] * xs[s];
+                for (int g = 0; g < AT_ONCE; ++g) {
+                    const int s = s0 + g;
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    before[s][i] = h[i];
-                    h[i] = __builtin_fmaf(exp2_of(a2[i] * dt[s]), h[i], u * bs[i]);
-                    part[i] = gy[s] * h[i];
-                    seen = __builtin_fmaf(cs[i], h[i], seen);
+                    for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
+                    if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
+                    const float u = dt[s] * xs[s];
+                    float seen = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        before[s][i] = h[i];
+                        h[i] = __builtin_fmaf(exp2_of(a2[i] * dt[s]), h[i], u * bs[i]);
+                        part[g * NS + i] = gy[s] * h[i];
+                        seen = __builtin_fmaf(cs[i], h[i], seen);
+                    }
+                    parts[at.wave][0][s][at.lane] = seen;
                 }
-                if (gate) parts[at.wave][0][s][at.lane] = seen;
-                const float sum = over.sum(part);
-                if (over.stores) mapped[1][s][at.n0 + over.index] = sum;
+                const float sum = over_channels(part);
+                if (over_stores) mapped[1][s0 + over / NS][at.n0 + over % NS] = sum;
                 STEP_FENCE();
             }
             at.maps(next_b, map[0], KEPT - 1);
             at.maps(next_c, map[1], KEPT - 1);
 #pragma unroll
-            for (int s = KEPT - 1; s >= 0; --s) {
+            for (int s0 = KEPT - AT_ONCE; s0 >= 0; s0 -= AT_ONCE) {
+                float part[8];
 #pragma unroll
-                for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                if (s > 0) { at.maps(next_b, map[0], s - 1); at.maps(next_c, map[1], s - 1); }
-                float part[NS], lb = 0.f, ea = 0.f;
-                const float u = dt[s] * xs[s];
+                for (int g = AT_ONCE - 1; g >= 0; --g) {
+                    const int s = s0 + g;
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    l[i] = __builtin_fmaf(gy[s], cs[i], l[i]);
-                    lb = __builtin_fmaf(l[i], bs[i], lb);
-                    part[i] = l[i] * u;
-                    l[i] *= exp2_of(a2[i] * dt[s]);
-                    const float e = l[i] * before[s][i];
-                    ea = __builtin_fmaf(e, a2[i], ea);
-                    da[i] = __builtin_fmaf(e, dt[s], da[i]);
+                    for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
+                    if (s > 0) { at.maps(next_b, map[0], s - 1); at.maps(next_c, map[1], s - 1); }
+                    const float u = dt[s] * xs[s];
+                    float lb = 0.f, ea = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        l[i] = __builtin_fmaf(gy[s], cs[i], l[i]);
+                        lb = __builtin_fmaf(l[i], bs[i], lb);
+                        part[g * NS + i] = l[i] * u;
+                        l[i] *= exp2_of(a2[i] * dt[s]);
+                        const float e = l[i] * before[s][i];
+                        ea = __builtin_fmaf(e, a2[i], ea);
+                        da[i] = __builtin_fmaf(e, dt[s], da[i]);
+                    }
+                    parts[at.wave][1][s][at.lane] = lb;
+                    parts[at.wave][2][s][at.lane] = ea;
                 }
-                parts[at.wave][1][s][at.lane] = lb;
-                parts[at.wave][2][s][at.lane] = ea;
-                const float sum = over.sum(part);
-                if (over.stores) mapped[0][s][at.n0 + over.index] = sum;
+                const float sum = over_channels(part);
+                if (over_stores) mapped[0][s0 + over / NS][at.n0 + over % NS] = sum;
                 STEP_FENCE();
             }
             at.meet();
@@ -525,8 +523,10 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 const int t = t0 + at.own(q);
                 if (t >= at.end) continue;
                 const bool taken = t < at.stop;
-                const int64_t row = at.row(P, t);
-                auto put = [&](float* p, float v) { if (p) { if (stream) __builtin_nontemporal_store(taken ? v : 0.f, p + row); else p[row] = taken ? v : 0.f; } };
+                auto put = [&](float* p, float v) {
+                    if (!p) return;
+                    if (stream) __builtin_nontemporal_store(taken ? v : 0.f, at.row(p, P, t) + at.c); else at.row(p, P, t)[at.c] = taken ? v : 0.f;
+                };
                 put(dx, vx[q]); put(ddelta, vd[q]); put(dgate, vz[q]);
             }
         // [strip][B][T][2 N]
@@ -536,7 +536,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             if (t >= at.end) break;
             maps[(((uint64_t)at.strip * P.B + at.b) * P.T + (uint32_t)t) * 2u * P.N + n] = t >= at.stop ? 0.f : n < P.N ? mapped[0][s][n] : mapped[1][s][n - P.N];
         }
-        at.meet();
+        // (what is read here is written again behind the next meeting, what the next turn writes in front of that was read in front of the last one)
     }
     // [B chunks][N + 2][C]
     prepared[0][at.wave][at.lane] = dD;
