@@ -10,7 +10,9 @@ import pytest
 from tests.test_gpu_operators import U, both, close
 from tests.test_operators import normal
 from tests.test_token_model_operators import OPTIONAL, loss_program, scan_inputs, scan_program
+from oracle import primitives as P
 from vkjax_amd import kernels as K, minijax as mj
+from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
 pytestmark = pytest.mark.gpu
 jnp, lax, nn = mj.numpy, mj.lax, mj.nn
@@ -406,3 +408,35 @@ def test_gradient_of_log_probs_with_and_without_the_operands_that_were_kept():
         return lax.linear_log_probs_grad(x, w, tokens, outs[2], outs[3], g, gs, parts=outs[4:]) + lax.linear_log_probs_grad(x, w, tokens, outs[2], outs[3], g, gs)
     (dx, dw, dx2, dw2), _, _ = both(both_ways, x, w, tokens, g, gs)
     assert np.array_equal(dx, dx2) and np.array_equal(dw, dw2)
+
+
+# ------------------------------------------------------------------ products whose contraction is shared
+
+@pytest.mark.parametrize('slices', [1, 2, 5, 40])
+@pytest.mark.parametrize('kernel,side', [(k[0], k[1]) for k in K.HALF_KERNELS])
+def test_products_that_share_contractions(kernel, side, slices, monkeypatch):
+    '''Several hundred blocks that leave parts of sums for one another: every kernel, some tiles by one block and the others shared, more slices than pairs of steps among them. The result does not
+    depend on who comes last.'''
+    print(f'shared contractions: {kernel}, {slices} slices', flush=True)
+    monkeypatch.setattr(K, 'half_plan', lambda tiles_of, pairs: K.HalfPlan(kernel, side, 0 if slices > 1 else tiles_of(side), min(slices, pairs)))
+    x = normal(1, 1100, 1300)
+    f = mj.make_jaxpr(lambda x: nn.orthogonalize(x, 1))(x)
+    program = JaxprInterpreter(f)
+    first, = program.run(x)
+    off = np.linalg.norm(first.astype(np.float64) - P.orthogonalize(x, 1, (3.4445, -4.7750, 2.0315), 1e-7))
+    assert off <= orthogonal_bound(x, 1, (3.4445, -4.7750, 2.0315)), off
+    for _ in range(4):
+        assert np.array_equal(program.run(x)[0], first)
+    y = normal(2, 1100, 1300)
+    other, = program.run(y)
+    assert np.linalg.norm(other.astype(np.float64) - P.orthogonalize(y, 1, (3.4445, -4.7750, 2.0315), 1e-7)) <= orthogonal_bound(y, 1, (3.4445, -4.7750, 2.0315))
+    assert np.array_equal(program.run(x)[0], first)
+
+
+def test_gradient_of_log_probs_with_shared_contractions(monkeypatch):
+    x, w, tokens, g, gs = loss_inputs(700, 300, 1500, False)
+    for kernel, side, *_ in K.HALF_KERNELS:
+        for slices in (1, 3):
+            print(f'gradient with shared contractions: {kernel}, {slices} slices', flush=True)
+            monkeypatch.setattr(K, 'half_plan', lambda tiles_of, pairs: K.HalfPlan(kernel, side, 3 if slices > 1 else tiles_of(side), min(slices, pairs)))
+            check_loss(x, w, tokens, g, gs, False)

@@ -186,14 +186,23 @@ __device__ __forceinline__ bool half_join(HalfSums<T>& sums, HalfShared<T, STAGE
 #pragma unroll
         for (int j = 0; j < T; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f32x4 v;
+            for (int k = 0; k < 16; ++k) sums.large[i][j][k] = __builtin_fmaf(sums.small[i][j][k], 1.f / HALF_REST, sums.large[i][j][k]);
+    // Stored from where they are and stay: a buffer store of 16 bytes whose offset is a scalar register still reads its first word, for the last quarter of a row's lanes, while the instruction
+    // behind it runs, and the compiler lets that one write the register (values of another part of the tile were found in their place).
+    HALF_FENCE();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(sums.small[i][j][4 * q + e], 1.f / HALF_REST, sums.large[i][j][4 * q + e]);
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = {sums.large[i][j][4 * q], sums.large[i][j][4 * q + 1], sums.large[i][j][4 * q + 2], sums.large[i][j][4 * q + 3]};
                 // (past the L2, which is not the other XCDs')
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, tid * 16u, slice * BYTES + (uint32_t)((i * T + j) * 4 + q) * 4096u, 16);
             }
+    HALF_FENCE();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the stores have reached memory
+    HALF_FENCE();
     __syncthreads();
     if (tid == 0u) {
         const uint32_t n = __hip_atomic_fetch_add(arrivals + mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
