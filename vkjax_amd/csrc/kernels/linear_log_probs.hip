@@ -152,31 +152,36 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
 }
 
 // ---- forward: a tile's peak and sum per row of x, [tile of tokens][rows]
-struct ScoresParams { uint32_t rows, V, pairs, steps_w, steps_x, tiles_m, tiles_n, blocks_w, blocks_x, tile0, Vp, pad; };
+struct ScoresParams { uint32_t rows, V, pairs, steps_w, steps_x, tiles_m, tiles_n, blocks_w, blocks_x, tile0, Vp; HalfShares shares; };
 
 __device__ __forceinline__ HalfOperand operand_of(const u32x4* parts, uint32_t blocks, uint32_t stride, uint32_t first = 0) { return HalfOperand{parts, blocks, stride, first}; }
 __device__ __forceinline__ float over_halves_max(float v) { return fmaxf(v, lane_xor<32>(v)); }
 __device__ __forceinline__ float over_halves_sum(float v) { return v + lane_xor<32>(v); }
 
-extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, const u32x4* __restrict__ w,
-                                                                   const u32x4* __restrict__ x, const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, ScoresParams P) {
-    __shared__ HalfShared<2, 2> shared;
-    uint32_t m, n;
-    half_tile(half_turn(blockIdx.x, gridDim.x), P.tiles_m, P.tiles_n, m, n);
-    HalfSums<2> acc = {};
-    half_product<2, 2>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, 0u, P.pairs);
+template <int T, int STAGES, bool SHARED>
+__device__ __forceinline__ void linear_scores_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ partial, uint32_t* __restrict__ arrivals,
+                                                   const u32x4* __restrict__ w, const u32x4* __restrict__ x, const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales,
+                                                   const ScoresParams& P) {
+    constexpr uint32_t SIDE = HalfTileOf<T>::SIDE;
+    __shared__ HalfShared<T, STAGES> shared;
+    uint32_t m, n, tile, slice, begin, end;
+    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_tile(tile, P.tiles_m, P.tiles_n, m, n);
+    HalfSums<T> acc = {};
+    half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, begin, end - begin);
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]);
-    float (*const met)[128][2] = reinterpret_cast<float (*)[128][2]>(&shared.stages[0]);           // [wm][column][peak, sum]
-    const uint32_t v0 = m * 128u + wm * 64u + 4u * (lane >> 5);
+    float (*const met)[SIDE][2] = reinterpret_cast<float (*)[SIDE][2]>(&shared.stages[0]);  // [wm][column][peak, sum]
+    const uint32_t v0 = m * SIDE + wm * 32u * T + 4u * (lane >> 5);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t column = wn * 64u + j * 32u + (lane & 31u), r = n * 128u + column;
+    for (int j = 0; j < T; ++j) {
+        const uint32_t column = (wn * T + j) * 32u + (lane & 31u), r = n * SIDE + column;
         const int32_t token = r < P.rows ? tokens[r] : -1;
         float peak = -__builtin_inff(), sum = 0.f, mine = 0.f;
         bool has = false;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
                 const uint32_t v = v0 + 32u * i + 8u * (q >> 2) + (q & 3);
@@ -190,15 +195,15 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __rest
         peak = over_halves_max(peak);
         const float base = peak == -__builtin_inff() ? 0.f : peak;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
             for (int q = 0; q < 16; ++q) sum += exp_of(acc.large[i][j][q] - base);
         sum = over_halves_sum(sum);
         if (lane < 32u) { met[wm][column][0] = peak; met[wm][column][1] = sum; }
     }
     __syncthreads();
-    if (threadIdx.x < 128u) {
-        const uint32_t r = n * 128u + threadIdx.x;
+    if (threadIdx.x < SIDE) {
+        const uint32_t r = n * SIDE + threadIdx.x;
         const float p0 = met[0][threadIdx.x][0], p1 = met[1][threadIdx.x][0], peak = fmaxf(p0, p1), base = peak == -__builtin_inff() ? 0.f : peak;
         if (r < P.rows) {
             peaks[(uint64_t)m * P.rows + r] = peak;
@@ -206,6 +211,15 @@ extern "C" __global__ __launch_bounds__(256, 2) void linear_scores(float* __rest
         }
     }
 }
+#define LINEAR_SCORES(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                                \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_scores##SUFFIX(float* peaks, float* sums, float* of_token, float* partial, uint32_t* arrivals,     \
+                                                                                    const u32x4* w, const u32x4* x, const int32_t* tokens, const int32_t* scales,       \
+                                                                                    ScoresParams P) {                                                                   \
+        linear_scores_body<T, STAGES, SHARED>(peaks, sums, of_token, partial, arrivals, w, x, tokens, scales, P);                                                       \
+    }
+// (the kernels of half_product.h, by suffix)
+#define LINEAR_KERNELS(F) F(_128, 2, 2, 2, false) F(_128_shared, 2, 2, 2, true) F(_64, 1, 4, 2, false) F(_64_shared, 1, 4, 2, true) F(_64_many, 1, 2, 4, false) F(_64_many_shared, 1, 2, 4, true)
+LINEAR_KERNELS(LINEAR_SCORES)
 
 // A row's tiles joined. A block has R rows (a power of two up to 64): 1024 / R lanes to a row, which take tiles in turn, eight at a time, and meet by butterflies and in shared memory.
 struct JoinParams { uint32_t log2_rows, rows, V, tiles; };
@@ -400,35 +414,46 @@ SCORES_ROWS(h_32, false, 1)
 SCORES_ROWS(h_64, false, 2)
 
 // ---- backward: a piece's q, as operands contracted over the vocabulary [rows][tokens] and over the rows [tokens][rows]
-extern "C" __global__ __launch_bounds__(256, 2) void linear_q(u32x4* __restrict__ by_row, u32x4* __restrict__ by_token, const u32x4* __restrict__ w, const u32x4* __restrict__ x,
-                                                              const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, const float* __restrict__ row_peaks,
-                                                              const float* __restrict__ row_totals, const float* __restrict__ factors, ScoresParams P) {
-    __shared__ HalfShared<2, 2> shared;
-    uint32_t m, n;
-    half_tile(half_turn(blockIdx.x, gridDim.x), P.tiles_m, P.tiles_n, m, n);
-    HalfSums<2> acc = {};
-    half_product<2, 2>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, 0u, P.pairs);
+template <int T, int STAGES, bool SHARED>
+__device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4* __restrict__ by_token, float* __restrict__ partial, uint32_t* __restrict__ arrivals, const u32x4* __restrict__ w,
+                                              const u32x4* __restrict__ x, const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, const float* __restrict__ row_peaks,
+                                              const float* __restrict__ row_totals, const float* __restrict__ factors, const ScoresParams& P) {
+    constexpr uint32_t SIDE = HalfTileOf<T>::SIDE;
+    __shared__ HalfShared<T, STAGES> shared;
+    uint32_t m, n, tile, slice, begin, end;
+    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_tile(tile, P.tiles_m, P.tiles_n, m, n);
+    HalfSums<T> acc = {};
+    half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, begin, end - begin);
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]), up = power_of_two(Q_SCALE);
-    const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * 128u;
-    // of this lane's two columns
-    bool given[2];
-    uint32_t token[2];
-    float peak[2], part[2], one[2];
+    const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * SIDE;
+    // of this lane's columns
+    bool given[T];
+    uint32_t token[T];
+    float peak[T], part[T], one[T];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t r = n * 128u + wn * 64u + 32u * j + (lane & 31u), at = min(r, P.rows - 1u);
+    for (int j = 0; j < T; ++j) {
+        const uint32_t r = n * SIDE + (wn * T + j) * 32u + (lane & 31u), at = min(r, P.rows - 1u);
         given[j] = r < P.rows && is_token(tokens[at], P.V);
         token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
         peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
-    half_store<2>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 4u, m * 8u}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 4u, n * 8u},
-               [&](int i, int j, int k, uint32_t row, uint32_t) {
+    half_store<T>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 2u * T, n * 4u * T},
+                  [&](int i, int j, int k, uint32_t row, uint32_t) {
         const uint32_t v = v0 + row;
         const float s = half_sum(acc, i, j, k) * down_w * down_x;
         const float q = part[j] * exp_of(s - peak[j]) + (v == token[j] ? one[j] : 0.f);
         return given[j] && v < P.V ? q : 0.f;
     });
 }
+#define LINEAR_Q(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                                     \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_q##SUFFIX(u32x4* by_row, u32x4* by_token, float* partial, uint32_t* arrivals, const u32x4* w,      \
+                                                                               const u32x4* x, const int32_t* tokens, const int32_t* scales, const float* row_peaks,    \
+                                                                               const float* row_totals, const float* factors, ScoresParams P) {                         \
+        linear_q_body<T, STAGES, SHARED>(by_row, by_token, partial, arrivals, w, x, tokens, scales, row_peaks, row_totals, factors, P);                                 \
+    }
+LINEAR_KERNELS(LINEAR_Q)
 
 // ---- a product of two operands to fp32 [M, N], rows by a factor each (every third word), added to what is there or in its place; not SHARED: a slice of the contraction to an array of its own
 struct ProductParams {
@@ -484,12 +509,7 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
                                                                                      const int32_t* scales, const float* factors, ProductParams P) {                    \
         linear_product_body<T, STAGES, SHARED>(out, partial, arrivals, a, b, scales, factors, P);                                                                       \
     }
-LINEAR_PRODUCT(_128, 2, 2, 2, false)
-LINEAR_PRODUCT(_128_shared, 2, 2, 2, true)
-LINEAR_PRODUCT(_64, 1, 4, 2, false)
-LINEAR_PRODUCT(_64_shared, 1, 4, 2, true)
-LINEAR_PRODUCT(_64_many, 1, 2, 4, false)
-LINEAR_PRODUCT(_64_many_shared, 1, 2, 4, true)
+LINEAR_KERNELS(LINEAR_PRODUCT)
 
 struct SumParams { uint32_t parts, pad; uint64_t n; };
 extern "C" __global__ __launch_bounds__(256) void linear_sum(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {

@@ -2754,6 +2754,14 @@ def half_plan(tiles_of, pairs: int) -> HalfPlan:
     return best[1]
 
 
+def half_share(plan: HalfPlan, tiles: int, scratch, zeroed):
+    '''(suffix of the kernel's name, blocks, an array for parts of sums and one for arrivals - None where no contraction is shared -) of a launch over so many tiles.'''
+    rest = tiles - plan.whole
+    if plan.slices == 1:
+        return plan.kernel, tiles, None, None
+    return (plan.kernel + '_shared', plan.whole + rest * plan.slices, scratch((rest * plan.slices, plan.side, plan.side)), zeroed(rest, 'arrivals at tiles of halves'))
+
+
 HALF_CUS = 256
 #kernels by tile: (name, side, blocks to a CU, us of a block beside its contraction, us of a pair of steps at least, us of a CU for one), by measurement: products of 512 x 512 x 512 alone 18.5,
 #11.0 and 11.7 us, of 512 x 512 x 4096 96, 53 and 64, of 2048^3 64, 84 and 67, 192 tiles of 128 x 16 pairs 21, 21.6 and 18. (A pair with a block of 128 to a CU: 0.68 us from the caches near by,
@@ -2820,19 +2828,35 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     return launches, (*behind, factors)
 
 
-def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, parts=None) -> tp.List[Launch]:
+def _linear_scores_launch(name: str, shape: LinearShape, tokens: int, tile0, width: int, buffers, written, shared, scratch, zeroed) -> tp.Tuple[Launch, int]:
+    '''A launch of the scores' product over `tokens` of the vocabulary (from tile0(side) tiles on), and the side of its tiles. `buffers` without the two of shared contractions,
+    which stand behind the first `shared`.'''
+    rows, h, v = shape
+    tiles_of = lambda side: _cdiv(tokens, side) * _cdiv(rows, side)
+    pairs = _half_steps(h) // 2
+    plan  = half_plan(tiles_of, pairs)
+    suffix, blocks, partial, arrivals = half_share(plan, tiles_of(plan.side), scratch, zeroed)
+    buffers = [*buffers[:shared], partial, arrivals, *buffers[shared:]]
+    return Launch(f'{name}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in buffers],
+                  _u32(rows, v, pairs, 2 * pairs, 2 * pairs, _cdiv(tokens, plan.side), _cdiv(rows, plan.side), _cdiv(v, 32), _cdiv(rows, 32), tile0(plan.side), width, plan.whole, plan.slices),
+                  bytes_moved=4 * h * (tokens + rows) + (8 * rows * tokens if width else 0), flops=2 * rows * h * tokens,
+                  written=written + ((shared, shared + 1) if partial is not None else ()), scratch=(shared + 1,) if partial is not None else ()), plan.side
+
+
+def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, zeroed, parts=None) -> tp.List[Launch]:
     shape = rows, h, v = _linear_shape(x, w, transposed)
-    tiles    = _cdiv(v, HALF_TILE)
+    tiles    = _cdiv(v, 64)
     of_tiles = [scratch((tiles, rows)), scratch((tiles, rows)), scratch((rows,))]           #peak and sum of each tile's scores, the token's score
     if rows <= LINEAR_ROWS and v >= 4 and not parts:
+        tiles    = _cdiv(v, 128)
         launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles, 1, 1), (512, 1, 1), [(b, 0) for b in (*of_tiles, x, w, tokens)],
                            _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2))]
     else:
         w_parts, x_parts, scales = parts or [scratch((n,), dtype) for n, dtype in zip(linear_parts(x.shape, w.shape, transposed), (np.uint32, np.uint32, np.int32))]
         launches, _ = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts))
-        launches.append(Launch('linear_scores', (tiles * _cdiv(rows, HALF_TILE), 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (*of_tiles, w_parts, x_parts, tokens, scales)],
-                               _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, _cdiv(rows, HALF_TILE), _cdiv(v, 32), _cdiv(rows, 32), 0, 0, 0),
-                               bytes_moved=4 * (w_parts.size + x_parts.size), flops=2 * rows * h * v, written=(0, 1, 2)))
+        scores, side = _linear_scores_launch('linear_scores', shape, v, lambda side: 0, 0, (*of_tiles, w_parts, x_parts, tokens, scales), (0, 1, 2), 3, scratch, zeroed)
+        launches.append(scores)
+        tiles = _cdiv(v, side)
     #rows of a block: a line of them, fewer where there are few
     join_rows = min(16, _pow2_at_least(rows))
     return launches + [Launch('linear_join', (_cdiv(rows, join_rows), 1, 1), (1024, 1, 1), [(b, 0) for b in (log_probs, log_sums, peaks, totals, *of_tiles, tokens)],
@@ -2861,15 +2885,13 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
 
     def product(out, offset, a, b, m, n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_b, scale_a, scale_b, ld, by_rows=False, add=False, parts=0):
         #(parts: slices to arrays of their own)
-        plan  = HalfPlan('_128', HALF_TILE, 0, parts) if parts else half_plan(lambda side: _cdiv(m, side) * _cdiv(n, side), pairs)
-        rest  = _cdiv(m, plan.side) * _cdiv(n, plan.side) - plan.whole
-        share = plan.slices > 1 and not parts
-        partial, arrivals = (scratch((rest * plan.slices, plan.side, plan.side)), zeroed(rest, 'arrivals at tiles of halves')) if share else (None, None)
-        return Launch(f'linear_product{plan.kernel}{"_shared" if share else ""}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1),
-                      [(out, 4 * offset), (partial, 0), (arrivals, 0), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
+        tiles_of = lambda side: _cdiv(m, side) * _cdiv(n, side)
+        plan = HalfPlan('_128', HALF_TILE, 0, parts) if parts else half_plan(tiles_of, pairs)
+        suffix, blocks, partial, arrivals = (plan.kernel, tiles_of(HALF_TILE) * parts, None, None) if parts else half_share(plan, tiles_of(plan.side), scratch, zeroed)
+        return Launch(f'linear_product{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(out, 4 * offset), (partial, 0), (arrivals, 0), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
                       _u32(m, n, _cdiv(m, plan.side), _cdiv(n, plan.side), pairs, blocks_a, blocks_b, steps_a, steps_b, 0, first_b, add) + _i32(scale_a, scale_b)
                       + _u32(plan.whole, plan.slices) + _u64(ld, m * n), bytes_moved=4 * (m + n) * 32 * pairs + 4 * m * n, flops=64 * m * n * pairs,
-                      written=(0, 1, 2) if share else (0,), scratch=(2,) if share else ())
+                      written=(0, 1, 2) if partial is not None else (0,), scratch=(2,) if partial is not None else ())
     #dx has few tiles and a long contraction: slices are added up by a launch of their own, not by the blocks that arrive last (321 x 500 over 50001 tokens: 105 + 8 us, 117; a piece of
     #4096 x 1024 over 8064: 202 + 8, 241, in one slice 277)
     tiles_x = tiles_r * _cdiv(h, HALF_TILE)
@@ -2881,9 +2903,8 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         first = piece * each
         tiles = min(each, all_tiles - first)
         v0, n = first * HALF_TILE, min(width, v - first * HALF_TILE)
-        launches.append(Launch('linear_q', (tiles * tiles_r, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors)],
-                               _u32(rows, v, _half_steps(h) // 2, _half_steps(h), _half_steps(h), tiles, tiles_r, _cdiv(v, 32), row_blocks, first, width, 0),
-                               bytes_moved=8 * 32 * row_blocks * width, flops=2 * rows * h * n, written=(0, 1)))
+        launches.append(_linear_scores_launch('linear_q', shape, tiles * HALF_TILE, lambda side: v0 // side, width, (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors),
+                                              (0, 1), 2, scratch, zeroed)[0])
         launches.append(product(sums, 0, by_row, w_by_h, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), v0 // 16, -1, _PACK_WEIGHTS, h,
                                 by_rows=True, add=piece > 0, parts=parts))
         steps = 2 * row_blocks
@@ -2943,16 +2964,12 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
         symmetric = name in ('square', 'polynomial')
         of_matrix = lambda side: _cdiv(m, side) * (_cdiv(m, side) + 1) // 2 if symmetric else _cdiv(m, side) * _cdiv(width, side)
         plan  = half_plan(lambda side: n * of_matrix(side), _half_steps(k) // 2)
-        tiles = n * of_matrix(plan.side)
-        rest  = tiles - plan.whole
-        partial  = scratch((rest * plan.slices, plan.side, plan.side)) if plan.slices > 1 else None
-        arrivals = zeroed(rest, 'arrivals at tiles of halves') if plan.slices > 1 else None
-        launch = Launch(f'orthogonal_{name}{plan.kernel}{"_shared" if plan.slices > 1 else ""}', (plan.whole + rest * plan.slices, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
-                        _u32(('square', 'polynomial', 'next', 'last').index(name), m, width, k, _cdiv(m, plan.side), _cdiv(width, plan.side), of_matrix(plan.side)) + _i32(*scales)
-                        + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, 0) + _u64(sr, sc),
-                        bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=(1 if symmetric else 2) * n * m * width * k,
-                        written=written + ((3, 4) if plan.slices > 1 else ()), scratch=(4,) if plan.slices > 1 else ())
-        return launch
+        suffix, blocks, partial, arrivals = half_share(plan, n * of_matrix(plan.side), scratch, zeroed)
+        return Launch(f'orthogonal_{name}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
+                      _u32(('square', 'polynomial', 'next', 'last').index(name), m, width, k, _cdiv(m, plan.side), _cdiv(width, plan.side), of_matrix(plan.side)) + _i32(*scales)
+                      + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, 0) + _u64(sr, sc),
+                      bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=(1 if symmetric else 2) * n * m * width * k,
+                      written=written + ((3, 4) if partial is not None else ()), scratch=(4,) if partial is not None else ())
     for i, (s, p) in enumerate(bounds):
         scale_x, scale_a, scale_p = _half_scale(s), _half_scale(s * s), _half_scale(p)
         launches += [product('square', (square_parts, square_parts, square), by_row, by_row, None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2)),

@@ -1238,7 +1238,8 @@ def linear_log_probs(bufferpool, equation):
         raise NotImplementedError(equation)
     if p.get('parts') and any(v is None for v in parts):
         raise NotImplementedError(equation)
-    return _operator_ops(equation, K.linear_log_probs(log_probs, log_sums, peaks, totals, x, weights, tokens, p['transposed'], scratch, parts or None))
+    return _operator_ops(equation, K.linear_log_probs(log_probs, log_sums, peaks, totals, x, weights, tokens, p['transposed'], scratch,
+                                                       bufferpool.zeroed_scratch, parts or None))
 
 
 def linear_log_probs_grad(bufferpool, equation):
