@@ -1064,7 +1064,7 @@ def linear_log_probs(x, weights, tokens, transposed, parts=False):
     if parts:
         #(what the device keeps of its operands for the gradient, which is worked out from the operands themselves here)
         from vkjax_amd.kernels import linear_parts
-        kept = tuple(np.zeros(n, dtype) for n, dtype in zip(linear_parts(np.shape(x), np.shape(weights), transposed), (np.uint32, np.uint32, i32)))
+        kept = tuple(np.zeros(n, dtype) for n, dtype in linear_parts(np.shape(x), np.shape(weights), transposed))
         return linear_log_probs(x, weights, tokens, transposed) + kept
     with np.errstate(**_EW_ERR):
         if np.size(tokens) == 0:

@@ -273,7 +273,7 @@ def loss_inputs(rows, hidden, vocabulary, transposed, seed=0):
 #(rows, hidden, vocabulary): one of everything; rows that the fp32 instructions take, in one block of 32 and in two, at the border and behind it; contractions of no whole pair of steps; vocabularies that are
 #smaller than a vector, end inside a vector, a tile, a block of 32; several tiles each way
 LOSSES = [(1, 1, 1), (1, 8, 4), (3, 5, 7), (2, 64, 3), (64, 32, 128), (65, 33, 129), (8, 64, 300), (33, 100, 1001), (130, 70, 515), (257, 128, 4099), (100, 300, 3), (66, 17, 2), (20, 515, 2050),
-          (300, 40, 640), (5, 1030, 131), (128, 128, 128), (1100, 9, 1300), (64, 7, 2049)]
+          (300, 40, 640), (5, 1030, 131), (128, 128, 128), (1100, 9, 1300), (64, 7, 2049), (32, 100, 515), (33, 4, 261), (64, 130, 5000), (7, 3, 50), (17, 257, 6), (1, 300, 9001), (64, 700, 4)]
 
 
 @pytest.mark.parametrize('transposed', [False, True])
@@ -330,6 +330,19 @@ def test_linear_log_probs_of_nothing_but_padding():
         x, w, tokens, g, gs = loss_inputs(rows, 40, 300, False)
         got = mj.tree_leaves(both(loss_program(False), np.full_like(x, np.nan), w, np.full_like(tokens, -1), g, gs)[0])
         assert not any(v.any() for v in got)
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('rows', [9, 40, 200])
+def test_linear_log_probs_of_weights_that_are_not_finite(rows, transposed):
+    x, w, tokens, g, gs = loss_inputs(rows, 40, 300, transposed)
+    tokens[::3] = -1
+    tokens[1::3] = 5
+    w[7, 9] = np.nan
+    got = mj.tree_leaves(both(loss_program(transposed), x, w, tokens, g, gs)[0])
+    given = (tokens >= 0) & (tokens < 300)
+    assert np.array_equal(np.isnan(got[0]), given) and np.array_equal(np.isnan(got[1]), given) and np.isnan(got[2][given]).all()
+    assert not any(v[~given].any() for v in got[:3])
 
 
 # ------------------------------------------------------------------ orthogonalised matrices
@@ -400,8 +413,9 @@ def test_orthogonalize_a_matrix_of_a_low_rank_and_of_zeros():
         assert np.linalg.norm(got[i].astype(np.float64) - expected[i]) <= orthogonal_bound(x[i], 5, (3.4445, -4.7750, 2.0315))
 
 
-def test_gradient_of_log_probs_with_and_without_the_operands_that_were_kept():
-    x, w, tokens, g, gs = loss_inputs(150, 70, 600, False)
+@pytest.mark.parametrize('rows', [9, 64, 150])
+def test_gradient_of_log_probs_with_and_without_what_was_kept(rows):
+    x, w, tokens, g, gs = loss_inputs(rows, 70, 600, False)
 
     def both_ways(x, w, tokens, g, gs):
         outs = lax.linear_log_probs(x, w, tokens, with_parts=True)

@@ -377,8 +377,11 @@ def test_log_probs_keep_their_operands_for_a_gradient_only():
         return lax.linear_log_probs_grad(x, w, t, outs[2], outs[3], g, parts=outs[4:]) + lax.linear_log_probs_grad(x, w, t, outs[2], outs[3], g)
     dx, dw, dx2, dw2 = evaluate(by_hand, x, w, t, g)
     assert np.array_equal(dx, dx2) and np.array_equal(dw, dw2)
-    words = [np.zeros(n, d) for n, d in zip(K.linear_parts(x.shape, w.shape, False), (np.uint32, np.uint32, np.int32))]
-    for at in range(3):
-        for bad in (words[at][:-1], words[at].astype(f32), words[at].reshape(1, -1)):
-            refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *(words[:at] + [bad] + words[at + 1:]))
-    refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *words[:2])
+    for rows in (5, 70):
+        x, t, g = normal(1, rows, 4), np.arange(rows, dtype=np.int32) % 7, normal(3, rows)
+        kept = [np.zeros(n, d) for n, d in K.linear_parts(x.shape, w.shape, False)]
+        assert len(kept) == (1 if rows == 5 else 3)
+        for at, v in enumerate(kept):
+            for bad in (v[:-1], v.astype(np.uint32 if v.dtype == f32 else f32), v.reshape(1, -1)):
+                refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *(kept[:at] + [bad] + kept[at + 1:]))
+        refused(TypeError, lambda *a: lax.linear_log_probs_grad(*a[:5], parts=a[5:]), x, w, t, g, g, *kept[:-1])

@@ -10,7 +10,7 @@
 //   * backward, in pieces of the vocabulary: the same product again, whose lanes turn scores into q = ds / m, |q| <= 2, with m = max(|g_lp|, |g_ls - g_lp|) of the row, and lay q out as an
 //     operand of both products that follow, contracted over the vocabulary (the lanes have it like that) and over the rows (turned in shared memory). q takes 8 bytes a score of one
 //     piece; the rows' m is a factor of dx's rows, and of the x that dW is made of.
-// Up to 64 rows take the fp32 matrix instructions (linear_scores_rows), which read W once, as it is: bound by memory.
+// Up to 64 rows take the fp32 matrix instructions (RowsProduct), which read W as it is, once forward and once for dx: bound by memory. The scores of so few rows are kept for the gradient.
 #include "half_product.h"
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -268,150 +268,351 @@ extern "C" __global__ __launch_bounds__(1024) void linear_join(float* __restrict
     if (row_totals) row_totals[r] = given ? all.sum : 1.f;
 }
 
-// ---- up to 32 NT rows: a block has 128 tokens, its waves parts of the contraction; W is read once. v_mfma_f32_32x32x2_f32: lane l has row l % 32 of a block of 32 and k = l / 32.
-// Which token a lane's row is, and in which order k comes, follows from how W lies: four neighbouring tokens to a lane's vector (ALONG_V), or 16 neighbouring h.
-struct RowsParams { uint32_t rows, H, V, pad; };
-template <bool ALONG_V, int NT>
-__device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, const float* __restrict__ x, const float* __restrict__ w,
-                                                 const int32_t* __restrict__ tokens, const RowsParams& P) {
-    constexpr int WAVES = 8;
-    __shared__ f32x4 met[WAVES / 2][NT * 16][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31u, v0 = blockIdx.x * 128u;
-    // groups of 8 (ALONG_V) or 32 h, to the waves in turn by contiguous ranges
-    constexpr uint32_t GROUP = ALONG_V ? 8u : 32u;
-    const uint32_t groups = (P.H + GROUP - 1u) / GROUP, begin = groups * wave / WAVES, end = groups * (wave + 1u) / WAVES;
-    f32x16 acc[4][NT] = {};
-    // (lanes behind the last token or row read the last ones again)
-    const uint32_t v_at = ALONG_V ? min(v0 + 4u * l32, P.V - 4u) : 0u;
-    uint32_t r_at[NT];
-    bool r_there[NT];
+// ---- up to 32 NT rows: out[m, r] = sum_k A[m, k] b[r, k] with fp32 matrix instructions, A as it lies (its columns along M: [K][M], or along K: [M][K]) and read once, b [rows][K].
+// v_mfma_f32_32x32x2_f32: lane l has row l % 32 of a block of 32 and k = l / 32; which m a lane's row is, and in which order k comes, follows from how A lies. A block has 128 m, its waves
+// parts of k, a wave's loads are a step ahead of its products, or three.
+//   * along M: four neighbouring m to a lane's vector, 8 k of 128 m a step;
+//   * along K: 32 k of 128 m a step, loaded in whole lines and turned in the wave's own part of shared memory, whose vectors of a row are exchanged so that 8 rows of one column lie in
+//     different banks. (Loaded as the instruction has them, 64 bytes of a row to a lane, lines were fetched several times: 53 x 776 x 112111 took 269 us, 1.3 TB/s.)
+// Bound by memory up to 32 rows (15 x 1973 x 128040: 200 us, 5 TB/s along M, 270 along K), and by memory and the products alike at 64 (64 x 4096 x 32000: 168 us, of which either takes 107 alone).
+// Blocks of four waves, two a CU, hide one another's ends: with eight waves to a block 14 x 47 x 107245 took 31 us, not 19, and 32 x 896 x 83954 93 us, not 76.
+template <int NT> struct RowsProduct {
+    static constexpr int WAVES = 4;
+    static constexpr uint32_t THREADS = 64u * WAVES;
+    union Shared { f32x4 turned[WAVES][4][32][8]; f32x4 met[WAVES / 2][NT * 16][64]; };
+    f32x16 acc[4][NT];
+
+    static __device__ __forceinline__ uint32_t lane() { return threadIdx.x & 63u; }
+    static __device__ __forceinline__ f32x4 load(const float* at) { return *reinterpret_cast<const f32x4_anywhere*>(at); }
+    // over the k of groups [all_begin, all_end); `there`: rows that are padding are zeros, whatever b holds. M and K are 4 at least: vectors that would end behind the last m or k are moved to
+    // the left, and of b the k's that come twice by that are zeros. (So nothing is loaded behind a branch: with one the loads of a last group waited for one another, 25 us of a block's 84 at
+    // 15 x 1973 x 128040.)
+    template <bool ALONG_M>
+    __device__ __forceinline__ void multiply(Shared& shared, const float* __restrict__ a, const float* __restrict__ b, uint32_t m0, uint32_t M, uint32_t K, const uint32_t (&r_at)[NT],
+                                             const bool (&there)[NT], uint32_t all_begin, uint32_t all_end) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane() >> 5, l32 = lane() & 31u;
+        const uint32_t groups = all_end - all_begin, begin = all_begin + groups * wave / WAVES, end = all_begin + groups * (wave + 1u) / WAVES;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const uint32_t r = 32u * j + l32;
-        r_at[j] = min(r, P.rows - 1u);
-        r_there[j] = r < P.rows && is_token(tokens[r_at[j]], P.V);
-    }
-    auto four = [&](const float* row, uint32_t h, bool there) {
-        f32x4 t = {0.f, 0.f, 0.f, 0.f};
-        if (!there) return t;
-        if (h + 4u <= P.H) return (f32x4)*reinterpret_cast<const f32x4_anywhere*>(row + h);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) if (h + q < P.H) t[q] = row[h + q];
-        return t;
-    };
-    if constexpr (ALONG_V) {
-        // (DEPTH - 1 groups are on their way while one is multiplied)
-        constexpr uint32_t DEPTH = 4u;
-        f32x4 ws[DEPTH][4], xs[DEPTH][NT];
-        auto request = [&](f32x4 (&wv)[4], f32x4 (&xv)[NT], uint32_t g) {
-            const uint32_t h0 = g * 8u + 4u * half;
+            for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
+        auto of_row = [&](int j, uint32_t k) { return load(b + (uint64_t)r_at[j] * K + min(k, K - 4u)); };
+        auto own = [&](f32x4 v, int j, uint32_t k) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) wv[q] = *reinterpret_cast<const f32x4_anywhere*>(w + (uint64_t)min(h0 + q, P.H - 1u) * P.V + v_at);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) xv[j] = four(x + (uint64_t)r_at[j] * P.H, h0, r_there[j]);
+            for (uint32_t e = 0; e < 4u; ++e) v[e] = there[j] && min(k, K - 4u) + e >= k ? v[e] : 0.f;
+            return v;
         };
-        auto multiply = [&](const f32x4 (&wv)[4], const f32x4 (&xv)[NT]) {
+        if constexpr (ALONG_M) {
+            // (lanes behind the last m read the last ones again)
+            const uint32_t m_at = min(m0 + 4u * l32, M - 4u);
+            constexpr uint32_t DEPTH = 4u;
+            f32x4 as[DEPTH][4], bs[DEPTH][NT];
+            auto request = [&](f32x4 (&av)[4], f32x4 (&bv)[NT], uint32_t g) {
+                const uint32_t k0 = g * 8u + 4u * half, k = min(k0, K - 4u);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q) av[q] = load(a + (uint64_t)(k + q) * M + m_at);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) bv[j] = of_row(j, k0);
+            };
+            auto products = [&](const f32x4 (&av)[4], f32x4 (&bv)[NT], uint32_t g) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) bv[j] = own(bv[j], j, g * 8u + 4u * half);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[q][i], bv[j][q], acc[i][j], 0, 0, 0);
+            };
+#pragma unroll
+            for (uint32_t k = 0; k < DEPTH - 1u; ++k) if (begin + k < end) request(as[k], bs[k], begin + k);
+            // (steps that request others without a test first: behind one, a wait for a step's loads is one for later steps' too)
+            uint32_t g = begin;
+            for (; g + 2u * DEPTH - 2u < end; g += DEPTH)
+#pragma unroll
+                for (uint32_t k = 0; k < DEPTH; ++k) {
+                    request(as[(k + DEPTH - 1u) % DEPTH], bs[(k + DEPTH - 1u) % DEPTH], g + k + DEPTH - 1u);
+                    __builtin_amdgcn_sched_barrier(0);
+                    products(as[k], bs[k], g + k);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            for (; g < end; g += DEPTH)
+#pragma unroll
+                for (uint32_t k = 0; k < DEPTH; ++k) {
+                    if (g + k + DEPTH - 1u < end) request(as[(k + DEPTH - 1u) % DEPTH], bs[(k + DEPTH - 1u) % DEPTH], g + k + DEPTH - 1u);
+                    if (g + k < end) products(as[k], bs[k], g + k);
+                }
+        } else {
+            f32x4 (&turned)[4][32][8] = shared.turned[wave];
+            const uint32_t row8 = lane() >> 3, column = lane() & 7u;
+            f32x4 next[4][4], bs[NT][4];
+            auto request = [&](uint32_t g) {
+                // (rows behind the last m are the last one again; 8 rows of fewer than 2^27 elements are 32 bits of bytes)
+                const uint32_t at = 4u * min(g * 32u + 4u * column, K - 4u);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(wv[q][i], xv[j][q], acc[i][j], 0, 0, 0);
-        };
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t first = min(m0 + 32u * i + 8u * t, M - 1u);
+                        next[i][t] = load(reinterpret_cast<const float*>(reinterpret_cast<const char*>(a + (uint64_t)first * K) + (uint64_t)(min(row8, M - 1u - first) * K * 4u) + at));
+                    }
+            };
+            auto request_rows = [&](uint32_t g) {
 #pragma unroll
-        for (uint32_t k = 0; k < DEPTH - 1u; ++k) if (begin + k < end) request(ws[k], xs[k], begin + k);
-        for (uint32_t g = begin; g < end; g += DEPTH)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (uint32_t k = 0; k < DEPTH; ++k) {
-                if (g + k + DEPTH - 1u < end) request(ws[(k + DEPTH - 1u) % DEPTH], xs[(k + DEPTH - 1u) % DEPTH], g + k + DEPTH - 1u);
-                if (g + k < end) multiply(ws[k], xs[k]);
+                    for (int c = 0; c < 4; ++c) bs[j][c] = of_row(j, g * 32u + 16u * half + 4u * c);
+            };
+            if (begin < end) { request(begin); request_rows(begin); }
+            for (uint32_t g = begin; g < end; ++g) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) turned[i][8 * t + row8][column ^ row8] = next[i][t];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                f32x4 now[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) now[j][c] = own(bs[j][c], j, g * 32u + 16u * half + 4u * c);
+                if (g + 1u < end) { request(g + 1u); request_rows(g + 1u); }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    f32x4 av[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) av[i] = turned[i][l32][(4u * half + c) ^ (l32 & 7u)];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[i][q], now[j][c][q], acc[i][j], 0, 0, 0);
+                }
             }
-    } else {
-        for (uint32_t g = begin; g < end; ++g) {
-            const uint32_t h0 = g * 32u + 16u * half;
-            f32x4 wv[4][4], xv[NT][4];
+            __syncthreads();                       // (the same memory follows)
+        }
+        // the waves' sums, the upper half of them to the lower half, until the first has all
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) wv[i][q] = four(w + (uint64_t)min(v0 + 32u * i + l32, P.V - 1u) * P.H, h0 + 4u * q, true);
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) xv[j][q] = four(x + (uint64_t)r_at[j] * P.H, h0 + 4u * q, r_there[j]);
-#pragma unroll
-            for (int q = 0; q < 16; ++q)
+        for (uint32_t half_of = WAVES / 2; half_of > 0u; half_of >>= 1) {
+            if (wave >= half_of && wave < 2u * half_of)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(wv[i][q >> 2][q & 3], xv[j][q >> 2][q & 3], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            shared.met[wave - half_of][(i * NT + j) * 4 + q][lane()] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            __syncthreads();
+            if (wave < half_of)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const f32x4 t = shared.met[wave][(i * NT + j) * 4 + q][lane()];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += t[e];
+                        }
+            __syncthreads();
         }
     }
-    // the waves' sums, the upper half of them to the lower half, three times
-#pragma unroll
-    for (uint32_t half_of = WAVES / 2; half_of > 0u; half_of >>= 1) {
-        if (wave >= half_of && wave < 2u * half_of)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) met[wave - half_of][(i * NT + j) * 4 + q][lane] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        __syncthreads();
-        if (wave < half_of)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const f32x4 t = met[wave][(i * NT + j) * 4 + q][lane];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += t[e];
-                    }
-        __syncthreads();
+    // the m of element q of block i. (Of a vector that was moved to the left to stay inside, those that are this lane's own: others are M)
+    template <bool ALONG_M> static __device__ __forceinline__ uint32_t m_of(uint32_t m0, uint32_t M, int i, int q) {
+        const uint32_t row = 8u * (q >> 2) + 4u * (lane() >> 5) + (q & 3);
+        if constexpr (!ALONG_M) return m0 + 32u * i + row;
+        const uint32_t first = m0 + 4u * row, m = min(first, M - 4u) + i;
+        return m >= first ? m : M;
     }
-    if (wave != 0u) return;
+    // to out[r][m], of columns r = 32 j + l % 32 < rows
+    template <bool ALONG_M> __device__ __forceinline__ void store(float* __restrict__ out, uint32_t m0, uint32_t M, uint32_t rows) const {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const uint32_t r = 32u * j + (lane() & 31u);
+            if (r >= rows) continue;
+            float* const to = out + (uint64_t)r * M;
+#pragma unroll
+            for (int p = 0; p < 16; ++p) {                 // four neighbours: of one row of a block along K, of the four blocks along M
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ALONG_M ? acc[e][j][p] : acc[p >> 2][j][4 * (p & 3) + e];
+                const uint32_t m = ALONG_M ? m0 + 4u * (8u * (p >> 2) + 4u * (lane() >> 5) + (p & 3)) : m0 + 32u * (p >> 2) + 8u * (p & 3) + 4u * (lane() >> 5);
+                if (m + 4u <= M) *reinterpret_cast<f32x4_anywhere*>(to + m) = v;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t at = m_of<ALONG_M>(m0, M, ALONG_M ? e : p >> 2, ALONG_M ? p : 4 * (p & 3) + e);
+                        if (at < M) to[at] = v[e];
+                    }
+            }
+        }
+    }
+};
+
+struct RowsParams { uint32_t rows, H, V, slices; };
+template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT], bool (&there)[NT], const int32_t* __restrict__ tokens, const RowsParams& P) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const uint32_t r = 32u * j + (threadIdx.x & 31u);
+        r_at[j] = min(r, P.rows - 1u);
+        there[j] = r < P.rows && is_token(tokens[r_at[j]], P.V);
+    }
+}
+
+// forward: 128 tokens' scores, their peak and sum per row; the scores [rows][V] themselves for a gradient
+template <bool ALONG_V, int NT>
+__device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ scores, const float* __restrict__ x,
+                                                 const float* __restrict__ w, const int32_t* __restrict__ tokens, const RowsParams& P) {
+    using Product = RowsProduct<NT>;
+    __shared__ typename Product::Shared shared;
+    const uint32_t lane = threadIdx.x & 63u, v0 = blockIdx.x * 128u;
+    uint32_t r_at[NT];
+    bool there[NT];
+    rows_there<NT>(r_at, there, tokens, P);
+    Product product;
+    product.template multiply<ALONG_V>(shared, w, x, v0, P.V, P.H, r_at, there, 0u, (P.H + (ALONG_V ? 7u : 31u)) / (ALONG_V ? 8u : 32u));
+    if (threadIdx.x >= 64u) return;
+    if (scores) product.template store<ALONG_V>(scores, v0, P.V, P.rows);
+    if (!peaks) return;
     // a lane has 64 scores of a row
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const uint32_t r = 32u * j + l32;
+        const uint32_t r = 32u * j + (lane & 31u);
         const int32_t token = r < P.rows ? tokens[r] : -1;
-        float peak = -__builtin_inff(), sum = 0.f;
-        const auto token_of = [&](int i, int q) -> uint32_t {
-            const uint32_t row = 8u * (q >> 2) + 4u * half + (q & 3);
-            if constexpr (!ALONG_V) return v0 + 32u * i + row;
-            // (of a vector that was moved to the left to stay inside, the tokens that are this block's and lane's own)
-            const uint32_t first = v0 + 4u * row, v = min(first, P.V - 4u) + i;
-            return v >= first ? v : P.V;
-        };
+        float peak = -__builtin_inff(), sum = 0.f, mine = 0.f;
+        bool has = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
-                const uint32_t v = token_of(i, q);
-                if (v == (uint32_t)token && v < P.V) of_token[r] = acc[i][j][q];
-                acc[i][j][q] = v < P.V ? acc[i][j][q] : -__builtin_inff();
-                peak = fmaxf(peak, acc[i][j][q]);
+                const uint32_t v = Product::template m_of<ALONG_V>(v0, P.V, i, q);
+                float s = product.acc[i][j][q];
+                if (v == (uint32_t)token) { mine = s; has = true; }
+                product.acc[i][j][q] = s = v < P.V ? s : -__builtin_inff();
+                peak = fmaxf(peak, s);
             }
+        if (has && is_token(token, P.V)) of_token[r] = mine;
         peak = over_halves_max(peak);
         const float base = peak == -__builtin_inff() ? 0.f : peak;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) sum += exp_of(acc[i][j][q] - base);
+            for (int q = 0; q < 16; ++q) sum += exp_of(product.acc[i][j][q] - base);
         sum = over_halves_sum(sum);
         if (lane < 32u && r < P.rows) { peaks[(uint64_t)blockIdx.x * P.rows + r] = peak; sums[(uint64_t)blockIdx.x * P.rows + r] = sum; }
     }
 }
-#define SCORES_ROWS(NAME, ALONG_V, NT)                                                                                                                             \
-    extern "C" __global__ __launch_bounds__(512) void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, const float* x, const float* w,        \
-                                                                                const int32_t* tokens, RowsParams P) {                                             \
-        scores_rows_body<ALONG_V, NT>(peaks, sums, of_token, x, w, tokens, P);                                                                                     \
+
+// backward: ds [rows][V] from the scores, zeros for padding
+extern "C" __global__ __launch_bounds__(256) void linear_rows_ds(float* __restrict__ ds, const float* __restrict__ scores, const int32_t* __restrict__ tokens, const float* __restrict__ row_peaks,
+                                                                 const float* __restrict__ row_totals, const float* __restrict__ g_log_probs, const float* __restrict__ g_log_sums, RowsParams P) {
+    const uint32_t r = blockIdx.y;
+    const int32_t token = tokens[r];
+    const bool given = is_token(token, P.V);
+    const float one = g_log_probs ? g_log_probs[r] : 0.f, part = ((g_log_sums ? g_log_sums[r] : 0.f) - one) / row_totals[r], peak = row_peaks[r];
+    const uint64_t row = (uint64_t)r * P.V;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k) {
+        const uint32_t v = (blockIdx.x * 4u + k) * 256u + threadIdx.x;
+        if (v < P.V) ds[row + v] = given ? part * exp_of(scores[row + v] - peak) + (v == (uint32_t)token ? one : 0.f) : 0.f;
     }
-SCORES_ROWS(v_32, true, 1)
-SCORES_ROWS(v_64, true, 2)
-SCORES_ROWS(h_32, false, 1)
-SCORES_ROWS(h_64, false, 2)
+}
+
+// dx = ds W^T: blocks of 128 features by slices of the vocabulary, a slice's sums to [slice][rows][H]; padding gets zeros whatever W holds
+template <bool ALONG_H, int NT>
+__device__ __forceinline__ void rows_dx_body(float* __restrict__ dx, const float* __restrict__ ds, const float* __restrict__ w, const int32_t* __restrict__ tokens, const RowsParams& P) {
+    using Product = RowsProduct<NT>;
+    __shared__ typename Product::Shared shared;
+    const uint32_t tiles = (P.H + 127u) / 128u, h0 = blockIdx.x % tiles * 128u, slice = blockIdx.x / tiles, group = ALONG_H ? 8u : 32u, groups = (P.V + group - 1u) / group;
+    uint32_t r_at[NT];
+    bool there[NT];
+    rows_there<NT>(r_at, there, tokens, P);
+    Product product;
+    product.template multiply<ALONG_H>(shared, w, ds, h0, P.H, P.V, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
+    if (threadIdx.x >= 64u) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+        if (!there[j])
+#pragma unroll
+            for (int i = 0; i < 4; ++i) product.acc[i][j] = f32x16{};
+    product.template store<ALONG_H>(dx + (uint64_t)slice * P.rows * P.H, h0, P.H, P.rows);
+}
+
+// dW[m, n] = sum_r a[r, m] b[r, n], of x and ds or the other way round as dW lies: a wave has 128 n, for which it holds b, and goes through its share of m, 32 at a time; four neighbouring n
+// are a lane's. Bound by the writing of dW (64 rows: as much by the products).
+struct OuterParams { uint32_t rows, M, N, V, steps, tiles_n, tasks, pad; };
+// (ROWS: 8, 16, 32 or 64. Everything is loaded without a branch, and whole steps are stored without one: a wait for a step's loads would be one for the stores too.)
+template <int ROWS>
+__device__ __forceinline__ void rows_dw_body(float* __restrict__ dw, const float* __restrict__ a, const float* __restrict__ b, const int32_t* __restrict__ tokens, const OuterParams& P) {
+    constexpr int STEPS = ROWS / 2;
+    const uint32_t task = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = threadIdx.x >> 5 & 1u, l32 = threadIdx.x & 31u;
+    if (task >= P.tasks) return;
+    // (vectors and rows behind the end are the last ones again, and write the same values once more)
+    const uint32_t n = min(task % P.tiles_n * 128u + 4u * l32, P.N - 4u), first = task / P.tiles_n * P.steps * 32u, m_end = min(P.M, first + P.steps * 32u);
+    f32x4 held[STEPS];
+    uint32_t there = 0;                            // bit k: this lane's row of step k, 2 k + half, is not padding
+#pragma unroll
+    for (uint32_t k = 0; k < STEPS; ++k) {
+        const uint32_t r = 2u * k + half, at = min(r, P.rows - 1u);
+        const int32_t token = tokens[at];
+        there |= (uint32_t)((r < P.rows) & is_token(token, P.V)) << k;
+        held[k] = *reinterpret_cast<const f32x4_anywhere*>(b + (uint64_t)at * P.N + n);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < STEPS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) held[k][e] = there >> k & 1u ? held[k][e] : 0.f;
+    float next[STEPS];
+    auto request = [&](uint32_t m0) {
+        const float* const from = a + min(m0 + l32, P.M - 1u);
+#pragma unroll
+        for (uint32_t k = 0; k < STEPS; ++k) next[k] = from[(uint64_t)min(2u * k + half, P.rows - 1u) * P.M];
+    };
+    auto step = [&](uint32_t m0, bool whole) {
+        float now[STEPS];
+#pragma unroll
+        for (uint32_t k = 0; k < STEPS; ++k) now[k] = there >> k & 1u ? next[k] : 0.f;
+        if (m0 + 32u < m_end) request(m0 + 32u);
+        f32x16 acc[4] = {};
+#pragma unroll
+        for (uint32_t k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(now[k], held[k][i], acc[i], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const uint32_t to = m0 + 8u * (q >> 2) + 4u * half + (q & 3);
+            if (whole || to < P.M) *reinterpret_cast<f32x4_anywhere*>(dw + (uint64_t)to * P.N + n) = f32x4{acc[0][q], acc[1][q], acc[2][q], acc[3][q]};
+        }
+    };
+    request(first);
+    uint32_t m0 = first;
+    for (; m0 + 32u <= m_end; m0 += 32u) step(m0, true);
+    if (m0 < m_end) step(m0, false);
+}
+// (two blocks a CU, one where A is turned for 64 rows: with half the registers those would not hold what is on its way)
+#define ROWS_KERNELS(NAME, ALONG_M, NT)                                                                                                                            \
+    extern "C" __global__ __launch_bounds__(256, ALONG_M || NT == 1 ? 2 : 1)                                                                                       \
+    void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, float* scores, const float* x, const float* w, const int32_t* tokens, RowsParams P) { \
+        scores_rows_body<ALONG_M, NT>(peaks, sums, of_token, scores, x, w, tokens, P);                                                                             \
+    }                                                                                                                                                              \
+    extern "C" __global__ __launch_bounds__(256, !ALONG_M || NT == 1 ? 2 : 1)                                                                                      \
+    void linear_rows_dx_##NAME(float* dx, const float* ds, const float* w, const int32_t* tokens, RowsParams P) {                                                  \
+        rows_dx_body<!ALONG_M, NT>(dx, ds, w, tokens, P);                                                                                                          \
+    }
+ROWS_KERNELS(v_32, true, 1)
+ROWS_KERNELS(v_64, true, 2)
+ROWS_KERNELS(h_32, false, 1)
+ROWS_KERNELS(h_64, false, 2)
+#define ROWS_DW(ROWS) extern "C" __global__ __launch_bounds__(256) void linear_rows_dw_##ROWS(float* dw, const float* a, const float* b, const int32_t* tokens, OuterParams P) { \
+        rows_dw_body<ROWS>(dw, a, b, tokens, P);                                                                                                                   \
+    }
+ROWS_DW(8)
+ROWS_DW(16)
+ROWS_DW(32)
+ROWS_DW(64)
 
 // ---- backward: a piece's q, as operands contracted over the vocabulary [rows][tokens] and over the rows [tokens][rows]
 template <int T, int STAGES, bool SHARED>
@@ -511,17 +712,28 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
     }
 LINEAR_KERNELS(LINEAR_PRODUCT)
 
+// ---- the slices of a contraction added up; with few elements by four waves, a quarter of the slices each
 struct SumParams { uint32_t parts, pad; uint64_t n; };
-extern "C" __global__ __launch_bounds__(256) void linear_sum(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {
-    const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    if (at >= P.n) return;
+__device__ __forceinline__ float sum_of(const float* __restrict__ parts, uint64_t at, uint64_t n, uint32_t begin, uint32_t end) {
     float s = 0.f;
-    for (uint32_t k0 = 0; k0 < P.parts; k0 += 8u) {
+    for (uint32_t k0 = begin; k0 < end; k0 += 8u) {
         float v[8];
 #pragma unroll
-        for (uint32_t k = 0; k < 8u; ++k) v[k] = k0 + k < P.parts ? parts[(k0 + k) * P.n + at] : 0.f;
+        for (uint32_t k = 0; k < 8u; ++k) v[k] = k0 + k < end ? parts[(k0 + k) * n + at] : 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) s += v[k];
     }
-    out[at] = s;
+    return s;
+}
+extern "C" __global__ __launch_bounds__(256) void linear_sum(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {
+    const uint64_t at = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (at < P.n) out[at] = sum_of(parts, at, P.n, 0u, P.parts);
+}
+extern "C" __global__ __launch_bounds__(256) void linear_sum_few(float* __restrict__ out, const float* __restrict__ parts, SumParams P) {
+    __shared__ float met[4][64];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const uint64_t at = (uint64_t)blockIdx.x * 64u + lane;
+    met[wave][lane] = at < P.n ? sum_of(parts, at, P.n, P.parts * wave / 4u, P.parts * (wave + 1u) / 4u) : 0.f;
+    __syncthreads();
+    if (wave == 0u && at < P.n) out[at] = (met[0][lane] + met[1][lane]) + (met[2][lane] + met[3][lane]);
 }

@@ -2793,10 +2793,56 @@ def _linear_shape(x: Buffer, w: Buffer, transposed: bool) -> LinearShape:
     return shape
 
 
-def linear_parts(x_shape, w_shape, transposed: bool) -> tp.Tuple[int, int, int]:
-    '''Words of the weights and of x, taken apart for the scores' product, and of their scales.'''
+def _linear_few(rows: int, h: int, v: int) -> bool:
+    return rows <= LINEAR_ROWS and min(h, v) >= 4
+
+
+def linear_parts(x_shape, w_shape, transposed: bool) -> tp.List[tp.Tuple[int, type]]:
+    '''(elements, type) of what a gradient takes from the forward pass: the weights and x, taken apart for the scores' product, and their scales - or the scores of few rows.'''
     h, v = reversed(w_shape) if transposed else w_shape
-    return _half_words(v, h), _half_words(math.prod(x_shape) // h, h), 4
+    rows = math.prod(x_shape) // h
+    if _linear_few(rows, h, v):
+        return [(rows * v, np.float32)]
+    return [(_half_words(v, h), np.uint32), (_half_words(rows, h), np.uint32), (4, np.int32)]
+
+
+def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, of_tiles, scores) -> Launch:
+    rows, h, v = shape
+    return Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (_cdiv(v, 128), 1, 1), (BLOCK, 1, 1),
+                  [(b, 0) for b in (*of_tiles, scores, x, w, tokens)], _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2, 3))
+
+
+def _linear_rows_grad(dx, dw, shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch,
+                      scores) -> tp.List[Launch]:
+    rows, h, v = shape
+    launches, suffix = [], 32 if rows <= 32 else 64
+    if scores is None:
+        scores = scratch((rows, v))
+        launches.append(_linear_rows_scores(shape, x, w, tokens, transposed, (None, None, None), scores))
+    ds = scratch((rows, v))
+    launches.append(Launch('linear_rows_ds', (_cdiv(v, 1024), rows, 1), (BLOCK, 1, 1), [(b, 0) for b in (ds, scores, tokens, peaks, totals, g_log_probs, g_log_sums)], _u32(rows, h, v, 0),
+                           bytes_moved=8 * rows * v))
+    #slices of the vocabulary, of four times the rows at least (their sums are written and read once more) and enough for the chip
+    slices = max(1, min(2 * HALF_CUS // _cdiv(h, 128), v // (4 * suffix)))
+    sums   = scratch((slices, rows, h)) if slices > 1 else dx
+    launches.append(Launch(f'linear_rows_dx_{"h" if transposed else "v"}_{suffix}', (_cdiv(h, 128) * slices, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (sums, ds, w, tokens)],
+                           _u32(rows, h, v, slices), bytes_moved=4 * (w.size + rows * v + slices * rows * h), flops=2 * rows * h * v))
+    if slices > 1:
+        launches.append(_linear_sum(dx, sums, slices, rows * h))
+    #dw: steps of 32 rows of it a wave, so many that what the wave holds is read seldom, with waves enough for the chip (a step each: 64 x 1024 x 32000 23 us more, 15 x 1973 x 128040 40 less)
+    a, b, m, n = (ds, x, v, h) if transposed else (x, ds, h, v)
+    tiles_n = _cdiv(n, 128)
+    steps   = max(1, min(16, tiles_n * _cdiv(m, 32) // (8 * HALF_CUS)))
+    tasks   = tiles_n * _cdiv(m, 32 * steps)
+    launches.append(Launch(f'linear_rows_dw_{max(8, _pow2_at_least(rows))}', (_cdiv(tasks, 4), 1, 1), (BLOCK, 1, 1), [(b_, 0) for b_ in (dw, a, b, tokens)], _u32(rows, m, n, v, steps, tiles_n, tasks, 0),
+                           bytes_moved=4 * (dw.size + rows * (h + v)), flops=2 * rows * h * v))
+    return launches
+
+
+def _linear_sum(out, parts: Buffer, count: int, n: int) -> Launch:
+    few = n <= 1 << 16
+    return Launch('linear_sum_few' if few else 'linear_sum', (_cdiv(n, 64 if few else BLOCK), 1, 1), (BLOCK, 1, 1), [(out, 0), (parts, 0)], _u32(count, 0) + _u64(n),
+                  bytes_moved=4 * (count + 1) * n)
 
 
 def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, known=None, cotangents=None):
@@ -2847,12 +2893,11 @@ def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, t
     shape = rows, h, v = _linear_shape(x, w, transposed)
     tiles    = _cdiv(v, 64)
     of_tiles = [scratch((tiles, rows)), scratch((tiles, rows)), scratch((rows,))]           #peak and sum of each tile's scores, the token's score
-    if rows <= LINEAR_ROWS and v >= 4 and not parts:
+    if _linear_few(rows, h, v):
         tiles    = _cdiv(v, 128)
-        launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles, 1, 1), (512, 1, 1), [(b, 0) for b in (*of_tiles, x, w, tokens)],
-                           _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2))]
+        launches = [_linear_rows_scores(shape, x, w, tokens, transposed, of_tiles, *(parts or [None]))]
     else:
-        w_parts, x_parts, scales = parts or [scratch((n,), dtype) for n, dtype in zip(linear_parts(x.shape, w.shape, transposed), (np.uint32, np.uint32, np.int32))]
+        w_parts, x_parts, scales = parts or [scratch((n,), dtype) for n, dtype in linear_parts(x.shape, w.shape, transposed)]
         launches, _ = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts))
         scores, side = _linear_scores_launch('linear_scores', shape, v, lambda side: 0, 0, (*of_tiles, w_parts, x_parts, tokens, scales), (0, 1, 2), 3, scratch, zeroed)
         launches.append(scores)
@@ -2866,12 +2911,14 @@ def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, t
 def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch, zeroed,
                           parts=None) -> tp.List[Launch]:
     shape = rows, h, v = _linear_shape(x, w, transposed)
+    if _linear_few(rows, h, v):
+        return _linear_rows_grad(dx, dw, shape, x, w, tokens, peaks, totals, g_log_probs, g_log_sums, transposed, scratch, *(parts or [None]))
     scales = scratch((4,), np.int32)                       #of all that is taken apart here
     if parts:
         w_parts, x_parts, score_scales = parts
         launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None, score_scales, (g_log_probs, g_log_sums))
     else:
-        w_parts, x_parts = [scratch((n,), np.uint32) for n in linear_parts(x.shape, w.shape, transposed)[:2]]
+        w_parts, x_parts = [scratch((n,), np.uint32) for n, _ in linear_parts(x.shape, w.shape, transposed)[:2]]
         score_scales = scales
         launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts), None, (g_log_probs, g_log_sums))
     #pieces of the vocabulary, of whole tiles
@@ -2913,7 +2960,7 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         else:
             launches.append(product(dw, v0, x_scaled, by_token, h, n, row_blocks, _cdiv(h, 32), tiles * 4, steps, steps, 0, _PACK_SCALED, -1, v))
     if parts:
-        launches.append(Launch('linear_sum', (_cdiv(rows * h, BLOCK), 1, 1), (BLOCK, 1, 1), [(dx, 0), (sums, 0)], _u32(parts, 0) + _u64(rows * h), bytes_moved=4 * (sums.size + rows * h)))
+        launches.append(_linear_sum(dx, sums, parts, rows * h))
     return launches
 
 

@@ -800,24 +800,24 @@ def _linear_log_probs_operands(name, x, weights, tokens, transposed):
 
 
 def _linear_log_probs_parts(x, weights, transposed):
-    '''What linear_log_probs keeps of its operands for a gradient: the weights and x as the matrix cores take them, and their scales.'''
+    '''What linear_log_probs keeps for a gradient: the weights and x as the matrix cores take them, and their scales - or the scores of few rows.'''
     from .. import kernels
-    return [_aval((n,), dtype) for n, dtype in zip(kernels.linear_parts(_shape(x), _shape(weights), transposed), (_u32, _u32, _i32))]
+    return [_aval((n,), np.dtype(dtype)) for n, dtype in kernels.linear_parts(_shape(x), _shape(weights), transposed)]
 
 
 def linear_log_probs(x, weights, tokens, transposed: bool = False, with_parts: bool = False):
     '''For rows x [..., hidden], weights [hidden, vocabulary] (`transposed`: [vocabulary, hidden]) and one token per row, with scores = x @ weights: (log softmax(scores)[token],
     log(sum(exp(scores)))), and what linear_log_probs_grad needs of them: each row's largest score and the sum of exp(scores - largest), all [...]. The scores are
-    not kept. `nn.linear_log_probs` says what becomes of padded rows and how exact the products are. With `with_parts` also, behind them, the operands as its products
-    take them (three arrays of words, which are for linear_log_probs_grad alone).'''
+    not kept. `nn.linear_log_probs` says what becomes of padded rows and how exact the products are. With `with_parts` also, behind them, what spares linear_log_probs_grad
+    work (arrays that are for it alone: the operands as the products take them, or the scores of few rows).'''
     x, weights, tokens = _linear_log_probs_operands('linear_log_probs', x, weights, tokens, transposed)
     avals = [_aval(_shape(tokens), _f32)] * 4 + (_linear_log_probs_parts(x, weights, transposed) if with_parts else [])
     return tuple(emit('linear_log_probs', [x, weights, tokens], avals, dict(transposed=bool(transposed), parts=bool(with_parts)), multiple_results=True))
 
 
 def linear_log_probs_grad(x, weights, tokens, peaks, totals, g_log_probs=None, g_log_sums=None, transposed: bool = False, parts=None):
-    '''(dx, dweights) for the cotangents (None: zeros) of linear_log_probs' first two results; peaks and totals are the next two, and parts the three behind them, of the same x,
-    weights and tokens, where it was called `with_parts` (without them x and weights are taken apart again).'''
+    '''(dx, dweights) for the cotangents (None: zeros) of linear_log_probs' first two results; peaks and totals are the next two, and parts those behind them, of the same x,
+    weights and tokens, where it was called `with_parts` (without them that work is done again).'''
     name = 'linear_log_probs_grad'
     x, weights, tokens = _linear_log_probs_operands(name, x, weights, tokens, transposed)
     rows = _shape(tokens)
@@ -825,7 +825,7 @@ def linear_log_probs_grad(x, weights, tokens, peaks, totals, g_log_probs=None, g
     operands += [_shaped_operand(name, 'a cotangent', v, rows) for v in (g_log_probs, g_log_sums) if v is not None]
     if parts is not None:
         avals = _linear_log_probs_parts(x, weights, transposed)
-        if len(parts) != 3 or builtins.any((_shape(v), dtype_of(v)[0]) != (a.shape, a.dtype) for v, a in zip(parts, avals)):
+        if len(parts) != len(avals) or builtins.any((_shape(v), dtype_of(v)[0]) != (a.shape, a.dtype) for v, a in zip(parts, avals)):
             raise TypeError(f'{name}: the parts must be {[f"{a.dtype} {a.shape}" for a in avals]}')
         operands += list(parts)
     return tuple(emit(name, operands, [_aval(_shape(x), _f32), _aval(_shape(weights), _f32)],
