@@ -808,7 +808,7 @@ def _linear_log_probs_parts(x, weights, transposed):
 def linear_log_probs(x, weights, tokens, transposed: bool = False, with_parts: bool = False):
     '''For rows x [..., hidden], weights [hidden, vocabulary] (`transposed`: [vocabulary, hidden]) and one token per row, with scores = x @ weights: (log softmax(scores)[token],
     log(sum(exp(scores)))), and what linear_log_probs_grad needs of them: each row's largest score and the sum of exp(scores - largest), all [...]. The scores are
-    not kept. `nn.linear_log_probs` says what becomes of padded rows and how exact the products are. With `with_parts` also, behind them, what spares linear_log_probs_grad
+    not kept (those of up to 64 rows are, for a gradient). `nn.linear_log_probs` says what becomes of padded rows and how exact the products are. With `with_parts` also, behind them, what spares linear_log_probs_grad
     work (arrays that are for it alone: the operands as the products take them, or the scores of few rows).'''
     x, weights, tokens = _linear_log_probs_operands('linear_log_probs', x, weights, tokens, transposed)
     avals = [_aval(_shape(tokens), _f32)] * 4 + (_linear_log_probs_parts(x, weights, transposed) if with_parts else [])

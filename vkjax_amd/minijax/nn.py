@@ -96,11 +96,11 @@ def selective_scan(x, delta, a, b, c, d=None, gate=None, state=None, lengths=Non
 def linear_log_probs(x, weights, tokens, transposed=False):
     '''Log probabilities of given tokens (or classes) under softmax(x @ weights), without keeping the scores: x [..., hidden], weights [hidden, vocabulary], or with `transposed` the
     rows of an embedding, [vocabulary, hidden]; tokens int32 [...]. Returns (log_probs [...], log_sums [...]), the latter being log(sum(exp(scores))) of each row. A cross entropy is
-    -log_probs; the gradient works the scores out again, a piece of the vocabulary at a time.
+    -log_probs; the gradient works the scores out again, a piece of the vocabulary at a time. (Of up to 64 rows it takes the scores of the forward pass.)
 
     * A row whose token lies outside the vocabulary (negative, say) is padding: its results are 0, no gradient comes from it, and its x is not looked at.
     * Products are as exact as fp32's for numbers down to 2^-28 of the largest of their operand (x's given rows, the weights); smaller ones are off by up to 2^-51 of that
-      largest. (Up to 64 rows, without a gradient, are computed by fp32 products.)
+      largest. (Up to 64 rows are computed by fp32 products.)
     * NaN and infinities in a row of x make that row's results NaN, in the weights those of every row.
 
     Differentiable with respect to x and weights, through both results.'''
