@@ -218,6 +218,20 @@ def test_selective_scan_keeps_what_is_not_finite_to_its_channel():
     assert np.array_equal(np.isnan(y), broken) and np.isnan(last[0, 66]).all() and np.isfinite(last).sum() == last.size - 16
 
 
+def test_selective_scan_with_states_that_are_forgotten_at_once():
+    #a factor of 0 per step; a sequence's state stays from its length on, which is no multiple of anything here
+    for time in (1, 13, 300):
+        arrays, _, _ = scan_inputs(3, time, 70, 5, ('state',), False)
+        arrays['a'][::7] = -np.inf
+        lengths = np.array([time, 0, time // 2], np.int32)
+        (y, last), expected, _ = both(lambda *v: nn.selective_scan(**dict(zip(arrays, v)), lengths=lengths), *arrays.values())
+        assert np.isfinite(y).all() and np.isfinite(last).all() and np.array_equal(last[1], arrays['state'][1])
+        #(one addition, and a sum of five states)
+        close(last[:, ::7], expected[1][:, ::7], 4 * U * np.abs(expected[1][:, ::7]) + 1e-37)
+        size = 0.2 * np.abs(arrays['x'][:, :, ::7]) * (np.abs(arrays['b']) * np.abs(arrays['c'])).sum(axis=2, keepdims=True)
+        close(y[0][:, ::7], expected[0][0][:, ::7], 8 * U * size[0] + 1e-37)
+
+
 # ------------------------------------------------------------------ log probabilities from weights
 
 def product_error(a, b, terms):
@@ -302,6 +316,16 @@ def test_linear_log_probs_of_numbers_far_apart():
     x, w, tokens, g, gs = loss_inputs(150, 60, 700, False)
     x[:, 0], w[0] = 1.0, np.linspace(-40, 0, 700)
     check_loss(x, w, tokens, g, gs, False)
+
+
+@pytest.mark.parametrize('large,small', [(1e33, 1e-33), (1e-33, 1e33), (1e-20, 1e20)])
+@pytest.mark.parametrize('rows', [40, 150])
+def test_linear_log_probs_of_rows_and_weights_of_different_sizes(rows, large, small):
+    x, w, tokens, g, gs = loss_inputs(rows, 60, 700, False)
+    x, w = (x * large).astype(f32), (w * small).astype(f32)
+    got, expected, _ = both(lambda x, w, t: nn.linear_log_probs(x, w, t), x, w, tokens)
+    for name, a, b, bound in zip(('log_probs', 'log_sums'), got, expected, loss_bounds(x, w, tokens, g, gs, False)):
+        close(a, b, bound, name)
 
 
 def test_linear_log_probs_of_one_result_only():

@@ -17,6 +17,8 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int Q_SCALE = 13;                              // |q| <= 2
 
 __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * LOG2E); }
+// (two operands' scales at once: one after the other, a factor beyond fp32's range would meet a number that is inside it in the end)
+__device__ __forceinline__ float scaled(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
 __device__ __forceinline__ bool is_token(int32_t t, uint32_t V) { return (uint32_t)t < V; }
 typedef f32x4 f32x4_anywhere __attribute__((aligned(4)));
 
@@ -171,7 +173,7 @@ __device__ __forceinline__ void linear_scores_body(float* __restrict__ peaks, fl
     half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
-    const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]);
+    const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
     float (*const met)[SIDE][2] = reinterpret_cast<float (*)[SIDE][2]>(&shared.stages[0]);  // [wm][column][peak, sum]
     const uint32_t v0 = m * SIDE + wm * 32u * T + 4u * (lane >> 5);
 #pragma unroll
@@ -185,7 +187,7 @@ __device__ __forceinline__ void linear_scores_body(float* __restrict__ peaks, fl
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
                 const uint32_t v = v0 + 32u * i + 8u * (q >> 2) + (q & 3);
-                float s = half_sum(acc, i, j, q) * down_w * down_x;
+                float s = scaled(half_sum(acc, i, j, q), down);
                 if (v == (uint32_t)token) { mine = s; has = true; }
                 s = v < P.V ? s : -__builtin_inff();
                 acc.large[i][j][q] = s;
@@ -627,7 +629,8 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4*
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
-    const float down_w = power_of_two(-scales[PACK_WEIGHTS]), down_x = power_of_two(-scales[PACK_ROWS]), up = power_of_two(Q_SCALE);
+    const float up = power_of_two(Q_SCALE);
+    const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
     const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * SIDE;
     // of this lane's columns
     bool given[T];
@@ -643,7 +646,7 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4*
     half_store<T>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 2u * T, n * 4u * T},
                   [&](int i, int j, int k, uint32_t row, uint32_t) {
         const uint32_t v = v0 + row;
-        const float s = half_sum(acc, i, j, k) * down_w * down_x;
+        const float s = scaled(half_sum(acc, i, j, k), down);
         const float q = part[j] * exp_of(s - peak[j]) + (v == token[j] ? one[j] : 0.f);
         return given[j] && v < P.V ? q : 0.f;
     });
@@ -675,7 +678,7 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = (m * 2u + (wave >> 1)) * 32u * T + 4u * (lane >> 5), lane_column = (n * 2u + (wave & 1u)) * 32u * T + (lane & 31u);
-    const float down = power_of_two(-(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a])), down_b = power_of_two(-(P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]));
+    const int down = -(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a]) - (P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]);
     float* const to = out + (SHARED ? 0u : P.slice * slice);
 #pragma unroll
     for (int i = 0; i < T; ++i) {
@@ -698,7 +701,7 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
             for (int j = 0; j < T; ++j) {
                 const uint32_t column = lane_column + 32u * j;
                 if (column >= P.N) continue;
-                float s = half_sum(acc, i, j, q) * down * down_b;
+                float s = scaled(half_sum(acc, i, j, q), down);
                 if (factors) s = f == 0.f ? 0.f : s * f;
                 to[P.ld * row + column] = s + before[j][q];
             }

@@ -28,6 +28,11 @@ struct ScanParams {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+// a as the factor of an exponent of 2, one that is infinite as the largest number, whose product with a width of zero (of a step that is not taken) is zero
+__device__ __forceinline__ float factor_of(float a) {
+    const float v = a * LOG2E;
+    return __builtin_fabsf(v) == __builtin_inff() ? __builtin_copysignf(3.4028234e38f, v) : v;
+}
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp2_of(z * -LOG2E)); }        // (see norm.hip)
 // log(1 + exp(v)) = max(v, 0) + log(1 + q), q = exp(-|v|) in (0, 1]: the logarithm as 2 atanh(s), s = q / (2 + q) <= 1/3, by its series up to s^15 (the rest is below 2e-9 of it),
 // so that it keeps its bits also where q is small.
@@ -84,7 +89,7 @@ struct Place {
     }
     __device__ void factors(float (&a2)[NS], const float* __restrict__ a, const ScanParams& P) const {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) a2[i] = has(P, i) ? a[(int64_t)c * P.N + n0 + i] * LOG2E : 0.f;
+        for (int i = 0; i < NS; ++i) a2[i] = has(P, i) ? factor_of(a[(int64_t)c * P.N + n0 + i]) : 0.f;
     }
     // behind a wave's writes to shared memory, in front of other waves' reads (of one wave: nothing to wait for but its own writes)
     __device__ static void meet() { if constexpr (M > 1) __syncthreads(); else __builtin_amdgcn_wave_barrier(); }
@@ -150,7 +155,7 @@ extern "C" __global__ __launch_bounds__(64) void selective_scan_join(float* __re
                                                                      const float* __restrict__ initial, ScanJoinParams P) {
     const uint32_t id = blockIdx.x * 64u + threadIdx.x, c = id % P.C, rest = id / P.C, n = rest % P.N, b = rest / P.N;
     if (b >= P.B) return;
-    const float a2 = a[(int64_t)c * P.N + n] * LOG2E;
+    const float a2 = factor_of(a[(int64_t)c * P.N + n]);
     const int64_t at = ((int64_t)b * P.C + c) * P.N + n, each = (int64_t)P.B * P.N * P.C, first = ((int64_t)b * P.N + n) * P.C + c;
     const int64_t s_each = (int64_t)P.B * P.C, s_first = (int64_t)b * P.C + c;
     float h = initial ? initial[at] : 0.f;
@@ -288,7 +293,7 @@ extern "C" __global__ __launch_bounds__(256) void selective_scan_step(float* __r
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            h[i] = __builtin_fmaf(exp2_of(as[i] * LOG2E * dt), h[i], u * bs[i]);
+            h[i] = __builtin_fmaf(exp2_of(factor_of(as[i]) * dt), h[i], u * bs[i]);
             sum = __builtin_fmaf(cs[i], h[i], sum);
         }
         out = sum;
