@@ -87,7 +87,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_largest(float* __restri
 enum PackKind : uint32_t { PACK_WEIGHTS = 0, PACK_ROWS = 1, PACK_SCALED = 2 };
 struct PackJob { uint32_t blocks, I, K, stride, kind, steps; uint64_t si, sk; };      // blocks of 256 threads; steps of 16 k; element strides of i and k; `stride`: steps that a wave takes
 struct PackParams { uint32_t weight_blocks, row_blocks, V, pad; PackJob jobs[4]; };
-struct PackOuts { u32x4* parts[4]; };
+struct PackOuts { void* parts[4]; };
 extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int32_t* __restrict__ scales, const float* __restrict__ x, const float* __restrict__ w,
                                                               const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors,
                                                               const int32_t* __restrict__ known, PackParams P) {
@@ -119,7 +119,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
     // (the operands of four steps at once)
     constexpr int AT_ONCE = 4;
     const uint32_t end = min(J.steps, (group + 1u) * J.stride);
-    u32x4* const to = outs.parts[job] + (uint64_t)rb * J.steps * 128u + lane;
+    u32x4* const to = reinterpret_cast<u32x4*>(outs.parts[job]) + (uint64_t)rb * J.steps * 128u + lane;
     for (uint32_t s0 = group * J.stride; s0 < end; s0 += AT_ONCE) {
         float v[AT_ONCE][8];
 #pragma unroll
@@ -154,7 +154,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
 }
 
 // ---- forward: a tile's peak and sum per row of x, [tile of tokens][rows]
-struct ScoresParams { uint32_t rows, V, pairs, steps_w, steps_x, tiles_m, tiles_n, blocks_w, blocks_x, tile0, Vp; HalfShares shares; };
+struct ScoresParams { uint32_t rows, V, pairs, steps_w, steps_x, tiles_m, tiles_n, blocks_w, blocks_x, tile0, Vp, whole, slices; };
 
 __device__ __forceinline__ HalfOperand operand_of(const u32x4* parts, uint32_t blocks, uint32_t stride, uint32_t first = 0) { return HalfOperand{parts, blocks, stride, first}; }
 __device__ __forceinline__ float over_halves_max(float v) { return fmaxf(v, lane_xor<32>(v)); }
@@ -167,11 +167,11 @@ __device__ __forceinline__ void linear_scores_body(float* __restrict__ peaks, fl
     constexpr uint32_t SIDE = HalfTileOf<T>::SIDE;
     __shared__ HalfShared<T, STAGES> shared;
     uint32_t m, n, tile, slice, begin, end;
-    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, begin, end - begin);
-    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
     float (*const met)[SIDE][2] = reinterpret_cast<float (*)[SIDE][2]>(&shared.stages[0]);  // [wm][column][peak, sum]
@@ -454,8 +454,8 @@ template <int NT> struct RowsProduct {
     }
 };
 
-struct RowsParams { uint32_t rows, H, V, slices; };
-template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT], bool (&there)[NT], const int32_t* __restrict__ tokens, const RowsParams& P) {
+struct LinearRowsParams { uint32_t rows, H, V, slices; };
+template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT], bool (&there)[NT], const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const uint32_t r = 32u * j + (threadIdx.x & 31u);
@@ -467,7 +467,7 @@ template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT
 // forward: 128 tokens' scores, their peak and sum per row; the scores [rows][V] themselves for a gradient
 template <bool ALONG_V, int NT>
 __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ scores, const float* __restrict__ x,
-                                                 const float* __restrict__ w, const int32_t* __restrict__ tokens, const RowsParams& P) {
+                                                 const float* __restrict__ w, const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
     using Product = RowsProduct<NT>;
     __shared__ typename Product::Shared shared;
     const uint32_t lane = threadIdx.x & 63u, v0 = blockIdx.x * 128u;
@@ -510,7 +510,7 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
 
 // backward: ds [rows][V] from the scores, zeros for padding
 extern "C" __global__ __launch_bounds__(256) void linear_rows_ds(float* __restrict__ ds, const float* __restrict__ scores, const int32_t* __restrict__ tokens, const float* __restrict__ row_peaks,
-                                                                 const float* __restrict__ row_totals, const float* __restrict__ g_log_probs, const float* __restrict__ g_log_sums, RowsParams P) {
+                                                                 const float* __restrict__ row_totals, const float* __restrict__ g_log_probs, const float* __restrict__ g_log_sums, LinearRowsParams P) {
     const uint32_t r = blockIdx.y;
     const int32_t token = tokens[r];
     const bool given = is_token(token, P.V);
@@ -525,7 +525,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_rows_ds(float* __restri
 
 // dx = ds W^T: blocks of 128 features by slices of the vocabulary, a slice's sums to [slice][rows][H]; padding gets zeros whatever W holds
 template <bool ALONG_H, int NT>
-__device__ __forceinline__ void rows_dx_body(float* __restrict__ dx, const float* __restrict__ ds, const float* __restrict__ w, const int32_t* __restrict__ tokens, const RowsParams& P) {
+__device__ __forceinline__ void rows_dx_body(float* __restrict__ dx, const float* __restrict__ ds, const float* __restrict__ w, const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
     using Product = RowsProduct<NT>;
     __shared__ typename Product::Shared shared;
     const uint32_t tiles = (P.H + 127u) / 128u, h0 = blockIdx.x % tiles * 128u, slice = blockIdx.x / tiles, group = ALONG_H ? 8u : 32u, groups = (P.V + group - 1u) / group;
@@ -597,11 +597,11 @@ __device__ __forceinline__ void rows_dw_body(float* __restrict__ dw, const float
 // (two blocks a CU, one where A is turned for 64 rows: with half the registers those would not hold what is on its way)
 #define ROWS_KERNELS(NAME, ALONG_M, NT)                                                                                                                            \
     extern "C" __global__ __launch_bounds__(256, ALONG_M || NT == 1 ? 2 : 1)                                                                                       \
-    void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, float* scores, const float* x, const float* w, const int32_t* tokens, RowsParams P) { \
+    void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, float* scores, const float* x, const float* w, const int32_t* tokens, LinearRowsParams P) { \
         scores_rows_body<ALONG_M, NT>(peaks, sums, of_token, scores, x, w, tokens, P);                                                                             \
     }                                                                                                                                                              \
     extern "C" __global__ __launch_bounds__(256, !ALONG_M || NT == 1 ? 2 : 1)                                                                                      \
-    void linear_rows_dx_##NAME(float* dx, const float* ds, const float* w, const int32_t* tokens, RowsParams P) {                                                  \
+    void linear_rows_dx_##NAME(float* dx, const float* ds, const float* w, const int32_t* tokens, LinearRowsParams P) {                                                  \
         rows_dx_body<!ALONG_M, NT>(dx, ds, w, tokens, P);                                                                                                          \
     }
 ROWS_KERNELS(v_32, true, 1)
@@ -624,11 +624,11 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4*
     constexpr uint32_t SIDE = HalfTileOf<T>::SIDE;
     __shared__ HalfShared<T, STAGES> shared;
     uint32_t m, n, tile, slice, begin, end;
-    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, begin, end - begin);
-    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const float up = power_of_two(Q_SCALE);
     const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
     const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * SIDE;
@@ -663,7 +663,7 @@ LINEAR_KERNELS(LINEAR_Q)
 struct ProductParams {
     uint32_t M, N, tiles_m, tiles_n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b, add;
     int32_t scale_a, scale_b;                            // the kind of operand whose scale it is, or -1: q
-    HalfShares shares;
+    uint32_t whole, slices;                              // (HalfShares)
     uint64_t ld, slice;                                  // elements from a row of the result to the next, from a slice's result to the next one's
 };
 template <int T, int STAGES, bool SHARED>
@@ -671,11 +671,11 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
                                                     const int32_t* __restrict__ scales, const float* __restrict__ factors, const ProductParams& P) {
     __shared__ HalfShared<T, STAGES> shared;
     uint32_t m, n, tile, slice, begin, end;
-    half_work(blockIdx.x, P.shares, P.pairs, tile, slice, begin, end);
+    half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
-    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = (m * 2u + (wave >> 1)) * 32u * T + 4u * (lane >> 5), lane_column = (n * 2u + (wave & 1u)) * 32u * T + (lane & 31u);
     const int down = -(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a]) - (P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]);

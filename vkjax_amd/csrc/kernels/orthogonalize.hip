@@ -97,7 +97,7 @@ enum OrthogonalKind : uint32_t { SQUARE = 0, POLYNOMIAL = 1, NEXT = 2, LAST = 3 
 struct OrthogonalParams {
     uint32_t kind, M, N, K, tiles_m, tiles_n, tiles;     // tiles of a matrix: those on and above the diagonal of a square
     int32_t scale_a, scale_b, scale_out;
-    float a, b, c; HalfShares shares; uint32_t pad;
+    float a, b, c; uint32_t whole, slices, pad;          // (HalfShares)
     uint64_t sr, sc;                                     // the last result's element strides
 };
 // (kinds in templates: their epilogues share no registers)
@@ -109,7 +109,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     constexpr uint32_t SIDE = 64u * T;
     const uint32_t steps_k = 2u * ((P.K + 31u) / 32u), blocks_m = (P.M + 31u) / 32u, blocks_n = (P.N + 31u) / 32u, steps_m = 2u * blocks_m, steps_n = 2u * blocks_n;
     uint32_t tile, slice, begin, end, m, n;
-    half_work(blockIdx.x, P.shares, steps_k / 2u, tile, slice, begin, end);
+    half_work(blockIdx.x, HalfShares{P.whole, P.slices}, steps_k / 2u, tile, slice, begin, end);
     const uint32_t matrix = tile / P.tiles, at = tile - matrix * P.tiles;
     if constexpr (SYMMETRIC) {
         // column by column of the triangle: n (n + 1) / 2 tiles in front of column n
@@ -121,7 +121,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     HalfSums<T> acc = {};
     half_product<T, STAGES>(acc, shared, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u},
                             HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
-    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, P.shares)) return;
+    if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
     const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = row0 + (wave >> 1) * 32u * T + 4u * (lane >> 5), lane_column = column0 + (wave & 1u) * 32u * T + (lane & 31u);
@@ -174,6 +174,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
 ORTHOGONAL_KINDS(_128, 2, 2, 2, false)
 ORTHOGONAL_KINDS(_128_shared, 2, 2, 2, true)
 ORTHOGONAL_KINDS(_64, 1, 4, 2, false)
-ORTHOGONAL_KINDS(_64_shared, 1, 4, 2, true)
+// (of the others half_plan shares none: their contractions are as long as the matrix has rows, and where that is long there are tiles enough)
+ORTHOGONAL(square, SQUARE, _64_shared, 1, 4, 2, true)
 ORTHOGONAL_KINDS(_64_many, 1, 2, 4, false)
 ORTHOGONAL_KINDS(_64_many_shared, 1, 2, 4, true)
