@@ -7,6 +7,8 @@
 // A thread has VEC channels and L steps that follow one another: it loads its rows and the K - 1 before them into registers at once (neighbouring
 // threads' rows overlap by those, which the caches serve) and goes through its steps from there. The gradient needs K - 1 steps on either side and works their
 // d out again. Lanes lie along channels: whole lines of 128 bytes wherever there are 32 channels. Bound by memory: 8 bytes a value, 12 with the gradient.
+// 8 x 2048 x 2048, 4 taps, silu, sequences of up to 2048 steps: forward 47 us, gradient 103 and 5 for the sums (what lies inside the lengths, at 4.9 TB/s: 97 us for both). One token of 64
+// sequences 3.6 us: a launch. Eight steps a thread, whose K - 1 rows in front come from the caches.
 // Sums over time (dw, dbias) are those of a thread's steps, then of the threads of a block, which walks `turns` tiles of time, then of the blocks in their order by
 // a second launch: no atomics.
 #include "common.h"
