@@ -8,11 +8,13 @@ import pytest
 
 from tests.test_gpu_token_model_operators import CONVS, LOSSES, MATRICES, SCANS
 from tests.test_operator_plans import TOOLS, buffer, kernels_of, log_int, scratch
-from vkjax_amd import kernels as K
+from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.csrc import build
+from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
 MODULES = ('causal_conv', 'selective_scan', 'linear_log_probs', 'orthogonalize')
 f32 = np.float32
+nn = mj.nn
 
 
 def zeroed(n, use):
@@ -155,3 +157,31 @@ def test_what_a_gradient_of_log_probs_holds_at_a_time():
         blocks = -(-rows // 32) * 32
         #q both ways, the operands of the other products, slices of dx
         assert max(taken) <= max(K.LINEAR_PIECE, 4 * 128 * (blocks + 128), 4 * (h + 32) * (v + 32), 4 * (h + 32) * (blocks + 32), 4 * 64 * rows * h), (taken, rows, h, v)
+
+
+@pytest.mark.parametrize('rows', [20, 300])
+@pytest.mark.parametrize('transposed', [False, True])
+def test_products_that_nobody_reads_are_left_out(rows, transposed):
+    '''Of weights that are not trained, and of rows that no gradient goes on from.'''
+    h, v = 200, 5000
+    x, w, t, r = buffer(rows, h), buffer(*((v, h) if transposed else (h, v))), buffer(rows, dtype=np.int32), buffer(rows)
+    parts = [buffer(n, dtype=d) for n, d in K.linear_parts(x.shape, w.shape, transposed)]
+    flops = [sum(launch.flops for launch in K.linear_log_probs_grad(dx, dw, x, w, t, r, r, r, r, transposed, scratch, zeroed, parts)) for dx, dw in ((x, w), (x, None), (None, w))]
+    assert all(f < 0.75 * flops[0] for f in flops[1:]), flops
+
+
+@pytest.mark.parametrize('which', [(0,), (1,), (0, 1)], ids=str)
+@pytest.mark.parametrize('rows', [20, 300])
+def test_a_program_computes_the_gradients_that_it_returns(rows, which):
+    x, w, t, g = np.zeros((rows, 200), f32), np.zeros((200, 5000), f32), np.zeros(rows, np.int32), np.ones(rows, f32)
+
+    def f(x, w):
+        given = [x, w]
+        return mj.vjp(lambda *a: nn.linear_log_probs(*(a[which.index(i)] if i in which else given[i] for i in range(2)), t)[0], *(given[i] for i in which))[1](g)
+    launched = {launch.kernel for launch in JaxprInterpreter(mj.make_jaxpr(f)(x, w), plan_only=True).launches if launch is not None}
+    products = {n for n in launched if n.startswith(('linear_product', 'linear_rows_d')) and n != 'linear_rows_ds'}
+    if rows == 20:
+        assert {n[:14] for n in products} == {('linear_rows_dx', 'linear_rows_dw')[i] for i in which}
+    else:
+        jobs = [launch for launch in JaxprInterpreter(mj.make_jaxpr(f)(x, w), plan_only=True).launches if launch is not None and launch.kernel.startswith('linear_product')]
+        assert len(jobs) == len(which)

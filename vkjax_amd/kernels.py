@@ -2815,28 +2815,35 @@ def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer
 def _linear_rows_grad(dx, dw, shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch,
                       scores) -> tp.List[Launch]:
     rows, h, v = shape
-    launches, suffix = [], 32 if rows <= 32 else 64
+    launches = []
     if scores is None:
         scores = scratch((rows, v))
         launches.append(_linear_rows_scores(shape, x, w, tokens, transposed, (None, None, None), scores))
     ds = scratch((rows, v))
     launches.append(Launch('linear_rows_ds', (_cdiv(v, 1024), rows, 1), (BLOCK, 1, 1), [(b, 0) for b in (ds, scores, tokens, peaks, totals, g_log_probs, g_log_sums)], _u32(rows, h, v, 0),
                            bytes_moved=8 * rows * v))
+    if dx is not None:
+        launches += _linear_rows_dx(dx, shape, w, tokens, ds, transposed, scratch)
+    if dw is not None:
+        #steps of 32 rows of it a wave, so many that what the wave holds is read seldom, with waves enough for the chip (a step each: 64 x 1024 x 32000 23 us more, 15 x 1973 x 128040 40 less)
+        a, b, m, n = (ds, x, v, h) if transposed else (x, ds, h, v)
+        tiles_n = _cdiv(n, 128)
+        steps   = max(1, min(16, tiles_n * _cdiv(m, 32) // (8 * HALF_CUS)))
+        tasks   = tiles_n * _cdiv(m, 32 * steps)
+        launches.append(Launch(f'linear_rows_dw_{max(8, _pow2_at_least(rows))}', (_cdiv(tasks, 4), 1, 1), (BLOCK, 1, 1), [(b_, 0) for b_ in (dw, a, b, tokens)],
+                               _u32(rows, m, n, v, steps, tiles_n, tasks, 0), bytes_moved=4 * (dw.size + rows * (h + v)), flops=2 * rows * h * v))
+    return launches
+
+
+def _linear_rows_dx(dx, shape: LinearShape, w: Buffer, tokens: Buffer, ds: Buffer, transposed: bool, scratch) -> tp.List[Launch]:
+    rows, h, v = shape
+    suffix = 32 if rows <= 32 else 64
     #slices of the vocabulary, of four times the rows at least (their sums are written and read once more) and enough for the chip
     slices = max(1, min(2 * HALF_CUS // _cdiv(h, 128), v // (4 * suffix)))
     sums   = scratch((slices, rows, h)) if slices > 1 else dx
-    launches.append(Launch(f'linear_rows_dx_{"h" if transposed else "v"}_{suffix}', (_cdiv(h, 128) * slices, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (sums, ds, w, tokens)],
-                           _u32(rows, h, v, slices), bytes_moved=4 * (w.size + rows * v + slices * rows * h), flops=2 * rows * h * v))
-    if slices > 1:
-        launches.append(_linear_sum(dx, sums, slices, rows * h))
-    #dw: steps of 32 rows of it a wave, so many that what the wave holds is read seldom, with waves enough for the chip (a step each: 64 x 1024 x 32000 23 us more, 15 x 1973 x 128040 40 less)
-    a, b, m, n = (ds, x, v, h) if transposed else (x, ds, h, v)
-    tiles_n = _cdiv(n, 128)
-    steps   = max(1, min(16, tiles_n * _cdiv(m, 32) // (8 * HALF_CUS)))
-    tasks   = tiles_n * _cdiv(m, 32 * steps)
-    launches.append(Launch(f'linear_rows_dw_{max(8, _pow2_at_least(rows))}', (_cdiv(tasks, 4), 1, 1), (BLOCK, 1, 1), [(b_, 0) for b_ in (dw, a, b, tokens)], _u32(rows, m, n, v, steps, tiles_n, tasks, 0),
-                           bytes_moved=4 * (dw.size + rows * (h + v)), flops=2 * rows * h * v))
-    return launches
+    launch = Launch(f'linear_rows_dx_{"h" if transposed else "v"}_{suffix}', (_cdiv(h, 128) * slices, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (sums, ds, w, tokens)],
+                    _u32(rows, h, v, slices), bytes_moved=4 * (w.size + rows * v + slices * rows * h), flops=2 * rows * h * v)
+    return [launch] + ([_linear_sum(dx, sums, slices, rows * h)] if slices > 1 else [])
 
 
 def _linear_sum(out, parts: Buffer, count: int, n: int) -> Launch:
@@ -2845,9 +2852,11 @@ def _linear_sum(out, parts: Buffer, count: int, n: int) -> Launch:
                   bytes_moved=4 * (count + 1) * n)
 
 
-def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, known=None, cotangents=None):
+def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, known=None, cotangents=None,
+                    wanted=(True, True)):
     '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x) - or, where that has been done, with the weights' scale from `known` -, and with cotangents
-    for those behind it, into (the weights contracted over the vocabulary, x with its rows' factors contracted over the rows, the factors), which are returned. Scales go to `scales`.'''
+    for those behind it, into (the weights contracted over the vocabulary, x with its rows' factors contracted over the rows - as they are `wanted` -, the factors), which are returned. Scales go
+    to `scales`.'''
     rows, h, v = shape
     row_blocks    = max(1, min(1024, _cdiv(rows, 4)))
     weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if known is None else 0
@@ -2858,8 +2867,8 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     jobs = [(forward[0], v, h, _PACK_WEIGHTS, by_v), (forward[1], rows, h, _PACK_ROWS, (h, 1))] if forward else []
     behind = (None, None)
     if cotangents:
-        behind = scratch((_half_words(h, v),), np.uint32), scratch((_half_words(h, rows),), np.uint32)
-        jobs += [(behind[0], h, v, _PACK_WEIGHTS, by_h), (behind[1], h, rows, _PACK_SCALED, (1, h))]
+        behind = tuple(scratch((_half_words(h, k),), np.uint32) if needed else None for k, needed in zip((v, rows), wanted))
+        jobs += [job for job in ((behind[0], h, v, _PACK_WEIGHTS, by_h), (behind[1], h, rows, _PACK_SCALED, (1, h))) if job[0] is not None]
     params, blocks = _u32(weight_blocks, row_blocks, v, 0), 0
     for _, i, k, kind, strides in jobs:
         steps  = _half_steps(k)
@@ -2914,20 +2923,21 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
     if _linear_few(rows, h, v):
         return _linear_rows_grad(dx, dw, shape, x, w, tokens, peaks, totals, g_log_probs, g_log_sums, transposed, scratch, *(parts or [None]))
     scales = scratch((4,), np.int32)                       #of all that is taken apart here
+    wanted = dx is not None, dw is not None
     if parts:
         w_parts, x_parts, score_scales = parts
-        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None, score_scales, (g_log_probs, g_log_sums))
+        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None, score_scales, (g_log_probs, g_log_sums), wanted)
     else:
         w_parts, x_parts = [scratch((n,), np.uint32) for n, _ in linear_parts(x.shape, w.shape, transposed)[:2]]
         score_scales = scales
-        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts), None, (g_log_probs, g_log_sums))
+        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts), None, (g_log_probs, g_log_sums), wanted)
     #pieces of the vocabulary, of whole tiles
     row_blocks, all_tiles = _cdiv(rows, 32), _cdiv(v, HALF_TILE)
     pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (8 * 32 * row_blocks * HALF_TILE)))
     each   = _cdiv(all_tiles, pieces)
     pieces = _cdiv(all_tiles, each)
     width  = each * HALF_TILE
-    by_row, by_token = scratch((row_blocks * (width // 16) * 512,), np.uint32), scratch((width // 32 * 2 * row_blocks * 512,), np.uint32)
+    by_row, by_token = (scratch((row_blocks * (width // 16) * 512,), np.uint32) if needed else None for needed in wanted)
     tiles_r = _cdiv(rows, HALF_TILE)
 
     def product(out, offset, a, b, m, n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_b, scale_a, scale_b, ld, by_rows=False, add=False, parts=0):
@@ -2944,17 +2954,20 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
     tiles_x = tiles_r * _cdiv(h, HALF_TILE)
     parts   = 2 * HALF_CUS // tiles_x if tiles_x <= HALF_CUS else 0
     parts   = min(parts, width // 32 // HALF_SLICE_PAIRS)
-    sums    = scratch((parts, rows, h)) if parts > 1 else dx
-    parts   = parts if parts > 1 else 0
+    parts   = parts if parts > 1 and dx is not None else 0
+    sums    = scratch((parts, rows, h)) if parts else dx
     for piece in range(pieces):
         first = piece * each
         tiles = min(each, all_tiles - first)
         v0, n = first * HALF_TILE, min(width, v - first * HALF_TILE)
         launches.append(_linear_scores_launch('linear_q', shape, tiles * HALF_TILE, lambda side: v0 // side, width, (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors),
                                               (0, 1), 2, scratch, zeroed)[0])
-        launches.append(product(sums, 0, by_row, w_by_h, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), v0 // 16, -1, _PACK_WEIGHTS, h,
-                                by_rows=True, add=piece > 0, parts=parts))
+        if dx is not None:
+            launches.append(product(sums, 0, by_row, w_by_h, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), v0 // 16, -1, _PACK_WEIGHTS, h,
+                                    by_rows=True, add=piece > 0, parts=parts))
         steps = 2 * row_blocks
+        if dw is None:
+            continue
         if transposed:
             launches.append(product(dw, v0 * h, by_token, x_scaled, n, h, row_blocks, tiles * 4, _cdiv(h, 32), steps, steps, 0, -1, _PACK_SCALED, h))
         else:

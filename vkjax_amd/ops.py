@@ -87,6 +87,8 @@ def analyze_jaxpr(bufferpool: BufferPool, jaxpr) -> tp.List[Op]:
             raise NotImplementedError(eq)
         if _reuse_equal_equation(bufferpool, eq):
             continue
+        if opname == 'linear_log_probs_grad' and bufferpool.fuse:
+            eq = _without_unread_results(eq, jaxpr)
         position   = bufferpool.op_counter
         method_ops = method(bufferpool, eq)
         for op in method_ops:
@@ -94,6 +96,12 @@ def analyze_jaxpr(bufferpool: BufferPool, jaxpr) -> tp.List[Op]:
                 op.index = position
         all_ops += method_ops
     return all_ops
+
+
+def _without_unread_results(eq, jaxpr):
+    '''The equation with results that nothing reads dropped (the gradient of weights that are not trained: a product and what leads to it).'''
+    read = {id(v) for e in jaxpr.eqns for v in e.invars} | {id(v) for v in jaxpr.outvars}
+    return core.JaxprEqn(eq.invars, [v if id(v) in read or core.is_dropped(v) else core.DropVar(v.aval) for v in eq.outvars], eq.primitive, eq.params)
 
 
 def _without_transposed_gradients(jaxpr) -> tp.List:
@@ -1253,9 +1261,6 @@ def linear_log_probs_grad(bufferpool, equation):
         raise NotImplementedError(equation)
     if x.size == 0:
         return [Op(equation, launch=K.fill(dweights, 0))] if dweights is not None else []          #a sum over no rows
-    if dx is None or dweights is None:
-        dx       = dx if dx is not None else scratch(x.shape)
-        dweights = dweights if dweights is not None else scratch(weights.shape)
     return _operator_ops(equation, K.linear_log_probs_grad(dx, dweights, x, weights, tokens, peaks, totals, g_log_probs, g_log_sums, p['transposed'], scratch,
                                                             bufferpool.zeroed_scratch, parts))
 
