@@ -152,32 +152,51 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
         if (at.has(P, i)) at.held(states, P, at.chunk, i)[at.c] = h[i];
 }
 
-// ---- the state in front of every chunk, in the place of its state from zero; the same for the adjoint from the last chunk on, and the initial state's cotangent
+// ---- the state in front of every chunk, in the place of its state from zero; the same for the adjoint from the last chunk on, and the initial state's cotangent. A block has 64
+// (sequence, state, channel) and up to 16 waves, of which each composes eight chunks to a map, h -> product h + own; what lies in front of its first chunk follows from the waves' maps in front of
+// it. (Chunk by chunk in one wave, loads wait for one another: 191 chunks took 50 us.)
 struct ScanJoinParams { uint32_t first, B, C, N, chunks, back; };
-extern "C" __global__ __launch_bounds__(64) void selective_scan_join(float* __restrict__ states, float* __restrict__ end, const float* __restrict__ sums, const float* __restrict__ a,
-                                                                     const float* __restrict__ initial, ScanJoinParams P) {
-    const uint32_t id = blockIdx.x * 64u + threadIdx.x, c = id % P.C, rest = id / P.C, n = rest % P.N, b = rest / P.N;
-    if (b >= P.B) return;
+extern "C" __global__ __launch_bounds__(1024) void selective_scan_join(float* __restrict__ states, float* __restrict__ end, const float* __restrict__ sums, const float* __restrict__ a,
+                                                                       const float* __restrict__ initial, ScanJoinParams P) {
+    constexpr uint32_t EACH = 8u;
+    __shared__ float maps[2][16][2][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const uint32_t all = P.B * P.N * P.C, place = blockIdx.x * 64u + lane, id = min(place, all - 1u), c = id % P.C, rest = id / P.C, n = rest % P.N, b = rest / P.N;
     const float a2 = factor_of(a[(int64_t)c * P.N + n]);
     const int64_t at = ((int64_t)b * P.C + c) * P.N + n, each = (int64_t)P.B * P.N * P.C, first = ((int64_t)b * P.N + n) * P.C + c;
     const int64_t s_each = (int64_t)P.B * P.C, s_first = (int64_t)b * P.C + c;
     float h = initial ? initial[at] : 0.f;
-    for (uint32_t k0 = 0; k0 < P.chunks; k0 += 8u) {
-        float own[8], sum[8];
+    for (uint32_t k0 = 0, turn = 0; k0 < P.chunks; k0 += EACH * waves, turn ^= 1u) {
+        const uint32_t mine = k0 + EACH * wave;
+        auto number = [&](uint32_t k) { return P.back ? P.chunks - 1u - k : k; };
+        float own[EACH], factor[EACH], product = 1.f, sum = 0.f;
 #pragma unroll
-        for (uint32_t q = 0; q < 8u; ++q) {
-            const uint32_t k = P.back ? P.chunks - 1u - min(k0 + q, P.chunks - 1u) : min(k0 + q, P.chunks - 1u);
-            own[q] = states[first + k * each]; sum[q] = sums[s_first + k * s_each];
+        for (uint32_t q = 0; q < EACH; ++q) {
+            const uint32_t k = number(min(mine + q, P.chunks - 1u));
+            own[q] = states[first + k * each]; factor[q] = sums[s_first + k * s_each];
         }
 #pragma unroll
-        for (uint32_t q = 0; q < 8u; ++q) {
-            if (k0 + q >= P.chunks) break;
-            const uint32_t k = P.back ? P.chunks - 1u - (k0 + q) : k0 + q;
-            states[first + k * each] = h;
-            h = __builtin_fmaf(exp2_of(a2 * sum[q]), h, own[q]);
+        for (uint32_t q = 0; q < EACH; ++q) {
+            const bool there = mine + q < P.chunks;
+            factor[q] = there ? exp2_of(a2 * factor[q]) : 1.f;
+            own[q] = there ? own[q] : 0.f;
+            product *= factor[q];
+            sum = __builtin_fmaf(factor[q], sum, own[q]);
+        }
+        maps[turn][wave][0][lane] = product; maps[turn][wave][1][lane] = sum;
+        __syncthreads();
+        float mine_h = h;
+        for (uint32_t w = 0; w < waves; ++w) {
+            if (w == wave) mine_h = h;
+            h = __builtin_fmaf(maps[turn][w][0][lane], h, maps[turn][w][1][lane]);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < EACH; ++q) {
+            if (mine + q < P.chunks && place < all) states[first + number(mine + q) * each] = mine_h;
+            mine_h = __builtin_fmaf(factor[q], mine_h, own[q]);
         }
     }
-    if (end) end[at] = h;
+    if (end && wave == 0u && place < all) end[at] = h;
 }
 
 // ---- the scan itself, a chunk from the state in front of it
@@ -449,27 +468,33 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             if (threadIdx.x < (uint32_t)at.STAGED) { (&map[0][0][0])[threadIdx.x] = rmap[0]; (&map[1][0][0])[threadIdx.x] = rmap[1]; }
             if (turn > 0) request(t0 - KEPT);
             at.meet();
-            float dt[KEPT], xs[KEPT], gy[KEPT], bs[NS], cs[NS], next_b[NS], next_c[NS];
+            // (a step's dt, x, gy and maps, and those of the step behind it: all eight's would take the registers of a third wave)
+            float dt, xs, gy, bs[NS], cs[NS], next_dt, next_x, next_gy, next_b[NS], next_c[NS];
+            auto next = [&](int s) {
+                next_dt = prepared[0][s][at.lane]; next_x = prepared[1][s][at.lane]; next_gy = prepared[2][s][at.lane];
+                at.maps(next_b, map[0], s); at.maps(next_c, map[1], s);
+            };
+            auto take = [&] {
+                dt = next_dt; xs = next_x; gy = next_gy;
 #pragma unroll
-            for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[0][s][at.lane]; xs[s] = prepared[1][s][at.lane]; gy[s] = prepared[2][s][at.lane]; }
-            at.maps(next_b, map[0], 0);
-            at.maps(next_c, map[1], 0);
+                for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
+            };
+            next(0);
 #pragma unroll
             for (int s0 = 0; s0 < KEPT; s0 += AT_ONCE) {
                 float part[8];
 #pragma unroll
                 for (int g = 0; g < AT_ONCE; ++g) {
                     const int s = s0 + g;
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                    if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
-                    const float u = dt[s] * xs[s];
+                    take();
+                    if (s + 1 < KEPT) next(s + 1);
+                    const float u = dt * xs;
                     float seen = 0.f;
 #pragma unroll
                     for (int i = 0; i < NS; ++i) {
                         before[s][i] = h[i];
-                        h[i] = __builtin_fmaf(exp2_of(a2[i] * dt[s]), h[i], u * bs[i]);
-                        part[g * NS + i] = gy[s] * h[i];
+                        h[i] = __builtin_fmaf(exp2_of(a2[i] * dt), h[i], u * bs[i]);
+                        part[g * NS + i] = gy * h[i];
                         seen = __builtin_fmaf(cs[i], h[i], seen);
                     }
                     parts[at.wave][0][s][at.lane] = seen;
@@ -478,28 +503,26 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 if (over_stores) mapped[1][s0 + over / NS][at.n0 + over % NS] = sum;
                 STEP_FENCE();
             }
-            at.maps(next_b, map[0], KEPT - 1);
-            at.maps(next_c, map[1], KEPT - 1);
+            next(KEPT - 1);
 #pragma unroll
             for (int s0 = KEPT - AT_ONCE; s0 >= 0; s0 -= AT_ONCE) {
                 float part[8];
 #pragma unroll
                 for (int g = AT_ONCE - 1; g >= 0; --g) {
                     const int s = s0 + g;
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
-                    if (s > 0) { at.maps(next_b, map[0], s - 1); at.maps(next_c, map[1], s - 1); }
-                    const float u = dt[s] * xs[s];
+                    take();
+                    if (s > 0) next(s - 1);
+                    const float u = dt * xs;
                     float lb = 0.f, ea = 0.f;
 #pragma unroll
                     for (int i = 0; i < NS; ++i) {
-                        l[i] = __builtin_fmaf(gy[s], cs[i], l[i]);
+                        l[i] = __builtin_fmaf(gy, cs[i], l[i]);
                         lb = __builtin_fmaf(l[i], bs[i], lb);
                         part[g * NS + i] = l[i] * u;
-                        l[i] *= exp2_of(a2[i] * dt[s]);
+                        l[i] *= exp2_of(a2[i] * dt);
                         const float e = l[i] * before[s][i];
                         ea = __builtin_fmaf(e, a2[i], ea);
-                        da[i] = __builtin_fmaf(e, dt[s], da[i]);
+                        da[i] = __builtin_fmaf(e, dt, da[i]);
                     }
                     parts[at.wave][1][s][at.lane] = lb;
                     parts[at.wave][2][s][at.lane] = ea;
@@ -576,7 +599,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                                                                                                 ScanParams P) {                                                                    \
         scan_grad_chunk_body<NS, M>(sums, states, delta, a, cmap, gate, bias, lengths, g, P);                                                                                      \
     }                                                                                                                                                                              \
-    extern "C" __global__ __launch_bounds__(64 * M, 2) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* maps, float* channel_sums, const float* x, \
+    extern "C" __global__ __launch_bounds__(64 * M, NS == 8 || M == 1 ? 2 : M == 8 ? 4 : 3) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* maps, float* channel_sums, const float* x, \
                                                                                           const float* delta, const float* a, const float* bmap, const float* cmap,                \
                                                                                           const float* through, const float* gate, const int32_t* lengths, const float* bias,      \
                                                                                           const float* kept, const float* g, const float* g_last, const float* adjoints,           \

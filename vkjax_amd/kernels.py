@@ -2626,8 +2626,9 @@ def causal_conv_grad(dx, dkernel, dbias, dstate, x: Buffer, kernel: Buffer, bias
 
 SELECTIVE_SCAN_KEPT       = 8           #steps between two states that a gradient's forward pass keeps
 SELECTIVE_SCAN_MAX_STATES = 64
-#waves that fill the machine; time is cut into chunks where there are fewer, of at least so many steps
-SELECTIVE_SCAN_WAVES, SELECTIVE_SCAN_CHUNK = 4096, 64
+#waves that fill the machine; time is cut into chunks where there are fewer, of at least so many steps (8 of them instead of 64: 3 x 1021 x 333 x 7 states with its gradient 103 -> 59 us, 4 x 1455 x
+#40 x 16 84 -> 49)
+SELECTIVE_SCAN_WAVES, SELECTIVE_SCAN_CHUNK = 4096, 8
 
 
 class ScanTiling(tp.NamedTuple):
@@ -2642,8 +2643,14 @@ def selective_scan_tiling(batch: int, time: int, channels: int, n: int) -> ScanT
     states = 4 if n <= 32 else 8
     waves  = _pow2_at_least(_cdiv(n, states))
     strips = _cdiv(channels, 64)
-    chunks = max(1, min(_cdiv(SELECTIVE_SCAN_WAVES, batch * strips * waves), time // SELECTIVE_SCAN_CHUNK))
-    chunk  = _cdiv(_cdiv(time, chunks), SELECTIVE_SCAN_KEPT) * SELECTIVE_SCAN_KEPT
+    needed  = max(1, min(_cdiv(SELECTIVE_SCAN_WAVES, batch * strips * waves), time // SELECTIVE_SCAN_CHUNK))
+    rounded = lambda chunks: _cdiv(_cdiv(time, chunks), SELECTIVE_SCAN_KEPT) * SELECTIVE_SCAN_KEPT
+    chunk   = rounded(needed)
+    #blocks that the CUs (of fewer than four waves: the SIMDs) have one of; where a few more would be a round of their own, up to twice as many chunks, so that rounds are full
+    #(1 x 1393 x 2824 x 24 states in 12 chunks, 540 blocks, 91 us, in 17, 765 blocks, 74)
+    places = 1024 // min(waves, 4)
+    if needed > 1 and batch * strips * needed > places:
+        chunk = min(sorted({rounded(n) for n in range(needed, 2 * needed + 1)}, reverse=True), key=lambda k: _cdiv(batch * strips * _cdiv(time, k), places) * (k + SELECTIVE_SCAN_KEPT))
     tiling = ScanTiling(states, waves, strips, _cdiv(time, chunk), chunk)
     if batch * strips * tiling.chunks * 64 * waves >= 2**32 or batch * channels * n >= 2**31 or max(time, channels) >= 2**30:
         raise NotImplementedError(f'a selective scan over {channels} channels of {n} states in {batch} sequences of {time} steps')
@@ -2658,7 +2665,7 @@ def _scan_launch(name: str, x: Buffer, tiling: ScanTiling, n: int, softplus, arr
 
 def _scan_join(states, end, sums, a: Buffer, initial, x: Buffer, tiling: ScanTiling, back: bool) -> Launch:
     (b, _, c), n = x.shape, a.shape[1]
-    return Launch('selective_scan_join', (_cdiv(b * c * n, 64), 1, 1), (64, 1, 1), [(v, 0) for v in (states, end, sums, a, initial)],
+    return Launch('selective_scan_join', (_cdiv(b * c * n, 64), 1, 1), (64 * min(16, _cdiv(tiling.chunks, 8)), 1, 1), [(v, 0) for v in (states, end, sums, a, initial)],
                   _u32(0, b, c, n, tiling.chunks, back), bytes_moved=8 * b * c * n * tiling.chunks, written=(0, 1))
 
 
