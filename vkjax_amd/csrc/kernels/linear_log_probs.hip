@@ -466,20 +466,22 @@ template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT
     }
 }
 
-// forward: 128 tokens' scores, their peak and sum per row; the scores [rows][V] themselves for a gradient
+// forward: 128 tokens' scores, their peak and sum per row; the scores [rows][V] themselves for a gradient. Where tiles are few, the features in slices, whose sums go to [slice][rows][V]
 template <bool ALONG_V, int NT>
 __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ scores, const float* __restrict__ x,
                                                  const float* __restrict__ w, const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
     using Product = RowsProduct<NT>;
     __shared__ typename Product::Shared shared;
-    const uint32_t lane = threadIdx.x & 63u, v0 = blockIdx.x * 128u;
+    const uint32_t lane = threadIdx.x & 63u, tiles = (P.V + 127u) / 128u, v0 = blockIdx.x % tiles * 128u, slice = blockIdx.x / tiles;
+    constexpr uint32_t GROUP = ALONG_V ? 8u : 32u;
+    const uint32_t groups = (P.H + GROUP - 1u) / GROUP;
     uint32_t r_at[NT];
     bool there[NT];
     rows_there<NT>(r_at, there, tokens, P);
     Product product;
-    product.template multiply<ALONG_V>(shared, w, x, v0, P.V, P.H, r_at, there, 0u, (P.H + (ALONG_V ? 7u : 31u)) / (ALONG_V ? 8u : 32u));
+    product.template multiply<ALONG_V>(shared, w, x, v0, P.V, P.H, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
     if (threadIdx.x >= 64u) return;
-    if (scores) product.template store<ALONG_V>(scores, v0, P.V, P.rows);
+    if (scores) product.template store<ALONG_V>(scores + (uint64_t)slice * P.rows * P.V, v0, P.V, P.rows);
     if (!peaks) return;
     // a lane has 64 scores of a row
 #pragma unroll
@@ -507,6 +509,41 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
             for (int q = 0; q < 16; ++q) sum += exp_of(product.acc[i][j][q] - base);
         sum = over_halves_sum(sum);
         if (lane < 32u && r < P.rows) { peaks[(uint64_t)blockIdx.x * P.rows + r] = peak; sums[(uint64_t)blockIdx.x * P.rows + r] = sum; }
+    }
+}
+
+// ... added up: 1024 tokens of a row, their peak and sum, the scores for a gradient
+extern "C" __global__ __launch_bounds__(256) void linear_rows_sum(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ scores,
+                                                                  const float* __restrict__ parts, const int32_t* __restrict__ tokens, LinearRowsParams P) {
+    __shared__ float met[2][4];
+    const uint32_t r = blockIdx.y, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, v0 = blockIdx.x * 1024u + threadIdx.x;
+    const int32_t token = tokens[r];
+    const uint64_t row = (uint64_t)r * P.V, each = (uint64_t)P.rows * P.V;
+    float s[4] = {}, peak = -__builtin_inff();
+    for (uint32_t k = 0; k < P.slices; ++k)
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) s[q] += parts[k * each + row + min(v0 + 256u * q, P.V - 1u)];
+#pragma unroll
+    for (uint32_t q = 0; q < 4u; ++q) {
+        const uint32_t v = v0 + 256u * q;
+        if (v >= P.V) { s[q] = -__builtin_inff(); continue; }
+        if (scores) scores[row + v] = s[q];
+        if (of_token && v == (uint32_t)token) of_token[r] = s[q];
+        peak = fmaxf(peak, s[q]);
+    }
+    if (!peaks) return;
+    peak = wave_largest(peak);
+    if (lane == 0u) met[0][wave] = peak;
+    __syncthreads();
+    peak = fmaxf(fmaxf(met[0][0], met[0][1]), fmaxf(met[0][2], met[0][3]));
+    const float base = peak == -__builtin_inff() ? 0.f : peak;
+    float sum = (exp_of(s[0] - base) + exp_of(s[1] - base)) + (exp_of(s[2] - base) + exp_of(s[3] - base));
+    wave_butterfly([&](auto step) { sum += lane_xor<decltype(step)::value>(sum); });
+    if (lane == 0u) met[1][wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0u) {
+        peaks[(uint64_t)blockIdx.x * P.rows + r] = peak;
+        sums[(uint64_t)blockIdx.x * P.rows + r]  = (met[1][0] + met[1][1]) + (met[1][2] + met[1][3]);
     }
 }
 

@@ -2813,10 +2813,22 @@ def linear_parts(x_shape, w_shape, transposed: bool) -> tp.List[tp.Tuple[int, ty
     return [(_half_words(v, h), np.uint32), (_half_words(rows, h), np.uint32), (4, np.int32)]
 
 
-def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, of_tiles, scores) -> Launch:
+def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, of_tiles, scores, scratch) -> tp.Tuple[tp.List[Launch], int]:
+    '''Launches for the scores of few rows, and the tiles that their peaks and sums are of.'''
     rows, h, v = shape
-    return Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (_cdiv(v, 128), 1, 1), (BLOCK, 1, 1),
-                  [(b, 0) for b in (*of_tiles, scores, x, w, tokens)], _u32(rows, h, v, 0), bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2, 3))
+    tiles  = _cdiv(v, 128)
+    #few tiles: slices of the features, of four times the rows and 64 at least, that a block to a CU makes (4 x 4096 x 1000 81 -> 22 us, 4 x 4096 x 16000 85 -> 53, 64 x 2048 x 8000 80 -> 37, with a
+    #launch more; two blocks to a CU 31, 55, 41)
+    slices = max(1, min(HALF_CUS // tiles, h // max(64, 4 * rows)))
+    parts  = scratch((slices, rows, v)) if slices > 1 else None
+    launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles * slices, 1, 1), (BLOCK, 1, 1),
+                       [(b, 0) for b in ((None, None, None, parts) if slices > 1 else (*of_tiles, scores)) + (x, w, tokens)], _u32(rows, h, v, slices),
+                       bytes_moved=4 * (x.size + w.size), flops=2 * rows * h * v, written=(0, 1, 2, 3))]
+    if slices > 1:
+        tiles = _cdiv(v, 1024)
+        launches.append(Launch('linear_rows_sum', (tiles, rows, 1), (BLOCK, 1, 1), [(b, 0) for b in (*of_tiles, scores, parts, tokens)], _u32(rows, h, v, slices),
+                               bytes_moved=4 * parts.size, written=(0, 1, 2, 3)))
+    return launches, tiles
 
 
 def _linear_rows_grad(dx, dw, shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, peaks: Buffer, totals: Buffer, g_log_probs, g_log_sums, transposed: bool, scratch,
@@ -2825,7 +2837,7 @@ def _linear_rows_grad(dx, dw, shape: LinearShape, x: Buffer, w: Buffer, tokens: 
     launches = []
     if scores is None:
         scores = scratch((rows, v))
-        launches.append(_linear_rows_scores(shape, x, w, tokens, transposed, (None, None, None), scores))
+        launches += _linear_rows_scores(shape, x, w, tokens, transposed, (None, None, None), scores, scratch)[0]
     ds = scratch((rows, v))
     launches.append(Launch('linear_rows_ds', (_cdiv(v, 1024), rows, 1), (BLOCK, 1, 1), [(b, 0) for b in (ds, scores, tokens, peaks, totals, g_log_probs, g_log_sums)], _u32(rows, h, v, 0),
                            bytes_moved=8 * rows * v))
@@ -2910,8 +2922,7 @@ def linear_log_probs(log_probs, log_sums, peaks, totals, x: Buffer, w: Buffer, t
     tiles    = _cdiv(v, 64)
     of_tiles = [scratch((tiles, rows)), scratch((tiles, rows)), scratch((rows,))]           #peak and sum of each tile's scores, the token's score
     if _linear_few(rows, h, v):
-        tiles    = _cdiv(v, 128)
-        launches = [_linear_rows_scores(shape, x, w, tokens, transposed, of_tiles, *(parts or [None]))]
+        launches, tiles = _linear_rows_scores(shape, x, w, tokens, transposed, tuple(of_tiles), *(parts or [None]), scratch)
     else:
         w_parts, x_parts, scales = parts or [scratch((n,), dtype) for n, dtype in linear_parts(x.shape, w.shape, transposed)]
         launches, _ = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts))
