@@ -280,24 +280,24 @@ extern "C" __global__ __launch_bounds__(1024) void linear_join(float* __restrict
 //     different banks. (Loaded as the instruction has them, 64 bytes of a row to a lane, lines were fetched several times: 53 x 776 x 112111 took 269 us, 1.3 TB/s.)
 // Bound by memory up to 32 rows (15 x 1973 x 128040: 200 us, 5 TB/s along M, 270 along K), and by memory and the products alike at 64 (64 x 4096 x 32000: 168 us, of which either takes 107 alone).
 // Blocks of four waves, two a CU, hide one another's ends: with eight waves to a block 14 x 47 x 107245 took 31 us, not 19, and 32 x 896 x 83954 93 us, not 76.
-template <int NT> struct RowsProduct {
-    static constexpr int WAVES = 4;
-    static constexpr uint32_t THREADS = 64u * WAVES;
-    union Shared { f32x4 turned[WAVES][4][32][8]; f32x4 met[WAVES / 2][NT * 16][64]; };
-    f32x16 acc[4][NT];
+template <bool ALONG_M, int NT> struct RowsProduct {
+    // blocks of 32 m: two where A is turned for 64 rows, so that two blocks of waves are there too (with four, whose sums leave room for one, 53 x 776 x 112111 takes 200 us, not 157)
+    static constexpr int WAVES = 4, MB = !ALONG_M && NT == 2 ? 2 : 4;
+    static constexpr uint32_t TILE = 32u * MB;
+    union Shared { f32x4 turned[ALONG_M ? 1 : WAVES][MB][32][8]; f32x4 met[WAVES / 2][NT * MB * 4][64]; };
+    f32x16 acc[MB][NT];
 
     static __device__ __forceinline__ uint32_t lane() { return threadIdx.x & 63u; }
     static __device__ __forceinline__ f32x4 load(const float* at) { return *reinterpret_cast<const f32x4_anywhere*>(at); }
     // over the k of groups [all_begin, all_end); `there`: rows that are padding are zeros, whatever b holds. M and K are 4 at least: vectors that would end behind the last m or k are moved to
     // the left, and of b the k's that come twice by that are zeros. (So nothing is loaded behind a branch: with one the loads of a last group waited for one another, 25 us of a block's 84 at
     // 15 x 1973 x 128040.)
-    template <bool ALONG_M>
     __device__ __forceinline__ void multiply(Shared& shared, const float* __restrict__ a, const float* __restrict__ b, uint32_t m0, uint32_t M, uint32_t K, const uint32_t (&r_at)[NT],
                                              const bool (&there)[NT], uint32_t all_begin, uint32_t all_end) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane() >> 5, l32 = lane() & 31u;
         const uint32_t groups = all_end - all_begin, begin = all_begin + groups * wave / WAVES, end = all_begin + groups * (wave + 1u) / WAVES;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
         auto of_row = [&](int j, uint32_t k) { return load(b + (uint64_t)r_at[j] * K + min(k, K - 4u)); };
@@ -324,7 +324,7 @@ template <int NT> struct RowsProduct {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < MB; ++i)
 #pragma unroll
                         for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[q][i], bv[j][q], acc[i][j], 0, 0, 0);
             };
@@ -347,14 +347,14 @@ template <int NT> struct RowsProduct {
                     if (g + k < end) products(as[k], bs[k], g + k);
                 }
         } else {
-            f32x4 (&turned)[4][32][8] = shared.turned[wave];
+            f32x4 (&turned)[MB][32][8] = shared.turned[wave];
             const uint32_t row8 = lane() >> 3, column = lane() & 7u;
-            f32x4 next[4][4], bs[NT][4];
+            f32x4 next[MB][4], bs[NT][4];
             auto request = [&](uint32_t g) {
                 // (rows behind the last m are the last one again; 8 rows of fewer than 2^27 elements are 32 bits of bytes)
                 const uint32_t at = 4u * min(g * 32u + 4u * column, K - 4u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         const uint32_t first = min(m0 + 32u * i + 8u * t, M - 1u);
@@ -372,7 +372,7 @@ template <int NT> struct RowsProduct {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
                     for (int t = 0; t < 4; ++t) turned[i][8 * t + row8][column ^ row8] = next[i][t];
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -385,13 +385,13 @@ template <int NT> struct RowsProduct {
                 if (g + 1u < end) { request(g + 1u); request_rows(g + 1u); }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    f32x4 av[4];
+                    f32x4 av[MB];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) av[i] = turned[i][l32][(4u * half + c) ^ (l32 & 7u)];
+                    for (int i = 0; i < MB; ++i) av[i] = turned[i][l32][(4u * half + c) ^ (l32 & 7u)];
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < MB; ++i)
 #pragma unroll
                             for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[i][q], now[j][c][q], acc[i][j], 0, 0, 0);
                 }
@@ -403,7 +403,7 @@ template <int NT> struct RowsProduct {
         for (uint32_t half_of = WAVES / 2; half_of > 0u; half_of >>= 1) {
             if (wave >= half_of && wave < 2u * half_of)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -412,7 +412,7 @@ template <int NT> struct RowsProduct {
             __syncthreads();
             if (wave < half_of)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MB; ++i)
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -425,30 +425,30 @@ template <int NT> struct RowsProduct {
         }
     }
     // the m of element q of block i. (Of a vector that was moved to the left to stay inside, those that are this lane's own: others are M)
-    template <bool ALONG_M> static __device__ __forceinline__ uint32_t m_of(uint32_t m0, uint32_t M, int i, int q) {
+    static __device__ __forceinline__ uint32_t m_of(uint32_t m0, uint32_t M, int i, int q) {
         const uint32_t row = 8u * (q >> 2) + 4u * (lane() >> 5) + (q & 3);
         if constexpr (!ALONG_M) return m0 + 32u * i + row;
         const uint32_t first = m0 + 4u * row, m = min(first, M - 4u) + i;
         return m >= first ? m : M;
     }
     // to out[r][m], of columns r = 32 j + l % 32 < rows
-    template <bool ALONG_M> __device__ __forceinline__ void store(float* __restrict__ out, uint32_t m0, uint32_t M, uint32_t rows) const {
+    __device__ __forceinline__ void store(float* __restrict__ out, uint32_t m0, uint32_t M, uint32_t rows) const {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const uint32_t r = 32u * j + (lane() & 31u);
             if (r >= rows) continue;
             float* const to = out + (uint64_t)r * M;
 #pragma unroll
-            for (int p = 0; p < 16; ++p) {                 // four neighbours: of one row of a block along K, of the four blocks along M
+            for (int p = 0; p < 4 * MB; ++p) {             // four neighbours: of one row of a block along K, of the four blocks along M
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ALONG_M ? acc[e][j][p] : acc[p >> 2][j][4 * (p & 3) + e];
+                for (int e = 0; e < 4; ++e) if constexpr (ALONG_M) v[e] = acc[e][j][p]; else v[e] = acc[p >> 2][j][4 * (p & 3) + e];
                 const uint32_t m = ALONG_M ? m0 + 4u * (8u * (p >> 2) + 4u * (lane() >> 5) + (p & 3)) : m0 + 32u * (p >> 2) + 8u * (p & 3) + 4u * (lane() >> 5);
                 if (m + 4u <= M) *reinterpret_cast<f32x4_anywhere*>(to + m) = v;
                 else
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t at = m_of<ALONG_M>(m0, M, ALONG_M ? e : p >> 2, ALONG_M ? p : 4 * (p & 3) + e);
+                        const uint32_t at = m_of(m0, M, ALONG_M ? e : p >> 2, ALONG_M ? p : 4 * (p & 3) + e);
                         if (at < M) to[at] = v[e];
                     }
             }
@@ -467,23 +467,23 @@ template <int NT> __device__ __forceinline__ void rows_there(uint32_t (&r_at)[NT
 }
 
 // forward: 128 tokens' scores, their peak and sum per row; the scores [rows][V] themselves for a gradient. Where tiles are few, the features in slices, whose sums go to [slice][rows][V]
-template <bool ALONG_V, int NT>
+template <bool ALONG, int NT>
 __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, float* __restrict__ sums, float* __restrict__ of_token, float* __restrict__ scores, const float* __restrict__ x,
                                                  const float* __restrict__ w, const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
-    using Product = RowsProduct<NT>;
+    using Product = RowsProduct<ALONG, NT>;
     __shared__ typename Product::Shared shared;
-    const uint32_t lane = threadIdx.x & 63u, tiles = (P.V + 127u) / 128u, v0 = blockIdx.x % tiles * 128u, slice = blockIdx.x / tiles;
-    constexpr uint32_t GROUP = ALONG_V ? 8u : 32u;
+    const uint32_t lane = threadIdx.x & 63u, tiles = (P.V + Product::TILE - 1u) / Product::TILE, v0 = blockIdx.x % tiles * Product::TILE, slice = blockIdx.x / tiles;
+    constexpr uint32_t GROUP = ALONG ? 8u : 32u;
     const uint32_t groups = (P.H + GROUP - 1u) / GROUP;
     uint32_t r_at[NT];
     bool there[NT];
     rows_there<NT>(r_at, there, tokens, P);
     Product product;
-    product.template multiply<ALONG_V>(shared, w, x, v0, P.V, P.H, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
+    product.multiply(shared, w, x, v0, P.V, P.H, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
     if (threadIdx.x >= 64u) return;
-    if (scores) product.template store<ALONG_V>(scores + (uint64_t)slice * P.rows * P.V, v0, P.V, P.rows);
+    if (scores) product.store(scores + (uint64_t)slice * P.rows * P.V, v0, P.V, P.rows);
     if (!peaks) return;
-    // a lane has 64 scores of a row
+    // a lane has 16 MB scores of a row
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const uint32_t r = 32u * j + (lane & 31u);
@@ -491,10 +491,10 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
         float peak = -__builtin_inff(), sum = 0.f, mine = 0.f;
         bool has = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < Product::MB; ++i)
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
-                const uint32_t v = Product::template m_of<ALONG_V>(v0, P.V, i, q);
+                const uint32_t v = Product::m_of(v0, P.V, i, q);
                 float s = product.acc[i][j][q];
                 if (v == (uint32_t)token) { mine = s; has = true; }
                 product.acc[i][j][q] = s = v < P.V ? s : -__builtin_inff();
@@ -504,7 +504,7 @@ __device__ __forceinline__ void scores_rows_body(float* __restrict__ peaks, floa
         peak = over_halves_max(peak);
         const float base = peak == -__builtin_inff() ? 0.f : peak;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < Product::MB; ++i)
 #pragma unroll
             for (int q = 0; q < 16; ++q) sum += exp_of(product.acc[i][j][q] - base);
         sum = over_halves_sum(sum);
@@ -563,23 +563,23 @@ extern "C" __global__ __launch_bounds__(256) void linear_rows_ds(float* __restri
 }
 
 // dx = ds W^T: blocks of 128 features by slices of the vocabulary, a slice's sums to [slice][rows][H]; padding gets zeros whatever W holds
-template <bool ALONG_H, int NT>
+template <bool ALONG, int NT>
 __device__ __forceinline__ void rows_dx_body(float* __restrict__ dx, const float* __restrict__ ds, const float* __restrict__ w, const int32_t* __restrict__ tokens, const LinearRowsParams& P) {
-    using Product = RowsProduct<NT>;
+    using Product = RowsProduct<ALONG, NT>;
     __shared__ typename Product::Shared shared;
-    const uint32_t tiles = (P.H + 127u) / 128u, h0 = blockIdx.x % tiles * 128u, slice = blockIdx.x / tiles, group = ALONG_H ? 8u : 32u, groups = (P.V + group - 1u) / group;
+    const uint32_t tiles = (P.H + Product::TILE - 1u) / Product::TILE, h0 = blockIdx.x % tiles * Product::TILE, slice = blockIdx.x / tiles, group = ALONG ? 8u : 32u, groups = (P.V + group - 1u) / group;
     uint32_t r_at[NT];
     bool there[NT];
     rows_there<NT>(r_at, there, tokens, P);
     Product product;
-    product.template multiply<ALONG_H>(shared, w, ds, h0, P.H, P.V, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
+    product.multiply(shared, w, ds, h0, P.H, P.V, r_at, there, (uint32_t)((uint64_t)groups * slice / P.slices), (uint32_t)((uint64_t)groups * (slice + 1u) / P.slices));
     if (threadIdx.x >= 64u) return;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
         if (!there[j])
 #pragma unroll
-            for (int i = 0; i < 4; ++i) product.acc[i][j] = f32x16{};
-    product.template store<ALONG_H>(dx + (uint64_t)slice * P.rows * P.H, h0, P.H, P.rows);
+            for (int i = 0; i < Product::MB; ++i) product.acc[i][j] = f32x16{};
+    product.store(dx + (uint64_t)slice * P.rows * P.H, h0, P.H, P.rows);
 }
 
 // dW[m, n] = sum_r a[r, m] b[r, n], of x and ds or the other way round as dW lies: a wave has 128 n, for which it holds b, and goes through its share of m, 32 at a time; four neighbouring n
@@ -633,15 +633,13 @@ __device__ __forceinline__ void rows_dw_body(float* __restrict__ dw, const float
     for (; m0 + 32u <= m_end; m0 += 32u) step(m0, true);
     if (m0 < m_end) step(m0, false);
 }
-// (two blocks a CU, one where A is turned for 64 rows: with half the registers those would not hold what is on its way)
-#define ROWS_KERNELS(NAME, ALONG_M, NT)                                                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, ALONG_M || NT == 1 ? 2 : 1)                                                                                       \
-    void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, float* scores, const float* x, const float* w, const int32_t* tokens, LinearRowsParams P) { \
-        scores_rows_body<ALONG_M, NT>(peaks, sums, of_token, scores, x, w, tokens, P);                                                                             \
+#define ROWS_KERNELS(NAME, ALONG_V, NT)                                                                                                                            \
+    extern "C" __global__ __launch_bounds__(256, 2) void linear_scores_rows_##NAME(float* peaks, float* sums, float* of_token, float* scores, const float* x,      \
+                                                                                   const float* w, const int32_t* tokens, LinearRowsParams P) {                    \
+        scores_rows_body<ALONG_V, NT>(peaks, sums, of_token, scores, x, w, tokens, P);                                                                             \
     }                                                                                                                                                              \
-    extern "C" __global__ __launch_bounds__(256, !ALONG_M || NT == 1 ? 2 : 1)                                                                                      \
-    void linear_rows_dx_##NAME(float* dx, const float* ds, const float* w, const int32_t* tokens, LinearRowsParams P) {                                                  \
-        rows_dx_body<!ALONG_M, NT>(dx, ds, w, tokens, P);                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256, 2) void linear_rows_dx_##NAME(float* dx, const float* ds, const float* w, const int32_t* tokens, LinearRowsParams P) { \
+        rows_dx_body<!ALONG_V, NT>(dx, ds, w, tokens, P);                                                                                                          \
     }
 ROWS_KERNELS(v_32, true, 1)
 ROWS_KERNELS(v_64, true, 2)

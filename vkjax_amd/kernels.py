@@ -2813,10 +2813,15 @@ def linear_parts(x_shape, w_shape, transposed: bool) -> tp.List[tp.Tuple[int, ty
     return [(_half_words(v, h), np.uint32), (_half_words(rows, h), np.uint32), (4, np.int32)]
 
 
+def _linear_rows_tile(rows: int, along: bool) -> int:
+    '''Of tokens (scores) or features (dx): 128, or 64 where the weights do not lie along them and there are more than 32 rows.'''
+    return 128 if along or rows <= 32 else 64
+
+
 def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, of_tiles, scores, scratch) -> tp.Tuple[tp.List[Launch], int]:
     '''Launches for the scores of few rows, and the tiles that their peaks and sums are of.'''
     rows, h, v = shape
-    tiles  = _cdiv(v, 128)
+    tiles  = _cdiv(v, _linear_rows_tile(rows, not transposed))
     #few tiles: slices of the features, of four times the rows and 64 at least, that a block to a CU makes (4 x 4096 x 1000 81 -> 22 us, 4 x 4096 x 16000 85 -> 53, 64 x 2048 x 8000 80 -> 37, with a
     #launch more; two blocks to a CU 31, 55, 41)
     slices = max(1, min(HALF_CUS // tiles, h // max(64, 4 * rows)))
@@ -2857,10 +2862,11 @@ def _linear_rows_grad(dx, dw, shape: LinearShape, x: Buffer, w: Buffer, tokens: 
 def _linear_rows_dx(dx, shape: LinearShape, w: Buffer, tokens: Buffer, ds: Buffer, transposed: bool, scratch) -> tp.List[Launch]:
     rows, h, v = shape
     suffix = 32 if rows <= 32 else 64
+    tiles  = _cdiv(h, _linear_rows_tile(rows, transposed))
     #slices of the vocabulary, of four times the rows at least (their sums are written and read once more) and enough for the chip
-    slices = max(1, min(2 * HALF_CUS // _cdiv(h, 128), v // (4 * suffix)))
+    slices = max(1, min(2 * HALF_CUS // tiles, v // (4 * suffix)))
     sums   = scratch((slices, rows, h)) if slices > 1 else dx
-    launch = Launch(f'linear_rows_dx_{"h" if transposed else "v"}_{suffix}', (_cdiv(h, 128) * slices, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (sums, ds, w, tokens)],
+    launch = Launch(f'linear_rows_dx_{"h" if transposed else "v"}_{suffix}', (tiles * slices, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (sums, ds, w, tokens)],
                     _u32(rows, h, v, slices), bytes_moved=4 * (w.size + rows * v + slices * rows * h), flops=2 * rows * h * v)
     return [launch] + ([_linear_sum(dx, sums, slices, rows * h)] if slices > 1 else [])
 
