@@ -94,7 +94,7 @@ def test_sizes_of_the_tests_on_the_gpu_reach_every_kernel():
     for shape in MATRICES:
         names.update(check(matrix_launches(*shape)))
     #(kernels of products, shared and not, have tests that choose the plan)
-    products = {f'{name}{k[0]}{shared}' for name in ('linear_scores', 'linear_q', 'linear_product', *(f'orthogonal_{n}' for n in ('square', 'polynomial', 'next', 'last')))
+    products = {f'{name}{k[0]}{shared}' for name in ('linear_scores', 'linear_q', 'linear_product_a', 'linear_product_b', *(f'orthogonal_{n}' for n in ('square', 'polynomial', 'next', 'last')))
                 for k in K.HALF_KERNELS for shared in ('', '_shared')}
     assert launched() - names <= products, launched() - names - products
 

@@ -11,6 +11,8 @@
 // A taken-apart operand is laid out as the lanes of a wave want it: [block of 32 rows][step of 16 k][hi, lo][lane] x 8 fp16; lane l has row l % 32, and with h = l / 32 its
 // element 4 i + j is k = 8 i + 4 h + j of the step. That is the order in which a lane has the rows of a 32 x 32 block of a result (register 4 i + j of a half of the block is row
 // 8 i + 4 h + j), so a result becomes an operand that is contracted over its rows without leaving its lanes. Rows and k beyond the end are zeros; k comes in pairs of steps.
+// The same operand also serves products that are contracted over its rows (TURNED): 32 rows are a pair of steps then, 16 k are half of a block, and the lanes get theirs by reads of shared
+// memory that transpose 4 rows x 16 columns (ds_read_b64_tr_b16: of 16 lanes, lane 4 a + b asks for 4 numbers of row a, and lane r is given column r of the four rows).
 #pragma once
 #include "common.h"
 
@@ -56,10 +58,16 @@ struct HalfOperand {
     const u32x4* parts;
     uint32_t blocks, stride, first;                      // blocks of 32 rows, steps of 16 k per block, and the step at which the contraction starts (even)
 };
+// (TURNED: blocks of 32 of what is a result's row or column, the steps of a block of 32 of what is contracted, and where the contraction starts, in steps of 16)
+enum HalfTurned { TURNED_NONE, TURNED_A, TURNED_B };
 
 template <int T> struct HalfSums { f32x16 large[T][T], small[T][T]; };      // of a wave's blocks of 32 x 32: hi.hi, and the others times 2^11
 
-template <int T>
+// A turned operand's half block [32 rows of it][16 k] lies in shared memory with a row's two lanes side by side, every other half block shifted by half of the banks: the reads that turn it
+// take two half blocks' rows v .. v + 3, which are all banks once.
+__device__ __forceinline__ uint32_t half_turned_place(uint32_t row, uint32_t h, uint32_t half_block) { return (2u * row + h) ^ (half_block << 3); }
+
+template <int T, HalfTurned TURNED>
 __device__ __forceinline__ void half_request(typename HalfTileOf<T>::Stage& to, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t step) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
 #pragma unroll
@@ -67,23 +75,39 @@ __device__ __forceinline__ void half_request(typename HalfTileOf<T>::Stage& to, 
         // a block of 32 rows of either operand (behind the last one, that one again: its results are nobody's)
         const uint32_t unit = wave * T + u, of_b = unit / (2u * T), block = unit % (2u * T);
         const HalfOperand& o = of_b ? b : a;
-        const u32x4* const from = o.parts + ((uint64_t)min((of_b ? n : m) * (2u * T) + block, o.blocks - 1u) * o.stride + o.first + step) * 128u + lane;
+        const uint32_t at = min((of_b ? n : m) * (2u * T) + block, o.blocks - 1u);
+        const bool turned = TURNED != TURNED_NONE && of_b == (TURNED == TURNED_B ? 1u : 0u);
+        const u32x4* const from = o.parts + (turned ? (uint64_t)((o.first + step) / 2u) * o.stride + 2u * at : (uint64_t)at * o.stride + o.first + step) * 128u;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + 64 * q), (__attribute__((address_space(3))) void*)&to[of_b][block][q >> 1][q & 1][0], 16, 0, 0);
+        for (int q = 0; q < 4; ++q) {
+            // (the lane whose numbers belong at place `lane`)
+            const uint32_t place = lane ^ ((uint32_t)(q >> 1) << 3), source = turned ? (place >> 1) + 32u * (place & 1u) : lane;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + 64 * q + source), (__attribute__((address_space(3))) void*)&to[of_b][block][q >> 1][q & 1][0], 16, 0, 0);
+        }
     }
 }
 // What a wave needs of a step of 16 k: its blocks' parts
-template <int T> struct HalfStep {
+template <int T, HalfTurned TURNED> struct HalfStep {
     f16x8 a[T][2], b[T][2];
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef u32x4 Block[2][2][64];
+    // rows 16 s .. 16 s + 15 of a turned block, as the operand of a step: lane l has column l % 32, rows 8 i + 4 h + j
+    __device__ __forceinline__ static f16x8 turned(const Block& from, int s, int t) {
+        const uint32_t lane = threadIdx.x & 63u, half_block = lane >> 4 & 1u, row = 4u * (lane >> 5) + (lane >> 2 & 3u), column = lane & 3u;
+        const uint32_t place = half_turned_place(row, column & 1u, half_block);
+        const __attribute__((address_space(3))) char* const at = (const __attribute__((address_space(3))) char*)&from[0][0][0] + half_block * 2048u + place * 16u + (column >> 1) * 8u + s * 512u + t * 1024u;
+        const s16x4 low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+        const s16x4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 256u));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
     __device__ __forceinline__ void read(const typename HalfTileOf<T>::Stage& from, int s) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
 #pragma unroll
         for (int i = 0; i < T; ++i)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                a[i][t] = __builtin_bit_cast(f16x8, from[0][T * wm + i][s][t][lane]);
-                b[i][t] = __builtin_bit_cast(f16x8, from[1][T * wn + i][s][t][lane]);
+                a[i][t] = TURNED == TURNED_A ? turned(from[0][T * wm + i], s, t) : __builtin_bit_cast(f16x8, from[0][T * wm + i][s][t][lane]);
+                b[i][t] = TURNED == TURNED_B ? turned(from[1][T * wn + i], s, t) : __builtin_bit_cast(f16x8, from[1][T * wn + i][s][t][lane]);
             }
     }
     __device__ __forceinline__ void multiply(HalfSums<T>& sums) const {
@@ -104,13 +128,13 @@ __device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ
 
 // The sums of tile (m, n) over `pairs` pairs of steps from pair `begin` on. With more than two buffers a wave has the parts of the next step in registers before it
 // multiplies those of this one: the barrier in front of a pair stands between the two steps of the pair before.
-template <int T, int STAGES>
+template <int T, int STAGES, HalfTurned TURNED = TURNED_NONE>
 __device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs) {
     static_assert(STAGES == 2 || STAGES == 4, "as many pairs are on their way as meet() counts");
     constexpr int LOADS = 4 * T;                         // of a wave per stage
     if (pairs == 0u) return;                             // (a slice of nothing)
     uint32_t asked = 0u;                                 // pairs that have been requested
-    auto request = [&](uint32_t at) { half_request<T>(shared.stages[at], a, b, m, n, 2u * (begin + asked)); ++asked; };
+    auto request = [&](uint32_t at) { half_request<T, TURNED>(shared.stages[at], a, b, m, n, 2u * (begin + asked)); ++asked; };
     // pair p has arrived, for all waves (those asked for behind it may be on their way); and all have read what they wanted of the pair before the last
     auto meet = [&](uint32_t p) {
         const uint32_t behind = asked - 1u - p;
@@ -127,7 +151,7 @@ __device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, ST
         for (uint32_t p = 0; p < pairs; ++p) {
             meet(p);
             if (asked < pairs) request(at ^ 1u);
-            HalfStep<T> step;
+            HalfStep<T, TURNED> step;
             step.read(shared.stages[at], 0);
             step.multiply(sums);
             step.read(shared.stages[at], 1);
@@ -135,7 +159,7 @@ __device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, ST
             at ^= 1u;
         }
     } else {
-        HalfStep<T> first, second;
+        HalfStep<T, TURNED> first, second;
         meet(0u);
         if (asked < pairs) request(STAGES - 1u);
         first.read(shared.stages[0], 0);

@@ -7,11 +7,11 @@
 // Products are those of half_product.h: x and W are taken apart first (the largest magnitudes, for their scales, then the parts), then
 //   * forward: a product whose rows are the vocabulary and whose columns are the rows of x, so that a lane has 32 scores of one row; a tile of 128 tokens leaves each row's peak and
 //     sum, a last launch joins the tiles. 4096 x 1024 x 32000: the product as fast as one that keeps its scores, and nothing of 0.5 GB is written.
-//   * backward, in pieces of the vocabulary: the same product again, whose lanes turn scores into q = ds / m, |q| <= 2, with m = max(|g_lp|, |g_ls - g_lp|) of the row, and lay q out as an
-//     operand of both products that follow, contracted over the vocabulary (the lanes have it like that) and over the rows (turned in shared memory). q takes 8 bytes a score of one
-//     piece; the rows' m is a factor of dx's rows, and of the x that dW is made of.
-// 4096 x 1024 x 32000 with its gradient, 3.45 ms: 743 us the scores (361 TFLOP/s of fp32 products), four pieces of 216 q, 190 dx and 195 dW (the floor of 268 GFLOP each at 378 TFLOP/s is 710 us), 150 us
-// to take operands apart. Bound by the matrix cores' power; with few rows by the weights' bytes: 321 x 500 x 50001 takes 460 us, of which 120 take the weights apart both ways.
+//   * backward, in pieces of the vocabulary: the same product again, whose lanes turn scores into q = ds / m, |q| <= 2, with m = max(|g_lp|, |g_ls - g_lp|) of the row, and store q as an operand
+//     (4 bytes a score of a piece). dx = q W^T reads q as it is and the forward pass's W turned, dW = x^T ds reads q turned (half_product.h), so neither is laid out twice; the rows' m is a factor
+//     of dx's rows, and of the x that dW is made of. (Taken apart both ways, W and q: 321 x 500 x 50001 490 us, not 424, 172 x 1400 x 46807 880, not 733, 4096 x 1024 x 32000 3500, not 3340.)
+// 4096 x 1024 x 32000 with its gradient: 745 us the scores (360 TFLOP/s of fp32 products), 780 q, 790 each dx and dW (the floor of 268 GFLOP each at 378 TFLOP/s is 710 us), 100 us to take
+// operands apart. Bound by the matrix cores' power; with few rows by the weights' bytes.
 // Up to 64 rows take the fp32 matrix instructions (RowsProduct), which read W as it is, once forward and once for dx: bound by memory. The scores of so few rows are kept for the gradient.
 #include "half_product.h"
 
@@ -88,17 +88,16 @@ extern "C" __global__ __launch_bounds__(256) void linear_largest(float* __restri
 // ---- operands taken apart (half_product.h). What element (i, k) of an operand is: W or x as they lie, x only of rows that are given, or with the rows' factors.
 enum PackKind : uint32_t { PACK_WEIGHTS = 0, PACK_ROWS = 1, PACK_SCALED = 2 };
 struct PackJob { uint32_t blocks, I, K, stride, kind, steps; uint64_t si, sk; };      // blocks of 256 threads; steps of 16 k; element strides of i and k; `stride`: steps that a wave takes
-struct PackParams { uint32_t weight_blocks, row_blocks, V, pad; PackJob jobs[4]; };
-struct PackOuts { void* parts[4]; };
+struct PackParams { uint32_t weight_blocks, row_blocks, V, pad; PackJob jobs[3]; };
+struct PackOuts { void* parts[3]; };
 extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int32_t* __restrict__ scales, const float* __restrict__ x, const float* __restrict__ w,
-                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors,
-                                                              const int32_t* __restrict__ known, PackParams P) {
+                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors, PackParams P) {
     __shared__ float part[4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t block = blockIdx.x, job = 0u;
-    while (job < 3u && block >= P.jobs[job].blocks) block -= P.jobs[job++].blocks;
+    while (job < 2u && block >= P.jobs[job].blocks) block -= P.jobs[job++].blocks;
     const PackJob J = P.jobs[job];
-    // the operand's scale, of its blocks' largest magnitudes, or the weights' that is known
+    // the operand's scale, of its blocks' largest magnitudes
     const bool weights = J.kind == PACK_WEIGHTS;
     float most = 0.f;
     for (uint32_t k = threadIdx.x; k < (weights ? P.weight_blocks : P.row_blocks); k += 256u)
@@ -106,7 +105,7 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
     most = wave_largest(most);
     if (lane == 0u) part[wave] = most;
     __syncthreads();
-    const int e = weights && known ? known[PACK_WEIGHTS] : half_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+    const int e = half_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
     if (block == 0u && threadIdx.x == 0u) scales[J.kind] = e;
     const float up = power_of_two(e);
     // waves beside one another along the side that is contiguous in memory
@@ -653,9 +652,9 @@ ROWS_DW(16)
 ROWS_DW(32)
 ROWS_DW(64)
 
-// ---- backward: a piece's q, as operands contracted over the vocabulary [rows][tokens] and over the rows [tokens][rows]
+// ---- backward: a piece's q as an operand [rows][tokens], which dx is contracted over the tokens of, and dW, turned, over the rows
 template <int T, int STAGES, bool SHARED>
-__device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4* __restrict__ by_token, float* __restrict__ partial, uint32_t* __restrict__ arrivals, const u32x4* __restrict__ w,
+__device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, float* __restrict__ partial, uint32_t* __restrict__ arrivals, const u32x4* __restrict__ w,
                                               const u32x4* __restrict__ x, const int32_t* __restrict__ tokens, const int32_t* __restrict__ scales, const float* __restrict__ row_peaks,
                                               const float* __restrict__ row_totals, const float* __restrict__ factors, const ScoresParams& P) {
     constexpr uint32_t SIDE = HalfTileOf<T>::SIDE;
@@ -680,7 +679,7 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4*
         token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
         peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
-    half_store<T>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, HalfTarget{by_token, P.Vp / 32u, P.blocks_x * 2u, m * 2u * T, n * 4u * T},
+    half_store<T>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, HalfTarget{nullptr, 0u, 0u, 0u, 0u},
                   [&](int i, int j, int k, uint32_t row, uint32_t) {
         const uint32_t v = v0 + row;
         const float s = scaled(half_sum(acc, i, j, k), down);
@@ -689,33 +688,33 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, u32x4*
     });
 }
 #define LINEAR_Q(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                                     \
-    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_q##SUFFIX(u32x4* by_row, u32x4* by_token, float* partial, uint32_t* arrivals, const u32x4* w,      \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_q##SUFFIX(u32x4* by_row, float* partial, uint32_t* arrivals, const u32x4* w,      \
                                                                                const u32x4* x, const int32_t* tokens, const int32_t* scales, const float* row_peaks,    \
                                                                                const float* row_totals, const float* factors, ScoresParams P) {                         \
-        linear_q_body<T, STAGES, SHARED>(by_row, by_token, partial, arrivals, w, x, tokens, scales, row_peaks, row_totals, factors, P);                                 \
+        linear_q_body<T, STAGES, SHARED>(by_row, partial, arrivals, w, x, tokens, scales, row_peaks, row_totals, factors, P);                                 \
     }
 LINEAR_KERNELS(LINEAR_Q)
 
-// ---- a product of two operands to fp32 [M, N], rows by a factor each (every third word), added to what is there or in its place; not SHARED: a slice of the contraction to an array of its own
+// ---- a product of two operands, one of them turned, to fp32 [M, N], rows by a factor each (every third word), added to what is there or in its place; not SHARED: a slice of the contraction to an array of its own
 struct ProductParams {
     uint32_t M, N, tiles_m, tiles_n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_a, first_b, add;
     int32_t scale_a, scale_b;                            // the kind of operand whose scale it is, or -1: q
     uint32_t whole, slices;                              // (HalfShares)
     uint64_t ld, slice;                                  // elements from a row of the result to the next, from a slice's result to the next one's
 };
-template <int T, int STAGES, bool SHARED>
+template <int T, int STAGES, bool SHARED, HalfTurned TURNED>
 __device__ __forceinline__ void linear_product_body(float* __restrict__ out, float* __restrict__ partial, uint32_t* __restrict__ arrivals, const u32x4* __restrict__ a, const u32x4* __restrict__ b,
-                                                    const int32_t* __restrict__ scales, const float* __restrict__ factors, const ProductParams& P) {
+                                                    const int32_t* __restrict__ scales_a, const int32_t* __restrict__ scales_b, const float* __restrict__ factors, const ProductParams& P) {
     __shared__ HalfShared<T, STAGES> shared;
     uint32_t m, n, tile, slice, begin, end;
     half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
-    half_product<T, STAGES>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
+    half_product<T, STAGES, TURNED>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = (m * 2u + (wave >> 1)) * 32u * T + 4u * (lane >> 5), lane_column = (n * 2u + (wave & 1u)) * 32u * T + (lane & 31u);
-    const int down = -(P.scale_a < 0 ? Q_SCALE : scales[P.scale_a]) - (P.scale_b < 0 ? Q_SCALE : scales[P.scale_b]);
+    const int down = -(P.scale_a < 0 ? Q_SCALE : scales_a[P.scale_a]) - (P.scale_b < 0 ? Q_SCALE : scales_b[P.scale_b]);
     float* const to = out + (SHARED ? 0u : P.slice * slice);
 #pragma unroll
     for (int i = 0; i < T; ++i) {
@@ -745,11 +744,13 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
         }
     }
 }
-#define LINEAR_PRODUCT(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                               \
-    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_product##SUFFIX(float* out, float* partial, uint32_t* arrivals, const u32x4* a, const u32x4* b,    \
-                                                                                     const int32_t* scales, const float* factors, ProductParams P) {                    \
-        linear_product_body<T, STAGES, SHARED>(out, partial, arrivals, a, b, scales, factors, P);                                                                       \
+#define LINEAR_PRODUCT_OF(NAME, TURNED, T, STAGES, BLOCKS, SHARED)                                                                                                      \
+    extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_product_##NAME(float* out, float* partial, uint32_t* arrivals, const u32x4* a, const u32x4* b,     \
+                                                                                    const int32_t* scales_a, const int32_t* scales_b, const float* factors, ProductParams P) { \
+        linear_product_body<T, STAGES, SHARED, TURNED>(out, partial, arrivals, a, b, scales_a, scales_b, factors, P);                                                     \
     }
+#define LINEAR_PRODUCT(SUFFIX, T, STAGES, BLOCKS, SHARED) \
+    LINEAR_PRODUCT_OF(a##SUFFIX, TURNED_A, T, STAGES, BLOCKS, SHARED) LINEAR_PRODUCT_OF(b##SUFFIX, TURNED_B, T, STAGES, BLOCKS, SHARED)
 LINEAR_KERNELS(LINEAR_PRODUCT)
 
 // ---- the slices of a contraction added up; with few elements by four waves, a quarter of the slices each

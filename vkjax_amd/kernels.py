@@ -2877,35 +2877,32 @@ def _linear_sum(out, parts: Buffer, count: int, n: int) -> Launch:
                   bytes_moved=4 * (count + 1) * n)
 
 
-def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, known=None, cotangents=None,
-                    wanted=(True, True)):
-    '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x) - or, where that has been done, with the weights' scale from `known` -, and with cotangents
-    for those behind it, into (the weights contracted over the vocabulary, x with its rows' factors contracted over the rows - as they are `wanted` -, the factors), which are returned. Scales go
-    to `scales`.'''
+def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, cotangents=None, scaled=False):
+    '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x); with cotangents also, into the first of what is returned, x with its rows' factors contracted
+    over the rows (where it is `scaled`), and the factors. Scales go to `scales`.'''
     rows, h, v = shape
     row_blocks    = max(1, min(1024, _cdiv(rows, 4)))
-    weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if known is None else 0
+    weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if forward else 0
     largest = scratch((weight_blocks + 2 * row_blocks,))
     factors = scratch((rows, 3)) if cotangents else None
     g_log_probs, g_log_sums = cotangents or (None, None)
-    by_v, by_h = ((h, 1), (1, h)) if transposed else ((1, v), (v, 1))                       #element strides of (token, h) and (h, token)
-    jobs = [(forward[0], v, h, _PACK_WEIGHTS, by_v), (forward[1], rows, h, _PACK_ROWS, (h, 1))] if forward else []
-    behind = (None, None)
-    if cotangents:
-        behind = tuple(scratch((_half_words(h, k),), np.uint32) if needed else None for k, needed in zip((v, rows), wanted))
-        jobs += [job for job in ((behind[0], h, v, _PACK_WEIGHTS, by_h), (behind[1], h, rows, _PACK_SCALED, (1, h))) if job[0] is not None]
+    jobs = [(forward[0], v, h, _PACK_WEIGHTS, (h, 1) if transposed else (1, v)), (forward[1], rows, h, _PACK_ROWS, (h, 1))] if forward else []
+    x_scaled = scratch((_half_words(h, rows),), np.uint32) if scaled else None
+    if scaled:
+        jobs.append((x_scaled, h, rows, _PACK_SCALED, (1, h)))
     params, blocks = _u32(weight_blocks, row_blocks, v, 0), 0
     for _, i, k, kind, strides in jobs:
         steps  = _half_steps(k)
         each   = min(steps, 8)
         blocks += _cdiv(_cdiv(i, 32) * _cdiv(steps, each), 4)
         params += _u32(_cdiv(_cdiv(i, 32) * _cdiv(steps, each), 4), i, k, each, kind, steps) + _u64(*strides)
-    params += bytes(40) * (4 - len(jobs))
+    params += bytes(40) * (3 - len(jobs))
     launches = [Launch('linear_largest', (weight_blocks + row_blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (largest, factors, x, w, tokens, g_log_probs, g_log_sums)],
-                       _u32(0, rows, h, v, weight_blocks, row_blocks), bytes_moved=4 * (x.size + w.size), written=(0, 1)),
-                Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(j[0], 0) for j in jobs] + [(None, 0)] * (4 - len(jobs)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors, known)],
-                       params, bytes_moved=8 * sum(i * k for _, i, k, _, _ in jobs), written=(0, 1, 2, 3, 4))]
-    return launches, (*behind, factors)
+                       _u32(0, rows, h, v, weight_blocks, row_blocks), bytes_moved=4 * (x.size + w.size), written=(0, 1))]
+    if jobs:
+        launches.append(Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(j[0], 0) for j in jobs] + [(None, 0)] * (3 - len(jobs)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors)],
+                               params, bytes_moved=8 * sum(i * k for _, i, k, _, _ in jobs), written=(0, 1, 2, 3)))
+    return launches, (x_scaled, factors)
 
 
 def _linear_scores_launch(name: str, shape: LinearShape, tokens: int, tile0, width: int, buffers, written, shared, scratch, zeroed) -> tp.Tuple[Launch, int]:
@@ -2919,7 +2916,7 @@ def _linear_scores_launch(name: str, shape: LinearShape, tokens: int, tile0, wid
     buffers = [*buffers[:shared], partial, arrivals, *buffers[shared:]]
     return Launch(f'{name}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in buffers],
                   _u32(rows, v, pairs, 2 * pairs, 2 * pairs, _cdiv(tokens, plan.side), _cdiv(rows, plan.side), _cdiv(v, 32), _cdiv(rows, 32), tile0(plan.side), width, plan.whole, plan.slices),
-                  bytes_moved=4 * h * (tokens + rows) + (8 * rows * tokens if width else 0), flops=2 * rows * h * tokens,
+                  bytes_moved=4 * h * (tokens + rows) + (4 * rows * tokens if width else 0), flops=2 * rows * h * tokens,
                   written=written + ((shared, shared + 1) if partial is not None else ()), scratch=(shared + 1,) if partial is not None else ()), plan.side
 
 
@@ -2946,30 +2943,26 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
     shape = rows, h, v = _linear_shape(x, w, transposed)
     if _linear_few(rows, h, v):
         return _linear_rows_grad(dx, dw, shape, x, w, tokens, peaks, totals, g_log_probs, g_log_sums, transposed, scratch, *(parts or [None]))
-    scales = scratch((4,), np.int32)                       #of all that is taken apart here
-    wanted = dx is not None, dw is not None
-    if parts:
-        w_parts, x_parts, score_scales = parts
-        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None, score_scales, (g_log_probs, g_log_sums), wanted)
-    else:
-        w_parts, x_parts = [scratch((n,), np.uint32) for n, _ in linear_parts(x.shape, w.shape, transposed)[:2]]
-        score_scales = scales
-        launches, (w_by_h, x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, (w_parts, x_parts), None, (g_log_probs, g_log_sums), wanted)
+    scales = scratch((4,), np.int32)                       #of what is taken apart here
+    w_parts, x_parts, score_scales = parts or [*(scratch((n,), np.uint32) for n, _ in linear_parts(x.shape, w.shape, transposed)[:2]), scales]
+    launches, (x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None if parts else (w_parts, x_parts), (g_log_probs, g_log_sums), dw is not None)
     #pieces of the vocabulary, of whole tiles
     row_blocks, all_tiles = _cdiv(rows, 32), _cdiv(v, HALF_TILE)
-    pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (8 * 32 * row_blocks * HALF_TILE)))
+    pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (4 * 32 * row_blocks * HALF_TILE)))
     each   = _cdiv(all_tiles, pieces)
     pieces = _cdiv(all_tiles, each)
     width  = each * HALF_TILE
-    by_row, by_token = (scratch((row_blocks * (width // 16) * 512,), np.uint32) if needed else None for needed in wanted)
+    q = scratch((row_blocks * (width // 16) * 512,), np.uint32)
     tiles_r = _cdiv(rows, HALF_TILE)
 
-    def product(out, offset, a, b, m, n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_b, scale_a, scale_b, ld, by_rows=False, add=False, parts=0):
-        #(parts: slices to arrays of their own)
+    def product(turned, out, offset, a, b, m, n, pairs, blocks_a, blocks_b, steps_a, steps_b, first_b, scale_a, scale_b, ld, by_rows=False, add=False, parts=0):
+        #(scales: an array and an element of it, or None for q's; parts: slices to arrays of their own)
         tiles_of = lambda side: _cdiv(m, side) * _cdiv(n, side)
         plan = HalfPlan('_128', HALF_TILE, 0, parts) if parts else half_plan(tiles_of, pairs)
         suffix, blocks, partial, arrivals = (plan.kernel, tiles_of(HALF_TILE) * parts, None, None) if parts else half_share(plan, tiles_of(plan.side), scratch, zeroed)
-        return Launch(f'linear_product{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(out, 4 * offset), (partial, 0), (arrivals, 0), (a, 0), (b, 0), (scales, 0), (factors if by_rows else None, 0)],
+        (array_a, scale_a), (array_b, scale_b) = (s or (None, -1) for s in (scale_a, scale_b))
+        return Launch(f'linear_product_{turned}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1),
+                      [(out, 4 * offset), (partial, 0), (arrivals, 0), (a, 0), (b, 0), (array_a, 0), (array_b, 0), (factors if by_rows else None, 0)],
                       _u32(m, n, _cdiv(m, plan.side), _cdiv(n, plan.side), pairs, blocks_a, blocks_b, steps_a, steps_b, 0, first_b, add) + _i32(scale_a, scale_b)
                       + _u32(plan.whole, plan.slices) + _u64(ld, m * n), bytes_moved=4 * (m + n) * 32 * pairs + 4 * m * n, flops=64 * m * n * pairs,
                       written=(0, 1, 2) if partial is not None else (0,), scratch=(2,) if partial is not None else ())
@@ -2984,18 +2977,17 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         first = piece * each
         tiles = min(each, all_tiles - first)
         v0, n = first * HALF_TILE, min(width, v - first * HALF_TILE)
-        launches.append(_linear_scores_launch('linear_q', shape, tiles * HALF_TILE, lambda side: v0 // side, width, (by_row, by_token, w_parts, x_parts, tokens, score_scales, peaks, totals, factors),
-                                              (0, 1), 2, scratch, zeroed)[0])
+        launches.append(_linear_scores_launch('linear_q', shape, tiles * HALF_TILE, lambda side: v0 // side, width, (q, w_parts, x_parts, tokens, score_scales, peaks, totals, factors),
+                                              (0,), 1, scratch, zeroed)[0])
         if dx is not None:
-            launches.append(product(sums, 0, by_row, w_by_h, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(v), v0 // 16, -1, _PACK_WEIGHTS, h,
+            launches.append(product('b', sums, 0, q, w_parts, rows, h, _cdiv(n, 32), row_blocks, _cdiv(h, 32), width // 16, _half_steps(h), v0 // 16, None, (score_scales, _PACK_WEIGHTS), h,
                                     by_rows=True, add=piece > 0, parts=parts))
-        steps = 2 * row_blocks
         if dw is None:
             continue
         if transposed:
-            launches.append(product(dw, v0 * h, by_token, x_scaled, n, h, row_blocks, tiles * 4, _cdiv(h, 32), steps, steps, 0, -1, _PACK_SCALED, h))
+            launches.append(product('a', dw, v0 * h, q, x_scaled, n, h, row_blocks, tiles * 4, _cdiv(h, 32), width // 16, 2 * row_blocks, 0, None, (scales, _PACK_SCALED), h))
         else:
-            launches.append(product(dw, v0, x_scaled, by_token, h, n, row_blocks, _cdiv(h, 32), tiles * 4, steps, steps, 0, _PACK_SCALED, -1, v))
+            launches.append(product('b', dw, v0, x_scaled, q, h, n, row_blocks, _cdiv(h, 32), tiles * 4, 2 * row_blocks, width // 16, 0, (scales, _PACK_SCALED), None, v))
     if parts:
         launches.append(_linear_sum(dx, sums, parts, rows * h))
     return launches
