@@ -1,7 +1,7 @@
 // Matrices with their singular values brought towards 1 by a polynomial: X = x / (|x| + eps) (Frobenius norm, per matrix), then `steps` times
 //   A = X X^T,  B = a I + b A + c A A,  X <- B X          (of the wide way round: a matrix with more rows than columns is transposed)
 // so that every singular value s becomes a s + b s^3 + c s^5. Products are those of half_product.h, between operands that never leave their taken-apart form: a product's tile
-// turns its results into the operands that the next ones need, contracted over its rows (as the lanes have them) and over its columns (turned in shared memory). A and B are symmetric:
+// turns its results into an operand, X into one contracted over its columns (turned in shared memory), which B X reads turned again (contracted over rows). A and B are symmetric:
 // of their tiles only those on and above the diagonal are computed, and stored both ways. Only A is kept as fp32 too, since b A is a term of B. X has 22 bits between the steps; no
 // operand's magnitude depends on the data beyond |x|, since a singular value's bound follows from the polynomial alone, so scales are known to the host.
 // Matrices of a stack lie side by side in every launch.
@@ -39,32 +39,31 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __re
     if (threadIdx.x == 0u) sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// X taken apart, contracted over its columns [rows][columns] and over its rows [columns][rows]. A wave takes up to `each` steps of a block of 32.
+// X taken apart, contracted over its columns [rows][columns]. A wave takes up to `each` steps of a block of 32.
 struct OrthogonalPackParams {
-    uint32_t matrices, R, C, sum_blocks, each_c, each_r, blocks_row, blocks_column;      // blocks_..: of 256 threads, per matrix
+    uint32_t matrices, R, C, sum_blocks, each, blocks;                                   // blocks of 256 threads, per matrix
     uint64_t sr, sc;                                                                     // element strides of row and column
     float eps; int32_t scale;
 };
-extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, u32x4* __restrict__ by_column, const float* __restrict__ x, const float* __restrict__ sums, OrthogonalPackParams P) {
+extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, const float* __restrict__ x, const float* __restrict__ sums, OrthogonalPackParams P) {
     __shared__ float part[4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t per = P.blocks_row + P.blocks_column, matrix = blockIdx.x / per, block = blockIdx.x - matrix * per;
+    const uint32_t matrix = blockIdx.x / P.blocks, block = blockIdx.x - matrix * P.blocks;
     float t = 0.f;
     for (uint32_t k = threadIdx.x; k < P.sum_blocks; k += 256u) t += sums[(uint64_t)matrix * P.sum_blocks + k];
     wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
     if (lane == 0u) part[wave] = t;
     __syncthreads();
     const float norm = __builtin_sqrtf((part[0] + part[1]) + (part[2] + part[3])) + P.eps, up = power_of_two(P.scale);
-    const bool rows = block < P.blocks_row;
-    const uint32_t I = rows ? P.R : P.C, K = rows ? P.C : P.R, steps = 2u * ((K + 31u) / 32u), each = rows ? P.each_c : P.each_r;
-    const uint64_t si = rows ? P.sr : P.sc, sk = rows ? P.sc : P.sr;
-    const uint32_t groups = (steps + each - 1u) / each, all = (rows ? block : block - P.blocks_row) * 4u + wave, blocks32 = (I + 31u) / 32u;
+    const uint32_t I = P.R, K = P.C, steps = 2u * ((K + 31u) / 32u), each = P.each;
+    const uint64_t si = P.sr, sk = P.sc;
+    const uint32_t groups = (steps + each - 1u) / each, all = block * 4u + wave, blocks32 = (I + 31u) / 32u;
     const bool along_k = sk == 1u;
     const uint32_t rb = along_k ? all / groups : all % blocks32, group = along_k ? all % groups : all / blocks32;
     if (rb >= blocks32 || group >= groups) return;
     const uint32_t i = rb * 32u + (lane & 31u), h4 = 4u * (lane >> 5);
     const float* const from = x + (uint64_t)matrix * P.R * P.C + (uint64_t)min(i, I - 1u) * si;
-    u32x4* const to = (rows ? by_row : by_column) + ((uint64_t)matrix * blocks32 + rb) * steps * 128u + lane;
+    u32x4* const to = by_row + ((uint64_t)matrix * blocks32 + rb) * steps * 128u + lane;
     // (the operands of four steps at once)
     constexpr int AT_ONCE = 4;
     const uint32_t end = min(steps, (group + 1u) * each);
@@ -121,8 +120,9 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
         m = at - n * (n + 1u) / 2u;
     } else half_tile(at, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
-    half_product<T, STAGES>(acc, shared, HalfOperand{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u},
-                            HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
+    const HalfOperand left{a + (uint64_t)matrix * blocks_m * steps_k * 128u, blocks_m, steps_k, 0u};
+    if constexpr (SYMMETRIC) half_product<T, STAGES>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
+    else half_product<T, STAGES, TURNED_B>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * (steps_k / 2u) * steps_n * 128u, blocks_n, steps_n, 0u}, m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
     const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
@@ -152,7 +152,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
                     const uint32_t row = min(lane_row + 32u * i + 8u * (k >> 2) + (k & 3), P.M - 1u), column = min(lane_column + 32u * j, P.N - 1u);
                     squares[i][j][k] = square[each + (uint64_t)row * P.N + column];
                 }
-    const HalfTarget columns{by_column + (uint64_t)matrix * blocks_n * steps_m * 128u, blocks_n, steps_m, n * 2u * T, m * 4u * T};
+    const HalfTarget columns{SYMMETRIC ? by_column + (uint64_t)matrix * blocks_n * steps_m * 128u : nullptr, blocks_n, steps_m, n * 2u * T, m * 4u * T};
     // (a tile on the diagonal of a square is its own mirror image)
     const HalfTarget rows{SYMMETRIC && m == n ? nullptr : by_row + (uint64_t)matrix * blocks_m * steps_n * 128u, blocks_m, steps_n, m * 2u * T, n * 4u * T};
     half_store<T>(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {

@@ -3022,19 +3022,18 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
     tall = rows > columns
     r, c = (columns, rows) if tall else (rows, columns)
     sr, sc = (1, columns) if tall else (columns, 1)                                         #element strides of the wide way round
-    if max(r, c) >= 2**20 or n * _cdiv(r, 64) * _cdiv(c, 64) >= 2**24 or n * (_cdiv(r, 32) * _half_steps(c) + _cdiv(c, 32) * _half_steps(r)) >= 2**28:
+    if max(r, c) >= 2**20 or n * _cdiv(r, 64) * _cdiv(c, 64) >= 2**24 or n * _cdiv(r, 32) * _half_steps(c) >= 2**27:
         raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
     sum_blocks = max(1, min(1024 if n == 1 else 256, _cdiv(r * c, 4096)))
     sums     = scratch((n, sum_blocks))
-    by_row   = scratch((n * _half_words(r, c),), np.uint32)
-    by_column = [scratch((n * _half_words(c, r),), np.uint32) for _ in range(2 if steps > 1 else 1)]
+    by_row   = [scratch((n * _half_words(r, c),), np.uint32) for _ in range(2 if steps > 1 else 1)]
     square, square_parts, polynomial = scratch((n, r, r)), scratch((n * _half_words(r, r),), np.uint32), scratch((n * _half_words(r, r),), np.uint32)
     bounds   = orthogonal_bounds(steps, coefficients)
-    each     = [min(_half_steps(k), 8) for k in (c, r)]
-    blocks   = [_cdiv(_cdiv(i, 32) * _cdiv(_half_steps(k), e), 4) for i, k, e in ((r, c, each[0]), (c, r, each[1]))]
+    each     = min(_half_steps(c), 8)
+    blocks   = _cdiv(_cdiv(r, 32) * _cdiv(_half_steps(c), each), 4)
     launches = [Launch('orthogonal_squares', (n * sum_blocks, 1, 1), (BLOCK, 1, 1), [(sums, 0), (x, 0)], _u32(sum_blocks, 0) + _u64(r * c), bytes_moved=4 * x.size),
-                Launch('orthogonal_pack', (n * sum(blocks), 1, 1), (BLOCK, 1, 1), [(by_row, 0), (by_column[0], 0), (x, 0), (sums, 0)],
-                       _u32(n, r, c, sum_blocks, *each, *blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])), bytes_moved=16 * x.size, written=(0, 1))]
+                Launch('orthogonal_pack', (n * blocks, 1, 1), (BLOCK, 1, 1), [(by_row[0], 0), (x, 0), (sums, 0)],
+                       _u32(n, r, c, sum_blocks, each, blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])), bytes_moved=8 * x.size)]
 
     def product(name, results, a, b, square, m, width, k, scales, written):
         symmetric = name in ('square', 'polynomial')
@@ -3048,10 +3047,10 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
                       written=written + ((3, 4) if partial is not None else ()), scratch=(4,) if partial is not None else ())
     for i, (s, p) in enumerate(bounds):
         scale_x, scale_a, scale_p = _half_scale(s), _half_scale(s * s), _half_scale(p)
-        launches += [product('square', (square_parts, square_parts, square), by_row, by_row, None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2)),
+        launches += [product('square', (square_parts, square_parts, square), by_row[i & 1], by_row[i & 1], None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2)),
                      product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, (scale_a, scale_a, scale_p), (0, 1))]
         last = i == steps - 1
         scale_next = 0 if last else _half_scale(bounds[i + 1][0])
-        launches.append(product('last' if last else 'next', (None, None, out) if last else (by_column[(i + 1) & 1], by_row, None), polynomial, by_column[i & 1], None, r, c, r,
-                                (scale_p, scale_x, scale_next), (2,) if last else (0, 1)))
+        launches.append(product('last' if last else 'next', (None, None, out) if last else (None, by_row[(i + 1) & 1], None), polynomial, by_row[i & 1], None, r, c, r,
+                                (scale_p, scale_x, scale_next), (2,) if last else (1,)))
     return launches
