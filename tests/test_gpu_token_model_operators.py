@@ -412,8 +412,8 @@ def orthogonal_bound(x, steps, coefficients, eps=1e-7):
     return total + 1e-30
 
 
-#shapes: one element, fewer rows than a block of 32, wide and tall, no multiples of anything, one tile and several, stacks
-MATRICES = [(1, 1), (1, 9), (5, 3), (2, 7, 40), (33, 65), (128, 128), (3, 130, 100), (2, 2, 64, 200), (257, 129), (300, 520), (20, 32, 31), (129, 1000)]
+#shapes: one element, up to 64 rows either way round (no multiples of 16, one slice of columns and many), fewer rows than a block of 32, wide and tall, no multiples of anything, one tile and several, stacks
+MATRICES = [(1, 1), (1, 9), (4, 4), (16, 17), (2, 20, 700), (3, 300, 10), (500, 50), (64, 64), (2, 48, 1000), (64, 5000), (9, 9000), (4097, 63), (40, 64, 20), (5, 3), (2, 7, 40), (33, 65), (128, 128), (3, 130, 100), (2, 2, 64, 200), (257, 129), (300, 520), (20, 32, 31), (129, 1000)]
 
 
 @pytest.mark.parametrize('steps,coefficients', [(5, (3.4445, -4.7750, 2.0315)), (1, (1.5, -0.5, 0.0)), (2, (2.0, -1.5, 0.5))], ids=str)
@@ -435,15 +435,27 @@ def test_orthogonalize_by_the_size_of_its_matrix(scale):
     assert np.linalg.norm(got.astype(np.float64) - expected) <= orthogonal_bound(x, 5, (3.4445, -4.7750, 2.0315))
 
 
-def test_orthogonalize_a_matrix_of_a_low_rank_and_of_zeros():
-    x = normal(1, 4, 150, 90, scale=1e-2)
-    x[1] = normal(2, 150, 2) @ normal(3, 2, 90)
+@pytest.mark.parametrize('rows,columns', [(150, 90), (40, 90), (300, 64)])
+def test_orthogonalize_a_matrix_of_a_low_rank_and_of_zeros(rows, columns):
+    x = normal(1, 4, rows, columns, scale=1e-2)
+    x[1] = normal(2, rows, 2) @ normal(3, 2, columns)
     x[2] = 0.0
     x[3, 7, 8] = np.nan
     (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x), x)
     assert not got[2].any() and np.isnan(got[3]).all()
     for i in (0, 1):
         assert np.linalg.norm(got[i].astype(np.float64) - expected[i]) <= orthogonal_bound(x[i], 5, (3.4445, -4.7750, 2.0315))
+
+
+@pytest.mark.parametrize('steps', [1, 5, 6, 7, 18, 32])
+def test_orthogonalize_singular_values_far_apart(steps):
+    #a few rows, of which the smallest singular values are 1e-4 of the largest: what the squares of those lose in fp32 would decide where they go
+    for coefficients in ((3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0)):
+        u, _, v = np.linalg.svd(normal(7, 30, 400), full_matrices=False)
+        x = (u * np.logspace(0, -4, 30) @ v).astype(f32)
+        (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, steps, coefficients), x)
+        off, bound = np.linalg.norm(got.astype(np.float64) - expected), orthogonal_bound(x, steps, coefficients)
+        assert off <= bound, (off, bound)
 
 
 @pytest.mark.parametrize('rows', [9, 64, 150])

@@ -180,3 +180,225 @@ ORTHOGONAL_KINDS(_64, 1, 4, 2, false)
 ORTHOGONAL(square, SQUARE, _64_shared, 1, 4, 2, true)
 ORTHOGONAL_KINDS(_64_many, 1, 2, 4, false)
 ORTHOGONAL_KINDS(_64_many_shared, 1, 2, 4, true)
+
+// ---- few rows (4 to 64 of the wide way round). All of the polynomials are functions of G = X X^T, so that G alone goes through the steps, G <- B G B, P <- B P, by a block per matrix, and X only
+// through the first product and the last, P X. That is three launches instead of two and three for every step. G starts in fp64, from products that are exact there, and stays in it (v_mfma_f64_16x16x4):
+// a small singular value s is there as s^2, and what fp32 would lose of that beside the largest is what decides its polynomial. P X is a product of fp32 numbers.
+// (Errors of G grow with the small eigenvalues and are not made good by a product X X^T in every step: for as many steps as leave them below 2^-24, six with a = 3.44, 18 with 1.5.)
+// Lanes of the instruction: operands row (column) l % 16 and k = l / 16, results row 4 q + l / 16, column l % 16. Symmetric matrices have their blocks on and above the diagonal computed.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t SMALL = 64u, SMALL_PITCH = 66u, SMALL_BLOCKS = 10u;     // (rows of 66 doubles: 16 rows' pairs of words lie in different banks)
+__device__ __forceinline__ uint32_t upper_block(uint32_t i, uint32_t j) { return j * (j + 1u) / 2u + i; }
+
+struct GramParams { uint32_t R, C, slices, each; uint64_t sr, sc; };        // each: columns of a slice, a multiple of 64
+// [matrix][slice][block][q][lane]
+extern "C" __global__ __launch_bounds__(256) void orthogonal_gram(double* __restrict__ sums, const float* __restrict__ x, GramParams P) {
+    __shared__ double met[3][SMALL_BLOCKS][4][64];
+    const uint32_t matrix = blockIdx.x / P.slices, slice = blockIdx.x % P.slices, lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t blocks = (P.R + 15u) / 16u, row = lane & 15u, quarter = lane >> 4, end = min(P.C, (slice + 1u) * P.each);
+    const float* const from = x + (uint64_t)matrix * P.R * P.C;
+    const bool along = P.sc == 1u;
+    f64x4 acc[SMALL_BLOCKS] = {};
+    float next[4][4];
+    // 16 columns: four to a lane's vector where they are neighbours, every fourth one otherwise
+    auto request = [&](uint32_t c0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            if (i >= blocks) continue;
+            const float* const at = from + min(16u * i + row, P.R - 1u) * P.sr;
+            if (along && c0 + 16u <= P.C) {
+                const f32x4 v = *reinterpret_cast<const f32x4_anywhere*>(at + c0 + 4u * quarter);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) next[i][e] = v[e];
+            } else
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) next[i][e] = at[min(c0 + (along ? 4u * quarter + e : 4u * e + quarter), P.C - 1u) * P.sc];
+        }
+    };
+    uint32_t c0 = slice * P.each + 16u * wave;
+    if (c0 < end) request(c0);
+    for (; c0 < end; c0 += 64u) {
+        double v[4][4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t c = c0 + (along ? 4u * quarter + e : 4u * e + quarter);
+                v[i][e] = i < blocks && 16u * i + row < P.R && c < end ? (double)next[i][e] : 0.0;
+            }
+        if (c0 + 64u < end) request(c0 + 64u);
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i <= j; ++i)
+                if (j < blocks)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[upper_block(i, j)] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[i][e], v[j][e], acc[upper_block(i, j)], 0, 0, 0);
+    }
+    if (wave > 0u)
+#pragma unroll
+        for (uint32_t b = 0; b < SMALL_BLOCKS; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) met[wave - 1u][b][q][lane] = acc[b][q];
+    __syncthreads();
+    if (wave > 0u) return;
+    double* const to = sums + (uint64_t)blockIdx.x * SMALL_BLOCKS * 256u + lane;
+#pragma unroll
+    for (uint32_t b = 0; b < SMALL_BLOCKS; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) to[(b * 4u + q) * 64u] = ((acc[b][q] + met[0][b][q][lane]) + met[1][b][q][lane]) + met[2][b][q][lane];
+}
+
+struct SmallParams { uint32_t R, slices, steps; float a, b, c, eps; uint32_t pad; };
+// P / (|x| + eps) of every matrix, fp32 [64][64], zeros behind its rows. 16 waves, so that a SIMD has others to multiply for while one waits for shared memory (with four, a block to each SIMD's
+// one wave, five steps of 64 x 64 took 56 us, not 36)
+extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __restrict__ polynomials, const double* __restrict__ sums, SmallParams P) {
+    __shared__ double G[SMALL * SMALL_PITCH], B[SMALL * SMALL_PITCH], Q[SMALL * SMALL_PITCH];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), blocks = (P.R + 15u) / 16u, upper = blocks * (blocks + 1u) / 2u;
+    // element q of this lane of an upper block, and its mirror image
+    auto block_of = [&](uint32_t number, uint32_t& i, uint32_t& j) { j = number < 1u ? 0u : number < 3u ? 1u : number < 6u ? 2u : 3u; i = number - j * (j + 1u) / 2u; };
+    auto put = [&](double* m, uint32_t i, uint32_t j, const f64x4& v) {
+#pragma unroll
+        for (uint32_t q = 0; q < 4u; ++q) {
+            const uint32_t r = 16u * i + 4u * q + (lane >> 4), c = 16u * j + (lane & 15u);
+            m[r * SMALL_PITCH + c] = v[q];
+            if (i != j) m[c * SMALL_PITCH + r] = v[q];
+        }
+    };
+    // block (i, j) of the product of two symmetric matrices
+    auto product = [&](const double* m, const double* n, uint32_t i, uint32_t j) {
+        f64x4 s = {0.0, 0.0, 0.0, 0.0};
+        const double* const a = m + (16u * i + (lane & 15u)) * SMALL_PITCH + (lane >> 4);
+        const double* const b = n + (16u * j + (lane & 15u)) * SMALL_PITCH + (lane >> 4);
+#pragma unroll 2
+        for (uint32_t k = 0; k < 16u * blocks; k += 16u)
+#pragma unroll
+            for (uint32_t e = 0; e < 16u; e += 4u) s = __builtin_amdgcn_mfma_f64_16x16x4f64(a[k + e], b[k + e], s, 0, 0, 0);
+        return s;
+    };
+    if (wave < upper) {
+        const uint32_t number = wave;
+        uint32_t i, j;
+        block_of(number, i, j);
+        const double* const from = sums + ((uint64_t)blockIdx.x * P.slices * SMALL_BLOCKS + number) * 256u + lane;
+        f64x4 s = {0.0, 0.0, 0.0, 0.0};
+        for (uint32_t k = 0; k < P.slices; k += 4u) {
+            f64x4 v[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u)
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q) v[u][q] = from[(uint64_t)min(k + u, P.slices - 1u) * SMALL_BLOCKS * 256u + q * 64u];
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u)
+                if (k + u < P.slices)
+#pragma unroll
+                    for (uint32_t q = 0; q < 4u; ++q) s[q] += v[u][q];
+        }
+        put(G, i, j, s);
+    }
+    __syncthreads();
+    double squares = 0.0;
+    for (uint32_t k = 0; k < P.R; ++k) squares += G[k * SMALL_PITCH + k];
+    const double norm = __builtin_sqrt(squares) + (double)P.eps, down = 1.0 / (norm * norm);
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < 16u * blocks * 16u * blocks; k += 1024u) G[k / (16u * blocks) * SMALL_PITCH + k % (16u * blocks)] *= down;
+    __syncthreads();
+    uint32_t i, j;
+    block_of(min(wave, upper - 1u), i, j);
+    for (uint32_t step = 0; step < P.steps; ++step) {
+        // B = a I + b G + c G G
+        if (wave < upper) {
+            f64x4 s = product(G, G, i, j);
+#pragma unroll
+            for (uint32_t q = 0; q < 4u; ++q) {
+                const uint32_t r = 16u * i + 4u * q + (lane >> 4), c = 16u * j + (lane & 15u);
+                s[q] = (double)P.c * s[q] + (double)P.b * G[r * SMALL_PITCH + c] + (r == c ? (double)P.a : 0.0);
+            }
+            put(B, i, j, s);
+        }
+        __syncthreads();
+        // P <- P B and G <- G B, then G <- G B once more; of the blocks of both (P's first), two at most to a wave
+        const bool last = step + 1u == P.steps;
+        const uint32_t units = last ? upper : 2u * upper;
+        f64x4 found[2];
+        auto unit = [&](uint32_t u, auto f) {
+            if (u >= units) return;
+            uint32_t bi, bj;
+            block_of(u < upper ? u : u - upper, bi, bj);
+            f(u < upper, bi, bj);
+        };
+#pragma unroll
+        for (uint32_t u = 0; u < 2u; ++u)
+            unit(wave + 16u * u, [&](bool of_p, uint32_t bi, uint32_t bj) {
+                if (of_p && step == 0u) {
+#pragma unroll
+                    for (uint32_t q = 0; q < 4u; ++q) found[u][q] = B[(16u * bi + 4u * q + (lane >> 4)) * SMALL_PITCH + 16u * bj + (lane & 15u)];
+                } else found[u] = product(of_p ? Q : G, B, bi, bj);
+            });
+        __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < 2u; ++u) unit(wave + 16u * u, [&](bool of_p, uint32_t bi, uint32_t bj) { put(of_p ? Q : G, bi, bj, found[u]); });
+        __syncthreads();
+        if (last) break;
+        if (wave < upper) found[0] = product(G, B, i, j);
+        __syncthreads();
+        if (wave < upper) put(G, i, j, found[0]);
+        __syncthreads();
+    }
+    for (uint32_t k = threadIdx.x; k < SMALL * SMALL; k += 1024u) {
+        const uint32_t r = k / SMALL, c = k % SMALL;
+        polynomials[(uint64_t)blockIdx.x * SMALL * SMALL + k] = r < P.R && c < P.R ? (float)(Q[r * SMALL_PITCH + c] / norm) : 0.f;
+    }
+}
+
+// P x, with the fp32 matrix instructions: a wave has up to 32 rows of the result and 32 of its columns, which are a lane each where x is [R][C] (four to a lane: a lone wave's products take 4 us,
+// not one, and large matrices gain nothing), and a row each where it lies the other way round.
+struct ApplyParams { uint32_t R, C, tasks, blocks; };                       // tasks of a matrix, one a wave; blocks of four waves a matrix
+template <bool WIDE, int ROWS>
+__device__ __forceinline__ void orthogonal_apply_body(float* __restrict__ out, const float* __restrict__ x, const float* __restrict__ polynomials, const ApplyParams& P) {
+    __shared__ float poly[SMALL][SMALL];
+    constexpr uint32_t HALVES = ROWS == 64 ? 2u : 1u;
+    const uint32_t matrix = blockIdx.x / P.blocks, task = (blockIdx.x % P.blocks) * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t half = threadIdx.x >> 5 & 1u, l32 = threadIdx.x & 31u, r0 = task % HALVES * 32u, c0 = task / HALVES * 32u, c = min(c0 + l32, P.C - 1u);
+    const uint64_t first = (uint64_t)matrix * P.R * P.C;
+    // (columns and rows behind the end are the last ones again; what is stored twice is the same)
+    float v[ROWS / 2];
+    if constexpr (WIDE) {
+#pragma unroll
+        for (uint32_t k = 0; k < ROWS / 2; ++k) v[k] = x[first + (uint64_t)min(2u * k + half, P.R - 1u) * P.C + c];
+    } else
+#pragma unroll
+        for (uint32_t k = 0; k < ROWS / 8; ++k) {
+            const f32x4 t = *reinterpret_cast<const f32x4_anywhere*>(x + first + (uint64_t)c * P.R + min(8u * k + 4u * half, P.R - 4u));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * k + e] = t[e];
+        }
+    for (uint32_t k = threadIdx.x; k < SMALL * SMALL / 4u; k += 256u) reinterpret_cast<f32x4*>(&poly[0][0])[k] = reinterpret_cast<const f32x4*>(polynomials + (uint64_t)matrix * SMALL * SMALL)[k];
+    __syncthreads();
+    if (task >= P.tasks || r0 >= P.R) return;
+    f32x16 acc = {};
+#pragma unroll
+    for (uint32_t k = 0; k < ROWS / 2; ++k) {
+        if constexpr (WIDE) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(poly[2u * k + half][r0 + l32], v[k], acc, 0, 0, 0);      // (behind the last row: zeros, times x's last row again)
+        else {
+            const uint32_t wanted = 8u * (k / 4u) + 4u * half, at = min(wanted, P.R - 4u) + k % 4u;
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(at >= wanted ? v[k] : 0.f, poly[at][r0 + l32], acc, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const uint32_t r = 8u * (q >> 2) + 4u * half + (q & 3);
+        if constexpr (WIDE) { if (r0 + r < P.R) out[first + (uint64_t)(r0 + r) * P.C + c] = acc[q]; }
+        else if (c0 + r < P.C && r0 + l32 < P.R) out[first + (uint64_t)(c0 + r) * P.R + r0 + l32] = acc[q];
+    }
+}
+#define ORTHOGONAL_APPLY(NAME, WIDE, ROWS)                                                                                                                            \
+    extern "C" __global__ __launch_bounds__(256) void orthogonal_apply_##NAME##_##ROWS(float* out, const float* x, const float* polynomials, ApplyParams P) {         \
+        orthogonal_apply_body<WIDE, ROWS>(out, x, polynomials, P);                                                                                                    \
+    }
+ORTHOGONAL_APPLY(wide, true, 16)
+ORTHOGONAL_APPLY(wide, true, 32)
+ORTHOGONAL_APPLY(wide, true, 64)
+ORTHOGONAL_APPLY(tall, false, 16)
+ORTHOGONAL_APPLY(tall, false, 32)
+ORTHOGONAL_APPLY(tall, false, 64)
