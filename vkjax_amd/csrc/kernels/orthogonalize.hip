@@ -191,7 +191,7 @@ constexpr uint32_t SMALL = 64u, SMALL_PITCH = 66u, SMALL_BLOCKS = 10u;     // (r
 __device__ __forceinline__ uint32_t upper_block(uint32_t i, uint32_t j) { return j * (j + 1u) / 2u + i; }
 
 struct GramParams { uint32_t R, C, slices, each; uint64_t sr, sc; };        // each: columns of a slice, a multiple of 64
-// [matrix][slice][block][q][lane]
+// [matrix][slice][upper block][q][lane]
 extern "C" __global__ __launch_bounds__(256) void orthogonal_gram(double* __restrict__ sums, const float* __restrict__ x, GramParams P) {
     __shared__ double met[3][SMALL_BLOCKS][4][64];
     const uint32_t matrix = blockIdx.x / P.slices, slice = blockIdx.x % P.slices, lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -242,15 +242,17 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_gram(double* __rest
             for (int q = 0; q < 4; ++q) met[wave - 1u][b][q][lane] = acc[b][q];
     __syncthreads();
     if (wave > 0u) return;
-    double* const to = sums + (uint64_t)blockIdx.x * SMALL_BLOCKS * 256u + lane;
+    const uint32_t upper = blocks * (blocks + 1u) / 2u;
+    double* const to = sums + (uint64_t)blockIdx.x * upper * 256u + lane;
 #pragma unroll
     for (uint32_t b = 0; b < SMALL_BLOCKS; ++b)
+        if (b < upper)
 #pragma unroll
         for (int q = 0; q < 4; ++q) to[(b * 4u + q) * 64u] = ((acc[b][q] + met[0][b][q][lane]) + met[1][b][q][lane]) + met[2][b][q][lane];
 }
 
 struct SmallParams { uint32_t R, slices, steps; float a, b, c, eps; uint32_t pad; };
-// P / (|x| + eps) of every matrix, fp32 [64][64], zeros behind its rows. 16 waves, so that a SIMD has others to multiply for while one waits for shared memory (with four, a block to each SIMD's
+// P / (|x| + eps) of every matrix, fp32, [S][S] for its rows in whole blocks of 16, zeros behind the last. 16 waves, so that a SIMD has others to multiply for while one waits for shared memory (with four, a block to each SIMD's
 // one wave, five steps of 64 x 64 took 56 us, not 36)
 extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __restrict__ polynomials, const double* __restrict__ sums, SmallParams P) {
     __shared__ double G[SMALL * SMALL_PITCH], B[SMALL * SMALL_PITCH], Q[SMALL * SMALL_PITCH];
@@ -280,14 +282,14 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
         const uint32_t number = wave;
         uint32_t i, j;
         block_of(number, i, j);
-        const double* const from = sums + ((uint64_t)blockIdx.x * P.slices * SMALL_BLOCKS + number) * 256u + lane;
+        const double* const from = sums + ((uint64_t)blockIdx.x * P.slices * upper + number) * 256u + lane;
         f64x4 s = {0.0, 0.0, 0.0, 0.0};
         for (uint32_t k = 0; k < P.slices; k += 4u) {
             f64x4 v[4];
 #pragma unroll
             for (uint32_t u = 0; u < 4u; ++u)
 #pragma unroll
-                for (uint32_t q = 0; q < 4u; ++q) v[u][q] = from[(uint64_t)min(k + u, P.slices - 1u) * SMALL_BLOCKS * 256u + q * 64u];
+                for (uint32_t q = 0; q < 4u; ++q) v[u][q] = from[(uint64_t)min(k + u, P.slices - 1u) * upper * 256u + q * 64u];
 #pragma unroll
             for (uint32_t u = 0; u < 4u; ++u)
                 if (k + u < P.slices)
@@ -345,9 +347,10 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
         if (wave < upper) put(G, i, j, found[0]);
         __syncthreads();
     }
-    for (uint32_t k = threadIdx.x; k < SMALL * SMALL; k += 1024u) {
-        const uint32_t r = k / SMALL, c = k % SMALL;
-        polynomials[(uint64_t)blockIdx.x * SMALL * SMALL + k] = r < P.R && c < P.R ? (float)(Q[r * SMALL_PITCH + c] / norm) : 0.f;
+    const uint32_t S = 16u * blocks;
+    for (uint32_t k = threadIdx.x; k < S * S; k += 1024u) {
+        const uint32_t r = k / S, c = k % S;
+        polynomials[(uint64_t)blockIdx.x * S * S + k] = r < P.R && c < P.R ? (float)(Q[r * SMALL_PITCH + c] / norm) : 0.f;
     }
 }
 
@@ -373,7 +376,15 @@ __device__ __forceinline__ void orthogonal_apply_body(float* __restrict__ out, c
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[4 * k + e] = t[e];
         }
-    for (uint32_t k = threadIdx.x; k < SMALL * SMALL / 4u; k += 256u) reinterpret_cast<f32x4*>(&poly[0][0])[k] = reinterpret_cast<const f32x4*>(polynomials + (uint64_t)matrix * SMALL * SMALL)[k];
+    const uint32_t S = (P.R + 15u) / 16u * 16u;
+    const float* const from = polynomials + (uint64_t)matrix * S * S;
+    constexpr uint32_t VECTORS = (ROWS < 32 ? 32 : ROWS) / 4;
+#pragma unroll
+    for (uint32_t k0 = 0; k0 < ROWS * VECTORS; k0 += 256u) {
+        const uint32_t k = k0 + threadIdx.x, r = k / VECTORS, at = k % VECTORS * 4u;
+        const f32x4 p = *reinterpret_cast<const f32x4*>(from + min(r, S - 1u) * S + min(at, S - 4u));
+        if (k < ROWS * VECTORS) *reinterpret_cast<f32x4*>(&poly[r][at]) = r < S && at < S ? p : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     __syncthreads();
     if (task >= P.tasks || r0 >= P.R) return;
     f32x16 acc = {};

@@ -3020,7 +3020,8 @@ def _orthogonalize_small(out: Buffer, x: Buffer, n: int, r: int, c: int, sr: int
     slices = max(1, min(64, _cdiv(c, 128), _cdiv(1024, n)))
     each   = _cdiv(_cdiv(c, slices), 64) * 64
     slices = _cdiv(c, each)
-    sums, polynomials = scratch((n, slices, 10, 4, 64, 2)), scratch((n, ORTHOGONAL_SMALL, ORTHOGONAL_SMALL))         #(fp64)
+    side   = _cdiv(r, 16)
+    sums, polynomials = scratch((n, slices, side * (side + 1) // 2, 4, 64, 2)), scratch((n, 16 * side, 16 * side))         #(the former fp64)
     rows   = max(16, _pow2_at_least(r))
     tasks  = _cdiv(c, 32) * _cdiv(rows, 32)
     blocks = _cdiv(tasks, 4)
