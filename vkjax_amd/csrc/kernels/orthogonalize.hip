@@ -5,8 +5,8 @@
 // of their tiles only those on and above the diagonal are computed, and stored both ways. Only A is kept as fp32 too, since b A is a term of B. X has 22 bits between the steps; no
 // operand's magnitude depends on the data beyond |x|, since a singular value's bound follows from the polynomial alone, so scales are known to the host.
 // Matrices of a stack lie side by side in every launch.
-// Bound by the matrix cores' power where a matrix fills the machine: 4096 x 4096 takes 211 us for a square, 260 for the polynomial (whose epilogue reads the square), 375 for B X (367 TFLOP/s of fp32
-// products), 4.4 ms for five steps, of which the products alone at that rate are 3.6. 12 of 512 x 512: 13 to 18 us a launch, whose contraction of 512 is 16 pairs of steps behind one another.
+// Bound by the matrix cores' power where a matrix fills the machine: 4096 x 4096 takes 212 us for a square, 257 for the polynomial (whose epilogue reads the square), 380 for B X (362 TFLOP/s of fp32
+// products), 4.45 ms for five steps, of which the products alone at that rate are 3.6. 12 of 512 x 512: 13 to 18 us a launch, whose contraction of 512 is 16 pairs of steps behind one another.
 #include "half_product.h"
 
 typedef f32x4 f32x4_anywhere __attribute__((aligned(4)));

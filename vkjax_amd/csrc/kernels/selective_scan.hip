@@ -10,9 +10,9 @@
 // A block has 64 channels, a lane of each of its M waves one of them and NS of its states in registers, so b and c, which all channels of a sequence share, come
 // from shared memory, a vector for all lanes. What a step needs once per channel (dt, the gates, loads and stores) is shared out: of every 8 steps a wave prepares 8 / M and puts them into shared memory, all waves go
 // through the 8 steps with their states and leave their parts of the sums over n there, and the wave that has prepared a step adds those up and stores its results. Bound by the
-// vector instructions: an exponential takes the time of four of them, a state and step that of eight, in the gradient 21.
-// 1 x 16384 x 2048 x 16 states: 122 us for the chunks' states and 176 for the scan (537 million exponentials each, which alone take 60 us: 16 cycles for a wave's 64), 11 between them; the
-// arrays alone are 110 us. 4 x 2048 x 2048 x 16 with its gradient: 59 + 111 forward, 66 + 281 + 17 backward. b and c through shared memory, eight steps at a time: read as scalars they took
+// vector instructions: an exponential takes the time of four of them, a state and step that of eight, in the gradient 27.
+// 1 x 16384 x 2048 x 16 states: 122 us for the chunks' states and 177 for the scan (537 million exponentials each, which alone take 60 us: 16 cycles for a wave's 64), 5 between them; the
+// arrays alone are 110 us. 4 x 2048 x 2048 x 16 with its gradient: 60 + 111 forward, 67 + 282 + 17 backward. b and c through shared memory, eight steps at a time: read as scalars they took
 // 603 us of the former in all.
 // A block goes through its steps one after the other; where batch and channels are too few to fill the machine, time is cut into chunks: a first launch leaves each chunk's
 // sum of dt (the product of its factors is exp(A sum dt)) and its state from zero, a second one follows those along the chunks, and the third has the state in front of
