@@ -152,11 +152,11 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
         if (at.has(P, i)) at.held(states, P, at.chunk, i)[at.c] = h[i];
 }
 
-// ---- the state in front of every chunk, in the place of its state from zero; the same for the adjoint from the last chunk on, and the initial state's cotangent. A block has 64
+// ---- the state in front of every chunk, in the place of its state from zero; the same for the adjoint from the last chunk on. A block has 64
 // (sequence, state, channel) and up to 16 waves, of which each composes eight chunks to a map, h -> product h + own; what lies in front of its first chunk follows from the waves' maps in front of
 // it. (Chunk by chunk in one wave, loads wait for one another: 191 chunks took 50 us.)
 struct ScanJoinParams { uint32_t first, B, C, N, chunks, back; };
-extern "C" __global__ __launch_bounds__(1024) void selective_scan_join(float* __restrict__ states, float* __restrict__ end, const float* __restrict__ sums, const float* __restrict__ a,
+extern "C" __global__ __launch_bounds__(1024) void selective_scan_join(float* __restrict__ states, const float* __restrict__ sums, const float* __restrict__ a,
                                                                        const float* __restrict__ initial, ScanJoinParams P) {
     constexpr uint32_t EACH = 8u;
     __shared__ float maps[2][16][2][64];
@@ -196,7 +196,6 @@ extern "C" __global__ __launch_bounds__(1024) void selective_scan_join(float* __
             mine_h = __builtin_fmaf(factor[q], mine_h, own[q]);
         }
     }
-    if (end && wave == 0u && place < all) end[at] = h;
 }
 
 // ---- the scan itself, a chunk from the state in front of it
@@ -408,9 +407,9 @@ __device__ __forceinline__ float over_channels(float (&v)[8]) {
     return s + lane_xor<1>(s);
 }
 
-// ---- the gradient of a chunk
+// ---- the gradient of a chunk; what the adjoint comes to in front of the first one is the initial state's cotangent
 template <int NS, int M>
-__device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __restrict__ ddelta, float* __restrict__ dgate, float* __restrict__ maps, float* __restrict__ channel_sums,
+__device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __restrict__ ddelta, float* __restrict__ dgate, float* __restrict__ dstate, float* __restrict__ maps, float* __restrict__ channel_sums,
                                                const float* __restrict__ x, const float* __restrict__ delta, const float* __restrict__ a, const float* __restrict__ bmap,
                                                const float* __restrict__ cmap, const float* __restrict__ through, const float* __restrict__ gate, const int32_t* __restrict__ lengths,
                                                const float* __restrict__ bias, const float* __restrict__ kept, const float* __restrict__ g, const float* __restrict__ g_last,
@@ -574,6 +573,9 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
     prepared[1][at.wave][at.lane] = dbias;
     at.meet();
     if (!at.there) return;
+    if (dstate && at.chunk == 0u)
+#pragma unroll
+        for (int i = 0; i < NS; ++i) if (at.has(P, i)) dstate[at.state(P, i)] = l[i];
     float* const row = channel_sums + ((uint64_t)at.b * P.chunks + at.chunk) * (P.N + 2u) * P.C + at.c;
 #pragma unroll
     for (int i = 0; i < NS; ++i) if (at.has(P, i)) row[(uint64_t)(at.n0 + i) * P.C] = da[i];
@@ -599,12 +601,12 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                                                                                                 ScanParams P) {                                                                    \
         scan_grad_chunk_body<NS, M>(sums, states, delta, a, cmap, gate, bias, lengths, g, P);                                                                                      \
     }                                                                                                                                                                              \
-    extern "C" __global__ __launch_bounds__(64 * M, NS == 8 || M == 1 ? 2 : M == 8 ? 4 : 3) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* maps, float* channel_sums, const float* x, \
+    extern "C" __global__ __launch_bounds__(64 * M, NS == 8 || M == 1 ? 2 : M == 8 ? 4 : 3) void selective_scan_grad_n##NS##_m##M(float* dx, float* ddelta, float* dgate, float* dstate, float* maps, float* channel_sums, const float* x, \
                                                                                           const float* delta, const float* a, const float* bmap, const float* cmap,                \
                                                                                           const float* through, const float* gate, const int32_t* lengths, const float* bias,      \
                                                                                           const float* kept, const float* g, const float* g_last, const float* adjoints,           \
                                                                                           ScanParams P) {                                                                          \
-        scan_grad_body<NS, M>(dx, ddelta, dgate, maps, channel_sums, x, delta, a, bmap, cmap, through, gate, lengths, bias, kept, g, g_last, adjoints, P);                         \
+        scan_grad_body<NS, M>(dx, ddelta, dgate, dstate, maps, channel_sums, x, delta, a, bmap, cmap, through, gate, lengths, bias, kept, g, g_last, adjoints, P);                         \
     }
 SELECTIVE_SCAN(4, 1)
 SELECTIVE_SCAN(4, 2)

@@ -2663,10 +2663,10 @@ def _scan_launch(name: str, x: Buffer, tiling: ScanTiling, n: int, softplus, arr
                   _u32(0, b, t, c, n, tiling.strips, tiling.chunks, tiling.chunk, bool(softplus)), bytes_moved=moved, written=written, streamable=bool(streamed), streamed=streamed or (0,))
 
 
-def _scan_join(states, end, sums, a: Buffer, initial, x: Buffer, tiling: ScanTiling, back: bool) -> Launch:
+def _scan_join(states, sums, a: Buffer, initial, x: Buffer, tiling: ScanTiling, back: bool) -> Launch:
     (b, _, c), n = x.shape, a.shape[1]
-    return Launch('selective_scan_join', (_cdiv(b * c * n, 64), 1, 1), (64 * min(16, _cdiv(tiling.chunks, 8)), 1, 1), [(v, 0) for v in (states, end, sums, a, initial)],
-                  _u32(0, b, c, n, tiling.chunks, back), bytes_moved=8 * b * c * n * tiling.chunks, written=(0, 1))
+    return Launch('selective_scan_join', (_cdiv(b * c * n, 64), 1, 1), (64 * min(16, _cdiv(tiling.chunks, 8)), 1, 1), [(v, 0) for v in (states, sums, a, initial)],
+                  _u32(0, b, c, n, tiling.chunks, back), bytes_moved=8 * b * c * n * tiling.chunks)
 
 
 def selective_scan(y, last, kept, x: Buffer, delta: Buffer, a: Buffer, b: Buffer, c: Buffer, d, gate, state, lengths, bias, softplus, scratch) -> tp.List[Launch]:
@@ -2684,7 +2684,7 @@ def selective_scan(y, last, kept, x: Buffer, delta: Buffer, a: Buffer, b: Buffer
     if tiling.chunks > 1:
         sums, states = scratch((tiling.chunks, batch, channels)), scratch((tiling.chunks, batch, n, channels))
         launches = [_scan_launch('selective_scan_chunk', x, tiling, n, softplus, (sums, states, x, delta, a, b, bias, lengths), (0, 1), 8 * x.size),
-                    _scan_join(states, None, sums, a, state, x, tiling, False)]
+                    _scan_join(states, sums, a, state, x, tiling, False)]
     return launches + [_scan_launch('selective_scan', x, tiling, n, softplus, (y, last, kept, x, delta, a, b, c, d, gate, state, lengths, bias, states),
                                     (0, 1, 2), moved, (0,) if y is not None else ())]
 
@@ -2694,14 +2694,14 @@ def selective_scan_grad(dx, ddelta, da, db, dc, dd, dgate, dstate, dbias, kept: 
     (batch, time, channels), n = x.shape, a.shape[1]
     tiling = selective_scan_tiling(batch, time, channels, n)
     adjoints, launches = None, []
-    if tiling.chunks > 1 or dstate is not None:
+    if tiling.chunks > 1:
         sums, adjoints = scratch((tiling.chunks, batch, channels)), scratch((tiling.chunks, batch, n, channels))
         launches = [_scan_launch('selective_scan_grad_chunk', x, tiling, n, softplus, (sums, adjoints, delta, a, c, gate, bias, lengths, g), (0, 1), 12 * x.size),
-                    _scan_join(adjoints, dstate, sums, a, g_last, x, tiling, True)]
+                    _scan_join(adjoints, sums, a, g_last, x, tiling, True)]
     maps = scratch((tiling.strips, batch * time, 2, n))
     rows = scratch((batch * tiling.chunks, n + 2, channels))
     launches.append(_scan_launch('selective_scan_grad', x, tiling, n, softplus,
-                                 (dx, ddelta, dgate, maps, rows, x, delta, a, b, c, d, gate, lengths, bias, kept, g, g_last, adjoints), (0, 1, 2, 3, 4),
+                                 (dx, ddelta, dgate, dstate, maps, rows, x, delta, a, b, c, d, gate, lengths, bias, kept, g, g_last, adjoints), (0, 1, 2, 3, 4, 5),
                                  4 * x.size * (5 + 2 * (gate is not None)), tuple(i for i, v in enumerate((dx, ddelta, dgate)) if v is not None)))
     map_blocks = _cdiv(batch * time * 2 * n, 1024)
     blocks     = map_blocks + _cdiv((n + 2) * channels, 64)
