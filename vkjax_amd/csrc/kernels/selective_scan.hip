@@ -53,6 +53,7 @@ __device__ __forceinline__ float width_of(float delta, float bias, uint32_t soft
 __device__ __forceinline__ int sequence_length(const int32_t* lengths, uint32_t b, uint32_t T) {
     return lengths ? min(max(lengths[b], 0), (int)T) : (int)T;
 }
+template <bool B> struct Whole { static constexpr bool value = B; };
 #define STEP_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 // Where a wave is: a strip of channels of one sequence, a chunk of its time, NS of the states. Lanes behind the last channel work on that one again and store nothing.
@@ -248,8 +249,12 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
             for (int s = 0; s < KEPT; ++s) { dt[s] = prepared[0][s][at.lane]; u[s] = prepared[1][s][at.lane]; }
             at.maps(next_b, map[0], 0);
             at.maps(next_c, map[1], 0);
+            // (steps behind the last are nobody's: a single one would take the time of eight. Whole turns have a loop of their own, which knows of none: 177 us of a prompt, not 184)
+            const int count = at.stop - t0;
+            auto steps = [&](auto whole) {
 #pragma unroll
             for (int s = 0; s < KEPT; ++s) {
+                if (!decltype(whole)::value && s >= count) break;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
                 if (s + 1 < KEPT) { at.maps(next_b, map[0], s + 1); at.maps(next_c, map[1], s + 1); }
@@ -262,6 +267,8 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
                 parts[at.wave][s][at.lane] = sum;
                 STEP_FENCE();
             }
+            };
+            if (count >= KEPT) steps(Whole<true>{}); else steps(Whole<false>{});
             at.meet();
 #pragma unroll
             for (int q = 0; q < at.OWN; ++q) {
@@ -479,8 +486,10 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 for (int i = 0; i < NS; ++i) { bs[i] = next_b[i]; cs[i] = next_c[i]; }
             };
             next(0);
+            const int count = at.stop - t0;
 #pragma unroll
             for (int s0 = 0; s0 < KEPT; s0 += AT_ONCE) {
+                if (s0 >= count) break;
                 float part[8];
 #pragma unroll
                 for (int g = 0; g < AT_ONCE; ++g) {
@@ -502,9 +511,10 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                 if (over_stores) mapped[1][s0 + over / NS][at.n0 + over % NS] = sum;
                 STEP_FENCE();
             }
-            next(KEPT - 1);
+            next(min(count, KEPT) - 1 | (AT_ONCE - 1));
 #pragma unroll
             for (int s0 = KEPT - AT_ONCE; s0 >= 0; s0 -= AT_ONCE) {
+                if (s0 >= count) continue;
                 float part[8];
 #pragma unroll
                 for (int g = AT_ONCE - 1; g >= 0; --g) {
@@ -590,7 +600,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
                                                                                            const float* bias, const int32_t* lengths, ScanParams P) {                              \
         scan_chunk_body<NS, M>(sums, states, x, delta, a, bmap, bias, lengths, P);                                                                                                 \
     }                                                                                                                                                                              \
-    extern "C" __global__ __launch_bounds__(64 * M) void selective_scan_n##NS##_m##M(float* y, float* last, float* kept, const float* x, const float* delta, const float* a,       \
+    extern "C" __global__ __launch_bounds__(64 * M, NS == 8 ? 4 : 1) void selective_scan_n##NS##_m##M(float* y, float* last, float* kept, const float* x, const float* delta, const float* a,       \
                                                                                      const float* bmap, const float* cmap, const float* through, const float* gate,                \
                                                                                      const float* state, const int32_t* lengths, const float* bias, const float* states,           \
                                                                                      ScanParams P) {                                                                               \
