@@ -222,6 +222,8 @@ CAUSAL_CONV_WIDTHS(CAUSAL_CONV, 4, 1)
 CAUSAL_CONV_WIDTHS(CAUSAL_CONV, 1, 1)
 CAUSAL_CONV_WIDTHS(CAUSAL_CONV, 4, 8)
 CAUSAL_CONV_WIDTHS(CAUSAL_CONV, 1, 8)
+CAUSAL_CONV_WIDTHS(CAUSAL_CONV_GRAD, 4, 1)
+CAUSAL_CONV_WIDTHS(CAUSAL_CONV_GRAD, 1, 1)
 CAUSAL_CONV_WIDTHS(CAUSAL_CONV_GRAD, 4, 8)
 CAUSAL_CONV_WIDTHS(CAUSAL_CONV_GRAD, 1, 8)
 

@@ -2608,11 +2608,11 @@ def causal_conv(y, last, x: Buffer, kernel: Buffer, bias, state, lengths, activa
 
 def causal_conv_grad(dx, dkernel, dbias, dstate, x: Buffer, kernel: Buffer, bias, state, lengths, g, g_last, activation, scratch) -> tp.List[Launch]:
     (b, t, c), k = x.shape, kernel.shape[0]
-    vec, _, lanes, cstrips, tiles = _causal_conv_tiling(b, max(t, 2), c)
+    vec, steps, lanes, cstrips, tiles = _causal_conv_tiling(b, t, c)
     turns  = max(1, min(tiles, b * cstrips * tiles // CAUSAL_CONV_GRAD_BLOCKS))
     rows   = b * _cdiv(tiles, turns)
     sums   = scratch((rows, k + 1, c)) if dkernel is not None or dbias is not None else None
-    launch = Launch(f'causal_conv_grad_k{k}_v{vec}_l{CAUSAL_CONV_STEPS}', _causal_conv_blocks(x, rows * cstrips), (BLOCK, 1, 1),
+    launch = Launch(f'causal_conv_grad_k{k}_v{vec}_l{steps}', _causal_conv_blocks(x, rows * cstrips), (BLOCK, 1, 1),
                     [(v, 0) for v in (dx, dstate, sums, x, kernel, bias, state, lengths, g, g_last)],
                     _u32(0, t, c, cstrips, tiles, turns, lanes.bit_length() - 1, activation == 'silu'), lds=4 * BLOCK * vec * (k + 1),
                     bytes_moved=12 * x.size, written=(0, 1, 2), streamable=dx is not None)
