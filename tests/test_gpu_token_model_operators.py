@@ -501,3 +501,13 @@ def test_gradient_of_log_probs_with_shared_contractions(monkeypatch):
             print(f'gradient with shared contractions: {kernel}, {slices} slices', flush=True)
             monkeypatch.setattr(K, 'half_plan', lambda tiles_of, pairs: K.HalfPlan(kernel, side, 3 if slices > 1 else tiles_of(side), min(slices, pairs)))
             check_loss(x, w, tokens, g, gs, False)
+
+
+@pytest.mark.parametrize('n,rows,columns,steps', [(700, 20, 30, 1), (700, 20, 30, 3), (600, 64, 66, 5), (1100, 12, 9, 2)])
+def test_orthogonalize_many_matrices(n, rows, columns, steps):
+    x = normal(n, n, rows, columns)
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, steps), x)
+    for i in (0, 1, n // 2, n - 2, n - 1):
+        off, bound = np.linalg.norm(got[i].astype(np.float64) - expected[i]), orthogonal_bound(x[i], steps, (3.4445, -4.7750, 2.0315))
+        assert off <= bound, (i, off, bound)
+    assert np.isfinite(got).all() and (np.linalg.norm(got - expected, axis=(1, 2)) < 0.05 * np.sqrt(min(rows, columns))).all()

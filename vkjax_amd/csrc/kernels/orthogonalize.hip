@@ -187,7 +187,7 @@ ORTHOGONAL_KINDS(_64_many_shared, 1, 2, 4, true)
 // (Errors of G grow with the small eigenvalues and are not made good by a product X X^T in every step: for as many steps as leave them below 2^-24, six with a = 3.44, 18 with 1.5.)
 // Lanes of the instruction: operands row (column) l % 16 and k = l / 16, results row 4 q + l / 16, column l % 16. Symmetric matrices have their blocks on and above the diagonal computed.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-constexpr uint32_t SMALL = 64u, SMALL_PITCH = 66u, SMALL_BLOCKS = 10u;     // (rows of 66 doubles: 16 rows' pairs of words lie in different banks)
+constexpr uint32_t SMALL = 64u, SMALL_BLOCKS = 10u;
 __device__ __forceinline__ uint32_t upper_block(uint32_t i, uint32_t j) { return j * (j + 1u) / 2u + i; }
 
 struct GramParams { uint32_t R, C, slices, each; uint64_t sr, sc; };        // each: columns of a slice, a multiple of 64
@@ -252,34 +252,36 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_gram(double* __rest
 }
 
 struct SmallParams { uint32_t R, slices, steps; float a, b, c, eps; uint32_t pad; };
-// P / (|x| + eps) of every matrix, fp32, [S][S] for its rows in whole blocks of 16, zeros behind the last. 16 waves, so that a SIMD has others to multiply for while one waits for shared memory (with four, a block to each SIMD's
-// one wave, five steps of 64 x 64 took 56 us, not 36)
+// P / (|x| + eps) of every matrix, fp32, [S][S] for its rows in whole blocks of 16, zeros behind the last. Up to 16 waves, so that a SIMD has others to multiply for while one waits for shared memory (with four,
+// a block to each SIMD's one wave, five steps of 64 x 64 took 56 us, not 36); waves and shared memory as the matrix wants them, so that a CU has several small ones. Rows of S + 2 doubles: 16 rows'
+// pairs of words lie in different banks.
 extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __restrict__ polynomials, const double* __restrict__ sums, SmallParams P) {
-    __shared__ double G[SMALL * SMALL_PITCH], B[SMALL * SMALL_PITCH], Q[SMALL * SMALL_PITCH];
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), blocks = (P.R + 15u) / 16u, upper = blocks * (blocks + 1u) / 2u;
+    extern __shared__ double memory[];                          // G, B, P
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, blocks = (P.R + 15u) / 16u, upper = blocks * (blocks + 1u) / 2u;
+    const uint32_t S = 16u * blocks, pitch = S + 2u;
+    double* const G = memory, * const B = G + S * pitch, * const Q = B + S * pitch;
     // element q of this lane of an upper block, and its mirror image
     auto block_of = [&](uint32_t number, uint32_t& i, uint32_t& j) { j = number < 1u ? 0u : number < 3u ? 1u : number < 6u ? 2u : 3u; i = number - j * (j + 1u) / 2u; };
     auto put = [&](double* m, uint32_t i, uint32_t j, const f64x4& v) {
 #pragma unroll
         for (uint32_t q = 0; q < 4u; ++q) {
             const uint32_t r = 16u * i + 4u * q + (lane >> 4), c = 16u * j + (lane & 15u);
-            m[r * SMALL_PITCH + c] = v[q];
-            if (i != j) m[c * SMALL_PITCH + r] = v[q];
+            m[r * pitch + c] = v[q];
+            if (i != j) m[c * pitch + r] = v[q];
         }
     };
     // block (i, j) of the product of two symmetric matrices
     auto product = [&](const double* m, const double* n, uint32_t i, uint32_t j) {
         f64x4 s = {0.0, 0.0, 0.0, 0.0};
-        const double* const a = m + (16u * i + (lane & 15u)) * SMALL_PITCH + (lane >> 4);
-        const double* const b = n + (16u * j + (lane & 15u)) * SMALL_PITCH + (lane >> 4);
+        const double* const a = m + (16u * i + (lane & 15u)) * pitch + (lane >> 4);
+        const double* const b = n + (16u * j + (lane & 15u)) * pitch + (lane >> 4);
 #pragma unroll 2
         for (uint32_t k = 0; k < 16u * blocks; k += 16u)
 #pragma unroll
             for (uint32_t e = 0; e < 16u; e += 4u) s = __builtin_amdgcn_mfma_f64_16x16x4f64(a[k + e], b[k + e], s, 0, 0, 0);
         return s;
     };
-    if (wave < upper) {
-        const uint32_t number = wave;
+    for (uint32_t number = wave; number < upper; number += waves) {
         uint32_t i, j;
         block_of(number, i, j);
         const double* const from = sums + ((uint64_t)blockIdx.x * P.slices * upper + number) * 256u + lane;
@@ -300,10 +302,10 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
     }
     __syncthreads();
     double squares = 0.0;
-    for (uint32_t k = 0; k < P.R; ++k) squares += G[k * SMALL_PITCH + k];
+    for (uint32_t k = 0; k < P.R; ++k) squares += G[k * pitch + k];
     const double norm = __builtin_sqrt(squares) + (double)P.eps, down = 1.0 / (norm * norm);
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k < 16u * blocks * 16u * blocks; k += 1024u) G[k / (16u * blocks) * SMALL_PITCH + k % (16u * blocks)] *= down;
+    for (uint32_t k = threadIdx.x; k < S * S; k += blockDim.x) G[k / S * pitch + k % S] *= down;
     __syncthreads();
     uint32_t i, j;
     block_of(min(wave, upper - 1u), i, j);
@@ -314,7 +316,7 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
 #pragma unroll
             for (uint32_t q = 0; q < 4u; ++q) {
                 const uint32_t r = 16u * i + 4u * q + (lane >> 4), c = 16u * j + (lane & 15u);
-                s[q] = (double)P.c * s[q] + (double)P.b * G[r * SMALL_PITCH + c] + (r == c ? (double)P.a : 0.0);
+                s[q] = (double)P.c * s[q] + (double)P.b * G[r * pitch + c] + (r == c ? (double)P.a : 0.0);
             }
             put(B, i, j, s);
         }
@@ -331,15 +333,15 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
         };
 #pragma unroll
         for (uint32_t u = 0; u < 2u; ++u)
-            unit(wave + 16u * u, [&](bool of_p, uint32_t bi, uint32_t bj) {
+            unit(wave + waves * u, [&](bool of_p, uint32_t bi, uint32_t bj) {
                 if (of_p && step == 0u) {
 #pragma unroll
-                    for (uint32_t q = 0; q < 4u; ++q) found[u][q] = B[(16u * bi + 4u * q + (lane >> 4)) * SMALL_PITCH + 16u * bj + (lane & 15u)];
+                    for (uint32_t q = 0; q < 4u; ++q) found[u][q] = B[(16u * bi + 4u * q + (lane >> 4)) * pitch + 16u * bj + (lane & 15u)];
                 } else found[u] = product(of_p ? Q : G, B, bi, bj);
             });
         __syncthreads();
 #pragma unroll
-        for (uint32_t u = 0; u < 2u; ++u) unit(wave + 16u * u, [&](bool of_p, uint32_t bi, uint32_t bj) { put(of_p ? Q : G, bi, bj, found[u]); });
+        for (uint32_t u = 0; u < 2u; ++u) unit(wave + waves * u, [&](bool of_p, uint32_t bi, uint32_t bj) { put(of_p ? Q : G, bi, bj, found[u]); });
         __syncthreads();
         if (last) break;
         if (wave < upper) found[0] = product(G, B, i, j);
@@ -347,10 +349,9 @@ extern "C" __global__ __launch_bounds__(1024) void orthogonal_small(float* __res
         if (wave < upper) put(G, i, j, found[0]);
         __syncthreads();
     }
-    const uint32_t S = 16u * blocks;
-    for (uint32_t k = threadIdx.x; k < S * S; k += 1024u) {
+    for (uint32_t k = threadIdx.x; k < S * S; k += blockDim.x) {
         const uint32_t r = k / S, c = k % S;
-        polynomials[(uint64_t)blockIdx.x * S * S + k] = r < P.R && c < P.R ? (float)(Q[r * SMALL_PITCH + c] / norm) : 0.f;
+        polynomials[(uint64_t)blockIdx.x * S * S + k] = r < P.R && c < P.R ? (float)(Q[r * pitch + c] / norm) : 0.f;
     }
 }
 

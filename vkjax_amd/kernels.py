@@ -3011,7 +3011,8 @@ def orthogonal_bounds(steps: int, coefficients) -> tp.List[tp.Tuple[float, float
     return found
 
 
-#matrices of 4 to 64 rows and up to 65536 columns go by their Gram matrices (5 x 122 x 19 five steps 73 -> 21 us, 32 x 64 x 4096 207 -> 90, 1 x 64 x 64 one step 20.6 -> 18)
+#matrices of 4 to 64 rows and up to 65536 columns go by their Gram matrices (5 x 122 x 19 five steps 73 -> 20 us, 32 x 64 x 4096 207 -> 93, 1 x 64 x 64 one step 20 -> 19, 4096 x 16 x 16
+#five 239 -> 49)
 ORTHOGONAL_SMALL, ORTHOGONAL_SMALL_COLUMNS = 64, 1 << 16         #(the wide way round)
 
 
@@ -3026,8 +3027,8 @@ def _orthogonalize_small(out: Buffer, x: Buffer, n: int, r: int, c: int, sr: int
     tasks  = _cdiv(c, 32) * _cdiv(rows, 32)
     blocks = _cdiv(tasks, 4)
     return [Launch('orthogonal_gram', (n * slices, 1, 1), (BLOCK, 1, 1), [(sums, 0), (x, 0)], _u32(r, c, slices, each) + _u64(sr, sc), bytes_moved=4 * x.size, flops=n * r * r * c),
-            Launch('orthogonal_small', (n, 1, 1), (1024, 1, 1), [(polynomials, 0), (sums, 0)], _u32(r, slices, steps) + np.asarray([*coefficients, eps], np.float32).tobytes() + _u32(0),
-                   bytes_moved=4 * sums.size),
+            Launch('orthogonal_small', (n, 1, 1), (64 * min(16, side * (side + 1)), 1, 1), [(polynomials, 0), (sums, 0)],
+                   _u32(r, slices, steps) + np.asarray([*coefficients, eps], np.float32).tobytes() + _u32(0), lds=3 * 8 * 16 * side * (16 * side + 2), bytes_moved=4 * sums.size),
             Launch(f'orthogonal_apply_{"wide" if sc == 1 else "tall"}_{rows}', (n * blocks, 1, 1), (BLOCK, 1, 1), [(out, 0), (x, 0), (polynomials, 0)],
                    _u32(r, c, tasks, blocks), bytes_moved=8 * x.size, flops=2 * n * r * r * c)]
 
@@ -3047,7 +3048,9 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
         raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
     #a Gram matrix's errors, 2^-46 of its largest eigenvalue (some of them negative ones where x has no rank), grow as small eigenvalues do, by the polynomials' squares: below 2^-24 in the end
     growth = math.prod(max(1.0, p / 1.25)**2 for _, p in orthogonal_bounds(steps, coefficients))
-    if 4 <= r <= ORTHOGONAL_SMALL and c <= ORTHOGONAL_SMALL_COLUMNS and n * c < 2**29 and growth <= 2**22:
+    #(many matrices that are hardly wider than high fill the machine in the general form too: 4096 of 64 x 64, one step 153 us, by Gram matrices 247, five 600 and 704; of 48 x 48 126 and 166, 534 and 415)
+    many = n > 512 and c < 4 * r and r > (16 if steps == 1 else 48)
+    if 4 <= r <= ORTHOGONAL_SMALL and c <= ORTHOGONAL_SMALL_COLUMNS and n * c < 2**29 and growth <= 2**22 and not many:
         return _orthogonalize_small(out, x, n, r, c, sr, sc, steps, coefficients, eps, scratch)
     sum_blocks = max(1, min(1024 if n == 1 else 256, _cdiv(r * c, 4096)))
     sums     = scratch((n, sum_blocks))
