@@ -134,9 +134,16 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
 #pragma unroll
             for (int j = 0; j < T; ++j)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const uint32_t row = lane_row + 32u * i + 8u * (k >> 2) + (k & 3), column = lane_column + 32u * j;
-                    if (row < P.M && column < P.N) out[each + row * P.sr + column * P.sc] = half_sum(acc, i, j, k) * down;
+                for (int k0 = 0; k0 < 16; k0 += 4) {
+                    // (four rows that are neighbours, in memory too where the matrix is tall)
+                    const uint32_t row = lane_row + 32u * i + 2u * k0, column = lane_column + 32u * j;
+                    float* const to = out + each + row * P.sr + column * P.sc;
+                    if (column >= P.N) continue;
+                    if (P.sr == 1u && row + 4u <= P.M)
+                        *reinterpret_cast<f32x4_anywhere*>(to) = f32x4{half_sum(acc, i, j, k0), half_sum(acc, i, j, k0 + 1), half_sum(acc, i, j, k0 + 2), half_sum(acc, i, j, k0 + 3)} * down;
+                    else
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; ++e) if (row + e < P.M) to[e * P.sr] = half_sum(acc, i, j, k0 + e) * down;
                 }
         return;
     }
