@@ -2824,7 +2824,9 @@ def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer
     tiles  = _cdiv(v, _linear_rows_tile(rows, not transposed))
     #few tiles: slices of the features, of four times the rows and 64 at least, that a block to a CU makes (4 x 4096 x 1000 81 -> 22 us, 4 x 4096 x 16000 85 -> 53, 64 x 2048 x 8000 80 -> 37, with a
     #launch more; two blocks to a CU 31, 55, 41)
-    slices = max(1, min(HALF_CUS // tiles, h // max(64, 4 * rows)))
+    #(tiles for half of the CUs and some: three slices, two blocks to most CUs: 6 x 2792 x 17351 63 -> 52 us, 6 x 4096 x 20000 89 -> 70; of 1024 features 30 and 29, of two slices 33)
+    blocks = HALF_CUS if tiles <= HALF_CUS // 2 or 3 * tiles > 2 * HALF_CUS or h < 2048 else 2 * HALF_CUS
+    slices = max(1, min(blocks // tiles, h // max(64, 4 * rows)))
     parts  = scratch((slices, rows, v)) if slices > 1 else None
     launches = [Launch(f'linear_scores_rows_{"h" if transposed else "v"}_{32 if rows <= 32 else 64}', (tiles * slices, 1, 1), (BLOCK, 1, 1),
                        [(b, 0) for b in ((None, None, None, parts) if slices > 1 else (*of_tiles, scores)) + (x, w, tokens)], _u32(rows, h, v, slices),
