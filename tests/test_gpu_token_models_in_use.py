@@ -195,6 +195,10 @@ def cases():
         yield f'loss {rows} x {h} x {v}', loss_program(transposed), list(w)
     yield 'orthogonal', lambda x: (nn.orthogonalize(x, 3),), [normal(7, 3, 200, 900)]
     yield 'orthogonal tall', lambda x: (nn.orthogonalize(x, 2),), [normal(8, 1500, 333)]
+    yield 'orthogonal of few rows', lambda x: (nn.orthogonalize(x),), [normal(9, 5, 50, 700)]
+    yield 'orthogonal of few columns', lambda x: (nn.orthogonalize(x),), [normal(10, 3, 2000, 21)]
+    yield 'conv of single steps', conv_program(None, 'silu', True, True), [normal(i, *s) for i, s in enumerate(((9, 1, 132), (4, 132), (9, 1, 132), (9, 3, 132), (132,), (9, 3, 132)))]
+    yield 'loss of many features', loss_program(True), list(loss_inputs(7, 2100, 17003, True))
 
 
 CASES = list(cases())
