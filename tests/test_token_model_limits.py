@@ -1,0 +1,19 @@
+'''Token models' operators at the ends of what they take: what is planned there, and what is refused (nothing is allocated).'''
+import numpy as np
+import pytest
+
+from tests.test_operator_plans import buffer, scratch
+from tests.test_token_model_plans import zeroed
+from vkjax_amd import kernels as K
+
+
+@pytest.mark.parametrize('steps,coefficients', [(32, (0.25, 0.0, 0.0)), (8, (0.0, 0.5, 0.0)), (2, (0.0, 0.0, 1e-20)), (2, (1e-30, 0.0, 0.0)), (3, (0.0, 0.0, 0.0)), (32, (3.4445, -4.7750, 2.0315))])
+def test_scales_of_polynomials_are_powers_that_fp32_has(steps, coefficients):
+    '''Polynomials under which singular values come to next to nothing: 2^scale and 2^-scale are factors on the device, of which it makes those from 2^-126 to 2^126.'''
+    x, seen = buffer(100, 100), 0
+    for launch in K.orthogonalize(x, x, steps, coefficients, 1e-7, scratch, zeroed):
+        words = np.frombuffer(launch.params, np.int32)
+        scales = words[7:10] if launch.kernel.startswith(('orthogonal_square_', 'orthogonal_poly', 'orthogonal_next', 'orthogonal_last')) else words[-1:] if launch.kernel == 'orthogonal_pack' else ()
+        assert all(-126 <= s <= 126 for s in scales), (launch.kernel, scales)
+        seen += len(scales)
+    assert seen == 1 + 9 * steps

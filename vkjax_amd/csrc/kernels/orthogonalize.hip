@@ -124,7 +124,10 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     if constexpr (SYMMETRIC) half_product<T, STAGES>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
     else half_product<T, STAGES, TURNED_B>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * (steps_k / 2u) * steps_n * 128u, blocks_n, steps_n, 0u}, m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
-    const float down = power_of_two(-P.scale_a) * power_of_two(-P.scale_b), up = power_of_two(P.scale_out);
+    // (both operands' scales at once: their factors' product may be below what fp32 has where a result is not)
+    const int down = -(P.scale_a + P.scale_b);
+    const float up = power_of_two(P.scale_out);
+    auto result = [&](int i, int j, int k) { return __builtin_amdgcn_ldexpf(half_sum(acc, i, j, k), down); };
     const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = row0 + (wave >> 1) * 32u * T + 4u * (lane >> 5), lane_column = column0 + (wave & 1u) * 32u * T + (lane & 31u);
     const uint64_t each = (uint64_t)matrix * P.M * P.N;
@@ -140,10 +143,10 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
                     float* const to = out + each + row * P.sr + column * P.sc;
                     if (column >= P.N) continue;
                     if (P.sr == 1u && row + 4u <= P.M)
-                        *reinterpret_cast<f32x4_anywhere*>(to) = f32x4{half_sum(acc, i, j, k0), half_sum(acc, i, j, k0 + 1), half_sum(acc, i, j, k0 + 2), half_sum(acc, i, j, k0 + 3)} * down;
+                        *reinterpret_cast<f32x4_anywhere*>(to) = f32x4{result(i, j, k0), result(i, j, k0 + 1), result(i, j, k0 + 2), result(i, j, k0 + 3)};
                     else
 #pragma unroll
-                        for (uint32_t e = 0; e < 4u; ++e) if (row + e < P.M) to[e * P.sr] = half_sum(acc, i, j, k0 + e) * down;
+                        for (uint32_t e = 0; e < 4u; ++e) if (row + e < P.M) to[e * P.sr] = result(i, j, k0 + e);
                 }
         return;
     }
@@ -165,7 +168,7 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     half_store<T>(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {
         row += row0; column += column0;
         if (row >= P.M || column >= P.N) return 0.f;
-        float v = half_sum(acc, i, j, k) * down;
+        float v = result(i, j, k);
         if constexpr (KIND == SQUARE) out[each + (uint64_t)row * P.N + column] = v;
         if constexpr (KIND == POLYNOMIAL) v = __builtin_fmaf(P.c, v, __builtin_fmaf(P.b, squares[i][j][k], row == column ? P.a : 0.f));
         return v * up;

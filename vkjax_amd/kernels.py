@@ -2775,6 +2775,7 @@ HALF_CUS = 256
 #1.1 in 4096 x 1024 x 8064)
 HALF_KERNELS = (('_128', 128, 2, 8.0, 0.90, 0.71), ('_64', 64, 2, 4.5, 0.38, 0.30), ('_64_many', 64, 4, 4.0, 0.47, 0.25))
 HALF_SLICE_PAIRS = 4                    #pairs of steps of a slice, at least
+HALF_MOST_SCALE  = 120                  #of an operand (half_scale in half_product.h)
 HALF_JOIN, HALF_JOIN_SLICE = 12.0, 0.6  #us of adding up slices of tiles of 128, and for each of them
 
 
@@ -3036,8 +3037,8 @@ def _orthogonalize_small(out: Buffer, x: Buffer, n: int, r: int, c: int, sr: int
 
 
 def _half_scale(largest: float) -> int:
-    '''The power of two that brings numbers up to `largest` below 2^15.'''
-    return 15 - int(math.frexp(largest)[1])
+    '''The power of two that brings numbers up to `largest` below 2^15, within what fp32 has both ways (half_product.h): numbers that a polynomial leaves beyond 2^-106 are scaled to less.'''
+    return min(15 - int(math.frexp(largest)[1]), HALF_MOST_SCALE)
 
 
 def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, scratch, zeroed) -> tp.List[Launch]:
