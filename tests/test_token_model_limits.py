@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests.test_operator_plans import buffer, scratch
-from tests.test_token_model_plans import zeroed
+from tests.test_token_model_plans import check, conv_launches, zeroed
 from vkjax_amd import kernels as K
 
 
@@ -17,3 +17,17 @@ def test_scales_of_polynomials_are_powers_that_fp32_has(steps, coefficients):
         assert all(-126 <= s <= 126 for s in scales), (launch.kernel, scales)
         seen += len(scales)
     assert seen == 1 + 9 * steps
+
+
+def test_gradients_of_convolutions_of_many_channels():
+    '''Sums over time go through a launch of 16 threads a channel and tap.'''
+    for t, c, k in ((4, 2**26, 4), (1, 2**26, 3), (1, 2**29 + 4, 8), (1, 2**28 // 9 + 1, 8)):
+        list(check(conv_launches(1, t, c, k, False)))
+        with pytest.raises(NotImplementedError):
+            list(check(conv_launches(1, t, c, k, True)))
+        #(without the kernel's and the bias' gradients there is no such launch)
+        x, w = buffer(1, t, c), buffer(k, c)
+        launch, = K.causal_conv_grad(x, None, None, None, x, w, None, None, None, x, None, None, scratch)
+        list(check([launch]))
+    for c, k in ((2**28 // 9 - 64, 8), (2**28 // 5 - 64, 4)):
+        list(check(conv_launches(1, 1, c, k, True)))

@@ -2611,6 +2611,9 @@ def causal_conv_grad(dx, dkernel, dbias, dstate, x: Buffer, kernel: Buffer, bias
     vec, steps, lanes, cstrips, tiles = _causal_conv_tiling(b, t, c)
     turns  = max(1, min(tiles, b * cstrips * tiles // CAUSAL_CONV_GRAD_BLOCKS))
     rows   = b * _cdiv(tiles, turns)
+    #(they are added up by 16 threads a column)
+    if (dkernel is not None or dbias is not None) and _cdiv((k + 1) * c, 64) * 1024 >= 2**32:
+        raise NotImplementedError(f'the gradient of a causal convolution of {c} channels by {k}')
     sums   = scratch((rows, k + 1, c)) if dkernel is not None or dbias is not None else None
     launch = Launch(f'causal_conv_grad_k{k}_v{vec}_l{steps}', _causal_conv_blocks(x, rows * cstrips), (BLOCK, 1, 1),
                     [(v, 0) for v in (dx, dstate, sums, x, kernel, bias, state, lengths, g, g_last)],
