@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests.test_operator_plans import buffer, scratch
-from tests.test_token_model_plans import check, conv_launches, zeroed
+from tests.test_token_model_plans import check, conv_launches, matrix_launches, zeroed
 from vkjax_amd import kernels as K
 
 
@@ -31,3 +31,13 @@ def test_gradients_of_convolutions_of_many_channels():
         list(check([launch]))
     for c, k in ((2**28 // 9 - 64, 8), (2**28 // 5 - 64, 4)):
         list(check(conv_launches(1, 1, c, k, True)))
+
+
+def test_matrices_of_few_rows_by_the_million():
+    '''A Gram matrix has a block of up to 1024 threads.'''
+    for shape in ((12_000_000, 20, 20), (6_000_000, 48, 48), (11_184_811, 17, 17), (6_000_000, 40, 48)):
+        for steps in (2, 5):
+            with pytest.raises(NotImplementedError):
+                list(check(matrix_launches(*shape, steps=steps)))
+    for shape in ((11_184_810, 17, 17), (16_000_000, 16, 16), (5_592_405, 48, 48), (2_000_000, 64, 256)):
+        assert 'orthogonal_small' in list(check(matrix_launches(*shape)))

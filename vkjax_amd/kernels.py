@@ -3028,12 +3028,15 @@ def _orthogonalize_small(out: Buffer, x: Buffer, n: int, r: int, c: int, sr: int
     each   = _cdiv(_cdiv(c, slices), 64) * 64
     slices = _cdiv(c, each)
     side   = _cdiv(r, 16)
-    sums, polynomials = scratch((n, slices, side * (side + 1) // 2, 4, 64, 2)), scratch((n, 16 * side, 16 * side))         #(the former fp64)
     rows   = max(16, _pow2_at_least(r))
     tasks  = _cdiv(c, 32) * _cdiv(rows, 32)
     blocks = _cdiv(tasks, 4)
+    waves  = min(16, side * (side + 1))
+    if n * max(64 * waves, slices * BLOCK, blocks * BLOCK) >= 2**32:
+        raise NotImplementedError(f'orthogonalising {n} matrices of {r} x {c}')
+    sums, polynomials = scratch((n, slices, side * (side + 1) // 2, 4, 64, 2)), scratch((n, 16 * side, 16 * side))         #(the former fp64)
     return [Launch('orthogonal_gram', (n * slices, 1, 1), (BLOCK, 1, 1), [(sums, 0), (x, 0)], _u32(r, c, slices, each) + _u64(sr, sc), bytes_moved=4 * x.size, flops=n * r * r * c),
-            Launch('orthogonal_small', (n, 1, 1), (64 * min(16, side * (side + 1)), 1, 1), [(polynomials, 0), (sums, 0)],
+            Launch('orthogonal_small', (n, 1, 1), (64 * waves, 1, 1), [(polynomials, 0), (sums, 0)],
                    _u32(r, slices, steps) + np.asarray([*coefficients, eps], np.float32).tobytes() + _u32(0), lds=3 * 8 * 16 * side * (16 * side + 2), bytes_moved=4 * sums.size),
             Launch(f'orthogonal_apply_{"wide" if sc == 1 else "tall"}_{rows}', (n * blocks, 1, 1), (BLOCK, 1, 1), [(out, 0), (x, 0), (polynomials, 0)],
                    _u32(r, c, tasks, blocks), bytes_moved=8 * x.size, flops=2 * n * r * r * c)]
