@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests.test_operator_plans import buffer, scratch
-from tests.test_token_model_plans import check, conv_launches, matrix_launches, zeroed
+from tests.test_token_model_plans import check, conv_launches, loss_launches, matrix_launches, zeroed
 from vkjax_amd import kernels as K
 
 
@@ -41,3 +41,13 @@ def test_matrices_of_few_rows_by_the_million():
                 list(check(matrix_launches(*shape, steps=steps)))
     for shape in ((11_184_810, 17, 17), (16_000_000, 16, 16), (5_592_405, 48, 48), (2_000_000, 64, 256)):
         assert 'orthogonal_small' in list(check(matrix_launches(*shape)))
+
+
+def test_log_probs_of_many_rows_of_few_features():
+    '''16 rows have a block of 1024 threads of the launch that joins their tiles.'''
+    for rows, h, v in ((2**26 - 15, 8, 100), (2**27 - 1, 4, 50)):
+        for gradient in (False, True):
+            with pytest.raises(NotImplementedError):
+                list(check(loss_launches(rows, h, v, False, gradient)))
+    for gradient in (False, True):
+        list(check(loss_launches(2**26 - 16, 8, 100, False, gradient)))

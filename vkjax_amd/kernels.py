@@ -2798,8 +2798,8 @@ class LinearShape(tp.NamedTuple):
 def _linear_shape(x: Buffer, w: Buffer, transposed: bool) -> LinearShape:
     h, v   = reversed(w.shape) if transposed else w.shape
     shape  = LinearShape(x.size // h, h, v)
-    #(indices of rows, tokens and steps are 32 bits, addresses 64)
-    if max(shape) >= 2**27 or shape.rows * h >= 2**31 or _cdiv(shape.rows, HALF_TILE) * _cdiv(v, HALF_TILE) >= 2**23:
+    #(indices of rows, tokens and steps are 32 bits, addresses 64; the launch that joins tiles has blocks of 1024 threads for 16 rows)
+    if max(shape) >= 2**27 or _cdiv(shape.rows, 16) >= 2**22 or shape.rows * h >= 2**31 or _cdiv(shape.rows, HALF_TILE) * _cdiv(v, HALF_TILE) >= 2**23:
         raise NotImplementedError(f'log probabilities of {shape.rows} rows of {h} over {v} tokens')
     return shape
 
