@@ -2756,6 +2756,8 @@ def half_plan(tiles_of, pairs: int) -> HalfPlan:
             whole = tiles if slices == 1 else tiles // slots * slots
             if slices > 1 and (slices * HALF_SLICE_PAIRS > pairs or whole == tiles):
                 continue
+            if (whole + (tiles - whole) * slices) * BLOCK >= 2**32:             #(a launch cannot have as many threads)
+                continue
             cost = time(whole, pairs)
             if whole < tiles:
                 cost += time((tiles - whole) * slices, _cdiv(pairs, slices)) + (HALF_JOIN + HALF_JOIN_SLICE * slices) * (side / 128)**2
