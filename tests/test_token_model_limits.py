@@ -3,8 +3,11 @@ import numpy as np
 import pytest
 
 from tests.test_operator_plans import buffer, scratch
+from tests.test_operators import normal, refused
 from tests.test_token_model_plans import check, conv_launches, loss_launches, matrix_launches, zeroed
-from vkjax_amd import kernels as K
+from vkjax_amd import kernels as K, minijax as mj
+
+jnp, lax = mj.numpy, mj.lax
 
 
 @pytest.mark.parametrize('steps,coefficients', [(32, (0.25, 0.0, 0.0)), (8, (0.0, 0.5, 0.0)), (2, (0.0, 0.0, 1e-20)), (2, (1e-30, 0.0, 0.0)), (3, (0.0, 0.0, 0.0)), (32, (3.4445, -4.7750, 2.0315))])
@@ -58,3 +61,11 @@ def test_log_probs_over_a_hundred_million_tokens():
     for rows, h, v in ((559, 54, 134200629), (832, 3, 132375801), (890, 8, 2**27 - 1)):
         for gradient in (False, True):
             assert any(name.endswith('_128') for name in check(loss_launches(rows, h, v, False, gradient)))
+
+
+def test_scores_that_are_kept_for_a_gradient_have_none():
+    '''Of few rows linear_log_probs keeps the scores, as float32: what a program makes of them has no part in its gradient, so that it is refused.'''
+    x, w, t = normal(1, 3, 8), normal(2, 8, 10), np.zeros(3, np.int32)
+    for at in range(2, 5):
+        refused(NotImplementedError, lambda x: mj.grad(lambda x: jnp.sum(lax.linear_log_probs(x, w, t, with_parts=True)[at]))(x), x)
+        refused(NotImplementedError, lambda x: mj.grad(lambda x: (lambda outs: jnp.sum(outs[0]) + jnp.sum(outs[at]))(lax.linear_log_probs(x, w, t, with_parts=True)))(x), x)

@@ -401,8 +401,8 @@ def _with_parts(eqn):
 
 @_rule('linear_log_probs')
 def _linear_log_probs(gs, x, weights, tokens, outs, transposed, parts):
-    if gs[2] is not None or gs[3] is not None:
-        raise NotImplementedError('differentiation through the largest scores and the sums of linear_log_probs')
+    if any(g is not None for g in gs[2:]):
+        raise NotImplementedError('differentiation through the largest scores, the sums and the parts of linear_log_probs')
     return lax.linear_log_probs_grad(x, weights, tokens, outs[2], outs[3], _or_none(gs[0], outs[0]), _or_none(gs[1], outs[1]), transposed,
                                      tuple(outs[4:]) if parts else None) + (None,)
 
