@@ -69,3 +69,36 @@ def test_scores_that_are_kept_for_a_gradient_have_none():
     for at in range(2, 5):
         refused(NotImplementedError, lambda x: mj.grad(lambda x: jnp.sum(lax.linear_log_probs(x, w, t, with_parts=True)[at]))(x), x)
         refused(NotImplementedError, lambda x: mj.grad(lambda x: (lambda outs: jnp.sum(outs[0]) + jnp.sum(outs[at]))(lax.linear_log_probs(x, w, t, with_parts=True)))(x), x)
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('rows,h,v', [(4096, 1024, 32000), (20000, 64, 130001), (2**20, 64, 5000), (2000, 300, 200000), (70000, 2000, 1100)])
+def test_a_gradient_of_log_probs_holds_no_scores(rows, h, v, transposed):
+    '''Array by array: a piece of the scores' cotangents, slices of dx, x as an operand, sums of shared contractions. All scores would be more than a piece.'''
+    assert 4 * rows * v > K.LINEAR_PIECE
+    x, w, t, r = buffer(rows, h), buffer(*((v, h) if transposed else (h, v))), buffer(rows, dtype=np.int32), buffer(rows)
+    parts = [buffer(n, dtype=d) for n, d in K.linear_parts(x.shape, w.shape, transposed)]
+    taken = []
+
+    def noting(shape, dtype=np.float32):
+        taken.append(scratch(shape, dtype))
+        return taken[-1]
+    dx, dw = buffer(*x.shape), buffer(*w.shape)
+    launches = K.linear_log_probs_grad(dx, dw, x, w, t, r, r, r, r, transposed, noting, zeroed, parts)
+    of = lambda name, at: {id(l.buffers[at][0]): l.buffers[at][0] for l in launches if l.kernel.startswith(name) and l.buffers[at][0] is not None}
+    size = lambda b: 4 * b.size
+    q, = of('linear_q', 0).values()
+    blocks = -(-rows // 32) * 32
+    tile = 4 * K.HALF_TILE * blocks
+    assert size(q) <= max(K.LINEAR_PIECE, tile)
+    sums = {k: b for k, b in of('linear_product', 0).items() if b is not dx and b is not dw}
+    tiles_x = -(-rows // K.HALF_TILE) * -(-h // K.HALF_TILE)
+    assert all(size(b) <= 2 * K.HALF_CUS // tiles_x * 4 * rows * h for b in sums.values()) and len(sums) <= 1
+    operands = {**of('linear_pack', 0), **of('linear_pack', 1), **of('linear_pack', 2)}
+    assert all(size(b) <= 4 * blocks * (-(-h // 32) * 32) for b in operands.values())
+    #(sums of shared contractions: at most a round of the machine's tiles in 64 slices)
+    shared = {**of('linear_product', 1), **of('linear_q', 1)}
+    assert all(size(b) <= 64 * 2**20 for b in shared.values())
+    named = {id(q), *sums, *operands, *shared}
+    assert all(size(b) <= 2**20 + 12 * rows for b in taken if id(b) not in named)
+    assert all(size(b) < 4 * rows * v for b in taken if id(b) not in {*sums, *operands})
