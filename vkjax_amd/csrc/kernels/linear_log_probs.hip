@@ -289,7 +289,7 @@ template <bool ALONG_M, int NT> struct RowsProduct {
     static __device__ __forceinline__ uint32_t lane() { return threadIdx.x & 63u; }
     static __device__ __forceinline__ f32x4 load(const float* at) { return *reinterpret_cast<const f32x4_anywhere*>(at); }
     // over the k of groups [all_begin, all_end); `there`: rows that are padding are zeros, whatever b holds. M and K are 4 at least: vectors that would end behind the last m or k are moved to
-    // the left, and of b the k's that come twice by that are zeros. (So nothing is loaded behind a branch: with one the loads of a last group waited for one another, 25 us of a block's 84 at
+    // the left, and the k's that come twice by that are zeros, of b and of A (whose infinities would be NaN otherwise). (So nothing is loaded behind a branch: with one the loads of a last group waited for one another, 25 us of a block's 84 at
     // 15 x 1973 x 128040.)
     __device__ __forceinline__ void multiply(Shared& shared, const float* __restrict__ a, const float* __restrict__ b, uint32_t m0, uint32_t M, uint32_t K, const uint32_t (&r_at)[NT],
                                              const bool (&there)[NT], uint32_t all_begin, uint32_t all_end) {
@@ -300,9 +300,10 @@ template <bool ALONG_M, int NT> struct RowsProduct {
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
         auto of_row = [&](int j, uint32_t k) { return load(b + (uint64_t)r_at[j] * K + min(k, K - 4u)); };
+        auto is_own = [&](uint32_t k, uint32_t e) { return min(k, K - 4u) + e >= k; };
         auto own = [&](f32x4 v, int j, uint32_t k) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4u; ++e) v[e] = there[j] && min(k, K - 4u) + e >= k ? v[e] : 0.f;
+            for (uint32_t e = 0; e < 4u; ++e) v[e] = there[j] && is_own(k, e) ? v[e] : 0.f;
             return v;
         };
         if constexpr (ALONG_M) {
@@ -343,7 +344,11 @@ template <bool ALONG_M, int NT> struct RowsProduct {
 #pragma unroll
                 for (uint32_t k = 0; k < DEPTH; ++k) {
                     if (g + k + DEPTH - 1u < end) request(as[(k + DEPTH - 1u) % DEPTH], bs[(k + DEPTH - 1u) % DEPTH], g + k + DEPTH - 1u);
-                    if (g + k < end) products(as[k], bs[k], g + k);
+                    if (g + k >= end) continue;
+                    if ((g + k + 1u) * 8u > K)
+#pragma unroll
+                        for (uint32_t q = 0; q < 4u; ++q) if (!is_own((g + k) * 8u + 4u * half, q)) as[k][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    products(as[k], bs[k], g + k);
                 }
         } else {
             f32x4 (&turned)[MB][32][8] = shared.turned[wave];
@@ -370,6 +375,13 @@ template <bool ALONG_M, int NT> struct RowsProduct {
             for (uint32_t g = begin; g < end; ++g) {
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
+                if ((g + 1u) * 32u > K)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (uint32_t e = 0; e < 4u; ++e) next[i][t][e] = is_own(g * 32u + 4u * column, e) ? next[i][t][e] : 0.f;
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
