@@ -1087,7 +1087,8 @@ def linear_log_probs_grad(x, weights, tokens, peaks, totals, *cotangents, transp
         d[np.arange(len(s)), token] += of_token
         d[~given] = 0.0
         dw = rows.T @ d
-        return (d @ w.T).reshape(x.shape).astype(f32), (dw.T if transposed else dw).astype(f32)
+        dx = np.where(given[:, None], d @ w.T, 0.0)                 #(padding has none, whatever the weights are)
+        return dx.reshape(x.shape).astype(f32), (dw.T if transposed else dw).astype(f32)
 
 
 def orthogonalize(x, steps, coefficients, eps):

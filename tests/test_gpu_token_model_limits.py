@@ -2,14 +2,17 @@
 import numpy as np
 import pytest
 
-from tests.test_gpu_operators import both, close
+import tests.test_gpu_token_model_operators as operators
+from tests.test_gpu_operators import U, both, close
 from tests.test_gpu_token_model_operators import loss_bounds, loss_inputs, orthogonal_bound
 from tests.test_operators import normal
 from tests.test_token_model_operators import loss_program
-from vkjax_amd import minijax as mj
+from vkjax_amd import kernels as K, minijax as mj
+from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
 pytestmark = pytest.mark.gpu
-nn = mj.nn
+lax, nn = mj.lax, mj.nn
+f32 = np.float32
 
 
 @pytest.mark.parametrize('steps,coefficients', [(32, (0.25, 0.0, 0.0)), (2, (0.0, 0.5, 0.0)), (2, (1e-12, 0.0, 0.0)), (1, (0.0, 0.0, 1e-20)), (5, (0.01, -0.01, 0.005))], ids=str)
@@ -63,3 +66,141 @@ def test_tokens_masked_by_infinite_weights_of_the_last_features(rows, hidden, tr
     '''Contractions that end inside a step of theirs, whose last vectors are read from further in front.'''
     for feature in (-1, -2, -4):
         check_masked(rows, hidden, 301, transposed, -np.inf, hidden + feature, [300, 299, 150, 0])
+
+
+@pytest.fixture
+def fp32_products(monkeypatch):
+    '''Bounds of products of more than 64 rows where their operands are too far apart for the fp16 matrix cores: one sum after the other, rounded for every term, at most twice where it is put
+    together from slices.'''
+    monkeypatch.setattr(operators, 'product_error', lambda a, b, terms: (terms + 70) * U * (a @ b))
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('mask', [-np.inf, -1e30, -3.4e38, -1e9])
+@pytest.mark.parametrize('rows,hidden,vocabulary', [(65, 41, 301), (70, 3, 200), (150, 131, 1300), (300, 64, 2049), (20, 2, 30)])
+def test_tokens_masked_by_weights_of_any_size(rows, hidden, vocabulary, mask, transposed, fp32_products):
+    for feature in (0, hidden - 1):
+        check_masked(rows, hidden, vocabulary, transposed, mask, feature, [0, 7, vocabulary - 1, vocabulary - 2])
+
+
+@pytest.mark.parametrize('slices', [1, 3])
+@pytest.mark.parametrize('kernel,side', [(k[0], k[1]) for k in K.HALF_KERNELS])
+def test_tokens_masked_in_every_kernel_of_a_product(kernel, side, slices, monkeypatch, fp32_products):
+    monkeypatch.setattr(K, 'half_plan', lambda tiles_of, pairs: K.HalfPlan(kernel, side, 3 if slices > 1 else tiles_of(side), min(slices, pairs)))
+    for transposed in (False, True):
+        check_masked(700, 300, 1500, transposed, -1e30, 17, [0, 129, 1499])
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+def test_tokens_masked_in_pieces_of_the_vocabulary(transposed, monkeypatch, fp32_products):
+    monkeypatch.setattr(K, 'LINEAR_PIECE', 1)
+    for rows, hidden, vocabulary in ((140, 70, 600), (520, 33, 300)):
+        check_masked(rows, hidden, vocabulary, transposed, -np.inf, 5, [0, 200, vocabulary - 1])
+
+
+def without_parts(transposed):
+    def f(x, w, tokens, g, gs):
+        outs = lax.linear_log_probs(x, w, tokens, transposed)
+        return outs[:2] + lax.linear_log_probs_grad(x, w, tokens, outs[2], outs[3], g, gs, transposed)
+    return f
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+def test_tokens_masked_where_nothing_was_kept(transposed, fp32_products):
+    check_masked(150, 70, 600, transposed, -1e30, 5, [0, 200, 599], without_parts)
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('size', [1e12, 1e20, 1e30])
+@pytest.mark.parametrize('rows', [30, 90, 400])
+def test_rows_beside_one_that_is_much_larger(rows, size, transposed, fp32_products):
+    '''The other rows are as exact as without it. Its own probabilities are 1 and 0 (scores lie apart by far more than they are off by), so that it adds to two tokens' weights alone.'''
+    x, w, tokens, g, gs = loss_inputs(rows, 70, 500, transposed)
+    tokens[:6] = np.arange(6)
+    x[5] *= f32(size)
+    got, expected, _ = both(loss_program(transposed), x, w, tokens, g, gs)
+    w64 = (w.T if transposed else w).astype(np.float64)
+    scores, others = x[5].astype(np.float64) @ w64, np.arange(rows) != 5
+    top = scores.argmax()
+    rounding = 140 * U * np.abs(x[5].astype(np.float64)) @ np.abs(w64)
+    assert top != tokens[5] and np.diff(np.sort(scores))[-1] > 1e3 * rounding.max()
+    bounds = loss_bounds(x, w, np.where(others, tokens, -1), g, gs, transposed)
+    for name, a, b, bound in zip(('log_probs', 'log_sums', 'dx'), got, expected, bounds):
+        close(a[others], b[others], bound[others], name)
+    close(got[0][5], expected[0][5], rounding[5] + rounding[top])
+    close(got[1][5], expected[1][5], rounding[top])
+    ds = {tokens[5]: abs(float(g[5])), top: abs(float(gs[5]) - float(g[5]))}
+    close(got[2][5], expected[2][5], 8 * U * sum(d * np.abs(w64[:, v]) for v, d in ds.items()))
+    own = np.zeros((500, 70))
+    for v, d in ds.items():
+        own[v] = 8 * U * d * np.abs(x[5].astype(np.float64))
+    close(got[3], expected[3], bounds[3] + (own if transposed else own.T), 'dweights')
+
+
+def test_cotangents_of_rows_that_are_much_larger(fp32_products):
+    #a row's own factor: the gradient of another row is what it is without it
+    x, w, tokens, g, gs = loss_inputs(90, 70, 500, False)
+    tokens[:6] = np.arange(6)
+    x[4] *= f32(1e15)
+    g[5], gs[5] = f32(1e15), f32(-1e12)
+    got, expected, _ = both(loss_program(False), x, w, tokens, g, gs)
+    for name, a, b, bound in zip(('log_probs', 'log_sums', 'dx', 'dweights'), got, expected, loss_bounds(x, w, tokens, g, gs, False)):
+        close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('power', [9, 10, 11])
+def test_scores_where_products_change(power, monkeypatch):
+    '''Largest numbers whose products with one another and with the number of features are at 2^26: either kind of product, whose bounds are added up.'''
+    one = operators.product_error
+    monkeypatch.setattr(operators, 'product_error', lambda a, b, terms: one(a, b, terms) + (terms + 70) * U * (a @ b))
+    x, w, tokens, g, gs = loss_inputs(100, 64, 400, False)
+    tokens[tokens == 9] = 8
+    x[:, 3], w[3] = 2.0 ** 10, 0.0
+    w[3, 9] = -2.0 ** power
+    got, expected, _ = both(loss_program(False), x, w, tokens, g, gs)
+    bounds = loss_bounds(x, w, tokens, g, gs, False)
+    for name, a, b, bound in zip(('log_probs', 'log_sums', 'dx', 'dweights'), got, expected, bounds):
+        close(a, b, bound, name)
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('graph', [False, True])
+def test_one_program_for_numbers_near_and_far(graph, transposed):
+    near = loss_inputs(150, 70, 600, transposed)
+    far = [v.copy() for v in near]
+    far[0][3] *= f32(1e25)
+    infinite = [v.copy() for v in near]
+    infinite[1][(8, 4) if transposed else (4, 8)] = np.inf
+    program = JaxprInterpreter(mj.make_jaxpr(loss_program(transposed))(*near), graph=graph)
+    alone = [JaxprInterpreter(mj.make_jaxpr(loss_program(transposed))(*v)).run(*v) for v in (near, far, infinite)]
+    assert np.isfinite(alone[0][3]).all() and not np.array_equal(alone[0][0], alone[1][0])
+    for which in (0, 1, 0, 2, 2, 0, 1, 1, 0):
+        values = (near, far, infinite)[which]
+        if graph:
+            program.upload_inputs(*values)
+            program.replay(2)
+            got = program.read_outputs()
+        else:
+            got = program.run(*values)
+        for a, b in zip(got, alone[which]):
+            assert np.array_equal(np.asarray(a).reshape(b.shape), b, equal_nan=True)
+
+
+@pytest.mark.parametrize('transposed', [False, True])
+@pytest.mark.parametrize('rows', [9, 40, 64, 65, 200])
+def test_infinite_weights_are_those_of_fp32_arithmetic(rows, transposed):
+    '''A score is infinite, and its probability 0, 1 or NaN, whatever the number of rows.'''
+    x, w, tokens, g, gs = loss_inputs(rows, 41, 300, transposed)
+    tokens[:] = np.arange(rows) % 7
+    x[::3, 7], x[1::3, 7], x[2::3, 7] = 1.0, -1.0, 0.0
+    for value in (np.inf, -np.inf):
+        w[(9, 7) if transposed else (7, 9)] = value
+        got, expected, _ = both(loss_program(transposed), x, w, tokens, g, gs)
+        fine = np.sign(x[:, 7]) == -np.sign(value)
+        assert np.array_equal(np.isfinite(expected[0]), fine)
+        for name, a, b in zip(('log_probs', 'log_sums', 'dx'), got, expected):
+            assert np.array_equal(np.isfinite(a), np.isfinite(b)), name
+        (w if transposed else w.T)[9, 7] = 0
+        bounds = loss_bounds(np.where(np.arange(41) == 7, 0, x).astype(f32), np.delete(w, 9, 0 if transposed else 1), tokens, g, gs, transposed)
+        for a, b, bound in zip(got[:2], expected, bounds):
+            close(a[fine], b[fine], bound[fine] + 41 * U * np.abs(b[fine]))

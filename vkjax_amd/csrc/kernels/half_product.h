@@ -13,6 +13,11 @@
 // 8 i + 4 h + j), so a result becomes an operand that is contracted over its rows without leaving its lanes. Rows and k beyond the end are zeros; k comes in pairs of steps.
 // The same operand also serves products that are contracted over its rows (TURNED): 32 rows are a pair of steps then, 16 k are half of a block, and the lanes get theirs by reads of shared
 // memory that transpose 4 rows x 16 columns (ds_read_b64_tr_b16: of 16 lanes, lane 4 a + b asks for 4 numbers of row a, and lane r is given column r of the four rows).
+//
+// PLAIN operands are for numbers that are too far apart for a scale, and for infinities and NaN: in the same places lie the upper and the lower halves of the numbers' own 32 bits. The same tiles, reads
+// and epilogues serve them; a step puts the halves together again and multiplies by v_mfma_f32_32x32x2_f32 (element e of both operands' lanes: two k), whose sums are `large`.
+// Log probabilities of 4096 x 1024 x 32000 with their gradient take 9400 us so, 3400 taken apart; 128 x 1024 x 32000 forward 175 and 108. (That a launch can do either costs it 1 to 2 us where it takes 70
+// to 90, and nothing that can be measured where it takes 400.)
 #pragma once
 #include "common.h"
 
@@ -29,6 +34,11 @@ __device__ __forceinline__ void half_parts(float a, float b, uint32_t& hi, uint3
     const f32x2 w = __builtin_convertvector(h, f32x2);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{(a - w.x) * HALF_REST, (b - w.y) * HALF_REST}), f16x2));
+}
+// ... and their own bits' halves, of a plain operand
+__device__ __forceinline__ void plain_parts(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = f2u(a) >> 16 | (f2u(b) & 0xFFFF0000u);
+    lo = (f2u(a) & 0xFFFFu) | f2u(b) << 16;
 }
 // The power of two that an operand with this largest magnitude is scaled by (within what fp32 has both ways: an operand that has nothing beyond 2^-106 is scaled to less)
 __device__ __forceinline__ int half_scale(float largest) {
@@ -110,7 +120,21 @@ template <int T, HalfTurned TURNED> struct HalfStep {
                 b[i][t] = TURNED == TURNED_B ? turned(from[1][T * wn + i], s, t) : __builtin_bit_cast(f16x8, from[1][T * wn + i][s][t][lane]);
             }
     }
-    __device__ __forceinline__ void multiply(HalfSums<T>& sums) const {
+    // number e of a lane's eight of a plain operand
+    __device__ __forceinline__ static float plain(const f16x8 (&parts)[2], int e) {
+        const uint32_t hi = __builtin_bit_cast(u32x4, parts[0])[e >> 1], lo = __builtin_bit_cast(u32x4, parts[1])[e >> 1];
+        return u2f(e & 1 ? (hi & 0xFFFF0000u) | lo >> 16 : hi << 16 | (lo & 0xFFFFu));
+    }
+    template <bool PLAIN> __device__ __forceinline__ void multiply(HalfSums<T>& sums) const {
+        if constexpr (PLAIN) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 0; i < T; ++i)
+#pragma unroll
+                    for (int j = 0; j < T; ++j) sums.large[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(plain(a[i], e), plain(b[j], e), sums.large[i][j], 0, 0, 0);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < T; ++i)
 #pragma unroll
@@ -126,10 +150,13 @@ template <int N> __device__ __forceinline__ void loads_left() { __builtin_amdgcn
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); asm volatile("" ::: "memory"); }
 #define HALF_FENCE() __builtin_amdgcn_sched_barrier(0)
 
+template <bool B> struct HalfPlain { static constexpr bool value = B; };
 // The sums of tile (m, n) over `pairs` pairs of steps from pair `begin` on. With more than two buffers a wave has the parts of the next step in registers before it
 // multiplies those of this one: the barrier in front of a pair stands between the two steps of the pair before.
-template <int T, int STAGES, HalfTurned TURNED = TURNED_NONE>
-__device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs) {
+// EITHER: operands that are plain where *plain says so, which is read while the first pairs are on their way.
+template <int T, int STAGES, HalfTurned TURNED = TURNED_NONE, bool EITHER = false>
+__device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, STAGES>& shared, const HalfOperand& a, const HalfOperand& b, uint32_t m, uint32_t n, uint32_t begin, uint32_t pairs,
+                                             const int32_t* plain = nullptr) {
     static_assert(STAGES == 2 || STAGES == 4, "as many pairs are on their way as meet() counts");
     constexpr int LOADS = 4 * T;                         // of a wave per stage
     if (pairs == 0u) return;                             // (a slice of nothing)
@@ -146,41 +173,47 @@ __device__ __forceinline__ void half_product(HalfSums<T>& sums, HalfShared<T, ST
 #pragma unroll
     for (uint32_t p = 0; p < STAGES - 1; ++p)
         if (p < pairs) request(p);
-    uint32_t at = 0u;
-    if constexpr (STAGES == 2) {
-        for (uint32_t p = 0; p < pairs; ++p) {
-            meet(p);
-            if (asked < pairs) request(at ^ 1u);
-            HalfStep<T, TURNED> step;
-            step.read(shared.stages[at], 0);
-            step.multiply(sums);
-            step.read(shared.stages[at], 1);
-            step.multiply(sums);
-            at ^= 1u;
-        }
-    } else {
-        HalfStep<T, TURNED> first, second;
-        meet(0u);
-        if (asked < pairs) request(STAGES - 1u);
-        first.read(shared.stages[0], 0);
-        for (uint32_t p = 0; p < pairs; ++p) {
-            second.read(shared.stages[at], 1);
-            HALF_FENCE();
-            first.multiply(sums);
-            HALF_FENCE();
-            const uint32_t next = at + 1u == STAGES ? 0u : at + 1u;
-            if (p + 1u < pairs) {
-                meet(p + 1u);
-                // (in the place of pair p - 1; reads of pair p may still be on their way)
-                if (p > 0u && asked < pairs) request(at == 0u ? STAGES - 1u : at - 1u);
-                first.read(shared.stages[next], 0);
+    auto multiply = [&](auto kind) {
+        constexpr bool PLAIN = decltype(kind)::value;
+        uint32_t at = 0u;
+        if constexpr (STAGES == 2) {
+            for (uint32_t p = 0; p < pairs; ++p) {
+                meet(p);
+                if (asked < pairs) request(at ^ 1u);
+                HalfStep<T, TURNED> step;
+                step.read(shared.stages[at], 0);
+                step.template multiply<PLAIN>(sums);
+                step.read(shared.stages[at], 1);
+                step.template multiply<PLAIN>(sums);
+                at ^= 1u;
             }
-            HALF_FENCE();
-            second.multiply(sums);
-            HALF_FENCE();
-            at = next;
+        } else {
+            HalfStep<T, TURNED> first, second;
+            meet(0u);
+            if (asked < pairs) request(STAGES - 1u);
+            first.read(shared.stages[0], 0);
+            for (uint32_t p = 0; p < pairs; ++p) {
+                second.read(shared.stages[at], 1);
+                HALF_FENCE();
+                first.template multiply<PLAIN>(sums);
+                HALF_FENCE();
+                const uint32_t next = at + 1u == STAGES ? 0u : at + 1u;
+                if (p + 1u < pairs) {
+                    meet(p + 1u);
+                    // (in the place of pair p - 1; reads of pair p may still be on their way)
+                    if (p > 0u && asked < pairs) request(at == 0u ? STAGES - 1u : at - 1u);
+                    first.read(shared.stages[next], 0);
+                }
+                HALF_FENCE();
+                second.template multiply<PLAIN>(sums);
+                HALF_FENCE();
+                at = next;
+            }
         }
-    }
+    };
+    // (the branch is the whole launch's)
+    if constexpr (EITHER) { if (__builtin_amdgcn_readfirstlane(*plain)) multiply(HalfPlain<true>{}); else multiply(HalfPlain<false>{}); }
+    else multiply(HalfPlain<false>{});
     __syncthreads();
 }
 
@@ -265,10 +298,10 @@ __device__ __forceinline__ void half_tile(uint32_t id, uint32_t tiles_m, uint32_
 }
 
 // ---- a tile of a result as an operand of products that follow: contracted over its rows, as the lanes have it (`by_column`: its index is the column), or over its columns (`by_row`),
-// turned in shared memory. value(block of rows i, of columns j, register, row, column) is what is taken apart, scaled; it is zero behind the result's last row and column.
+// turned in shared memory. value(block of rows i, of columns j, register, row, column) is what is taken apart, scaled (PLAIN: as it is); it is zero behind the result's last row and column.
 struct HalfTarget { u32x4* parts; uint32_t blocks, steps, block, step; };      // blocks of 32 of its index, steps of 16 k per block (all of them); where this tile's begin
 
-template <int T, class F>
+template <int T, bool PLAIN = false, class F>
 __device__ __forceinline__ void half_store(typename HalfTileOf<T>::Turned& turned, const HalfTarget& by_column, const HalfTarget& by_row, F value) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
 #pragma unroll
@@ -281,7 +314,8 @@ __device__ __forceinline__ void half_store(typename HalfTileOf<T>::Turned& turne
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t row = row0 + 8u * (k >> 1) + 2u * (k & 1);
-                half_parts(value(i, j, 2 * k, row, column), value(i, j, 2 * k + 1, row + 1u, column), hi[k], lo[k]);
+                const float one = value(i, j, 2 * k, row, column), two = value(i, j, 2 * k + 1, row + 1u, column);
+                if constexpr (PLAIN) plain_parts(one, two, hi[k], lo[k]); else half_parts(one, two, hi[k], lo[k]);
             }
             if (by_column.parts && block < by_column.blocks)
 #pragma unroll

@@ -4,7 +4,7 @@
 //   ds = g_lp [v = token] + (g_ls - g_lp) p,  p = exp(s - peak) / total;  dx = ds W^T,  dW = x^T ds
 // A row whose token lies outside the vocabulary is padding: zeros, x is not looked at there, no gradient.
 //
-// Products are those of half_product.h: x and W are taken apart first (the largest magnitudes, for their scales, then the parts), then
+// Products are those of half_product.h: x and W are taken apart first (the largest magnitudes, for their scales, then the parts; numbers that are too far apart for that stay as they are), then
 //   * forward: a product whose rows are the vocabulary and whose columns are the rows of x, so that a lane has 32 scores of one row; a tile of 128 tokens leaves each row's peak and
 //     sum, a last launch joins the tiles. 4096 x 1024 x 32000: the product as fast as one that keeps its scores, and nothing of 0.5 GB is written.
 //   * backward, in pieces of the vocabulary: the same product again, whose lanes turn scores into q = ds / m, |q| <= 2, with m = max(|g_lp|, |g_ls - g_lp|) of the row, and store q as an operand
@@ -24,8 +24,8 @@ __device__ __forceinline__ float scaled(float v, int e) { return __builtin_amdgc
 __device__ __forceinline__ bool is_token(int32_t t, uint32_t V) { return (uint32_t)t < V; }
 typedef f32x4 f32x4_anywhere __attribute__((aligned(4)));
 
-// A finite number's magnitude (others have no part in a scale)
-__device__ __forceinline__ float magnitude(float v) { const float a = __builtin_fabsf(v); return a < __builtin_inff() ? a : 0.f; }
+// (NaN counts as infinite)
+__device__ __forceinline__ float magnitude(float v) { const float a = __builtin_fabsf(v); return a < __builtin_inff() ? a : __builtin_inff(); }
 __device__ __forceinline__ float wave_largest(float v) {
     wave_butterfly([&](auto s) { v = fmaxf(v, lane_xor<decltype(s)::value>(v)); });
     return v;
@@ -73,7 +73,8 @@ extern "C" __global__ __launch_bounds__(256) void linear_largest(float* __restri
                 }
                 for (uint32_t e = 0; e < 4u; ++e) if (h + e < P.H) row = fmaxf(row, magnitude(from[h + e]));
             }
-            one = fmaxf(one, row); two = fmaxf(two, magnitude(row * m));
+            const float scaled_row = row * m;
+            one = fmaxf(one, row); two = fmaxf(two, scaled_row < __builtin_inff() ? scaled_row : 0.f);           // (what is not finite has no part in a scale)
         }
     one = wave_largest(one); two = wave_largest(two);
     if (lane == 0u) { part[0][wave] = one; part[1][wave] = two; }
@@ -85,28 +86,44 @@ extern "C" __global__ __launch_bounds__(256) void linear_largest(float* __restri
     else { const uint32_t at = P.weight_blocks + 2u * (blockIdx.x - P.weight_blocks); largest[at] = one; largest[at + 1u] = two; }
 }
 
-// ---- operands taken apart (half_product.h). What element (i, k) of an operand is: W or x as they lie, x only of rows that are given, or with the rows' factors.
+// ---- operands taken apart (half_product.h), or plain ones. A taken-apart number is off by 2^-51 of its operand's largest (or 2^-22 of itself), so a score by up to 2^-50 H times the largest
+// magnitudes of x and W: where that is above 2^-24, half a step of a number between 1 and 2, or a number is not finite, the operands are plain, and with them x and q of the gradient. A row of x that is
+// 10^20 times as large as the others, or a token that is masked by a weight of -10^30, leaves the other rows and tokens what they are by themselves.
+// `scales`: of the kinds of operands, and whether they are plain. (`given`: the scales of the forward pass, where its operands are taken as they are.)
+constexpr int PLAIN = 3;
+__device__ __forceinline__ bool too_far_apart(float largest_w, float largest_x, uint32_t H) { return !(largest_w * largest_x * (float)H <= 0x1p26f); }
+
+// What element (i, k) of an operand is: W or x as they lie, x only of rows that are given, or with the rows' factors.
 enum PackKind : uint32_t { PACK_WEIGHTS = 0, PACK_ROWS = 1, PACK_SCALED = 2 };
 struct PackJob { uint32_t blocks, I, K, stride, kind, steps; uint64_t si, sk; };      // blocks of 256 threads; steps of 16 k; element strides of i and k; `stride`: steps that a wave takes
-struct PackParams { uint32_t weight_blocks, row_blocks, V, pad; PackJob jobs[3]; };
+struct PackParams { uint32_t weight_blocks, row_blocks, V, H; PackJob jobs[3]; };
 struct PackOuts { void* parts[3]; };
 extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int32_t* __restrict__ scales, const float* __restrict__ x, const float* __restrict__ w,
-                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors, PackParams P) {
-    __shared__ float part[4];
+                                                              const int32_t* __restrict__ tokens, const float* __restrict__ largest, const float* __restrict__ factors,
+                                                              const int32_t* __restrict__ given, PackParams P) {
+    __shared__ float part[3][4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t block = blockIdx.x, job = 0u;
     while (job < 2u && block >= P.jobs[job].blocks) block -= P.jobs[job++].blocks;
     const PackJob J = P.jobs[job];
-    // the operand's scale, of its blocks' largest magnitudes
+    // the operands' scales, of their blocks' largest magnitudes
     const bool weights = J.kind == PACK_WEIGHTS;
-    float most = 0.f;
-    for (uint32_t k = threadIdx.x; k < (weights ? P.weight_blocks : P.row_blocks); k += 256u)
-        most = fmaxf(most, weights ? largest[k] : largest[P.weight_blocks + 2u * k + (J.kind == PACK_SCALED ? 1u : 0u)]);
-    most = wave_largest(most);
-    if (lane == 0u) part[wave] = most;
+    float most[3] = {};
+    for (uint32_t k = threadIdx.x; k < P.weight_blocks; k += 256u) most[0] = fmaxf(most[0], largest[k]);
+    for (uint32_t k = threadIdx.x; k < P.row_blocks; k += 256u)
+#pragma unroll
+        for (uint32_t kind = 1; kind < 3u; ++kind) most[kind] = fmaxf(most[kind], largest[P.weight_blocks + 2u * k + kind - 1u]);
+#pragma unroll
+    for (int kind = 0; kind < 3; ++kind) {
+        most[kind] = wave_largest(most[kind]);
+        if (lane == 0u) part[kind][wave] = most[kind];
+    }
     __syncthreads();
-    const int e = half_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-    if (block == 0u && threadIdx.x == 0u) scales[J.kind] = e;
+#pragma unroll
+    for (int kind = 0; kind < 3; ++kind) most[kind] = fmaxf(fmaxf(part[kind][0], part[kind][1]), fmaxf(part[kind][2], part[kind][3]));
+    const bool plain = given ? given[PLAIN] != 0 : too_far_apart(most[PACK_WEIGHTS], most[PACK_ROWS], P.H);
+    const int e = plain ? 0 : half_scale(weights ? most[PACK_WEIGHTS] : J.kind == PACK_ROWS ? most[PACK_ROWS] : most[PACK_SCALED]);
+    if (block == 0u && threadIdx.x == 0u) { scales[J.kind] = e; if (job == 0u) scales[PLAIN] = plain; }
     const float up = power_of_two(e);
     // waves beside one another along the side that is contiguous in memory
     const uint32_t groups = (J.steps + J.stride - 1u) / J.stride, all = block * 4u + wave, rows32 = (J.I + 31u) / 32u;
@@ -144,11 +161,15 @@ extern "C" __global__ __launch_bounds__(256) void linear_pack(PackOuts outs, int
                 for (int q = 0; q < 8; ++q) {
                     const uint32_t k = (s0 + t) * 16u + h4 + 8u * (q >> 2) + (q & 3);
                     const float m = k < J.K ? factors[3u * k] : 0.f;
-                    v[t][q] = m == 0.f ? 0.f : v[t][q] * m;           // (a row without a cotangent has none, whatever its x is)
+                    v[t][q] = m == 0.f ? 0.f : plain ? v[t][q] : v[t][q] * m;           // (a row without a cotangent has none, whatever its x is)
                 }
             u32x4 hi, lo;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[t][2 * q] * up, v[t][2 * q + 1] * up, a, b); hi[q] = a; lo[q] = b; }
+            for (int q = 0; q < 4; ++q) {
+                uint32_t a, b;
+                if (plain) plain_parts(v[t][2 * q], v[t][2 * q + 1], a, b); else half_parts(v[t][2 * q] * up, v[t][2 * q + 1] * up, a, b);
+                hi[q] = a; lo[q] = b;
+            }
             to[(s0 + t) * 128u] = hi; to[(s0 + t) * 128u + 64u] = lo;
         }
     }
@@ -171,7 +192,7 @@ __device__ __forceinline__ void linear_scores_body(float* __restrict__ peaks, fl
     half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
-    half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, begin, end - begin);
+    half_product<T, STAGES, TURNED_NONE, true>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), m, n, begin, end - begin, scales + PLAIN);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, wm = wave >> 1, wn = wave & 1u;
     const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
@@ -675,9 +696,9 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, float*
     half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
-    half_product<T, STAGES>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, begin, end - begin);
+    half_product<T, STAGES, TURNED_NONE, true>(acc, shared, operand_of(w, P.blocks_w, P.steps_w), operand_of(x, P.blocks_x, P.steps_x), P.tile0 + m, n, begin, end - begin, scales + PLAIN);
+    const bool plain = scales[PLAIN] != 0;
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
-    const float up = power_of_two(Q_SCALE);
     const int down = -(scales[PACK_WEIGHTS] + scales[PACK_ROWS]);
     const uint32_t lane = threadIdx.x & 63u, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1u, v0 = (P.tile0 + m) * SIDE;
     // of this lane's columns
@@ -689,15 +710,18 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, float*
         const uint32_t r = n * SIDE + (wn * T + j) * 32u + (lane & 31u), at = min(r, P.rows - 1u);
         given[j] = r < P.rows && is_token(tokens[at], P.V);
         token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
+        // (plain: ds itself, the rows' m has no part in the products)
+        const float up = plain ? factors[3u * at] : power_of_two(Q_SCALE);
         peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
-    half_store<T>(shared.turned, HalfTarget{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, HalfTarget{nullptr, 0u, 0u, 0u, 0u},
-                  [&](int i, int j, int k, uint32_t row, uint32_t) {
+    const HalfTarget to{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, none{nullptr, 0u, 0u, 0u, 0u};
+    auto q_of = [&](int i, int j, int k, uint32_t row, uint32_t) {
         const uint32_t v = v0 + row;
         const float s = scaled(half_sum(acc, i, j, k), down);
         const float q = part[j] * exp_of(s - peak[j]) + (v == token[j] ? one[j] : 0.f);
         return given[j] && v < P.V ? q : 0.f;
-    });
+    };
+    if (plain) half_store<T, true>(shared.turned, to, none, q_of); else half_store<T>(shared.turned, to, none, q_of);
 }
 #define LINEAR_Q(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                                     \
     extern "C" __global__ __launch_bounds__(256, BLOCKS) void linear_q##SUFFIX(u32x4* by_row, float* partial, uint32_t* arrivals, const u32x4* w,      \
@@ -722,11 +746,13 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
     half_work(blockIdx.x, HalfShares{P.whole, P.slices}, P.pairs, tile, slice, begin, end);
     half_tile(tile, P.tiles_m, P.tiles_n, m, n);
     HalfSums<T> acc = {};
-    half_product<T, STAGES, TURNED>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin);
+    const int32_t* const kind = (scales_a ? scales_a : scales_b) + PLAIN;
+    half_product<T, STAGES, TURNED, true>(acc, shared, operand_of(a, P.blocks_a, P.steps_a, P.first_a), operand_of(b, P.blocks_b, P.steps_b, P.first_b), m, n, begin, end - begin, kind);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = (m * 2u + (wave >> 1)) * 32u * T + 4u * (lane >> 5), lane_column = (n * 2u + (wave & 1u)) * 32u * T + (lane & 31u);
-    const int down = -(P.scale_a < 0 ? Q_SCALE : scales_a[P.scale_a]) - (P.scale_b < 0 ? Q_SCALE : scales_b[P.scale_b]);
+    const bool plain = *kind != 0;
+    const int q_scale = plain ? 0 : Q_SCALE, down = -(P.scale_a < 0 ? q_scale : scales_a[P.scale_a]) - (P.scale_b < 0 ? q_scale : scales_b[P.scale_b]);
     float* const to = out + (SHARED ? 0u : P.slice * slice);
 #pragma unroll
     for (int i = 0; i < T; ++i) {
@@ -750,7 +776,7 @@ __device__ __forceinline__ void linear_product_body(float* __restrict__ out, flo
                 const uint32_t column = lane_column + 32u * j;
                 if (column >= P.N) continue;
                 float s = scaled(half_sum(acc, i, j, q), down);
-                if (factors) s = f == 0.f ? 0.f : s * f;
+                if (factors) s = f == 0.f ? 0.f : plain ? s : s * f;
                 to[P.ld * row + column] = s + before[j][q];
             }
         }

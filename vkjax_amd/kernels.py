@@ -2885,9 +2885,9 @@ def _linear_sum(out, parts: Buffer, count: int, n: int) -> Launch:
                   bytes_moved=4 * (count + 1) * n)
 
 
-def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, cotangents=None, scaled=False):
+def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, transposed: bool, scratch, scales: Buffer, forward=None, cotangents=None, scaled=False, given=None):
     '''Launches that take operands apart: for the scores' product, into `forward` (the weights, x); with cotangents also, into the first of what is returned, x with its rows' factors contracted
-    over the rows (where it is `scaled`), and the factors. Scales go to `scales`.'''
+    over the rows (where it is `scaled`), and the factors. Scales go to `scales`; `given`: those of the forward pass, where that has taken its operands apart.'''
     rows, h, v = shape
     row_blocks    = max(1, min(1024, _cdiv(rows, 4)))
     weight_blocks = max(1, min(512, _cdiv(h * v, 4096))) if forward else 0
@@ -2898,7 +2898,7 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     x_scaled = scratch((_half_words(h, rows),), np.uint32) if scaled else None
     if scaled:
         jobs.append((x_scaled, h, rows, _PACK_SCALED, (1, h)))
-    params, blocks = _u32(weight_blocks, row_blocks, v, 0), 0
+    params, blocks = _u32(weight_blocks, row_blocks, v, h), 0
     for _, i, k, kind, strides in jobs:
         steps  = _half_steps(k)
         each   = min(steps, 8)
@@ -2908,7 +2908,7 @@ def _linear_prepare(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer, tr
     launches = [Launch('linear_largest', (weight_blocks + row_blocks, 1, 1), (BLOCK, 1, 1), [(b, 0) for b in (largest, factors, x, w, tokens, g_log_probs, g_log_sums)],
                        _u32(0, rows, h, v, weight_blocks, row_blocks), bytes_moved=4 * (x.size + w.size), written=(0, 1))]
     if jobs:
-        launches.append(Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(j[0], 0) for j in jobs] + [(None, 0)] * (3 - len(jobs)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors)],
+        launches.append(Launch('linear_pack', (blocks, 1, 1), (BLOCK, 1, 1), [(j[0], 0) for j in jobs] + [(None, 0)] * (3 - len(jobs)) + [(b, 0) for b in (scales, x, w, tokens, largest, factors, given)],
                                params, bytes_moved=8 * sum(i * k for _, i, k, _, _ in jobs), written=(0, 1, 2, 3)))
     return launches, (x_scaled, factors)
 
@@ -2953,7 +2953,8 @@ def linear_log_probs_grad(dx, dw, x: Buffer, w: Buffer, tokens: Buffer, peaks: B
         return _linear_rows_grad(dx, dw, shape, x, w, tokens, peaks, totals, g_log_probs, g_log_sums, transposed, scratch, *(parts or [None]))
     scales = scratch((4,), np.int32)                       #of what is taken apart here
     w_parts, x_parts, score_scales = parts or [*(scratch((n,), np.uint32) for n, _ in linear_parts(x.shape, w.shape, transposed)[:2]), scales]
-    launches, (x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None if parts else (w_parts, x_parts), (g_log_probs, g_log_sums), dw is not None)
+    launches, (x_scaled, factors) = _linear_prepare(shape, x, w, tokens, transposed, scratch, scales, None if parts else (w_parts, x_parts), (g_log_probs, g_log_sums), dw is not None,
+                                                    score_scales if parts else None)
     #pieces of the vocabulary, of whole tiles
     row_blocks, all_tiles = _cdiv(rows, 32), _cdiv(v, HALF_TILE)
     pieces = _cdiv(all_tiles, max(1, LINEAR_PIECE // (4 * 32 * row_blocks * HALF_TILE)))

@@ -96,12 +96,15 @@ def selective_scan(x, delta, a, b, c, d=None, gate=None, state=None, lengths=Non
 def linear_log_probs(x, weights, tokens, transposed=False):
     '''Log probabilities of given tokens (or classes) under softmax(x @ weights), without keeping the scores: x [..., hidden], weights [hidden, vocabulary], or with `transposed` the
     rows of an embedding, [vocabulary, hidden]; tokens int32 [...]. Returns (log_probs [...], log_sums [...]), the latter being log(sum(exp(scores))) of each row. A cross entropy is
-    -log_probs; the gradient works the scores out again, a piece of the vocabulary at a time. (Of up to 64 rows it takes the scores of the forward pass.)
+    -log_probs; the gradient works the scores out again, a piece of the vocabulary at a time. (Of up to 64 rows it takes the scores of the forward pass.) For a gradient the forward pass
+    keeps, until that is done, the weights and x once more as the products take them, or the scores of up to 64 rows.
 
     * A row whose token lies outside the vocabulary (negative, say) is padding: its results are 0, no gradient comes from it, and its x is not looked at.
-    * Products are as exact as fp32's for numbers down to 2^-28 of the largest of their operand (x's given rows, the weights); smaller ones are off by up to 2^-51 of that
-      largest. (Up to 64 rows are computed by fp32 products.)
-    * NaN and infinities in a row of x make that row's results NaN, in the weights those of every row.
+    * Up to 64 rows are computed by fp32 products. With more, numbers are held to 2^-22 of themselves or 2^-51 of the largest of their operand (x's given rows, the weights), and sums are rounded an
+      eighth as often, as long as no score is off by more than 2^-24 by the latter: where the largest magnitudes of x and of the weights, times one another and the features, pass 2^26, or a number is not
+      finite, fp32 products take their place (at a third to a half of the speed). So a row does not depend on what the others hold.
+    * The scores' cotangents, g p, are held in the same way for more than 64 rows, to 2^-51 of the row's larger cotangent: what tokens with probabilities below 2^-28 get has fewer bits, below 2^-52 none.
+    * Infinities and NaN are those of fp32 arithmetic: a NaN in a row of x makes that row's results NaN, one in the weights those of every row; a token whose weights make its score -inf has probability 0.
 
     Differentiable with respect to x and weights, through both results.'''
     return lax.linear_log_probs(x, weights, tokens, transposed)[:2]
