@@ -6,7 +6,7 @@ import tests.test_gpu_token_model_operators as operators
 from tests.test_gpu_operators import U, both, close
 from tests.test_gpu_token_model_operators import loss_bounds, loss_inputs, orthogonal_bound
 from tests.test_operators import normal
-from tests.test_token_model_operators import loss_program
+from tests.test_token_model_operators import loss_program, scan_inputs, scan_program
 from vkjax_amd import kernels as K, minijax as mj
 from vkjax_amd.jaxpr_interpreter import JaxprInterpreter
 
@@ -204,3 +204,25 @@ def test_infinite_weights_are_those_of_fp32_arithmetic(rows, transposed):
         bounds = loss_bounds(np.where(np.arange(41) == 7, 0, x).astype(f32), np.delete(w, 9, 0 if transposed else 1), tokens, g, gs, transposed)
         for a, b, bound in zip(got[:2], expected, bounds):
             close(a[fine], b[fine], bound[fine] + 41 * U * np.abs(b[fine]))
+
+
+# ------------------------------------------------------------------ selective scans
+
+@pytest.mark.parametrize('n', [3, 7, 16, 30, 64])
+@pytest.mark.parametrize('time', [5, 300])
+def test_scans_whose_last_step_is_infinite(time, n):
+    '''A state that becomes infinite in the last step of a sequence is that behind its length too; a cotangent that does in the gradient's first step is what goes on from there (where time is
+    not cut: products of many factors may be 0, and NaN times that).'''
+    arrays, g, g_last = scan_inputs(3, time, 64, n, (), False)
+    lengths = np.array([time, time // 2 + 1, 3], np.int32)
+    for name in ('b', 'c'):
+        spoiled = {k: v.copy() for k, v in arrays.items()}
+        for i, end in enumerate(lengths):
+            spoiled[name][i, end - 1, 1] = np.inf
+        got, expected, _ = both(scan_program(list(arrays), lengths, False), g, g_last, *spoiled.values())
+        outs = dict(zip(['y', 'last', *arrays], zip(got, expected)))
+        for result in ('y', 'last') + (('x', 'b', 'c') if name == 'c' and time < 8 else ()):
+            a, b = outs[result]
+            assert np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(np.sign(a[np.isinf(b)]), np.sign(b[np.isinf(b)])) and np.array_equal(np.isinf(a), np.isinf(b)), (name, result)
+        a, b = outs['last']
+        assert not np.isnan(a).any() and (np.isinf(a[:, :, 1]).all() if name == 'b' else np.isfinite(a).all())

@@ -77,12 +77,16 @@ struct Place {
     __device__ int64_t state(const ScanParams& P, int i) const { return ((int64_t)b * P.C + c) * P.N + n0 + i; }
     __device__ bool has(const ScanParams& P, int i) const { return n0 + i < P.N; }
     __device__ int own(int q) const { return (int)wave * OWN + q; }
-    // This thread's element of the eight steps' values from [B, T, N], as they lie in shared memory, [step][NS * M]: zeros for states that there are not
+    // This thread's element of the eight steps' values from [B, T, N], as they lie in shared memory, [step][NS * M]: zeros for states that there are not. TAKEN_ONLY: and for steps that are not taken,
+    // whose width of zero times an infinite value of the last one would be NaN (where they are not gone through, that one again)
     static constexpr int STAGED = KEPT * NS * M;
-    __device__ float staged(const float* __restrict__ p, const ScanParams& P, int t0) const {
+    template <bool TAKEN_ONLY> __device__ float staged(const float* __restrict__ p, const ScanParams& P, int t0) const {
         const uint32_t s = threadIdx.x / (uint32_t)(NS * M), n = threadIdx.x % (uint32_t)(NS * M);
-        return threadIdx.x < (uint32_t)STAGED && n < P.N ? p[((int64_t)b * P.T + min(t0 + (int)s, stop - 1)) * P.N + n] : 0.f;
+        const bool has = threadIdx.x < (uint32_t)STAGED && n < P.N;
+        if constexpr (TAKEN_ONLY) return has && t0 + (int)s < stop ? p[((int64_t)b * P.T + t0 + (int)s) * P.N + n] : 0.f;
+        return has ? p[((int64_t)b * P.T + min(t0 + (int)s, stop - 1)) * P.N + n] : 0.f;
     }
+    __device__ void stage(float (&rows)[KEPT][NS * M], float v) const { if (threadIdx.x < (uint32_t)STAGED) (&rows[0][0])[threadIdx.x] = v; }
     // ... and from there to the registers of the wave that has these states
     __device__ void maps(float (&v)[NS], const float (&rows)[KEPT][NS * M], int s) const {
 #pragma unroll
@@ -116,7 +120,7 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
             const int t = min(t0 + at.own(q), at.stop - 1);
             xs[q] = at.row(x, P, t)[at.c]; ds[q] = at.row(delta, P, t)[at.c];
         }
-        mapped = at.staged(bmap, P, t0);
+        mapped = at.template staged<true>(bmap, P, t0);
     };
     if (at.begin < at.stop) request(at.begin);
     int parity = 0;
@@ -128,7 +132,7 @@ __device__ __forceinline__ void scan_chunk_body(float* __restrict__ sums, float*
             prepared[parity][0][at.own(q)][at.lane] = taken ? w : 0.f;
             prepared[parity][1][at.own(q)][at.lane] = taken ? w * xs[q] : 0.f;
         }
-        if (threadIdx.x < (uint32_t)at.STAGED) (&map[parity][0][0])[threadIdx.x] = mapped;
+        at.stage(map[parity], mapped);
         if (t0 + KEPT < at.stop) request(t0 + KEPT);
         at.meet();
         float dt[KEPT], u[KEPT], bs[NS], next[NS];
@@ -222,7 +226,7 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
             xs[q] = at.row(x, P, t)[at.c]; ds[q] = at.row(delta, P, t)[at.c];
             if (gate) gs[q] = at.row(gate, P, t)[at.c];
         }
-        mapped[0] = at.staged(bmap, P, t0); mapped[1] = at.staged(cmap, P, t0);
+        mapped[0] = at.template staged<false>(bmap, P, t0); mapped[1] = at.template staged<false>(cmap, P, t0);
     };
     if (at.begin < at.stop) request(at.begin);
     for (int t0 = at.begin; t0 < at.end; t0 += KEPT) {
@@ -241,7 +245,7 @@ __device__ __forceinline__ void scan_body(float* __restrict__ y, float* __restri
                 ys[q] = D * xs[q];
                 open[q] = gate ? gs[q] * sigmoid(gs[q]) : 1.f;
             }
-            if (threadIdx.x < (uint32_t)at.STAGED) { (&map[0][0][0])[threadIdx.x] = mapped[0]; (&map[1][0][0])[threadIdx.x] = mapped[1]; }
+            at.stage(map[0], mapped[0]); at.stage(map[1], mapped[1]);
             if (t0 + KEPT < at.stop) request(t0 + KEPT);
             at.meet();
             float dt[KEPT], u[KEPT], bs[NS], cs[NS], next_b[NS], next_c[NS];
@@ -363,7 +367,7 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
             ds[q] = at.row(delta, P, t)[at.c]; gs[q] = g ? at.row(g, P, t)[at.c] : 0.f;
             if (gate) gates[q] = at.row(gate, P, t)[at.c];
         }
-        mapped = at.staged(cmap, P, t0);
+        mapped = at.template staged<true>(cmap, P, t0);
     };
     if (turns) request(at.begin + (turns - 1) * KEPT);
     for (int turn = turns - 1; turn >= 0; --turn) {
@@ -374,7 +378,7 @@ __device__ __forceinline__ void scan_grad_chunk_body(float* __restrict__ sums, f
             prepared[parity][0][at.own(q)][at.lane] = taken ? width_of(ds[q], add, P.softplus) : 0.f;
             prepared[parity][1][at.own(q)][at.lane] = taken ? (gate ? gs[q] * (gates[q] * sigmoid(gates[q])) : gs[q]) : 0.f;
         }
-        if (threadIdx.x < (uint32_t)at.STAGED) (&map[parity][0][0])[threadIdx.x] = mapped;
+        at.stage(map[parity], mapped);
         if (turn > 0) request(t0 - KEPT);
         at.meet();
         float dt[KEPT], gy[KEPT], cs[NS], next[NS];
@@ -445,7 +449,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) rh[i] = at.has(P, i) ? at.held(kept, P, (uint32_t)t0 / KEPT, i)[at.c] : 0.f;
-        rmap[0] = at.staged(bmap, P, t0); rmap[1] = at.staged(cmap, P, t0);
+        rmap[0] = at.template staged<(AT_ONCE > 1)>(bmap, P, t0); rmap[1] = at.template staged<(AT_ONCE > 1)>(cmap, P, t0);
     };
     bool requested = false;
     for (int turn = turns - 1; turn >= 0; --turn) {
@@ -471,7 +475,7 @@ __device__ __forceinline__ void scan_grad_body(float* __restrict__ dx, float* __
             float h[NS], before[KEPT][NS];
 #pragma unroll
             for (int i = 0; i < NS; ++i) h[i] = rh[i];
-            if (threadIdx.x < (uint32_t)at.STAGED) { (&map[0][0][0])[threadIdx.x] = rmap[0]; (&map[1][0][0])[threadIdx.x] = rmap[1]; }
+            at.stage(map[0], rmap[0]); at.stage(map[1], rmap[1]);
             if (turn > 0) request(t0 - KEPT);
             at.meet();
             // (a step's dt, x, gy and maps, and those of the step behind it: all eight's would take the registers of a third wave)
