@@ -226,3 +226,28 @@ def test_scans_whose_last_step_is_infinite(time, n):
             assert np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(np.sign(a[np.isinf(b)]), np.sign(b[np.isinf(b)])) and np.array_equal(np.isinf(a), np.isinf(b)), (name, result)
         a, b = outs['last']
         assert not np.isnan(a).any() and (np.isinf(a[:, :, 1]).all() if name == 'b' else np.isfinite(a).all())
+
+
+# ------------------------------------------------------------------ orthogonalised matrices of any size
+
+@pytest.mark.parametrize('scale,eps', [(1e-37, 1e-38), (1e-30, 1e-36), (1e-25, 1e-30), (1e-22, 1e-45), (1e18, 1e-7), (1e22, 1e-7), (1e37, 1e-7), (8e37, 1e30)])
+@pytest.mark.parametrize('shape', [(100, 100), (70, 300), (300, 70), (2, 65, 3), (2, 3, 1200), (40, 50)], ids=str)
+def test_orthogonalize_by_the_norm_of_its_matrix(shape, scale, eps):
+    '''Squares that fp32 does not have, either way; a norm beside which eps is nothing, or the other way round.'''
+    if min(shape[-2:]) in range(4, 65) and not 1e-36 < scale < 1e35:
+        scale = 1e-35 if scale < 1 else 1e34
+    x = normal(7, *shape)
+    x *= f32(min(scale, 3.2e38 / float(np.abs(x).max())))
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, 3, (1.5, -0.5, 0.0), eps), x)
+    for a, b, m in zip(got.reshape(-1, *shape[-2:]), expected.reshape(-1, *shape[-2:]), x.reshape(-1, *shape[-2:])):
+        off, bound = np.linalg.norm(a.astype(np.float64) - b), orthogonal_bound(m, 3, (1.5, -0.5, 0.0), float(f32(eps)))
+        assert off <= bound, (off, bound, np.linalg.norm(b.astype(np.float64)))
+
+
+def test_orthogonalize_a_matrix_that_is_not_finite():
+    for value in (np.inf, -np.inf, np.nan):
+        for rows, columns in ((150, 90), (40, 90), (3, 70)):
+            x = normal(1, 3, rows, columns)
+            x[1, rows // 2, 5] = value
+            got, = JaxprInterpreter(mj.make_jaxpr(lambda x: nn.orthogonalize(x))(x)).run(x)
+            assert np.isnan(got[1]).all() and np.isfinite(got[0]).all() and np.isfinite(got[2]).all()

@@ -11,14 +11,18 @@
 
 typedef f32x4 f32x4_anywhere __attribute__((aligned(4)));
 
+__device__ __forceinline__ double wave_sum(double t) {
+    wave_butterfly([&](auto step) { t += __builtin_bit_cast(double, lane_xor<decltype(step)::value>(__builtin_bit_cast(uint64_t, t))); });
+    return t;
+}
 struct SquaresParams { uint32_t blocks, pad; uint64_t n; };
-// [matrix][block]: sums of squares
-extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __restrict__ sums, const float* __restrict__ x, SquaresParams P) {
-    __shared__ float part[4];
+// [matrix][block]: sums of squares, in fp64, whose range has the squares of all fp32 numbers (and whose rate leaves the launch to memory)
+extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(double* __restrict__ sums, const float* __restrict__ x, SquaresParams P) {
+    __shared__ double part[4];
     const uint32_t matrix = blockIdx.x / P.blocks, block = blockIdx.x % P.blocks;
     const float* const from = x + matrix * P.n;
     const uint64_t stride = (uint64_t)P.blocks * 256u;
-    float s[4] = {};
+    double s[4] = {};
     // (vectors wherever every matrix begins at one)
     const uint64_t vectors = (P.n & 3u) == 0u ? P.n / 4u : 0u;
     uint64_t at = (uint64_t)block * 256u + threadIdx.x;
@@ -29,11 +33,10 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(float* __re
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(v[k][e], v[k][e], s[e]);
+            for (int e = 0; e < 4; ++e) s[e] = __builtin_fma((double)v[k][e], (double)v[k][e], s[e]);
     }
-    for (at = 4u * vectors + (uint64_t)block * 256u + threadIdx.x; at < P.n; at += stride) s[0] = __builtin_fmaf(from[at], from[at], s[0]);
-    float t = (s[0] + s[1]) + (s[2] + s[3]);
-    wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
+    for (at = 4u * vectors + (uint64_t)block * 256u + threadIdx.x; at < P.n; at += stride) s[0] = __builtin_fma((double)from[at], (double)from[at], s[0]);
+    const double t = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
     if ((threadIdx.x & 63u) == 0u) part[threadIdx.x >> 6] = t;
     __syncthreads();
     if (threadIdx.x == 0u) sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
@@ -45,16 +48,19 @@ struct OrthogonalPackParams {
     uint64_t sr, sc;                                                                     // element strides of row and column
     float eps; int32_t scale;
 };
-extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, const float* __restrict__ x, const float* __restrict__ sums, OrthogonalPackParams P) {
-    __shared__ float part[4];
+extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, const float* __restrict__ x, const double* __restrict__ sums, OrthogonalPackParams P) {
+    __shared__ double part[4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t matrix = blockIdx.x / P.blocks, block = blockIdx.x - matrix * P.blocks;
-    float t = 0.f;
+    double t = 0.0;
     for (uint32_t k = threadIdx.x; k < P.sum_blocks; k += 256u) t += sums[(uint64_t)matrix * P.sum_blocks + k];
-    wave_butterfly([&](auto step) { t += lane_xor<decltype(step)::value>(t); });
+    t = wave_sum(t);
     if (lane == 0u) part[wave] = t;
     __syncthreads();
-    const float norm = __builtin_sqrtf((part[0] + part[1]) + (part[2] + part[3])) + P.eps, up = power_of_two(P.scale);
+    // the norm as a number between 1 and 2 and a power of two, which fp32's range need not have (one that is not finite makes all of its matrix NaN)
+    const double all_norm = __builtin_sqrt((part[0] + part[1]) + (part[2] + part[3])) + (double)P.eps;
+    const int up = P.scale - (int)((__builtin_bit_cast(uint64_t, all_norm) >> 52 & 0x7FFu) - 1023u);
+    const float norm = all_norm < __builtin_inf() ? (float)__builtin_bit_cast(double, (__builtin_bit_cast(uint64_t, all_norm) & 0xFFFFFFFFFFFFFull) | 1023ull << 52) : __builtin_nanf("");
     const uint32_t I = P.R, K = P.C, steps = 2u * ((K + 31u) / 32u), each = P.each;
     const uint64_t si = P.sr, sk = P.sc;
     const uint32_t groups = (steps + each - 1u) / each, all = block * 4u + wave, blocks32 = (I + 31u) / 32u;
@@ -87,7 +93,7 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restr
             if (s0 + t >= end) break;
             u32x4 hi, lo;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(v[t][2 * q] / norm * up, v[t][2 * q + 1] / norm * up, a, b); hi[q] = a; lo[q] = b; }
+            for (int q = 0; q < 4; ++q) { uint32_t a, b; half_parts(__builtin_amdgcn_ldexpf(v[t][2 * q] / norm, up), __builtin_amdgcn_ldexpf(v[t][2 * q + 1] / norm, up), a, b); hi[q] = a; lo[q] = b; }
             to[(s0 + t) * 128u] = hi; to[(s0 + t) * 128u + 64u] = lo;
         }
     }

@@ -3065,7 +3065,7 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
     if 4 <= r <= ORTHOGONAL_SMALL and c <= ORTHOGONAL_SMALL_COLUMNS and n * c < 2**29 and growth <= 2**22 and not many:
         return _orthogonalize_small(out, x, n, r, c, sr, sc, steps, coefficients, eps, scratch)
     sum_blocks = max(1, min(1024 if n == 1 else 256, _cdiv(r * c, 4096)))
-    sums     = scratch((n, sum_blocks))
+    sums     = scratch((n, sum_blocks, 2))                                                  #(fp64)
     by_row   = [scratch((n * _half_words(r, c),), np.uint32) for _ in range(2 if steps > 1 else 1)]
     square, square_parts, polynomial = scratch((n, r, r)), scratch((n * _half_words(r, r),), np.uint32), scratch((n * _half_words(r, r),), np.uint32)
     bounds   = orthogonal_bounds(steps, coefficients)

@@ -113,7 +113,7 @@ def linear_log_probs(x, weights, tokens, transposed=False):
 def orthogonalize(x, steps=5, coefficients=lax.ORTHOGONALIZE_COEFFICIENTS, eps=1e-7):
     '''Every matrix of x [..., rows, columns] with its singular values brought to about 1, as an optimiser does it with the momentum of a weight's gradients before the weight is updated:
     x / (|x| + eps), then `steps` (1 to 32) times the polynomial a s + b s^3 + c s^5 of the singular values, by products of matrices. With the default coefficients five steps bring singular values
-    from 0.01 of the norm on to between 0.7 and 1.2; (1.5, -0.5, 0) approaches 1 itself, more slowly. Matrices of zeros stay zeros; NaN and infinities in a matrix spoil that one only; one whose
-    norm is beyond 1e19 may come out as zeros.
+    from 0.01 of the norm on to between 0.7 and 1.2; (1.5, -0.5, 0) approaches 1 itself, more slowly. Matrices of zeros stay zeros; NaN and infinities in a matrix spoil that one only; one of up
+    to 64 rows or columns whose norm (with eps) is below 1e-36 or beyond 1e36 may lose bits.
     Coefficients with which singular values do not stay small are refused. Not differentiable.'''
     return lax.orthogonalize(x, steps, coefficients, eps)
