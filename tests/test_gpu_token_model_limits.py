@@ -230,7 +230,7 @@ def test_scans_whose_last_step_is_infinite(time, n):
 
 # ------------------------------------------------------------------ orthogonalised matrices of any size
 
-@pytest.mark.parametrize('scale,eps', [(1e-37, 1e-38), (1e-30, 1e-36), (1e-25, 1e-30), (1e-22, 1e-45), (1e18, 1e-7), (1e22, 1e-7), (1e37, 1e-7), (8e37, 1e30)])
+@pytest.mark.parametrize('scale,eps', [(1e-37, 1e-38), (1e-30, 1e-36), (1e-25, 1e-30), (1e-22, 1e-45), (1e-19, 1e-7), (1e18, 1e-7), (1e22, 1e-7), (1e37, 1e-7), (8e37, 1e30)])
 @pytest.mark.parametrize('shape', [(100, 100), (70, 300), (300, 70), (2, 65, 3), (2, 3, 1200), (40, 50)], ids=str)
 def test_orthogonalize_by_the_norm_of_its_matrix(shape, scale, eps):
     '''Squares that fp32 does not have, either way; a norm beside which eps is nothing, or the other way round.'''
@@ -241,6 +241,19 @@ def test_orthogonalize_by_the_norm_of_its_matrix(shape, scale, eps):
     (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, 3, (1.5, -0.5, 0.0), eps), x)
     for a, b, m in zip(got.reshape(-1, *shape[-2:]), expected.reshape(-1, *shape[-2:]), x.reshape(-1, *shape[-2:])):
         off, bound = np.linalg.norm(a.astype(np.float64) - b), orthogonal_bound(m, 3, (1.5, -0.5, 0.0), float(f32(eps)))
+        assert off <= bound, (off, bound, np.linalg.norm(b.astype(np.float64)))
+
+
+@pytest.mark.parametrize('steps,coefficients', [(1, (3.4445, -4.7750, 2.0315)), (5, (3.4445, -4.7750, 2.0315)), (32, (1.5, -0.5, 0.0)), (4, (0.1, 0.0, 0.0)), (10, (2.0, -1.5, 0.5)), (9, (3.4445, -4.7750, 2.0315))], ids=str)
+@pytest.mark.parametrize('shape', [(100, 100), (70, 300), (300, 70), (3, 1200), (40, 50)], ids=str)
+def test_orthogonalize_matrices_that_eps_leaves_small(shape, steps, coefficients):
+    '''Norms far below eps: a stack of matrices, of which each has the bits that it has by itself, whatever the steps raise it to.'''
+    sizes = np.array([1.0, 1e-3, 1e-5, 1e-8, 1e-12, 1e-17, 1e-25, 0.0])
+    x = (normal(8, len(sizes), *shape) * sizes[:, None, None]).astype(f32)
+    (got,), (expected,), _ = both(lambda x: nn.orthogonalize(x, steps, coefficients, 1.0), x)
+    assert not got[-1].any()
+    for a, b, m in zip(got[:-1], expected, x):
+        off, bound = np.linalg.norm(a.astype(np.float64) - b), orthogonal_bound(m, steps, coefficients, 1.0)
         assert off <= bound, (off, bound, np.linalg.norm(b.astype(np.float64)))
 
 

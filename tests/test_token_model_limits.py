@@ -16,7 +16,7 @@ def test_scales_of_polynomials_are_powers_that_fp32_has(steps, coefficients):
     x, seen = buffer(100, 100), 0
     for launch in K.orthogonalize(x, x, steps, coefficients, 1e-7, scratch, zeroed):
         words = np.frombuffer(launch.params, np.int32)
-        scales = words[7:10] if launch.kernel.startswith(('orthogonal_square_', 'orthogonal_poly', 'orthogonal_next', 'orthogonal_last')) else words[-1:] if launch.kernel == 'orthogonal_pack' else ()
+        scales = words[7:10] if launch.kernel.startswith(('orthogonal_square_', 'orthogonal_poly', 'orthogonal_next', 'orthogonal_last')) else words[-3:-2] if launch.kernel == 'orthogonal_pack' else ()
         assert all(-126 <= s <= 126 for s in scales), (launch.kernel, scales)
         seen += len(scales)
     assert seen == 1 + 9 * steps

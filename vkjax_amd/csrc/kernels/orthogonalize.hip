@@ -3,7 +3,8 @@
 // so that every singular value s becomes a s + b s^3 + c s^5. Products are those of half_product.h, between operands that never leave their taken-apart form: a product's tile
 // turns its results into an operand, X into one contracted over its columns (turned in shared memory), which B X reads turned again (contracted over rows). A and B are symmetric:
 // of their tiles only those on and above the diagonal are computed, and stored both ways. Only A is kept as fp32 too, since b A is a term of B. X has 22 bits between the steps; no
-// operand's magnitude depends on the data beyond |x|, since a singular value's bound follows from the polynomial alone, so scales are known to the host.
+// operand's magnitude depends on the data beyond |x|, since a singular value's bound follows from the polynomial alone, so scales are known to the host - but for a matrix that eps leaves small: X is
+// scaled by 2^small more then, small by how far |x| / (|x| + eps) is below 1, less `grown`, what the steps in front may have made of it.
 // Matrices of a stack lie side by side in every launch.
 // Bound by the matrix cores' power where a matrix fills the machine: 4096 x 4096 takes 212 us for a square, 257 for the polynomial (whose epilogue reads the square), 380 for B X (362 TFLOP/s of fp32
 // products), 4.45 ms for five steps, of which the products alone at that rate are 3.6. 12 of 512 x 512: 13 to 18 us a launch, whose contraction of 512 is 16 pairs of steps behind one another.
@@ -46,9 +47,11 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_squares(double* __r
 struct OrthogonalPackParams {
     uint32_t matrices, R, C, sum_blocks, each, blocks;                                   // blocks of 256 threads, per matrix
     uint64_t sr, sc;                                                                     // element strides of row and column
-    float eps; int32_t scale;
+    float eps; int32_t scale; uint32_t grown, pad;
 };
-extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, const float* __restrict__ x, const double* __restrict__ sums, OrthogonalPackParams P) {
+__device__ __forceinline__ int exponent_of(double v) { return (int)(__builtin_bit_cast(uint64_t, v) >> 52 & 0x7FFu) - 1023; }
+__device__ __forceinline__ int more_scale(uint32_t small, uint32_t grown) { return (int)(small > grown ? small - grown : 0u); }
+extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restrict__ by_row, uint32_t* __restrict__ smalls, const float* __restrict__ x, const double* __restrict__ sums, OrthogonalPackParams P) {
     __shared__ double part[4];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t matrix = blockIdx.x / P.blocks, block = blockIdx.x - matrix * P.blocks;
@@ -58,8 +61,11 @@ extern "C" __global__ __launch_bounds__(256) void orthogonal_pack(u32x4* __restr
     if (lane == 0u) part[wave] = t;
     __syncthreads();
     // the norm as a number between 1 and 2 and a power of two, which fp32's range need not have (one that is not finite makes all of its matrix NaN)
-    const double all_norm = __builtin_sqrt((part[0] + part[1]) + (part[2] + part[3])) + (double)P.eps;
-    const int up = P.scale - (int)((__builtin_bit_cast(uint64_t, all_norm) >> 52 & 0x7FFu) - 1023u);
+    const double own_norm = __builtin_sqrt((part[0] + part[1]) + (part[2] + part[3])), all_norm = own_norm + (double)P.eps;
+    // (a matrix of zeros has no exponent)
+    const uint32_t small = own_norm > 0.0 ? (uint32_t)(exponent_of(all_norm) - exponent_of(own_norm)) : 0u;
+    if (block == 0u && threadIdx.x == 0u) smalls[matrix] = small;
+    const int up = P.scale + more_scale(small, P.grown) - exponent_of(all_norm);
     const float norm = all_norm < __builtin_inf() ? (float)__builtin_bit_cast(double, (__builtin_bit_cast(uint64_t, all_norm) & 0xFFFFFFFFFFFFFull) | 1023ull << 52) : __builtin_nanf("");
     const uint32_t I = P.R, K = P.C, steps = 2u * ((K + 31u) / 32u), each = P.each;
     const uint64_t si = P.sr, sk = P.sc;
@@ -104,13 +110,14 @@ enum OrthogonalKind : uint32_t { SQUARE = 0, POLYNOMIAL = 1, NEXT = 2, LAST = 3 
 struct OrthogonalParams {
     uint32_t kind, M, N, K, tiles_m, tiles_n, tiles;     // tiles of a matrix: those on and above the diagonal of a square
     int32_t scale_a, scale_b, scale_out;
-    float a, b, c; uint32_t whole, slices, pad;          // (HalfShares)
+    float a, b, c; uint32_t whole, slices;               // (HalfShares)
+    uint32_t grown, grown_next, pad;
     uint64_t sr, sc;                                     // the last result's element strides
 };
 // (kinds in templates: their epilogues share no registers)
 template <uint32_t KIND, int T, int STAGES, bool SHARED>
 __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u32x4* __restrict__ by_row, float* __restrict__ out, float* __restrict__ partial, uint32_t* __restrict__ arrivals,
-                                                const u32x4* __restrict__ a, const u32x4* __restrict__ b, const float* __restrict__ square, const OrthogonalParams& P) {
+                                                const u32x4* __restrict__ a, const u32x4* __restrict__ b, const float* __restrict__ square, const uint32_t* __restrict__ smalls, const OrthogonalParams& P) {
     __shared__ HalfShared<T, STAGES> shared;
     constexpr bool SYMMETRIC = KIND == SQUARE || KIND == POLYNOMIAL;
     constexpr uint32_t SIDE = 64u * T;
@@ -130,9 +137,9 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     if constexpr (SYMMETRIC) half_product<T, STAGES>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * blocks_n * steps_k * 128u, blocks_n, steps_k, 0u}, m, n, begin, end - begin);
     else half_product<T, STAGES, TURNED_B>(acc, shared, left, HalfOperand{b + (uint64_t)matrix * (steps_k / 2u) * steps_n * 128u, blocks_n, steps_n, 0u}, m, n, begin, end - begin);
     if constexpr (SHARED) if (!half_join<T, STAGES>(acc, shared, partial, arrivals, tile, slice, HalfShares{P.whole, P.slices})) return;
-    // (both operands' scales at once: their factors' product may be below what fp32 has where a result is not)
-    const int down = -(P.scale_a + P.scale_b);
-    const float up = power_of_two(P.scale_out);
+    // (both operands' scales at once: their factors' product may be below what fp32 has where a result is not; X's own is what the matrix has more)
+    const int more = KIND == POLYNOMIAL ? 0 : more_scale(smalls[matrix], P.grown);
+    const int down = -(P.scale_a + P.scale_b) - (KIND == SQUARE ? 2 : 1) * more, up = P.scale_out + (KIND == NEXT ? more_scale(smalls[matrix], P.grown_next) : 0);
     auto result = [&](int i, int j, int k) { return __builtin_amdgcn_ldexpf(half_sum(acc, i, j, k), down); };
     const uint32_t row0 = m * SIDE, column0 = n * SIDE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t lane_row = row0 + (wave >> 1) * 32u * T + 4u * (lane >> 5), lane_column = column0 + (wave & 1u) * 32u * T + (lane & 31u);
@@ -174,16 +181,18 @@ __device__ __forceinline__ void orthogonal_body(u32x4* __restrict__ by_column, u
     half_store<T>(shared.turned, columns, rows, [&](int i, int j, int k, uint32_t row, uint32_t column) {
         row += row0; column += column0;
         if (row >= P.M || column >= P.N) return 0.f;
+        if constexpr (KIND == NEXT) return __builtin_amdgcn_ldexpf(half_sum(acc, i, j, k), down + up);
         float v = result(i, j, k);
         if constexpr (KIND == SQUARE) out[each + (uint64_t)row * P.N + column] = v;
         if constexpr (KIND == POLYNOMIAL) v = __builtin_fmaf(P.c, v, __builtin_fmaf(P.b, squares[i][j][k], row == column ? P.a : 0.f));
-        return v * up;
+        return __builtin_amdgcn_ldexpf(v, up);
     });
 }
 #define ORTHOGONAL(NAME, KIND, SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                     \
     extern "C" __global__ __launch_bounds__(256, BLOCKS) void orthogonal_##NAME##SUFFIX(u32x4* by_column, u32x4* by_row, float* out, float* partial, uint32_t* arrivals, \
-                                                                                        const u32x4* a, const u32x4* b, const float* square, OrthogonalParams P) {    \
-        orthogonal_body<KIND, T, STAGES, SHARED>(by_column, by_row, out, partial, arrivals, a, b, square, P);                                                         \
+                                                                                        const u32x4* a, const u32x4* b, const float* square, const uint32_t* smalls,  \
+                                                                                        OrthogonalParams P) {                                                         \
+        orthogonal_body<KIND, T, STAGES, SHARED>(by_column, by_row, out, partial, arrivals, a, b, square, smalls, P);                                                 \
     }
 #define ORTHOGONAL_KINDS(SUFFIX, T, STAGES, BLOCKS, SHARED)                                                                                                           \
     ORTHOGONAL(square, SQUARE, SUFFIX, T, STAGES, BLOCKS, SHARED) ORTHOGONAL(polynomial, POLYNOMIAL, SUFFIX, T, STAGES, BLOCKS, SHARED)                               \

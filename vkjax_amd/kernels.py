@@ -3069,28 +3069,33 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
     by_row   = [scratch((n * _half_words(r, c),), np.uint32) for _ in range(2 if steps > 1 else 1)]
     square, square_parts, polynomial = scratch((n, r, r)), scratch((n * _half_words(r, r),), np.uint32), scratch((n * _half_words(r, r),), np.uint32)
     bounds   = orthogonal_bounds(steps, coefficients)
+    #powers of two that X may have grown by in front of each step, beside its bound (a matrix that eps leaves small has X below 2^(1 - small) at first)
+    log      = lambda v: math.log2(max(v, 1e-300))
+    grown    = [max(0, math.ceil(1 + sum(log(p) for _, p in bounds[:i]) - log(s))) for i, (s, _) in enumerate(bounds)] + [0]
+    smalls   = scratch((n,), np.uint32)
     each     = min(_half_steps(c), 8)
     blocks   = _cdiv(_cdiv(r, 32) * _cdiv(_half_steps(c), each), 4)
     launches = [Launch('orthogonal_squares', (n * sum_blocks, 1, 1), (BLOCK, 1, 1), [(sums, 0), (x, 0)], _u32(sum_blocks, 0) + _u64(r * c), bytes_moved=4 * x.size),
-                Launch('orthogonal_pack', (n * blocks, 1, 1), (BLOCK, 1, 1), [(by_row[0], 0), (x, 0), (sums, 0)],
-                       _u32(n, r, c, sum_blocks, each, blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])), bytes_moved=8 * x.size)]
+                Launch('orthogonal_pack', (n * blocks, 1, 1), (BLOCK, 1, 1), [(by_row[0], 0), (smalls, 0), (x, 0), (sums, 0)],
+                       _u32(n, r, c, sum_blocks, each, blocks) + _u64(sr, sc) + np.float32(eps).tobytes() + _i32(_half_scale(bounds[0][0])) + _u32(grown[0], 0), bytes_moved=8 * x.size,
+                       written=(0, 1))]
 
-    def product(name, results, a, b, square, m, width, k, scales, written):
+    def product(name, results, a, b, square, m, width, k, scales, written, step):
         symmetric = name in ('square', 'polynomial')
         of_matrix = lambda side: _cdiv(m, side) * (_cdiv(m, side) + 1) // 2 if symmetric else _cdiv(m, side) * _cdiv(width, side)
         plan  = half_plan(lambda side: n * of_matrix(side), _half_steps(k) // 2)
         suffix, blocks, partial, arrivals = half_share(plan, n * of_matrix(plan.side), scratch, zeroed)
-        return Launch(f'orthogonal_{name}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square)],
+        return Launch(f'orthogonal_{name}{suffix}', (blocks, 1, 1), (BLOCK, 1, 1), [(v, 0) for v in (*results, partial, arrivals, a, b, square, smalls)],
                       _u32(('square', 'polynomial', 'next', 'last').index(name), m, width, k, _cdiv(m, plan.side), _cdiv(width, plan.side), of_matrix(plan.side)) + _i32(*scales)
-                      + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, 0) + _u64(sr, sc),
+                      + np.asarray(coefficients, np.float32).tobytes() + _u32(plan.whole, plan.slices, grown[step], grown[step + 1], 0) + _u64(sr, sc),
                       bytes_moved=4 * n * (m * k + width * k + 2 * m * width), flops=(1 if symmetric else 2) * n * m * width * k,
                       written=written + ((3, 4) if partial is not None else ()), scratch=(4,) if partial is not None else ())
     for i, (s, p) in enumerate(bounds):
         scale_x, scale_a, scale_p = _half_scale(s), _half_scale(s * s), _half_scale(p)
-        launches += [product('square', (square_parts, square_parts, square), by_row[i & 1], by_row[i & 1], None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2)),
-                     product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, (scale_a, scale_a, scale_p), (0, 1))]
+        launches += [product('square', (square_parts, square_parts, square), by_row[i & 1], by_row[i & 1], None, r, r, c, (scale_x, scale_x, scale_a), (0, 1, 2), i),
+                     product('polynomial', (polynomial, polynomial, None), square_parts, square_parts, square, r, r, r, (scale_a, scale_a, scale_p), (0, 1), i)]
         last = i == steps - 1
         scale_next = 0 if last else _half_scale(bounds[i + 1][0])
         launches.append(product('last' if last else 'next', (None, None, out) if last else (None, by_row[(i + 1) & 1], None), polynomial, by_row[i & 1], None, r, c, r,
-                                (scale_p, scale_x, scale_next), (2,) if last else (1,)))
+                                (scale_p, scale_x, scale_next), (2,) if last else (1,), i))
     return launches
