@@ -2577,7 +2577,8 @@ def linear_recurrence_grad(dfactor, dx, dstate, h: Buffer, factor: Buffer, x: Bu
 
 CAUSAL_CONV_WIDTHS = range(2, 9)
 CAUSAL_CONV_STEPS  = 8                  #of a thread, where time has more than one
-#blocks that the gradient's tiles of time are shared out to
+#blocks that the gradient's tiles of time are shared out to: a step of 8 x 2048 x 2048 takes 152 us (512 blocks 148, 256 187, a tile each 164), of 1 x 16384 x 2048 169 (159, 201, 179), of
+#64 x 256 x 1024 69 (70, 69, 73); smaller ones have fewer tiles
 CAUSAL_CONV_GRAD_BLOCKS = 1024
 
 
@@ -2830,7 +2831,7 @@ def _linear_rows_scores(shape: LinearShape, x: Buffer, w: Buffer, tokens: Buffer
     tiles  = _cdiv(v, _linear_rows_tile(rows, not transposed))
     #few tiles: slices of the features, of four times the rows and 64 at least, that a block to a CU makes (4 x 4096 x 1000 81 -> 22 us, 4 x 4096 x 16000 85 -> 53, 64 x 2048 x 8000 80 -> 37, with a
     #launch more; two blocks to a CU 31, 55, 41)
-    #(tiles for half of the CUs and some: three slices, two blocks to most CUs: 6 x 2792 x 17351 63 -> 52 us, 6 x 4096 x 20000 89 -> 70; of 1024 features 30 and 29, of two slices 33)
+    #(tiles for half of the CUs and some: three slices, two blocks to most CUs: 6 x 2792 x 17351 63 -> 52 us, 6 x 4096 x 20000 89 -> 70; of 1024 features 30 and 29, of two slices 33. Of nine sizes of 1 to 64 rows and 2048 to 8192 features, either way round, 9 to 18 % less each)
     blocks = HALF_CUS if tiles <= HALF_CUS // 2 or 3 * tiles > 2 * HALF_CUS or h < 2048 else 2 * HALF_CUS
     slices = max(1, min(blocks // tiles, h // max(64, 4 * rows)))
     parts  = scratch((slices, rows, v)) if slices > 1 else None
@@ -3060,7 +3061,8 @@ def orthogonalize(out: Buffer, x: Buffer, steps: int, coefficients, eps: float, 
         raise NotImplementedError(f'orthogonalising {n} matrices of {rows} x {columns}')
     #a Gram matrix's errors, 2^-46 of its largest eigenvalue (some of them negative ones where x has no rank), grow as small eigenvalues do, by the polynomials' squares: below 2^-24 in the end
     growth = math.prod(max(1.0, p / 1.25)**2 for _, p in orthogonal_bounds(steps, coefficients))
-    #(many matrices that are hardly wider than high fill the machine in the general form too: 4096 of 64 x 64, one step 153 us, by Gram matrices 247, five 600 and 704; of 48 x 48 126 and 166, 534 and 415)
+    #(many matrices that are hardly wider than high fill the machine in the general form too: 4096 of 64 x 64, one step 153 us, by Gram matrices 247, five 600 and 704; of 48 x 48 126 and 166, 534 and 415. 2000 of 64 x 64, one step, 73 and 124, of 17 x 20 37 and 40, of 17 x 60 44 and 43; 600 of 64 x 64, five, 122 and 130, of 48 x 48
+    #112 and 80, 1000 of 56 x 100 207 and 187, of 64 x 300 354 and 251)
     many = n > 512 and c < 4 * r and r > (16 if steps == 1 else 48)
     if 4 <= r <= ORTHOGONAL_SMALL and c <= ORTHOGONAL_SMALL_COLUMNS and n * c < 2**29 and growth <= 2**22 and not many:
         return _orthogonalize_small(out, x, n, r, c, sr, sc, steps, coefficients, eps, scratch)
