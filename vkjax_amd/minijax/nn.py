@@ -103,7 +103,8 @@ def linear_log_probs(x, weights, tokens, transposed=False):
     * Up to 64 rows are computed by fp32 products. With more, numbers are held to 2^-22 of themselves or 2^-51 of the largest of their operand (x's given rows, the weights), and sums are rounded an
       eighth as often, as long as no score is off by more than 2^-24 by the latter: where the largest magnitudes of x and of the weights, times one another and the features, pass 2^26, or a number is not
       finite, fp32 products take their place (at a third to a half of the speed). So a row does not depend on what the others hold.
-    * The scores' cotangents, g p, are held in the same way for more than 64 rows, to 2^-51 of the row's larger cotangent: what tokens with probabilities below 2^-28 get has fewer bits, below 2^-52 none.
+    * The scores' cotangents, g p, are held in the same way for more than 64 rows, to 2^-51 of the row's larger cotangent: what tokens with probabilities below 2^-28 get has fewer bits, below 2^-52 none; and of dweights a row's part
+      (its cotangent times its x) to 2^-51 of the largest row's.
     * Infinities and NaN are those of fp32 arithmetic: a NaN in a row of x makes that row's results NaN, one in the weights those of every row; a token whose weights make its score -inf has probability 0.
 
     Differentiable with respect to x and weights, through both results.'''
