@@ -711,7 +711,7 @@ __device__ __forceinline__ void linear_q_body(u32x4* __restrict__ by_row, float*
         given[j] = r < P.rows && is_token(tokens[at], P.V);
         token[j] = given[j] ? (uint32_t)tokens[at] : 0xFFFFFFFFu;
         // (plain: ds itself, the rows' m has no part in the products)
-        const float m = factors[3u * at], up = plain ? m : power_of_two(Q_SCALE);
+        const float up = plain ? factors[3u * at] : power_of_two(Q_SCALE);
         peak[j] = row_peaks[at]; one[j] = factors[3u * at + 2u] * up; part[j] = factors[3u * at + 1u] * up / row_totals[at];
     }
     const HalfTarget to{by_row, P.blocks_x, P.Vp / 16u, n * 2u * T, m * 4u * T}, none{nullptr, 0u, 0u, 0u, 0u};
